@@ -73,6 +73,12 @@ SIGNATURES = {
     "akv_rope_split": (_I, [_P] * 5 + [_I] * 4 + [_F, _P]),
     "akv_rms_norm": (_I, [_P] * 3 + [_I] * 2 + [_F, _P]),
     "akv_silu_mul": (_I, [_P] * 2 + [_I] * 2 + [_P]),
+    "akv_tree_scratch_bytes": (ctypes.c_longlong, [_I] * 6),
+    "akv_tree_attention": (_I, [_P] * 5 + [ctypes.c_longlong, _P, ctypes.c_longlong, _P, _P] + [_I] * 3 + [_F, _P]),
+    "akv_tree_weights": (_I, [_P] * 4 + [ctypes.c_longlong, _P] + [_I] * 3 + [_F, _P]),
+    "akv_tree_commit": (_I, [_P] * 4 + [_I] * 4 + [_P]),
+    "akv_evict_scratch_bytes": (ctypes.c_longlong, [_I] * 4),
+    "akv_evict": (_I, [_P] * 3 + [_I] * 6 + [_P]),
     "akv_timing_reset": (_I, []),
     "akv_timing_read": (_I, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
 }

@@ -1,0 +1,212 @@
+"""Operators around the plane cache for programs that draft several tokens at a time and keep their caches bounded.
+
+  tree_attention   a tree of drafted tokens attends to the cache and to its own ancestors
+  tree_weights     adds the attention weight that such queries give each cached token to fp32 sums
+  tree_commit      the accepted path of the tree enters the cache
+  evict            every (sequence, KV head) keeps its heaviest cached tokens
+
+The reference has no counterpart: it decodes one token at a time and never drops one (model/KVCache_AlignedKV.py:81-135).
+
+`cache` is anything with the tensors of a layer as attributes - k_first_8, k_mid_4, k_last_4, v_first_8, v_mid_4, v_last_4,
+k_exp_max, v_exp_max, restk, restv, laid out as in `decode.DecodeLayer`, which is one - and `rest_start`, `rest_len` say how many
+tokens are in the planes and in the residual buffers.  `DecodeLayer` offers the same operators as methods that keep those counts.
+Everything is launched on torch's current stream of the tensors' device; nothing synchronises.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .extension._planes import cdiv, column_block
+
+__all__ = ["tree_attention", "tree_weights", "tree_commit", "evict"]
+
+_nothing = contextlib.nullcontext()
+_PLANES = ("k_first_8", "k_mid_4", "k_last_4", "v_first_8", "v_mid_4", "v_last_4", "k_exp_max", "v_exp_max")
+MOST_DRAFTED = 64
+
+
+def _need(name: str, t, shape: tuple, dtype: torch.dtype, device: torch.device) -> None:
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on {device}")
+
+
+class _Call:
+    """A cache's tensors, checked, as the library takes them; a context in which its device is the current one."""
+
+    def __init__(self, cache, rest_len: int, rest_start: int):
+        f8 = cache.k_first_8
+        if not isinstance(f8, torch.Tensor) or not f8.is_cuda or f8.dim() != 5 or f8.shape[4] != column_block:
+            raise RuntimeError(f"k_first_8: expected a CUDA tensor of shape [B, H, blocks, D, {column_block}]")
+        self.device = dev = f8.device
+        self.index = dev.index
+        B, H, nmb, D, _ = f8.shape
+        self.B, self.H, self.D = B, H, D
+        self.L = L = cache.v_first_8.shape[2] if cache.v_first_8.dim() == 4 else -1
+        if self.D not in (64, 128):
+            raise RuntimeError(f"head size {self.D}: these operators cover 64 and 128")
+        if nmb != cdiv(L, column_block):
+            raise RuntimeError(f"k_first_8 has {nmb} blocks, v_first_8 {L} tokens")
+        half = column_block // 2
+        shapes = ((B, H, nmb, D, column_block), (B, H, nmb, D, half), (B, H, nmb, D, half), (B, H, L, D), (B, H, L, D // 2),
+                  (B, H, L, D // 2), (B, 1, H, D), (B, 1, H, D))
+        ptrs = []
+        for name, shape in zip(_PLANES, shapes):
+            t = getattr(cache, name)
+            _need(name, t, shape, torch.uint8, dev)
+            ptrs.append(t.data_ptr())
+        for name in ("restk", "restv"):
+            t = getattr(cache, name)
+            _need(name, t, (B, column_block, H, D), torch.half, dev)
+            ptrs.append(t.data_ptr())
+        if rest_start % column_block or not 0 <= rest_len < column_block or rest_start < 0 or rest_start + rest_len > L:
+            raise RuntimeError(f"{rest_start} tokens in planes of {L} and {rest_len} residual ones: expected whole blocks of "
+                               f"{column_block} and at most {column_block - 1}")
+        self.ptrs, self.tokens = ptrs, rest_start + rest_len
+
+    def queries(self, q: torch.Tensor) -> tuple:
+        """(drafted tokens, query heads) of q [B,T,Hq,D]."""
+        if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[0] != self.B or q.shape[3] != self.D or \
+                q.dtype != torch.half or q.device != self.device or not q.is_contiguous():
+            raise RuntimeError(f"q: expected a contiguous fp16 tensor of shape [{self.B}, T, Hq, {self.D}] on {self.device}")
+        T, Hq = q.shape[1], q.shape[2]
+        if not 1 <= T <= MOST_DRAFTED:
+            raise RuntimeError(f"q: {T} drafted tokens, expected 1 to {MOST_DRAFTED}")
+        if Hq % self.H or Hq == 0:
+            raise RuntimeError(f"q: {Hq} query heads are no multiple of {self.H} KV heads")
+        return T, Hq
+
+    def mask(self, mask) -> tuple:
+        if mask is None:
+            return None, 0
+        if not isinstance(mask, torch.Tensor) or mask.dtype != torch.half or mask.device != self.device or mask.dim() != 4 or \
+                mask.shape[1:3] != (1, 1) or mask.shape[0] not in (1, self.B) or mask.shape[3] < self.tokens or \
+                (mask.stride(3) != 1 and mask.shape[3] > 1):
+            raise RuntimeError(f"mask: expected a CUDA fp16 tensor of shape [{self.B} or 1, 1, 1, >= {self.tokens}] with a unit "
+                               "stride along the positions")
+        return mask.data_ptr(), (mask.stride(0) if mask.shape[0] == self.B else 0)
+
+    def layer(self, group: int, scratch: torch.Tensor | None):
+        return ctypes.byref(_lib.Layer(*self.ptrs, None if scratch is None else scratch.data_ptr(),
+                                       0 if scratch is None else scratch.numel(), self.B, self.H, group, self.D, self.L))
+
+    def here(self):
+        return _nothing if torch.cuda.current_device() == self.index else torch.cuda.device(self.index)
+
+
+def tree_attention(cache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: torch.Tensor, *, rest_len: int,
+                   rest_start: int, mask: torch.Tensor | None = None, scale: float | None = None, lse: bool = False,
+                   out: torch.Tensor | None = None):
+    """Attention output [B,T,Hq,D] of T drafted tokens (1 to 64) that are not in the cache.
+
+    q [B,T,Hq,D], k and v [B,T,Hkv,D] fp16; query head i reads KV head i // (Hq / Hkv).  tree: bool [T,T] or [B,T,T], True where
+    the drafted token of the row sees that of the column (itself among them: nothing is implied).  Every row sees the whole cache,
+    except where `mask` - the additive fp16 row of `DecodeLayer.decode`, [B,1,1,n] or [1,1,1,n] with n >= the cached tokens - is
+    -inf; a token taken away by either has no part in the output, whatever its values are.  A row that sees nothing is zero.
+
+    All planes are read: the output is that of dense attention over the cached fp16 values, with fp32 scores (times `scale`, by
+    default D**-0.5), softmax and sums and one rounding to fp16.  (`DecodeLayer.decode` skips plane rows by its read decisions,
+    rounds scores to fp16 and adds a mask there; the two agree within the decisions' error, not bit for bit.)
+
+    lse=True also returns the logarithm of the rows' sums of exponentials, fp32 [B,T,Hq] (-inf where nothing is seen), which
+    `tree_weights` takes.  The cache is not changed; `tree_commit` appends the accepted tokens."""
+    c = _Call(cache, rest_len, rest_start)
+    T, Hq = c.queries(q)
+    for name, t in (("k", k), ("v", v)):
+        _need(name, t, (c.B, T, c.H, c.D), torch.half, c.device)
+    if not isinstance(tree, torch.Tensor) or tree.dtype != torch.bool or tree.device != c.device or not tree.is_contiguous() or \
+            tuple(tree.shape) not in ((T, T), (c.B, T, T)):
+        raise RuntimeError(f"tree: expected a contiguous bool tensor of shape [{T}, {T}] or [{c.B}, {T}, {T}] on {c.device}")
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _need("out", out, tuple(q.shape), torch.half, c.device)
+    mask_ptr, mask_stride = c.mask(mask)
+    group, lib = Hq // c.H, _lib.load()
+    sums = torch.empty((c.B, T, Hq), dtype=torch.float32, device=c.device) if lse else None
+    with c.here():
+        ws = torch.empty(lib.akv_tree_scratch_bytes(c.B, c.H, group, c.D, rest_start, T), dtype=torch.uint8, device=c.device)
+        rc = lib.akv_tree_attention(
+            c.layer(group, ws), q.data_ptr(), k.data_ptr(), v.data_ptr(), tree.data_ptr(), T * T if tree.dim() == 3 else 0,
+            mask_ptr, mask_stride, out.data_ptr(), sums.data_ptr() if lse else None, T, rest_len, rest_start,
+            1.0 / math.sqrt(c.D) if scale is None else scale, _lib.raw_stream(c.index))
+    _lib.check("tree_attention", rc)
+    return (out, sums) if lse else out
+
+
+def tree_weights(cache, q: torch.Tensor, lse: torch.Tensor, weights: torch.Tensor, *, rest_len: int, rest_start: int,
+                 mask: torch.Tensor | None = None, scale: float | None = None) -> None:
+    """weights[b,h,t] += sum over the query rows of KV head h of exp(score(row, t) - lse[row]) for every cached token t.
+
+    q as in `tree_attention`, which gives lse fp32 [B,T,Hq] (its normalisation includes the drafted tokens); mask and scale as
+    there.  weights: fp32 [B,Hkv,max_seq_len]; entries behind the cached tokens are left alone.  The sums are formed in one order
+    (rows ascending within a lane, lanes in a fixed tree): the same call on the same state gives the same bits."""
+    c = _Call(cache, rest_len, rest_start)
+    T, Hq = c.queries(q)
+    _need("lse", lse, (c.B, T, Hq), torch.float32, c.device)
+    _need("weights", weights, (c.B, c.H, c.L), torch.float32, c.device)
+    mask_ptr, mask_stride = c.mask(mask)
+    with c.here():
+        rc = _lib.load().akv_tree_weights(
+            c.layer(Hq // c.H, None), q.data_ptr(), lse.data_ptr(), mask_ptr, mask_stride, weights.data_ptr(), T, rest_len,
+            rest_start, 1.0 / math.sqrt(c.D) if scale is None else scale, _lib.raw_stream(c.index))
+    _lib.check("tree_weights", rc)
+
+
+def tree_commit(cache, k: torch.Tensor, v: torch.Tensor, path: torch.Tensor, *, rest_len: int, rest_start: int) -> None:
+    """Append the drafted tokens path[b, 0], path[b, 1], ... of every sequence b to the cache.
+
+    k, v [B,T,Hkv,D] as given to `tree_attention` (T 1 to 64); path int32 [B,n], n 1 to 64, node indices in the order in which they
+    are appended (an index outside the tree is clamped into it; every sequence accepts the same number of tokens).  The cache is
+    then what n steps of `DecodeLayer.decode` would have left: exponent maxima, residual rows, and the planes of a block that
+    fills up.  The caller's counts become (rest_len + n) % 64 and rest_start + 64 if a block was filled."""
+    c = _Call(cache, rest_len, rest_start)
+    if not isinstance(k, torch.Tensor) or k.dim() != 4 or not 1 <= k.shape[1] <= MOST_DRAFTED:
+        raise RuntimeError(f"k: expected a tensor of shape [B, T, H, D] with T 1 to {MOST_DRAFTED}")
+    T = k.shape[1]
+    for name, t in (("k", k), ("v", v)):
+        _need(name, t, (c.B, T, c.H, c.D), torch.half, c.device)
+    if not isinstance(path, torch.Tensor) or path.dim() != 2 or not 1 <= path.shape[1] <= MOST_DRAFTED:
+        raise RuntimeError(f"path: expected a tensor of shape [{c.B}, n] with n 1 to {MOST_DRAFTED}")
+    n = path.shape[1]
+    _need("path", path, (c.B, n), torch.int32, c.device)
+    if c.tokens + n > c.L:
+        raise RuntimeError(f"cache is full ({c.L} tokens): no room for {n} behind {c.tokens}")
+    with c.here():
+        rc = _lib.load().akv_tree_commit(c.layer(1, None), k.data_ptr(), v.data_ptr(), path.data_ptr(), T, n, rest_len, rest_start,
+                                         _lib.raw_stream(c.index))
+    _lib.check("tree_commit", rc)
+
+
+def evict(cache, weights: torch.Tensor, positions: torch.Tensor, *, rest_len: int, rest_start: int, keep: int, recent: int = 0,
+          arranged: int = 0, shift: int = 0) -> None:
+    """Reduce the rest_start tokens in the planes to `keep` (a positive multiple of 64) per (sequence, KV head), in place.
+
+    weights fp32 [B,Hkv,max_seq_len] (`tree_weights`): the heaviest tokens stay, of equal ones those in the lower places; NaN counts
+    as more than infinity.  Tokens at the last `recent` positions (at most `keep`) stay whatever their weight, residual tokens
+    are not touched.  The i-th survivor in a place >= keep moves into the i-th place < keep that became free, its weight with it:
+    attention does not ask for the order of cached tokens, and moving only those touches each once.
+
+    positions int32 [B,Hkv,max_seq_len]: the sequence position of the token in each place, which an eviction writes for the
+    places below `keep`.  Places from `arranged` on hold tokens in order, place p that at position p + shift: (0, 0) before the
+    first eviction, after one (keep, shift + rest_start - keep).
+
+    Afterwards: rest_start = keep; K nibble planes behind it are zero as the K writers expect; the residual tokens' weights follow
+    at keep.., zeros behind them.  Exponent maxima stay (they remain upper bounds)."""
+    c = _Call(cache, rest_len, rest_start)
+    _need("weights", weights, (c.B, c.H, c.L), torch.float32, c.device)
+    _need("positions", positions, (c.B, c.H, c.L), torch.int32, c.device)
+    if keep <= 0 or keep % column_block or keep > rest_start:
+        raise RuntimeError(f"keep: {keep}, expected a positive multiple of {column_block} of at most {rest_start}")
+    if not 0 <= recent <= keep or not 0 <= arranged <= rest_start or shift < 0:
+        raise RuntimeError(f"recent {recent} [0..keep], arranged {arranged} [0..{rest_start}], shift {shift} [>= 0]")
+    lib = _lib.load()
+    with c.here():
+        ws = torch.empty(lib.akv_evict_scratch_bytes(c.B, c.H, rest_start, keep), dtype=torch.uint8, device=c.device)
+        rc = lib.akv_evict(c.layer(1, ws), weights.data_ptr(), positions.data_ptr(), rest_len, rest_start, keep, recent, arranged,
+                           shift, _lib.raw_stream(c.index))
+    _lib.check("evict", rc)

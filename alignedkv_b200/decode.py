@@ -13,7 +13,7 @@ import math
 
 import torch
 
-from . import _lib
+from . import _lib, cache_ops
 from .extension._planes import cdiv, column_block, exponent_field
 from .extension.KV_cache_cpp_extention import cuda_module
 
@@ -70,6 +70,8 @@ class DecodeLayer:
         self._index = self.device.index if self.device.index is not None else torch.cuda.current_device()
         self._q_shape, self._kv_shape = (bsz, 1, self.Hq, head_dim), (bsz, 1, n_heads, head_dim)
         self.launches = 0
+        self.weights = self.positions = None  # fp32 / int32 [B,Hkv,L], made by the first tree_weights or evict
+        self.evictions = self.arranged = self.shift = 0
 
     @property
     def launches(self) -> int:
@@ -158,6 +160,7 @@ class DecodeLayer:
         mask_ptr, mask_stride = None, 0
         if mask is not None:
             need = self.cache_len + (1 if append else 0)
+            self._no_mask_after_eviction()
             if mask.dtype != torch.half or not mask.is_cuda or mask.dim() != 4 or mask.shape[1] != 1 or \
                     mask.shape[2] != 1 or mask.shape[0] not in (1, self.B) or mask.shape[3] < need or mask.stride(3) != 1:
                 raise RuntimeError(f"mask: expected a CUDA fp16 tensor of shape [{self.B} or 1, 1, 1, >= {need}] with a "
@@ -209,17 +212,76 @@ class DecodeLayer:
             self.cache_len += 1
         return out if exchange is not None else (rec if packed else out)
 
+    # ------------------------------------------------------------------ drafted tokens, bounded cache (`cache_ops`)
+    def _no_mask_after_eviction(self) -> None:
+        if self.evictions:
+            raise RuntimeError("mask: after an eviction the cached positions differ from head to head (`positions`)")
+
+    def _counts(self) -> dict:
+        return dict(rest_len=self.rest_len, rest_start=self.rest_start)
+
+    def tree_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: torch.Tensor, *,
+                       mask: torch.Tensor | None = None, lse: bool = False, out: torch.Tensor | None = None):
+        """Attention of T drafted tokens (q [B,T,Hq,D], k and v [B,T,H,D]) over the cache and over those of themselves that
+        `tree` ([T,T] or [B,T,T] bool) lets them see; the cache stays as it is (`cache_ops.tree_attention`)."""
+        if mask is not None:
+            self._no_mask_after_eviction()
+        if q.dim() == 4 and q.shape[2] != self.Hq:
+            raise RuntimeError(f"q: {q.shape[2]} query heads, the layer has {self.Hq}")
+        return cache_ops.tree_attention(self, q, k, v, tree, mask=mask, lse=lse, out=out, **self._counts())
+
+    def tree_weights(self, q: torch.Tensor, lse: torch.Tensor, *, mask: torch.Tensor | None = None) -> torch.Tensor:
+        """Add the attention weight that these queries give each cached token to `weights` [B,H,L], fp32, and return it
+        (`cache_ops.tree_weights`; q and lse as given to and returned by `tree_attention`)."""
+        if mask is not None:
+            self._no_mask_after_eviction()
+        if q.dim() == 4 and q.shape[2] != self.Hq:
+            raise RuntimeError(f"q: {q.shape[2]} query heads, the layer has {self.Hq}")
+        if self.weights is None:
+            self.weights = torch.zeros((self.B, self.H, self.L), dtype=torch.float32, device=self.device)
+        cache_ops.tree_weights(self, q, lse, self.weights, mask=mask, **self._counts())
+        return self.weights
+
+    def tree_commit(self, k: torch.Tensor, v: torch.Tensor, path: torch.Tensor) -> None:
+        """Append drafted tokens path[b, 0..n-1] (int32 [B,n]) of k and v [B,T,H,D], as n decode steps would
+        (`cache_ops.tree_commit`).  Their entries of `weights` start at zero."""
+        cache_ops.tree_commit(self, k, v, path, **self._counts())
+        n = path.shape[1]
+        filled = self.rest_len + n >= column_block
+        self.rest_start += column_block if filled else 0
+        self.rest_len = (self.rest_len + n) % column_block
+        self.cache_len += n
+
+    def evict(self, keep: int, recent: int = 0) -> None:
+        """Reduce the tokens in the planes to the `keep` heaviest per (sequence, KV head) by `weights`, the last `recent`
+        positions among them; residual tokens stay (`cache_ops.evict`).  The cache is then keep + rest_len tokens long, and
+        `positions` [B,H,L] holds the sequence position of the token in each of the first `arranged` places (place p behind them:
+        p + shift)."""
+        if self.weights is None:
+            self.weights = torch.zeros((self.B, self.H, self.L), dtype=torch.float32, device=self.device)
+        if self.positions is None:
+            self.positions = torch.zeros((self.B, self.H, self.L), dtype=torch.int32, device=self.device)
+        cache_ops.evict(self, self.weights, self.positions, keep=keep, recent=recent, arranged=self.arranged, shift=self.shift,
+                        **self._counts())
+        gone = self.rest_start - keep
+        self.evictions += 1
+        self.arranged, self.shift = keep, self.shift + gone
+        self.rest_start -= gone
+        self.cache_len -= gone
+
     # ------------------------------------------------------------------ benchmark helpers
     def snapshot(self):
         """What is needed to come back to the current length later (`restore`): the counters and the exponent maxima."""
         return dict(rest_len=self.rest_len, rest_start=self.rest_start, cache_len=self.cache_len,
-                    k_exp=self.k_exp_max.clone(), v_exp=self.v_exp_max.clone())
+                    k_exp=self.k_exp_max.clone(), v_exp=self.v_exp_max.clone(), evictions=self.evictions)
 
     def restore(self, snap) -> None:
         """Roll the cache back to a snapshot (`akv_rollback`): the exponent maxima are put back and the K nibble planes
         of blocks written since are cleared, because the K writer accumulates nibbles
         (extension/csrc/K_cache.cu:52-56).  Tokens that were still in the residual buffer at the snapshot stay
-        there: later appends only wrote rows behind them."""
+        there: later appends only wrote rows behind them.  Weights of the tokens that go are set to zero."""
+        if snap.get("evictions", 0) != self.evictions:
+            raise RuntimeError("restore: tokens have been evicted since the snapshot")
         first_blk = snap["rest_start"] // column_block
         last_blk = self.rest_start // column_block
         appended = self.cache_len - snap["cache_len"]
@@ -231,6 +293,8 @@ class DecodeLayer:
                                        self.B, self.H, self.D, self.L, first_blk, max(0, last_blk - first_blk),
                                        _lib.raw_stream(self._index))
         _lib.check("rollback", rc)
+        if self.weights is not None and appended:
+            self.weights[..., snap["cache_len"]:self.cache_len] = 0
         self.rest_len, self.rest_start, self.cache_len = snap["rest_len"], snap["rest_start"], snap["cache_len"]
 
     def reset_counters(self) -> None:

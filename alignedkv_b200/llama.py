@@ -248,10 +248,64 @@ class LlamaDecoder:
     @torch.no_grad()
     def step(self, ids: torch.Tensor) -> torch.Tensor:
         """ids [B] (one token per sequence) -> logits [B,V]; appends to every layer's cache."""
-        assert self.pos + 1 <= self.L
+        assert (self.caches[0].cache_len if self.attention == "alignedkv" else self.pos) + 1 <= self.L
         if getattr(self, "_segs", None) is not None:
             return self._step_graphs(ids)       # (the returned logits are overwritten by the next step)
         return self._forward(ids.view(self.B, 1), False)
+
+    @torch.no_grad()
+    def verify(self, ids: torch.Tensor, parents: torch.Tensor, weights: bool = False) -> torch.Tensor:
+        """Logits [B,T,V] of T drafted tokens (ids [B,T], T at most 64) that are not in the caches yet.  parents: int64 [T], the
+        tree they form in every sequence: the node that each one follows, a lower index, or -1 for the last cached token.
+        `accept` appends some of them.  weights=True also adds the queries' attention weights to each layer's (`evict`)."""
+        assert self.attention == "alignedkv", "only the AlignedKV path drafts tokens"
+        cfg = self.cfg
+        H, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        B, T = ids.shape
+        up = parents.tolist()
+        if len(up) != T or any(type(j) is not int or not -1 <= j < i for i, j in enumerate(up)):
+            raise RuntimeError(f"parents: expected {T} indices of earlier nodes, or -1")
+        tree = torch.eye(T, dtype=torch.bool)
+        for i, j in enumerate(up):
+            if j >= 0:
+                tree[i] |= tree[j]
+        tree = tree.to(self.device)
+        tables = _rope_tables(self.pos + tree.sum(1) - 1, D, cfg.rope_theta)
+        x = self.embed[ids]
+        drafts = []
+        for p, cache in zip(self.layers, self.caches):
+            h = _rms_norm(x, p["norm1"], cfg.rms_norm_eps)
+            qkv = F.linear(h, p["wqkv"]).view(B, T, H + 2 * Hkv, D)
+            qk = _rope(qkv[:, :, :H + Hkv], tables)
+            q, k, v = qk[:, :, :H].contiguous(), qk[:, :, H:].contiguous(), qkv[:, :, H + Hkv:].contiguous()
+            o = cache.tree_attention(q, k, v, tree, lse=weights)
+            if weights:
+                o, lse = o
+                cache.tree_weights(q, lse)
+            drafts.append((k, v))
+            x = torch.addmm(x.view(B * T, -1), o.view(B * T, H * D), p["wo"].t()).view(B, T, -1)
+            h = _rms_norm(x, p["norm2"], cfg.rms_norm_eps)
+            gate, wide = F.linear(h, p["w_gate_up"]).chunk(2, dim=-1)
+            x = torch.addmm(x.view(B * T, -1), F.silu(gate).mul_(wide).view(B * T, -1), p["w_down"].t()).view(B, T, -1)
+        self._drafts = drafts
+        return F.linear(_rms_norm(x, self.final_norm, cfg.rms_norm_eps), self.lm_head)
+
+    @torch.no_grad()
+    def accept(self, path: torch.Tensor) -> None:
+        """Append nodes path[b, 0..n-1] (int [B,n]: a chain from the root) of the last `verify` to the caches; once."""
+        drafts, self._drafts = getattr(self, "_drafts", None), None
+        if drafts is None:
+            raise RuntimeError("accept: no drafted tokens (call verify first)")
+        path = path.to(device=self.device, dtype=torch.int32).contiguous()
+        for cache, (k, v) in zip(self.caches, drafts):
+            cache.tree_commit(k, v, path)
+        self.pos += path.shape[1]
+
+    @torch.no_grad()
+    def evict(self, keep: int, recent: int = 0) -> None:
+        """Reduce every layer's quantized tokens to the `keep` heaviest per head (`DecodeLayer.evict`); positions go on counting."""
+        for cache in self.caches:
+            cache.evict(keep, recent)
 
     @torch.no_grad()
     def generate(self, ids: torch.Tensor, new_tokens: int) -> torch.Tensor:

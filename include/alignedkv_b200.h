@@ -394,6 +394,45 @@ int akv_shard_step(void* k_first_8, void* k_mid_4, void* k_last_4, void* v_first
                    int token_base, int chunks_total, int n_ranks, int out_chunks, int flags, int phase, void* stream);
 
 /*
+ * Attention of a tree of drafted tokens over the cache, the weights of its queries, and what enters and leaves the cache with it
+ * (no counterpart in the reference, which decodes one token at a time and never drops one).  `layer`: planes, residual buffers,
+ * extents; exponent maxima and scratch where an entry says so.  rest_len (0..63) tokens in the residual buffers behind rest_start
+ * (a multiple of 64) in the planes.  head_dim 64 or 128; `drafted` 1..64 tokens T per sequence.  fp16 tensors contiguous and
+ * 16-byte aligned: q, out [B,T,Hq,D], k_new, v_new [B,T,Hkv,D]; query head i reads KV head i / group.
+ *
+ * akv_tree_attention: out[r] = softmax over the tokens that row r sees of (scale q_r . k + mask), times v; fp32 scores, softmax and
+ * sums over the exact cached values (every plane is read), rounded once.  tree: bytes [T,T] per sequence, tree_stride bytes apart
+ * (0 = one for all), non-zero where the row's token sees the column's.  mask (NULL = none): fp16 row per sequence as in
+ * akv_decode_step_masked, entries [0, rest_start + rest_len); -inf takes a token away whatever its values are.  A row that sees
+ * nothing is 0, its lse -inf.  lse (may be NULL): fp32 [B,T,Hq], log of the sum of exponentials.  scratch: at least
+ * akv_tree_scratch_bytes(..., rest_start, drafted) bytes, any contents.
+ *
+ * akv_tree_weights: weights fp32 [B,Hkv,max_seq_len], entry t of head h += sum over its T * group rows of exp(score - lse[r]) for
+ * t < rest_start + rest_len.  No atomics: the same call on the same state gives the same bits.
+ *
+ * akv_tree_commit: appends drafted tokens path[b][0..accepted-1] (int32 [B, accepted], clamped into 0..drafted-1; accepted 1..64)
+ * as that many akv_decode_step calls would: exponent maxima, residual rows, and the planes of a block that fills up (its K
+ * nibbles are stored, not added).  The caller then sets rest_len = (rest_len + accepted) % 64, and rest_start + 64 if it wrapped.
+ *
+ * akv_evict: of the rest_start tokens in the planes every (batch, KV head) keeps `keep` (a multiple of 64): those at the last
+ * `recent` positions, then the largest weights, of equal ones the lower places (NaN above infinity).  The i-th survivor in a place
+ * >= keep moves to the i-th free place < keep with its weight; positions int32 [B,Hkv,max_seq_len] are written for places < keep.
+ * Places >= arranged hold tokens in order, place p that at position p + shift.  K nibble planes of the freed blocks are
+ * cleared, the residual tokens' weights move to keep.., zeros behind.  scratch: akv_evict_scratch_bytes(...) bytes.
+ */
+long long akv_tree_scratch_bytes(int bsz, int n_kv_heads, int group, int head_dim, int n_tokens, int drafted);
+int akv_tree_attention(const akv_layer* layer, const void* q, const void* k_new, const void* v_new, const void* tree,
+                       long long tree_stride, const void* mask, long long mask_stride, void* out, void* lse, int drafted,
+                       int rest_len, int rest_start, float scale, void* stream);
+int akv_tree_weights(const akv_layer* layer, const void* q, const void* lse, const void* mask, long long mask_stride,
+                     void* weights, int drafted, int rest_len, int rest_start, float scale, void* stream);
+int akv_tree_commit(const akv_layer* layer, const void* k_new, const void* v_new, const void* path, int drafted, int accepted,
+                    int rest_len, int rest_start, void* stream);
+long long akv_evict_scratch_bytes(int bsz, int n_kv_heads, int n_tokens, int keep);
+int akv_evict(const akv_layer* layer, void* weights, void* positions, int rest_len, int rest_start, int keep, int recent,
+              int arranged, int shift, void* stream);
+
+/*
  * Benchmark instrumentation (no counterpart in the reference): with akv_set_tuning("timing", 1), akv_decode_step
  * records CUDA events around its q.K^T and P.V launches.  akv_timing_read returns how many steps were recorded
  * since akv_timing_reset and their median launch durations in microseconds; synchronise the stream first.

@@ -110,3 +110,42 @@ def test_step_under_autocast(akv_lib):
         assert torch.equal(a.step(ids[:, 70]), tensor_step(b, ids[:, 70]))
     with torch.autocast("cuda", torch.bfloat16), pytest.raises(RuntimeError, match="fp16"):
         a.step(ids[:, 70])
+
+
+def test_verify_accept_evict(akv_lib):
+    """A chain of drafted tokens gives the logits of that many steps (within the steps' read decisions), a branch does not notice
+    its siblings, the accepted tokens are in the caches, and decoding goes on after an eviction."""
+    from alignedkv_b200.llama import LlamaConfig, LlamaDecoder
+    cfg = LlamaConfig(hidden_size=512, intermediate_size=1024, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                      vocab_size=1000)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    B, S = 2, 190
+    ids = torch.randint(0, cfg.vocab_size, (B, S + 8), device="cuda", generator=gen)
+    a, b, d = (LlamaDecoder(cfg, B, S + 40, "cuda:0", seed=1, attention=m) for m in ("alignedkv", "alignedkv", "dense"))
+    for dec in (a, b, d):
+        dec.prefill(ids[:, :S])
+    want = torch.stack([d.step(ids[:, S + i]) for i in range(4)], 1)
+    # nodes 0, 2, 3, 5 are the chain, 1 and 4 are branches of other tokens
+    drafts = torch.stack([ids[:, S], ids[:, S + 5], ids[:, S + 1], ids[:, S + 2], ids[:, S + 6], ids[:, S + 3]], 1)
+    parents = torch.tensor([-1, -1, 0, 2, 2, 3])
+    logits = a.verify(drafts, parents, weights=True)
+    chain = [0, 2, 3, 5]
+    # fp16 activations through two layers in another order of additions
+    assert float((logits[:, chain].float() - want.float()).abs().max()) <= 1e-2 * float(want.float().abs().max())
+    alone = b.verify(drafts[:, chain].contiguous(), torch.tensor([-1, 0, 1, 2]))
+    assert float((logits[:, chain].float() - alone.float()).abs().max()) <= 1e-2 * float(want.float().abs().max())
+    a.accept(torch.tensor([chain] * B))
+    b.accept(torch.arange(4).expand(B, -1))
+    assert a.pos == b.pos == S + 4 and a.caches[0].cache_len == S + 4
+    for x, y in zip(a.caches, b.caches):
+        assert (x.rest_len, x.rest_start) == (y.rest_len, y.rest_start) == (2, 192)
+        assert float((x.restk[:, :2].float() - y.restk[:, :2].float()).abs().max()) <= 2e-2
+    with pytest.raises(RuntimeError, match="call verify"):
+        a.accept(torch.tensor([chain] * B))
+    with pytest.raises(RuntimeError, match="parents"):
+        a.verify(drafts, torch.tensor([-1, -1, 0, 3, 2, 3]))
+    a.evict(128, recent=32)
+    assert a.caches[1].cache_len == 130 and a.pos == S + 4
+    for i in range(40):                       # more steps than the room behind the uncut cache
+        out = a.step(ids[:, i])
+    assert bool(torch.isfinite(out.float()).all()) and a.pos == S + 44 and a.caches[0].cache_len == 170
