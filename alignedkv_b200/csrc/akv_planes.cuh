@@ -29,22 +29,22 @@ __device__ __forceinline__ void line8(uint32_t (&w)[4], uint32_t h0, uint32_t h1
     w[3] = __byte_perm(odd, h1, 0x7352);
 }
 
-// What a lane loads of one line: N elements, N / 8 groups of eight.
+// What a lane holds of one line: N elements, N / 8 groups of eight.
 template <int N>
 struct Line {
     uint32_t h[N / 4], m[N / 8], l[N / 8];
-    __device__ __forceinline__ void load(const uint8_t* f8, const uint8_t* m4, const uint8_t* l4) {
+    __device__ __forceinline__ void load(uint32_t f8, uint32_t m4, uint32_t l4) {      // shared memory
         if constexpr (N == 16) {
-            const uint4 a = ld_stream<uint4>(f8);
-            const uint2 b = ld_stream<uint2>(m4), c = ld_stream<uint2>(l4);
+            const uint4 a = lds128(f8);
+            const uint2 b = lds64(m4), c = lds64(l4);
             h[0] = a.x; h[1] = a.y; h[2] = a.z; h[3] = a.w;
             m[0] = b.x; m[1] = b.y;
             l[0] = c.x; l[1] = c.y;
         } else {
-            const uint2 a = ld_stream<uint2>(f8);
+            const uint2 a = lds64(f8);
             h[0] = a.x; h[1] = a.y;
-            m[0] = ld_stream<uint32_t>(m4);
-            l[0] = ld_stream<uint32_t>(l4);
+            m[0] = lds32(m4);
+            l[0] = lds32(l4);
         }
     }
     __device__ __forceinline__ void clear() {
@@ -53,8 +53,6 @@ struct Line {
 #pragma unroll
         for (int i = 0; i < N / 8; ++i) m[i] = l[i] = 0;
     }
-    template <class T>
-    static __device__ __forceinline__ T ld_stream(const uint8_t* p) { return __ldg(reinterpret_cast<const T*>(p)); }
 };
 
 // acc[j] += A (16 x 16) times column j of the four lines, for the lane's N elements.

@@ -8,7 +8,7 @@
 //
 // All planes are read: 2 bytes per cached element, once per 16 rows.  Bound by HBM while the rows of a KV head are few.
 // Work: a unit is 16 query rows of one (batch, KV head); its tiles are 128 tokens of the planes each, and one tail tile of the
-// residual (slots 0..63) and the drafted tokens (slots 64..127).  The tiles of all units in a row are dealt to the warps in equal
+// residual tokens with the drafted ones behind them (at most 127).  The tiles of all units in a row are dealt to the warps in equal
 // contiguous runs, so that every SM gets the same whatever the number of units and their length.  A warp needs no other one: it
 // turns plane bytes into operand fragments in registers (akv_planes.cuh), keeps the scores of its tile and the output of its unit
 // there, and leaves a record (maximum, sum, output) where a run begins or ends inside a unit.
@@ -32,85 +32,225 @@ struct TreeArgs {
     long long tree_stride, mask_stride;
     __half* out;
     float *lse, *part;
-    int H, G, T, nmb, L, nb, rest, rt, tiles;
+    int H, G, T, nmb, L, nb, rest, rt, tiles, tail;       // tail: tokens of the tail tile
     long long total, nw;       // tiles of all units, warps that they are dealt to (at most as many)
-    float scale2;              // scale * log2(e)
+    float scale, scale2;       // scale2 = scale * log2(e)
 };
 
-__device__ __forceinline__ float ex2(float x) { return exp2f(x); }
-
-// One K step: 16 channels of the tile's 128 tokens; lane (g, t): channels 16 kk + 4t .. + 3, tokens 16g .. 16g + 15.
-template <int D>
-__device__ __forceinline__ void load_k(Line<16> (&x)[4], const TreeArgs& p, long long bh, int tile, int kk, int g, int t) {
-    const int blk = 2 * tile + (g >> 2);
-    if (blk < p.nb) {
-        const long long row = (bh * p.nmb + blk) * D + 16 * kk + 4 * t;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            x[i].load(p.k8 + (row + i) * BLK + 16 * (g & 3), p.km + (row + i) * (BLK / 2) + 8 * (g & 3),
-                      p.kl + (row + i) * (BLK / 2) + 8 * (g & 3));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i].clear();
-    }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // Token of line i of V step st within a tile, for lane column t: the tokens whose probabilities this lane holds.
 __device__ __forceinline__ int v_token(int st, int t, int i) { return 32 * t + 2 * st + (i & 1) + (i >> 1) * 16; }
 
-template <int D>
-__device__ __forceinline__ void load_v(Line<D / 8> (&x)[4], const TreeArgs& p, long long bh, int tile, int st, int g, int t,
-                                       const __half* mask) {
-    constexpr int N = D / 8;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int tok = tile * TILE + v_token(st, t, i);
-        // (a token that the mask takes away counts as zero, whatever its values are: 0 * NaN would be NaN)
-        if (tok < p.nb * BLK && !(mask && __ldg(reinterpret_cast<const uint16_t*>(mask) + tok) == 0xFC00u)) {
-            const long long row = bh * p.L + tok;
-            x[i].load(p.v8 + row * D + N * g, p.vm + row * (D / 2) + N / 2 * g, p.vl + row * (D / 2) + N / 2 * g);
-        } else {
-            x[i].clear();
-        }
-    }
+// 16 bytes global -> shared past L1; with `there` false zeros, and nothing is read.
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
-// Scores of a plane tile: s[j][c] = row g (c < 2) or g + 8, token 16 (2t + (c & 1)) + j.
+// A warp's ring of 4 KB steps in shared memory, filled STEPS - 1 steps ahead by its own asynchronous copies.
+//   K step    16 channels of the tile's 128 tokens: high bytes [block][channel][64], nibbles [block][channel][32] twice
+//   V step    32 (D = 128: 16) tokens: for each 16 of them high bytes [4t + i][D], nibbles [..][D / 2] twice
+//   tail      16 tokens of the tail as fp16 rows [token][D]: a K step, then (WITH_V) their V step
+// The 16-byte pieces of a 128-byte line are swapped by XOR so that a quarter (half) warp's 16-byte (8-byte) loads of a line's
+// pieces by lane (g, t) fall into different banks.
+constexpr int STEPS = 5, STEP_BYTES = 4096;
+
+constexpr int WARP_BYTES = STEPS * STEP_BYTES + 8192;            // the ring, query fragments, probabilities
+
 template <int D>
-__device__ __forceinline__ void plane_scores(float (&s)[16][4], const uint4* qf, const TreeArgs& p, long long bh, int tile,
-                                             int lane) {
-    const int g = lane >> 2, t = lane & 3;
+struct Ring {
+    static constexpr int KSTEPS = D / 16, VSTEPS = D / 16, SUB = 128 / D;     // SUB: products of 16 tokens per V step
+    uint32_t base;                 // of the warp's ring
+    int lane, put, get;            // steps: slots filled next, read next
+    // what is copied next: step of a tile of (batch, KV head) bh; left = tiles from this one on.  Every tile `times` times.
+    long long bh, left;
+    int step, tile, unit, units_per_head, time, times, plane_tiles;
+
+    // Tiles first .. last - 1 of units of p.tiles tiles.
+    template <bool WITH_V>
+    __device__ __forceinline__ void start(const TreeArgs& p, uint32_t at, int of_lane, long long first, long long last,
+                                          int per_head, int reps) {
+        base = at;
+        lane = of_lane;
+        put = get = step = time = 0;
+        units_per_head = per_head;
+        times = reps;
+        plane_tiles = (p.nb + 1) >> 1;
+        unit = (int)(first / p.tiles);
+        tile = (int)(first - (long long)unit * p.tiles);
+        left = (last - first) * reps;
+        bh = unit / units_per_head;
+#pragma unroll 1
+        for (int i = 0; i < STEPS - 1; ++i) fill<WITH_V>(p);
+    }
+    __device__ __forceinline__ uint32_t slot(int i) const { return base + (uint32_t)i * STEP_BYTES; }
+
+    __device__ __forceinline__ void copy_k(const TreeArgs& p, uint32_t to) const {
+        const bool two = 2 * tile + 1 < p.nb;
+        const long long row = (bh * p.nmb + 2 * tile) * D + 16 * step;
+        const uint8_t *h = p.k8 + row * BLK + lane * 16, *m = p.km + row * (BLK / 2) + lane * 16, *l = p.kl + row * (BLK / 2) + lane * 16;
+        // (lane: channel lane / 4 of 8, piece lane % 4; of nibbles channel lane / 2 of 16, piece lane % 2)
+        const uint32_t at = (lane >> 3) * 128 + ((((lane >> 2) & 1) * 4 + (lane & 3)) ^ (2 * (lane >> 4))) * 16;
+        const uint32_t nib = (lane >> 3) * 128 + ((((lane >> 1) & 3) * 2 + (lane & 1)) ^ (2 * (lane >> 3))) * 16;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const bool there = b == 0 || two;
+            const long long o = there ? (long long)b * D : 0;
+            copy16(to + b * 1024 + at, h + o * BLK, there);
+            copy16(to + b * 1024 + 512 + (at ^ 64), h + o * BLK + 512, there);
+            copy16(to + 2048 + b * 512 + nib, m + o * (BLK / 2), there);
+            copy16(to + 3072 + b * 512 + nib, l + o * (BLK / 2), there);
+        }
+    }
+    __device__ __forceinline__ void copy_v(const TreeArgs& p, uint32_t to, int vs) const {
+        const bool two = 2 * tile + 1 < p.nb;
+        const long long row = bh * p.L + tile * TILE;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            const int st = vs * SUB + u;
+            const uint32_t d = to + u * (STEP_BYTES / SUB);
+            // rows of 128, 64 or 32 bytes: PIECES of 16 each
+            auto rows = [&](const uint8_t* src, uint32_t dst, auto pieces) {
+                constexpr int PIECES = decltype(pieces)::value;
+#pragma unroll
+                for (int j = 0; j < PIECES / 2; ++j) {
+                    const int id = j * 32 + lane, r = id / PIECES, q = id % PIECES, t = r >> 2, i = r & 3;
+                    const bool there = t < 2 || two;
+                    const uint8_t* from = src + (row + (there ? v_token(st, t, i) : 0)) * (PIECES * 16) + q * 16;
+                    copy16(dst + place<PIECES>(t, i, q), from, there);
+                }
+            };
+            rows(p.v8, d, Int<D / 16>{});
+            rows(p.vm, d + D * 16, Int<D / 32>{});
+            rows(p.vl, d + D * 24, Int<D / 32>{});
+        }
+    }
+    template <int X> struct Int { static constexpr int value = X; };
+    // Where piece q of V row (t, i) lies, rows of PIECES pieces.
+    template <int PIECES>
+    static __device__ __forceinline__ uint32_t place(int t, int i, int q) {
+        if constexpr (PIECES == 8) return (4 * t + i) * 128 + ((q ^ (2 * t)) << 4);
+        else if constexpr (PIECES == 4) return (2 * i + (t >> 1)) * 128 + ((((t & 1) * 4 + q) ^ (2 * (t >> 1))) << 4);
+        else return i * 128 + ((2 * t + q) << 4);
+    }
+
+    // Rows 16 c .. of the tail: the residual tokens, the drafted ones behind them; zeros behind those.
+    __device__ __forceinline__ void copy_tail(const TreeArgs& p, uint32_t to, int c, bool value) const {
+        const __half *rest = value ? p.restv : p.restk, *drafted = value ? p.vd : p.kd;
+        const long long b = bh / p.H, h = bh - b * p.H;
+        constexpr int PIECES = D / 8;
+#pragma unroll
+        for (int j = 0; j < PIECES / 2; ++j) {
+            const int id = j * 32 + lane, r = id / PIECES, q = id % PIECES, i = 16 * c + r, d = i - p.rest;
+            const bool there = i < p.tail;
+            const __half* row = d < 0 ? rest + ((b * BLK + i) * p.H + h) * D : drafted + ((b * p.T + (there ? d : 0)) * p.H + h) * D;
+            copy16(to + tail_place(r, q, value), reinterpret_cast<const uint8_t*>(there ? row : p.q) + (there ? q * 16 : 0), there);
+        }
+    }
+    // Where piece q of tail row r lies.  K is read by lane (g, t) = (row, 8 bytes of piece 2 kk + t / 2), V by (pieces of channels
+    // N g .., rows 2t, 2t + 1, 2t + 8, 2t + 9).
+    static __device__ __forceinline__ uint32_t tail_place(int r, int q, bool value) {
+        const int t = (r >> 1) & 3;
+        const int x = !value ? 2 * (r & 3) : D == 128 ? (t & 1) + 4 * (t >> 1) : 2 * t;
+        return r * (2 * D) + ((q ^ x) << 4);
+    }
+
+    // One step further, if there is one; always a group, so that the groups count the steps.
+    template <bool WITH_V>
+    __device__ __forceinline__ void fill(const TreeArgs& p) {
+        if (left > 0) {
+            const uint32_t to = slot(put);
+            int steps = WITH_V ? KSTEPS + VSTEPS : KSTEPS;
+            if (tile == plane_tiles) {
+                steps = ((p.tail + 15) >> 4) * (WITH_V ? 2 : 1);
+                copy_tail(p, to, WITH_V ? step >> 1 : step, WITH_V && (step & 1));
+            } else if (!WITH_V || step < KSTEPS) {
+                copy_k(p, to);
+            } else {
+                copy_v(p, to, step - KSTEPS);
+            }
+            if (++step == steps) {
+                step = 0;
+                --left;
+                next(p);
+            }
+        }
+        cp_async_commit();
+        put = put + 1 == STEPS ? 0 : put + 1;
+    }
+    __device__ __forceinline__ void next(const TreeArgs& p) {
+        if (++time < times) return;
+        time = 0;
+        if (++tile == p.tiles) {
+            tile = 0;
+            bh = ++unit / units_per_head;
+        }
+    }
+    // Waits for the step that is read next, requests the one whose slot the last read has left.
+    template <bool WITH_V>
+    __device__ __forceinline__ uint32_t take(const TreeArgs& p) {
+        cp_async_wait<STEPS - 2>();
+        __syncwarp();
+        fill<WITH_V>(p);
+        const uint32_t at = slot(get);
+        get = get + 1 == STEPS ? 0 : get + 1;
+        return at;
+    }
+
+    __device__ __forceinline__ void lines_k(Line<16> (&x)[4], uint32_t at) const {
+        const int g = lane >> 2, t = lane & 3;
+        const uint32_t h = at + (g >> 2) * 1024 + 2 * t * 128 + (((g & 3) ^ (2 * t)) << 4);
+        const uint32_t m = at + 2048 + (g >> 2) * 512 + t * 128 + (g & 1) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t n = m + (((2 * i + ((g & 3) >> 1)) ^ (2 * t)) << 4);
+            x[i].load((h ^ ((i & 1) * 64)) + (i >> 1) * 128, n, n + 1024);
+        }
+    }
+    __device__ __forceinline__ void lines_v(Line<D / 8> (&x)[4], uint32_t at) const {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // the lane's D / 8 high bytes and D / 16 bytes of nibbles lie within one piece
+            constexpr int HP = D / 16, NP = D / 32;
+            const uint32_t h = at + place<HP>(t, i, D == 128 ? g : g >> 1) + (D == 128 ? 0 : (g & 1) * 8);
+            const uint32_t n = at + D * 16 + place<NP>(t, i, D == 128 ? g >> 1 : g >> 2) + (D == 128 ? (g & 1) * 8 : (g & 3) * 4);
+            x[i].load(h, n, n + D * 8);
+        }
+    }
+};
+
+// Scores of a plane tile: s[j][c] = row g (c < 2) or g + 8, token 16 (2t + (c & 1)) + j.
+template <int D, bool WITH_V>
+__device__ __forceinline__ void plane_scores(float (&s)[16][4], const uint4* qf, const TreeArgs& p, Ring<D>& ring) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll 1
     for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t at = ring.template take<WITH_V>(p);
         Line<16> x[4];
-        load_k<D>(x, p, bh, tile, kk, g, t);
-        mma_lines<16>(s, qf[kk * 32 + lane], x);
+        ring.lines_k(x, at);
+        mma_lines<16>(s, qf[kk * 32 + ring.lane], x);
     }
 }
 
-// Row of the tail tile's slot (0..63 residual, 64.. drafted) in an fp16 tensor pair; nullptr: there is none.
-__device__ __forceinline__ const __half* tail_row(const __half* rest, const __half* drafted, const TreeArgs& p, int D, long long b,
-                                                  int h, int slot) {
-    if (slot < BLK) return slot < p.rest ? rest + ((b * BLK + slot) * p.H + h) * D : nullptr;
-    return drafted && slot - BLK < p.T ? drafted + ((b * p.T + slot - BLK) * p.H + h) * D : nullptr;
-}
-
+// Scores of 16 tail tokens: s[j][c] = row g (c < 2) or g + 8, token 8 j + 2t + (c & 1) of them.
 template <int D>
-__device__ __forceinline__ void tail_scores(float (&s)[16][4], const uint4* qf, const TreeArgs& p, long long b, int h, int lane) {
+__device__ __forceinline__ void tail_scores(float (&s)[2][4], const uint4* qf, uint32_t at, int lane) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+    for (int j = 0; j < 2; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        const __half* row = tail_row(p.restk, p.kd, p, D, b, h, 16 * g + j);
+    for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            const uint2 w = row ? __ldg(reinterpret_cast<const uint2*>(row + 16 * kk + 4 * t)) : make_uint2(0, 0);
+        for (int j = 0; j < 2; ++j) {
+            const uint2 w = lds64(at + Ring<D>::tail_place(g + 8 * j, 2 * kk + (t >> 1), false) + (t & 1) * 8);
             mma_f16(s[j], qf[kk * 32 + lane], w.x, w.y);
         }
-    }
 }
 
 // The unit's query rows as fragments in shared memory (every lane stores and reads its own).
@@ -133,37 +273,55 @@ __device__ __forceinline__ void load_q(uint4* qf, const TreeArgs& p, long long b
     }
 }
 
-// Scores to base 2 of a plane tile or of the tail's residual half; tokens that do not exist or are masked away: -inf.
-__device__ __forceinline__ void scale_mask(float (&s)[16][4], const TreeArgs& p, const __half* mask, int first, int count, int t) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int tok = 16 * (2 * t + c) + j;
-            float add = 0.f;
-            if (mask && tok < count) add = __half2float(mask[first + tok]);
-            const bool gone = tok >= count || add == -INFINITY;
-            s[j][c] = gone ? -INFINITY : fmaf(s[j][c], p.scale2, add * LOG2E);
-            s[j][c + 2] = gone ? -INFINITY : fmaf(s[j][c + 2], p.scale2, add * LOG2E);
-        }
-}
-
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Running maximum m, sum l (of this lane's tokens) and output o of rows g and g + 8, taken on by scores s to base 2 of NJ n-tiles;
+// s becomes the probabilities, relative to the maximum and times 2^LIFT.
+template <int NJ, int N>
+__device__ __forceinline__ void soften(float (&s)[NJ][4], float (&m)[2], float (&l)[2], float (&o)[N][4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float top = m[i];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) top = fmaxf(top, fmaxf(s[j][2 * i], s[j][2 * i + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        const float base = (top == -INFINITY ? 0.f : top) - LIFT;
+        const float keep = ex2((m[i] - LIFT) - base);          // (nothing yet: 0)
+        m[i] = top;
+        l[i] *= keep;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            o[j][2 * i] *= keep;
+            o[j][2 * i + 1] *= keep;
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                s[j][2 * i + c] = ex2(s[j][2 * i + c] - base);
+                l[i] += s[j][2 * i + c];
+            }
+    }
+}
+
 template <int D>
 __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
     constexpr int N = D / 8;
-    __shared__ __align__(16) uint4 frag[WARPS][256];
+    extern __shared__ __align__(128) uint8_t smem[];
     pdl_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int R = p.T * p.G;
     const long long w = (long long)warp * gridDim.x + blockIdx.x;
     if (w >= p.nw) return;
     const long long first = w * p.total / p.nw, last = (w + 1) * p.total / p.nw;
-    uint4* qf = frag[warp];
+    uint4* qf = reinterpret_cast<uint4*>(smem + (size_t)warp * WARP_BYTES + STEPS * STEP_BYTES);
+    uint4* pf = qf + 256;
+    Ring<D> ring;
+    ring.template start<true>(p, smem_u32(smem) + warp * WARP_BYTES, lane, first, last, p.rt, 1);
     for (long long at = first; at < last;) {
         const long long unit = at / p.tiles, bh = unit / p.rt, b = bh / p.H;
         const int h = (int)(bh - b * p.H), row0 = (int)(unit - bh * p.rt) * ROWS;
@@ -174,133 +332,134 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
 #pragma unroll
         for (int j = 0; j < N; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 #pragma unroll 1
-        for (int tile = t0; tile < t1; ++tile) {
-            const bool tail = tile == p.tiles - 1;
-            float s[16][4];
-            if (!tail) {
-                plane_scores<D>(s, qf, p, bh, tile, lane);
-                scale_mask(s, p, mask, tile * TILE, min(TILE, p.nb * BLK - tile * TILE), t);
-            } else {
-                tail_scores<D>(s, qf, p, b, h, lane);
-                if (t < 2) {
-                    scale_mask(s, p, mask, p.nb * BLK, p.rest, t);
+        for (int tile = t0; tile < min(t1, p.tiles - 1); ++tile) {
+            {
+                float s[16][4];
+                plane_scores<D, true>(s, qf, p, ring);
+                const int count = p.nb * BLK - tile * TILE;
+                if (mask || count < TILE) {             // tokens that do not exist or are masked away: -inf
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int tok = 16 * (2 * t + c) + j;
+                            const float add = mask && tok < count ? __half2float(mask[tile * TILE + tok]) : 0.f;
+                            const bool gone = tok >= count || add == -INFINITY;
+                            s[j][c] = gone ? -INFINITY : fmaf(s[j][c], p.scale2, add * LOG2E);
+                            s[j][c + 2] = gone ? -INFINITY : fmaf(s[j][c + 2], p.scale2, add * LOG2E);
+                        }
                 } else {
-                    const uint8_t* seen = p.tree + b * p.tree_stride;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int r = row0 + g + 8 * i;
-                        const uint8_t* mine = seen + (long long)(r / p.G) * p.T;
+                    for (int j = 0; j < 16; ++j)
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
+                        for (int c = 0; c < 4; ++c) s[j][c] *= p.scale2;
+                }
+                soften(s, m, l, o);
+                // (through shared memory, every lane its own: the loop over the V steps stays a loop - unrolled eight times, with
+                // the copies in each, the kernel was bound by the fetch of its instructions, 195 us against 113 at 8 x 32 x 4096 tokens)
 #pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                const int d = 16 * (2 * t + c) + j - BLK;
-                                s[j][2 * i + c] = r < R && d < p.T && mine[d] ? s[j][2 * i + c] * p.scale2 : -INFINITY;
-                            }
+                for (int st = 0; st < 8; ++st)
+                    pf[st * 32 + lane] = make_uint4(pack_half2(s[2 * st][0], s[2 * st + 1][0]), pack_half2(s[2 * st][2], s[2 * st + 1][2]),
+                                                    pack_half2(s[2 * st][1], s[2 * st + 1][1]), pack_half2(s[2 * st][3], s[2 * st + 1][3]));
+            }
+#pragma unroll 1
+            for (int vs = 0; vs < Ring<D>::VSTEPS; ++vs) {
+                const uint32_t from = ring.template take<true>(p);
+#pragma unroll
+                for (int u = 0; u < Ring<D>::SUB; ++u) {
+                    const int st = vs * Ring<D>::SUB + u;
+                    Line<N> x[4];
+                    ring.lines_v(x, from + u * (STEP_BYTES / Ring<D>::SUB));
+                    if (mask) {      // a token that is masked away counts as zero, whatever its values are: 0 * NaN would be NaN
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int tok = tile * TILE + v_token(st, t, i);
+                            if (tok < p.nb * BLK && __half_as_ushort(mask[tok]) == 0xFC00u) x[i].clear();
+                        }
                     }
+                    mma_lines<N>(o, pf[st * 32 + lane], x);
                 }
             }
-            uint32_t pf[16][2];      // probabilities of rows g and g + 8 as they enter the product: [j] = tokens 16 (2t) + j ...
-            float base[2];
+        }
+        if (t1 == p.tiles) {
+            // The tail, 16 tokens at a time: rows of fp16 values.
+            const uint8_t* seen = p.tree + b * p.tree_stride;
+            const uint8_t* mine[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float top = m[i];
+            for (int i = 0; i < 2; ++i) mine[i] = seen + (long long)(min(row0 + g + 8 * i, R - 1) / p.G) * p.T;
+#pragma unroll 1
+            for (int c0 = 0; c0 < p.tail; c0 += 16) {
+                float s[2][4];
+                tail_scores<D>(s, qf, ring.template take<true>(p), lane);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) top = fmaxf(top, fmaxf(s[j][2 * i], s[j][2 * i + 1]));
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                base[i] = (top == -INFINITY ? 0.f : top) - LIFT;
-                const float keep = ex2((m[i] - LIFT) - base[i]);          // (nothing yet: 0)
-                m[i] = top;
-                l[i] *= keep;
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    o[j][2 * i] *= keep;
-                    o[j][2 * i + 1] *= keep;
-                }
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        s[j][2 * i + c] = ex2(s[j][2 * i + c] - base[i]);
-                        l[i] += s[j][2 * i + c];
+                        const int tok = c0 + 8 * j + 2 * t + c, d = tok - p.rest;
+                        const float add = mask && d < 0 ? __half2float(mask[p.nb * BLK + tok]) : 0.f;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const bool here = d < 0 ? add != -INFINITY : d < p.T && mine[i][d];
+                            s[j][2 * i + c] = here ? fmaf(s[j][2 * i + c], p.scale2, add * LOG2E) : -INFINITY;
+                        }
                     }
-            }
-#pragma unroll
-            for (int st = 0; st < 8; ++st) {
-                pf[2 * st][0] = pack_half2(s[2 * st][0], s[2 * st + 1][0]);
-                pf[2 * st][1] = pack_half2(s[2 * st][2], s[2 * st + 1][2]);
-                pf[2 * st + 1][0] = pack_half2(s[2 * st][1], s[2 * st + 1][1]);
-                pf[2 * st + 1][1] = pack_half2(s[2 * st][3], s[2 * st + 1][3]);
-            }
-            if (!tail) {
-#pragma unroll
-                for (int st = 0; st < 8; ++st) {
-                    Line<N> x[4];
-                    load_v<D>(x, p, bh, tile, st, g, t, mask);
-                    mma_lines<N>(o, make_uint4(pf[2 * st][0], pf[2 * st][1], pf[2 * st + 1][0], pf[2 * st + 1][1]), x);
-                }
-                continue;
-            }
-            // The tail: rows of fp16 values.  What one row of the tree sees is masked for another, and 0 * inf would be NaN:
-            // drafted values that are not finite are left out of the product and added by the rows that see them.
-            bool odd = false;
-#pragma unroll
-            for (int st = 0; st < 8; ++st) {
+                soften(s, m, l, o);
+                const uint4 a = make_uint4(pack_half2(s[0][0], s[0][1]), pack_half2(s[0][2], s[0][3]), pack_half2(s[1][0], s[1][1]),
+                                           pack_half2(s[1][2], s[1][3]));
+                // What one row sees is masked for another, and 0 * inf would be NaN: values that are not finite are left
+                // out of the product and added by the rows that see them.
+                const uint32_t from = ring.template take<true>(p);
+                bool odd = false;
                 uint32_t x[4][N / 2];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int slot = v_token(st, t, i);
-                    const __half* row = tail_row(p.restv, p.vd, p, D, b, h, slot);
-                    if (row && slot < BLK && mask && __half_as_ushort(mask[p.nb * BLK + slot]) == 0xFC00u) row = nullptr;
+                    const int r = 2 * t + (i & 1) + 8 * (i >> 1);
 #pragma unroll
                     for (int v = 0; v < N / 8; ++v) {
-                        const uint4 y = row ? __ldg(reinterpret_cast<const uint4*>(row + N * g) + v) : make_uint4(0, 0, 0, 0);
+                        const uint4 y = lds128(from + Ring<D>::tail_place(r, N / 8 * g + v, true));
                         x[i][4 * v] = y.x; x[i][4 * v + 1] = y.y; x[i][4 * v + 2] = y.z; x[i][4 * v + 3] = y.w;
                     }
-                    if (slot >= BLK) {
 #pragma unroll
-                        for (int v = 0; v < N / 2; ++v) {
-                            if ((x[i][v] & 0x7C00u) == 0x7C00u) { x[i][v] &= 0xFFFF0000u; odd = true; }
-                            if ((x[i][v] & 0x7C000000u) == 0x7C000000u) { x[i][v] &= 0xFFFFu; odd = true; }
-                        }
+                    for (int v = 0; v < N / 2; ++v) {
+                        if ((x[i][v] & 0x7C00u) == 0x7C00u) { x[i][v] &= 0xFFFF0000u; odd = true; }
+                        if ((x[i][v] & 0x7C000000u) == 0x7C000000u) { x[i][v] &= 0xFFFFu; odd = true; }
                     }
                 }
-                const uint4 a = make_uint4(pf[2 * st][0], pf[2 * st][1], pf[2 * st + 1][0], pf[2 * st + 1][1]);
 #pragma unroll
                 for (int v = 0; v < N / 2; ++v) {
                     mma_f16(o[2 * v], a, __byte_perm(x[0][v], x[1][v], 0x5410), __byte_perm(x[2][v], x[3][v], 0x5410));
                     mma_f16(o[2 * v + 1], a, __byte_perm(x[0][v], x[1][v], 0x7632), __byte_perm(x[2][v], x[3][v], 0x7632));
                 }
-            }
-            if (__any_sync(0xFFFFFFFFu, odd)) {
-                float* pr = reinterpret_cast<float*>(qf);               // [16 rows][64 drafted tokens]; the unit's last use of qf
-                __syncwarp();
-                if (t >= 2) {
+                if (__any_sync(0xFFFFFFFFu, odd)) {
+                    float* pr = reinterpret_cast<float*>(pf);               // [16 rows][16 tokens], absent ones below zero
+                    __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
+                    for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) pr[(g + 8 * (c >> 1)) * 64 + 16 * (2 * t + (c & 1)) + j - BLK] = s[j][c];
-                }
-                __syncwarp();
-                const uint8_t* seen = p.tree + b * p.tree_stride;
-                for (int d = 0; d < p.T; ++d) {
-                    const uint16_t* v = reinterpret_cast<const uint16_t*>(p.vd) + ((b * p.T + d) * p.H + h) * D;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int r = row0 + g + 8 * i;
-                        if (r >= R || !seen[(long long)(r / p.G) * p.T + d]) continue;
-                        const float pd = pr[(g + 8 * i) * 64 + d];
+                        for (int c = 0; c < 4; ++c) {
+                            const int tok = c0 + 8 * j + 2 * t + (c & 1), d = tok - p.rest;
+                            const bool here = d < 0 ? !(mask && __half_as_ushort(mask[p.nb * BLK + tok]) == 0xFC00u)
+                                                    : d < p.T && mine[c >> 1][d];
+                            pr[(g + 8 * (c >> 1)) * 16 + 8 * j + 2 * t + (c & 1)] = here ? s[j][c] : -1.f;
+                        }
+                    __syncwarp();
+#pragma unroll 1
+                    for (int k = 0; k < min(16, p.tail - c0); ++k) {
+                        const float p0 = pr[g * 16 + k], p1 = pr[(g + 8) * 16 + k];
 #pragma unroll
                         for (int j = 0; j < N; ++j)
 #pragma unroll
                             for (int c = 0; c < 2; ++c) {
-                                const uint16_t y = v[N * (2 * t + c) + j];
-                                if ((y & 0x7C00u) == 0x7C00u) o[j][2 * i + c] += pd * __half2float(__ushort_as_half(y));
+                                const int ch = N * (2 * t + c) + j;
+                                const uint32_t y = lds16(from + Ring<D>::tail_place(k, ch >> 3, true) + (ch & 7) * 2);
+                                if ((y & 0x7C00u) != 0x7C00u) continue;
+                                const float v = __half2float(__ushort_as_half((unsigned short)y));
+                                if (!(p0 < 0.f)) o[j][c] += p0 * v;
+                                if (!(p1 < 0.f)) o[j][2 + c] += p1 * v;
                             }
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
         }
 #pragma unroll
@@ -393,38 +552,63 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs p) {
 // A warp per 128 cached tokens of a (batch, KV head); all query rows of the head, 16 at a time, added in their order.
 template <int D>
 __global__ void __launch_bounds__(32 * WARPS, 1) weights_kernel(const TreeArgs p, float* __restrict__ weights) {
-    __shared__ __align__(16) uint4 frag[WARPS][256];
+    extern __shared__ __align__(128) uint8_t smem[];
     pdl_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int R = p.T * p.G, full = (p.nb + 1) >> 1;
-    uint4* qf = frag[warp];
-    for (long long at = (long long)warp * gridDim.x + blockIdx.x; at < p.total; at += p.nw) {
+    const long long w = (long long)warp * gridDim.x + blockIdx.x;
+    if (w >= p.nw) return;
+    const long long first = w * p.total / p.nw, last = (w + 1) * p.total / p.nw;
+    uint4* qf = reinterpret_cast<uint4*>(smem + (size_t)warp * WARP_BYTES + STEPS * STEP_BYTES);
+    Ring<D> ring;
+    ring.template start<false>(p, smem_u32(smem) + warp * WARP_BYTES, lane, first, last, 1, (R + ROWS - 1) / ROWS);
+    for (long long at = first; at < last; ++at) {
         const long long bh = at / p.tiles, b = bh / p.H;
         const int h = (int)(bh - b * p.H), tile = (int)(at - bh * p.tiles);
         const bool tail = tile == full;
         const int start = tail ? p.nb * BLK : tile * TILE, count = tail ? p.rest : min(TILE, p.nb * BLK - start);
         const __half* mask = p.mask ? p.mask + b * p.mask_stride : nullptr;
-        float sum[16][2];
+        float* into = weights + bh * p.L + start;
+        float sum[16][2];          // of plane token 16 (2t + c) + j; of the tail's 16 i + 8 j + 2t + c in sum[2 i + j]
 #pragma unroll
         for (int j = 0; j < 16; ++j) sum[j][0] = sum[j][1] = 0.f;
+        auto token = [&](int j, int c) { return tail ? 8 * j + 2 * t + c : 16 * (2 * t + c) + j; };
 #pragma unroll 1
         for (int row0 = 0; row0 < R; row0 += ROWS) {
             load_q<D>(qf, p, b, h, row0, lane);
             float s[16][4], off[2];
-            if (tail) tail_scores<D>(s, qf, p, b, h, lane);
-            else plane_scores<D>(s, qf, p, bh, tile, lane);
-            scale_mask(s, p, mask, start, count, t);
+            if (!tail) {
+                plane_scores<D, false>(s, qf, p, ring);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (16 * i >= p.rest) break;
+                    float part[2][4];
+                    tail_scores<D>(part, qf, ring.template take<false>(p), lane);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        s[2 * i][c] = part[0][c];
+                        s[2 * i + 1][c] = part[1][c];
+                    }
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = row0 + g + 8 * i;
-                off[i] = -INFINITY;
-                if (r < R) off[i] = p.lse[(b * p.T + r / p.G) * p.H * p.G + (long long)h * p.G + r % p.G] * LOG2E;
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)        // (a row that sees nothing has lse = -inf)
-                        if (off[i] != -INFINITY && s[j][2 * i + c] != -INFINITY) sum[j][c] += ex2(s[j][2 * i + c] - off[i]);
+                off[i] = r < R ? p.lse[(b * p.T + r / p.G) * p.H * p.G + (long long)h * p.G + r % p.G] : -INFINITY;
             }
+            // exp(score - lse) with one rounding of the small difference: scores of 25 are half of 2e-6 off themselves
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int tok = token(j, c);
+                    const float add = mask && tok < count ? __half2float(mask[start + tok]) : 0.f;
+                    if (tok >= count || add == -INFINITY) continue;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)        // (a row that sees nothing has lse = -inf)
+                        if (off[i] != -INFINITY) sum[j][c] += ex2(fmaf(s[j][2 * i + c], p.scale, add - off[i]) * LOG2E);
+                }
         }
 #pragma unroll
         for (int j = 0; j < 16; ++j)
@@ -432,8 +616,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) weights_kernel(const TreeArgs p
             for (int c = 0; c < 2; ++c) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) sum[j][c] += __shfl_xor_sync(0xFFFFFFFFu, sum[j][c], o);
-                const int tok = 16 * (2 * t + c) + j;
-                if (g == (j >> 1) && tok < count) weights[bh * p.L + start + tok] += sum[j][c];
+                if (g == (j >> 1) && token(j, c) < count) into[token(j, c)] += sum[j][c];
             }
     }
 }
@@ -451,6 +634,16 @@ Deal deal(long long total) {
     d.wpc = (int)(per < WARPS ? per : WARPS);
     d.warps = total < (long long)d.grid * d.wpc ? total : (long long)d.grid * d.wpc;
     return d;
+}
+
+// (the limit is raised for what eight warps take, whatever this launch does: it is a property of the kernel, not of the call)
+template <class Kernel, class... Args>
+int launch_warps(Kernel kernel, const Deal& d, cudaStream_t st, Args... args) {
+    const int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WARPS * WARP_BYTES),
+                               "tree kernel shared memory");
+    if (rc != AKV_OK) return rc;
+    launch_chained(kernel, dim3(d.grid), dim3(32 * d.wpc), (size_t)d.wpc * WARP_BYTES, st, args...);
+    return AKV_OK;
 }
 
 int check_layer(const char* fn, const akv_layer* a, const void* q, int T, int rest_len, int rest_start, const void* mask,
@@ -494,6 +687,7 @@ TreeArgs make_args(const akv_layer* a, const void* q, int T, int rest_len, int r
     p.nmb = (a->max_seq_len + BLK - 1) / BLK;
     p.nb = rest_start / BLK;
     p.rest = rest_len;
+    p.scale = scale;
     p.scale2 = scale * LOG2E;
     return p;
 }
@@ -537,12 +731,14 @@ int akv_tree_attention(const akv_layer* layer, const void* q, const void* k_new,
     p.part = static_cast<float*>(layer->scratch);
     p.rt = (drafted * p.G + ROWS - 1) / ROWS;
     p.tiles = (p.nb + 1) / 2 + 1;
+    p.tail = rest_len + drafted;
     const long long units = (long long)layer->bsz * p.H * p.rt;
     p.total = units * p.tiles;
     const Deal d = deal(p.total);
     p.nw = d.warps;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    launch_chained(D == 128 ? tree_kernel<128> : tree_kernel<64>, dim3(d.grid), dim3(32 * d.wpc), 0, st, p);
+    rc = launch_warps(D == 128 ? tree_kernel<128> : tree_kernel<64>, d, st, p);
+    if (rc != AKV_OK) return rc;
     rc = cuda_status(cudaGetLastError(), "tree_attention launch");
     if (rc != AKV_OK || p.tiles == 1) return rc;                 // (units of one tile: none is shared)
     launch_chained(D == 128 ? tree_merge_kernel<128> : tree_merge_kernel<64>, dim3((unsigned)(units * (ROWS / 4))), dim3(128), 0, st,
@@ -559,12 +755,14 @@ int akv_tree_weights(const akv_layer* layer, const void* q, const void* lse, con
     TreeArgs p = make_args(layer, q, drafted, rest_len, rest_start, mask, mask_stride, scale);
     p.lse = static_cast<float*>(const_cast<void*>(lse));
     p.tiles = (p.nb + 1) / 2 + (rest_len > 0);
+    p.tail = rest_len;
     p.total = (long long)layer->bsz * p.H * p.tiles;
     if (p.total == 0) return AKV_OK;
     const Deal d = deal(p.total);
-    p.nw = (long long)d.grid * d.wpc;
-    launch_chained(layer->head_dim == 128 ? weights_kernel<128> : weights_kernel<64>, dim3(d.grid), dim3(32 * d.wpc), 0,
-                   static_cast<cudaStream_t>(stream), p, static_cast<float*>(weights));
+    p.nw = d.warps;
+    rc = launch_warps(layer->head_dim == 128 ? weights_kernel<128> : weights_kernel<64>, d, static_cast<cudaStream_t>(stream), p,
+                      static_cast<float*>(weights));
+    if (rc != AKV_OK) return rc;
     return cuda_status(cudaGetLastError(), "tree_weights launch");
 }
 
