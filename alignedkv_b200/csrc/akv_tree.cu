@@ -15,33 +15,12 @@
 #include <limits.h>
 
 #include "akv_planes.cuh"
+#include "akv_tree.cuh"
 
 namespace akv {
 namespace {
 
-constexpr int BLK = 64, TILE = 128, ROWS = 16, WARPS = 8;
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-// Probabilities enter their product as fp16, relative to the running maximum and times 2^15: at most 32768, and down to 2^-29 of the
-// largest with all 11 bits (2^-14 without the factor).
-constexpr float LIFT = 15.f;
-
-struct TreeArgs {
-    const uint8_t *k8, *km, *kl, *v8, *vm, *vl;
-    const __half *restk, *restv, *q, *kd, *vd, *mask;
-    const uint8_t* tree;
-    long long tree_stride, mask_stride;
-    __half* out;
-    float *lse, *part;
-    int H, G, T, nmb, L, nb, rest, rt, tiles, tail;       // tail: tokens of the tail tile
-    long long total, nw;       // tiles of all units, warps that they are dealt to (at most as many)
-    float scale, scale2;       // scale2 = scale * log2(e)
-};
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
+constexpr int ROWS = 16, WARPS = 8;
 
 // Token of line i of V step st within a tile, for lane column t: the tokens whose probabilities this lane holds.
 __device__ __forceinline__ int v_token(int st, int t, int i) { return 32 * t + 2 * st + (i & 1) + (i >> 1) * 16; }
@@ -261,7 +240,7 @@ __device__ __forceinline__ void load_q(uint4* qf, const TreeArgs& p, long long b
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int r = row0 + g + 8 * i;
-        src[i] = r < R ? p.q + ((b * p.T + r / p.G) * p.H * p.G + (long long)h * p.G + r % p.G) * D : nullptr;
+        src[i] = r < R ? p.q + row_of(p, b, h, r) * D : nullptr;
     }
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
@@ -271,11 +250,6 @@ __device__ __forceinline__ void load_q(uint4* qf, const TreeArgs& p, long long b
             w[i] = src[i] ? __ldg(reinterpret_cast<const uint2*>(src[i] + 16 * kk + 4 * t)) : make_uint2(0, 0);
         qf[kk * 32 + lane] = make_uint4(w[0].x, w[1].x, w[0].y, w[1].y);
     }
-}
-
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // Running maximum m, sum l (of this lane's tokens) and output o of rows g and g + 8, taken on by scores s to base 2 of NJ n-tiles;
@@ -469,7 +443,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
             const int r = row0 + g + 8 * i;
             if (r >= R) continue;
             if (t0 == 0 && t1 == p.tiles) {
-                const long long row = (b * p.T + r / p.G) * p.H * p.G + (long long)h * p.G + r % p.G;
+                const long long row = row_of(p, b, h, r);
                 const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
                 uint4* dst = reinterpret_cast<uint4*>(p.out + row * D + 2 * N * t);
 #pragma unroll
@@ -508,21 +482,22 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
 // Warp that holds tile i when `total` tiles are dealt to nw warps: the largest w with floor(w total / nw) <= i.
 __device__ __forceinline__ long long warp_of(long long i, long long total, long long nw) { return ((i + 1) * nw - 1) / total; }
 
-// One warp per query row: the records of the warps that share its unit, in the order of the tokens.
+// One warp per query row: the records of the runs that share its unit, in the order of the tokens.
 template <int D>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs p) {
     pdl_enter();
     const int lane = threadIdx.x & 31;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);       // unit * 16 + row of the unit
-    const long long unit = row / ROWS, bh = unit / p.rt, b = bh / p.H;
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);       // unit * rowsu + row of the unit
+    const long long unit = row / p.rowsu, bh = unit / p.rt, b = bh / p.H;
+    const int of_unit = (int)(row - unit * p.rowsu);
     if (unit * p.tiles >= p.total) return;
-    const int h = (int)(bh - b * p.H), r = (int)(unit - bh * p.rt) * ROWS + (int)(row % ROWS);
+    const int h = (int)(bh - b * p.H), r = (int)(unit - bh * p.rt) * p.rowsu + of_unit;
     if (r >= p.T * p.G) return;
     const long long w0 = warp_of(unit * p.tiles, p.total, p.nw), w1 = warp_of(unit * p.tiles + p.tiles - 1, p.total, p.nw);
     if (w0 == w1) return;                                                       // a whole unit: written by its warp
     auto record = [&](long long w) {
         const int slot = unit != (w * p.total / p.nw) / p.tiles;
-        return p.part + ((2 * w + slot) * ROWS + row % ROWS) * (D + 4);
+        return p.part + ((2 * w + slot) * p.rowsu + of_unit) * (D + 4);
     };
     float top = -INFINITY;
     for (long long w = w0 + lane; w <= w1; w += 32) top = fmaxf(top, record(w)[0]);
@@ -541,7 +516,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs p) {
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[c] = fmaf(f, rec[4 + C * lane + c], acc[c]);
     }
-    const long long to = (b * p.T + r / p.G) * p.H * p.G + (long long)h * p.G + r % p.G;
+    const long long to = row_of(p, b, h, r);
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int c = 0; c < C; c += 2)
@@ -595,7 +570,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) weights_kernel(const TreeArgs p
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = row0 + g + 8 * i;
-                off[i] = r < R ? p.lse[(b * p.T + r / p.G) * p.H * p.G + (long long)h * p.G + r % p.G] : -INFINITY;
+                off[i] = r < R ? p.lse[row_of(p, b, h, r)] : -INFINITY;
             }
             // exp(score - lse) with one rounding of the small difference: scores of 25 are half of 2e-6 off themselves
 #pragma unroll
@@ -624,16 +599,38 @@ __global__ void __launch_bounds__(32 * WARPS, 1) weights_kernel(const TreeArgs p
 // Warps for `total` tiles: one an SM while there are that few, then up to eight.
 struct Deal {
     int grid, wpc;
-    long long warps;
+    long long runs;
 };
-Deal deal(long long total) {
+Deal deal(long long total, int most = WARPS) {
     const int sms = sm_count();
     Deal d;
     d.grid = (int)(total < sms ? total : sms);
     const long long per = (total + d.grid - 1) / d.grid;
-    d.wpc = (int)(per < WARPS ? per : WARPS);
-    d.warps = total < (long long)d.grid * d.wpc ? total : (long long)d.grid * d.wpc;
+    d.wpc = (int)(per < most ? per : most);
+    d.runs = total < (long long)d.grid * d.wpc ? total : (long long)d.grid * d.wpc;
     return d;
+}
+
+// How the attention of T drafted tokens behind rest_start tokens is cut up.
+struct Shape {
+    bool wide;
+    int groups, rowsg, rowsu, rt, tiles;
+    long long units, total;
+    Deal d;
+};
+Shape shape_of(int bsz, int H, int G, int T, int rest_start) {
+    Shape s;
+    const int R = T * G;
+    s.wide = R > ROWS;
+    s.groups = R > 128 ? 2 : 1;
+    s.rt = s.wide ? (R + 128 * s.groups - 1) / (128 * s.groups) : 1;
+    s.rowsu = s.wide ? (R + s.rt - 1) / s.rt : ROWS;
+    s.rowsg = (s.rowsu + s.groups - 1) / s.groups;
+    s.tiles = (rest_start / BLK + 1) / 2 + 1;
+    s.units = (long long)bsz * H * s.rt;
+    s.total = s.units * s.tiles;
+    s.d = deal(s.total, s.wide ? 1 : WARPS);
+    return s;
 }
 
 // (the limit is raised for what eight warps take, whatever this launch does: it is a property of the kernel, not of the call)
@@ -703,9 +700,8 @@ long long akv_tree_scratch_bytes(int bsz, int n_kv_heads, int group, int head_di
     if (bsz <= 0 || n_kv_heads <= 0 || group <= 0 || (head_dim != 64 && head_dim != 128) || n_tokens < 0 || drafted < 1 ||
         drafted > BLK)
         return -1;
-    const long long units = (long long)bsz * n_kv_heads * (((long long)drafted * group + ROWS - 1) / ROWS);
-    const Deal d = deal(units * ((n_tokens / BLK + 1) / 2 + 1));
-    return 2 * d.warps * ROWS * (head_dim + 4) * 4;
+    const Shape s = shape_of(bsz, n_kv_heads, group, drafted, n_tokens);
+    return 2 * s.d.runs * s.rowsu * (head_dim + 4) * 4;
 }
 
 int akv_tree_attention(const akv_layer* layer, const void* q, const void* k_new, const void* v_new, const void* tree,
@@ -729,20 +725,22 @@ int akv_tree_attention(const akv_layer* layer, const void* q, const void* k_new,
     p.out = static_cast<__half*>(out);
     p.lse = static_cast<float*>(lse);
     p.part = static_cast<float*>(layer->scratch);
-    p.rt = (drafted * p.G + ROWS - 1) / ROWS;
-    p.tiles = (p.nb + 1) / 2 + 1;
     p.tail = rest_len + drafted;
-    const long long units = (long long)layer->bsz * p.H * p.rt;
-    p.total = units * p.tiles;
-    const Deal d = deal(p.total);
-    p.nw = d.warps;
+    const Shape s = shape_of(layer->bsz, p.H, p.G, drafted, rest_start);
+    p.groups = s.groups;
+    p.rowsg = s.rowsg;
+    p.rowsu = s.rowsu;
+    p.rt = s.rt;
+    p.tiles = s.tiles;
+    p.total = s.total;
+    p.nw = s.d.runs;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    rc = launch_warps(D == 128 ? tree_kernel<128> : tree_kernel<64>, d, st, p);
+    rc = s.wide ? launch_tree_wide(p, D, s.d.grid, st) : launch_warps(D == 128 ? tree_kernel<128> : tree_kernel<64>, s.d, st, p);
     if (rc != AKV_OK) return rc;
     rc = cuda_status(cudaGetLastError(), "tree_attention launch");
     if (rc != AKV_OK || p.tiles == 1) return rc;                 // (units of one tile: none is shared)
-    launch_chained(D == 128 ? tree_merge_kernel<128> : tree_merge_kernel<64>, dim3((unsigned)(units * (ROWS / 4))), dim3(128), 0, st,
-                   p);
+    launch_chained(D == 128 ? tree_merge_kernel<128> : tree_merge_kernel<64>, dim3((unsigned)((s.units * s.rowsu + 3) / 4)),
+                   dim3(128), 0, st, p);
     return cuda_status(cudaGetLastError(), "tree_attention merge launch");
 }
 
@@ -759,7 +757,7 @@ int akv_tree_weights(const akv_layer* layer, const void* q, const void* lse, con
     p.total = (long long)layer->bsz * p.H * p.tiles;
     if (p.total == 0) return AKV_OK;
     const Deal d = deal(p.total);
-    p.nw = d.warps;
+    p.nw = d.runs;
     rc = launch_warps(layer->head_dim == 128 ? weights_kernel<128> : weights_kernel<64>, d, static_cast<cudaStream_t>(stream), p,
                       static_cast<float*>(weights));
     if (rc != AKV_OK) return rc;

@@ -1,0 +1,706 @@
+// Attention of drafted tokens where more than 16 query rows share a KV head: the fifth-generation tensor cores.
+//
+// CTA = one SM, a contiguous run of 128-token tiles as in akv_tree.cu; a unit is up to 256 query rows of a (batch, KV head).
+//   warps 8..15   decode: plane bytes from global memory to registers two tiles ahead, there to fp16, and into a ring of operand tiles
+//   warp  16      one thread issues the products: S = Q K^T (128 rows x 128 tokens), O += P V
+//   warps 0..7    two softmax groups of 128 threads, a thread per query row: S from tensor memory, P back into its place
+// Everything comes in twos: S, O, P and a softmax group per slot.  With up to 128 rows the slots take the tiles in turn (each
+// with an output of its own, joined at the end), with more each has half of the rows and takes every tile.  While one slot's
+// softmax runs, the other's products do.
+// K planes run along tokens and V planes along channels - along the n of either product, not along its sum: the operand tiles
+// are "MN-major", rows of 64 elements (128 bytes), so that a decoded piece of 16 elements is two 16-byte stores.  Only the
+// tail's keys (fp16 rows of channels) are K-major.
+// Tensor memory: columns 0..255 S (P in the same columns as fp16), 256..511 O.
+#include "akv_tree.cuh"
+
+namespace akv {
+
+__device__ unsigned int g_tree_wait_gave_up = 0;     // set when a bounded wait ran out (never expected)
+unsigned int tree_error_flag(cudaError_t* e) {
+    unsigned int v = 0;
+    *e = cudaMemcpyFromSymbol(&v, g_tree_wait_gave_up, sizeof(v));
+    return v;
+}
+cudaError_t tree_error_clear() {
+    const unsigned int v = 0;
+    return cudaMemcpyToSymbol(g_tree_wait_gave_up, &v, sizeof(v));
+}
+
+namespace {
+
+constexpr int SOFT = 8, DECODE = 8, THREADS = 32 * (SOFT + DECODE + 1), RING = 4;
+// A row's reference maximum moves only when a score exceeds it by 2^SLACK: probabilities are at most 2^(WIDE_LIFT + SLACK) in fp16.
+constexpr float WIDE_LIFT = 7.f, SLACK = 8.f;
+
+template <int D>
+struct Plan {
+    static constexpr int TILE_BYTES = TILE * D * 2, Q_HALF = 16384, Q_BYTES = Q_HALF * (D / 64);
+    static constexpr int RING_AT = 0, Q_AT = RING * TILE_BYTES;
+    // the second row group's queries; with one group the place where the slots' outputs are joined (128 rows x 64 channels)
+    static constexpr int JOIN_BYTES = 128 * 64 * 4, Q2_AT = Q_AT + Q_BYTES;
+    static constexpr int XM_AT = Q2_AT + (Q_BYTES > JOIN_BYTES ? Q_BYTES : JOIN_BYTES), XL_AT = XM_AT + 512;
+    static constexpr int BAR_AT = XL_AT + 512, BYTES = BAR_AT + 256 + 1024;     // (1024: the base is aligned up)
+};
+// barriers, 8 bytes each, then the tensor memory's address, the flag that a wait gave up, odd values of the last four segments
+enum Bar { FULL = 0, EMPTY = RING, S_FULL = 2 * RING, P_FULL = S_FULL + 2, O_FULL = P_FULL + 2, Q_FULL = O_FULL + 2, BARS };
+
+__device__ __forceinline__ void bar_init(uint32_t a, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(a), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t a) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(a) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t a, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(a), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Bounded (about a second); once one has given up, none waits any more and the outputs become NaN.
+__device__ __noinline__ void bar_wait_slow(uint32_t a, uint32_t parity, volatile int* dead) {
+    unsigned long long t0 = 0;
+    for (unsigned spin = 0; !bar_try(a, parity); ++spin) {
+        if (*dead) return;
+        if ((spin & 63) == 63) {
+            unsigned long long t;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > 1000000000ull) {
+                *dead = 1;
+                atomicOr(&g_tree_wait_gave_up, 4u);
+                return;
+            }
+        }
+    }
+}
+__device__ __forceinline__ void bar_wait(uint32_t a, uint32_t parity, volatile int* dead) {
+    if (__builtin_expect(!bar_try(a, parity), 0)) bar_wait_slow(a, parity, dead);
+}
+
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void fence_shared() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
+}
+// D (fp32, tensor memory) = A B (+ D): A, B fp16 in shared memory by descriptor, or A in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+// Shared-memory operand with 128-byte swizzle.  MN-major: `lead` = bytes between pieces of 64 elements, `stride` = between groups of
+// eight of the sum's indices.  K-major: stride = between groups of eight rows (lead unused).
+__device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t lead, uint32_t stride) {
+    return (uint64_t)(at >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// fp16 x fp16 -> fp32, 128 rows, n columns; A K-major, B MN-major if so.
+__device__ __forceinline__ constexpr uint32_t instruction(int n, bool b_mn) {
+    return 1u << 4 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+}
+// 32 columns of this thread's lane
+__device__ __forceinline__ void tmem_ld(uint32_t (&v)[32], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+                 "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                   "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]),
+                   "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
+                   "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(at) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+                 "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n"
+                 ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                   "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+                   "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
+                   "r"(v[30]), "r"(v[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n"
+                 ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                   "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void soft_sync() {
+    __syncwarp();
+    asm volatile("bar.sync 1, %0;\n" ::"n"(32 * SOFT) : "memory");
+}
+
+// ---------------------------------------------------------------- the run of a CTA, piece by piece
+// Segment: consecutive tiles t0 .. t0 + c - 1 of one unit.
+struct Segment {
+    long long unit, bh, b;
+    int h, super, t0, c, index;
+    __device__ __forceinline__ void at(const TreeArgs& p, long long tile, long long last) {
+        unit = tile / p.tiles;
+        t0 = (int)(tile - unit * p.tiles);
+        c = (int)min((long long)p.tiles - t0, last - tile);
+        bh = unit / p.rt;
+        super = (int)(unit - bh * p.rt);
+        b = bh / p.H;
+        h = (int)(bh - b * p.H);
+    }
+};
+// Operand tile q (0 .. 2c - 1) of a segment, in the order in which the products need them: with `ahead` scores under way,
+// K(0 .. ahead - 1), then V(i), K(i + ahead).
+__device__ __forceinline__ int tile_of(int q, int c, int ahead, bool& value) {
+    ahead = min(ahead, c);
+    if (q < ahead) {
+        value = false;
+        return q;
+    }
+    const int r = q - ahead, pairs = 2 * (c - ahead);
+    value = r >= pairs || !(r & 1);
+    return r >= pairs ? (c - ahead) + (r - pairs) : value ? r >> 1 : (r >> 1) + ahead;
+}
+__device__ __forceinline__ int place_of(int i, bool value, int c, int ahead) {
+    ahead = min(ahead, c);
+    if (!value) return i < ahead ? i : ahead + 2 * (i - ahead) + 1;
+    return i < c - ahead ? ahead + 2 * i : ahead + 2 * (c - ahead) + i - (c - ahead);
+}
+
+// ---------------------------------------------------------------- decode
+__device__ __forceinline__ uint4 ldg128(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ldg64(const void* p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+// Eight elements in order from their high bytes and nibbles.
+__device__ __forceinline__ uint4 halves8(uint32_t h0, uint32_t h1, uint32_t m, uint32_t l) {
+    const uint32_t even = (m & 0xF0F0F0F0u) | ((l >> 4) & 0x0F0F0F0Fu), odd = ((m << 4) & 0xF0F0F0F0u) | (l & 0x0F0F0F0Fu);
+    const uint32_t a = __byte_perm(even, odd, 0x5140), b = __byte_perm(even, odd, 0x7362);
+    return make_uint4(__byte_perm(a, h0, 0x5140), __byte_perm(a, h0, 0x7362), __byte_perm(b, h1, 0x5140), __byte_perm(b, h1, 0x7362));
+}
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w, bool& odd) {
+    if ((w & 0x7C00u) == 0x7C00u) { w &= 0xFFFF0000u; odd = true; }
+    if ((w & 0x7C000000u) == 0x7C000000u) { w &= 0xFFFFu; odd = true; }
+    return w;
+}
+
+// What is decoded: operand tile `q` of the segment, in pieces of 16 elements: a thread takes D / 32 of them.
+template <int D>
+struct Piece {
+    uint32_t w[D / 32][8];
+    bool value, tail;
+
+    // Piece u of a thread: quarter lane % 4 of (half, row).  Rows of 128 bytes: K planes [block][channel], else [channel half][token].
+    static __device__ __forceinline__ void where(int u, int warp, int lane, bool k_plane, int& half, int& row) {
+        const int i = u * DECODE + warp, halves = k_plane ? 2 : D / 64;
+        half = i & (halves - 1);
+        row = (halves == 2 ? i >> 1 : i) * 8 + (lane >> 2);
+    }
+    __device__ __forceinline__ void load(const TreeArgs& p, const Segment& s, int q, int warp, int lane) {
+        const int i = s.t0 + tile_of(q, s.c, 3 - p.groups, value);
+        tail = i == p.tiles - 1;
+        const int qd = lane & 3;
+        const __half* mask = p.mask ? p.mask + s.b * p.mask_stride : nullptr;
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u) {
+            int half, row;
+            where(u, warp, lane, !value && !tail, half, row);
+            const uint8_t *a = nullptr, *m = nullptr, *l = nullptr;
+            if (tail) {
+                if (row < p.tail) {
+                    const int d = row - p.rest;
+                    const __half* src = d < 0 ? (value ? p.restv : p.restk) + ((s.b * BLK + row) * p.H + s.h) * D
+                                              : (value ? p.vd : p.kd) + ((s.b * p.T + d) * p.H + s.h) * D;
+                    a = reinterpret_cast<const uint8_t*>(src + half * 64 + qd * 16);
+                }
+            } else if (!value) {
+                if (2 * i + half < p.nb) {
+                    const long long at = (s.bh * p.nmb + 2 * i + half) * D + row;
+                    a = p.k8 + at * 64 + qd * 16;
+                    m = p.km + at * 32 + qd * 8;
+                    l = p.kl + at * 32 + qd * 8;
+                }
+            } else {
+                const int tok = i * TILE + row;
+                // (a token that is masked away counts as zero, whatever its values are: 0 * NaN would be NaN)
+                if (tok < p.nb * BLK && !(mask && __half_as_ushort(mask[tok]) == 0xFC00u)) {
+                    const long long at = s.bh * p.L + tok;
+                    a = p.v8 + at * D + half * 64 + qd * 16;
+                    m = p.vm + at * (D / 2) + half * 32 + qd * 8;
+                    l = p.vl + at * (D / 2) + half * 32 + qd * 8;
+                }
+            }
+            uint4 x = make_uint4(0, 0, 0, 0), y = x;
+            if (a) {
+                x = ldg128(a);
+                if (tail) {
+                    y = ldg128(a + 16);
+                } else {
+                    const uint2 b = ldg64(m), c = ldg64(l);
+                    y = make_uint4(b.x, b.y, c.x, c.y);
+                }
+            }
+            w[u][0] = x.x; w[u][1] = x.y; w[u][2] = x.z; w[u][3] = x.w;
+            w[u][4] = y.x; w[u][5] = y.y; w[u][6] = y.z; w[u][7] = y.w;
+        }
+    }
+    // Whether the tail's values hold one that is not finite (those are stored as zeros).
+    __device__ __forceinline__ bool store(uint32_t to, int warp, int lane) {
+        bool odd = false;
+        const int qd = lane & 3;
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u) {
+            int half, row;
+            where(u, warp, lane, !value && !tail, half, row);
+            uint4 x, y;
+            if (tail) {
+                if (value) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[u][j] = finite_halves(w[u][j], odd);
+                }
+                x = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
+                y = make_uint4(w[u][4], w[u][5], w[u][6], w[u][7]);
+            } else {
+                x = halves8(w[u][0], w[u][1], w[u][4], w[u][6]);
+                y = halves8(w[u][2], w[u][3], w[u][5], w[u][7]);
+            }
+            const uint32_t at = to + half * (!value && !tail ? D * 128 : 16384) + row * 128;
+            const uint32_t c0 = ((2 * qd) ^ (row & 7)) << 4;
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at + c0), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at + (c0 ^ 16)), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+        }
+        return odd;
+    }
+};
+
+template <int D>
+__device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t base, uint32_t bars, volatile int* dead, volatile int* odd,
+                                            long long first, long long last, int warp, int lane) {
+    // two pieces under way: the one that is stored next and the one behind it
+    Piece<D> x[2];
+    Segment s;
+    long long tile = first;
+    int q = 0, index = 0;
+    int seg_of[2];
+    s.at(p, tile, last);
+    auto advance = [&]() {
+        if (++q == 2 * s.c) {
+            q = 0;
+            ++index;
+            tile += s.c;
+            if (tile < last) s.at(p, tile, last);
+        }
+    };
+    const long long count = 2 * (last - first);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        seg_of[i] = index;
+        x[i].load(p, s, q, warp, lane);            // (at least two: a K and a V tile)
+        advance();
+    }
+    for (long long n = 0; n < count; n += 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int buf = (int)((n + i) % RING);
+            const uint32_t turn = (uint32_t)((n + i) / RING);
+            bar_wait(bars + 8 * (EMPTY + buf), (turn & 1) ^ 1, dead);
+            if (x[i].store(base + Plan<D>::RING_AT + buf * Plan<D>::TILE_BYTES, warp, lane)) odd[seg_of[i] & 3] = seg_of[i] + 1;
+            fence_shared();
+            __syncwarp();
+            if (lane == 0) bar_arrive(bars + 8 * (FULL + buf));
+            if (tile < last) {
+                seg_of[i] = index;
+                x[i].load(p, s, q, warp, lane);
+                advance();
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- products
+template <int D>
+__device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, uint32_t bars, uint32_t tmem, volatile int* dead,
+                                             long long first, long long last) {
+    const int ahead = 3 - p.groups;
+    long long passed = 0;                          // operand tiles of the segments before
+    uint32_t items[2] = {0, 0}, seg = 0;           // of each slot so far
+    for (long long tile = first; tile < last; ++seg) {
+        Segment s;
+        s.at(p, tile, last);
+        tile += s.c;
+        bar_wait(bars + 8 * Q_FULL, seg & 1, dead);
+        fence_after();
+        const int n_items = p.groups * s.c;
+        auto operand_at = [&](int n, bool value, int& buf) {
+            const long long pos = passed + place_of(p.groups == 1 ? n : n >> 1, value, s.c, ahead);
+            buf = (int)(pos % RING);
+            bar_wait(bars + 8 * (FULL + buf), (uint32_t)(pos / RING) & 1, dead);
+            return base + Plan<D>::RING_AT + buf * Plan<D>::TILE_BYTES;
+        };
+        auto scores = [&](int n) {
+            const int slot = n & 1;
+            const bool tail = s.t0 + (p.groups == 1 ? n : n >> 1) == p.tiles - 1;
+            int buf;
+            const uint32_t k = operand_at(n, false, buf);
+            const uint32_t q = base + (p.groups == 2 && slot ? Plan<D>::Q2_AT : Plan<D>::Q_AT);
+            fence_after();
+            const uint32_t idesc = instruction(TILE, !tail);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t major = (kk >> 2) * 16384 + (kk & 3) * 32;           // K-major: 16 channels of rows of 64
+                mma_ss(tmem + slot * TILE, operand(q + major, 16, 1024),
+                       tail ? operand(k + major, 16, 1024) : operand(k + kk * 2048, D * 128, 1024), idesc, kk > 0);
+            }
+            commit(bars + 8 * (S_FULL + slot));
+            if (p.groups == 1 || slot) commit(bars + 8 * (EMPTY + buf));
+        };
+        scores(0);
+        if (n_items > 1) scores(1);
+        for (int n = 0; n < n_items; ++n) {
+            const int slot = n & 1;
+            bar_wait(bars + 8 * (P_FULL + slot), items[slot] & 1, dead);
+            int buf;
+            const uint32_t v = operand_at(n, true, buf);
+            fence_after();
+#pragma unroll
+            for (int kk = 0; kk < TILE / 16; ++kk)
+                mma_ts(tmem + 256 + slot * 128, tmem + slot * TILE + kk * 8, operand(v + kk * 2048, 16384, 1024), instruction(D, true),
+                       n >= 2 || kk > 0);
+            commit(bars + 8 * (O_FULL + slot));
+            if (p.groups == 1 || slot) commit(bars + 8 * (EMPTY + buf));
+            if (n + 2 < n_items) {
+                // (S takes P's place: the product that reads P has to be over)
+                bar_wait(bars + 8 * (O_FULL + slot), items[slot] & 1, dead);
+                fence_after();
+                scores(n + 2);
+            }
+            ++items[slot];
+        }
+        passed += 2 * s.c;
+    }
+}
+
+// ---------------------------------------------------------------- softmax
+// What a row of the tail sees of it, and scores at the edges: x = score to base 2 of tile token `tok`, or -inf.
+struct Edge {
+    const __half* mask;         // of the tile's first token, or nullptr
+    int count, rest;            // tokens of the tile; of them cached (the others are drafted)
+    unsigned long long seen;    // drafted tokens that the row sees
+    __device__ __forceinline__ float operator()(float x, float scale2, int tok) const {
+        if (tok < rest) {
+            const float add = mask ? __half2float(mask[tok]) : 0.f;
+            return add == -INFINITY ? -INFINITY : fmaf(x, scale2, add * LOG2E);
+        }
+        return tok < count && (seen >> ((tok - rest) & 63) & 1) ? x * scale2 : -INFINITY;
+    }
+};
+
+// p . v of the tail values that are not finite (they are zeros in the operand), for 32 channels of a row: the rare way.
+template <int D>
+__device__ __noinline__ void add_odd(const TreeArgs& p, const Segment& s, int r, unsigned long long seen, float base, int ch0,
+                                     float* o) {
+    const __half* q = p.q + row_of(p, s.b, s.h, r) * D;
+    const __half* mask = p.mask ? p.mask + s.b * p.mask_stride + p.nb * BLK : nullptr;
+    for (int i = 0; i < p.tail; ++i) {
+        const int d = i - p.rest;
+        const __half* k = d < 0 ? p.restk + ((s.b * BLK + i) * p.H + s.h) * D : p.kd + ((s.b * p.T + d) * p.H + s.h) * D;
+        const __half* v = d < 0 ? p.restv + ((s.b * BLK + i) * p.H + s.h) * D : p.vd + ((s.b * p.T + d) * p.H + s.h) * D;
+        const float add = d < 0 && mask ? __half2float(mask[i]) : 0.f;
+        if (d < 0 ? add == -INFINITY : !(seen >> d & 1)) continue;
+        float pr = -1.f;
+        for (int c = 0; c < 32; ++c) {
+            const float x = __half2float(v[ch0 + c]);
+            if (isfinite(x)) continue;
+            if (pr < 0.f) {
+                float dot = 0.f;
+                for (int j = 0; j < D; ++j) dot = fmaf(__half2float(q[j]), __half2float(k[j]), dot);
+                pr = ex2(fmaf(dot, p.scale2, add * LOG2E) - base);
+            }
+            o[c] += pr * x;
+        }
+    }
+}
+
+template <int D>
+__device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, uint32_t base, uint32_t bars, uint32_t tmem,
+                                             volatile int* dead, volatile int* odd, long long first, long long last, int warp, int lane) {
+    const int slot = warp >> 2, idx = (warp & 3) * 32 + lane, R = p.T * p.G, group = p.groups == 2 ? slot : 0;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + slot * TILE, o_at = tmem + lanes + 256 + slot * 128;
+    const float scale2 = fabsf(p.scale2);          // (the queries take the sign)
+    const uint32_t sign = p.scale2 < 0.f ? 0x80008000u : 0u;
+    float* xm = reinterpret_cast<float*>(smem + Plan<D>::XM_AT);
+    float* xl = reinterpret_cast<float*>(smem + Plan<D>::XL_AT);
+    uint32_t done = 0;
+    int seg = 0;
+    for (long long tile = first; tile < last; ++seg) {
+        Segment s;
+        s.at(p, tile, last);
+        tile += s.c;
+        const int of_unit = group * p.rowsg + idx, r = s.super * p.rowsu + of_unit;
+        const bool mine = idx < p.rowsg && of_unit < p.rowsu && r < R;
+        const bool busy = __any_sync(0xFFFFFFFFu, mine);
+        // queries: 16-byte piece c of a row's half at c ^ (row & 7)
+        soft_sync();
+        {
+            const uint4* src = reinterpret_cast<const uint4*>(p.q + (mine ? row_of(p, s.b, s.h, r) : 0) * D);
+            const uint32_t to = base + (group ? Plan<D>::Q2_AT : Plan<D>::Q_AT) + idx * 128;
+            const int c0 = p.groups == 1 ? slot * (D / 16) : 0, c1 = p.groups == 1 ? c0 + D / 16 : D / 8;
+            for (int c = c0; c < c1; ++c) {
+                uint4 x = mine ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(to + (c >> 3) * Plan<D>::Q_HALF + (((c & 7) ^ (idx & 7)) << 4)),
+                             "r"(x.x ^ sign), "r"(x.y ^ sign), "r"(x.z ^ sign), "r"(x.w ^ sign) : "memory");
+            }
+            fence_shared();
+            __syncwarp();
+            if (lane == 0) bar_arrive(bars + 8 * Q_FULL);
+        }
+        const bool with_tail = s.t0 + s.c == p.tiles;
+        unsigned long long seen = 0;
+        if (with_tail && mine) {
+            const uint8_t* row = p.tree + s.b * p.tree_stride + (long long)(r / p.G) * p.T;
+            for (int d = 0; d < p.T; ++d) seen |= (unsigned long long)(row[d] != 0) << d;
+        }
+        const __half* mask = p.mask ? p.mask + s.b * p.mask_stride : nullptr;
+        float ref = -INFINITY, l = 0.f;
+        const int n_items = p.groups * s.c;
+        bool any = false;
+        for (int n = slot; n < n_items; n += 2, ++done) {
+            const int i = s.t0 + (p.groups == 1 ? n : n >> 1);
+            bar_wait(bars + 8 * (S_FULL + slot), done & 1, dead);
+            __syncwarp();
+            fence_after();
+            if (busy) {
+                const bool tail = i == p.tiles - 1;
+                Edge edge;
+                edge.count = tail ? p.tail : min(TILE, p.nb * BLK - i * TILE);
+                edge.rest = tail ? p.rest : edge.count;
+                edge.mask = mask ? mask + (long long)min(i * TILE, p.nb * BLK) : nullptr;
+                edge.seen = seen;
+                const bool plain = !tail && !mask && edge.count == TILE;
+                uint32_t v[32];
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < TILE; c += 32) {
+                    __syncwarp();
+                    tmem_ld(v, s_at + c);
+                    if (plain) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(v[j]));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) top = fmaxf(top, edge(__uint_as_float(v[j]), scale2, c + j));
+                    }
+                }
+                if (plain) top *= scale2;
+                const bool up = top > ref + SLACK;           // (-inf: the first score that is there)
+                if (__any_sync(0xFFFFFFFFu, up)) {
+                    const float to = fmaxf(ref, top), keep = ref == -INFINITY ? 0.f : ex2(ref - to);
+                    ref = to;
+                    l *= keep;
+                    if (any) {
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            tmem_ld(v, o_at + c);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * keep);
+                            tmem_st32(o_at + c, v);
+                        }
+                    }
+                }
+                const float off = (ref == -INFINITY ? 0.f : ref) - WIDE_LIFT;
+#pragma unroll 1
+                for (int c = 0; c < TILE; c += 32) {
+                    __syncwarp();
+                    tmem_ld(v, s_at + c);
+                    uint32_t h[16];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        float a, b;
+                        if (plain) {
+                            a = fmaf(__uint_as_float(v[j]), scale2, -off);
+                            b = fmaf(__uint_as_float(v[j + 1]), scale2, -off);
+                        } else {
+                            a = edge(__uint_as_float(v[j]), scale2, c + j) - off;
+                            b = edge(__uint_as_float(v[j + 1]), scale2, c + j + 1) - off;
+                        }
+                        a = ex2(a);
+                        b = ex2(b);
+                        l += a;
+                        l += b;
+                        h[j / 2] = pack_half2(a, b);
+                    }
+                    __syncwarp();
+                    tmem_st16(s_at + c / 2, h);
+                }
+                tmem_st_wait();
+                any = true;
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(bars + 8 * (P_FULL + slot));
+        }
+        // ---- the segment's result: with one group the slots' two, joined
+        const bool have = n_items > slot;
+        if (have) bar_wait(bars + 8 * (O_FULL + slot), (done - 1) & 1, dead);
+        __syncwarp();
+        fence_after();
+        float f0 = 1.f, f1 = 0.f;
+        if (p.groups == 1) {
+            if (slot) {
+                xm[idx] = have ? ref : -INFINITY;
+                xl[idx] = have ? l : 0.f;
+            }
+            soft_sync();
+            if (!slot && n_items > 1) {
+                const float to = fmaxf(ref, xm[idx]);
+                f0 = ref == -INFINITY ? 0.f : ex2(ref - to);
+                f1 = xm[idx] == -INFINITY ? 0.f : ex2(xm[idx] - to);
+                // (a sum that is not a number stays one: 0 * NaN)
+                l = f0 * l + f1 * xl[idx];
+                ref = to;
+            }
+        }
+        const bool whole = s.c == p.tiles, odd_tail = with_tail && odd[seg & 3] == seg + 1;
+        if (*dead) l = __int_as_float(0x7FC00000);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int rec_slot = s.unit != first / p.tiles;
+        float* rec = p.part + ((2 * (long long)blockIdx.x + rec_slot) * p.rowsu + of_unit) * (D + 4);
+        float4* join = reinterpret_cast<float4*>(smem + Plan<D>::Q2_AT);              // [16 channel quads][128 rows]
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            if (p.groups == 1 && c % 64 == 0) {
+                if (c > 0) soft_sync();
+                if (slot && have && busy) {
+#pragma unroll 1
+                    for (int e = 0; e < 64; e += 32) {
+                        uint32_t v[32];
+                        __syncwarp();
+                        tmem_ld(v, o_at + c + e);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            join[(e / 4 + j) * 128 + idx] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
+                                                                        __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
+                    }
+                }
+                soft_sync();
+            }
+            if ((p.groups == 1 && slot) || !busy) continue;
+            uint32_t v[32];
+            __syncwarp();
+            tmem_ld(v, o_at + c);
+            float o[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(v[j]);
+            if (p.groups == 1 && n_items > 1) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float4 x = join[((c & 63) / 4 + j) * 128 + idx];
+                    o[4 * j] = fmaf(o[4 * j], f0, x.x * f1);
+                    o[4 * j + 1] = fmaf(o[4 * j + 1], f0, x.y * f1);
+                    o[4 * j + 2] = fmaf(o[4 * j + 2], f0, x.z * f1);
+                    o[4 * j + 3] = fmaf(o[4 * j + 3], f0, x.w * f1);
+                }
+            }
+            if (!mine) continue;
+            if (odd_tail) {
+                float x[32];
+                for (int j = 0; j < 32; ++j) x[j] = 0.f;
+                add_odd<D>(p, s, r, seen, (ref == -INFINITY ? 0.f : ref) - WIDE_LIFT, c, x);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] += x[j];
+            }
+            if (whole) {
+                uint4* dst = reinterpret_cast<uint4*>(p.out + row_of(p, s.b, s.h, r) * D + c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    dst[j] = make_uint4(pack_half2(o[8 * j] * inv, o[8 * j + 1] * inv), pack_half2(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
+                                        pack_half2(o[8 * j + 4] * inv, o[8 * j + 5] * inv), pack_half2(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    reinterpret_cast<float4*>(rec + 4 + c)[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            }
+        }
+        if (mine && !(p.groups == 1 && slot)) {
+            if (!whole) {
+                rec[0] = ref + (LIFT - WIDE_LIFT);
+                rec[1] = l;
+            } else if (p.lse) {
+                p.lse[row_of(p, s.b, s.h, r)] = l == 0.f ? -INFINITY : (ref - WIDE_LIFT + log2f(l)) * LN2;
+            }
+        }
+        fence_before();
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p) {
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    const uint32_t base = smem_u32(smem), bars = base + Plan<D>::BAR_AT;
+    uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(smem + Plan<D>::BAR_AT + 8 * BARS);
+    volatile int* dead = reinterpret_cast<volatile int*>(slot_tmem + 1);
+    volatile int* odd = dead + 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < RING; ++i) {
+            bar_init(bars + 8 * (FULL + i), DECODE);
+            bar_init(bars + 8 * (EMPTY + i), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(bars + 8 * (S_FULL + i), 1);
+            bar_init(bars + 8 * (P_FULL + i), SOFT / 2);
+            bar_init(bars + 8 * (O_FULL + i), 1);
+        }
+        bar_init(bars + 8 * Q_FULL, SOFT);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        *dead = 0;
+        for (int i = 0; i < 4; ++i) odd[i] = 0;
+    }
+    // (the memory is taken once the kernel in front is over: it might want some, and this one would hold it while it waits)
+    pdl_enter();
+    __syncwarp();
+    if (warp == SOFT + DECODE) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(slot_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(slot_tmem);
+    const long long w = blockIdx.x, first = w * p.total / p.nw, last = (w + 1) * p.total / p.nw;
+    if (warp < SOFT) {
+        softmax_role<D>(p, smem, base, bars, tmem, dead, odd, first, last, warp, lane);
+    } else if (warp < SOFT + DECODE) {
+        decode_role<D>(p, base, bars, dead, odd, first, last, warp - SOFT, lane);
+    } else if (lane == 0) {
+        product_role<D>(p, base, bars, tmem, dead, first, last);
+    }
+    __syncwarp();
+    __syncthreads();
+    if (*dead) {
+        // (never expected) products may still run: time for them to end before their memory is released
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+        __syncthreads();
+    }
+    fence_after();
+    if (warp == SOFT + DECODE)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+}
+
+}  // namespace
+
+int launch_tree_wide(const TreeArgs& p, int D, int ctas, cudaStream_t st) {
+    auto kernel = D == 128 ? tree_wide_kernel<128> : tree_wide_kernel<64>;
+    const int bytes = D == 128 ? Plan<128>::BYTES : Plan<64>::BYTES;
+    const int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                               "tree_attention shared memory");
+    if (rc != AKV_OK) return rc;
+    launch_chained(kernel, dim3(ctas), dim3(THREADS), (size_t)bytes, st, p);
+    return AKV_OK;
+}
+
+}  // namespace akv

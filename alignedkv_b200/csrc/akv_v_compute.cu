@@ -656,9 +656,11 @@ int launch_v_split_stream(const uint8_t* first8, const uint8_t* mid4, const uint
     return launch_v_stream(p, BH, st);
 }
 
-// (the peer exchange kernel keeps a flag of its own: akv_exchange.cu)
+// (the peer exchange kernel and the tree attention keep flags of their own: akv_exchange.cu, akv_tree_wide.cu)
 unsigned int exchange_error_flag(cudaError_t* e);
 cudaError_t exchange_error_clear();
+unsigned int tree_error_flag(cudaError_t* e);
+cudaError_t tree_error_clear();
 
 }  // namespace akv
 
@@ -670,6 +672,8 @@ extern "C" int akv_device_error_flag(void) {
     if (e != cudaSuccess) return akv::cuda_status(e, "device_error_flag");
     v |= akv::exchange_error_flag(&e);
     if (e != cudaSuccess) return akv::cuda_status(e, "device_error_flag");
+    v |= akv::tree_error_flag(&e);
+    if (e != cudaSuccess) return akv::cuda_status(e, "device_error_flag");
     return (int)v;
 }
 
@@ -678,6 +682,7 @@ extern "C" int akv_device_error_clear(void) {
     const unsigned int v = 0;
     cudaError_t e = cudaMemcpyToSymbol(akv::g_v_wait_gave_up, &v, sizeof(v));
     if (e == cudaSuccess) e = akv::exchange_error_clear();
+    if (e == cudaSuccess) e = akv::tree_error_clear();
     if (e != cudaSuccess) return akv::cuda_status(e, "device_error_clear");
     return AKV_OK;
 }
