@@ -1,7 +1,8 @@
 // Attention of drafted tokens where more than 16 query rows share a KV head: the fifth-generation tensor cores.
 //
 // CTA = one SM, a contiguous run of 128-token tiles as in akv_tree.cu; a unit is up to 256 query rows of a (batch, KV head).
-//   warps 8..15   decode: plane bytes from global memory to registers two tiles ahead, there to fp16, and into a ring of operand tiles
+//   warp  17      one thread copies the planes of a tile (K or V: 32 KB at head size 128) into a ring, three to six bulk copies each
+//   warps 8..15   decode: a ring tile's bytes to fp16 operands in the same place - they take as much - by way of registers
 //   warp  16      one thread issues the products: S = Q K^T (128 rows x 128 tokens), O += P V
 //   warps 0..7    two softmax groups of 128 threads, a thread per query row: S from tensor memory, P back into its place
 // Everything comes in twos: S, O, P and a softmax group per slot.  With up to 128 rows the slots take the tiles in turn (each
@@ -11,6 +12,8 @@
 // are "MN-major", rows of 64 elements (128 bytes), so that a decoded piece of 16 elements is two 16-byte stores.  Only the
 // tail's keys (fp16 rows of channels) are K-major.
 // Tensor memory: columns 0..255 S (P in the same columns as fp16), 256..511 O.
+#include <limits.h>
+
 #include "akv_tree.cuh"
 
 namespace akv {
@@ -28,21 +31,24 @@ cudaError_t tree_error_clear() {
 
 namespace {
 
-constexpr int SOFT = 8, DECODE = 8, THREADS = 32 * (SOFT + DECODE + 1), RING = 4;
+constexpr int SOFT = 8, DECODE = 8, THREADS = 32 * (SOFT + DECODE + 2);
 // A row's reference maximum moves only when a score exceeds it by 2^SLACK: probabilities are at most 2^(WIDE_LIFT + SLACK) in fp16.
 constexpr float WIDE_LIFT = 7.f, SLACK = 8.f;
 
 template <int D>
 struct Plan {
+    static constexpr int RING = D == 128 ? 5 : 8;
     static constexpr int TILE_BYTES = TILE * D * 2, Q_HALF = 16384, Q_BYTES = Q_HALF * (D / 64);
     static constexpr int RING_AT = 0, Q_AT = RING * TILE_BYTES;
     // the second row group's queries; with one group the place where the slots' outputs are joined (128 rows x 64 channels)
     static constexpr int JOIN_BYTES = 128 * 64 * 4, Q2_AT = Q_AT + Q_BYTES;
     static constexpr int XM_AT = Q2_AT + (Q_BYTES > JOIN_BYTES ? Q_BYTES : JOIN_BYTES), XL_AT = XM_AT + 512;
-    static constexpr int BAR_AT = XL_AT + 512, BYTES = BAR_AT + 256 + 1024;     // (1024: the base is aligned up)
+    // barriers, 8 bytes each, then the tensor memory's address, the flag that a wait gave up, odd values of the last segments
+    static constexpr int BAR_AT = XL_AT + 512, RAW = 0, FULL = RING, EMPTY = 2 * RING, S_FULL = 3 * RING, P_FULL = S_FULL + 2,
+                         O_FULL = P_FULL + 2, Q_FULL = O_FULL + 2, BARS = Q_FULL + 1;
+    static constexpr int SEGMENTS = 8, BYTES = BAR_AT + 8 * BARS + 8 + 4 * SEGMENTS + 1024;      // (1024: the base is aligned up)
 };
-// barriers, 8 bytes each, then the tensor memory's address, the flag that a wait gave up, odd values of the last four segments
-enum Bar { FULL = 0, EMPTY = RING, S_FULL = 2 * RING, P_FULL = S_FULL + 2, O_FULL = P_FULL + 2, Q_FULL = O_FULL + 2, BARS };
+static_assert(Plan<128>::BYTES <= 232448 && Plan<64>::BYTES <= 232448, "shared memory of a block");
 
 __device__ __forceinline__ void bar_init(uint32_t a, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(a), "r"(count) : "memory");
@@ -57,7 +63,7 @@ __device__ __forceinline__ bool bar_try(uint32_t a, uint32_t parity) {
     return ok != 0;
 }
 // Bounded (about a second); once one has given up, none waits any more and the outputs become NaN.
-__device__ __noinline__ void bar_wait_slow(uint32_t a, uint32_t parity, volatile int* dead) {
+__device__ __forceinline__ void bar_wait_slow(uint32_t a, uint32_t parity, volatile int* dead) {
     unsigned long long t0 = 0;
     for (unsigned spin = 0; !bar_try(a, parity); ++spin) {
         if (*dead) return;
@@ -131,6 +137,15 @@ __device__ __forceinline__ void soft_sync() {
     asm volatile("bar.sync 1, %0;\n" ::"n"(32 * SOFT) : "memory");
 }
 
+__device__ __forceinline__ void decode_sync() {
+    __syncwarp();
+    asm volatile("bar.sync 2, %0;\n" ::"n"(32 * DECODE) : "memory");
+}
+__device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
 // ---------------------------------------------------------------- the run of a CTA, piece by piece
 // Segment: consecutive tiles t0 .. t0 + c - 1 of one unit.
 struct Segment {
@@ -165,16 +180,6 @@ __device__ __forceinline__ int place_of(int i, bool value, int c, int ahead) {
 }
 
 // ---------------------------------------------------------------- decode
-__device__ __forceinline__ uint4 ldg128(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 ldg64(const void* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
 // Eight elements in order from their high bytes and nibbles.
 __device__ __forceinline__ uint4 halves8(uint32_t h0, uint32_t h1, uint32_t m, uint32_t l) {
     const uint32_t even = (m & 0xF0F0F0F0u) | ((l >> 4) & 0x0F0F0F0Fu), odd = ((m << 4) & 0xF0F0F0F0u) | (l & 0x0F0F0F0Fu);
@@ -187,134 +192,139 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w, bool& odd) {
     return w;
 }
 
-// What is decoded: operand tile `q` of the segment, in pieces of 16 elements: a thread takes D / 32 of them.
+// Raw tile in its ring slot: K [block][channel][64] high bytes, then [block][channel][32] twice; V [token][D], then [token][D / 2] twice.
 template <int D>
-struct Piece {
-    uint32_t w[D / 32][8];
-    bool value, tail;
-
-    // Piece u of a thread: quarter lane % 4 of (half, row).  Rows of 128 bytes: K planes [block][channel], else [channel half][token].
-    static __device__ __forceinline__ void where(int u, int warp, int lane, bool k_plane, int& half, int& row) {
-        const int i = u * DECODE + warp, halves = k_plane ? 2 : D / 64;
-        half = i & (halves - 1);
-        row = (halves == 2 ? i >> 1 : i) * 8 + (lane >> 2);
-    }
-    __device__ __forceinline__ void load(const TreeArgs& p, const Segment& s, int q, int warp, int lane) {
-        const int i = s.t0 + tile_of(q, s.c, 3 - p.groups, value);
-        tail = i == p.tiles - 1;
-        const int qd = lane & 3;
-        const __half* mask = p.mask ? p.mask + s.b * p.mask_stride : nullptr;
-#pragma unroll
-        for (int u = 0; u < D / 32; ++u) {
-            int half, row;
-            where(u, warp, lane, !value && !tail, half, row);
-            const uint8_t *a = nullptr, *m = nullptr, *l = nullptr;
-            if (tail) {
-                if (row < p.tail) {
-                    const int d = row - p.rest;
-                    const __half* src = d < 0 ? (value ? p.restv : p.restk) + ((s.b * BLK + row) * p.H + s.h) * D
-                                              : (value ? p.vd : p.kd) + ((s.b * p.T + d) * p.H + s.h) * D;
-                    a = reinterpret_cast<const uint8_t*>(src + half * 64 + qd * 16);
-                }
-            } else if (!value) {
-                if (2 * i + half < p.nb) {
-                    const long long at = (s.bh * p.nmb + 2 * i + half) * D + row;
-                    a = p.k8 + at * 64 + qd * 16;
-                    m = p.km + at * 32 + qd * 8;
-                    l = p.kl + at * 32 + qd * 8;
-                }
+__device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t base, uint32_t bars, volatile int* dead, long long first,
+                                          long long last) {
+    using L = Plan<D>;
+    uint32_t buf = 0, turn = 0;
+    for (long long tile = first; tile < last;) {
+        Segment s;
+        s.at(p, tile, last);
+        tile += s.c;
+        for (int q = 0; q < 2 * s.c; ++q) {
+            bool value;
+            const int i = s.t0 + tile_of(q, s.c, 3 - p.groups, value);
+            const uint32_t to = base + L::RING_AT + buf * L::TILE_BYTES, bar = bars + 8 * (L::RAW + buf);
+            bar_wait(bars + 8 * (L::EMPTY + buf), (turn & 1) ^ 1, dead);
+            if (i == p.tiles - 1) {
+                bar_arrive(bar);                       // (the tail is read by the decoding warps themselves)
             } else {
-                const int tok = i * TILE + row;
-                // (a token that is masked away counts as zero, whatever its values are: 0 * NaN would be NaN)
-                if (tok < p.nb * BLK && !(mask && __half_as_ushort(mask[tok]) == 0xFC00u)) {
-                    const long long at = s.bh * p.L + tok;
-                    a = p.v8 + at * D + half * 64 + qd * 16;
-                    m = p.vm + at * (D / 2) + half * 32 + qd * 8;
-                    l = p.vl + at * (D / 2) + half * 32 + qd * 8;
-                }
-            }
-            uint4 x = make_uint4(0, 0, 0, 0), y = x;
-            if (a) {
-                x = ldg128(a);
-                if (tail) {
-                    y = ldg128(a + 16);
+                const int blocks = min(2, p.nb - 2 * i);
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(blocks * BLK * D * 2) : "memory");
+                if (!value) {
+                    const long long at = (s.bh * p.nmb + 2 * i) * D;
+                    for (int b = 0; b < blocks; ++b) {
+                        bulk(to + b * D * BLK, p.k8 + (at + b * D) * BLK, D * BLK, bar);
+                        bulk(to + D * TILE + b * D * (BLK / 2), p.km + (at + b * D) * (BLK / 2), D * (BLK / 2), bar);
+                        bulk(to + D * TILE * 3 / 2 + b * D * (BLK / 2), p.kl + (at + b * D) * (BLK / 2), D * (BLK / 2), bar);
+                    }
                 } else {
-                    const uint2 b = ldg64(m), c = ldg64(l);
-                    y = make_uint4(b.x, b.y, c.x, c.y);
+                    const long long at = s.bh * p.L + i * TILE;
+                    bulk(to, p.v8 + at * D, blocks * BLK * D, bar);
+                    bulk(to + D * TILE, p.vm + at * (D / 2), blocks * BLK * (D / 2), bar);
+                    bulk(to + D * TILE * 3 / 2, p.vl + at * (D / 2), blocks * BLK * (D / 2), bar);
                 }
             }
-            w[u][0] = x.x; w[u][1] = x.y; w[u][2] = x.z; w[u][3] = x.w;
-            w[u][4] = y.x; w[u][5] = y.y; w[u][6] = y.z; w[u][7] = y.w;
-        }
-    }
-    // Whether the tail's values hold one that is not finite (those are stored as zeros).
-    __device__ __forceinline__ bool store(uint32_t to, int warp, int lane) {
-        bool odd = false;
-        const int qd = lane & 3;
-#pragma unroll
-        for (int u = 0; u < D / 32; ++u) {
-            int half, row;
-            where(u, warp, lane, !value && !tail, half, row);
-            uint4 x, y;
-            if (tail) {
-                if (value) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) w[u][j] = finite_halves(w[u][j], odd);
-                }
-                x = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
-                y = make_uint4(w[u][4], w[u][5], w[u][6], w[u][7]);
-            } else {
-                x = halves8(w[u][0], w[u][1], w[u][4], w[u][6]);
-                y = halves8(w[u][2], w[u][3], w[u][5], w[u][7]);
+            if (++buf == L::RING) {
+                buf = 0;
+                ++turn;
             }
-            const uint32_t at = to + half * (!value && !tail ? D * 128 : 16384) + row * 128;
-            const uint32_t c0 = ((2 * qd) ^ (row & 7)) << 4;
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at + c0), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at + (c0 ^ 16)), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
         }
-        return odd;
     }
-};
+}
 
+// Operand rows of 128 bytes: K planes [block][channel], else [channel half][token].  A thread has U = D / 32 pieces of 16 elements:
+// quarter lane % 4 of rows `row` + u * `step` of one half.  (Neighbouring rows of V in different halves: neither the loads of the
+// bytes nor the stores of the operands meet in a bank.)
 template <int D>
 __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t base, uint32_t bars, volatile int* dead, volatile int* odd,
                                             long long first, long long last, int warp, int lane) {
-    // two pieces under way: the one that is stored next and the one behind it
-    Piece<D> x[2];
-    Segment s;
-    long long tile = first;
-    int q = 0, index = 0;
-    int seg_of[2];
-    s.at(p, tile, last);
-    auto advance = [&]() {
-        if (++q == 2 * s.c) {
-            q = 0;
-            ++index;
-            tile += s.c;
-            if (tile < last) s.at(p, tile, last);
-        }
-    };
-    const long long count = 2 * (last - first);
+    using L = Plan<D>;
+    constexpr int U = D / 32;
+    const int qd = lane & 3, k = lane >> 2;
+    uint32_t buf = 0, turn = 0;
+    int index = 0;
+    for (long long tile = first; tile < last; ++index) {
+        Segment s;
+        s.at(p, tile, last);
+        tile += s.c;
+#pragma unroll 1
+        for (int q = 0; q < 2 * s.c; ++q) {
+            bool value;
+            const int i = s.t0 + tile_of(q, s.c, 3 - p.groups, value);
+            const bool tail = i == p.tiles - 1, by_channel = !value && !tail;
+            const int half = by_channel ? warp & 1 : D == 128 ? (warp ^ k) & 1 : 0;
+            const int row = (D == 128 || by_channel ? warp >> 1 : warp) * 8 + k, step = D == 128 || by_channel ? 32 : 64;
+            const uint32_t slot = base + L::RING_AT + buf * L::TILE_BYTES;
+            bar_wait(bars + 8 * (L::RAW + buf), turn & 1, dead);
+            uint32_t w[U][8];
+            if (!tail) {
+                const uint32_t h = slot + (by_channel ? half * D * BLK + row * 64 : row * D + half * 64) + qd * 16;
+                const uint32_t n = slot + D * TILE + (by_channel ? half * D * 32 + row * 32 : row * (D / 2) + half * 32) + qd * 8;
+                const uint32_t hs = step * (by_channel ? 64 : D), ns = hs / 2;
+                const uint16_t* mask = value && p.mask ? reinterpret_cast<const uint16_t*>(p.mask) + s.b * p.mask_stride + i * TILE : nullptr;
+                const int some = by_channel ? 2 * i + half < p.nb ? D : 0 : p.nb * BLK - i * TILE;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        seg_of[i] = index;
-        x[i].load(p, s, q, warp, lane);            // (at least two: a K and a V tile)
-        advance();
-    }
-    for (long long n = 0; n < count; n += 2) {
+                for (int u = 0; u < U; ++u) {
+                    const uint4 x = lds128(h + u * hs);
+                    const uint2 m = lds64(n + u * ns), l = lds64(n + D * BLK + u * ns);
+                    w[u][0] = x.x; w[u][1] = x.y; w[u][2] = x.z; w[u][3] = x.w;
+                    w[u][4] = m.x; w[u][5] = m.y; w[u][6] = l.x; w[u][7] = l.y;
+                }
+                if (mask || some < TILE) {
+                    // (a token that does not exist or is masked away counts as zero, whatever there is: 0 * NaN would be NaN)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int buf = (int)((n + i) % RING);
-            const uint32_t turn = (uint32_t)((n + i) / RING);
-            bar_wait(bars + 8 * (EMPTY + buf), (turn & 1) ^ 1, dead);
-            if (x[i].store(base + Plan<D>::RING_AT + buf * Plan<D>::TILE_BYTES, warp, lane)) odd[seg_of[i] & 3] = seg_of[i] + 1;
+                    for (int u = 0; u < U; ++u) {
+                        const int r = row + u * step;
+                        if (r >= some || (mask && mask[r] == 0xFC00u)) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) w[u][j] = 0;
+                        }
+                    }
+                }
+                decode_sync();                         // all bytes are in registers
+            } else {
+                bool mine = false;
+                const __half *rest = value ? p.restv : p.restk, *drafted = value ? p.vd : p.kd;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int x = row + u * step, d = x - p.rest;
+                    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+                    if (x < p.tail) {
+                        const __half* src = d < 0 ? rest + ((s.b * BLK + x) * p.H + s.h) * D : drafted + ((s.b * p.T + d) * p.H + s.h) * D;
+                        const uint4* from = reinterpret_cast<const uint4*>(src + half * 64 + qd * 16);
+                        a = __ldg(from);
+                        b = __ldg(from + 1);
+                    }
+                    w[u][0] = a.x; w[u][1] = a.y; w[u][2] = a.z; w[u][3] = a.w;
+                    w[u][4] = b.x; w[u][5] = b.y; w[u][6] = b.z; w[u][7] = b.w;
+                    // (values that are not finite: zeros here, added where a row sees them)
+                    if (value) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) w[u][j] = finite_halves(w[u][j], mine);
+                    }
+                }
+                if (mine) odd[index % L::SEGMENTS] = index + 1;
+            }
+            const uint32_t at = slot + half * (by_channel ? D * 128 : 16384) + row * 128 + (((2 * qd) ^ (row & 7)) << 4);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                uint4 x = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]), y = make_uint4(w[u][4], w[u][5], w[u][6], w[u][7]);
+                if (!tail) {
+                    const uint4 h = x, n = y;
+                    x = halves8(h.x, h.y, n.x, n.z);
+                    y = halves8(h.z, h.w, n.y, n.w);
+                }
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at + u * step * 128), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"((at ^ 16) + u * step * 128), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+            }
             fence_shared();
             __syncwarp();
-            if (lane == 0) bar_arrive(bars + 8 * (FULL + buf));
-            if (tile < last) {
-                seg_of[i] = index;
-                x[i].load(p, s, q, warp, lane);
-                advance();
+            if (lane == 0) bar_arrive(bars + 8 * (L::FULL + buf));
+            if (++buf == L::RING) {
+                buf = 0;
+                ++turn;
             }
         }
     }
@@ -325,20 +335,21 @@ template <int D>
 __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, uint32_t bars, uint32_t tmem, volatile int* dead,
                                              long long first, long long last) {
     const int ahead = 3 - p.groups;
-    long long passed = 0;                          // operand tiles of the segments before
+    using L = Plan<D>;
+    uint32_t passed = 0;                           // operand tiles of the segments before
     uint32_t items[2] = {0, 0}, seg = 0;           // of each slot so far
     for (long long tile = first; tile < last; ++seg) {
         Segment s;
         s.at(p, tile, last);
         tile += s.c;
-        bar_wait(bars + 8 * Q_FULL, seg & 1, dead);
+        bar_wait(bars + 8 * Plan<D>::Q_FULL, seg & 1, dead);
         fence_after();
         const int n_items = p.groups * s.c;
         auto operand_at = [&](int n, bool value, int& buf) {
-            const long long pos = passed + place_of(p.groups == 1 ? n : n >> 1, value, s.c, ahead);
-            buf = (int)(pos % RING);
-            bar_wait(bars + 8 * (FULL + buf), (uint32_t)(pos / RING) & 1, dead);
-            return base + Plan<D>::RING_AT + buf * Plan<D>::TILE_BYTES;
+            const uint32_t pos = passed + place_of(p.groups == 1 ? n : n >> 1, value, s.c, ahead), turn = pos / L::RING;
+            buf = (int)(pos - turn * L::RING);
+            bar_wait(bars + 8 * (L::FULL + buf), turn & 1, dead);
+            return base + L::RING_AT + buf * L::TILE_BYTES;
         };
         auto scores = [&](int n) {
             const int slot = n & 1;
@@ -354,14 +365,14 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
                 mma_ss(tmem + slot * TILE, operand(q + major, 16, 1024),
                        tail ? operand(k + major, 16, 1024) : operand(k + kk * 2048, D * 128, 1024), idesc, kk > 0);
             }
-            commit(bars + 8 * (S_FULL + slot));
-            if (p.groups == 1 || slot) commit(bars + 8 * (EMPTY + buf));
+            commit(bars + 8 * (Plan<D>::S_FULL + slot));
+            if (p.groups == 1 || slot) commit(bars + 8 * (Plan<D>::EMPTY + buf));
         };
         scores(0);
         if (n_items > 1) scores(1);
         for (int n = 0; n < n_items; ++n) {
             const int slot = n & 1;
-            bar_wait(bars + 8 * (P_FULL + slot), items[slot] & 1, dead);
+            bar_wait(bars + 8 * (Plan<D>::P_FULL + slot), items[slot] & 1, dead);
             int buf;
             const uint32_t v = operand_at(n, true, buf);
             fence_after();
@@ -369,11 +380,11 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
             for (int kk = 0; kk < TILE / 16; ++kk)
                 mma_ts(tmem + 256 + slot * 128, tmem + slot * TILE + kk * 8, operand(v + kk * 2048, 16384, 1024), instruction(D, true),
                        n >= 2 || kk > 0);
-            commit(bars + 8 * (O_FULL + slot));
-            if (p.groups == 1 || slot) commit(bars + 8 * (EMPTY + buf));
+            commit(bars + 8 * (Plan<D>::O_FULL + slot));
+            if (p.groups == 1 || slot) commit(bars + 8 * (Plan<D>::EMPTY + buf));
             if (n + 2 < n_items) {
                 // (S takes P's place: the product that reads P has to be over)
-                bar_wait(bars + 8 * (O_FULL + slot), items[slot] & 1, dead);
+                bar_wait(bars + 8 * (Plan<D>::O_FULL + slot), items[slot] & 1, dead);
                 fence_after();
                 scores(n + 2);
             }
@@ -455,7 +466,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
             }
             fence_shared();
             __syncwarp();
-            if (lane == 0) bar_arrive(bars + 8 * Q_FULL);
+            if (lane == 0) bar_arrive(bars + 8 * Plan<D>::Q_FULL);
         }
         const bool with_tail = s.t0 + s.c == p.tiles;
         unsigned long long seen = 0;
@@ -469,7 +480,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
         bool any = false;
         for (int n = slot; n < n_items; n += 2, ++done) {
             const int i = s.t0 + (p.groups == 1 ? n : n >> 1);
-            bar_wait(bars + 8 * (S_FULL + slot), done & 1, dead);
+            bar_wait(bars + 8 * (Plan<D>::S_FULL + slot), done & 1, dead);
             __syncwarp();
             fence_after();
             if (busy) {
@@ -479,22 +490,30 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                 edge.rest = tail ? p.rest : edge.count;
                 edge.mask = mask ? mask + (long long)min(i * TILE, p.nb * BLK) : nullptr;
                 edge.seen = seen;
+                // edges: scores to base 2 go back to where they came from; elsewhere they stay products until the exponential
                 const bool plain = !tail && !mask && edge.count == TILE;
+                const float mul = plain ? scale2 : 1.f;
                 uint32_t v[32];
-                float top = -INFINITY;
+                if (!plain) {
+#pragma unroll 1
+                    for (int c = 0; c < TILE; c += 32) {
+                        __syncwarp();
+                        tmem_ld(v, s_at + c);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(edge(__uint_as_float(v[j]), scale2, c + j));
+                        __syncwarp();
+                        tmem_st32(s_at + c, v);
+                    }
+                    tmem_st_wait();
+                }
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
                 for (int c = 0; c < TILE; c += 32) {
-                    __syncwarp();
                     tmem_ld(v, s_at + c);
-                    if (plain) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(v[j]));
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) top = fmaxf(top, edge(__uint_as_float(v[j]), scale2, c + j));
-                    }
+                    for (int j = 0; j < 32; ++j) tops[j & 3] = fmaxf(tops[j & 3], __uint_as_float(v[j]));
                 }
-                if (plain) top *= scale2;
+                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * mul;
                 const bool up = top > ref + SLACK;           // (-inf: the first score that is there)
                 if (__any_sync(0xFFFFFFFFu, up)) {
                     const float to = fmaxf(ref, top), keep = ref == -INFINITY ? 0.f : ex2(ref - to);
@@ -511,40 +530,31 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                     }
                 }
                 const float off = (ref == -INFINITY ? 0.f : ref) - WIDE_LIFT;
+                float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
                 for (int c = 0; c < TILE; c += 32) {
-                    __syncwarp();
                     tmem_ld(v, s_at + c);
                     uint32_t h[16];
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
-                        float a, b;
-                        if (plain) {
-                            a = fmaf(__uint_as_float(v[j]), scale2, -off);
-                            b = fmaf(__uint_as_float(v[j + 1]), scale2, -off);
-                        } else {
-                            a = edge(__uint_as_float(v[j]), scale2, c + j) - off;
-                            b = edge(__uint_as_float(v[j + 1]), scale2, c + j + 1) - off;
-                        }
-                        a = ex2(a);
-                        b = ex2(b);
-                        l += a;
-                        l += b;
+                        const float a = ex2(fmaf(__uint_as_float(v[j]), mul, -off)), b = ex2(fmaf(__uint_as_float(v[j + 1]), mul, -off));
+                        sums[j & 2] += a;
+                        sums[(j & 2) + 1] += b;
                         h[j / 2] = pack_half2(a, b);
                     }
-                    __syncwarp();
                     tmem_st16(s_at + c / 2, h);
                 }
+                l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
                 tmem_st_wait();
                 any = true;
             }
             fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(bars + 8 * (P_FULL + slot));
+            if (lane == 0) bar_arrive(bars + 8 * (Plan<D>::P_FULL + slot));
         }
         // ---- the segment's result: with one group the slots' two, joined
         const bool have = n_items > slot;
-        if (have) bar_wait(bars + 8 * (O_FULL + slot), (done - 1) & 1, dead);
+        if (have) bar_wait(bars + 8 * (Plan<D>::O_FULL + slot), (done - 1) & 1, dead);
         __syncwarp();
         fence_after();
         float f0 = 1.f, f1 = 0.f;
@@ -563,7 +573,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                 ref = to;
             }
         }
-        const bool whole = s.c == p.tiles, odd_tail = with_tail && odd[seg & 3] == seg + 1;
+        const bool whole = s.c == p.tiles, odd_tail = with_tail && odd[seg % Plan<D>::SEGMENTS] == seg + 1;
         if (*dead) l = __int_as_float(0x7FC00000);
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int rec_slot = s.unit != first / p.tiles;
@@ -641,24 +651,26 @@ __global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p)
     extern __shared__ uint8_t raw[];
     uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     const uint32_t base = smem_u32(smem), bars = base + Plan<D>::BAR_AT;
-    uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(smem + Plan<D>::BAR_AT + 8 * BARS);
+    using L = Plan<D>;
+    uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(smem + L::BAR_AT + 8 * L::BARS);
     volatile int* dead = reinterpret_cast<volatile int*>(slot_tmem + 1);
     volatile int* odd = dead + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < RING; ++i) {
-            bar_init(bars + 8 * (FULL + i), DECODE);
-            bar_init(bars + 8 * (EMPTY + i), 1);
+        for (int i = 0; i < L::RING; ++i) {
+            bar_init(bars + 8 * (L::RAW + i), 1);
+            bar_init(bars + 8 * (L::FULL + i), DECODE);
+            bar_init(bars + 8 * (L::EMPTY + i), 1);
         }
         for (int i = 0; i < 2; ++i) {
-            bar_init(bars + 8 * (S_FULL + i), 1);
-            bar_init(bars + 8 * (P_FULL + i), SOFT / 2);
-            bar_init(bars + 8 * (O_FULL + i), 1);
+            bar_init(bars + 8 * (L::S_FULL + i), 1);
+            bar_init(bars + 8 * (L::P_FULL + i), SOFT / 2);
+            bar_init(bars + 8 * (L::O_FULL + i), 1);
         }
-        bar_init(bars + 8 * Q_FULL, SOFT);
+        bar_init(bars + 8 * L::Q_FULL, SOFT);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         *dead = 0;
-        for (int i = 0; i < 4; ++i) odd[i] = 0;
+        for (int i = 0; i < L::SEGMENTS; ++i) odd[i] = 0;
     }
     // (the memory is taken once the kernel in front is over: it might want some, and this one would hold it while it waits)
     pdl_enter();
@@ -677,7 +689,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p)
     } else if (warp < SOFT + DECODE) {
         decode_role<D>(p, base, bars, dead, odd, first, last, warp - SOFT, lane);
     } else if (lane == 0) {
-        product_role<D>(p, base, bars, tmem, dead, first, last);
+        if (warp == SOFT + DECODE) product_role<D>(p, base, bars, tmem, dead, first, last);
+        else copy_role<D>(p, base, bars, dead, first, last);
     }
     __syncwarp();
     __syncthreads();
