@@ -1,8 +1,8 @@
 // Attention of drafted tokens where more than 16 query rows share a KV head: the fifth-generation tensor cores.
 //
 // CTA = one SM, a contiguous run of 128-token tiles as in akv_tree.cu; a unit is up to 256 query rows of a (batch, KV head).
-//   warp  17      one thread copies the planes of a tile (K or V: 32 KB at head size 128) into a ring, three to six bulk copies each
-//   warps 8..15   decode: a ring tile's bytes to fp16 operands in the same place - they take as much - by way of registers
+//   warp  17      copies the planes of a tile (K or V: 32 KB at head size 128) into a ring, three bulk copies for 64 tokens
+//   warps 8..15   decode: four warps for 64 tokens' bytes, to fp16 operands in the same place - they take as much - by way of registers
 //   warp  16      one thread issues the products: S = Q K^T (128 rows x 128 tokens), O += P V
 //   warps 0..7    two softmax groups of 128 threads, a thread per query row: S from tensor memory, P back into its place
 // Everything comes in twos: S, O, P and a softmax group per slot.  With up to 128 rows the slots take the tiles in turn (each
@@ -137,15 +137,6 @@ __device__ __forceinline__ void soft_sync() {
     asm volatile("bar.sync 1, %0;\n" ::"n"(32 * SOFT) : "memory");
 }
 
-__device__ __forceinline__ void decode_sync() {
-    __syncwarp();
-    asm volatile("bar.sync 2, %0;\n" ::"n"(32 * DECODE) : "memory");
-}
-__device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-
 // ---------------------------------------------------------------- the run of a CTA, piece by piece
 // Segment: consecutive tiles t0 .. t0 + c - 1 of one unit.
 struct Segment {
@@ -192,11 +183,16 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w, bool& odd) {
     return w;
 }
 
-// Raw tile in its ring slot: K [block][channel][64] high bytes, then [block][channel][32] twice; V [token][D], then [token][D / 2] twice.
+// A ring tile is two regions of 64 tokens, D * 128 bytes each.  As copied: the high bytes, then either nibble plane.  As operand: K rows
+// [channel] of 64 tokens; V [channel half][token] rows of 64 channels; 16-byte piece c of row r at c ^ (r & 7).  (The tail's keys:
+// [channel half][token] over the whole tile, for groups of eight tokens at one distance.)
 template <int D>
 __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t base, uint32_t bars, volatile int* dead, long long first,
-                                          long long last) {
+                                          long long last, int lane) {
     using L = Plan<D>;
+    const int region = lane / 3, plane = lane - 3 * region;
+    const int part = plane == 0 ? 1 : 2;               // (a nibble plane has half the bytes)
+    const uint32_t bytes = D * BLK / part;
     uint32_t buf = 0, turn = 0;
     for (long long tile = first; tile < last;) {
         Segment s;
@@ -205,25 +201,23 @@ __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t base, uint
         for (int q = 0; q < 2 * s.c; ++q) {
             bool value;
             const int i = s.t0 + tile_of(q, s.c, 3 - p.groups, value);
-            const uint32_t to = base + L::RING_AT + buf * L::TILE_BYTES, bar = bars + 8 * (L::RAW + buf);
+            const uint32_t bar = bars + 8 * (L::RAW + buf);
             bar_wait(bars + 8 * (L::EMPTY + buf), (turn & 1) ^ 1, dead);
+            __syncwarp();
             if (i == p.tiles - 1) {
-                bar_arrive(bar);                       // (the tail is read by the decoding warps themselves)
+                if (lane == 0) bar_arrive(bar);        // (the tail is read by the decoding warps themselves)
             } else {
                 const int blocks = min(2, p.nb - 2 * i);
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(blocks * BLK * D * 2) : "memory");
-                if (!value) {
-                    const long long at = (s.bh * p.nmb + 2 * i) * D;
-                    for (int b = 0; b < blocks; ++b) {
-                        bulk(to + b * D * BLK, p.k8 + (at + b * D) * BLK, D * BLK, bar);
-                        bulk(to + D * TILE + b * D * (BLK / 2), p.km + (at + b * D) * (BLK / 2), D * (BLK / 2), bar);
-                        bulk(to + D * TILE * 3 / 2 + b * D * (BLK / 2), p.kl + (at + b * D) * (BLK / 2), D * (BLK / 2), bar);
-                    }
-                } else {
-                    const long long at = s.bh * p.L + i * TILE;
-                    bulk(to, p.v8 + at * D, blocks * BLK * D, bar);
-                    bulk(to + D * TILE, p.vm + at * (D / 2), blocks * BLK * (D / 2), bar);
-                    bulk(to + D * TILE * 3 / 2, p.vl + at * (D / 2), blocks * BLK * (D / 2), bar);
+                if (lane == 0)
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(blocks * BLK * D * 2) : "memory");
+                __syncwarp();
+                if (region < blocks) {
+                    const uint8_t* src = value ? plane == 0 ? p.v8 : plane == 1 ? p.vm : p.vl : plane == 0 ? p.k8 : plane == 1 ? p.km : p.kl;
+                    // (regions follow one another in either plane)
+                    const long long at = (value ? s.bh * p.L + i * TILE : (s.bh * p.nmb + 2 * i) * BLK) * D / part + region * bytes;
+                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                                 ::"r"(base + L::RING_AT + buf * L::TILE_BYTES + region * D * 128 + (plane ? D * 32 * (plane + 1) : 0)), "l"(src + at),
+                                 "r"(bytes), "r"(bar) : "memory");
                 }
             }
             if (++buf == L::RING) {
@@ -234,15 +228,14 @@ __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t base, uint
     }
 }
 
-// Operand rows of 128 bytes: K planes [block][channel], else [channel half][token].  A thread has U = D / 32 pieces of 16 elements:
-// quarter lane % 4 of rows `row` + u * `step` of one half.  (Neighbouring rows of V in different halves: neither the loads of the
-// bytes nor the stores of the operands meet in a bank.)
+// Four warps decode a region: U = D / 32 pieces of 16 elements a lane, quarter lane % 4 of rows of 64 elements.  (Of V
+// and the tail, neighbouring rows in different halves: neither the loads of the bytes nor the stores of the operands meet in a bank.)
 template <int D>
 __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t base, uint32_t bars, volatile int* dead, volatile int* odd,
                                             long long first, long long last, int warp, int lane) {
     using L = Plan<D>;
     constexpr int U = D / 32;
-    const int qd = lane & 3, k = lane >> 2;
+    const int qd = lane & 3, k = (warp & 3) * 8 + (lane >> 2), side = (lane >> 2 ^ lane >> 3) & 1;
     uint32_t buf = 0, turn = 0;
     int index = 0;
     for (long long tile = first; tile < last; ++index) {
@@ -254,46 +247,48 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t base, ui
             bool value;
             const int i = s.t0 + tile_of(q, s.c, 3 - p.groups, value);
             const bool tail = i == p.tiles - 1, by_channel = !value && !tail;
-            const int half = by_channel ? warp & 1 : D == 128 ? (warp ^ k) & 1 : 0;
-            const int row = (D == 128 || by_channel ? warp >> 1 : warp) * 8 + k, step = D == 128 || by_channel ? 32 : 64;
-            const uint32_t slot = base + L::RING_AT + buf * L::TILE_BYTES;
+            const uint32_t region = base + L::RING_AT + buf * L::TILE_BYTES + (warp >> 2) * D * 128;
+            // piece u: row (u or u / 2) * 32 + k, half side ^ (u & 1) where rows have two
+            const bool halves = D == 128 && !by_channel;
+            auto row = [&](int u) { return (halves ? u >> 1 : u) * 32 + k; };
+            auto half = [&](int u) { return halves ? side ^ (u & 1) : 0; };
             bar_wait(bars + 8 * (L::RAW + buf), turn & 1, dead);
             uint32_t w[U][8];
             if (!tail) {
-                const uint32_t h = slot + (by_channel ? half * D * BLK + row * 64 : row * D + half * 64) + qd * 16;
-                const uint32_t n = slot + D * TILE + (by_channel ? half * D * 32 + row * 32 : row * (D / 2) + half * 32) + qd * 8;
-                const uint32_t hs = step * (by_channel ? 64 : D), ns = hs / 2;
-                const uint16_t* mask = value && p.mask ? reinterpret_cast<const uint16_t*>(p.mask) + s.b * p.mask_stride + i * TILE : nullptr;
-                const int some = by_channel ? 2 * i + half < p.nb ? D : 0 : p.nb * BLK - i * TILE;
+                const int pitch = by_channel ? 64 : D;
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const uint4 x = lds128(h + u * hs);
-                    const uint2 m = lds64(n + u * ns), l = lds64(n + D * BLK + u * ns);
+                    const int o = row(u) * pitch + half(u) * 64 + qd * 16;
+                    const uint4 x = lds128(region + o);
+                    const uint2 m = lds64(region + D * 64 + o / 2), l = lds64(region + D * 96 + o / 2);
                     w[u][0] = x.x; w[u][1] = x.y; w[u][2] = x.z; w[u][3] = x.w;
                     w[u][4] = m.x; w[u][5] = m.y; w[u][6] = l.x; w[u][7] = l.y;
                 }
-                if (mask || some < TILE) {
+                const int some = p.nb * BLK - i * TILE;
+                if (some < TILE || (value && p.mask)) {
                     // (a token that does not exist or is masked away counts as zero, whatever there is: 0 * NaN would be NaN)
+                    const uint16_t* mask = value && p.mask ? reinterpret_cast<const uint16_t*>(p.mask) + s.b * p.mask_stride + i * TILE : nullptr;
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
-                        const int r = row + u * step;
-                        if (r >= some || (mask && mask[r] == 0xFC00u)) {
+                        const int tok = (warp >> 2) * BLK + (by_channel ? 0 : row(u));
+                        if (tok >= some || (mask && mask[tok] == 0xFC00u)) {
 #pragma unroll
                             for (int j = 0; j < 8; ++j) w[u][j] = 0;
                         }
                     }
                 }
-                decode_sync();                         // all bytes are in registers
+                __syncwarp();                          // the region's bytes are in registers
+                asm volatile("bar.sync %0, 128;\n" ::"r"(2 + (warp >> 2)) : "memory");
             } else {
                 bool mine = false;
                 const __half *rest = value ? p.restv : p.restk, *drafted = value ? p.vd : p.kd;
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const int x = row + u * step, d = x - p.rest;
+                    const int x = (warp >> 2) * BLK + row(u), d = x - p.rest;
                     uint4 a = make_uint4(0, 0, 0, 0), b = a;
                     if (x < p.tail) {
                         const __half* src = d < 0 ? rest + ((s.b * BLK + x) * p.H + s.h) * D : drafted + ((s.b * p.T + d) * p.H + s.h) * D;
-                        const uint4* from = reinterpret_cast<const uint4*>(src + half * 64 + qd * 16);
+                        const uint4* from = reinterpret_cast<const uint4*>(src + half(u) * 64 + qd * 16);
                         a = __ldg(from);
                         b = __ldg(from + 1);
                     }
@@ -307,7 +302,6 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t base, ui
                 }
                 if (mine) odd[index % L::SEGMENTS] = index + 1;
             }
-            const uint32_t at = slot + half * (by_channel ? D * 128 : 16384) + row * 128 + (((2 * qd) ^ (row & 7)) << 4);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 uint4 x = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]), y = make_uint4(w[u][4], w[u][5], w[u][6], w[u][7]);
@@ -316,8 +310,10 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t base, ui
                     x = halves8(h.x, h.y, n.x, n.z);
                     y = halves8(h.z, h.w, n.y, n.w);
                 }
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at + u * step * 128), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"((at ^ 16) + u * step * 128), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+                const uint32_t at = (tail && !value ? region + half(u) * 16384 - (warp >> 2) * (D - 64) * 128 : region + half(u) * 8192) +
+                                    row(u) * 128 + (((2 * qd) ^ (k & 7)) << 4);
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at ^ 16), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
             }
             fence_shared();
             __syncwarp();
@@ -361,7 +357,8 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
             const uint32_t idesc = instruction(TILE, !tail);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
-                const uint32_t major = (kk >> 2) * 16384 + (kk & 3) * 32;           // K-major: 16 channels of rows of 64
+                // 16 channels: of Q and of the tail's keys 32 bytes of rows of 64 (K-major), of K's planes 16 rows of 64 tokens
+                const uint32_t major = (kk >> 2) * 16384 + (kk & 3) * 32;
                 mma_ss(tmem + slot * TILE, operand(q + major, 16, 1024),
                        tail ? operand(k + major, 16, 1024) : operand(k + kk * 2048, D * 128, 1024), idesc, kk > 0);
             }
@@ -378,7 +375,7 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
             fence_after();
 #pragma unroll
             for (int kk = 0; kk < TILE / 16; ++kk)
-                mma_ts(tmem + 256 + slot * 128, tmem + slot * TILE + kk * 8, operand(v + kk * 2048, 16384, 1024), instruction(D, true),
+                mma_ts(tmem + 256 + slot * 128, tmem + slot * TILE + kk * 8, operand(v + (kk >> 2) * D * 128 + (kk & 3) * 2048, 8192, 1024), instruction(D, true),
                        n >= 2 || kk > 0);
             commit(bars + 8 * (Plan<D>::O_FULL + slot));
             if (p.groups == 1 || slot) commit(bars + 8 * (Plan<D>::EMPTY + buf));
@@ -688,9 +685,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p)
         softmax_role<D>(p, smem, base, bars, tmem, dead, odd, first, last, warp, lane);
     } else if (warp < SOFT + DECODE) {
         decode_role<D>(p, base, bars, dead, odd, first, last, warp - SOFT, lane);
+    } else if (warp == SOFT + DECODE + 1) {
+        copy_role<D>(p, base, bars, dead, first, last, lane);
     } else if (lane == 0) {
-        if (warp == SOFT + DECODE) product_role<D>(p, base, bars, tmem, dead, first, last);
-        else copy_role<D>(p, base, bars, dead, first, last);
+        product_role<D>(p, base, bars, tmem, dead, first, last);
     }
     __syncwarp();
     __syncthreads();
