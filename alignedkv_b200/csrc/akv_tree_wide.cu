@@ -137,6 +137,11 @@ __device__ __forceinline__ void soft_sync() {
     asm volatile("bar.sync 1, %0;\n" ::"n"(32 * SOFT) : "memory");
 }
 
+__device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
 // ---------------------------------------------------------------- the run of a CTA, piece by piece
 // Segment: consecutive tiles t0 .. t0 + c - 1 of one unit.
 struct Segment {
@@ -171,11 +176,16 @@ __device__ __forceinline__ int place_of(int i, bool value, int c, int ahead) {
 }
 
 // ---------------------------------------------------------------- decode
-// Eight elements in order from their high bytes and nibbles.
+// Eight elements from their high bytes and nibbles, in the order in which two permutes a pair suffice: 0 2 1 3, 4 6 5 7.  Of K that is
+// the order of the scores' columns, and V's tokens are stored in it; of V it is the order of the output's columns.
+__device__ __forceinline__ constexpr int swapped(int i) { return (i & ~3) | (i & 1) << 1 | (i >> 1 & 1); }     // (its own inverse)
 __device__ __forceinline__ uint4 halves8(uint32_t h0, uint32_t h1, uint32_t m, uint32_t l) {
     const uint32_t even = (m & 0xF0F0F0F0u) | ((l >> 4) & 0x0F0F0F0Fu), odd = ((m << 4) & 0xF0F0F0F0u) | (l & 0x0F0F0F0Fu);
-    const uint32_t a = __byte_perm(even, odd, 0x5140), b = __byte_perm(even, odd, 0x7362);
-    return make_uint4(__byte_perm(a, h0, 0x5140), __byte_perm(a, h0, 0x7362), __byte_perm(b, h1, 0x5140), __byte_perm(b, h1, 0x7362));
+    return make_uint4(__byte_perm(even, h0, 0x6140), __byte_perm(odd, h0, 0x7150), __byte_perm(even, h1, 0x6342), __byte_perm(odd, h1, 0x7352));
+}
+// The same order for eight fp16 values.
+__device__ __forceinline__ uint4 reorder8(const uint4& x) {
+    return make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632), __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
 }
 __device__ __forceinline__ uint32_t finite_halves(uint32_t w, bool& odd) {
     if ((w & 0x7C00u) == 0x7C00u) { w &= 0xFFFF0000u; odd = true; }
@@ -188,11 +198,8 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w, bool& odd) {
 // [channel half][token] over the whole tile, for groups of eight tokens at one distance.)
 template <int D>
 __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t base, uint32_t bars, volatile int* dead, long long first,
-                                          long long last, int lane) {
+                                          long long last) {
     using L = Plan<D>;
-    const int region = lane / 3, plane = lane - 3 * region;
-    const int part = plane == 0 ? 1 : 2;               // (a nibble plane has half the bytes)
-    const uint32_t bytes = D * BLK / part;
     uint32_t buf = 0, turn = 0;
     for (long long tile = first; tile < last;) {
         Segment s;
@@ -203,21 +210,18 @@ __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t base, uint
             const int i = s.t0 + tile_of(q, s.c, 3 - p.groups, value);
             const uint32_t bar = bars + 8 * (L::RAW + buf);
             bar_wait(bars + 8 * (L::EMPTY + buf), (turn & 1) ^ 1, dead);
-            __syncwarp();
             if (i == p.tiles - 1) {
-                if (lane == 0) bar_arrive(bar);        // (the tail is read by the decoding warps themselves)
+                bar_arrive(bar);                       // (the tail is read by the decoding warps themselves)
             } else {
                 const int blocks = min(2, p.nb - 2 * i);
-                if (lane == 0)
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(blocks * BLK * D * 2) : "memory");
-                __syncwarp();
-                if (region < blocks) {
-                    const uint8_t* src = value ? plane == 0 ? p.v8 : plane == 1 ? p.vm : p.vl : plane == 0 ? p.k8 : plane == 1 ? p.km : p.kl;
-                    // (regions follow one another in either plane)
-                    const long long at = (value ? s.bh * p.L + i * TILE : (s.bh * p.nmb + 2 * i) * BLK) * D / part + region * bytes;
-                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
-                                 ::"r"(base + L::RING_AT + buf * L::TILE_BYTES + region * D * 128 + (plane ? D * 32 * (plane + 1) : 0)), "l"(src + at),
-                                 "r"(bytes), "r"(bar) : "memory");
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(blocks * BLK * D * 2) : "memory");
+                const uint8_t *f = value ? p.v8 : p.k8, *m = value ? p.vm : p.km, *l = value ? p.vl : p.kl;
+                long long at = (value ? s.bh * p.L + i * TILE : (s.bh * p.nmb + 2 * i) * BLK) * D;
+                uint32_t to = base + L::RING_AT + buf * L::TILE_BYTES;
+                for (int b = 0; b < blocks; ++b, at += BLK * D, to += D * 128) {
+                    bulk(to, f + at, D * BLK, bar);
+                    bulk(to + D * 64, m + at / 2, D * BLK / 2, bar);
+                    bulk(to + D * 96, l + at / 2, D * BLK / 2, bar);
                 }
             }
             if (++buf == L::RING) {
@@ -250,7 +254,8 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t base, ui
             const uint32_t region = base + L::RING_AT + buf * L::TILE_BYTES + (warp >> 2) * D * 128;
             // piece u: row (u or u / 2) * 32 + k, half side ^ (u & 1) where rows have two
             const bool halves = D == 128 && !by_channel;
-            auto row = [&](int u) { return (halves ? u >> 1 : u) * 32 + k; };
+            const int kr = value && !tail ? swapped(k) : k;        // (V's tokens are stored in the order of the scores' columns)
+            auto row = [&](int u) { return (halves ? u >> 1 : u) * 32 + kr; };
             auto half = [&](int u) { return halves ? side ^ (u & 1) : 0; };
             bar_wait(bars + 8 * (L::RAW + buf), turn & 1, dead);
             uint32_t w[U][8];
@@ -309,9 +314,12 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t base, ui
                     const uint4 h = x, n = y;
                     x = halves8(h.x, h.y, n.x, n.z);
                     y = halves8(h.z, h.w, n.y, n.w);
+                } else if (value) {
+                    x = reorder8(x);
+                    y = reorder8(y);
                 }
                 const uint32_t at = (tail && !value ? region + half(u) * 16384 - (warp >> 2) * (D - 64) * 128 : region + half(u) * 8192) +
-                                    row(u) * 128 + (((2 * qd) ^ (k & 7)) << 4);
+                                    (row(u) - kr + k) * 128 + (((2 * qd) ^ (k & 7)) << 4);
                 asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
                 asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at ^ 16), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
             }
@@ -497,7 +505,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                         __syncwarp();
                         tmem_ld(v, s_at + c);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(edge(__uint_as_float(v[j]), scale2, c + j));
+                        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(edge(__uint_as_float(v[j]), scale2, c + (tail ? j : swapped(j))));
                         __syncwarp();
                         tmem_st32(s_at + c, v);
                     }
@@ -588,8 +596,8 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                         tmem_ld(v, o_at + c + e);
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
-                            join[(e / 4 + j) * 128 + idx] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
-                                                                        __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
+                            join[(e / 4 + j) * 128 + idx] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 2]),
+                                                                        __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 3]));
                     }
                 }
                 soft_sync();
@@ -600,7 +608,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
             tmem_ld(v, o_at + c);
             float o[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(v[j]);
+            for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(v[swapped(j)]);
             if (p.groups == 1 && n_items > 1) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -685,10 +693,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p)
         softmax_role<D>(p, smem, base, bars, tmem, dead, odd, first, last, warp, lane);
     } else if (warp < SOFT + DECODE) {
         decode_role<D>(p, base, bars, dead, odd, first, last, warp - SOFT, lane);
-    } else if (warp == SOFT + DECODE + 1) {
-        copy_role<D>(p, base, bars, dead, first, last, lane);
     } else if (lane == 0) {
-        product_role<D>(p, base, bars, tmem, dead, first, last);
+        if (warp == SOFT + DECODE) product_role<D>(p, base, bars, tmem, dead, first, last);
+        else copy_role<D>(p, base, bars, dead, first, last);
     }
     __syncwarp();
     __syncthreads();
