@@ -26,52 +26,52 @@ from .extension._planes import cdiv, column_block
 __all__ = ["tree_attention", "tree_weights", "tree_commit", "evict"]
 
 _nothing = contextlib.nullcontext()
-_PLANES = ("k_first_8", "k_mid_4", "k_last_4", "v_first_8", "v_mid_4", "v_last_4", "k_exp_max", "v_exp_max")
 MOST_DRAFTED = 64
 
 
-def _need(name: str, t, shape: tuple, dtype: torch.dtype, device: torch.device) -> None:
-    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on {device}")
+def _need(name: str, t, shape: tuple, dtype: torch.dtype, index: int) -> int:
+    """The address of t, a contiguous tensor of that shape and type on that CUDA device."""
+    if type(t) is not torch.Tensor and not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype or \
+            t.get_device() != index or not t.is_contiguous():
+        raise RuntimeError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on cuda:{index}")
+    return t.data_ptr()
 
 
 class _Call:
-    """A cache's tensors, checked, as the library takes them; a context in which its device is the current one."""
+    """A cache's tensors, checked, as the library takes them; a context in which its device is the current one.  (The checks are most of
+    what a call on a short cache costs, so they are few: one look at shape, type, device and layout of each tensor that is used.)"""
+    __slots__ = ("device", "index", "B", "H", "D", "L", "ptrs", "tokens")
 
-    def __init__(self, cache, rest_len: int, rest_start: int):
+    def __init__(self, cache, rest_len: int, rest_start: int, maxima: bool = False):
         f8 = cache.k_first_8
         if not isinstance(f8, torch.Tensor) or not f8.is_cuda or f8.dim() != 5 or f8.shape[4] != column_block:
             raise RuntimeError(f"k_first_8: expected a CUDA tensor of shape [B, H, blocks, D, {column_block}]")
-        self.device = dev = f8.device
-        self.index = dev.index
+        self.device = f8.device
+        self.index = dev = f8.get_device()
         B, H, nmb, D, _ = f8.shape
         self.B, self.H, self.D = B, H, D
         self.L = L = cache.v_first_8.shape[2] if cache.v_first_8.dim() == 4 else -1
-        if self.D not in (64, 128):
-            raise RuntimeError(f"head size {self.D}: these operators cover 64 and 128")
+        if D != 128 and D != 64:
+            raise RuntimeError(f"head size {D}: these operators cover 64 and 128")
         if nmb != cdiv(L, column_block):
             raise RuntimeError(f"k_first_8 has {nmb} blocks, v_first_8 {L} tokens")
-        half = column_block // 2
-        shapes = ((B, H, nmb, D, column_block), (B, H, nmb, D, half), (B, H, nmb, D, half), (B, H, L, D), (B, H, L, D // 2),
-                  (B, H, L, D // 2), (B, 1, H, D), (B, 1, H, D))
-        ptrs = []
-        for name, shape in zip(_PLANES, shapes):
-            t = getattr(cache, name)
-            _need(name, t, shape, torch.uint8, dev)
-            ptrs.append(t.data_ptr())
-        for name in ("restk", "restv"):
-            t = getattr(cache, name)
-            _need(name, t, (B, column_block, H, D), torch.half, dev)
-            ptrs.append(t.data_ptr())
-        if rest_start % column_block or not 0 <= rest_len < column_block or rest_start < 0 or rest_start + rest_len > L:
+        u8, nk, nv, ex, rs = torch.uint8, (B, H, nmb, D, column_block // 2), (B, H, L, D // 2), (B, 1, H, D), (B, column_block, H, D)
+        self.ptrs = [
+            _need("k_first_8", f8, (B, H, nmb, D, column_block), u8, dev), _need("k_mid_4", cache.k_mid_4, nk, u8, dev),
+            _need("k_last_4", cache.k_last_4, nk, u8, dev), _need("v_first_8", cache.v_first_8, (B, H, L, D), u8, dev),
+            _need("v_mid_4", cache.v_mid_4, nv, u8, dev), _need("v_last_4", cache.v_last_4, nv, u8, dev),
+            _need("k_exp_max", cache.k_exp_max, ex, u8, dev) if maxima else None,
+            _need("v_exp_max", cache.v_exp_max, ex, u8, dev) if maxima else None,
+            _need("restk", cache.restk, rs, torch.half, dev), _need("restv", cache.restv, rs, torch.half, dev)]
+        self.tokens = rest_start + rest_len
+        if rest_start % column_block or not 0 <= rest_len < column_block or rest_start < 0 or self.tokens > L:
             raise RuntimeError(f"{rest_start} tokens in planes of {L} and {rest_len} residual ones: expected whole blocks of "
                                f"{column_block} and at most {column_block - 1}")
-        self.ptrs, self.tokens = ptrs, rest_start + rest_len
 
     def queries(self, q: torch.Tensor) -> tuple:
         """(drafted tokens, query heads) of q [B,T,Hq,D]."""
         if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[0] != self.B or q.shape[3] != self.D or \
-                q.dtype != torch.half or q.device != self.device or not q.is_contiguous():
+                q.dtype is not torch.half or q.get_device() != self.index or not q.is_contiguous():
             raise RuntimeError(f"q: expected a contiguous fp16 tensor of shape [{self.B}, T, Hq, {self.D}] on {self.device}")
         T, Hq = q.shape[1], q.shape[2]
         if not 1 <= T <= MOST_DRAFTED:
@@ -116,22 +116,21 @@ def tree_attention(cache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tre
     `tree_weights` takes.  The cache is not changed; `tree_commit` appends the accepted tokens."""
     c = _Call(cache, rest_len, rest_start)
     T, Hq = c.queries(q)
-    for name, t in (("k", k), ("v", v)):
-        _need(name, t, (c.B, T, c.H, c.D), torch.half, c.device)
-    if not isinstance(tree, torch.Tensor) or tree.dtype != torch.bool or tree.device != c.device or not tree.is_contiguous() or \
-            tuple(tree.shape) not in ((T, T), (c.B, T, T)):
+    k_ptr, v_ptr = _need("k", k, (c.B, T, c.H, c.D), torch.half, c.index), _need("v", v, (c.B, T, c.H, c.D), torch.half, c.index)
+    if not isinstance(tree, torch.Tensor) or tree.dtype is not torch.bool or tree.get_device() != c.index or \
+            not tree.is_contiguous() or tree.shape != (T, T) and tree.shape != (c.B, T, T):
         raise RuntimeError(f"tree: expected a contiguous bool tensor of shape [{T}, {T}] or [{c.B}, {T}, {T}] on {c.device}")
     if out is None:
         out = torch.empty_like(q)
     else:
-        _need("out", out, tuple(q.shape), torch.half, c.device)
+        _need("out", out, tuple(q.shape), torch.half, c.index)
     mask_ptr, mask_stride = c.mask(mask)
     group, lib = Hq // c.H, _lib.load()
     sums = torch.empty((c.B, T, Hq), dtype=torch.float32, device=c.device) if lse else None
     with c.here():
         ws = torch.empty(lib.akv_tree_scratch_bytes(c.B, c.H, group, c.D, rest_start, T), dtype=torch.uint8, device=c.device)
         rc = lib.akv_tree_attention(
-            c.layer(group, ws), q.data_ptr(), k.data_ptr(), v.data_ptr(), tree.data_ptr(), T * T if tree.dim() == 3 else 0,
+            c.layer(group, ws), q.data_ptr(), k_ptr, v_ptr, tree.data_ptr(), T * T if tree.dim() == 3 else 0,
             mask_ptr, mask_stride, out.data_ptr(), sums.data_ptr() if lse else None, T, rest_len, rest_start,
             1.0 / math.sqrt(c.D) if scale is None else scale, _lib.raw_stream(c.index))
     _lib.check("tree_attention", rc)
@@ -147,8 +146,8 @@ def tree_weights(cache, q: torch.Tensor, lse: torch.Tensor, weights: torch.Tenso
     (rows ascending within a lane, lanes in a fixed tree): the same call on the same state gives the same bits."""
     c = _Call(cache, rest_len, rest_start)
     T, Hq = c.queries(q)
-    _need("lse", lse, (c.B, T, Hq), torch.float32, c.device)
-    _need("weights", weights, (c.B, c.H, c.L), torch.float32, c.device)
+    _need("lse", lse, (c.B, T, Hq), torch.float32, c.index)
+    _need("weights", weights, (c.B, c.H, c.L), torch.float32, c.index)
     mask_ptr, mask_stride = c.mask(mask)
     with c.here():
         rc = _lib.load().akv_tree_weights(
@@ -164,20 +163,19 @@ def tree_commit(cache, k: torch.Tensor, v: torch.Tensor, path: torch.Tensor, *, 
     are appended (an index outside the tree is clamped into it; every sequence accepts the same number of tokens).  The cache is
     then what n steps of `DecodeLayer.decode` would have left: exponent maxima, residual rows, and the planes of a block that
     fills up.  The caller's counts become (rest_len + n) % 64 and rest_start + 64 if a block was filled."""
-    c = _Call(cache, rest_len, rest_start)
+    c = _Call(cache, rest_len, rest_start, maxima=True)
     if not isinstance(k, torch.Tensor) or k.dim() != 4 or not 1 <= k.shape[1] <= MOST_DRAFTED:
         raise RuntimeError(f"k: expected a tensor of shape [B, T, H, D] with T 1 to {MOST_DRAFTED}")
     T = k.shape[1]
-    for name, t in (("k", k), ("v", v)):
-        _need(name, t, (c.B, T, c.H, c.D), torch.half, c.device)
+    k_ptr, v_ptr = _need("k", k, (c.B, T, c.H, c.D), torch.half, c.index), _need("v", v, (c.B, T, c.H, c.D), torch.half, c.index)
     if not isinstance(path, torch.Tensor) or path.dim() != 2 or not 1 <= path.shape[1] <= MOST_DRAFTED:
         raise RuntimeError(f"path: expected a tensor of shape [{c.B}, n] with n 1 to {MOST_DRAFTED}")
     n = path.shape[1]
-    _need("path", path, (c.B, n), torch.int32, c.device)
+    path_ptr = _need("path", path, (c.B, n), torch.int32, c.index)
     if c.tokens + n > c.L:
         raise RuntimeError(f"cache is full ({c.L} tokens): no room for {n} behind {c.tokens}")
     with c.here():
-        rc = _lib.load().akv_tree_commit(c.layer(1, None), k.data_ptr(), v.data_ptr(), path.data_ptr(), T, n, rest_len, rest_start,
+        rc = _lib.load().akv_tree_commit(c.layer(1, None), k_ptr, v_ptr, path_ptr, T, n, rest_len, rest_start,
                                          _lib.raw_stream(c.index))
     _lib.check("tree_commit", rc)
 
@@ -198,8 +196,8 @@ def evict(cache, weights: torch.Tensor, positions: torch.Tensor, *, rest_len: in
     Afterwards: rest_start = keep; K nibble planes behind it are zero as the K writers expect; the residual tokens' weights follow
     at keep.., zeros behind them.  Exponent maxima stay (they remain upper bounds)."""
     c = _Call(cache, rest_len, rest_start)
-    _need("weights", weights, (c.B, c.H, c.L), torch.float32, c.device)
-    _need("positions", positions, (c.B, c.H, c.L), torch.int32, c.device)
+    _need("weights", weights, (c.B, c.H, c.L), torch.float32, c.index)
+    _need("positions", positions, (c.B, c.H, c.L), torch.int32, c.index)
     if keep <= 0 or keep % column_block or keep > rest_start:
         raise RuntimeError(f"keep: {keep}, expected a positive multiple of {column_block} of at most {rest_start}")
     if not 0 <= recent <= keep or not 0 <= arranged <= rest_start or shift < 0:

@@ -87,184 +87,308 @@ struct EvictArgs {
     float* weights;
     int* positions;
     uint8_t *k8, *km, *kl, *v8, *vm, *vl;
-    int *holes, *movers, *count;       // [rows][most], [rows][most], [rows]
+    int *holes, *movers, *start;       // [rows][most] twice; [rows][keep / 64 + 1]: free places in front of each block's
     int D, L, nmb, n, rest, keep, recent, arranged, shift, most;
+    int share;                         // places of a CTA of select_kernel's cluster, a multiple of SEL_NT
+    int held;                          // whether their keys are kept in shared memory
 };
 
 __device__ __forceinline__ int position_of(const EvictArgs& a, const int* pos, int i) { return i < a.arranged ? pos[i] : i + a.shift; }
 
-// One CTA per row.  The keep-th largest key by four counts of eight bits; then one pass in order that numbers the free places and the
-// survivors behind.
-constexpr int SEL_NT = 1024;
+// ---- cluster: barrier, and a word of another CTA's shared memory
+__device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_ld(const void* p, uint32_t cta) {
+    uint32_t at, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(smem_u32(p)), "r"(cta));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// A cluster per row; a CTA has `share` consecutive places and keeps their keys in shared memory: one read of the weights, whatever is
+// counted.  The keep-th largest key by four counts of eight bits (a column of the count per lane: no two lanes of a warp meet, although
+// weights crowd into few exponents), added up over the cluster through distributed shared memory; every CTA draws the same
+// conclusion.  Then ties, free places and survivors behind are numbered in order: per warp, per CTA, per cluster.
+constexpr int SEL_NT = 1024, SEL_W = SEL_NT / 32, SEL_MOST = 40960;      // SEL_MOST: keys a CTA can keep
 __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
-    __shared__ int hist[256], warp_sum[3][SEL_NT / 32], total[3];
-    __shared__ uint32_t found[2];
+    extern __shared__ __align__(16) uint32_t keys[];
+    __shared__ int hist[256 * 32];
+    __shared__ uint32_t sums[2][256];              // this CTA's counts: two buffers, so that one barrier a round is enough
+    __shared__ uint32_t found[2], scan[3][SEL_W + 1], totals[2][2];
     pdl_enter();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const size_t row = blockIdx.x;
+    uint32_t ctas, rank;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const size_t row = blockIdx.y;
     const float* w = a.weights + row * a.L;
     int* pos = a.positions + row * a.L;
     const int safe_from = a.n + a.shift - a.recent;
+    const int first = min((int)rank * a.share, a.n), count = min(a.share, a.n - first);
+    auto key = [&](int i) { return key_of(w[first + i], position_of(a, pos, first + i) >= safe_from); };
+    if (a.held)
+        for (int i = tid; i < count; i += SEL_NT) keys[i] = key(i);
+    auto at = [&](int i) { return a.held ? keys[i] : key(i); };
     uint32_t prefix = 0;
-    int want = a.keep;                                 // how many of the keys that share the prefix stay
-    for (int bit = 24; bit >= 0; bit -= 8) {
-        if (tid < 256) hist[tid] = 0;
+    uint32_t want = a.keep;                            // how many of the keys that share the prefix stay
+    for (int round = 0; round < 4; ++round) {
+        const int bit = 24 - 8 * round;
+        for (int i = tid; i < 256 * 32; i += SEL_NT) hist[i] = 0;
         __syncthreads();
-        for (int i = tid; i < a.n; i += SEL_NT) {
-            const uint32_t k = key_of(w[i], position_of(a, pos, i) >= safe_from);
-            if (bit == 24 || (k >> (bit + 8)) == (prefix >> (bit + 8))) atomicAdd(&hist[(k >> bit) & 255], 1);
+        for (int i = tid; i < count; i += SEL_NT) {
+            const uint32_t k = at(i);
+            if (round == 0 || (k >> (bit + 8)) == (prefix >> (bit + 8))) atomicAdd(&hist[((k >> bit) & 255) * 32 + lane], 1);
         }
         __syncthreads();
-        if (tid == 0) {
-            int d = 255, above = 0;
-            while (d > 0 && above + hist[d] < want) above += hist[d--];
-            found[0] = d;
-            found[1] = above;
+        for (int d = warp; d < 256; d += SEL_W) {
+            int c = hist[d * 32 + lane];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xFFFFFFFFu, c, o);
+            if (lane == 0) sums[round & 1][d] = c;
+        }
+        cluster_sync();
+        if (warp == 0) {
+            // lane: digits 255 - 8 lane .. 248 - 8 lane, from above
+            uint32_t c[8], mine = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                c[j] = 0;
+                for (uint32_t r = 0; r < ctas; ++r) c[j] += cluster_ld(&sums[round & 1][255 - 8 * lane - j], r);
+                mine += c[j];
+            }
+            uint32_t above = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, above, o);
+                if (lane >= o) above += x;
+            }
+            above -= mine;
+            if (above < want && above + mine >= want) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (above < want && above + c[j] >= want) {
+                        found[0] = 255 - 8 * lane - j;
+                        found[1] = above;
+                    }
+                    above += c[j];
+                }
+            }
         }
         __syncthreads();
         prefix |= found[0] << bit;
-        want -= (int)found[1];
+        want -= found[1];
         __syncthreads();
     }
-    int ties = 0, holes = 0, movers = 0;               // so far
-    for (int i0 = 0; i0 < a.n; i0 += SEL_NT) {
-        const int i = i0 + tid;
-        const uint32_t k = i < a.n ? key_of(w[i], position_of(a, pos, i) >= safe_from) : 0;
-        const bool tie = i < a.n && k == prefix;
-        const uint32_t below = (1u << lane) - 1;
+    // A warp's places: share / 32 consecutive ones.  Numbers in front of it: `scan` of the CTA's warps, `base` of the CTAs before.
+    const int part = a.share / SEL_W, i0 = warp * part, i1 = min(i0 + part, count);
+    const uint32_t below = (1u << lane) - 1;
+    auto number = [&](int s, uint32_t mine) {          // (lane 0: exclusive sums of the warps' counts)
+        if (lane == 0) scan[s][warp] = mine;
+        __syncthreads();
+        if (warp == 0) {
+            uint32_t x = scan[s][lane], y = x;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t z = __shfl_up_sync(0xFFFFFFFFu, y, o);
+                if (lane >= o) y += z;
+            }
+            scan[s][lane] = y - x;
+            if (lane == 31) scan[s][SEL_W] = y;
+        }
+        __syncthreads();
+    };
+    uint32_t ties = 0;
+    for (int i = i0; i < i1; i += 32) ties += __popc(__ballot_sync(0xFFFFFFFFu, i + lane < i1 && at(i + lane) == prefix));
+    number(0, ties);
+    if (tid == 0) totals[0][0] = scan[0][SEL_W];
+    cluster_sync();
+    uint32_t tie0 = scan[0][warp];
+    for (uint32_t r = 0; r < rank; ++r) tie0 += cluster_ld(&totals[0][0], r);
+    // (bits: the place's token stays; as many words as the warp has groups of 32, in the same order twice)
+    uint32_t holes = 0, movers = 0, seen = tie0;
+    auto stays = [&](int i, uint32_t& before) {
+        const uint32_t k = i + lane < i1 ? at(i + lane) : 0;
+        const bool tie = i + lane < i1 && k == prefix;
         const uint32_t tb = __ballot_sync(0xFFFFFFFFu, tie);
-        if (lane == 0) warp_sum[0][warp] = __popc(tb);
-        __syncthreads();
-        int before = ties;
-        for (int j = 0; j < warp; ++j) before += warp_sum[0][j];
-        const bool stays = i < a.n && (k > prefix || (tie && before + __popc(tb & below) < want));
-        const bool hole = i < a.keep && !stays, mover = stays && i >= a.keep;
+        const bool s = i + lane < i1 && (k > prefix || (tie && before + __popc(tb & below) < want));
+        before += __popc(tb);
+        return s;
+    };
+    for (int i = i0; i < i1; i += 32) {
+        const bool s = stays(i, seen);
+        const int place = first + i + lane;
+        holes += __popc(__ballot_sync(0xFFFFFFFFu, i + lane < i1 && !s && place < a.keep));
+        movers += __popc(__ballot_sync(0xFFFFFFFFu, s && place >= a.keep));
+    }
+    number(1, holes);
+    number(2, movers);
+    if (tid == 0) {
+        totals[1][0] = scan[1][SEL_W];
+        totals[1][1] = scan[2][SEL_W];
+    }
+    cluster_sync();
+    uint32_t h = scan[1][warp], m = scan[2][warp];
+    for (uint32_t r = 0; r < rank; ++r) {
+        h += cluster_ld(&totals[1][0], r);
+        m += cluster_ld(&totals[1][1], r);
+    }
+    int *hole_to = a.holes + row * a.most, *mover_to = a.movers + row * a.most, *start = a.start + row * (a.keep / BLK + 1);
+    seen = tie0;
+    for (int i = i0; i < i1; i += 32) {
+        const bool s = stays(i, seen);
+        const int place = first + i + lane;
+        const bool hole = i + lane < i1 && !s && place < a.keep, mover = s && place >= a.keep;
         const uint32_t hb = __ballot_sync(0xFFFFFFFFu, hole), mb = __ballot_sync(0xFFFFFFFFu, mover);
-        if (lane == 0) {
-            warp_sum[1][warp] = __popc(hb);
-            warp_sum[2][warp] = __popc(mb);
-        }
-        __syncthreads();
-        int h = holes, m = movers;
-        for (int j = 0; j < warp; ++j) {
-            h += warp_sum[1][j];
-            m += warp_sum[2][j];
-        }
-        if (hole) a.holes[row * a.most + h + __popc(hb & below)] = i;
-        if (mover) a.movers[row * a.most + m + __popc(mb & below)] = i;
-        if (stays && i < a.keep && i >= a.arranged) pos[i] = i + a.shift;
-        if (tid < 3) {
-            int s = 0;
-            for (int j = 0; j < SEL_NT / 32; ++j) s += warp_sum[tid][j];
-            total[tid] = s;
-        }
-        __syncthreads();
-        ties += total[0];
-        holes += total[1];
-        movers += total[2];
-        __syncthreads();
+        if (lane == 0 && place % BLK == 0 && place <= a.keep) start[place / BLK] = h;
+        if (hole) hole_to[h + __popc(hb & below)] = place;
+        if (mover) mover_to[m + __popc(mb & below)] = place;
+        if (s && place < a.keep && place >= a.arranged) pos[place] = place + a.shift;
+        h += __popc(hb);
+        m += __popc(mb);
     }
-    if (tid == 0) a.count[row] = movers;
-}
-
-// Index of the first free place that is not below `slot`.
-__device__ __forceinline__ int first_hole(const int* holes, int count, int slot) {
-    int lo = 0, hi = count;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (holes[mid] < slot) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo;
+    if (a.keep == a.n && rank == 0 && tid == 0) start[a.keep / BLK] = 0;      // (no place behind: nothing moves)
+    cluster_sync();                                    // (no CTA leaves while another reads its counts)
 }
 
 // CTA = one block of 64 places in front of `keep`: its free places take the survivors of the same numbers.  Survivors are read
 // only behind `keep` and places are written only in front of it, each by its own CTA: no order among the CTAs.
-__global__ void __launch_bounds__(256) move_kernel(const EvictArgs a) {
-    extern __shared__ __align__(16) uint8_t tile[];     // K: [D][64] high bytes, [D][32] twice
-    __shared__ int src[BLK], dst[BLK];
+// K, token-minor: one survivor is a byte of each of D rows and half a byte of 2 D.  The block and the blocks that its survivors come
+// from are staged in shared memory, three at a time; a warp takes a channel, a lane two neighbouring places (whose nibbles share a
+// byte), so that a row's bytes are read and written without a conflict.  V: rows of 16-byte pieces through registers.
+// Bound by HBM: the block twice, the blocks behind once.
+constexpr int MOVE_NT = 256, STAGED = 3;
+template <int D>
+__global__ void __launch_bounds__(MOVE_NT) move_kernel(const EvictArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];     // blocks of [D][64] high bytes, [D][32] twice: the places', then survivors'
+    __shared__ int from[BLK], to[BLK], src[BLK];
+    constexpr int BYTES = D * 128, PIECES = D / 8, PER = BLK * PIECES / MOVE_NT;
     pdl_enter();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = a.D;
-    const size_t row = blockIdx.x;
-    const int blk = blockIdx.y;
-    const int count = a.count[row];
-    const int *holes = a.holes + row * a.most, *movers = a.movers + row * a.most;
-    const int i0 = first_hole(holes, count, blk * BLK), i1 = first_hole(holes, count, blk * BLK + BLK), m = i1 - i0;
-    if (m == 0) return;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const size_t row = blockIdx.y;
+    const int blk = blockIdx.x;
+    const int* start = a.start + row * (a.keep / BLK + 1) + blk;
+    const int i0 = start[0], m = start[1] - i0;
+    if (m <= 0) return;
+    auto stage = [&](int b, int of) {
+        const size_t at = (row * a.nmb + b) * D;
+        const uint32_t dst = smem_u32(smem) + of * BYTES;
+        for (int i = tid; i < D * 8; i += MOVE_NT)
+            cp_async16(dst + i * 16, i < D * 4 ? a.k8 + at * 64 + i * 16 : i < D * 6 ? a.km + at * 32 + (i - D * 4) * 16
+                                                                                : a.kl + at * 32 + (i - D * 6) * 16);
+    };
+    stage(blk, 0);
+    if (tid < BLK) from[tid] = -1;
+    __syncthreads();
     if (tid < m) {
-        const int d = holes[i0 + tid], s = movers[i0 + tid];
-        dst[tid] = d - blk * BLK;
+        const int d = a.holes[row * a.most + i0 + tid], s = a.movers[row * a.most + i0 + tid];
+        to[tid] = d;
         src[tid] = s;
+        from[d - blk * BLK] = s;
         a.weights[row * a.L + d] = a.weights[row * a.L + s];
         a.positions[row * a.L + d] = position_of(a, a.positions + row * a.L, s);
     }
-    const size_t t0 = row * a.nmb * D;                  // rows of 64 (32) bytes: [block][channel]
-    const uint4 *k8 = reinterpret_cast<const uint4*>(a.k8 + (t0 + (size_t)blk * D) * 64),
-                *km = reinterpret_cast<const uint4*>(a.km + (t0 + (size_t)blk * D) * 32),
-                *kl = reinterpret_cast<const uint4*>(a.kl + (t0 + (size_t)blk * D) * 32);
-    uint4* t4 = reinterpret_cast<uint4*>(tile);
-    for (int i = tid; i < D * 8; i += 256)
-        t4[i] = i < D * 4 ? k8[i] : i < D * 6 ? km[i - D * 4] : kl[i - D * 6];
     __syncthreads();
-    uint8_t *tm = tile + D * 64, *tl = tm + D * 32;
-    // high bytes and nibbles of one channel: a lane per free place; two places may share a nibble byte, so each nibble is
-    // cleared and set with an atomic on its word
-    for (int c = warp; c < D; c += 8)
-        for (int j = lane; j < m; j += 32) {
-            const int s = src[j], d = dst[j];
-            const size_t at = t0 + (size_t)(s >> 6) * D + c;
-            tile[c * 64 + d] = a.k8[at * 64 + (s & 63)];
-            const int from = 4 * (1 - (s & 1)), to = 8 * ((d >> 1) & 3) + 4 * (1 - (d & 1));
-            const uint32_t x = (a.km[at * 32 + ((s & 63) >> 1)] >> from) & 15u, y = (a.kl[at * 32 + ((s & 63) >> 1)] >> from) & 15u;
-            unsigned* wm = reinterpret_cast<unsigned*>(tm + c * 32) + (d >> 3);
-            unsigned* wl = reinterpret_cast<unsigned*>(tl + c * 32) + (d >> 3);
-            atomicAnd(wm, ~(15u << to));
-            atomicOr(wm, x << to);
-            atomicAnd(wl, ~(15u << to));
-            atomicOr(wl, y << to);
-        }
-    // V rows: 16 lanes per token, 16 bytes each (D = 128: 8 of high bytes, 4 of either nibble plane)
-    const int per = D >> 3;
-    for (int i = tid; i < m * per; i += 256) {
-        const int j = i / per, v = i - j * per;
-        const size_t s = row * a.L + src[j], d = row * a.L + (size_t)blk * BLK + dst[j];
-        if (v < D / 16)
-            reinterpret_cast<uint4*>(a.v8 + d * D)[v] = reinterpret_cast<const uint4*>(a.v8 + s * D)[v];
-        else if (v < D / 16 + D / 32)
-            reinterpret_cast<uint4*>(a.vm + d * (D / 2))[v - D / 16] = reinterpret_cast<const uint4*>(a.vm + s * (D / 2))[v - D / 16];
-        else
-            reinterpret_cast<uint4*>(a.vl + d * (D / 2))[v - D / 16 - D / 32] =
-                reinterpret_cast<const uint4*>(a.vl + s * (D / 2))[v - D / 16 - D / 32];
+    const int b0 = src[0] >> 6, b1 = src[m - 1] >> 6;   // (survivors ascend)
+    for (int b = b0; b <= min(b0 + STAGED - 1, b1); ++b) stage(b, 1 + b - b0);
+    cp_async_commit();
+    // V while the blocks are on their way
+    uint4 v[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int i = tid + e * MOVE_NT, j = i / PIECES, c = i % PIECES;
+        if (j >= m) continue;
+        const size_t s = row * a.L + src[j];
+        v[e] = *reinterpret_cast<const uint4*>(c < D / 16 ? a.v8 + s * D + c * 16 : c < D * 3 / 32 ? a.vm + s * (D / 2) + (c - D / 16) * 16
+                                                                                           : a.vl + s * (D / 2) + (c - D * 3 / 32) * 16);
     }
-    __syncthreads();
-    uint4 *o8 = reinterpret_cast<uint4*>(a.k8 + (t0 + (size_t)blk * D) * 64), *om = reinterpret_cast<uint4*>(a.km + (t0 + (size_t)blk * D) * 32),
-          *ol = reinterpret_cast<uint4*>(a.kl + (t0 + (size_t)blk * D) * 32);
-    for (int i = tid; i < D * 8; i += 256) {
-        if (i < D * 4) o8[i] = t4[i];
-        else if (i < D * 6) om[i - D * 4] = t4[i];
-        else ol[i - D * 6] = t4[i];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int i = tid + e * MOVE_NT, j = i / PIECES, c = i % PIECES;
+        if (j >= m) continue;
+        const size_t d = row * a.L + to[j];
+        *reinterpret_cast<uint4*>(c < D / 16 ? a.v8 + d * D + c * 16 : c < D * 3 / 32 ? a.vm + d * (D / 2) + (c - D / 16) * 16
+                                                                                : a.vl + d * (D / 2) + (c - D * 3 / 32) * 16) = v[e];
+    }
+    const int s0 = from[2 * lane], s1 = from[2 * lane + 1];
+    for (int b = b0; b <= b1; b += STAGED) {
+        cp_async_wait<0>();
+        __syncthreads();
+        const int r0 = s0 < 0 ? -1 : (s0 >> 6) - b, r1 = s1 < 0 ? -1 : (s1 >> 6) - b;
+        const bool t0 = r0 >= 0 && r0 < STAGED, t1 = r1 >= 0 && r1 < STAGED;
+        const uint8_t *x0 = smem + (t0 ? (1 + r0) * BYTES : 0), *x1 = smem + (t1 ? (1 + r1) * BYTES : 0);
+        // (a place that takes nothing here reads itself)
+        const int c0 = t0 ? s0 & 63 : 2 * lane, c1 = t1 ? s1 & 63 : 2 * lane + 1;
+        const int n0 = 4 * (1 - (c0 & 1)), n1 = 4 * (1 - (c1 & 1));
+        if (t0 || t1) {
+#pragma unroll 4
+            for (int c = warp; c < D; c += MOVE_NT / 32) {
+                const uint32_t h0 = x0[c * 64 + c0], h1 = x1[c * 64 + c1];
+                const uint32_t m0 = x0[D * 64 + c * 32 + (c0 >> 1)], m1 = x1[D * 64 + c * 32 + (c1 >> 1)];
+                const uint32_t l0 = x0[D * 96 + c * 32 + (c0 >> 1)], l1 = x1[D * 96 + c * 32 + (c1 >> 1)];
+                *reinterpret_cast<uint16_t*>(smem + c * 64 + 2 * lane) = (uint16_t)(h0 | h1 << 8);
+                smem[D * 64 + c * 32 + lane] = (uint8_t)((m0 >> n0 & 15u) << 4 | (m1 >> n1 & 15u));
+                smem[D * 96 + c * 32 + lane] = (uint8_t)((l0 >> n0 & 15u) << 4 | (l1 >> n1 & 15u));
+            }
+        }
+        __syncthreads();
+        for (int e = b + STAGED; e <= min(b + 2 * STAGED - 1, b1); ++e) stage(e, 1 + e - b - STAGED);
+        cp_async_commit();
+    }
+    uint4* o8 = reinterpret_cast<uint4*>(a.k8 + (row * a.nmb + blk) * (size_t)(D * 64));
+    uint4* om = reinterpret_cast<uint4*>(a.km + (row * a.nmb + blk) * (size_t)(D * 32));
+    uint4* ol = reinterpret_cast<uint4*>(a.kl + (row * a.nmb + blk) * (size_t)(D * 32));
+    for (int i = tid; i < D * 8; i += MOVE_NT) {
+        const uint4 x = reinterpret_cast<const uint4*>(smem)[i];
+        if (i < D * 4) o8[i] = x;
+        else if (i < D * 6) om[i - D * 4] = x;
+        else ol[i - D * 6] = x;
     }
 }
 
-// blockIdx.y == 0: the weights of the residual tokens follow the survivors, zeros behind them; else: K nibble planes of a freed
+// blockIdx.x == 0: the weights of the residual tokens follow the survivors, zeros behind them; else: K nibble planes of a freed
 // block (the K writer adds nibbles, so a block is zero before it is written again).
 __global__ void __launch_bounds__(256) clear_kernel(const EvictArgs a) {
     __shared__ float tail[BLK];
     pdl_enter();
-    const size_t row = blockIdx.x;
+    const size_t row = blockIdx.y;
     const int tid = threadIdx.x;
-    if (blockIdx.y == 0) {
+    if (blockIdx.x == 0) {
         float* w = a.weights + row * a.L;
         if (tid < a.rest) tail[tid] = w[a.n + tid];
         __syncthreads();
         for (int i = a.keep + tid; i < a.n + a.rest; i += 256) w[i] = i - a.keep < a.rest ? tail[i - a.keep] : 0.f;
         return;
     }
-    const size_t at = (row * a.nmb + a.keep / BLK + blockIdx.y - 1) * (size_t)a.D * 2;
+    const size_t at = (row * a.nmb + a.keep / BLK + blockIdx.x - 1) * (size_t)a.D * 2;
     for (int i = tid; i < a.D * 2; i += 256) {
         reinterpret_cast<uint4*>(a.km)[at + i] = make_uint4(0, 0, 0, 0);
         reinterpret_cast<uint4*>(a.kl)[at + i] = make_uint4(0, 0, 0, 0);
     }
+}
+
+int launch_select(const EvictArgs& a, int rows, int ctas, cudaStream_t st) {
+    const size_t smem = a.held ? (size_t)a.share * 4 : 0;
+    int rc = cuda_status(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MOST * 4),
+                         "evict select shared memory");
+    if (rc != AKV_OK) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas, rows);
+    cfg.blockDim = dim3(SEL_NT);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = ctas;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = tuning().pdl ? 2 : 1;
+    count_launch();
+    rc = cuda_status(cudaLaunchKernelEx(&cfg, select_kernel, a), "evict select launch");
+    return rc;
 }
 
 int check_planes(const char* fn, const akv_layer* a) {
@@ -274,7 +398,7 @@ int check_planes(const char* fn, const akv_layer* a) {
                 a->max_seq_len <= INT_MAX - 128, AKV_ERR_SHAPE,
                 "%s: unsupported extent (bsz %d, KV heads %d, head_dim %d [64 or 128], max_seq_len %d)", fn, a->bsz, a->n_kv_heads,
                 a->head_dim, a->max_seq_len);
-    AKV_REQUIRE((long long)a->bsz * a->n_kv_heads < (1ll << 30), AKV_ERR_OVERFLOW, "%s: too many rows", fn);
+    AKV_REQUIRE((long long)a->bsz * a->n_kv_heads <= 65535, AKV_ERR_OVERFLOW, "%s: more than 65535 (batch, KV head) rows", fn);
     AKV_REQUIRE(aligned16(a->k_first_8) && aligned16(a->k_mid_4) && aligned16(a->k_last_4) && aligned16(a->v_first_8) &&
                 aligned16(a->v_mid_4) && aligned16(a->v_last_4), AKV_ERR_ALIGN, "%s: pointers must be 16-byte aligned", fn);
     return AKV_OK;
@@ -316,7 +440,7 @@ int akv_tree_commit(const akv_layer* layer, const void* k_new, const void* v_new
 long long akv_evict_scratch_bytes(int bsz, int n_kv_heads, int n_tokens, int keep) {
     if (bsz <= 0 || n_kv_heads <= 0 || keep <= 0 || keep > n_tokens) return -1;
     const long long most = keep < n_tokens - keep ? keep : n_tokens - keep;
-    return (long long)bsz * n_kv_heads * (2 * most + 1) * 4;
+    return (long long)bsz * n_kv_heads * (2 * most + keep / BLK + 1) * 4;
 }
 
 int akv_evict(const akv_layer* layer, void* weights, void* positions, int rest_len, int rest_start, int keep, int recent,
@@ -332,7 +456,6 @@ int akv_evict(const akv_layer* layer, void* weights, void* positions, int rest_l
                 shift <= INT_MAX - 64 - l.max_seq_len, AKV_ERR_SHAPE,
                 "evict: keep %d [multiple of 64], recent %d of %d + %d tokens of %d, %d arranged, shift %d", keep, recent, rest_start,
                 rest_len, l.max_seq_len, arranged, shift);
-    AKV_REQUIRE(rest_start / BLK < 65535, AKV_ERR_OVERFLOW, "evict: more than 65534 blocks");
     AKV_REQUIRE((reinterpret_cast<uintptr_t>(weights) & 3u) == 0 && (reinterpret_cast<uintptr_t>(positions) & 3u) == 0 &&
                 aligned16(l.scratch), AKV_ERR_ALIGN, "evict: weights and positions must be 4-byte, scratch 16-byte aligned");
     AKV_REQUIRE(l.scratch_bytes >= akv_evict_scratch_bytes(l.bsz, l.n_kv_heads, rest_start, keep), AKV_ERR_SHAPE,
@@ -348,9 +471,9 @@ int akv_evict(const akv_layer* layer, void* weights, void* positions, int rest_l
     a.vm = static_cast<uint8_t*>(l.v_mid_4);
     a.vl = static_cast<uint8_t*>(l.v_last_4);
     a.most = keep < rest_start - keep ? keep : rest_start - keep;
-    a.count = static_cast<int*>(l.scratch);
-    a.holes = a.count + rows;
+    a.holes = static_cast<int*>(l.scratch);
     a.movers = a.holes + (size_t)rows * a.most;
+    a.start = a.movers + (size_t)rows * a.most;
     a.D = l.head_dim;
     a.L = l.max_seq_len;
     a.nmb = (l.max_seq_len + BLK - 1) / BLK;
@@ -361,11 +484,20 @@ int akv_evict(const akv_layer* layer, void* weights, void* positions, int rest_l
     a.arranged = arranged;
     a.shift = shift;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    launch_chained(select_kernel, dim3(rows), dim3(SEL_NT), 0, st, a);
-    if ((rc = cuda_status(cudaGetLastError(), "evict select launch")) != AKV_OK || keep == rest_start) return rc;
-    launch_chained(move_kernel, dim3(rows, keep / BLK), dim3(256), (size_t)l.head_dim * 128, st, a);
+    // CTAs of a row: so many that all SMs have some and none has less than two thousand places, at most eight (what a cluster may
+    // have everywhere)
+    int ctas = 1;
+    while (ctas < 8 && ((rest_start + ctas - 1) / ctas > SEL_MOST || (rows * ctas < sm_count() && rest_start / ctas > 2 * SEL_NT))) ctas *= 2;
+    a.share = ((rest_start + ctas - 1) / ctas + SEL_NT - 1) / SEL_NT * SEL_NT;
+    a.held = a.share <= SEL_MOST;
+    if ((rc = launch_select(a, rows, ctas, st)) != AKV_OK || keep == rest_start) return rc;
+    const size_t smem = (size_t)(1 + STAGED) * l.head_dim * 128;
+    auto move = l.head_dim == 128 ? move_kernel<128> : move_kernel<64>;
+    rc = cuda_status(cudaFuncSetAttribute(move, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "evict shared memory");
+    if (rc != AKV_OK) return rc;
+    launch_chained(move, dim3(keep / BLK, rows), dim3(MOVE_NT), smem, st, a);
     if ((rc = cuda_status(cudaGetLastError(), "evict move launch")) != AKV_OK) return rc;
-    launch_chained(clear_kernel, dim3(rows, 1 + (rest_start - keep) / BLK), dim3(256), 0, st, a);
+    launch_chained(clear_kernel, dim3(1 + (rest_start - keep) / BLK, rows), dim3(256), 0, st, a);
     return cuda_status(cudaGetLastError(), "evict clear launch");
 }
 
