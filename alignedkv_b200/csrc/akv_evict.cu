@@ -5,6 +5,7 @@
 //   clear_kernel     K nibble planes, weights behind the survivors
 #include <limits.h>
 
+#include "akv_planes.cuh"
 #include "akv_save.cuh"
 
 namespace akv {
@@ -108,15 +109,15 @@ __device__ __forceinline__ uint32_t cluster_ld(const void* p, uint32_t cta) {
 }
 
 // A cluster per row; a CTA has `share` consecutive places and keeps their keys in shared memory: one read of the weights, whatever is
-// counted.  The keep-th largest key by four counts of eight bits (a column of the count per lane: no two lanes of a warp meet, although
-// weights crowd into few exponents), added up over the cluster through distributed shared memory; every CTA draws the same
+// counted.  The keep-th largest key by four counts of eight bits (in eight columns: few lanes of a warp meet, although weights crowd into
+// few exponents), added up over the cluster through distributed shared memory; every CTA draws the same
 // conclusion.  Then ties, free places and survivors behind are numbered in order: per warp, per CTA, per cluster.
 constexpr int SEL_NT = 1024, SEL_W = SEL_NT / 32, SEL_MOST = 40960;      // SEL_MOST: keys a CTA can keep
 __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
     extern __shared__ __align__(16) uint32_t keys[];
-    __shared__ int hist[256 * 32];
+    __shared__ int hist[8 * 257];                  // [column][digit], columns a bank apart
     __shared__ uint32_t sums[2][256];              // this CTA's counts: two buffers, so that one barrier a round is enough
-    __shared__ uint32_t found[2], scan[3][SEL_W + 1], totals[2][2];
+    __shared__ uint32_t found[2], warp_sum[8], scan[3][SEL_W + 1], totals[2][2];
     pdl_enter();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint32_t ctas, rank;
@@ -127,53 +128,50 @@ __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
     int* pos = a.positions + row * a.L;
     const int safe_from = a.n + a.shift - a.recent;
     const int first = min((int)rank * a.share, a.n), count = min(a.share, a.n - first);
-    auto key = [&](int i) { return key_of(w[first + i], position_of(a, pos, first + i) >= safe_from); };
-    if (a.held)
+    auto key = [&](int i) { return key_of(w[first + i], a.recent && position_of(a, pos, first + i) >= safe_from); };
+    if (a.held) {
+#pragma unroll 8
         for (int i = tid; i < count; i += SEL_NT) keys[i] = key(i);
+    }
     auto at = [&](int i) { return a.held ? keys[i] : key(i); };
     uint32_t prefix = 0;
     uint32_t want = a.keep;                            // how many of the keys that share the prefix stay
     for (int round = 0; round < 4; ++round) {
         const int bit = 24 - 8 * round;
-        for (int i = tid; i < 256 * 32; i += SEL_NT) hist[i] = 0;
+        for (int i = tid; i < 8 * 257; i += SEL_NT) hist[i] = 0;
         __syncthreads();
+#pragma unroll 4
         for (int i = tid; i < count; i += SEL_NT) {
             const uint32_t k = at(i);
-            if (round == 0 || (k >> (bit + 8)) == (prefix >> (bit + 8))) atomicAdd(&hist[((k >> bit) & 255) * 32 + lane], 1);
+            if (round == 0 || (k >> (bit + 8)) == (prefix >> (bit + 8))) atomicAdd(&hist[(lane & 7) * 257 + ((k >> bit) & 255)], 1);
         }
         __syncthreads();
-        for (int d = warp; d < 256; d += SEL_W) {
-            int c = hist[d * 32 + lane];
+        if (tid < 256) {
+            uint32_t c = 0;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xFFFFFFFFu, c, o);
-            if (lane == 0) sums[round & 1][d] = c;
+            for (int j = 0; j < 8; ++j) c += hist[j * 257 + tid];
+            sums[round & 1][tid] = c;
         }
         cluster_sync();
-        if (warp == 0) {
-            // lane: digits 255 - 8 lane .. 248 - 8 lane, from above
-            uint32_t c[8], mine = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                c[j] = 0;
-                for (uint32_t r = 0; r < ctas; ++r) c[j] += cluster_ld(&sums[round & 1][255 - 8 * lane - j], r);
-                mine += c[j];
-            }
-            uint32_t above = mine;
+        // thread: digit 255 - tid; keys with a larger one, by the sums of the lanes and warps in front
+        uint32_t c = 0, above = 0;
+        if (tid < 256) {
+            for (uint32_t r = 0; r < ctas; ++r) c += cluster_ld(&sums[round & 1][255 - tid], r);
+            above = c;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, above, o);
                 if (lane >= o) above += x;
             }
-            above -= mine;
-            if (above < want && above + mine >= want) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (above < want && above + c[j] >= want) {
-                        found[0] = 255 - 8 * lane - j;
-                        found[1] = above;
-                    }
-                    above += c[j];
-                }
+            if (lane == 31) warp_sum[warp] = above;
+            above -= c;
+        }
+        __syncthreads();
+        if (tid < 256) {
+            for (int j = 0; j < warp; ++j) above += warp_sum[j];
+            if (above < want && above + c >= want) {
+                found[0] = 255 - tid;
+                found[1] = above;
             }
         }
         __syncthreads();
@@ -255,15 +253,17 @@ __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
 // CTA = one block of 64 places in front of `keep`: its free places take the survivors of the same numbers.  Survivors are read
 // only behind `keep` and places are written only in front of it, each by its own CTA: no order among the CTAs.
 // K, token-minor: one survivor is a byte of each of D rows and half a byte of 2 D.  The block and the blocks that its survivors come
-// from are staged in shared memory, three at a time; a warp takes a channel, a lane two neighbouring places (whose nibbles share a
-// byte), so that a row's bytes are read and written without a conflict.  V: rows of 16-byte pieces through registers.
-// Bound by HBM: the block twice, the blocks behind once.
-constexpr int MOVE_NT = 256, STAGED = 3;
+// from are put together to fp16 rows [channel][64 tokens] in shared memory, two of the latter at a time; a warp takes a channel, a lane
+// two neighbouring places, a survivor's value is one 2-byte load and store; at the end the block is split again.  (On the plane bytes
+// themselves that were three loads and, with the neighbour's nibble in the same byte, more than one store per value: shared memory's
+// pipe was 69% busy at 142 us for 8 x 32 x 4096 tokens to 2048.)  V: rows of 16-byte pieces through registers.
+// Floor: the block twice, the blocks behind once, V's rows twice.
+constexpr int MOVE_NT = 256, STAGED = 2;
 template <int D>
 __global__ void __launch_bounds__(MOVE_NT) move_kernel(const EvictArgs a) {
-    extern __shared__ __align__(16) uint8_t smem[];     // blocks of [D][64] high bytes, [D][32] twice: the places', then survivors'
+    extern __shared__ __align__(16) uint8_t smem[];     // blocks of [D] rows of 128 bytes, 16-byte piece q of row c at q ^ (c & 1)
     __shared__ int from[BLK], to[BLK], src[BLK];
-    constexpr int BYTES = D * 128, PIECES = D / 8, PER = BLK * PIECES / MOVE_NT;
+    constexpr int BYTES = D * 128, PIECES = D / 8, PER = BLK * PIECES / MOVE_NT, U = D * 4 / MOVE_NT;
     pdl_enter();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const size_t row = blockIdx.y;
@@ -271,14 +271,32 @@ __global__ void __launch_bounds__(MOVE_NT) move_kernel(const EvictArgs a) {
     const int* start = a.start + row * (a.keep / BLK + 1) + blk;
     const int i0 = start[0], m = start[1] - i0;
     if (m <= 0) return;
-    auto stage = [&](int b, int of) {
+    // thread: 16 tokens of U channels of a block
+    struct Bytes { uint4 h[U]; uint2 m[U], l[U]; };
+    auto load = [&](Bytes& x, int b) {
         const size_t at = (row * a.nmb + b) * D;
-        const uint32_t dst = smem_u32(smem) + of * BYTES;
-        for (int i = tid; i < D * 8; i += MOVE_NT)
-            cp_async16(dst + i * 16, i < D * 4 ? a.k8 + at * 64 + i * 16 : i < D * 6 ? a.km + at * 32 + (i - D * 4) * 16
-                                                                                : a.kl + at * 32 + (i - D * 6) * 16);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const size_t o = at * 4 + tid + u * MOVE_NT;
+            x.h[u] = reinterpret_cast<const uint4*>(a.k8)[o];
+            x.m[u] = reinterpret_cast<const uint2*>(a.km)[o];
+            x.l[u] = reinterpret_cast<const uint2*>(a.kl)[o];
+        }
     };
-    stage(blk, 0);
+    auto place = [&](int u) {                           // of the first of the thread's two pieces
+        const int i = tid + u * MOVE_NT, c = i >> 2;
+        return c * 128 + (((2 * (i & 3)) ^ (c & 1)) << 4);
+    };
+    auto put = [&](const Bytes& x, int of) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int o = place(u);
+            *reinterpret_cast<uint4*>(smem + of * BYTES + o) = halves8(x.h[u].x, x.h[u].y, x.m[u].x, x.l[u].x);
+            *reinterpret_cast<uint4*>(smem + of * BYTES + (o ^ 16)) = halves8(x.h[u].z, x.h[u].w, x.m[u].y, x.l[u].y);
+        }
+    };
+    Bytes mine, other[STAGED];
+    load(mine, blk);
     if (tid < BLK) from[tid] = -1;
     __syncthreads();
     if (tid < m) {
@@ -291,9 +309,9 @@ __global__ void __launch_bounds__(MOVE_NT) move_kernel(const EvictArgs a) {
     }
     __syncthreads();
     const int b0 = src[0] >> 6, b1 = src[m - 1] >> 6;   // (survivors ascend)
-    for (int b = b0; b <= min(b0 + STAGED - 1, b1); ++b) stage(b, 1 + b - b0);
-    cp_async_commit();
-    // V while the blocks are on their way
+#pragma unroll
+    for (int e = 0; e < STAGED; ++e)
+        if (b0 + e <= b1) load(other[e], b0 + e);
     uint4 v[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
@@ -303,6 +321,27 @@ __global__ void __launch_bounds__(MOVE_NT) move_kernel(const EvictArgs a) {
         v[e] = *reinterpret_cast<const uint4*>(c < D / 16 ? a.v8 + s * D + c * 16 : c < D * 3 / 32 ? a.vm + s * (D / 2) + (c - D / 16) * 16
                                                                                            : a.vl + s * (D / 2) + (c - D * 3 / 32) * 16);
     }
+    put(mine, 0);
+    const int s0 = from[2 * lane], s1 = from[2 * lane + 1], swap = (warp & 1) << 4;      // (a warp's channels are all odd or all even)
+    for (int b = b0; b <= b1; b += STAGED) {
+#pragma unroll
+        for (int e = 0; e < STAGED; ++e)
+            if (b + e <= b1) put(other[e], 1 + e);
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < STAGED; ++e)
+            if (b + STAGED + e <= b1) load(other[e], b + STAGED + e);
+        const int r0 = s0 < 0 ? -1 : (s0 >> 6) - b, r1 = s1 < 0 ? -1 : (s1 >> 6) - b;
+        const uint8_t *x0 = smem + (1 + r0) * BYTES + ((2 * (s0 & 63)) ^ swap), *x1 = smem + (1 + r1) * BYTES + ((2 * (s1 & 63)) ^ swap);
+        uint8_t* y = smem + ((4 * lane) ^ swap);
+        const bool t0 = r0 >= 0 && r0 < STAGED, t1 = r1 >= 0 && r1 < STAGED;
+#pragma unroll 4
+        for (int c = warp; c < D; c += MOVE_NT / 32) {
+            if (t0) *reinterpret_cast<uint16_t*>(y + c * 128) = *reinterpret_cast<const uint16_t*>(x0 + c * 128);
+            if (t1) *reinterpret_cast<uint16_t*>(y + c * 128 + 2) = *reinterpret_cast<const uint16_t*>(x1 + c * 128);
+        }
+        __syncthreads();
+    }
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
         const int i = tid + e * MOVE_NT, j = i / PIECES, c = i % PIECES;
@@ -311,39 +350,18 @@ __global__ void __launch_bounds__(MOVE_NT) move_kernel(const EvictArgs a) {
         *reinterpret_cast<uint4*>(c < D / 16 ? a.v8 + d * D + c * 16 : c < D * 3 / 32 ? a.vm + d * (D / 2) + (c - D / 16) * 16
                                                                                 : a.vl + d * (D / 2) + (c - D * 3 / 32) * 16) = v[e];
     }
-    const int s0 = from[2 * lane], s1 = from[2 * lane + 1];
-    for (int b = b0; b <= b1; b += STAGED) {
-        cp_async_wait<0>();
-        __syncthreads();
-        const int r0 = s0 < 0 ? -1 : (s0 >> 6) - b, r1 = s1 < 0 ? -1 : (s1 >> 6) - b;
-        const bool t0 = r0 >= 0 && r0 < STAGED, t1 = r1 >= 0 && r1 < STAGED;
-        const uint8_t *x0 = smem + (t0 ? (1 + r0) * BYTES : 0), *x1 = smem + (t1 ? (1 + r1) * BYTES : 0);
-        // (a place that takes nothing here reads itself)
-        const int c0 = t0 ? s0 & 63 : 2 * lane, c1 = t1 ? s1 & 63 : 2 * lane + 1;
-        const int n0 = 4 * (1 - (c0 & 1)), n1 = 4 * (1 - (c1 & 1));
-        if (t0 || t1) {
-#pragma unroll 4
-            for (int c = warp; c < D; c += MOVE_NT / 32) {
-                const uint32_t h0 = x0[c * 64 + c0], h1 = x1[c * 64 + c1];
-                const uint32_t m0 = x0[D * 64 + c * 32 + (c0 >> 1)], m1 = x1[D * 64 + c * 32 + (c1 >> 1)];
-                const uint32_t l0 = x0[D * 96 + c * 32 + (c0 >> 1)], l1 = x1[D * 96 + c * 32 + (c1 >> 1)];
-                *reinterpret_cast<uint16_t*>(smem + c * 64 + 2 * lane) = (uint16_t)(h0 | h1 << 8);
-                smem[D * 64 + c * 32 + lane] = (uint8_t)((m0 >> n0 & 15u) << 4 | (m1 >> n1 & 15u));
-                smem[D * 96 + c * 32 + lane] = (uint8_t)((l0 >> n0 & 15u) << 4 | (l1 >> n1 & 15u));
-            }
-        }
-        __syncthreads();
-        for (int e = b + STAGED; e <= min(b + 2 * STAGED - 1, b1); ++e) stage(e, 1 + e - b - STAGED);
-        cp_async_commit();
-    }
-    uint4* o8 = reinterpret_cast<uint4*>(a.k8 + (row * a.nmb + blk) * (size_t)(D * 64));
-    uint4* om = reinterpret_cast<uint4*>(a.km + (row * a.nmb + blk) * (size_t)(D * 32));
-    uint4* ol = reinterpret_cast<uint4*>(a.kl + (row * a.nmb + blk) * (size_t)(D * 32));
-    for (int i = tid; i < D * 8; i += MOVE_NT) {
-        const uint4 x = reinterpret_cast<const uint4*>(smem)[i];
-        if (i < D * 4) o8[i] = x;
-        else if (i < D * 6) om[i - D * 4] = x;
-        else ol[i - D * 6] = x;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int o = place(u);
+        const uint4 x = *reinterpret_cast<const uint4*>(smem + o), y = *reinterpret_cast<const uint4*>(smem + (o ^ 16));
+        uint4 h;
+        uint2 n, l;
+        v_split4(x.x, x.y, x.z, x.w, h.x, h.y, n.x, l.x);
+        v_split4(y.x, y.y, y.z, y.w, h.z, h.w, n.y, l.y);
+        const size_t at = (row * a.nmb + blk) * D * 4 + tid + u * MOVE_NT;
+        reinterpret_cast<uint4*>(a.k8)[at] = h;
+        reinterpret_cast<uint2*>(a.km)[at] = n;
+        reinterpret_cast<uint2*>(a.kl)[at] = l;
     }
 }
 

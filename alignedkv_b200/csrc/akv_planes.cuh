@@ -29,6 +29,13 @@ __device__ __forceinline__ void line8(uint32_t (&w)[4], uint32_t h0, uint32_t h1
     w[3] = __byte_perm(odd, h1, 0x7352);
 }
 
+// The same eight elements in order.
+__device__ __forceinline__ uint4 halves8(uint32_t h0, uint32_t h1, uint32_t m, uint32_t l) {
+    const uint32_t even = (m & 0xF0F0F0F0u) | ((l >> 4) & 0x0F0F0F0Fu), odd = ((m << 4) & 0xF0F0F0F0u) | (l & 0x0F0F0F0Fu);
+    const uint32_t a = __byte_perm(even, odd, 0x5140), b = __byte_perm(even, odd, 0x7362);
+    return make_uint4(__byte_perm(a, h0, 0x5140), __byte_perm(a, h0, 0x7362), __byte_perm(b, h1, 0x5140), __byte_perm(b, h1, 0x7362));
+}
+
 // What a lane holds of one line: N elements, N / 8 groups of eight.
 template <int N>
 struct Line {
