@@ -1,12 +1,11 @@
-// Attention of a tree of drafted tokens over the plane cache, and the attention weights of its queries.
-//   tree_kernel      per (batch, KV head): the T * group query rows against the planes, the residual tokens and the drafted
-//                    tokens that the tree lets them see; one pass with a running maximum and sum
-//   tree_merge_kernel   joins the partial results of units that several warps share
-//   weights_kernel   weights[t] += sum over the rows of exp(s_t - lse)
+// Attention of a tree of drafted tokens over the plane cache, and the entries of it and of its queries' weights.
+//   tree_kernel         per (batch, KV head): up to 16 query rows against the planes, the residual tokens and the drafted tokens that
+//                       the tree lets them see; one pass with a running maximum and sum (more rows: akv_tree_wide.cu)
+//   tree_merge_kernel   joins the partial results of units that several runs share
 //
 //   s_rj = scale q_r . k_j (+ mask_j), o_r = sum_j exp(s_rj - m_r) v_j / l_r, l_r = sum_j exp(s_rj - m_r).
 //
-// All planes are read: 2 bytes per cached element, once per 16 rows.  Bound by HBM while the rows of a KV head are few.
+// All planes are read: 2 bytes per cached element, once.  Bound by HBM.
 // Work: a unit is 16 query rows of one (batch, KV head); its tiles are 128 tokens of the planes each, and one tail tile of the
 // residual tokens with the drafted ones behind them (at most 127).  The tiles of all units in a row are dealt to the warps in equal
 // contiguous runs, so that every SM gets the same whatever the number of units and their length.  A warp needs no other one: it
@@ -33,7 +32,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool th
 // A warp's ring of 4 KB steps in shared memory, filled STEPS - 1 steps ahead by its own asynchronous copies.
 //   K step    16 channels of the tile's 128 tokens: high bytes [block][channel][64], nibbles [block][channel][32] twice
 //   V step    32 (D = 128: 16) tokens: for each 16 of them high bytes [4t + i][D], nibbles [..][D / 2] twice
-//   tail      16 tokens of the tail as fp16 rows [token][D]: a K step, then (WITH_V) their V step
+//   tail      16 tokens of the tail as fp16 rows [token][D]: a K step, then their V step
 // The 16-byte pieces of a 128-byte line are swapped by XOR so that a quarter (half) warp's 16-byte (8-byte) loads of a line's
 // pieces by lane (g, t) fall into different banks.
 constexpr int STEPS = 5, STEP_BYTES = 4096;
@@ -45,26 +44,22 @@ struct Ring {
     static constexpr int KSTEPS = D / 16, VSTEPS = D / 16, SUB = 128 / D;     // SUB: products of 16 tokens per V step
     uint32_t base;                 // of the warp's ring
     int lane, put, get;            // steps: slots filled next, read next
-    // what is copied next: step of a tile of (batch, KV head) bh; left = tiles from this one on.  Every tile `times` times.
+    // what is copied next: step of a tile of (batch, KV head) bh; left = tiles from this one on
     long long bh, left;
-    int step, tile, unit, units_per_head, time, times, plane_tiles;
+    int step, tile, unit, plane_tiles;
 
     // Tiles first .. last - 1 of units of p.tiles tiles.
-    template <bool WITH_V>
-    __device__ __forceinline__ void start(const TreeArgs& p, uint32_t at, int of_lane, long long first, long long last,
-                                          int per_head, int reps) {
+    __device__ __forceinline__ void start(const TreeArgs& p, uint32_t at, int of_lane, long long first, long long last) {
         base = at;
         lane = of_lane;
-        put = get = step = time = 0;
-        units_per_head = per_head;
-        times = reps;
+        put = get = step = 0;
         plane_tiles = (p.nb + 1) >> 1;
         unit = (int)(first / p.tiles);
         tile = (int)(first - (long long)unit * p.tiles);
-        left = (last - first) * reps;
-        bh = unit / units_per_head;
+        left = last - first;
+        bh = unit / p.rt;
 #pragma unroll 1
-        for (int i = 0; i < STEPS - 1; ++i) fill<WITH_V>(p);
+        for (int i = 0; i < STEPS - 1; ++i) fill(p);
     }
     __device__ __forceinline__ uint32_t slot(int i) const { return base + (uint32_t)i * STEP_BYTES; }
 
@@ -139,15 +134,14 @@ struct Ring {
     }
 
     // One step further, if there is one; always a group, so that the groups count the steps.
-    template <bool WITH_V>
     __device__ __forceinline__ void fill(const TreeArgs& p) {
         if (left > 0) {
             const uint32_t to = slot(put);
-            int steps = WITH_V ? KSTEPS + VSTEPS : KSTEPS;
+            int steps = KSTEPS + VSTEPS;
             if (tile == plane_tiles) {
-                steps = ((p.tail + 15) >> 4) * (WITH_V ? 2 : 1);
-                copy_tail(p, to, WITH_V ? step >> 1 : step, WITH_V && (step & 1));
-            } else if (!WITH_V || step < KSTEPS) {
+                steps = ((p.tail + 15) >> 4) * 2;
+                copy_tail(p, to, step >> 1, step & 1);
+            } else if (step < KSTEPS) {
                 copy_k(p, to);
             } else {
                 copy_v(p, to, step - KSTEPS);
@@ -155,26 +149,20 @@ struct Ring {
             if (++step == steps) {
                 step = 0;
                 --left;
-                next(p);
+                if (++tile == p.tiles) {
+                    tile = 0;
+                    bh = ++unit / p.rt;
+                }
             }
         }
         cp_async_commit();
         put = put + 1 == STEPS ? 0 : put + 1;
     }
-    __device__ __forceinline__ void next(const TreeArgs& p) {
-        if (++time < times) return;
-        time = 0;
-        if (++tile == p.tiles) {
-            tile = 0;
-            bh = ++unit / units_per_head;
-        }
-    }
     // Waits for the step that is read next, requests the one whose slot the last read has left.
-    template <bool WITH_V>
     __device__ __forceinline__ uint32_t take(const TreeArgs& p) {
         cp_async_wait<STEPS - 2>();
         __syncwarp();
-        fill<WITH_V>(p);
+        fill(p);
         const uint32_t at = slot(get);
         get = get + 1 == STEPS ? 0 : get + 1;
         return at;
@@ -204,13 +192,13 @@ struct Ring {
 };
 
 // Scores of a plane tile: s[j][c] = row g (c < 2) or g + 8, token 16 (2t + (c & 1)) + j.
-template <int D, bool WITH_V>
+template <int D>
 __device__ __forceinline__ void plane_scores(float (&s)[16][4], const uint4* qf, const TreeArgs& p, Ring<D>& ring) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll 1
     for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t at = ring.template take<WITH_V>(p);
+        const uint32_t at = ring.take(p);
         Line<16> x[4];
         ring.lines_k(x, at);
         mma_lines<16>(s, qf[kk * 32 + ring.lane], x);
@@ -295,7 +283,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
     uint4* qf = reinterpret_cast<uint4*>(smem + (size_t)warp * WARP_BYTES + STEPS * STEP_BYTES);
     uint4* pf = qf + 256;
     Ring<D> ring;
-    ring.template start<true>(p, smem_u32(smem) + warp * WARP_BYTES, lane, first, last, p.rt, 1);
+    ring.start(p, smem_u32(smem) + warp * WARP_BYTES, lane, first, last);
     for (long long at = first; at < last;) {
         const long long unit = at / p.tiles, bh = unit / p.rt, b = bh / p.H;
         const int h = (int)(bh - b * p.H), row0 = (int)(unit - bh * p.rt) * ROWS;
@@ -309,7 +297,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
         for (int tile = t0; tile < min(t1, p.tiles - 1); ++tile) {
             {
                 float s[16][4];
-                plane_scores<D, true>(s, qf, p, ring);
+                plane_scores<D>(s, qf, p, ring);
                 const int count = p.nb * BLK - tile * TILE;
                 if (mask || count < TILE) {             // tokens that do not exist or are masked away: -inf
 #pragma unroll
@@ -338,7 +326,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
             }
 #pragma unroll 1
             for (int vs = 0; vs < Ring<D>::VSTEPS; ++vs) {
-                const uint32_t from = ring.template take<true>(p);
+                const uint32_t from = ring.take(p);
 #pragma unroll
                 for (int u = 0; u < Ring<D>::SUB; ++u) {
                     const int st = vs * Ring<D>::SUB + u;
@@ -364,7 +352,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
 #pragma unroll 1
             for (int c0 = 0; c0 < p.tail; c0 += 16) {
                 float s[2][4];
-                tail_scores<D>(s, qf, ring.template take<true>(p), lane);
+                tail_scores<D>(s, qf, ring.take(p), lane);
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -382,7 +370,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
                                            pack_half2(s[1][2], s[1][3]));
                 // What one row sees is masked for another, and 0 * inf would be NaN: values that are not finite are left
                 // out of the product and added by the rows that see them.
-                const uint32_t from = ring.template take<true>(p);
+                const uint32_t from = ring.take(p);
                 bool odd = false;
                 uint32_t x[4][N / 2];
 #pragma unroll
@@ -522,78 +510,6 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs p) {
     for (int c = 0; c < C; c += 2)
         *reinterpret_cast<uint32_t*>(p.out + to * D + C * lane + c) = pack_half2(acc[c] * inv, acc[c + 1] * inv);
     if (p.lse && lane == 0) p.lse[to] = l == 0.f ? -INFINITY : (base - LIFT + log2f(l)) * LN2;
-}
-
-// A warp per 128 cached tokens of a (batch, KV head); all query rows of the head, 16 at a time, added in their order.
-template <int D>
-__global__ void __launch_bounds__(32 * WARPS, 1) weights_kernel(const TreeArgs p, float* __restrict__ weights) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    pdl_enter();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int R = p.T * p.G, full = (p.nb + 1) >> 1;
-    const long long w = (long long)warp * gridDim.x + blockIdx.x;
-    if (w >= p.nw) return;
-    const long long first = w * p.total / p.nw, last = (w + 1) * p.total / p.nw;
-    uint4* qf = reinterpret_cast<uint4*>(smem + (size_t)warp * WARP_BYTES + STEPS * STEP_BYTES);
-    Ring<D> ring;
-    ring.template start<false>(p, smem_u32(smem) + warp * WARP_BYTES, lane, first, last, 1, (R + ROWS - 1) / ROWS);
-    for (long long at = first; at < last; ++at) {
-        const long long bh = at / p.tiles, b = bh / p.H;
-        const int h = (int)(bh - b * p.H), tile = (int)(at - bh * p.tiles);
-        const bool tail = tile == full;
-        const int start = tail ? p.nb * BLK : tile * TILE, count = tail ? p.rest : min(TILE, p.nb * BLK - start);
-        const __half* mask = p.mask ? p.mask + b * p.mask_stride : nullptr;
-        float* into = weights + bh * p.L + start;
-        float sum[16][2];          // of plane token 16 (2t + c) + j; of the tail's 16 i + 8 j + 2t + c in sum[2 i + j]
-#pragma unroll
-        for (int j = 0; j < 16; ++j) sum[j][0] = sum[j][1] = 0.f;
-        auto token = [&](int j, int c) { return tail ? 8 * j + 2 * t + c : 16 * (2 * t + c) + j; };
-#pragma unroll 1
-        for (int row0 = 0; row0 < R; row0 += ROWS) {
-            load_q<D>(qf, p, b, h, row0, lane);
-            float s[16][4], off[2];
-            if (!tail) {
-                plane_scores<D, false>(s, qf, p, ring);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (16 * i >= p.rest) break;
-                    float part[2][4];
-                    tail_scores<D>(part, qf, ring.template take<false>(p), lane);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        s[2 * i][c] = part[0][c];
-                        s[2 * i + 1][c] = part[1][c];
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = row0 + g + 8 * i;
-                off[i] = r < R ? p.lse[row_of(p, b, h, r)] : -INFINITY;
-            }
-            // exp(score - lse) with one rounding of the small difference: scores of 25 are half of 2e-6 off themselves
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int tok = token(j, c);
-                    const float add = mask && tok < count ? __half2float(mask[start + tok]) : 0.f;
-                    if (tok >= count || add == -INFINITY) continue;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)        // (a row that sees nothing has lse = -inf)
-                        if (off[i] != -INFINITY) sum[j][c] += ex2(fmaf(s[j][2 * i + c], p.scale, add - off[i]) * LOG2E);
-                }
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) sum[j][c] += __shfl_xor_sync(0xFFFFFFFFu, sum[j][c], o);
-                if (g == (j >> 1) && token(j, c) < count) into[token(j, c)] += sum[j][c];
-            }
-    }
 }
 
 // Warps for `total` tiles: one an SM while there are that few, then up to eight.
@@ -756,12 +672,10 @@ int akv_tree_weights(const akv_layer* layer, const void* q, const void* lse, con
     p.tail = rest_len;
     p.total = (long long)layer->bsz * p.H * p.tiles;
     if (p.total == 0) return AKV_OK;
-    const Deal d = deal(p.total);
+    const Deal d = deal(p.total, 1);
     p.nw = d.runs;
-    rc = launch_warps(layer->head_dim == 128 ? weights_kernel<128> : weights_kernel<64>, d, static_cast<cudaStream_t>(stream), p,
-                      static_cast<float*>(weights));
-    if (rc != AKV_OK) return rc;
-    return cuda_status(cudaGetLastError(), "tree_weights launch");
+    p.rt = 1;
+    return launch_weights_wide(p, layer->head_dim, d.grid, static_cast<float*>(weights), static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

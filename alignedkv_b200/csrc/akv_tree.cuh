@@ -43,5 +43,6 @@ __device__ __forceinline__ long long row_of(const TreeArgs& p, long long b, int 
 
 // Tensor-core form (akv_tree_wide.cu).
 int launch_tree_wide(const TreeArgs& p, int D, int ctas, cudaStream_t st);
+int launch_weights_wide(const TreeArgs& p, int D, int ctas, float* weights, cudaStream_t st);
 
 }  // namespace akv

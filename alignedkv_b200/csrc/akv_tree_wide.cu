@@ -103,9 +103,9 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 __device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t lead, uint32_t stride) {
     return (uint64_t)(at >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
-// fp16 x fp16 -> fp32, 128 rows, n columns; A K-major, B MN-major if so.
-__device__ __forceinline__ constexpr uint32_t instruction(int n, bool b_mn) {
-    return 1u << 4 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+// fp16 x fp16 -> fp32, 128 rows, n columns; K-major, or MN-major if so.
+__device__ __forceinline__ constexpr uint32_t instruction(int n, bool b_mn, bool a_mn = false) {
+    return 1u << 4 | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
 }
 // 32 columns of this thread's lane
 __device__ __forceinline__ void tmem_ld(uint32_t (&v)[32], uint32_t at) {
@@ -196,35 +196,35 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w, bool& odd) {
 // A ring tile is two regions of 64 tokens, D * 128 bytes each.  As copied: the high bytes, then either nibble plane.  As operand: K rows
 // [channel] of 64 tokens; V [channel half][token] rows of 64 channels; 16-byte piece c of row r at c ^ (r & 7).  (The tail's keys:
 // [channel half][token] over the whole tile, for groups of eight tokens at one distance.)
-template <int D>
-__device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t base, uint32_t bars, volatile int* dead, long long first,
-                                          long long last) {
-    using L = Plan<D>;
+// L: the kernel's plan; KEYS: keys alone, tile after tile.  `has_tail`: whether the units' last tiles are tails.
+template <class L, int D, bool KEYS>
+__device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t ring_at, uint32_t ring, uint32_t bars, volatile int* dead,
+                                          long long first, long long last, bool has_tail) {
     uint32_t buf = 0, turn = 0;
     for (long long tile = first; tile < last;) {
         Segment s;
         s.at(p, tile, last);
         tile += s.c;
-        for (int q = 0; q < 2 * s.c; ++q) {
-            bool value;
-            const int i = s.t0 + tile_of(q, s.c, 3 - p.groups, value);
+        for (int q = 0; q < (KEYS ? 1 : 2) * s.c; ++q) {
+            bool value = false;
+            const int i = s.t0 + (KEYS ? q : tile_of(q, s.c, 3 - p.groups, value));
             const uint32_t bar = bars + 8 * (L::RAW + buf);
             bar_wait(bars + 8 * (L::EMPTY + buf), (turn & 1) ^ 1, dead);
-            if (i == p.tiles - 1) {
+            if (has_tail && i == p.tiles - 1) {
                 bar_arrive(bar);                       // (the tail is read by the decoding warps themselves)
             } else {
                 const int blocks = min(2, p.nb - 2 * i);
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(blocks * BLK * D * 2) : "memory");
                 const uint8_t *f = value ? p.v8 : p.k8, *m = value ? p.vm : p.km, *l = value ? p.vl : p.kl;
                 long long at = (value ? s.bh * p.L + i * TILE : (s.bh * p.nmb + 2 * i) * BLK) * D;
-                uint32_t to = base + L::RING_AT + buf * L::TILE_BYTES;
+                uint32_t to = ring_at + buf * L::TILE_BYTES;
                 for (int b = 0; b < blocks; ++b, at += BLK * D, to += D * 128) {
                     bulk(to, f + at, D * BLK, bar);
                     bulk(to + D * 64, m + at / 2, D * BLK / 2, bar);
                     bulk(to + D * 96, l + at / 2, D * BLK / 2, bar);
                 }
             }
-            if (++buf == L::RING) {
+            if (++buf == ring) {
                 buf = 0;
                 ++turn;
             }
@@ -234,10 +234,9 @@ __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t base, uint
 
 // Four warps decode a region: U = D / 32 pieces of 16 elements a lane, quarter lane % 4 of rows of 64 elements.  (Of V
 // and the tail, neighbouring rows in different halves: neither the loads of the bytes nor the stores of the operands meet in a bank.)
-template <int D>
-__device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t base, uint32_t bars, volatile int* dead, volatile int* odd,
-                                            long long first, long long last, int warp, int lane) {
-    using L = Plan<D>;
+template <class L, int D, bool KEYS>
+__device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t ring_at, uint32_t ring, uint32_t bars, volatile int* dead,
+                                            volatile int* odd, long long first, long long last, bool has_tail, int warp, int lane) {
     constexpr int U = D / 32;
     const int qd = lane & 3, k = (warp & 3) * 8 + (lane >> 2), side = (lane >> 2 ^ lane >> 3) & 1;
     uint32_t buf = 0, turn = 0;
@@ -247,11 +246,11 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t base, ui
         s.at(p, tile, last);
         tile += s.c;
 #pragma unroll 1
-        for (int q = 0; q < 2 * s.c; ++q) {
-            bool value;
-            const int i = s.t0 + tile_of(q, s.c, 3 - p.groups, value);
-            const bool tail = i == p.tiles - 1, by_channel = !value && !tail;
-            const uint32_t region = base + L::RING_AT + buf * L::TILE_BYTES + (warp >> 2) * D * 128;
+        for (int q = 0; q < (KEYS ? 1 : 2) * s.c; ++q) {
+            bool value = false;
+            const int i = s.t0 + (KEYS ? q : tile_of(q, s.c, 3 - p.groups, value));
+            const bool tail = has_tail && i == p.tiles - 1, by_channel = !value && !tail;
+            const uint32_t region = ring_at + buf * L::TILE_BYTES + (warp >> 2) * D * 128;
             // piece u: row (u or u / 2) * 32 + k, half side ^ (u & 1) where rows have two
             const bool halves = D == 128 && !by_channel;
             const int kr = value && !tail ? swapped(k) : k;        // (V's tokens are stored in the order of the scores' columns)
@@ -305,7 +304,7 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t base, ui
                         for (int j = 0; j < 8; ++j) w[u][j] = finite_halves(w[u][j], mine);
                     }
                 }
-                if (mine) odd[index % L::SEGMENTS] = index + 1;
+                if (!KEYS && mine) odd[index % L::SEGMENTS] = index + 1;
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -326,7 +325,7 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t base, ui
             fence_shared();
             __syncwarp();
             if (lane == 0) bar_arrive(bars + 8 * (L::FULL + buf));
-            if (++buf == L::RING) {
+            if (++buf == ring) {
                 buf = 0;
                 ++turn;
             }
@@ -692,15 +691,189 @@ __global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p)
     if (warp < SOFT) {
         softmax_role<D>(p, smem, base, bars, tmem, dead, odd, first, last, warp, lane);
     } else if (warp < SOFT + DECODE) {
-        decode_role<D>(p, base, bars, dead, odd, first, last, warp - SOFT, lane);
+        decode_role<L, D, false>(p, base + L::RING_AT, L::RING, bars, dead, odd, first, last, true, warp - SOFT, lane);
     } else if (lane == 0) {
         if (warp == SOFT + DECODE) product_role<D>(p, base, bars, tmem, dead, first, last);
-        else copy_role<D>(p, base, bars, dead, first, last);
+        else copy_role<L, D, false>(p, base + L::RING_AT, L::RING, bars, dead, first, last, true);
     }
     __syncwarp();
     __syncthreads();
     if (*dead) {
         // (never expected) products may still run: time for them to end before their memory is released
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+        __syncthreads();
+    }
+    fence_after();
+    if (warp == SOFT + DECODE)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+}
+
+// ---------------------------------------------------------------- weights
+// weights[t] += sum over the rows of exp(s_t - lse): keys alone, and the product the other way round: S^T = K Q^T, a tile's 128 tokens
+// by up to 256 rows, so that a thread has a token and adds its rows up by itself.  Copy and decode as above, the ring as deep as
+// the queries leave room for; two score slots, the tiles in turn.
+template <int D>
+struct KeysPlan {
+    static constexpr int RING = D == 128 ? 6 : 8, TILE_BYTES = TILE * D * 2, SEGMENTS = 8;
+    static constexpr int RAW = 0, FULL = RING, EMPTY = 2 * RING, S_FULL = 3 * RING, S_FREE = S_FULL + 2, Q_FULL = S_FREE + 2, BARS = Q_FULL + 1;
+    static constexpr int ROWS = 512, OFF_AT = 512, Q_AT = OFF_AT + ROWS * 4 + 512;          // barriers and words; -lse of the rows; queries
+    static_assert(8 * BARS + 8 + ROWS / 32 * 4 <= OFF_AT && Q_AT % 1024 == 0, "layout");
+    static __host__ __device__ int padded(int rows) { return (rows + 15) & ~15; }
+    static __host__ __device__ int ring_at(int rows) { return (Q_AT + padded(rows) * D * 2 + 1023) & ~1023; }
+    static __host__ __device__ int depth(int rows) {
+        const int fit = (232448 - 1024 - ring_at(rows)) / TILE_BYTES;
+        return fit < RING ? fit : RING;
+    }
+    static __host__ __device__ int bytes(int rows) { return 1024 + ring_at(rows) + depth(rows) * TILE_BYTES; }
+};
+
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const TreeArgs p, float* __restrict__ weights, int row0, int rows) {
+    using L = KeysPlan<D>;
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    const uint32_t base = smem_u32(smem), bars = base;
+    uint32_t* slot_tmem = reinterpret_cast<uint32_t*>(smem + 8 * L::BARS);
+    volatile int* dead = reinterpret_cast<volatile int*>(slot_tmem + 1);
+    uint32_t* absent = slot_tmem + 2;              // a bit per row: it sees nothing, or there is none
+    float* off = reinterpret_cast<float*>(smem + L::OFF_AT);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = L::depth(rows), ring_at = base + L::ring_at(rows), q_half = L::padded(rows) * 128;
+    const int groups = (rows + 255) >> 8;
+    const bool has_tail = p.rest > 0;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::RING; ++i) {
+            bar_init(bars + 8 * (L::RAW + i), 1);
+            bar_init(bars + 8 * (L::FULL + i), DECODE);
+            bar_init(bars + 8 * (L::EMPTY + i), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(bars + 8 * (L::S_FULL + i), 1);
+            bar_init(bars + 8 * (L::S_FREE + i), SOFT / 2);
+        }
+        bar_init(bars + 8 * L::Q_FULL, SOFT);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        *dead = 0;
+    }
+    pdl_enter();
+    __syncwarp();
+    if (warp == SOFT + DECODE) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(slot_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(slot_tmem);
+    const long long w = blockIdx.x, first = w * p.total / p.nw, last = (w + 1) * p.total / p.nw;
+    if (warp < SOFT) {
+        const int slot = warp >> 2, idx = (warp & 3) * 32 + lane;
+        const uint32_t s_at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + slot * 256;
+        uint32_t done = 0;
+        for (long long tile = first; tile < last;) {
+            Segment s;
+            s.at(p, tile, last);
+            tile += s.c;
+            soft_sync();                               // (all products with the queries before are over: their scores have been read)
+            for (int i = threadIdx.x; i < L::padded(rows) * (D / 8); i += 32 * SOFT) {
+                const int r = i / (D / 8), c = i % (D / 8);
+                const uint4 x = r < rows ? __ldg(reinterpret_cast<const uint4*>(p.q + row_of(p, s.b, s.h, row0 + r) * D) + c) : make_uint4(0, 0, 0, 0);
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(base + L::Q_AT + (c >> 3) * q_half + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                             "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+            }
+            for (int r = warp * 32; r < L::ROWS; r += 32 * SOFT) {
+                const float x = r + lane < rows ? p.lse[row_of(p, s.b, s.h, row0 + r + lane)] : -INFINITY;
+                const uint32_t none = __ballot_sync(0xFFFFFFFFu, x == -INFINITY);
+                off[r + lane] = x == -INFINITY ? x : -x;
+                if (lane == 0) absent[r >> 5] = none;
+            }
+            fence_shared();
+            soft_sync();                               // (`off` is everybody's)
+            if (lane == 0) bar_arrive(bars + 8 * L::Q_FULL);
+            for (int j = slot; j < s.c; j += 2) {
+                const int i = s.t0 + j;
+                const bool tail = has_tail && i == p.tiles - 1;
+                const int at = tail ? p.nb * BLK : i * TILE, tok = tail ? idx : swapped(idx);
+                const int count = tail ? p.rest : min(TILE, p.nb * BLK - at);
+                float add = 0.f, sum[4] = {0.f, 0.f, 0.f, 0.f};
+                if (p.mask && tok < count) add = __half2float(p.mask[s.b * p.mask_stride + at + tok]);
+                const bool gone = tok >= count || add == -INFINITY;
+                add *= LOG2E;
+                for (int g = 0; g < groups; ++g, ++done) {
+                    bar_wait(bars + 8 * (L::S_FULL + slot), done & 1, dead);
+                    __syncwarp();
+                    fence_after();
+                    const int n = min(256, rows - 256 * g);
+                    if (!__all_sync(0xFFFFFFFFu, gone)) {
+#pragma unroll 1
+                        for (int c = 0; c < n; c += 32) {
+                            uint32_t v[32];
+                            __syncwarp();
+                            tmem_ld(v, s_at + c);
+                            const float4* o4 = reinterpret_cast<const float4*>(off + 256 * g + c);
+                            if (const uint32_t none = absent[8 * g + (c >> 5)]) {
+                                // (no weight from these, whatever their scores are: 0 - inf)
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) v[e] = none >> e & 1 ? 0 : v[e];
+                            }
+                            // exp(score - lse), one rounding of the small difference: scores of 25 are half of 2e-6 off themselves
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float4 o = o4[e];
+                                sum[0] += ex2(fmaf(fmaf(__uint_as_float(v[4 * e]), p.scale, o.x), LOG2E, add));
+                                sum[1] += ex2(fmaf(fmaf(__uint_as_float(v[4 * e + 1]), p.scale, o.y), LOG2E, add));
+                                sum[2] += ex2(fmaf(fmaf(__uint_as_float(v[4 * e + 2]), p.scale, o.z), LOG2E, add));
+                                sum[3] += ex2(fmaf(fmaf(__uint_as_float(v[4 * e + 3]), p.scale, o.w), LOG2E, add));
+                            }
+                        }
+                    }
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(bars + 8 * (L::S_FREE + slot));
+                }
+                if (!gone) {
+                    float x = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    if (*dead) x = __int_as_float(0x7FC00000);
+                    weights[s.bh * p.L + at + tok] += x;
+                }
+            }
+        }
+    } else if (warp < SOFT + DECODE) {
+        decode_role<L, D, true>(p, ring_at, ring, bars, dead, nullptr, first, last, has_tail, warp - SOFT, lane);
+    } else if (lane == 0 && warp == SOFT + DECODE) {
+        uint32_t passed = 0, items[2] = {0, 0}, seg = 0;
+        for (long long tile = first; tile < last; ++seg) {
+            Segment s;
+            s.at(p, tile, last);
+            tile += s.c;
+            bar_wait(bars + 8 * L::Q_FULL, seg & 1, dead);
+            // a tile's groups go to its slot one after the other; the slots alternate
+            const int steps = 2 * groups * ((s.c + 1) >> 1);
+            for (int t = 0; t < steps; ++t) {
+                const int slot = t & 1, g = (t >> 1) % groups, j = 2 * ((t >> 1) / groups) + slot;
+                if (j >= s.c) continue;
+                const bool tail = has_tail && s.t0 + j == p.tiles - 1;
+                const uint32_t pos = passed + j, turn = pos / ring, buf = pos - turn * ring, k = ring_at + buf * L::TILE_BYTES;
+                bar_wait(bars + 8 * (L::FULL + buf), turn & 1, dead);
+                bar_wait(bars + 8 * (L::S_FREE + slot), (items[slot] & 1) ^ 1, dead);
+                fence_after();
+                const uint32_t idesc = instruction(min(256, L::padded(rows) - 256 * g), false, !tail);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    mma_ss(tmem + slot * 256, tail ? operand(k + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024) : operand(k + kk * 2048, D * 128, 1024),
+                           operand(base + L::Q_AT + g * 32768 + (kk >> 2) * q_half + (kk & 3) * 32, 16, 1024), idesc, kk > 0);
+                commit(bars + 8 * (L::S_FULL + slot));
+                if (g == groups - 1) commit(bars + 8 * (L::EMPTY + buf));
+                ++items[slot];
+            }
+            passed += s.c;
+        }
+    } else if (lane == 0) {
+        copy_role<L, D, true>(p, ring_at, ring, bars, dead, first, last, has_tail);
+    }
+    __syncwarp();
+    __syncthreads();
+    if (*dead) {
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
         __syncthreads();
     }
@@ -719,6 +892,19 @@ int launch_tree_wide(const TreeArgs& p, int D, int ctas, cudaStream_t st) {
     if (rc != AKV_OK) return rc;
     launch_chained(kernel, dim3(ctas), dim3(THREADS), (size_t)bytes, st, p);
     return AKV_OK;
+}
+
+int launch_weights_wide(const TreeArgs& p, int D, int ctas, float* weights, cudaStream_t st) {
+    auto kernel = D == 128 ? weights_wide_kernel<128> : weights_wide_kernel<64>;
+    int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448), "tree_weights shared memory");
+    // (more rows than the queries' place holds: one launch after the other)
+    for (int row0 = 0; rc == AKV_OK && row0 < p.T * p.G; row0 += KeysPlan<128>::ROWS) {
+        const int left = p.T * p.G - row0, rows = left < KeysPlan<128>::ROWS ? left : KeysPlan<128>::ROWS;
+        launch_chained(kernel, dim3(ctas), dim3(THREADS), (size_t)(D == 128 ? KeysPlan<128>::bytes(rows) : KeysPlan<64>::bytes(rows)), st, p,
+                       weights, row0, rows);
+        rc = cuda_status(cudaGetLastError(), "tree_weights launch");
+    }
+    return rc;
 }
 
 }  // namespace akv

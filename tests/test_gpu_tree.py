@@ -185,7 +185,9 @@ def test_commit_clamps_and_repeats(akv_lib):
 
 
 @pytest.mark.parametrize("B,n,Hq,H,D,T", [(1, 1, 2, 2, 128, 1), (2, 64, 4, 1, 128, 2), (1, 127, 8, 2, 64, 5), (2, 193, 6, 2, 128, 17),
-                                          (1, 2000, 8, 1, 128, 32), (3, 700, 4, 4, 128, 1)])
+                                          (1, 2000, 8, 1, 128, 32), (3, 700, 4, 4, 128, 1),
+                                          (1, 300, 8, 1, 128, 64), (1, 260, 16, 1, 64, 40), (1, 130, 12, 1, 128, 64), (2, 1290, 40, 2, 64, 13),
+                                          (1, 450, 5, 1, 128, 55), (1, 5000, 1, 1, 128, 1)])
 @pytest.mark.parametrize("masked", [False, True])
 def test_weights(akv_lib, B, n, Hq, H, D, T, masked):
     x = make(B, n, Hq, H, D, T, seed=n)
@@ -210,7 +212,12 @@ def test_weights(akv_lib, B, n, Hq, H, D, T, masked):
     assert bool(((got[..., :n].double() - want).abs() <= bound).all())
     assert not bool(got[..., n:].any())
     twice = x.layer.tree_weights(x.q, lse, mask=wide)
-    assert torch.equal(twice, got * 2), "sums go on; doubling is exact"
+    if rows <= 512:
+        assert torch.equal(twice, got * 2), "sums go on; doubling is exact"
+    else:
+        # 512 rows are added at a time: got = fl(a + b), twice = fl(fl(got + a) + b).  Three roundings of at most 2^-24 of sums of
+        # numbers >= 0 that are at most `twice` (and the rounding itself): under 2^-22 of it
+        assert rows <= 1024 and bool(((twice - got * 2).abs() <= twice * 2.0 ** -22).all())
 
 
 def test_replayed_and_on_a_side_stream(akv_lib):
