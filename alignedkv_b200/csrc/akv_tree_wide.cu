@@ -58,7 +58,8 @@ __device__ __forceinline__ void bar_arrive(uint32_t a) {
 }
 __device__ __forceinline__ bool bar_try(uint32_t a, uint32_t parity) {
     uint32_t ok;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+    // (a waiting thread sleeps up to 20 us at a time: its polls would take issue slots from those that work)
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\nselp.u32 %0, 1, 0, p;\n}\n"
                  : "=r"(ok) : "r"(a), "r"(parity) : "memory");
     return ok != 0;
 }
@@ -89,19 +90,21 @@ __device__ __forceinline__ void fence_shared() { asm volatile("fence.proxy.async
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
 }
-// D (fp32, tensor memory) = A B (+ D): A, B fp16 in shared memory by descriptor, or A in tensor memory.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+// Shared-memory operand with 128-byte swizzle, as the two words of its descriptor: the upper is the same for all (groups of eight - rows
+// if K-major, of the sum's indices if MN-major - lie 1024 bytes apart), the lower has the address and, MN-major, `lead`: the bytes
+// between pieces of 64 elements.
+constexpr uint32_t OPERAND_HI = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t operand(uint32_t at, uint32_t lead) { return at >> 4 | (lead >> 4) << 16; }
+// D (fp32, tensor memory) = A B (+ D): A, B fp16 in shared memory, or A in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 x, y;\nmov.b64 x, {%1, %5};\nmov.b64 y, {%2, %5};\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(OPERAND_HI) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
-}
-// Shared-memory operand with 128-byte swizzle.  MN-major: `lead` = bytes between pieces of 64 elements, `stride` = between groups of
-// eight of the sum's indices.  K-major: stride = between groups of eight rows (lead unused).
-__device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t lead, uint32_t stride) {
-    return (uint64_t)(at >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 y;\nmov.b64 y, {%2, %5};\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(OPERAND_HI) : "memory");
 }
 // fp16 x fp16 -> fp32, 128 rows, n columns; K-major, or MN-major if so.
 __device__ __forceinline__ constexpr uint32_t instruction(int n, bool b_mn, bool a_mn = false) {
@@ -169,11 +172,6 @@ __device__ __forceinline__ int tile_of(int q, int c, int ahead, bool& value) {
     value = r >= pairs || !(r & 1);
     return r >= pairs ? (c - ahead) + (r - pairs) : value ? r >> 1 : (r >> 1) + ahead;
 }
-__device__ __forceinline__ int place_of(int i, bool value, int c, int ahead) {
-    ahead = min(ahead, c);
-    if (!value) return i < ahead ? i : ahead + 2 * (i - ahead) + 1;
-    return i < c - ahead ? ahead + 2 * i : ahead + 2 * (c - ahead) + i - (c - ahead);
-}
 
 // ---------------------------------------------------------------- decode
 // Eight elements from their high bytes and nibbles, in the order in which two permutes a pair suffice: 0 2 1 3, 4 6 5 7.  Of K that is
@@ -199,7 +197,7 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w, bool& odd) {
 // L: the kernel's plan; KEYS: keys alone, tile after tile.  `has_tail`: whether the units' last tiles are tails.
 template <class L, int D, bool KEYS>
 __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t ring_at, uint32_t ring, uint32_t bars, volatile int* dead,
-                                          long long first, long long last, bool has_tail) {
+                                          long long first, long long last, bool has_tail, bool leader) {
     uint32_t buf = 0, turn = 0;
     for (long long tile = first; tile < last;) {
         Segment s;
@@ -211,19 +209,25 @@ __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t ring_at, u
             const uint32_t bar = bars + 8 * (L::RAW + buf);
             bar_wait(bars + 8 * (L::EMPTY + buf), (turn & 1) ^ 1, dead);
             if (has_tail && i == p.tiles - 1) {
-                bar_arrive(bar);                       // (the tail is read by the decoding warps themselves)
+                if (leader) bar_arrive(bar);           // (the tail is read by the decoding warps themselves)
             } else {
                 const int blocks = min(2, p.nb - 2 * i);
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(blocks * BLK * D * 2) : "memory");
                 const uint8_t *f = value ? p.v8 : p.k8, *m = value ? p.vm : p.km, *l = value ? p.vl : p.kl;
-                long long at = (value ? s.bh * p.L + i * TILE : (s.bh * p.nmb + 2 * i) * BLK) * D;
-                uint32_t to = ring_at + buf * L::TILE_BYTES;
-                for (int b = 0; b < blocks; ++b, at += BLK * D, to += D * 128) {
+                const long long at = (value ? s.bh * p.L + i * TILE : (s.bh * p.nmb + 2 * i) * BLK) * D;
+                const uint32_t to = ring_at + buf * L::TILE_BYTES;
+                if (leader) {
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(blocks * BLK * D * 2) : "memory");
                     bulk(to, f + at, D * BLK, bar);
                     bulk(to + D * 64, m + at / 2, D * BLK / 2, bar);
                     bulk(to + D * 96, l + at / 2, D * BLK / 2, bar);
+                    if (blocks == 2) {
+                        bulk(to + D * 128, f + at + D * BLK, D * BLK, bar);
+                        bulk(to + D * 192, m + (at + D * BLK) / 2, D * BLK / 2, bar);
+                        bulk(to + D * 224, l + (at + D * BLK) / 2, D * BLK / 2, bar);
+                    }
                 }
             }
+            __syncwarp();
             if (++buf == ring) {
                 buf = 0;
                 ++turn;
@@ -232,169 +236,216 @@ __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t ring_at, u
     }
 }
 
-// Four warps decode a region: U = D / 32 pieces of 16 elements a lane, quarter lane % 4 of rows of 64 elements.  (Of V
-// and the tail, neighbouring rows in different halves: neither the loads of the bytes nor the stores of the operands meet in a bank.)
+// A thread's share of a tile: of one region (four warps each) U = D / 32 pieces of 16 elements, quarter lane % 4 of rows of 64.  Where
+// pieces lie, as bytes and as operand: e0, e1, e0 + t, e1 + t and f0, f1, f0 + 4096, f1 + 4096, whatever the tile is - K: channels k,
+// 64 + k, 32 + k, 96 + k (k = 8 warp + lane / 4 of 32); V: tokens k, k, 32 + k, 32 + k and both their channel halves, of neighbouring
+// lanes different ones (neither the loads of the bytes nor the stores of the operands meet in a bank); D = 64: rows k, 32 + k.
+template <int D>
+struct Share {
+    static constexpr int U = D / 32;
+    uint32_t w[U][8];
+    uint32_t f0, f1;            // from the ring slot
+    bool bytes, value;          // not yet fp16; V
+    int index;                  // segment
+
+    __device__ __forceinline__ void load(const TreeArgs& p, const Segment& s, int i, bool of_values, bool tail, uint32_t slot, int warp,
+                                         int lane) {
+        const int region = warp >> 2, k = (warp & 3) * 8 + (lane >> 2), qd = lane & 3, x = ((2 * qd) ^ (k & 7)) << 4;
+        const uint32_t side = D == 128 ? (lane >> 2 ^ lane >> 3) & 1 : 0;
+        value = of_values;
+        bytes = !tail;
+        const int kr = value && !tail ? swapped(k) : k;            // (V's tokens are stored in the order of the scores' columns)
+        const bool by_half = D == 128 && (value || tail);
+        auto row = [&](int u) { return D == 64 ? u * 32 + kr : by_half ? (u >> 1) * 32 + kr : (u & 1) * 64 + (u >> 1) * 32 + kr; };
+        f0 = region * D * 128 + k * 128 + x + side * 8192 * by_half;
+        f1 = region * D * 128 + k * 128 + x + (D == 64 ? 4096 : by_half ? (side ^ 1) * 8192 : 8192);
+        if (tail && !value) {
+            f0 = region * 8192 + k * 128 + x + side * 16384;
+            f1 = region * 8192 + k * 128 + x + (D == 64 ? 4096 : (side ^ 1) * 16384);
+        }
+        if (!tail) {
+            const uint32_t at = slot + region * D * 128;
+            const uint32_t e0 = by_half ? kr * 128 + side * 64 + qd * 16 : kr * 64 + qd * 16;
+            const uint32_t e1 = by_half ? e0 ^ 64 : D == 64 ? e0 + 2048 : e0 + 4096, t = by_half ? 4096 : 2048;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t e = (u & 1 ? e1 : e0) + (u >> 1) * t;
+                const uint4 h = lds128(at + e);
+                const uint2 m = lds64(at + D * 64 + e / 2), l = lds64(at + D * 96 + e / 2);
+                w[u][0] = h.x; w[u][1] = h.y; w[u][2] = h.z; w[u][3] = h.w;
+                w[u][4] = m.x; w[u][5] = m.y; w[u][6] = l.x; w[u][7] = l.y;
+            }
+            const int some = p.nb * BLK - i * TILE;
+            if (some < TILE || (value && p.mask)) {
+                // (a token that does not exist or is masked away counts as zero, whatever there is: 0 * NaN would be NaN)
+                const uint16_t* mask = value && p.mask ? reinterpret_cast<const uint16_t*>(p.mask) + s.b * p.mask_stride + i * TILE : nullptr;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int tok = region * BLK + (value ? row(u) : 0);
+                    if (tok >= some || (mask && mask[tok] == 0xFC00u)) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) w[u][j] = 0;
+                    }
+                }
+            }
+        } else {
+            const __half *rest = value ? p.restv : p.restk, *drafted = value ? p.vd : p.kd;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int y = region * BLK + row(u), d = y - p.rest;
+                uint4 a = make_uint4(0, 0, 0, 0), b = a;
+                if (y < p.tail) {
+                    const __half* src = d < 0 ? rest + ((s.b * BLK + y) * p.H + s.h) * D : drafted + ((s.b * p.T + d) * p.H + s.h) * D;
+                    const uint4* from = reinterpret_cast<const uint4*>(src + (side ^ (u & 1)) * 64 * (D == 128) + qd * 16);
+                    a = __ldg(from);
+                    b = __ldg(from + 1);
+                }
+                if (value) {
+                    a = reorder8(a);
+                    b = reorder8(b);
+                }
+                w[u][0] = a.x; w[u][1] = a.y; w[u][2] = a.z; w[u][3] = a.w;
+                w[u][4] = b.x; w[u][5] = b.y; w[u][6] = b.z; w[u][7] = b.w;
+            }
+        }
+    }
+    // Whether the tail's values hold one that is not finite: zeros in the operand, added where a row sees them.
+    __device__ __forceinline__ bool store(uint32_t slot) {
+        bool odd = false;
+        if (!bytes && value) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[u][j] = finite_halves(w[u][j], odd);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            uint4 x = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]), y = make_uint4(w[u][4], w[u][5], w[u][6], w[u][7]);
+            if (bytes) {
+                const uint4 h = x, n = y;
+                x = halves8(h.x, h.y, n.x, n.z);
+                y = halves8(h.z, h.w, n.y, n.w);
+            }
+            const uint32_t at = slot + (u & 1 ? f1 : f0) + (u >> 1) * 4096;
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at ^ 16), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+        }
+        return odd;
+    }
+};
+
+// The next tile's bytes are on their way to registers while this one's are decoded; the barrier of the region's four warps between a
+// tile's loads and its stores in the same place finds them there.
 template <class L, int D, bool KEYS>
 __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t ring_at, uint32_t ring, uint32_t bars, volatile int* dead,
                                             volatile int* odd, long long first, long long last, bool has_tail, int warp, int lane) {
-    constexpr int U = D / 32;
-    const int qd = lane & 3, k = (warp & 3) * 8 + (lane >> 2), side = (lane >> 2 ^ lane >> 3) & 1;
-    uint32_t buf = 0, turn = 0;
-    int index = 0;
-    for (long long tile = first; tile < last; ++index) {
-        Segment s;
-        s.at(p, tile, last);
-        tile += s.c;
-#pragma unroll 1
-        for (int q = 0; q < (KEYS ? 1 : 2) * s.c; ++q) {
-            bool value = false;
-            const int i = s.t0 + (KEYS ? q : tile_of(q, s.c, 3 - p.groups, value));
-            const bool tail = has_tail && i == p.tiles - 1, by_channel = !value && !tail;
-            const uint32_t region = ring_at + buf * L::TILE_BYTES + (warp >> 2) * D * 128;
-            // piece u: row (u or u / 2) * 32 + k, half side ^ (u & 1) where rows have two
-            const bool halves = D == 128 && !by_channel;
-            const int kr = value && !tail ? swapped(k) : k;        // (V's tokens are stored in the order of the scores' columns)
-            auto row = [&](int u) { return (halves ? u >> 1 : u) * 32 + kr; };
-            auto half = [&](int u) { return halves ? side ^ (u & 1) : 0; };
-            bar_wait(bars + 8 * (L::RAW + buf), turn & 1, dead);
-            uint32_t w[U][8];
-            if (!tail) {
-                const int pitch = by_channel ? 64 : D;
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int o = row(u) * pitch + half(u) * 64 + qd * 16;
-                    const uint4 x = lds128(region + o);
-                    const uint2 m = lds64(region + D * 64 + o / 2), l = lds64(region + D * 96 + o / 2);
-                    w[u][0] = x.x; w[u][1] = x.y; w[u][2] = x.z; w[u][3] = x.w;
-                    w[u][4] = m.x; w[u][5] = m.y; w[u][6] = l.x; w[u][7] = l.y;
-                }
-                const int some = p.nb * BLK - i * TILE;
-                if (some < TILE || (value && p.mask)) {
-                    // (a token that does not exist or is masked away counts as zero, whatever there is: 0 * NaN would be NaN)
-                    const uint16_t* mask = value && p.mask ? reinterpret_cast<const uint16_t*>(p.mask) + s.b * p.mask_stride + i * TILE : nullptr;
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const int tok = (warp >> 2) * BLK + (by_channel ? 0 : row(u));
-                        if (tok >= some || (mask && mask[tok] == 0xFC00u)) {
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) w[u][j] = 0;
-                        }
-                    }
-                }
-                __syncwarp();                          // the region's bytes are in registers
-                asm volatile("bar.sync %0, 128;\n" ::"r"(2 + (warp >> 2)) : "memory");
-            } else {
-                bool mine = false;
-                const __half *rest = value ? p.restv : p.restk, *drafted = value ? p.vd : p.kd;
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int x = (warp >> 2) * BLK + row(u), d = x - p.rest;
-                    uint4 a = make_uint4(0, 0, 0, 0), b = a;
-                    if (x < p.tail) {
-                        const __half* src = d < 0 ? rest + ((s.b * BLK + x) * p.H + s.h) * D : drafted + ((s.b * p.T + d) * p.H + s.h) * D;
-                        const uint4* from = reinterpret_cast<const uint4*>(src + half(u) * 64 + qd * 16);
-                        a = __ldg(from);
-                        b = __ldg(from + 1);
-                    }
-                    w[u][0] = a.x; w[u][1] = a.y; w[u][2] = a.z; w[u][3] = a.w;
-                    w[u][4] = b.x; w[u][5] = b.y; w[u][6] = b.z; w[u][7] = b.w;
-                    // (values that are not finite: zeros here, added where a row sees them)
-                    if (value) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) w[u][j] = finite_halves(w[u][j], mine);
-                    }
-                }
-                if (!KEYS && mine) odd[index % L::SEGMENTS] = index + 1;
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                uint4 x = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]), y = make_uint4(w[u][4], w[u][5], w[u][6], w[u][7]);
-                if (!tail) {
-                    const uint4 h = x, n = y;
-                    x = halves8(h.x, h.y, n.x, n.z);
-                    y = halves8(h.z, h.w, n.y, n.w);
-                } else if (value) {
-                    x = reorder8(x);
-                    y = reorder8(y);
-                }
-                const uint32_t at = (tail && !value ? region + half(u) * 16384 - (warp >> 2) * (D - 64) * 128 : region + half(u) * 8192) +
-                                    (row(u) - kr + k) * 128 + (((2 * qd) ^ (k & 7)) << 4);
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at ^ 16), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
-            }
-            fence_shared();
-            __syncwarp();
-            if (lane == 0) bar_arrive(bars + 8 * (L::FULL + buf));
-            if (++buf == ring) {
-                buf = 0;
-                ++turn;
-            }
+    uint32_t buf = 0, turn = 0;          // of the tile that is loaded next
+    int q = 0, index = 0;
+    long long tile = first;
+    Segment s;
+    s.at(p, tile, last);
+    const int count = (KEYS ? 1 : 2) * (int)(last - first);
+    Share<D> a;
+    auto load = [&](Share<D>& x) {
+        bool value = false;
+        const int i = s.t0 + (KEYS ? q : tile_of(q, s.c, 3 - p.groups, value));
+        bar_wait(bars + 8 * (L::RAW + buf), turn & 1, dead);
+        x.index = index;
+        x.load(p, s, i, value, has_tail && i == p.tiles - 1, ring_at + buf * L::TILE_BYTES, warp, lane);
+        if (++buf == ring) {
+            buf = 0;
+            ++turn;
         }
+        if (++q == (KEYS ? 1 : 2) * s.c) {
+            q = 0;
+            ++index;
+            tile += s.c;
+            if (tile < last) s.at(p, tile, last);
+        }
+    };
+    auto store = [&](Share<D>& x, uint32_t slot) {
+        if (x.store(ring_at + slot * L::TILE_BYTES) && !KEYS) odd[x.index % L::SEGMENTS] = x.index + 1;
+        fence_shared();
+        __syncwarp();
+        if (lane == 0) bar_arrive(bars + 8 * (L::FULL + slot));
+    };
+    auto loaded = [&]() {
+        __syncwarp();
+        asm volatile("bar.sync %0, 128;\n" ::"r"(2 + (warp >> 2)) : "memory");
+    };
+#pragma unroll 1
+    for (int n = 0; n < count; ++n) {
+        const uint32_t slot = buf;
+        load(a);
+        loaded();
+        store(a, slot);
     }
 }
 
 // ---------------------------------------------------------------- products
+// The whole warp goes through this, one lane issues: addresses and descriptors are then the same for all lanes and come from uniform
+// registers (by one lane alone a product took about 100 cycles to issue, and the issuing thread bound the kernel).
 template <int D>
 __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, uint32_t bars, uint32_t tmem, volatile int* dead,
-                                             long long first, long long last) {
-    const int ahead = 3 - p.groups;
+                                             long long first, long long last, bool leader) {
     using L = Plan<D>;
-    uint32_t passed = 0;                           // operand tiles of the segments before
-    uint32_t items[2] = {0, 0}, seg = 0;           // of each slot so far
+    uint32_t buf = 0, turn = 0, k_at = 0, k_buf = 0, v_at = 0, v_buf = 0;
+    uint32_t items0 = 0, items1 = 0, seg = 0;          // of each slot so far
+    const bool one = p.groups == 1;
+    // the next operand tile: they come in the order in which they are first used
+    auto take = [&](uint32_t& at, uint32_t& of) {
+        bar_wait(bars + 8 * (L::FULL + buf), turn & 1, dead);
+        at = base + L::RING_AT + buf * L::TILE_BYTES;
+        of = buf;
+        if (++buf == L::RING) {
+            buf = 0;
+            ++turn;
+        }
+    };
     for (long long tile = first; tile < last; ++seg) {
         Segment s;
         s.at(p, tile, last);
         tile += s.c;
-        bar_wait(bars + 8 * Plan<D>::Q_FULL, seg & 1, dead);
-        fence_after();
-        const int n_items = p.groups * s.c;
-        auto operand_at = [&](int n, bool value, int& buf) {
-            const uint32_t pos = passed + place_of(p.groups == 1 ? n : n >> 1, value, s.c, ahead), turn = pos / L::RING;
-            buf = (int)(pos - turn * L::RING);
-            bar_wait(bars + 8 * (L::FULL + buf), turn & 1, dead);
-            return base + L::RING_AT + buf * L::TILE_BYTES;
-        };
-        auto scores = [&](int n) {
-            const int slot = n & 1;
-            const bool tail = s.t0 + (p.groups == 1 ? n : n >> 1) == p.tiles - 1;
-            int buf;
-            const uint32_t k = operand_at(n, false, buf);
-            const uint32_t q = base + (p.groups == 2 && slot ? Plan<D>::Q2_AT : Plan<D>::Q_AT);
-            fence_after();
-            const uint32_t idesc = instruction(TILE, !tail);
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-                // 16 channels: of Q and of the tail's keys 32 bytes of rows of 64 (K-major), of K's planes 16 rows of 64 tokens
-                const uint32_t major = (kk >> 2) * 16384 + (kk & 3) * 32;
-                mma_ss(tmem + slot * TILE, operand(q + major, 16, 1024),
-                       tail ? operand(k + major, 16, 1024) : operand(k + kk * 2048, D * 128, 1024), idesc, kk > 0);
-            }
-            commit(bars + 8 * (Plan<D>::S_FULL + slot));
-            if (p.groups == 1 || slot) commit(bars + 8 * (Plan<D>::EMPTY + buf));
-        };
-        scores(0);
-        if (n_items > 1) scores(1);
-        for (int n = 0; n < n_items; ++n) {
-            const int slot = n & 1;
-            bar_wait(bars + 8 * (Plan<D>::P_FULL + slot), items[slot] & 1, dead);
-            int buf;
-            const uint32_t v = operand_at(n, true, buf);
-            fence_after();
-#pragma unroll
-            for (int kk = 0; kk < TILE / 16; ++kk)
-                mma_ts(tmem + 256 + slot * 128, tmem + slot * TILE + kk * 8, operand(v + (kk >> 2) * D * 128 + (kk & 3) * 2048, 8192, 1024), instruction(D, true),
-                       n >= 2 || kk > 0);
-            commit(bars + 8 * (Plan<D>::O_FULL + slot));
-            if (p.groups == 1 || slot) commit(bars + 8 * (Plan<D>::EMPTY + buf));
-            if (n + 2 < n_items) {
-                // (S takes P's place: the product that reads P has to be over)
-                bar_wait(bars + 8 * (Plan<D>::O_FULL + slot), items[slot] & 1, dead);
+        bar_wait(bars + 8 * L::Q_FULL, seg & 1, dead);
+        const int n_items = p.groups * s.c, tail_from = s.t0 + s.c == p.tiles ? n_items - p.groups : n_items;
+#pragma unroll 1
+        for (int n = -2; n < n_items; ++n) {           // output of item n, scores of item n + 2
+            const uint32_t slot = n & 1, parity = (slot ? items1 : items0) & 1;
+            if (n >= 0) {
+                bar_wait(bars + 8 * (L::P_FULL + slot), parity, dead);
+                if (one || !slot) take(v_at, v_buf);
                 fence_after();
-                scores(n + 2);
+                const uint32_t v = operand(v_at, 8192), o = tmem + 256 + slot * 128, pr = tmem + slot * TILE;
+                if (leader) {
+#pragma unroll
+                    for (int kk = 0; kk < TILE / 16; ++kk)
+                        mma_ts(o, pr + kk * 8, v + (kk >> 2) * (D * 128 >> 4) + (kk & 3) * (2048 >> 4), instruction(D, true), n >= 2 || kk > 0);
+                    commit(bars + 8 * (L::O_FULL + slot));
+                    if (one || slot) commit(bars + 8 * (L::EMPTY + v_buf));
+                }
+                __syncwarp();
+                if (slot) ++items1;
+                else ++items0;
             }
-            ++items[slot];
+            if (n + 2 >= n_items) continue;
+            if (one || !slot) take(k_at, k_buf);
+            // (S takes P's place: the product that reads P has to be over)
+            if (n >= 0) bar_wait(bars + 8 * (L::O_FULL + slot), parity, dead);
+            fence_after();
+            // 16 channels: of Q and of the tail's keys 32 bytes of rows of 64 (K-major), of K's planes 16 rows of 64 tokens
+            const bool tail = n + 2 >= tail_from;
+            const uint32_t q = operand(base + (!one && slot ? L::Q2_AT : L::Q_AT), 16), k = operand(k_at, tail ? 16 : D * 128);
+            const uint32_t near = tail ? 32 >> 4 : 2048 >> 4, far = tail ? 16384 >> 4 : 8192 >> 4;
+            const uint32_t idesc = tail ? instruction(TILE, false) : instruction(TILE, true), d = tmem + slot * TILE;
+            if (leader) {
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    mma_ss(d, q + (kk >> 2) * (16384 >> 4) + (kk & 3) * (32 >> 4), k + (kk >> 2) * far + (kk & 3) * near, idesc, kk > 0);
+                commit(bars + 8 * (L::S_FULL + slot));
+                if (one || slot) commit(bars + 8 * (L::EMPTY + k_buf));
+            }
+            __syncwarp();
         }
-        passed += 2 * s.c;
     }
 }
 
@@ -692,9 +743,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p)
         softmax_role<D>(p, smem, base, bars, tmem, dead, odd, first, last, warp, lane);
     } else if (warp < SOFT + DECODE) {
         decode_role<L, D, false>(p, base + L::RING_AT, L::RING, bars, dead, odd, first, last, true, warp - SOFT, lane);
-    } else if (lane == 0) {
-        if (warp == SOFT + DECODE) product_role<D>(p, base, bars, tmem, dead, first, last);
-        else copy_role<L, D, false>(p, base + L::RING_AT, L::RING, bars, dead, first, last, true);
+    } else if (warp == SOFT + DECODE) {
+        product_role<D>(p, base, bars, tmem, dead, first, last, lane == 0);
+    } else {
+        copy_role<L, D, false>(p, base + L::RING_AT, L::RING, bars, dead, first, last, true, lane == 0);
     }
     __syncwarp();
     __syncthreads();
@@ -840,36 +892,62 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const TreeArgs
         }
     } else if (warp < SOFT + DECODE) {
         decode_role<L, D, true>(p, ring_at, ring, bars, dead, nullptr, first, last, has_tail, warp - SOFT, lane);
-    } else if (lane == 0 && warp == SOFT + DECODE) {
-        uint32_t passed = 0, items[2] = {0, 0}, seg = 0;
+    } else if (warp == SOFT + DECODE) {
+        uint32_t buf = 0, turn = 0, items0 = 0, items1 = 0, seg = 0, k_at[2] = {0, 0}, k_buf[2] = {0, 0};
         for (long long tile = first; tile < last; ++seg) {
             Segment s;
             s.at(p, tile, last);
             tile += s.c;
             bar_wait(bars + 8 * L::Q_FULL, seg & 1, dead);
-            // a tile's groups go to its slot one after the other; the slots alternate
-            const int steps = 2 * groups * ((s.c + 1) >> 1);
-            for (int t = 0; t < steps; ++t) {
-                const int slot = t & 1, g = (t >> 1) % groups, j = 2 * ((t >> 1) / groups) + slot;
-                if (j >= s.c) continue;
-                const bool tail = has_tail && s.t0 + j == p.tiles - 1;
-                const uint32_t pos = passed + j, turn = pos / ring, buf = pos - turn * ring, k = ring_at + buf * L::TILE_BYTES;
-                bar_wait(bars + 8 * (L::FULL + buf), turn & 1, dead);
-                bar_wait(bars + 8 * (L::S_FREE + slot), (items[slot] & 1) ^ 1, dead);
-                fence_after();
-                const uint32_t idesc = instruction(min(256, L::padded(rows) - 256 * g), false, !tail);
+            // a pair of tiles, one for each slot, and of them the row groups one after the other
+#pragma unroll 1
+            for (int j0 = 0; j0 < s.c; j0 += 2) {
+                for (int g = 0; g < groups; ++g) {
+                    const uint32_t idesc_n = (uint32_t)(min(256, L::padded(rows) - 256 * g) >> 3) << 17;
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk)
-                    mma_ss(tmem + slot * 256, tail ? operand(k + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024) : operand(k + kk * 2048, D * 128, 1024),
-                           operand(base + L::Q_AT + g * 32768 + (kk >> 2) * q_half + (kk & 3) * 32, 16, 1024), idesc, kk > 0);
-                commit(bars + 8 * (L::S_FULL + slot));
-                if (g == groups - 1) commit(bars + 8 * (L::EMPTY + buf));
-                ++items[slot];
+                    for (int slot = 0; slot < 2; ++slot) {
+                        if (j0 + slot >= s.c) continue;
+                        if (g == 0) {
+                            bar_wait(bars + 8 * (L::FULL + buf), turn & 1, dead);
+                            k_at[slot] = ring_at + buf * L::TILE_BYTES;
+                            k_buf[slot] = buf;
+                            if (++buf == ring) {
+                                buf = 0;
+                                ++turn;
+                            }
+                        }
+                        bar_wait(bars + 8 * (L::S_FREE + slot), ((slot ? items1 : items0) & 1) ^ 1, dead);
+                        fence_after();
+                        const bool tail = has_tail && s.t0 + j0 + slot == p.tiles - 1;
+                        const uint32_t q = operand(base + L::Q_AT + g * 32768, 16), d = tmem + slot * 256, half = q_half >> 4;
+                        if (tail) {
+                            const uint32_t k = operand(k_at[slot], 16), idesc = instruction(0, false) | idesc_n;
+                            if (lane == 0) {
+#pragma unroll
+                                for (int kk = 0; kk < D / 16; ++kk)
+                                    mma_ss(d, k + (kk >> 2) * (16384 >> 4) + (kk & 3) * (32 >> 4), q + (kk >> 2) * half + (kk & 3) * (32 >> 4), idesc, kk > 0);
+                            }
+                        } else {
+                            const uint32_t k = operand(k_at[slot], D * 128), idesc = instruction(0, false, true) | idesc_n;
+                            if (lane == 0) {
+#pragma unroll
+                                for (int kk = 0; kk < D / 16; ++kk)
+                                    mma_ss(d, k + kk * (2048 >> 4), q + (kk >> 2) * half + (kk & 3) * (32 >> 4), idesc, kk > 0);
+                            }
+                        }
+                        if (lane == 0) {
+                            commit(bars + 8 * (L::S_FULL + slot));
+                            if (g == groups - 1) commit(bars + 8 * (L::EMPTY + k_buf[slot]));
+                        }
+                        __syncwarp();
+                        if (slot) ++items1;
+                        else ++items0;
+                    }
+                }
             }
-            passed += s.c;
         }
-    } else if (lane == 0) {
-        copy_role<L, D, true>(p, ring_at, ring, bars, dead, first, last, has_tail);
+    } else {
+        copy_role<L, D, true>(p, ring_at, ring, bars, dead, first, last, has_tail, lane == 0);
     }
     __syncwarp();
     __syncthreads();
