@@ -95,6 +95,12 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 // between pieces of 64 elements.
 constexpr uint32_t OPERAND_HI = 1024 >> 4 | 1u << 14 | 2u << 29;
 __device__ __forceinline__ uint32_t operand(uint32_t at, uint32_t lead) { return at >> 4 | (lead >> 4) << 16; }
+// True in one lane of a whole warp, in a form in which the compiler still knows the warp to be whole.
+__device__ __forceinline__ bool elect() {
+    uint32_t x;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(x));
+    return x != 0;
+}
 // D (fp32, tensor memory) = A B (+ D): A, B fp16 in shared memory, or A in tensor memory.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
     asm volatile("{\n.reg .pred p;\n.reg .b64 x, y;\nmov.b64 x, {%1, %5};\nmov.b64 y, {%2, %5};\nsetp.ne.b32 p, %4, 0;\n"
@@ -197,7 +203,7 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w, bool& odd) {
 // L: the kernel's plan; KEYS: keys alone, tile after tile.  `has_tail`: whether the units' last tiles are tails.
 template <class L, int D, bool KEYS>
 __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t ring_at, uint32_t ring, uint32_t bars, volatile int* dead,
-                                          long long first, long long last, bool has_tail, bool leader) {
+                                          long long first, long long last, bool has_tail) {
     uint32_t buf = 0, turn = 0;
     for (long long tile = first; tile < last;) {
         Segment s;
@@ -209,13 +215,13 @@ __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t ring_at, u
             const uint32_t bar = bars + 8 * (L::RAW + buf);
             bar_wait(bars + 8 * (L::EMPTY + buf), (turn & 1) ^ 1, dead);
             if (has_tail && i == p.tiles - 1) {
-                if (leader) bar_arrive(bar);           // (the tail is read by the decoding warps themselves)
+                if (elect()) bar_arrive(bar);           // (the tail is read by the decoding warps themselves)
             } else {
                 const int blocks = min(2, p.nb - 2 * i);
                 const uint8_t *f = value ? p.v8 : p.k8, *m = value ? p.vm : p.km, *l = value ? p.vl : p.kl;
                 const long long at = (value ? s.bh * p.L + i * TILE : (s.bh * p.nmb + 2 * i) * BLK) * D;
                 const uint32_t to = ring_at + buf * L::TILE_BYTES;
-                if (leader) {
+                if (elect()) {
                     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(blocks * BLK * D * 2) : "memory");
                     bulk(to, f + at, D * BLK, bar);
                     bulk(to + D * 64, m + at / 2, D * BLK / 2, bar);
@@ -387,7 +393,7 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t ring_at,
 // registers (by one lane alone a product took about 100 cycles to issue, and the issuing thread bound the kernel).
 template <int D>
 __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, uint32_t bars, uint32_t tmem, volatile int* dead,
-                                             long long first, long long last, bool leader) {
+                                             long long first, long long last) {
     using L = Plan<D>;
     uint32_t buf = 0, turn = 0, k_at = 0, k_buf = 0, v_at = 0, v_buf = 0;
     uint32_t items0 = 0, items1 = 0, seg = 0;          // of each slot so far
@@ -416,7 +422,7 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
                 if (one || !slot) take(v_at, v_buf);
                 fence_after();
                 const uint32_t v = operand(v_at, 8192), o = tmem + 256 + slot * 128, pr = tmem + slot * TILE;
-                if (leader) {
+                if (elect()) {
 #pragma unroll
                     for (int kk = 0; kk < TILE / 16; ++kk)
                         mma_ts(o, pr + kk * 8, v + (kk >> 2) * (D * 128 >> 4) + (kk & 3) * (2048 >> 4), instruction(D, true), n >= 2 || kk > 0);
@@ -437,7 +443,7 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
             const uint32_t q = operand(base + (!one && slot ? L::Q2_AT : L::Q_AT), 16), k = operand(k_at, tail ? 16 : D * 128);
             const uint32_t near = tail ? 32 >> 4 : 2048 >> 4, far = tail ? 16384 >> 4 : 8192 >> 4;
             const uint32_t idesc = tail ? instruction(TILE, false) : instruction(TILE, true), d = tmem + slot * TILE;
-            if (leader) {
+            if (elect()) {
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk)
                     mma_ss(d, q + (kk >> 2) * (16384 >> 4) + (kk & 3) * (32 >> 4), k + (kk >> 2) * far + (kk & 3) * near, idesc, kk > 0);
@@ -744,9 +750,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p)
     } else if (warp < SOFT + DECODE) {
         decode_role<L, D, false>(p, base + L::RING_AT, L::RING, bars, dead, odd, first, last, true, warp - SOFT, lane);
     } else if (warp == SOFT + DECODE) {
-        product_role<D>(p, base, bars, tmem, dead, first, last, lane == 0);
+        product_role<D>(p, base, bars, tmem, dead, first, last);
     } else {
-        copy_role<L, D, false>(p, base + L::RING_AT, L::RING, bars, dead, first, last, true, lane == 0);
+        copy_role<L, D, false>(p, base + L::RING_AT, L::RING, bars, dead, first, last, true);
     }
     __syncwarp();
     __syncthreads();
@@ -922,20 +928,20 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const TreeArgs
                         const uint32_t q = operand(base + L::Q_AT + g * 32768, 16), d = tmem + slot * 256, half = q_half >> 4;
                         if (tail) {
                             const uint32_t k = operand(k_at[slot], 16), idesc = instruction(0, false) | idesc_n;
-                            if (lane == 0) {
+                            if (elect()) {
 #pragma unroll
                                 for (int kk = 0; kk < D / 16; ++kk)
                                     mma_ss(d, k + (kk >> 2) * (16384 >> 4) + (kk & 3) * (32 >> 4), q + (kk >> 2) * half + (kk & 3) * (32 >> 4), idesc, kk > 0);
                             }
                         } else {
                             const uint32_t k = operand(k_at[slot], D * 128), idesc = instruction(0, false, true) | idesc_n;
-                            if (lane == 0) {
+                            if (elect()) {
 #pragma unroll
                                 for (int kk = 0; kk < D / 16; ++kk)
                                     mma_ss(d, k + kk * (2048 >> 4), q + (kk >> 2) * half + (kk & 3) * (32 >> 4), idesc, kk > 0);
                             }
                         }
-                        if (lane == 0) {
+                        if (elect()) {
                             commit(bars + 8 * (L::S_FULL + slot));
                             if (g == groups - 1) commit(bars + 8 * (L::EMPTY + k_buf[slot]));
                         }
@@ -947,7 +953,7 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const TreeArgs
             }
         }
     } else {
-        copy_role<L, D, true>(p, ring_at, ring, bars, dead, first, last, has_tail, lane == 0);
+        copy_role<L, D, true>(p, ring_at, ring, bars, dead, first, last, has_tail);
     }
     __syncwarp();
     __syncthreads();
