@@ -45,19 +45,18 @@ struct Ring {
     uint32_t base;                 // of the warp's ring
     int lane, put, get;            // steps: slots filled next, read next
     // what is copied next: step of a tile of (batch, KV head) bh; left = tiles from this one on
-    long long bh, left;
-    int step, tile, unit, plane_tiles;
+    int bh, left, step, tile, unit, plane_tiles;
 
     // Tiles first .. last - 1 of units of p.tiles tiles.
-    __device__ __forceinline__ void start(const TreeArgs& p, uint32_t at, int of_lane, long long first, long long last) {
+    __device__ __forceinline__ void start(const TreeArgs& p, uint32_t at, int of_lane, int first, int last) {
         base = at;
         lane = of_lane;
         put = get = step = 0;
         plane_tiles = (p.nb + 1) >> 1;
-        unit = (int)(first / p.tiles);
-        tile = (int)(first - (long long)unit * p.tiles);
+        unit = (unsigned)first / (unsigned)p.tiles;
+        tile = first - unit * p.tiles;
         left = last - first;
-        bh = unit / p.rt;
+        bh = (unsigned)unit / (unsigned)p.rt;
 #pragma unroll 1
         for (int i = 0; i < STEPS - 1; ++i) fill(p);
     }
@@ -65,7 +64,7 @@ struct Ring {
 
     __device__ __forceinline__ void copy_k(const TreeArgs& p, uint32_t to) const {
         const bool two = 2 * tile + 1 < p.nb;
-        const long long row = (bh * p.nmb + 2 * tile) * D + 16 * step;
+        const long long row = ((long long)bh * p.nmb + 2 * tile) * D + 16 * step;
         const uint8_t *h = p.k8 + row * BLK + lane * 16, *m = p.km + row * (BLK / 2) + lane * 16, *l = p.kl + row * (BLK / 2) + lane * 16;
         // (lane: channel lane / 4 of 8, piece lane % 4; of nibbles channel lane / 2 of 16, piece lane % 2)
         const uint32_t at = (lane >> 3) * 128 + ((((lane >> 2) & 1) * 4 + (lane & 3)) ^ (2 * (lane >> 4))) * 16;
@@ -82,7 +81,7 @@ struct Ring {
     }
     __device__ __forceinline__ void copy_v(const TreeArgs& p, uint32_t to, int vs) const {
         const bool two = 2 * tile + 1 < p.nb;
-        const long long row = bh * p.L + tile * TILE;
+        const long long row = (long long)bh * p.L + tile * TILE;
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
             const int st = vs * SUB + u;
@@ -115,13 +114,14 @@ struct Ring {
     // Rows 16 c .. of the tail: the residual tokens, the drafted ones behind them; zeros behind those.
     __device__ __forceinline__ void copy_tail(const TreeArgs& p, uint32_t to, int c, bool value) const {
         const __half *rest = value ? p.restv : p.restk, *drafted = value ? p.vd : p.kd;
-        const long long b = bh / p.H, h = bh - b * p.H;
+        const int b = (unsigned)bh / (unsigned)p.H, h = bh - b * p.H;
         constexpr int PIECES = D / 8;
 #pragma unroll
         for (int j = 0; j < PIECES / 2; ++j) {
             const int id = j * 32 + lane, r = id / PIECES, q = id % PIECES, i = 16 * c + r, d = i - p.rest;
             const bool there = i < p.tail;
-            const __half* row = d < 0 ? rest + ((b * BLK + i) * p.H + h) * D : drafted + ((b * p.T + (there ? d : 0)) * p.H + h) * D;
+            const __half* row = d < 0 ? rest + ((long long)(b * BLK + i) * p.H + h) * D
+                                      : drafted + ((long long)(b * p.T + (there ? d : 0)) * p.H + h) * D;
             copy16(to + tail_place(r, q, value), reinterpret_cast<const uint8_t*>(there ? row : p.q) + (there ? q * 16 : 0), there);
         }
     }
@@ -151,7 +151,7 @@ struct Ring {
                 --left;
                 if (++tile == p.tiles) {
                     tile = 0;
-                    bh = ++unit / p.rt;
+                    bh = (unsigned)++unit / (unsigned)p.rt;
                 }
             }
         }
@@ -222,13 +222,13 @@ __device__ __forceinline__ void tail_scores(float (&s)[2][4], const uint4* qf, u
 
 // The unit's query rows as fragments in shared memory (every lane stores and reads its own).
 template <int D>
-__device__ __forceinline__ void load_q(uint4* qf, const TreeArgs& p, long long b, int h, int row0, int lane) {
+__device__ __forceinline__ void load_q(uint4* qf, const TreeArgs& p, int b, int h, int row0, int lane) {
     const int g = lane >> 2, t = lane & 3, R = p.T * p.G;
     const __half* src[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int r = row0 + g + 8 * i;
-        src[i] = r < R ? p.q + row_of(p, b, h, r) * D : nullptr;
+        src[i] = r < R ? p.q + (long long)row_of(p, b, h, r) * D : nullptr;
     }
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
@@ -277,17 +277,17 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
     pdl_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int R = p.T * p.G;
-    const long long w = (long long)warp * gridDim.x + blockIdx.x;
+    const int w = warp * gridDim.x + blockIdx.x;
     if (w >= p.nw) return;
-    const long long first = w * p.total / p.nw, last = (w + 1) * p.total / p.nw;
+    const int first = run_start(p, w), last = run_start(p, w + 1), unit0 = (unsigned)first / (unsigned)p.tiles;
     uint4* qf = reinterpret_cast<uint4*>(smem + (size_t)warp * WARP_BYTES + STEPS * STEP_BYTES);
     uint4* pf = qf + 256;
     Ring<D> ring;
     ring.start(p, smem_u32(smem) + warp * WARP_BYTES, lane, first, last);
-    for (long long at = first; at < last;) {
-        const long long unit = at / p.tiles, bh = unit / p.rt, b = bh / p.H;
-        const int h = (int)(bh - b * p.H), row0 = (int)(unit - bh * p.rt) * ROWS;
-        const int t0 = (int)(at - unit * p.tiles), t1 = (int)min((long long)p.tiles, last - unit * p.tiles);
+    for (int at = first; at < last;) {
+        const int unit = (unsigned)at / (unsigned)p.tiles, bh = unit, b = (unsigned)bh / (unsigned)p.H, h = bh - b * p.H;
+        const int row0 = 0;      // (one unit per KV head: more rows than 16 are the other kernel's)
+        const int t0 = at - unit * p.tiles, t1 = min(p.tiles, last - unit * p.tiles);
         const __half* mask = p.mask ? p.mask + b * p.mask_stride : nullptr;
         load_q<D>(qf, p, b, h, row0, lane);
         float o[N][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
             const uint8_t* seen = p.tree + b * p.tree_stride;
             const uint8_t* mine[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) mine[i] = seen + (long long)(min(row0 + g + 8 * i, R - 1) / p.G) * p.T;
+            for (int i = 0; i < 2; ++i) mine[i] = seen + (unsigned)min(row0 + g + 8 * i, R - 1) / (unsigned)p.G * p.T;
 #pragma unroll 1
             for (int c0 = 0; c0 < p.tail; c0 += 16) {
                 float s[2][4];
@@ -447,8 +447,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
                 if (p.lse && t == 0) p.lse[row] = l[i] == 0.f ? -INFINITY : (m[i] - LIFT + log2f(l[i])) * LN2;
             } else {
                 // record of this warp: its first unit in slot 0, its last in slot 1 (those between are whole)
-                const int slot = unit != first / p.tiles;
-                float* rec = p.part + ((2 * w + slot) * ROWS + g + 8 * i) * (D + 4);
+                const int slot = unit != unit0;
+                float* rec = p.part + (size_t)((2 * w + slot) * ROWS + g + 8 * i) * (D + 4);
                 if (t == 0) {
                     rec[0] = m[i];
                     rec[1] = l[i];
@@ -467,28 +467,26 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
     }
 }
 
-// Warp that holds tile i when `total` tiles are dealt to nw warps: the largest w with floor(w total / nw) <= i.
-__device__ __forceinline__ long long warp_of(long long i, long long total, long long nw) { return ((i + 1) * nw - 1) / total; }
-
 // One warp per query row: the records of the runs that share its unit, in the order of the tokens.
 template <int D>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs p) {
     pdl_enter();
     const int lane = threadIdx.x & 31;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);       // unit * rowsu + row of the unit
-    const long long unit = row / p.rowsu, bh = unit / p.rt, b = bh / p.H;
-    const int of_unit = (int)(row - unit * p.rowsu);
-    if (unit * p.tiles >= p.total) return;
-    const int h = (int)(bh - b * p.H), r = (int)(unit - bh * p.rt) * p.rowsu + of_unit;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 5);                        // unit * rowsu + row of the unit
+    const int unit = (unsigned)row / (unsigned)p.rowsu, of_unit = row - unit * p.rowsu;
+    const int bh = (unsigned)unit / (unsigned)p.rt, b = (unsigned)bh / (unsigned)p.H, h = bh - b * p.H;
+    if ((unsigned)unit >= (unsigned)p.total / (unsigned)p.tiles) return;
+    const int r = (unit - bh * p.rt) * p.rowsu + of_unit;
     if (r >= p.T * p.G) return;
-    const long long w0 = warp_of(unit * p.tiles, p.total, p.nw), w1 = warp_of(unit * p.tiles + p.tiles - 1, p.total, p.nw);
-    if (w0 == w1) return;                                                       // a whole unit: written by its warp
-    auto record = [&](long long w) {
-        const int slot = unit != (w * p.total / p.nw) / p.tiles;
-        return p.part + ((2 * w + slot) * p.rowsu + of_unit) * (D + 4);
+    const int w0 = run_with(p, unit * p.tiles), w1 = run_with(p, unit * p.tiles + p.tiles - 1);
+    if (w0 == w1) return;                                                       // a whole unit: written by its run
+    // a run's record of its first unit is in slot 0, of its last in slot 1: only the first of this unit's may have begun before it
+    const int slot0 = run_start(p, w0) < unit * p.tiles;
+    auto record = [&](int w) {
+        return p.part + (size_t)((2 * w + (w == w0 ? slot0 : 0)) * p.rowsu + of_unit) * (D + 4);
     };
     float top = -INFINITY;
-    for (long long w = w0 + lane; w <= w1; w += 32) top = fmaxf(top, record(w)[0]);
+    for (int w = w0 + lane; w <= w1; w += 32) top = fmaxf(top, record(w)[0]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     const float base = top == -INFINITY ? 0.f : top;
@@ -497,7 +495,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs p) {
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = 0.f;
 #pragma unroll 4
-    for (long long w = w0; w <= w1; ++w) {
+    for (int w = w0; w <= w1; ++w) {
         const float* rec = record(w);
         const float f = ex2(rec[0] - base);
         l = fmaf(f, rec[1], l);
@@ -514,8 +512,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs p) {
 
 // Warps for `total` tiles: one an SM while there are that few, then up to eight.
 struct Deal {
-    int grid, wpc;
-    long long runs;
+    int grid, wpc, runs;
 };
 Deal deal(long long total, int most = WARPS) {
     const int sms = sm_count();
@@ -523,7 +520,7 @@ Deal deal(long long total, int most = WARPS) {
     d.grid = (int)(total < sms ? total : sms);
     const long long per = (total + d.grid - 1) / d.grid;
     d.wpc = (int)(per < most ? per : most);
-    d.runs = total < (long long)d.grid * d.wpc ? total : (long long)d.grid * d.wpc;
+    d.runs = total < (long long)d.grid * d.wpc ? (int)total : d.grid * d.wpc;
     return d;
 }
 
@@ -617,7 +614,7 @@ long long akv_tree_scratch_bytes(int bsz, int n_kv_heads, int group, int head_di
         drafted > BLK)
         return -1;
     const Shape s = shape_of(bsz, n_kv_heads, group, drafted, n_tokens);
-    return 2 * s.d.runs * s.rowsu * (head_dim + 4) * 4;
+    return 2ll * s.d.runs * s.rowsu * (head_dim + 4) * 4;
 }
 
 int akv_tree_attention(const akv_layer* layer, const void* q, const void* k_new, const void* v_new, const void* tree,
@@ -648,7 +645,8 @@ int akv_tree_attention(const akv_layer* layer, const void* q, const void* k_new,
     p.rowsu = s.rowsu;
     p.rt = s.rt;
     p.tiles = s.tiles;
-    p.total = s.total;
+    AKV_REQUIRE(s.total < INT_MAX, AKV_ERR_OVERFLOW, "tree_attention: too many tiles of 128 tokens");
+    p.total = (int)s.total;
     p.nw = s.d.runs;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     rc = s.wide ? launch_tree_wide(p, D, s.d.grid, st) : launch_warps(D == 128 ? tree_kernel<128> : tree_kernel<64>, s.d, st, p);
@@ -670,8 +668,10 @@ int akv_tree_weights(const akv_layer* layer, const void* q, const void* lse, con
     p.lse = static_cast<float*>(const_cast<void*>(lse));
     p.tiles = (p.nb + 1) / 2 + (rest_len > 0);
     p.tail = rest_len;
-    p.total = (long long)layer->bsz * p.H * p.tiles;
-    if (p.total == 0) return AKV_OK;
+    const long long total = (long long)layer->bsz * p.H * p.tiles;
+    AKV_REQUIRE(total < INT_MAX, AKV_ERR_OVERFLOW, "tree_weights: too many tiles of 128 tokens");
+    p.total = (int)total;
+    if (total == 0) return AKV_OK;
     const Deal d = deal(p.total, 1);
     p.nw = d.runs;
     p.rt = 1;

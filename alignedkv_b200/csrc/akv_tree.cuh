@@ -20,7 +20,7 @@ struct TreeArgs {
     int H, G, T, nmb, L, nb, rest;
     int rowsu, rt;             // query rows of a unit, units of a (batch, KV head)
     int tiles, tail;           // tiles of a unit; tokens of its last, the tail tile
-    long long total, nw;       // tiles of all units, runs that they are dealt to (at most as many): warps, or CTAs
+    int total, nw;             // tiles of all units, runs that they are dealt to (at most as many): warps, or CTAs
     int groups, rowsg;         // (tree_wide_kernel) row groups of a unit, rows of a group
     float scale, scale2;       // scale2 = scale * log2(e)
 };
@@ -36,9 +36,22 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Element of a row's tensors [B,T,Hq,...]: query row r of KV head h of sequence b.
-__device__ __forceinline__ long long row_of(const TreeArgs& p, long long b, int h, int r) {
-    return (b * p.T + r / p.G) * p.H * p.G + (long long)h * p.G + r % p.G;
+// (Indices of tiles, units and rows fit 32 bits - the launchers see to it - and are divided as such: a 64-bit division is a hundred
+// instructions, and the kernels are bound by the fetch of their instructions before anything else is used up.)
+// Row of the tensors [B,T,Hq,...]: query row r of KV head h of sequence b.
+__device__ __forceinline__ int row_of(const TreeArgs& p, int b, int h, int r) {
+    const int t = (unsigned)r / (unsigned)p.G;
+    return (b * p.T + t) * (p.H * p.G) + h * p.G + r - t * p.G;
+}
+// First tile of run w (of run w + 1: its end): the first total % nw runs have one more.
+__device__ __forceinline__ int run_start(const TreeArgs& p, int w) {
+    const unsigned each = (unsigned)p.total / (unsigned)p.nw;
+    return w * each + min(w, (int)(p.total - each * p.nw));
+}
+// Run that has tile i.
+__device__ __forceinline__ int run_with(const TreeArgs& p, int i) {
+    const unsigned each = (unsigned)p.total / (unsigned)p.nw, more = p.total - each * p.nw, bound = more * (each + 1);
+    return (unsigned)i < bound ? (unsigned)i / (each + 1) : more + ((unsigned)i - bound) / each;
 }
 
 // Tensor-core form (akv_tree_wide.cu).

@@ -64,7 +64,7 @@ __device__ __forceinline__ bool bar_try(uint32_t a, uint32_t parity) {
     return ok != 0;
 }
 // Bounded (about a second); once one has given up, none waits any more and the outputs become NaN.
-__device__ __forceinline__ void bar_wait_slow(uint32_t a, uint32_t parity, volatile int* dead) {
+__device__ __noinline__ void bar_wait_slow(uint32_t a, uint32_t parity, volatile int* dead) {
     unsigned long long t0 = 0;
     for (unsigned spin = 0; !bar_try(a, parity); ++spin) {
         if (*dead) return;
@@ -154,16 +154,15 @@ __device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t byt
 // ---------------------------------------------------------------- the run of a CTA, piece by piece
 // Segment: consecutive tiles t0 .. t0 + c - 1 of one unit.
 struct Segment {
-    long long unit, bh, b;
-    int h, super, t0, c, index;
-    __device__ __forceinline__ void at(const TreeArgs& p, long long tile, long long last) {
-        unit = tile / p.tiles;
-        t0 = (int)(tile - unit * p.tiles);
-        c = (int)min((long long)p.tiles - t0, last - tile);
-        bh = unit / p.rt;
-        super = (int)(unit - bh * p.rt);
-        b = bh / p.H;
-        h = (int)(bh - b * p.H);
+    int unit, bh, b, h, super, t0, c;
+    __device__ __forceinline__ void at(const TreeArgs& p, int tile, int last) {
+        unit = (unsigned)tile / (unsigned)p.tiles;
+        t0 = tile - unit * p.tiles;
+        c = min(p.tiles - t0, last - tile);
+        bh = (unsigned)unit / (unsigned)p.rt;
+        super = unit - bh * p.rt;
+        b = (unsigned)bh / (unsigned)p.H;
+        h = bh - b * p.H;
     }
 };
 // Operand tile q (0 .. 2c - 1) of a segment, in the order in which the products need them: with `ahead` scores under way,
@@ -203,9 +202,9 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w, bool& odd) {
 // L: the kernel's plan; KEYS: keys alone, tile after tile.  `has_tail`: whether the units' last tiles are tails.
 template <class L, int D, bool KEYS>
 __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t ring_at, uint32_t ring, uint32_t bars, volatile int* dead,
-                                          long long first, long long last, bool has_tail) {
+                                          int first, int last, bool has_tail) {
     uint32_t buf = 0, turn = 0;
-    for (long long tile = first; tile < last;) {
+    for (int tile = first; tile < last;) {
         Segment s;
         s.at(p, tile, last);
         tile += s.c;
@@ -219,7 +218,7 @@ __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t ring_at, u
             } else {
                 const int blocks = min(2, p.nb - 2 * i);
                 const uint8_t *f = value ? p.v8 : p.k8, *m = value ? p.vm : p.km, *l = value ? p.vl : p.kl;
-                const long long at = (value ? s.bh * p.L + i * TILE : (s.bh * p.nmb + 2 * i) * BLK) * D;
+                const long long at = (value ? (long long)s.bh * p.L + i * TILE : ((long long)s.bh * p.nmb + 2 * i) * BLK) * D;
                 const uint32_t to = ring_at + buf * L::TILE_BYTES;
                 if (elect()) {
                     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(blocks * BLK * D * 2) : "memory");
@@ -301,7 +300,7 @@ struct Share {
                 const int y = region * BLK + row(u), d = y - p.rest;
                 uint4 a = make_uint4(0, 0, 0, 0), b = a;
                 if (y < p.tail) {
-                    const __half* src = d < 0 ? rest + ((s.b * BLK + y) * p.H + s.h) * D : drafted + ((s.b * p.T + d) * p.H + s.h) * D;
+                    const __half* src = d < 0 ? rest + ((long long)(s.b * BLK + y) * p.H + s.h) * D : drafted + ((long long)(s.b * p.T + d) * p.H + s.h) * D;
                     const uint4* from = reinterpret_cast<const uint4*>(src + (side ^ (u & 1)) * 64 * (D == 128) + qd * 16);
                     a = __ldg(from);
                     b = __ldg(from + 1);
@@ -344,10 +343,10 @@ struct Share {
 // tile's loads and its stores in the same place finds them there.
 template <class L, int D, bool KEYS>
 __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t ring_at, uint32_t ring, uint32_t bars, volatile int* dead,
-                                            volatile int* odd, long long first, long long last, bool has_tail, int warp, int lane) {
+                                            volatile int* odd, int first, int last, bool has_tail, int warp, int lane) {
     uint32_t buf = 0, turn = 0;          // of the tile that is loaded next
     int q = 0, index = 0;
-    long long tile = first;
+    int tile = first;
     Segment s;
     s.at(p, tile, last);
     const int count = (KEYS ? 1 : 2) * (int)(last - first);
@@ -393,7 +392,7 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t ring_at,
 // registers (by one lane alone a product took about 100 cycles to issue, and the issuing thread bound the kernel).
 template <int D>
 __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, uint32_t bars, uint32_t tmem, volatile int* dead,
-                                             long long first, long long last) {
+                                             int first, int last) {
     using L = Plan<D>;
     uint32_t buf = 0, turn = 0, k_at = 0, k_buf = 0, v_at = 0, v_buf = 0;
     uint32_t items0 = 0, items1 = 0, seg = 0;          // of each slot so far
@@ -408,7 +407,7 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
             ++turn;
         }
     };
-    for (long long tile = first; tile < last; ++seg) {
+    for (int tile = first; tile < last; ++seg) {
         Segment s;
         s.at(p, tile, last);
         tile += s.c;
@@ -474,12 +473,12 @@ struct Edge {
 template <int D>
 __device__ __noinline__ void add_odd(const TreeArgs& p, const Segment& s, int r, unsigned long long seen, float base, int ch0,
                                      float* o) {
-    const __half* q = p.q + row_of(p, s.b, s.h, r) * D;
+    const __half* q = p.q + (long long)row_of(p, s.b, s.h, r) * D;
     const __half* mask = p.mask ? p.mask + s.b * p.mask_stride + p.nb * BLK : nullptr;
     for (int i = 0; i < p.tail; ++i) {
         const int d = i - p.rest;
-        const __half* k = d < 0 ? p.restk + ((s.b * BLK + i) * p.H + s.h) * D : p.kd + ((s.b * p.T + d) * p.H + s.h) * D;
-        const __half* v = d < 0 ? p.restv + ((s.b * BLK + i) * p.H + s.h) * D : p.vd + ((s.b * p.T + d) * p.H + s.h) * D;
+        const __half* k = d < 0 ? p.restk + ((long long)(s.b * BLK + i) * p.H + s.h) * D : p.kd + ((long long)(s.b * p.T + d) * p.H + s.h) * D;
+        const __half* v = d < 0 ? p.restv + ((long long)(s.b * BLK + i) * p.H + s.h) * D : p.vd + ((long long)(s.b * p.T + d) * p.H + s.h) * D;
         const float add = d < 0 && mask ? __half2float(mask[i]) : 0.f;
         if (d < 0 ? add == -INFINITY : !(seen >> d & 1)) continue;
         float pr = -1.f;
@@ -498,7 +497,7 @@ __device__ __noinline__ void add_odd(const TreeArgs& p, const Segment& s, int r,
 
 template <int D>
 __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, uint32_t base, uint32_t bars, uint32_t tmem,
-                                             volatile int* dead, volatile int* odd, long long first, long long last, int warp, int lane) {
+                                             volatile int* dead, volatile int* odd, int first, int last, int warp, int lane) {
     const int slot = warp >> 2, idx = (warp & 3) * 32 + lane, R = p.T * p.G, group = p.groups == 2 ? slot : 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + slot * TILE, o_at = tmem + lanes + 256 + slot * 128;
     const float scale2 = fabsf(p.scale2);          // (the queries take the sign)
@@ -507,7 +506,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
     float* xl = reinterpret_cast<float*>(smem + Plan<D>::XL_AT);
     uint32_t done = 0;
     int seg = 0;
-    for (long long tile = first; tile < last; ++seg) {
+    for (int tile = first; tile < last; ++seg) {
         Segment s;
         s.at(p, tile, last);
         tile += s.c;
@@ -517,7 +516,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
         // queries: 16-byte piece c of a row's half at c ^ (row & 7)
         soft_sync();
         {
-            const uint4* src = reinterpret_cast<const uint4*>(p.q + (mine ? row_of(p, s.b, s.h, r) : 0) * D);
+            const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(mine ? row_of(p, s.b, s.h, r) : 0) * D);
             const uint32_t to = base + (group ? Plan<D>::Q2_AT : Plan<D>::Q_AT) + idx * 128;
             const int c0 = p.groups == 1 ? slot * (D / 16) : 0, c1 = p.groups == 1 ? c0 + D / 16 : D / 8;
             for (int c = c0; c < c1; ++c) {
@@ -532,7 +531,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
         const bool with_tail = s.t0 + s.c == p.tiles;
         unsigned long long seen = 0;
         if (with_tail && mine) {
-            const uint8_t* row = p.tree + s.b * p.tree_stride + (long long)(r / p.G) * p.T;
+            const uint8_t* row = p.tree + s.b * p.tree_stride + (unsigned)r / (unsigned)p.G * p.T;
             for (int d = 0; d < p.T; ++d) seen |= (unsigned long long)(row[d] != 0) << d;
         }
         const __half* mask = p.mask ? p.mask + s.b * p.mask_stride : nullptr;
@@ -549,7 +548,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                 Edge edge;
                 edge.count = tail ? p.tail : min(TILE, p.nb * BLK - i * TILE);
                 edge.rest = tail ? p.rest : edge.count;
-                edge.mask = mask ? mask + (long long)min(i * TILE, p.nb * BLK) : nullptr;
+                edge.mask = mask ? mask + min(i * TILE, p.nb * BLK) : nullptr;
                 edge.seen = seen;
                 // edges: scores to base 2 go back to where they came from; elsewhere they stay products until the exponential
                 const bool plain = !tail && !mask && edge.count == TILE;
@@ -637,8 +636,8 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
         const bool whole = s.c == p.tiles, odd_tail = with_tail && odd[seg % Plan<D>::SEGMENTS] == seg + 1;
         if (*dead) l = __int_as_float(0x7FC00000);
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int rec_slot = s.unit != first / p.tiles;
-        float* rec = p.part + ((2 * (long long)blockIdx.x + rec_slot) * p.rowsu + of_unit) * (D + 4);
+        const int rec_slot = s.unit != (unsigned)first / (unsigned)p.tiles;
+        float* rec = p.part + (size_t)((2 * blockIdx.x + rec_slot) * p.rowsu + of_unit) * (D + 4);
         float4* join = reinterpret_cast<float4*>(smem + Plan<D>::Q2_AT);              // [16 channel quads][128 rows]
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
@@ -684,7 +683,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                 for (int j = 0; j < 32; ++j) o[j] += x[j];
             }
             if (whole) {
-                uint4* dst = reinterpret_cast<uint4*>(p.out + row_of(p, s.b, s.h, r) * D + c);
+                uint4* dst = reinterpret_cast<uint4*>(p.out + (long long)row_of(p, s.b, s.h, r) * D + c);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     dst[j] = make_uint4(pack_half2(o[8 * j] * inv, o[8 * j + 1] * inv), pack_half2(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
@@ -744,7 +743,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p)
     __syncthreads();
     fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(slot_tmem);
-    const long long w = blockIdx.x, first = w * p.total / p.nw, last = (w + 1) * p.total / p.nw;
+    const int first = run_start(p, blockIdx.x), last = run_start(p, blockIdx.x + 1);
     if (warp < SOFT) {
         softmax_role<D>(p, smem, base, bars, tmem, dead, odd, first, last, warp, lane);
     } else if (warp < SOFT + DECODE) {
@@ -823,19 +822,19 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const TreeArgs
     __syncthreads();
     fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(slot_tmem);
-    const long long w = blockIdx.x, first = w * p.total / p.nw, last = (w + 1) * p.total / p.nw;
+    const int first = run_start(p, blockIdx.x), last = run_start(p, blockIdx.x + 1);
     if (warp < SOFT) {
         const int slot = warp >> 2, idx = (warp & 3) * 32 + lane;
         const uint32_t s_at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + slot * 256;
         uint32_t done = 0;
-        for (long long tile = first; tile < last;) {
+        for (int tile = first; tile < last;) {
             Segment s;
             s.at(p, tile, last);
             tile += s.c;
             soft_sync();                               // (all products with the queries before are over: their scores have been read)
             for (int i = threadIdx.x; i < L::padded(rows) * (D / 8); i += 32 * SOFT) {
                 const int r = i / (D / 8), c = i % (D / 8);
-                const uint4 x = r < rows ? __ldg(reinterpret_cast<const uint4*>(p.q + row_of(p, s.b, s.h, row0 + r) * D) + c) : make_uint4(0, 0, 0, 0);
+                const uint4 x = r < rows ? __ldg(reinterpret_cast<const uint4*>(p.q + (long long)row_of(p, s.b, s.h, row0 + r) * D) + c) : make_uint4(0, 0, 0, 0);
                 asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(base + L::Q_AT + (c >> 3) * q_half + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
                              "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
             }
@@ -892,7 +891,7 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const TreeArgs
                 if (!gone) {
                     float x = (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     if (*dead) x = __int_as_float(0x7FC00000);
-                    weights[s.bh * p.L + at + tok] += x;
+                    weights[(long long)s.bh * p.L + at + tok] += x;
                 }
             }
         }
@@ -900,7 +899,7 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const TreeArgs
         decode_role<L, D, true>(p, ring_at, ring, bars, dead, nullptr, first, last, has_tail, warp - SOFT, lane);
     } else if (warp == SOFT + DECODE) {
         uint32_t buf = 0, turn = 0, items0 = 0, items1 = 0, seg = 0, k_at[2] = {0, 0}, k_buf[2] = {0, 0};
-        for (long long tile = first; tile < last; ++seg) {
+        for (int tile = first; tile < last; ++seg) {
             Segment s;
             s.at(p, tile, last);
             tile += s.c;
