@@ -222,12 +222,12 @@ __device__ __forceinline__ void tail_scores(float (&s)[2][4], const uint4* qf, u
 
 // The unit's query rows as fragments in shared memory (every lane stores and reads its own).
 template <int D>
-__device__ __forceinline__ void load_q(uint4* qf, const TreeArgs& p, int b, int h, int row0, int lane) {
+__device__ __forceinline__ void load_q(uint4* qf, const TreeArgs& p, int b, int h, int lane) {
     const int g = lane >> 2, t = lane & 3, R = p.T * p.G;
     const __half* src[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int r = row0 + g + 8 * i;
+        const int r = g + 8 * i;
         src[i] = r < R ? p.q + (long long)row_of(p, b, h, r) * D : nullptr;
     }
 #pragma unroll
@@ -271,7 +271,7 @@ __device__ __forceinline__ void soften(float (&s)[NJ][4], float (&m)[2], float (
 }
 
 template <int D>
-__global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
+__global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_constant__ TreeArgs p) {
     constexpr int N = D / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_enter();
@@ -285,12 +285,13 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
     Ring<D> ring;
     ring.start(p, smem_u32(smem) + warp * WARP_BYTES, lane, first, last);
     for (int at = first; at < last;) {
-        const int unit = (unsigned)at / (unsigned)p.tiles, bh = unit, b = (unsigned)bh / (unsigned)p.H, h = bh - b * p.H;
-        const int row0 = 0;      // (one unit per KV head: more rows than 16 are the other kernel's)
+        // (one unit per KV head: more rows than 16 are the other kernel's)
+        const int unit = (unsigned)at / (unsigned)p.tiles, b = (unsigned)unit / (unsigned)p.H, h = unit - b * p.H;
         const int t0 = at - unit * p.tiles, t1 = min(p.tiles, last - unit * p.tiles);
         const __half* mask = p.mask ? p.mask + b * p.mask_stride : nullptr;
-        load_q<D>(qf, p, b, h, row0, lane);
+        load_q<D>(qf, p, b, h, lane);
         float o[N][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        bool odd = false;                               // whether the tail has values that are not finite
 #pragma unroll
         for (int j = 0; j < N; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 #pragma unroll 1
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
             const uint8_t* seen = p.tree + b * p.tree_stride;
             const uint8_t* mine[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) mine[i] = seen + (unsigned)min(row0 + g + 8 * i, R - 1) / (unsigned)p.G * p.T;
+            for (int i = 0; i < 2; ++i) mine[i] = seen + (unsigned)min(g + 8 * i, R - 1) / (unsigned)p.G * p.T;
 #pragma unroll 1
             for (int c0 = 0; c0 < p.tail; c0 += 16) {
                 float s[2][4];
@@ -368,10 +369,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
                 soften(s, m, l, o);
                 const uint4 a = make_uint4(pack_half2(s[0][0], s[0][1]), pack_half2(s[0][2], s[0][3]), pack_half2(s[1][0], s[1][1]),
                                            pack_half2(s[1][2], s[1][3]));
-                // What one row sees is masked for another, and 0 * inf would be NaN: values that are not finite are left
-                // out of the product and added by the rows that see them.
                 const uint32_t from = ring.take(p);
-                bool odd = false;
                 uint32_t x[4][N / 2];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -382,53 +380,21 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
                         x[i][4 * v] = y.x; x[i][4 * v + 1] = y.y; x[i][4 * v + 2] = y.z; x[i][4 * v + 3] = y.w;
                     }
 #pragma unroll
-                    for (int v = 0; v < N / 2; ++v) {
-                        if ((x[i][v] & 0x7C00u) == 0x7C00u) { x[i][v] &= 0xFFFF0000u; odd = true; }
-                        if ((x[i][v] & 0x7C000000u) == 0x7C000000u) { x[i][v] &= 0xFFFFu; odd = true; }
-                    }
+                    for (int v = 0; v < N / 2; ++v) x[i][v] = finite_halves(x[i][v], odd);
                 }
 #pragma unroll
                 for (int v = 0; v < N / 2; ++v) {
                     mma_f16(o[2 * v], a, __byte_perm(x[0][v], x[1][v], 0x5410), __byte_perm(x[2][v], x[3][v], 0x5410));
                     mma_f16(o[2 * v + 1], a, __byte_perm(x[0][v], x[1][v], 0x7632), __byte_perm(x[2][v], x[3][v], 0x7632));
                 }
-                if (__any_sync(0xFFFFFFFFu, odd)) {
-                    float* pr = reinterpret_cast<float*>(pf);               // [16 rows][16 tokens], absent ones below zero
-                    __syncwarp();
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const int tok = c0 + 8 * j + 2 * t + (c & 1), d = tok - p.rest;
-                            const bool here = d < 0 ? !(mask && __half_as_ushort(mask[p.nb * BLK + tok]) == 0xFC00u)
-                                                    : d < p.T && mine[c >> 1][d];
-                            pr[(g + 8 * (c >> 1)) * 16 + 8 * j + 2 * t + (c & 1)] = here ? s[j][c] : -1.f;
-                        }
-                    __syncwarp();
-#pragma unroll 1
-                    for (int k = 0; k < min(16, p.tail - c0); ++k) {
-                        const float p0 = pr[g * 16 + k], p1 = pr[(g + 8) * 16 + k];
-#pragma unroll
-                        for (int j = 0; j < N; ++j)
-#pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                const int ch = N * (2 * t + c) + j;
-                                const uint32_t y = lds16(from + Ring<D>::tail_place(k, ch >> 3, true) + (ch & 7) * 2);
-                                if ((y & 0x7C00u) != 0x7C00u) continue;
-                                const float v = __half2float(__ushort_as_half((unsigned short)y));
-                                if (!(p0 < 0.f)) o[j][c] += p0 * v;
-                                if (!(p1 < 0.f)) o[j][2 + c] += p1 * v;
-                            }
-                    }
-                    __syncwarp();
-                }
             }
+            odd = __any_sync(0xFFFFFFFFu, odd);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
             l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
-            const int r = row0 + g + 8 * i;
+            const int r = g + 8 * i;
             if (r >= R) continue;
             if (t0 == 0 && t1 == p.tiles) {
                 const long long row = row_of(p, b, h, r);
@@ -462,14 +428,26 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const TreeArgs p) {
                                         o[4 * v + 3][2 * i + c]);
             }
         }
-        at = unit * p.tiles + t1;
         __syncwarp();
+        if (odd && t == 0) {
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+                const int r = g + 8 * i;
+                if (r >= R) continue;
+                const float top = i ? m[1] : m[0], sum = i ? l[1] : l[0], base = (top == -INFINITY ? 0.f : top) - LIFT;
+                if (t0 == 0 && t1 == p.tiles)
+                    add_odd(p, b, h, r, D, base, sum == 0.f ? 0.f : 1.f / sum, p.out + (long long)row_of(p, b, h, r) * D);
+                else
+                    add_odd(p, b, h, r, D, base, 1.f, p.part + (size_t)((2 * w + (unit != unit0)) * ROWS + r) * (D + 4) + 4);
+            }
+        }
+        at = unit * p.tiles + t1;
     }
 }
 
 // One warp per query row: the records of the runs that share its unit, in the order of the tokens.
 template <int D>
-__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeArgs p) {
+__global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeArgs p) {
     pdl_enter();
     const int lane = threadIdx.x & 31;
     const int row = blockIdx.x * 4 + (threadIdx.x >> 5);                        // unit * rowsu + row of the unit

@@ -54,6 +54,42 @@ __device__ __forceinline__ int run_with(const TreeArgs& p, int i) {
     return (unsigned)i < bound ? (unsigned)i / (each + 1) : more + ((unsigned)i - bound) / each;
 }
 
+// Tail values that are not finite.  What one row sees of the drafted tokens is masked for another, and 0 * inf would be NaN: such
+// values enter the product as zeros, and a row that sees them adds p . v to what it has written (p relative to 2^base, times `inv`).
+// The rare way: by itself, and out of line.
+template <class T>
+static __device__ __noinline__ void add_odd(const TreeArgs& p, int b, int h, int r, int D, float base, float inv, T* to) {
+    const __half* q = p.q + (long long)row_of(p, b, h, r) * D;
+    const __half* mask = p.mask ? p.mask + b * p.mask_stride + p.nb * BLK : nullptr;
+    const uint8_t* seen = p.tree + b * p.tree_stride + (unsigned)r / (unsigned)p.G * p.T;
+#pragma unroll 1
+    for (int i = 0; i < p.tail; ++i) {
+        const int d = i - p.rest;
+        const long long at = ((long long)(d < 0 ? b * BLK + i : b * p.T + d) * p.H + h) * D;
+        const __half *k = (d < 0 ? p.restk : p.kd) + at, *v = (d < 0 ? p.restv : p.vd) + at;
+        const float add = d < 0 && mask ? __half2float(mask[i]) : 0.f;
+        if (d < 0 ? add == -INFINITY : !seen[d]) continue;
+        float pr = -1.f;
+#pragma unroll 1
+        for (int c = 0; c < D; ++c) {
+            const float x = __half2float(v[c]);
+            if (isfinite(x)) continue;
+            if (pr < 0.f) {
+                float dot = 0.f;
+#pragma unroll 1
+                for (int j = 0; j < D; ++j) dot = fmaf(__half2float(q[j]), __half2float(k[j]), dot);
+                pr = ex2(fmaf(dot, p.scale2, add * LOG2E) - base) * inv;
+            }
+            to[c] = (T)((float)to[c] + pr * x);
+        }
+    }
+}
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w, bool& odd) {
+    if ((w & 0x7C00u) == 0x7C00u) { w &= 0xFFFF0000u; odd = true; }
+    if ((w & 0x7C000000u) == 0x7C000000u) { w &= 0xFFFFu; odd = true; }
+    return w;
+}
+
 // Tensor-core form (akv_tree_wide.cu).
 int launch_tree_wide(const TreeArgs& p, int D, int ctas, cudaStream_t st);
 int launch_weights_wide(const TreeArgs& p, int D, int ctas, float* weights, cudaStream_t st);

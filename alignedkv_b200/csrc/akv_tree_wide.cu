@@ -140,6 +140,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) 
                  ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
                    "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t (&v)[8], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(at) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
+                 ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void soft_sync() {
     __syncwarp();
@@ -190,16 +199,6 @@ __device__ __forceinline__ uint4 halves8(uint32_t h0, uint32_t h1, uint32_t m, u
 __device__ __forceinline__ uint4 reorder8(const uint4& x) {
     return make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632), __byte_perm(x.z, x.w, 0x5410), __byte_perm(x.z, x.w, 0x7632));
 }
-__device__ __forceinline__ uint32_t finite_halves(uint32_t w, bool& odd) {
-    if ((w & 0x7C00u) == 0x7C00u) { w &= 0xFFFF0000u; odd = true; }
-    if ((w & 0x7C000000u) == 0x7C000000u) { w &= 0xFFFFu; odd = true; }
-    return w;
-}
-
-// A ring tile is two regions of 64 tokens, D * 128 bytes each.  As copied: the high bytes, then either nibble plane.  As operand: K rows
-// [channel] of 64 tokens; V [channel half][token] rows of 64 channels; 16-byte piece c of row r at c ^ (r & 7).  (The tail's keys:
-// [channel half][token] over the whole tile, for groups of eight tokens at one distance.)
-// L: the kernel's plan; KEYS: keys alone, tile after tile.  `has_tail`: whether the units' last tiles are tails.
 template <class L, int D, bool KEYS>
 __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t ring_at, uint32_t ring, uint32_t bars, volatile int* dead,
                                           int first, int last, bool has_tail) {
@@ -245,145 +244,109 @@ __device__ __forceinline__ void copy_role(const TreeArgs& p, uint32_t ring_at, u
 // pieces lie, as bytes and as operand: e0, e1, e0 + t, e1 + t and f0, f1, f0 + 4096, f1 + 4096, whatever the tile is - K: channels k,
 // 64 + k, 32 + k, 96 + k (k = 8 warp + lane / 4 of 32); V: tokens k, k, 32 + k, 32 + k and both their channel halves, of neighbouring
 // lanes different ones (neither the loads of the bytes nor the stores of the operands meet in a bank); D = 64: rows k, 32 + k.
+__device__ __forceinline__ void sts128(uint32_t at, const uint4& x) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+}
+
+// The tail's share: rows of fp16 values from the residual buffers and the drafted tensors, straight to the operand.  Whether V has
+// values that are not finite (zeros in the operand, see add_odd).
 template <int D>
-struct Share {
-    static constexpr int U = D / 32;
-    uint32_t w[U][8];
-    uint32_t f0, f1;            // from the ring slot
-    bool bytes, value;          // not yet fp16; V
-    int index;                  // segment
-
-    __device__ __forceinline__ void load(const TreeArgs& p, const Segment& s, int i, bool of_values, bool tail, uint32_t slot, int warp,
-                                         int lane) {
-        const int region = warp >> 2, k = (warp & 3) * 8 + (lane >> 2), qd = lane & 3, x = ((2 * qd) ^ (k & 7)) << 4;
-        const uint32_t side = D == 128 ? (lane >> 2 ^ lane >> 3) & 1 : 0;
-        value = of_values;
-        bytes = !tail;
-        const int kr = value && !tail ? swapped(k) : k;            // (V's tokens are stored in the order of the scores' columns)
-        const bool by_half = D == 128 && (value || tail);
-        auto row = [&](int u) { return D == 64 ? u * 32 + kr : by_half ? (u >> 1) * 32 + kr : (u & 1) * 64 + (u >> 1) * 32 + kr; };
-        f0 = region * D * 128 + k * 128 + x + side * 8192 * by_half;
-        f1 = region * D * 128 + k * 128 + x + (D == 64 ? 4096 : by_half ? (side ^ 1) * 8192 : 8192);
-        if (tail && !value) {
-            f0 = region * 8192 + k * 128 + x + side * 16384;
-            f1 = region * 8192 + k * 128 + x + (D == 64 ? 4096 : (side ^ 1) * 16384);
+__device__ __noinline__ bool tail_share(const TreeArgs& p, int b, int h, bool value, uint32_t slot, int warp, int lane) {
+    const int region = warp >> 2, k = (warp & 3) * 8 + (lane >> 2), qd = lane & 3, x = ((2 * qd) ^ (k & 7)) << 4;
+    const __half *rest = value ? p.restv : p.restk, *drafted = value ? p.vd : p.kd;
+    bool odd = false;
+#pragma unroll 1
+    for (int u = 0; u < D / 32; ++u) {
+        const int half = D == 128 ? ((lane >> 2 ^ lane >> 3) ^ u) & 1 : 0, row = (D == 128 ? u >> 1 : u) * 32 + k;
+        const int y = region * BLK + row, d = y - p.rest;
+        uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if (y < p.tail) {
+            const __half* src = d < 0 ? rest + ((long long)(b * BLK + y) * p.H + h) * D : drafted + ((long long)(b * p.T + d) * p.H + h) * D;
+            const uint4* from = reinterpret_cast<const uint4*>(src + half * 64 + qd * 16);
+            v[0] = __ldg(from);
+            v[1] = __ldg(from + 1);
         }
-        if (!tail) {
-            const uint32_t at = slot + region * D * 128;
-            const uint32_t e0 = by_half ? kr * 128 + side * 64 + qd * 16 : kr * 64 + qd * 16;
-            const uint32_t e1 = by_half ? e0 ^ 64 : D == 64 ? e0 + 2048 : e0 + 4096, t = by_half ? 4096 : 2048;
+        const uint32_t at = slot + (value ? region * D * 128 + half * 8192 : region * 8192 + half * 16384) + row * 128 + x;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t e = (u & 1 ? e1 : e0) + (u >> 1) * t;
-                const uint4 h = lds128(at + e);
-                const uint2 m = lds64(at + D * 64 + e / 2), l = lds64(at + D * 96 + e / 2);
-                w[u][0] = h.x; w[u][1] = h.y; w[u][2] = h.z; w[u][3] = h.w;
-                w[u][4] = m.x; w[u][5] = m.y; w[u][6] = l.x; w[u][7] = l.y;
+        for (int e = 0; e < 2; ++e) {
+            if (value) {
+                v[e] = make_uint4(finite_halves(v[e].x, odd), finite_halves(v[e].y, odd), finite_halves(v[e].z, odd), finite_halves(v[e].w, odd));
+                v[e] = reorder8(v[e]);
             }
-            const int some = p.nb * BLK - i * TILE;
-            if (some < TILE || (value && p.mask)) {
-                // (a token that does not exist or is masked away counts as zero, whatever there is: 0 * NaN would be NaN)
-                const uint16_t* mask = value && p.mask ? reinterpret_cast<const uint16_t*>(p.mask) + s.b * p.mask_stride + i * TILE : nullptr;
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int tok = region * BLK + (value ? row(u) : 0);
-                    if (tok >= some || (mask && mask[tok] == 0xFC00u)) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) w[u][j] = 0;
-                    }
-                }
-            }
-        } else {
-            const __half *rest = value ? p.restv : p.restk, *drafted = value ? p.vd : p.kd;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int y = region * BLK + row(u), d = y - p.rest;
-                uint4 a = make_uint4(0, 0, 0, 0), b = a;
-                if (y < p.tail) {
-                    const __half* src = d < 0 ? rest + ((long long)(s.b * BLK + y) * p.H + s.h) * D : drafted + ((long long)(s.b * p.T + d) * p.H + s.h) * D;
-                    const uint4* from = reinterpret_cast<const uint4*>(src + (side ^ (u & 1)) * 64 * (D == 128) + qd * 16);
-                    a = __ldg(from);
-                    b = __ldg(from + 1);
-                }
-                if (value) {
-                    a = reorder8(a);
-                    b = reorder8(b);
-                }
-                w[u][0] = a.x; w[u][1] = a.y; w[u][2] = a.z; w[u][3] = a.w;
-                w[u][4] = b.x; w[u][5] = b.y; w[u][6] = b.z; w[u][7] = b.w;
-            }
+            sts128(at ^ (16 * e), v[e]);
         }
     }
-    // Whether the tail's values hold one that is not finite: zeros in the operand, added where a row sees them.
-    __device__ __forceinline__ bool store(uint32_t slot) {
-        bool odd = false;
-        if (!bytes && value) {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[u][j] = finite_halves(w[u][j], odd);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            uint4 x = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]), y = make_uint4(w[u][4], w[u][5], w[u][6], w[u][7]);
-            if (bytes) {
-                const uint4 h = x, n = y;
-                x = halves8(h.x, h.y, n.x, n.z);
-                y = halves8(h.z, h.w, n.y, n.w);
-            }
-            const uint32_t at = slot + (u & 1 ? f1 : f0) + (u >> 1) * 4096;
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(at ^ 16), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
-        }
-        return odd;
-    }
-};
+    return odd;
+}
 
-// The next tile's bytes are on their way to registers while this one's are decoded; the barrier of the region's four warps between a
-// tile's loads and its stores in the same place finds them there.
 template <class L, int D, bool KEYS>
 __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t ring_at, uint32_t ring, uint32_t bars, volatile int* dead,
                                             volatile int* odd, int first, int last, bool has_tail, int warp, int lane) {
-    uint32_t buf = 0, turn = 0;          // of the tile that is loaded next
-    int q = 0, index = 0;
-    int tile = first;
-    Segment s;
-    s.at(p, tile, last);
-    const int count = (KEYS ? 1 : 2) * (int)(last - first);
-    Share<D> a;
-    auto load = [&](Share<D>& x) {
-        bool value = false;
-        const int i = s.t0 + (KEYS ? q : tile_of(q, s.c, 3 - p.groups, value));
-        bar_wait(bars + 8 * (L::RAW + buf), turn & 1, dead);
-        x.index = index;
-        x.load(p, s, i, value, has_tail && i == p.tiles - 1, ring_at + buf * L::TILE_BYTES, warp, lane);
-        if (++buf == ring) {
-            buf = 0;
-            ++turn;
-        }
-        if (++q == (KEYS ? 1 : 2) * s.c) {
-            q = 0;
-            ++index;
-            tile += s.c;
-            if (tile < last) s.at(p, tile, last);
-        }
-    };
-    auto store = [&](Share<D>& x, uint32_t slot) {
-        if (x.store(ring_at + slot * L::TILE_BYTES) && !KEYS) odd[x.index % L::SEGMENTS] = x.index + 1;
-        fence_shared();
-        __syncwarp();
-        if (lane == 0) bar_arrive(bars + 8 * (L::FULL + slot));
-    };
-    auto loaded = [&]() {
-        __syncwarp();
-        asm volatile("bar.sync %0, 128;\n" ::"r"(2 + (warp >> 2)) : "memory");
-    };
+    constexpr int U = D / 32;
+    const int region = warp >> 2, k = (warp & 3) * 8 + (lane >> 2), qd = lane & 3;
+    const uint32_t side = D == 128 ? (lane >> 2 ^ lane >> 3) & 1 : 0;
+    const uint32_t to = region * D * 128 + k * 128 + (((2 * qd) ^ (k & 7)) << 4);
+    uint32_t buf = 0, turn = 0;
+    int index = 0;
+    for (int tile = first; tile < last; ++index) {
+        Segment s;
+        s.at(p, tile, last);
+        tile += s.c;
 #pragma unroll 1
-    for (int n = 0; n < count; ++n) {
-        const uint32_t slot = buf;
-        load(a);
-        loaded();
-        store(a, slot);
+        for (int q = 0; q < (KEYS ? 1 : 2) * s.c; ++q) {
+            bool value = false;
+            const int i = s.t0 + (KEYS ? q : tile_of(q, s.c, 3 - p.groups, value));
+            const uint32_t slot = ring_at + buf * L::TILE_BYTES;
+            bar_wait(bars + 8 * (L::RAW + buf), turn & 1, dead);
+            if (has_tail && i == p.tiles - 1) {
+                if (tail_share<D>(p, s.b, s.h, value, slot, warp, lane) && !KEYS) odd[index % L::SEGMENTS] = index + 1;
+            } else {
+                const int kr = value ? swapped(k) : k;             // (V's tokens are stored in the order of the scores' columns)
+                const bool by_half = D == 128 && value;
+                const uint32_t at = slot + region * D * 128;
+                const uint32_t e0 = by_half ? kr * 128 + side * 64 + qd * 16 : kr * 64 + qd * 16;
+                const uint32_t e1 = by_half ? e0 ^ 64 : D == 64 ? e0 + 2048 : e0 + 4096, t = by_half ? 4096 : 2048;
+                uint32_t w[U][8];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const uint32_t e = (u & 1 ? e1 : e0) + (u >> 1) * t;
+                    const uint4 h = lds128(at + e);
+                    const uint2 m = lds64(at + D * 64 + e / 2), l = lds64(at + D * 96 + e / 2);
+                    w[u][0] = h.x; w[u][1] = h.y; w[u][2] = h.z; w[u][3] = h.w;
+                    w[u][4] = m.x; w[u][5] = m.y; w[u][6] = l.x; w[u][7] = l.y;
+                }
+                __syncwarp();                          // the region's bytes are in registers
+                asm volatile("bar.sync %0, 128;\n" ::"r"(2 + region) : "memory");
+                const uint32_t f0 = slot + to + (by_half ? side * 8192 : 0), f1 = slot + to + (by_half ? (side ^ 1) * 8192 : D == 64 ? 4096 : 8192);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const uint32_t f = (u & 1 ? f1 : f0) + (u >> 1) * 4096;
+                    sts128(f, halves8(w[u][0], w[u][1], w[u][4], w[u][6]));
+                    sts128(f ^ 16, halves8(w[u][2], w[u][3], w[u][5], w[u][7]));
+                }
+                const int some = p.nb * BLK - i * TILE;
+                if (some < TILE || (value && p.mask)) {
+                    // (a token that does not exist or is masked away counts as zero, whatever there is: 0 * NaN would be NaN)
+                    const uint16_t* mask = value && p.mask ? reinterpret_cast<const uint16_t*>(p.mask) + s.b * p.mask_stride + i * TILE : nullptr;
+#pragma unroll 1
+                    for (int u = 0; u < U; ++u) {
+                        const int tok = region * BLK + (value ? (D == 128 ? u >> 1 : u) * 32 + kr : 0);
+                        if (tok >= some || (mask && mask[tok] == 0xFC00u)) {
+                            const uint32_t f = (u & 1 ? f1 : f0) + (u >> 1) * 4096;
+                            sts128(f, make_uint4(0, 0, 0, 0));
+                            sts128(f ^ 16, make_uint4(0, 0, 0, 0));
+                        }
+                    }
+                }
+            }
+            fence_shared();
+            __syncwarp();
+            if (lane == 0) bar_arrive(bars + 8 * (L::FULL + buf));
+            if (++buf == ring) {
+                buf = 0;
+                ++turn;
+            }
+        }
     }
 }
 
@@ -469,32 +432,6 @@ struct Edge {
     }
 };
 
-// p . v of the tail values that are not finite (they are zeros in the operand), for 32 channels of a row: the rare way.
-template <int D>
-__device__ __noinline__ void add_odd(const TreeArgs& p, const Segment& s, int r, unsigned long long seen, float base, int ch0,
-                                     float* o) {
-    const __half* q = p.q + (long long)row_of(p, s.b, s.h, r) * D;
-    const __half* mask = p.mask ? p.mask + s.b * p.mask_stride + p.nb * BLK : nullptr;
-    for (int i = 0; i < p.tail; ++i) {
-        const int d = i - p.rest;
-        const __half* k = d < 0 ? p.restk + ((long long)(s.b * BLK + i) * p.H + s.h) * D : p.kd + ((long long)(s.b * p.T + d) * p.H + s.h) * D;
-        const __half* v = d < 0 ? p.restv + ((long long)(s.b * BLK + i) * p.H + s.h) * D : p.vd + ((long long)(s.b * p.T + d) * p.H + s.h) * D;
-        const float add = d < 0 && mask ? __half2float(mask[i]) : 0.f;
-        if (d < 0 ? add == -INFINITY : !(seen >> d & 1)) continue;
-        float pr = -1.f;
-        for (int c = 0; c < 32; ++c) {
-            const float x = __half2float(v[ch0 + c]);
-            if (isfinite(x)) continue;
-            if (pr < 0.f) {
-                float dot = 0.f;
-                for (int j = 0; j < D; ++j) dot = fmaf(__half2float(q[j]), __half2float(k[j]), dot);
-                pr = ex2(fmaf(dot, p.scale2, add * LOG2E) - base);
-            }
-            o[c] += pr * x;
-        }
-    }
-}
-
 template <int D>
 __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, uint32_t base, uint32_t bars, uint32_t tmem,
                                              volatile int* dead, volatile int* odd, int first, int last, int warp, int lane) {
@@ -519,6 +456,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
             const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(mine ? row_of(p, s.b, s.h, r) : 0) * D);
             const uint32_t to = base + (group ? Plan<D>::Q2_AT : Plan<D>::Q_AT) + idx * 128;
             const int c0 = p.groups == 1 ? slot * (D / 16) : 0, c1 = p.groups == 1 ? c0 + D / 16 : D / 8;
+#pragma unroll 1
             for (int c = c0; c < c1; ++c) {
                 uint4 x = mine ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
                 asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(to + (c >> 3) * Plan<D>::Q_HALF + (((c & 7) ^ (idx & 7)) << 4)),
@@ -532,6 +470,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
         unsigned long long seen = 0;
         if (with_tail && mine) {
             const uint8_t* row = p.tree + s.b * p.tree_stride + (unsigned)r / (unsigned)p.G * p.T;
+#pragma unroll 1
             for (int d = 0; d < p.T; ++d) seen |= (unsigned long long)(row[d] != 0) << d;
         }
         const __half* mask = p.mask ? p.mask + s.b * p.mask_stride : nullptr;
@@ -556,13 +495,14 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                 uint32_t v[32];
                 if (!plain) {
 #pragma unroll 1
-                    for (int c = 0; c < TILE; c += 32) {
+                    for (int c = 0; c < TILE; c += 8) {
+                        uint32_t x[8];
                         __syncwarp();
-                        tmem_ld(v, s_at + c);
+                        tmem_ld8(x, s_at + c);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(edge(__uint_as_float(v[j]), scale2, c + (tail ? j : swapped(j))));
+                        for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(edge(__uint_as_float(x[j]), scale2, c + (tail ? j : swapped(j))));
                         __syncwarp();
-                        tmem_st32(s_at + c, v);
+                        tmem_st8(s_at + c, x);
                     }
                     tmem_st_wait();
                 }
@@ -675,13 +615,6 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                 }
             }
             if (!mine) continue;
-            if (odd_tail) {
-                float x[32];
-                for (int j = 0; j < 32; ++j) x[j] = 0.f;
-                add_odd<D>(p, s, r, seen, (ref == -INFINITY ? 0.f : ref) - WIDE_LIFT, c, x);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] += x[j];
-            }
             if (whole) {
                 uint4* dst = reinterpret_cast<uint4*>(p.out + (long long)row_of(p, s.b, s.h, r) * D + c);
 #pragma unroll
@@ -695,6 +628,11 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
             }
         }
         if (mine && !(p.groups == 1 && slot)) {
+            if (odd_tail) {
+                const float off = (ref == -INFINITY ? 0.f : ref) - WIDE_LIFT;
+                if (whole) add_odd(p, s.b, s.h, r, D, off, inv, p.out + (long long)row_of(p, s.b, s.h, r) * D);
+                else add_odd(p, s.b, s.h, r, D, off, 1.f, rec + 4);
+            }
             if (!whole) {
                 rec[0] = ref + (LIFT - WIDE_LIFT);
                 rec[1] = l;
@@ -707,7 +645,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
 }
 
 template <int D>
-__global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p) {
+__global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const __grid_constant__ TreeArgs p) {
     extern __shared__ uint8_t raw[];
     uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     const uint32_t base = smem_u32(smem), bars = base + Plan<D>::BAR_AT;
@@ -717,6 +655,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p)
     volatile int* odd = dead + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
+#pragma unroll 1
         for (int i = 0; i < L::RING; ++i) {
             bar_init(bars + 8 * (L::RAW + i), 1);
             bar_init(bars + 8 * (L::FULL + i), DECODE);
@@ -730,6 +669,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p)
         bar_init(bars + 8 * L::Q_FULL, SOFT);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         *dead = 0;
+#pragma unroll 1
         for (int i = 0; i < L::SEGMENTS; ++i) odd[i] = 0;
     }
     // (the memory is taken once the kernel in front is over: it might want some, and this one would hold it while it waits)
@@ -757,6 +697,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const TreeArgs p)
     __syncthreads();
     if (*dead) {
         // (never expected) products may still run: time for them to end before their memory is released
+#pragma unroll 1
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
         __syncthreads();
     }
@@ -785,7 +726,7 @@ struct KeysPlan {
 };
 
 template <int D>
-__global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const TreeArgs p, float* __restrict__ weights, int row0, int rows) {
+__global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_constant__ TreeArgs p, float* __restrict__ weights, int row0, int rows) {
     using L = KeysPlan<D>;
     extern __shared__ uint8_t raw[];
     uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
@@ -799,6 +740,7 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const TreeArgs
     const int groups = (rows + 255) >> 8;
     const bool has_tail = p.rest > 0;
     if (threadIdx.x == 0) {
+#pragma unroll 1
         for (int i = 0; i < L::RING; ++i) {
             bar_init(bars + 8 * (L::RAW + i), 1);
             bar_init(bars + 8 * (L::FULL + i), DECODE);
@@ -832,12 +774,14 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const TreeArgs
             s.at(p, tile, last);
             tile += s.c;
             soft_sync();                               // (all products with the queries before are over: their scores have been read)
+#pragma unroll 1
             for (int i = threadIdx.x; i < L::padded(rows) * (D / 8); i += 32 * SOFT) {
                 const int r = i / (D / 8), c = i % (D / 8);
                 const uint4 x = r < rows ? __ldg(reinterpret_cast<const uint4*>(p.q + (long long)row_of(p, s.b, s.h, row0 + r) * D) + c) : make_uint4(0, 0, 0, 0);
                 asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(base + L::Q_AT + (c >> 3) * q_half + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
                              "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
             }
+#pragma unroll 1
             for (int r = warp * 32; r < L::ROWS; r += 32 * SOFT) {
                 const float x = r + lane < rows ? p.lse[row_of(p, s.b, s.h, row0 + r + lane)] : -INFINITY;
                 const uint32_t none = __ballot_sync(0xFFFFFFFFu, x == -INFINITY);
@@ -957,6 +901,7 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const TreeArgs
     __syncwarp();
     __syncthreads();
     if (*dead) {
+#pragma unroll 1
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
         __syncthreads();
     }
