@@ -39,10 +39,11 @@ template <int D>
 struct Plan {
     static constexpr int RING = D == 128 ? 5 : 8;
     static constexpr int TILE_BYTES = TILE * D * 2, Q_HALF = 16384, Q_BYTES = Q_HALF * (D / 64);
-    static constexpr int RING_AT = 0, Q_AT = RING * TILE_BYTES;
-    // the second row group's queries; with one group the place where the slots' outputs are joined (128 rows x 64 channels)
-    static constexpr int JOIN_BYTES = 128 * 64 * 4, Q2_AT = Q_AT + Q_BYTES;
-    static constexpr int XM_AT = Q2_AT + (Q_BYTES > JOIN_BYTES ? Q_BYTES : JOIN_BYTES), XL_AT = XM_AT + 512;
+    // Two places for queries: of the two row groups, or of one group and, with one group, of the segment behind.  With one group the
+    // slots' outputs are joined (128 rows x 64 channels at a time) where the queries of the segment that ends were.
+    static constexpr int JOIN_BYTES = 128 * 64 * 4, Q_PLACE = Q_BYTES > JOIN_BYTES ? Q_BYTES : JOIN_BYTES;
+    static constexpr int RING_AT = 0, Q_AT = RING * TILE_BYTES, Q2_AT = Q_AT + Q_PLACE;
+    static constexpr int XM_AT = Q2_AT + Q_PLACE, XL_AT = XM_AT + 512;
     // barriers, 8 bytes each, then the tensor memory's address, the flag that a wait gave up, odd values of the last segments
     static constexpr int BAR_AT = XL_AT + 512, RAW = 0, FULL = RING, EMPTY = 2 * RING, S_FULL = 3 * RING, P_FULL = S_FULL + 2,
                          O_FULL = P_FULL + 2, Q_FULL = O_FULL + 2, BARS = Q_FULL + 1;
@@ -378,9 +379,9 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
         const int n_items = p.groups * s.c, tail_from = s.t0 + s.c == p.tiles ? n_items - p.groups : n_items;
 #pragma unroll 1
         for (int n = -2; n < n_items; ++n) {           // output of item n, scores of item n + 2
-            const uint32_t slot = n & 1, parity = (slot ? items1 : items0) & 1;
+            const uint32_t slot = n & 1;
             if (n >= 0) {
-                bar_wait(bars + 8 * (L::P_FULL + slot), parity, dead);
+                bar_wait(bars + 8 * (L::P_FULL + slot), (slot ? items1 : items0) & 1, dead);
                 if (one || !slot) take(v_at, v_buf);
                 fence_after();
                 const uint32_t v = operand(v_at, 8192), o = tmem + 256 + slot * 128, pr = tmem + slot * TILE;
@@ -397,12 +398,13 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
             }
             if (n + 2 >= n_items) continue;
             if (one || !slot) take(k_at, k_buf);
-            // (S takes P's place: the product that reads P has to be over)
-            if (n >= 0) bar_wait(bars + 8 * (L::O_FULL + slot), parity, dead);
+            // (S takes P's place: the product that reads P has to be over, that of the segment before too)
+            const uint32_t before = slot ? items1 : items0;
+            if (before) bar_wait(bars + 8 * (L::O_FULL + slot), (before - 1) & 1, dead);
             fence_after();
             // 16 channels: of Q and of the tail's keys 32 bytes of rows of 64 (K-major), of K's planes 16 rows of 64 tokens
             const bool tail = n + 2 >= tail_from;
-            const uint32_t q = operand(base + (!one && slot ? L::Q2_AT : L::Q_AT), 16), k = operand(k_at, tail ? 16 : D * 128);
+            const uint32_t q = operand(base + ((one ? seg & 1 : slot) ? L::Q2_AT : L::Q_AT), 16), k = operand(k_at, tail ? 16 : D * 128);
             const uint32_t near = tail ? 32 >> 4 : 2048 >> 4, far = tail ? 16384 >> 4 : 8192 >> 4;
             const uint32_t idesc = tail ? instruction(TILE, false) : instruction(TILE, true), d = tmem + slot * TILE;
             if (elect()) {
@@ -441,8 +443,27 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
     const uint32_t sign = p.scale2 < 0.f ? 0x80008000u : 0u;
     float* xm = reinterpret_cast<float*>(smem + Plan<D>::XM_AT);
     float* xl = reinterpret_cast<float*>(smem + Plan<D>::XL_AT);
+    // Queries of the segment that begins with `tile`, 16-byte piece c of a row's half at c ^ (row & 7).
+    auto queries = [&](int tile, int index) {
+        Segment s;
+        s.at(p, tile, last);
+        const int of_unit = group * p.rowsg + idx, r = s.super * p.rowsu + of_unit;
+        const bool mine = idx < p.rowsg && of_unit < p.rowsu && r < R;
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(mine ? row_of(p, s.b, s.h, r) : 0) * D);
+        const uint32_t to = base + ((p.groups == 2 ? group : index & 1) ? Plan<D>::Q2_AT : Plan<D>::Q_AT) + idx * 128;
+        const int c0 = p.groups == 1 ? slot * (D / 16) : 0, c1 = p.groups == 1 ? c0 + D / 16 : D / 8;
+#pragma unroll 4
+        for (int c = c0; c < c1; ++c) {
+            const uint4 x = mine ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+            sts128(to + (c >> 3) * Plan<D>::Q_HALF + (((c & 7) ^ (idx & 7)) << 4), make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign));
+        }
+        fence_shared();
+        __syncwarp();
+        if (lane == 0) bar_arrive(bars + 8 * Plan<D>::Q_FULL);
+    };
     uint32_t done = 0;
     int seg = 0;
+    queries(first, 0);
     for (int tile = first; tile < last; ++seg) {
         Segment s;
         s.at(p, tile, last);
@@ -450,27 +471,12 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
         const int of_unit = group * p.rowsg + idx, r = s.super * p.rowsu + of_unit;
         const bool mine = idx < p.rowsg && of_unit < p.rowsu && r < R;
         const bool busy = __any_sync(0xFFFFFFFFu, mine);
-        // queries: 16-byte piece c of a row's half at c ^ (row & 7)
-        soft_sync();
-        {
-            const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(mine ? row_of(p, s.b, s.h, r) : 0) * D);
-            const uint32_t to = base + (group ? Plan<D>::Q2_AT : Plan<D>::Q_AT) + idx * 128;
-            const int c0 = p.groups == 1 ? slot * (D / 16) : 0, c1 = p.groups == 1 ? c0 + D / 16 : D / 8;
-#pragma unroll 1
-            for (int c = c0; c < c1; ++c) {
-                uint4 x = mine ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(to + (c >> 3) * Plan<D>::Q_HALF + (((c & 7) ^ (idx & 7)) << 4)),
-                             "r"(x.x ^ sign), "r"(x.y ^ sign), "r"(x.z ^ sign), "r"(x.w ^ sign) : "memory");
-            }
-            fence_shared();
-            __syncwarp();
-            if (lane == 0) bar_arrive(bars + 8 * Plan<D>::Q_FULL);
-        }
+        soft_sync();                                   // (the join of the segment before has been read)
         const bool with_tail = s.t0 + s.c == p.tiles;
         unsigned long long seen = 0;
         if (with_tail && mine) {
             const uint8_t* row = p.tree + s.b * p.tree_stride + (unsigned)r / (unsigned)p.G * p.T;
-#pragma unroll 1
+#pragma unroll 8
             for (int d = 0; d < p.T; ++d) seen |= (unsigned long long)(row[d] != 0) << d;
         }
         const __half* mask = p.mask ? p.mask + s.b * p.mask_stride : nullptr;
@@ -552,6 +558,9 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
             __syncwarp();
             if (lane == 0) bar_arrive(bars + 8 * (Plan<D>::P_FULL + slot));
         }
+        // (this slot's products with the queries are over - with one group the next ones have a place of their own - while its last
+        // output is still under way)
+        if (tile < last) queries(tile, seg + 1);
         // ---- the segment's result: with one group the slots' two, joined
         const bool have = n_items > slot;
         if (have) bar_wait(bars + 8 * (Plan<D>::O_FULL + slot), (done - 1) & 1, dead);
@@ -578,7 +587,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int rec_slot = s.unit != (unsigned)first / (unsigned)p.tiles;
         float* rec = p.part + (size_t)((2 * blockIdx.x + rec_slot) * p.rowsu + of_unit) * (D + 4);
-        float4* join = reinterpret_cast<float4*>(smem + Plan<D>::Q2_AT);              // [16 channel quads][128 rows]
+        float4* join = reinterpret_cast<float4*>(smem + (seg & 1 ? Plan<D>::Q2_AT : Plan<D>::Q_AT));              // [16 channel quads][128 rows]
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
             if (p.groups == 1 && c % 64 == 0) {
@@ -774,7 +783,7 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_c
             s.at(p, tile, last);
             tile += s.c;
             soft_sync();                               // (all products with the queries before are over: their scores have been read)
-#pragma unroll 1
+#pragma unroll 4
             for (int i = threadIdx.x; i < L::padded(rows) * (D / 8); i += 32 * SOFT) {
                 const int r = i / (D / 8), c = i % (D / 8);
                 const uint4 x = r < rows ? __ldg(reinterpret_cast<const uint4*>(p.q + (long long)row_of(p, s.b, s.h, row0 + r) * D) + c) : make_uint4(0, 0, 0, 0);
