@@ -445,47 +445,70 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
     }
 }
 
-// One warp per query row: the records of the runs that share its unit, in the order of the tokens.
+// One warp per query row: the records of the runs that share its unit, in the order of the tokens, eight under way at a time.  Bound by
+// latency: where the row lies is worked out before the kernel in front has ended.
 template <int D>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeArgs p) {
-    pdl_enter();
+    pdl_trigger();
+    constexpr int C = D / 32, STEP = 8;                 // channels of a lane
     const int lane = threadIdx.x & 31;
     const int row = blockIdx.x * 4 + (threadIdx.x >> 5);                        // unit * rowsu + row of the unit
     const int unit = (unsigned)row / (unsigned)p.rowsu, of_unit = row - unit * p.rowsu;
     const int bh = (unsigned)unit / (unsigned)p.rt, b = (unsigned)bh / (unsigned)p.H, h = bh - b * p.H;
-    if ((unsigned)unit >= (unsigned)p.total / (unsigned)p.tiles) return;
     const int r = (unit - bh * p.rt) * p.rowsu + of_unit;
-    if (r >= p.T * p.G) return;
     const int w0 = run_with(p, unit * p.tiles), w1 = run_with(p, unit * p.tiles + p.tiles - 1);
-    if (w0 == w1) return;                                                       // a whole unit: written by its run
+    const long long to = row_of(p, b, h, r);
     // a run's record of its first unit is in slot 0, of its last in slot 1: only the first of this unit's may have begun before it
-    const int slot0 = run_start(p, w0) < unit * p.tiles;
-    auto record = [&](int w) {
-        return p.part + (size_t)((2 * w + (w == w0 ? slot0 : 0)) * p.rowsu + of_unit) * (D + 4);
-    };
-    float top = -INFINITY;
-    for (int w = w0 + lane; w <= w1; w += 32) top = fmaxf(top, record(w)[0]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    const float base = top == -INFINITY ? 0.f : top;
-    constexpr int C = D / 32;
-    float acc[C], l = 0.f;
+    const float* rec = p.part + (size_t)(2 * w0 * p.rowsu + of_unit) * (D + 4);
+    const size_t pitch = (size_t)2 * p.rowsu * (D + 4);
+    const float* rec0 = run_start(p, w0) < unit * p.tiles ? rec + pitch / 2 : rec;
+    pdl_wait();
+    // (a whole unit has been written by its run)
+    if ((unsigned)unit >= (unsigned)p.total / (unsigned)p.tiles || r >= p.T * p.G || w0 == w1) return;
+    float acc[C], l = 0.f, top = -INFINITY;
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = 0.f;
-#pragma unroll 4
-    for (int w = w0; w <= w1; ++w) {
-        const float* rec = record(w);
-        const float f = ex2(rec[0] - base);
-        l = fmaf(f, rec[1], l);
+#pragma unroll 1
+    for (int w = w0; w <= w1; w += STEP) {
+        float2 ml[STEP];
+        float o[STEP][C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) acc[c] = fmaf(f, rec[4 + C * lane + c], acc[c]);
+        for (int k = 0; k < STEP; ++k) {
+            const float* x = w + k == w0 ? rec0 : rec + (w + k - w0) * pitch;
+            ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int c = 0; c < C; ++c) o[k][c] = 0.f;
+            if (w + k > w1) continue;
+            ml[k] = *reinterpret_cast<const float2*>(x);
+            if constexpr (C == 4) {
+                const float4 y = *reinterpret_cast<const float4*>(x + 4 + 4 * lane);
+                o[k][0] = y.x; o[k][1] = y.y; o[k][2] = y.z; o[k][3] = y.w;
+            } else {
+                const float2 y = *reinterpret_cast<const float2*>(x + 4 + 2 * lane);
+                o[k][0] = y.x; o[k][1] = y.y;
+            }
+        }
+        float t = top;
+#pragma unroll
+        for (int k = 0; k < STEP; ++k) t = fmaxf(t, ml[k].x);
+        const float base = t == -INFINITY ? 0.f : t, keep = ex2(top - base);
+        top = t;
+        l *= keep;
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] *= keep;
+#pragma unroll
+        for (int k = 0; k < STEP; ++k) {
+            const float f = ex2(ml[k].x - base);
+            l = fmaf(f, ml[k].y, l);
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[c] = fmaf(f, o[k][c], acc[c]);
+        }
     }
-    const long long to = row_of(p, b, h, r);
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int c = 0; c < C; c += 2)
         *reinterpret_cast<uint32_t*>(p.out + to * D + C * lane + c) = pack_half2(acc[c] * inv, acc[c + 1] * inv);
-    if (p.lse && lane == 0) p.lse[to] = l == 0.f ? -INFINITY : (base - LIFT + log2f(l)) * LN2;
+    if (p.lse && lane == 0) p.lse[to] = l == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) - LIFT + log2f(l)) * LN2;
 }
 
 // Warps for `total` tiles: one an SM while there are that few, then up to eight.
