@@ -90,7 +90,7 @@ struct EvictArgs {
     uint8_t *k8, *km, *kl, *v8, *vm, *vl;
     int *holes, *movers, *start;       // [rows][most] twice; [rows][keep / 64 + 1]: free places in front of each block's
     int D, L, nmb, n, rest, keep, recent, arranged, shift, most;
-    int share;                         // places of a CTA of select_kernel's cluster, a multiple of SEL_NT
+    int share;                         // places of a CTA of select_kernel's cluster, a multiple of its threads
     int held;                          // whether their keys are kept in shared memory
 };
 
@@ -112,8 +112,10 @@ __device__ __forceinline__ uint32_t cluster_ld(const void* p, uint32_t cta) {
 // counted.  The keep-th largest key by four counts of eight bits (in eight columns: few lanes of a warp meet, although weights crowd into
 // few exponents), added up over the cluster through distributed shared memory; every CTA draws the same
 // conclusion.  Then ties, free places and survivors behind are numbered in order: per warp, per CTA, per cluster.
-constexpr int SEL_NT = 1024, SEL_W = SEL_NT / 32, SEL_MOST = 40960;      // SEL_MOST: keys a CTA can keep
+constexpr int SEL_MOST = 40960, SEL_CTAS = 8;      // keys a CTA can keep, CTAs of a row
+template <int SEL_NT>
 __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
+    constexpr int SEL_W = SEL_NT / 32;
     extern __shared__ __align__(16) uint32_t keys[];
     __shared__ int hist[8 * 257];                  // [column][digit], columns a bank apart
     __shared__ uint32_t sums[2][256];              // this CTA's counts: two buffers, so that one barrier a round is enough
@@ -130,8 +132,23 @@ __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
     const int first = min((int)rank * a.share, a.n), count = min(a.share, a.n - first);
     auto key = [&](int i) { return key_of(w[first + i], a.recent && position_of(a, pos, first + i) >= safe_from); };
     if (a.held) {
-#pragma unroll 8
-        for (int i = tid; i < count; i += SEL_NT) keys[i] = key(i);
+        // (eight at a time: all weights requested, then the positions that matter, then used)
+#pragma unroll 1
+        for (int i0 = tid; i0 < count; i0 += 8 * SEL_NT) {
+            float x[8];
+            int at[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = i0 + j * SEL_NT < count ? w[first + i0 + j * SEL_NT] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = first + i0 + j * SEL_NT;
+                at[j] = i + a.shift;
+                if (a.recent && i < a.arranged && i0 + j * SEL_NT < count) at[j] = pos[i];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (i0 + j * SEL_NT < count) keys[i0 + j * SEL_NT] = key_of(x[j], a.recent && at[j] >= safe_from);
+        }
     }
     auto at = [&](int i) { return a.held ? keys[i] : key(i); };
     uint32_t prefix = 0;
@@ -186,13 +203,13 @@ __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
         if (lane == 0) scan[s][warp] = mine;
         __syncthreads();
         if (warp == 0) {
-            uint32_t x = scan[s][lane], y = x;
+            uint32_t x = lane < SEL_W ? scan[s][lane] : 0, y = x;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint32_t z = __shfl_up_sync(0xFFFFFFFFu, y, o);
                 if (lane >= o) y += z;
             }
-            scan[s][lane] = y - x;
+            if (lane < SEL_W) scan[s][lane] = y - x;
             if (lane == 31) scan[s][SEL_W] = y;
         }
         __syncthreads();
@@ -253,12 +270,12 @@ __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
 // CTA = one block of 64 places in front of `keep`: its free places take the survivors of the same numbers.  Survivors are read
 // only behind `keep` and places are written only in front of it, each by its own CTA: no order among the CTAs.
 // K, token-minor: one survivor is a byte of each of D rows and half a byte of 2 D.  The block and the blocks that its survivors come
-// from are put together to fp16 rows [channel][64 tokens] in shared memory, two of the latter at a time; a warp takes a channel, a lane
+// from are put together to fp16 rows [channel][64 tokens] in shared memory, the latter one after the other; a warp takes a channel, a lane
 // two neighbouring places, a survivor's value is one 2-byte load and store; at the end the block is split again.  (On the plane bytes
 // themselves that were three loads and, with the neighbour's nibble in the same byte, more than one store per value: shared memory's
 // pipe was 69% busy at 142 us for 8 x 32 x 4096 tokens to 2048.)  V: rows of 16-byte pieces through registers.
 // Floor: the block twice, the blocks behind once, V's rows twice.
-constexpr int MOVE_NT = 256, STAGED = 2;
+constexpr int MOVE_NT = 256, STAGED = 1;
 template <int D>
 __global__ void __launch_bounds__(MOVE_NT) move_kernel(const EvictArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];     // blocks of [D] rows of 128 bytes, 16-byte piece q of row c at q ^ (c & 1)
@@ -312,14 +329,16 @@ __global__ void __launch_bounds__(MOVE_NT) move_kernel(const EvictArgs a) {
 #pragma unroll
     for (int e = 0; e < STAGED; ++e)
         if (b0 + e <= b1) load(other[e], b0 + e);
+    // V: thread = one 16-byte piece, of which plane is the same for all rows
+    const int piece = tid % PIECES, j0 = tid / PIECES;
+    const int pitch = piece < D / 16 ? D : D / 2;
+    uint8_t* vp = (piece < D / 16 ? a.v8 + piece * 16 : piece < D * 3 / 32 ? a.vm + (piece - D / 16) * 16 : a.vl + (piece - D * 3 / 32) * 16) +
+                  row * a.L * pitch;
     uint4 v[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-        const int i = tid + e * MOVE_NT, j = i / PIECES, c = i % PIECES;
-        if (j >= m) continue;
-        const size_t s = row * a.L + src[j];
-        v[e] = *reinterpret_cast<const uint4*>(c < D / 16 ? a.v8 + s * D + c * 16 : c < D * 3 / 32 ? a.vm + s * (D / 2) + (c - D / 16) * 16
-                                                                                           : a.vl + s * (D / 2) + (c - D * 3 / 32) * 16);
+        const int j = j0 + e * (MOVE_NT / PIECES);
+        if (j < m) v[e] = *reinterpret_cast<const uint4*>(vp + (size_t)src[j] * pitch);
     }
     put(mine, 0);
     const int s0 = from[2 * lane], s1 = from[2 * lane + 1], swap = (warp & 1) << 4;      // (a warp's channels are all odd or all even)
@@ -344,11 +363,8 @@ __global__ void __launch_bounds__(MOVE_NT) move_kernel(const EvictArgs a) {
     }
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-        const int i = tid + e * MOVE_NT, j = i / PIECES, c = i % PIECES;
-        if (j >= m) continue;
-        const size_t d = row * a.L + to[j];
-        *reinterpret_cast<uint4*>(c < D / 16 ? a.v8 + d * D + c * 16 : c < D * 3 / 32 ? a.vm + d * (D / 2) + (c - D / 16) * 16
-                                                                                : a.vl + d * (D / 2) + (c - D * 3 / 32) * 16) = v[e];
+        const int j = j0 + e * (MOVE_NT / PIECES);
+        if (j < m) *reinterpret_cast<uint4*>(vp + (size_t)to[j] * pitch) = v[e];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -386,14 +402,16 @@ __global__ void __launch_bounds__(256) clear_kernel(const EvictArgs a) {
     }
 }
 
-int launch_select(const EvictArgs& a, int rows, int ctas, cudaStream_t st) {
+// Threads: 512 where a CTA has few keys, so that two rows share an SM; 1024 for long ones.
+int launch_select(const EvictArgs& a, int rows, int ctas, int threads, cudaStream_t st) {
     const size_t smem = a.held ? (size_t)a.share * 4 : 0;
-    int rc = cuda_status(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MOST * 4),
+    auto kernel = threads == 512 ? select_kernel<512> : select_kernel<1024>;
+    int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MOST * 4),
                          "evict select shared memory");
     if (rc != AKV_OK) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, rows);
-    cfg.blockDim = dim3(SEL_NT);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
@@ -405,7 +423,7 @@ int launch_select(const EvictArgs& a, int rows, int ctas, cudaStream_t st) {
     cfg.attrs = at;
     cfg.numAttrs = tuning().pdl ? 2 : 1;
     count_launch();
-    rc = cuda_status(cudaLaunchKernelEx(&cfg, select_kernel, a), "evict select launch");
+    rc = cuda_status(cudaLaunchKernelEx(&cfg, kernel, a), "evict select launch");
     return rc;
 }
 
@@ -505,10 +523,11 @@ int akv_evict(const akv_layer* layer, void* weights, void* positions, int rest_l
     // CTAs of a row: so many that all SMs have some and none has less than two thousand places, at most eight (what a cluster may
     // have everywhere)
     int ctas = 1;
-    while (ctas < 8 && ((rest_start + ctas - 1) / ctas > SEL_MOST || (rows * ctas < sm_count() && rest_start / ctas > 2 * SEL_NT))) ctas *= 2;
-    a.share = ((rest_start + ctas - 1) / ctas + SEL_NT - 1) / SEL_NT * SEL_NT;
+    while (ctas < SEL_CTAS && ((rest_start + ctas - 1) / ctas > SEL_MOST || (rows * ctas < sm_count() && rest_start / ctas > 2048))) ctas *= 2;
+    const int threads = (rest_start + ctas - 1) / ctas > 8192 ? 1024 : 512;
+    a.share = ((rest_start + ctas - 1) / ctas + threads - 1) / threads * threads;
     a.held = a.share <= SEL_MOST;
-    if ((rc = launch_select(a, rows, ctas, st)) != AKV_OK || keep == rest_start) return rc;
+    if ((rc = launch_select(a, rows, ctas, threads, st)) != AKV_OK || keep == rest_start) return rc;
     const size_t smem = (size_t)(1 + STAGED) * l.head_dim * 128;
     auto move = l.head_dim == 128 ? move_kernel<128> : move_kernel<64>;
     rc = cuda_status(cudaFuncSetAttribute(move, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "evict shared memory");
