@@ -16,63 +16,85 @@ constexpr int BLK = 64;
 // ------------------------------------------------------------------ accepted path
 // CTA = (batch, KV head) and one of K, V.  Rows in front of the accepted tokens: the residual buffer.  The two together are at most
 // 127 rows: one block fills up at most, its rows go to the planes, and the rows behind it begin the next residual block.
-__global__ void __launch_bounds__(256)
+// All rows that matter are requested at once and staged in shared memory; maxima, planes and residual rows are made from there.
+// Bound by latency: one load, one barrier, one store.  (Maxima read row after row from global memory took 29 us at 512 heads and 48
+// tokens.)
+constexpr int COMMIT_NT = 256;
+template <int D>
+__global__ void __launch_bounds__(COMMIT_NT)
 commit_kernel(uint8_t* __restrict__ f8, uint8_t* __restrict__ m4, uint8_t* __restrict__ l4, uint8_t* __restrict__ vf8,
               uint8_t* __restrict__ vm4, uint8_t* __restrict__ vl4, uint16_t* __restrict__ k_exp, uint16_t* __restrict__ v_exp,
               uint8_t* restk, uint8_t* restv, const uint8_t* __restrict__ kd, const uint8_t* __restrict__ vd,
-              const int* __restrict__ path, int H, int D, int T, int n, int rest, int qn, int nmb, int L) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int node[BLK];
+              const int* __restrict__ path, int H, int T, int n, int rest, int qn, int nmb, int L) {
+    constexpr int PITCH = 2 * D, VEC = D / 8, HD = D / 2;
+    extern __shared__ __align__(16) uint8_t rows[];     // [row from `first` on][D] fp16
+    __shared__ uint32_t part[COMMIT_NT];
     pdl_enter();
-    const int bh = blockIdx.x, b = bh / H, h = bh - b * H, tid = threadIdx.x;
-    const bool value = blockIdx.y;
+    const int bh = blockIdx.x, b = (unsigned)bh / (unsigned)H, h = bh - b * H, tid = threadIdx.x;
+    const bool value = blockIdx.y, full = rest + n >= BLK;
     uint8_t* buffer = value ? restv : restk;
     const uint8_t* drafted = value ? vd : kd;
-    if (tid < n) node[tid] = min(max(path[(size_t)b * n + tid], 0), T - 1);
-    __syncthreads();
-    const size_t pitch = 2 * (size_t)D;
-    auto slot = [&](int i) { return buffer + (((size_t)b * BLK + i) * H + h) * pitch; };
-    auto fresh = [&](int i) { return drafted + (((size_t)b * T + node[i]) * H + h) * pitch; };
-    // exponent maxima, two channels a word
-    uint16_t* top = (value ? v_exp : k_exp) + (size_t)bh * (D >> 1);
-    for (int c = tid; c < (D >> 1); c += blockDim.x) {
-        uint32_t m = top[c];
-        for (int i = 0; i < n; ++i) {
-            const uint32_t w = reinterpret_cast<const uint32_t*>(fresh(i))[c];
-            m = __vmaxu4(m, ((w >> 10) & 0x1Fu) | (((w >> 26) & 0x1Fu) << 8));
-        }
-        top[c] = (uint16_t)m;
+    const int first = full ? 0 : rest, count = rest + n - first;      // (without a full block the residual rows stay where they are)
+    auto slot = [&](int i) { return buffer + ((size_t)(b * BLK + i) * H + h) * PITCH; };
+#pragma unroll 4
+    for (int i = tid; i < count * VEC; i += COMMIT_NT) {
+        const int r = first + i / VEC, v = i % VEC;
+        // (a node outside the tree is clamped into it; rows of the residual buffer are written further down: no read-only loads)
+        const uint8_t* src = r < rest ? slot(r)
+                                      : drafted + ((size_t)(b * T + min(max(path[b * n + r - rest], 0), T - 1)) * H + h) * PITCH;
+        *reinterpret_cast<uint4*>(rows + i * 16) = *(reinterpret_cast<const uint4*>(src) + v);
     }
-    int done = 0, at = rest;                           // accepted tokens that have gone, row of the next
-    if (rest + n >= BLK) {
-        auto row = [&](int i) { return i < rest ? static_cast<const uint8_t*>(slot(i)) : fresh(i - rest); };
-        // (rows of the residual buffer are read and, further down, written: no read-only loads)
-        const int vec = (int)(pitch >> 4);
-        for (int i = tid; i < BLK * vec; i += blockDim.x) {
-            const int r = i / vec, v = i - r * vec;
-            reinterpret_cast<uint4*>(smem + r * pitch)[v] = reinterpret_cast<const uint4*>(row(r))[v];
-        }
-        __syncthreads();
-        if (!value) {
-            k_emit_block64<false, true>(smem, f8, m4, l4, (long long)bh * nmb + qn / BLK, D, nullptr);
-        } else {
-            const int per = D >> 5;
-            for (int i = tid; i < BLK * per; i += blockDim.x) {
-                const int r = i / per, c = i - r * per;
-                const uint4* src = reinterpret_cast<const uint4*>(smem + r * pitch + c * 64);
+    __syncthreads();
+    // exponent maxima, two channels a word, the tokens dealt to COMMIT_NT / HD shares
+    uint32_t m = 0;
+    for (int i = rest - first + tid / HD; i < count; i += COMMIT_NT / HD) {
+        const uint32_t w = reinterpret_cast<const uint32_t*>(rows + i * PITCH)[tid % HD];
+        m = __vmaxu4(m, ((w >> 10) & 0x1Fu) | (((w >> 26) & 0x1Fu) << 8));
+    }
+    part[tid] = m;
+    __syncthreads();
+    if (tid < HD) {
+        uint16_t* top = (value ? v_exp : k_exp) + (size_t)bh * HD + tid;
+#pragma unroll
+        for (int j = 1; j < COMMIT_NT / HD; ++j) m = __vmaxu4(m, part[j * HD + tid]);
+        *top = (uint16_t)__vmaxu4(m, *top);
+    }
+    if (full) {
+        const size_t block = (size_t)bh * nmb + qn / BLK;
+        for (int i = tid; i < 2 * D; i += COMMIT_NT) {
+            if (!value) {
+                // 32 tokens of a channel
+                const int c = i % D, t0 = i / D * 32;
+                uint4 hi[2], mid, low;
+                uint32_t *hw = reinterpret_cast<uint32_t*>(hi), *mw = reinterpret_cast<uint32_t*>(&mid), *lw = reinterpret_cast<uint32_t*>(&low);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint8_t* x = rows + (t0 + 8 * g + 2 * j) * PITCH + 2 * c;
+                        w[j] = *reinterpret_cast<const uint16_t*>(x) | (uint32_t)*reinterpret_cast<const uint16_t*>(x + PITCH) << 16;
+                    }
+                    v_split4(w[0], w[1], w[2], w[3], hw[2 * g], hw[2 * g + 1], mw[g], lw[g]);
+                }
+                uint4* f = reinterpret_cast<uint4*>(f8 + (block * D + c) * BLK + t0);
+                f[0] = hi[0];
+                f[1] = hi[1];
+                *reinterpret_cast<uint4*>(m4 + (block * D + c) * (BLK / 2) + t0 / 2) = mid;
+                *reinterpret_cast<uint4*>(l4 + (block * D + c) * (BLK / 2) + t0 / 2) = low;
+            } else {
+                // 32 channels of a token
+                const int r = i / (D / 32), c = i % (D / 32);
+                const uint4* src = reinterpret_cast<const uint4*>(rows + r * PITCH + c * 64);
                 const size_t to = (size_t)bh * L + qn + r;
-                v_write32(src[0], src[1], src[2], src[3], vf8 + to * D + c * 32, vm4 + to * (D >> 1) + c * 16,
-                          vl4 + to * (D >> 1) + c * 16);
+                v_write32(src[0], src[1], src[2], src[3], vf8 + to * D + c * 32, vm4 + to * HD + c * 16, vl4 + to * HD + c * 16);
             }
         }
-        done = BLK - rest;
-        at = 0;
     }
-    const int vec = (int)(pitch >> 4);
-    for (int i = tid; i < (n - done) * vec; i += blockDim.x) {
-        const int r = i / vec, v = i - r * vec;
-        reinterpret_cast<uint4*>(slot(at + r))[v] = reinterpret_cast<const uint4*>(fresh(done + r))[v];
-    }
+    const int from = full ? BLK : rest - first;         // staged row that goes to residual row `at`
+    const int at = full ? 0 : rest;
+    for (int i = tid; i < (count - from) * VEC; i += COMMIT_NT)
+        reinterpret_cast<uint4*>(slot(at + i / VEC))[i % VEC] = *reinterpret_cast<const uint4*>(rows + from * PITCH + i * 16);
 }
 
 // ------------------------------------------------------------------ eviction
@@ -462,14 +484,14 @@ int akv_tree_commit(const akv_layer* layer, const void* k_new, const void* v_new
     AKV_REQUIRE(aligned16(k_new) && aligned16(v_new) && aligned16(a.restk) && aligned16(a.restv) && aligned16(a.k_exp_max) &&
                 aligned16(a.v_exp_max) && (reinterpret_cast<uintptr_t>(path) & 3u) == 0, AKV_ERR_ALIGN,
                 "tree_commit: pointers must be 16-byte aligned");
-    const int D = a.head_dim;
-    launch_chained(commit_kernel, dim3(a.bsz * a.n_kv_heads, 2), dim3(256), rest_len + accepted >= BLK ? (size_t)BLK * 2 * D : 0,
-                   static_cast<cudaStream_t>(stream), static_cast<uint8_t*>(a.k_first_8), static_cast<uint8_t*>(a.k_mid_4),
-                   static_cast<uint8_t*>(a.k_last_4), static_cast<uint8_t*>(a.v_first_8), static_cast<uint8_t*>(a.v_mid_4),
-                   static_cast<uint8_t*>(a.v_last_4), static_cast<uint16_t*>(a.k_exp_max), static_cast<uint16_t*>(a.v_exp_max),
-                   static_cast<uint8_t*>(a.restk), static_cast<uint8_t*>(a.restv), static_cast<const uint8_t*>(k_new),
-                   static_cast<const uint8_t*>(v_new), static_cast<const int*>(path), a.n_kv_heads, D, drafted, accepted, rest_len,
-                   rest_start, (a.max_seq_len + BLK - 1) / BLK, a.max_seq_len);
+    const int D = a.head_dim, staged = rest_len + accepted >= BLK ? rest_len + accepted : accepted;
+    launch_chained(D == 128 ? commit_kernel<128> : commit_kernel<64>, dim3(a.bsz * a.n_kv_heads, 2), dim3(COMMIT_NT),
+                   (size_t)staged * 2 * D, static_cast<cudaStream_t>(stream), static_cast<uint8_t*>(a.k_first_8),
+                   static_cast<uint8_t*>(a.k_mid_4), static_cast<uint8_t*>(a.k_last_4), static_cast<uint8_t*>(a.v_first_8),
+                   static_cast<uint8_t*>(a.v_mid_4), static_cast<uint8_t*>(a.v_last_4), static_cast<uint16_t*>(a.k_exp_max),
+                   static_cast<uint16_t*>(a.v_exp_max), static_cast<uint8_t*>(a.restk), static_cast<uint8_t*>(a.restv),
+                   static_cast<const uint8_t*>(k_new), static_cast<const uint8_t*>(v_new), static_cast<const int*>(path),
+                   a.n_kv_heads, drafted, accepted, rest_len, rest_start, (a.max_seq_len + BLK - 1) / BLK, a.max_seq_len);
     return cuda_status(cudaGetLastError(), "tree_commit launch");
 }
 

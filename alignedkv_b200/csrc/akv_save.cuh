@@ -54,8 +54,8 @@ __device__ __forceinline__ void stage_tile64(uint8_t* smem, RowPtr row, int D, i
 
 // Emit one K block from a staged tile (see k_write_block64).  MAXOUT: also return, per channel, the signed maximum
 // over the 64 tokens as fp16 bits in max_out[d] (the prompt's exponent maxima use the signed maximum,
-// extension/k_cache_file.py:77-78).  STORE: the nibbles are stored, not added (a block that nothing was written to).
-template <bool MAXOUT, bool STORE = false>
+// extension/k_cache_file.py:77-78).
+template <bool MAXOUT>
 __device__ __forceinline__ void k_emit_block64(const uint8_t* smem, uint8_t* __restrict__ first8,
                                                uint8_t* __restrict__ mid4, uint8_t* __restrict__ last4, long long tile,
                                                int D, uint16_t* max_out) {
@@ -65,12 +65,7 @@ __device__ __forceinline__ void k_emit_block64(const uint8_t* smem, uint8_t* __r
         // the nibble rows this thread adds onto: requested before the gather so that their latency overlaps it
         uint4* mdst = reinterpret_cast<uint4*>(mid4 + (tile * D + d) * (DB / 2));
         uint4* ldst = reinterpret_cast<uint4*>(last4 + (tile * D + d) * (DB / 2));
-        uint4 om[2], ol[2];
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            om[v] = STORE ? make_uint4(0, 0, 0, 0) : mdst[v];
-            ol[v] = STORE ? make_uint4(0, 0, 0, 0) : ldst[v];
-        }
+        uint4 om[2] = {mdst[0], mdst[1]}, ol[2] = {ldst[0], ldst[1]};
         uint32_t f[16], m[8], l[8];
         float mx = -INFINITY;
 #pragma unroll
