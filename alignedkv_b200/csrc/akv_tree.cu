@@ -35,7 +35,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool th
 //   tail      16 tokens of the tail as fp16 rows [token][D]: a K step, then their V step
 // The 16-byte pieces of a 128-byte line are swapped by XOR so that a quarter (half) warp's 16-byte (8-byte) loads of a line's
 // pieces by lane (g, t) fall into different banks.
-constexpr int STEPS = 5, STEP_BYTES = 4096;
+constexpr int STEPS = 4, STEP_BYTES = 4096;
 
 constexpr int WARP_BYTES = STEPS * STEP_BYTES + 8192;            // the ring, query fragments, probabilities
 

@@ -476,7 +476,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
         unsigned long long seen = 0;
         if (with_tail && mine) {
             const uint8_t* row = p.tree + s.b * p.tree_stride + (unsigned)r / (unsigned)p.G * p.T;
-#pragma unroll 8
+#pragma unroll 16
             for (int d = 0; d < p.T; ++d) seen |= (unsigned long long)(row[d] != 0) << d;
         }
         const __half* mask = p.mask ? p.mask + s.b * p.mask_stride : nullptr;
