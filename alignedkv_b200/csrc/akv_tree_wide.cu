@@ -141,15 +141,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) 
                  ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
                    "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
-__device__ __forceinline__ void tmem_ld8(uint32_t (&v)[8], uint32_t at) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(at) : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
-                 ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
-}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void soft_sync() {
     __syncwarp();
@@ -186,6 +177,20 @@ __device__ __forceinline__ int tile_of(int q, int c, int ahead, bool& value) {
     const int r = q - ahead, pairs = 2 * (c - ahead);
     value = r >= pairs || !(r & 1);
     return r >= pairs ? (c - ahead) + (r - pairs) : value ? r >> 1 : (r >> 1) + ahead;
+}
+
+// What a plane tile's mask leaves of it: a padded batch has tiles of all tokens and of none, and few others.  By a warp.
+enum Masked { ALL, SOME, NONE };
+__device__ __forceinline__ Masked mask_of(const __half* mask, int count, int lane) {
+    bool zero = true, gone = true;
+#pragma unroll
+    for (int e = 0; e < TILE; e += 32) {
+        if (lane + e >= count) continue;
+        const uint32_t x = reinterpret_cast<const uint16_t*>(mask)[lane + e];
+        zero = zero && !(x & 0x7FFFu);
+        gone = gone && x == 0xFC00u;
+    }
+    return __all_sync(0xFFFFFFFFu, zero) ? ALL : __all_sync(0xFFFFFFFFu, gone) ? NONE : SOME;
 }
 
 // ---------------------------------------------------------------- decode
@@ -298,6 +303,8 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t ring_at,
             bool value = false;
             const int i = s.t0 + (KEYS ? q : tile_of(q, s.c, 3 - p.groups, value));
             const uint32_t slot = ring_at + buf * L::TILE_BYTES;
+            const int some = p.nb * BLK - i * TILE;    // (the tail's: none, or an odd block's)
+            const Masked left = value && p.mask && some > 0 ? mask_of(p.mask + s.b * p.mask_stride + i * TILE, some, lane) : ALL;
             bar_wait(bars + 8 * (L::RAW + buf), turn & 1, dead);
             if (has_tail && i == p.tiles - 1) {
                 if (tail_share<D>(p, s.b, s.h, value, slot, warp, lane) && !KEYS) odd[index % L::SEGMENTS] = index + 1;
@@ -325,14 +332,13 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t ring_at,
                     sts128(f, halves8(w[u][0], w[u][1], w[u][4], w[u][6]));
                     sts128(f ^ 16, halves8(w[u][2], w[u][3], w[u][5], w[u][7]));
                 }
-                const int some = p.nb * BLK - i * TILE;
-                if (some < TILE || (value && p.mask)) {
+                if (some < TILE || left != ALL) {
                     // (a token that does not exist or is masked away counts as zero, whatever there is: 0 * NaN would be NaN)
-                    const uint16_t* mask = value && p.mask ? reinterpret_cast<const uint16_t*>(p.mask) + s.b * p.mask_stride + i * TILE : nullptr;
+                    const uint16_t* mask = left == SOME ? reinterpret_cast<const uint16_t*>(p.mask) + s.b * p.mask_stride + i * TILE : nullptr;
 #pragma unroll 1
                     for (int u = 0; u < U; ++u) {
                         const int tok = region * BLK + (value ? (D == 128 ? u >> 1 : u) * 32 + kr : 0);
-                        if (tok >= some || (mask && mask[tok] == 0xFC00u)) {
+                        if (tok >= some || left == NONE || (mask && mask[tok] == 0xFC00u)) {
                             const uint32_t f = (u & 1 ? f1 : f0) + (u >> 1) * 4096;
                             sts128(f, make_uint4(0, 0, 0, 0));
                             sts128(f ^ 16, make_uint4(0, 0, 0, 0));
@@ -420,20 +426,6 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
 }
 
 // ---------------------------------------------------------------- softmax
-// What a row of the tail sees of it, and scores at the edges: x = score to base 2 of tile token `tok`, or -inf.
-struct Edge {
-    const __half* mask;         // of the tile's first token, or nullptr
-    int count, rest;            // tokens of the tile; of them cached (the others are drafted)
-    unsigned long long seen;    // drafted tokens that the row sees
-    __device__ __forceinline__ float operator()(float x, float scale2, int tok) const {
-        if (tok < rest) {
-            const float add = mask ? __half2float(mask[tok]) : 0.f;
-            return add == -INFINITY ? -INFINITY : fmaf(x, scale2, add * LOG2E);
-        }
-        return tok < count && (seen >> ((tok - rest) & 63) & 1) ? x * scale2 : -INFINITY;
-    }
-};
-
 template <int D>
 __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, uint32_t base, uint32_t bars, uint32_t tmem,
                                              volatile int* dead, volatile int* odd, int first, int last, int warp, int lane) {
@@ -484,31 +476,45 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
         const int n_items = p.groups * s.c;
         bool any = false;
         for (int n = slot; n < n_items; n += 2, ++done) {
-            const int i = s.t0 + (p.groups == 1 ? n : n >> 1);
+            const int i = s.t0 + (p.groups == 1 ? n : n >> 1), cached = p.nb * BLK - i * TILE;
+            const bool tail = i == p.tiles - 1;
+            const Masked left = mask && !tail ? mask_of(mask + i * TILE, cached, lane) : ALL;
             bar_wait(bars + 8 * (Plan<D>::S_FULL + slot), done & 1, dead);
             __syncwarp();
             fence_after();
-            if (busy) {
-                const bool tail = i == p.tiles - 1;
-                Edge edge;
-                edge.count = tail ? p.tail : min(TILE, p.nb * BLK - i * TILE);
-                edge.rest = tail ? p.rest : edge.count;
-                edge.mask = mask ? mask + min(i * TILE, p.nb * BLK) : nullptr;
-                edge.seen = seen;
+            if (left == NONE) {
+                const uint32_t zeros[16] = {0};
+#pragma unroll
+                for (int c = 0; c < TILE / 2; c += 16) tmem_st16(s_at + c, zeros);
+                tmem_st_wait();
+                any = true;
+            } else if (busy) {
                 // edges: scores to base 2 go back to where they came from; elsewhere they stay products until the exponential
-                const bool plain = !tail && !mask && edge.count == TILE;
+                const bool plain = !tail && left == ALL && cached >= TILE;
                 const float mul = plain ? scale2 : 1.f;
                 uint32_t v[32];
                 if (!plain) {
+                    // tokens that are there for this row, a bit each (a block that is missing: 64 columns in any order)
+                    const int count = tail ? p.rest : cached;
+                    unsigned long long there = ~0ull, above = cached >= TILE ? there : 0;
+                    if (tail) {
+                        there = seen << p.rest | ((1ull << p.rest) - 1);
+                        above = p.rest ? seen >> (64 - p.rest) : 0;
+                    }
 #pragma unroll 1
-                    for (int c = 0; c < TILE; c += 8) {
-                        uint32_t x[8];
+                    for (int c = 0; c < TILE; c += 32) {
+                        const int tok = c + (tail ? lane : swapped(lane));
+                        const uint32_t bits = (uint32_t)((c & 64 ? above : there) >> (c & 32));
+                        float add = 0.f;
+                        if (mask && tok < count) add = __half2float(mask[min(i * TILE, p.nb * BLK) + tok]) * LOG2E;
                         __syncwarp();
-                        tmem_ld8(x, s_at + c);
+                        tmem_ld(v, s_at + c);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(edge(__uint_as_float(x[j]), scale2, c + (tail ? j : swapped(j))));
-                        __syncwarp();
-                        tmem_st8(s_at + c, x);
+                        for (int j = 0; j < 32; ++j) {
+                            const float a = __shfl_sync(0xFFFFFFFFu, add, j);
+                            v[j] = __float_as_uint((bits >> j & 1) && a != -INFINITY ? fmaf(__uint_as_float(v[j]), scale2, a) : -INFINITY);
+                        }
+                        tmem_st32(s_at + c, v);
                     }
                     tmem_st_wait();
                 }
