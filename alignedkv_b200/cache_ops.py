@@ -143,7 +143,7 @@ def tree_weights(cache, q: torch.Tensor, lse: torch.Tensor, weights: torch.Tenso
 
     q as in `tree_attention`, which gives lse fp32 [B,T,Hq] (its normalisation includes the drafted tokens); mask and scale as
     there.  weights: fp32 [B,Hkv,max_seq_len]; entries behind the cached tokens are left alone.  The sums are formed in one order
-    (rows ascending within a lane, lanes in a fixed tree): the same call on the same state gives the same bits."""
+    (four interleaved ones over the rows, 512 rows at a time): the same call on the same state gives the same bits."""
     c = _Call(cache, rest_len, rest_start)
     T, Hq = c.queries(q)
     _need("lse", lse, (c.B, T, Hq), torch.float32, c.index)

@@ -118,11 +118,7 @@ struct EvictArgs {
 
 __device__ __forceinline__ int position_of(const EvictArgs& a, const int* pos, int i) { return i < a.arranged ? pos[i] : i + a.shift; }
 
-// ---- cluster: barrier, and a word of another CTA's shared memory
-__device__ __forceinline__ void cluster_sync() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
+// A word of another CTA's shared memory.
 __device__ __forceinline__ uint32_t cluster_ld(const void* p, uint32_t cta) {
     uint32_t at, v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(smem_u32(p)), "r"(cta));
@@ -431,22 +427,7 @@ int launch_select(const EvictArgs& a, int rows, int ctas, int threads, cudaStrea
     int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MOST * 4),
                          "evict select shared memory");
     if (rc != AKV_OK) return rc;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, rows);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ctas;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = tuning().pdl ? 2 : 1;
-    count_launch();
-    rc = cuda_status(cudaLaunchKernelEx(&cfg, kernel, a), "evict select launch");
-    return rc;
+    return cuda_status(launch_cluster(kernel, ctas, dim3(ctas, rows), dim3(threads), smem, st, a), "evict select launch");
 }
 
 int check_planes(const char* fn, const akv_layer* a) {

@@ -270,20 +270,84 @@ __device__ __forceinline__ void soften(float (&s)[NJ][4], float (&m)[2], float (
     }
 }
 
-template <int D>
+// One warp per query row: n records of its tokens, in their order, eight under way at a time; record i lies at at(i).
+template <int D, class At>
+__device__ __forceinline__ void join(const TreeArgs& p, At at, int n, long long to, int lane) {
+    constexpr int C = D / 32, STEP = 8;                 // channels of a lane
+    float acc[C], l = 0.f, top = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] = 0.f;
+#pragma unroll 1
+    for (int w = 0; w < n; w += STEP) {
+        float2 ml[STEP];
+        float o[STEP][C];
+#pragma unroll
+        for (int k = 0; k < STEP; ++k) {
+            ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int c = 0; c < C; ++c) o[k][c] = 0.f;
+            if (w + k >= n) continue;
+            const float* x = at(w + k);
+            ml[k] = *reinterpret_cast<const float2*>(x);
+            if constexpr (C == 4) {
+                const float4 y = *reinterpret_cast<const float4*>(x + 4 + 4 * lane);
+                o[k][0] = y.x; o[k][1] = y.y; o[k][2] = y.z; o[k][3] = y.w;
+            } else {
+                const float2 y = *reinterpret_cast<const float2*>(x + 4 + 2 * lane);
+                o[k][0] = y.x; o[k][1] = y.y;
+            }
+        }
+        float t = top;
+#pragma unroll
+        for (int k = 0; k < STEP; ++k) t = fmaxf(t, ml[k].x);
+        const float base = t == -INFINITY ? 0.f : t, keep = ex2(top - base);
+        top = t;
+        l *= keep;
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] *= keep;
+#pragma unroll
+        for (int k = 0; k < STEP; ++k) {
+            const float f = ex2(ml[k].x - base);
+            l = fmaf(f, ml[k].y, l);
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[c] = fmaf(f, o[k][c], acc[c]);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int c = 0; c < C; c += 2)
+        *reinterpret_cast<uint32_t*>(p.out + to * D + C * lane + c) = pack_half2(acc[c] * inv, acc[c + 1] * inv);
+    if (p.lse && lane == 0) p.lse[to] = l == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) - LIFT + log2f(l)) * LN2;
+}
+
+// TEAM: the warps of a cluster have one unit between them and join their records themselves, in shared memory.
+template <int D, bool TEAM>
 __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_constant__ TreeArgs p) {
     constexpr int N = D / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int R = p.T * p.G;
-    const int w = warp * gridDim.x + blockIdx.x;
-    if (w >= p.nw) return;
-    const int first = run_start(p, w), last = run_start(p, w + 1), unit0 = (unsigned)first / (unsigned)p.tiles;
+    const int w = TEAM ? ((blockIdx.x % p.team) * blockDim.x >> 5) + warp : warp * gridDim.x + blockIdx.x;
+    if (!TEAM && w >= p.nw) return;
+    int first, last;
+    if (TEAM) {                                        // p.nw runs of a unit, the first of them one tile longer, the last none
+        const int each = p.tiles / p.nw, more = p.tiles - each * p.nw;
+        first = blockIdx.x / (unsigned)p.team * p.tiles + w * each + min(w, more);
+        last = first + each + (w < more);
+    } else {
+        first = run_start(p, w), last = run_start(p, w + 1);
+    }
+    const int unit0 = (unsigned)first / (unsigned)p.tiles;
     uint4* qf = reinterpret_cast<uint4*>(smem + (size_t)warp * WARP_BYTES + STEPS * STEP_BYTES);
     uint4* pf = qf + 256;
     Ring<D> ring;
     ring.start(p, smem_u32(smem) + warp * WARP_BYTES, lane, first, last);
+    // records: of a run's first unit in slot 0, of its last in slot 1 (those between are whole); a team's in place of the rings
+    auto record = [&](int unit, int r) {
+        return TEAM ? reinterpret_cast<float*>(smem + (size_t)warp * WARP_BYTES) + r * (D + 4)
+                    : p.part + (size_t)((2 * w + (unit != unit0)) * ROWS + r) * (D + 4);
+    };
     for (int at = first; at < last;) {
         // (one unit per KV head: more rows than 16 are the other kernel's)
         const int unit = (unsigned)at / (unsigned)p.tiles, b = (unsigned)unit / (unsigned)p.H, h = unit - b * p.H;
@@ -390,6 +454,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
             }
             odd = __any_sync(0xFFFFFFFFu, odd);
         }
+        if (TEAM) __syncwarp();                        // (the ring has been read)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
@@ -412,9 +477,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
                     }
                 if (p.lse && t == 0) p.lse[row] = l[i] == 0.f ? -INFINITY : (m[i] - LIFT + log2f(l[i])) * LN2;
             } else {
-                // record of this warp: its first unit in slot 0, its last in slot 1 (those between are whole)
-                const int slot = unit != unit0;
-                float* rec = p.part + (size_t)((2 * w + slot) * ROWS + g + 8 * i) * (D + 4);
+                float* rec = record(unit, r);
                 if (t == 0) {
                     rec[0] = m[i];
                     rec[1] = l[i];
@@ -438,19 +501,32 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
                 if (t0 == 0 && t1 == p.tiles)
                     add_odd(p, b, h, r, D, base, sum == 0.f ? 0.f : 1.f / sum, p.out + (long long)row_of(p, b, h, r) * D);
                 else
-                    add_odd(p, b, h, r, D, base, 1.f, p.part + (size_t)((2 * w + (unit != unit0)) * ROWS + r) * (D + 4) + 4);
+                    add_odd(p, b, h, r, D, base, 1.f, record(unit, r) + 4);
             }
         }
         at = unit * p.tiles + t1;
     }
+    if constexpr (TEAM) {
+        const int wpc = blockDim.x >> 5, unit = blockIdx.x / (unsigned)p.team, b = (unsigned)unit / (unsigned)p.H, h = unit - b * p.H;
+        cluster_sync();
+        for (int r = w; r < R; r += p.nw) {
+            auto at = [&](int i) {
+                const float* x = reinterpret_cast<const float*>(smem + (size_t)(i % wpc) * WARP_BYTES) + r * (D + 4);
+                uint64_t y;
+                asm("mapa.u64 %0, %1, %2;\n" : "=l"(y) : "l"(x), "r"(i / wpc));
+                return reinterpret_cast<const float*>(y);
+            };
+            join<D>(p, at, min(p.nw, p.tiles), row_of(p, b, h, r), lane);
+        }
+        cluster_sync();                                // (no CTA leaves while another reads its records)
+    }
 }
 
-// One warp per query row: the records of the runs that share its unit, in the order of the tokens, eight under way at a time.  Bound by
-// latency: where the row lies is worked out before the kernel in front has ended.
+// One warp per query row: the records of the runs that share its unit.  Bound by latency: where the row lies is worked out before the
+// kernel in front has ended.
 template <int D>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeArgs p) {
     pdl_trigger();
-    constexpr int C = D / 32, STEP = 8;                 // channels of a lane
     const int lane = threadIdx.x & 31;
     const int row = blockIdx.x * 4 + (threadIdx.x >> 5);                        // unit * rowsu + row of the unit
     const int unit = (unsigned)row / (unsigned)p.rowsu, of_unit = row - unit * p.rowsu;
@@ -465,50 +541,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
     pdl_wait();
     // (a whole unit has been written by its run)
     if ((unsigned)unit >= (unsigned)p.total / (unsigned)p.tiles || r >= p.T * p.G || w0 == w1) return;
-    float acc[C], l = 0.f, top = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] = 0.f;
-#pragma unroll 1
-    for (int w = w0; w <= w1; w += STEP) {
-        float2 ml[STEP];
-        float o[STEP][C];
-#pragma unroll
-        for (int k = 0; k < STEP; ++k) {
-            const float* x = w + k == w0 ? rec0 : rec + (w + k - w0) * pitch;
-            ml[k] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-            for (int c = 0; c < C; ++c) o[k][c] = 0.f;
-            if (w + k > w1) continue;
-            ml[k] = *reinterpret_cast<const float2*>(x);
-            if constexpr (C == 4) {
-                const float4 y = *reinterpret_cast<const float4*>(x + 4 + 4 * lane);
-                o[k][0] = y.x; o[k][1] = y.y; o[k][2] = y.z; o[k][3] = y.w;
-            } else {
-                const float2 y = *reinterpret_cast<const float2*>(x + 4 + 2 * lane);
-                o[k][0] = y.x; o[k][1] = y.y;
-            }
-        }
-        float t = top;
-#pragma unroll
-        for (int k = 0; k < STEP; ++k) t = fmaxf(t, ml[k].x);
-        const float base = t == -INFINITY ? 0.f : t, keep = ex2(top - base);
-        top = t;
-        l *= keep;
-#pragma unroll
-        for (int c = 0; c < C; ++c) acc[c] *= keep;
-#pragma unroll
-        for (int k = 0; k < STEP; ++k) {
-            const float f = ex2(ml[k].x - base);
-            l = fmaf(f, ml[k].y, l);
-#pragma unroll
-            for (int c = 0; c < C; ++c) acc[c] = fmaf(f, o[k][c], acc[c]);
-        }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int c = 0; c < C; c += 2)
-        *reinterpret_cast<uint32_t*>(p.out + to * D + C * lane + c) = pack_half2(acc[c] * inv, acc[c + 1] * inv);
-    if (p.lse && lane == 0) p.lse[to] = l == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) - LIFT + log2f(l)) * LN2;
+    join<D>(p, [&](int i) { return i == 0 ? rec0 : rec + i * pitch; }, w1 - w0 + 1, to, lane);
 }
 
 // Warps for `total` tiles: one an SM while there are that few, then up to eight.
@@ -528,6 +561,7 @@ Deal deal(long long total, int most = WARPS) {
 // How the attention of T drafted tokens behind rest_start tokens is cut up.
 struct Shape {
     bool wide;
+    int team, team_runs;       // CTAs of a cluster that has a unit to itself and its warps, or 0: runs of equal length
     int groups, rowsg, rowsu, rt, tiles;
     long long units, total;
     Deal d;
@@ -544,16 +578,31 @@ Shape shape_of(int bsz, int H, int G, int T, int rest_start) {
     s.units = (long long)bsz * H * s.rt;
     s.total = s.units * s.tiles;
     s.d = deal(s.total, s.wide ? 1 : WARPS);
+    s.team = 0;
+    // A cluster per unit, one launch and no records in memory, where no warp gets more tiles by it (clusters of one size leave some SMs
+    // without any, so an eighth of them is not counted on).  All dealt, merged by a kernel of its own: TEAMTEXT.
+    int ctas = 8;
+    while (ctas > 1 && s.units * ctas > sm_count() * 7 / 8) ctas /= 2;
+    if (s.wide || s.tiles == 1 || s.units * ctas > sm_count()) return s;
+    const int per = (s.tiles + ctas - 1) / ctas, wpc = per < WARPS ? per : WARPS, n = ctas * wpc;
+    if ((s.tiles + n - 1) / n <= (s.total + s.d.runs - 1) / s.d.runs) {
+        s.team = ctas;
+        s.d.grid = (int)s.units * ctas;
+        s.d.wpc = wpc;
+        s.team_runs = n;
+    }
     return s;
 }
 
 // (the limit is raised for what eight warps take, whatever this launch does: it is a property of the kernel, not of the call)
-template <class Kernel, class... Args>
-int launch_warps(Kernel kernel, const Deal& d, cudaStream_t st, Args... args) {
+template <class Kernel>
+int launch_warps(Kernel kernel, const Deal& d, cudaStream_t st, const TreeArgs& p) {
     const int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WARPS * WARP_BYTES),
                                "tree kernel shared memory");
     if (rc != AKV_OK) return rc;
-    launch_chained(kernel, dim3(d.grid), dim3(32 * d.wpc), (size_t)d.wpc * WARP_BYTES, st, args...);
+    const dim3 grid(d.grid), block(32 * d.wpc);
+    if (p.team) launch_cluster(kernel, p.team, grid, block, (size_t)d.wpc * WARP_BYTES, st, p);
+    else launch_chained(kernel, grid, block, (size_t)d.wpc * WARP_BYTES, st, p);
     return AKV_OK;
 }
 
@@ -648,12 +697,15 @@ int akv_tree_attention(const akv_layer* layer, const void* q, const void* k_new,
     p.tiles = s.tiles;
     AKV_REQUIRE(s.total < INT_MAX, AKV_ERR_OVERFLOW, "tree_attention: too many tiles of 128 tokens");
     p.total = (int)s.total;
-    p.nw = s.d.runs;
+    p.nw = s.team ? s.team_runs : s.d.runs;
+    p.team = s.team;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    rc = s.wide ? launch_tree_wide(p, D, s.d.grid, st) : launch_warps(D == 128 ? tree_kernel<128> : tree_kernel<64>, s.d, st, p);
+    rc = s.wide ? launch_tree_wide(p, D, s.d.grid, st)
+         : s.team ? launch_warps(D == 128 ? tree_kernel<128, true> : tree_kernel<64, true>, s.d, st, p)
+                  : launch_warps(D == 128 ? tree_kernel<128, false> : tree_kernel<64, false>, s.d, st, p);
     if (rc != AKV_OK) return rc;
     rc = cuda_status(cudaGetLastError(), "tree_attention launch");
-    if (rc != AKV_OK || p.tiles == 1) return rc;                 // (units of one tile: none is shared)
+    if (rc != AKV_OK || p.tiles == 1 || s.team) return rc;       // (units of one tile: none is shared)
     launch_chained(D == 128 ? tree_merge_kernel<128> : tree_merge_kernel<64>, dim3((unsigned)((s.units * s.rowsu + 3) / 4)),
                    dim3(128), 0, st, p);
     return cuda_status(cudaGetLastError(), "tree_attention merge launch");

@@ -21,6 +21,7 @@ struct TreeArgs {
     int rowsu, rt;             // query rows of a unit, units of a (batch, KV head)
     int tiles, tail;           // tiles of a unit; tokens of its last, the tail tile
     int total, nw;             // tiles of all units, runs that they are dealt to (at most as many): warps, or CTAs
+    int team;                  // (tree_kernel) CTAs of a cluster that has a unit to itself, or 0
     int groups, rowsg;         // (tree_wide_kernel) row groups of a unit, rows of a group
     float scale, scale2;       // scale2 = scale * log2(e)
 };
