@@ -11,6 +11,7 @@
 // contiguous runs, so that every SM gets the same whatever the number of units and their length.  A warp needs no other one: it
 // turns plane bytes into operand fragments in registers (akv_planes.cuh), keeps the scores of its tile and the output of its unit
 // there, and leaves a record (maximum, sum, output) where a run begins or ends inside a unit.
+// 8 x 32 x 4096 tokens, 16 rows: 103 us with the merge, 5.2 TB/s of 6.5 (its own share 96 us).
 #include <limits.h>
 
 #include "akv_planes.cuh"
@@ -35,11 +36,15 @@ __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool th
 //   tail      16 tokens of the tail as fp16 rows [token][D]: a K step, then their V step
 // The 16-byte pieces of a 128-byte line are swapped by XOR so that a quarter (half) warp's 16-byte (8-byte) loads of a line's
 // pieces by lane (g, t) fall into different banks.
-constexpr int STEPS = 4, STEP_BYTES = 4096;
+// Steps: four for eight warps with many tiles each (8 x 32 x 4096 tokens: 104 us, with three 107, with five 104).  A team (see
+// Shape) has few warps with a tile or two each, which wait for the first bytes, not for the bandwidth: eight (1 x 32 x 1500 tokens:
+// 12.9 us, with four 14.8).
+constexpr int STEP_BYTES = 4096;
+template <bool TEAM> constexpr int steps_of = TEAM ? 8 : 4;
+template <bool TEAM> constexpr int warp_bytes = steps_of<TEAM> * STEP_BYTES + 8192;            // the ring, query fragments, probabilities
+constexpr int TEAM_WARPS = 5;
 
-constexpr int WARP_BYTES = STEPS * STEP_BYTES + 8192;            // the ring, query fragments, probabilities
-
-template <int D>
+template <int D, int STEPS>
 struct Ring {
     static constexpr int KSTEPS = D / 16, VSTEPS = D / 16, SUB = 128 / D;     // SUB: products of 16 tokens per V step
     uint32_t base;                 // of the warp's ring
@@ -192,8 +197,8 @@ struct Ring {
 };
 
 // Scores of a plane tile: s[j][c] = row g (c < 2) or g + 8, token 16 (2t + (c & 1)) + j.
-template <int D>
-__device__ __forceinline__ void plane_scores(float (&s)[16][4], const uint4* qf, const TreeArgs& p, Ring<D>& ring) {
+template <int D, int STEPS>
+__device__ __forceinline__ void plane_scores(float (&s)[16][4], const uint4* qf, const TreeArgs& p, Ring<D, STEPS>& ring) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll 1
@@ -215,7 +220,7 @@ __device__ __forceinline__ void tail_scores(float (&s)[2][4], const uint4* qf, u
     for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint2 w = lds64(at + Ring<D>::tail_place(g + 8 * j, 2 * kk + (t >> 1), false) + (t & 1) * 8);
+            const uint2 w = lds64(at + Ring<D, 4>::tail_place(g + 8 * j, 2 * kk + (t >> 1), false) + (t & 1) * 8);
             mma_f16(s[j], qf[kk * 32 + lane], w.x, w.y);
         }
 }
@@ -323,7 +328,8 @@ __device__ __forceinline__ void join(const TreeArgs& p, At at, int n, long long 
 // TEAM: the warps of a cluster have one unit between them and join their records themselves, in shared memory.
 template <int D, bool TEAM>
 __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_constant__ TreeArgs p) {
-    constexpr int N = D / 8;
+    constexpr int N = D / 8, WARP_BYTES = warp_bytes<TEAM>;
+    using Ring = Ring<D, steps_of<TEAM>>;
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -339,9 +345,9 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
         first = run_start(p, w), last = run_start(p, w + 1);
     }
     const int unit0 = (unsigned)first / (unsigned)p.tiles;
-    uint4* qf = reinterpret_cast<uint4*>(smem + (size_t)warp * WARP_BYTES + STEPS * STEP_BYTES);
+    uint4* qf = reinterpret_cast<uint4*>(smem + (size_t)warp * WARP_BYTES + steps_of<TEAM> * STEP_BYTES);
     uint4* pf = qf + 256;
-    Ring<D> ring;
+    Ring ring;
     ring.start(p, smem_u32(smem) + warp * WARP_BYTES, lane, first, last);
     // records: of a run's first unit in slot 0, of its last in slot 1 (those between are whole); a team's in place of the rings
     auto record = [&](int unit, int r) {
@@ -362,7 +368,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
         for (int tile = t0; tile < min(t1, p.tiles - 1); ++tile) {
             {
                 float s[16][4];
-                plane_scores<D>(s, qf, p, ring);
+                plane_scores(s, qf, p, ring);
                 const int count = p.nb * BLK - tile * TILE;
                 if (mask || count < TILE) {             // tokens that do not exist or are masked away: -inf
 #pragma unroll
@@ -383,20 +389,20 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
                 }
                 soften(s, m, l, o);
                 // (through shared memory, every lane its own: the loop over the V steps stays a loop - unrolled eight times, with
-                // the copies in each, the kernel was bound by the fetch of its instructions, 195 us against 113 at 8 x 32 x 4096 tokens)
+                // the copies in each, the kernel was bound by the fetch of its instructions, 195 us against 113 then at 8 x 32 x 4096 tokens)
 #pragma unroll
                 for (int st = 0; st < 8; ++st)
                     pf[st * 32 + lane] = make_uint4(pack_half2(s[2 * st][0], s[2 * st + 1][0]), pack_half2(s[2 * st][2], s[2 * st + 1][2]),
                                                     pack_half2(s[2 * st][1], s[2 * st + 1][1]), pack_half2(s[2 * st][3], s[2 * st + 1][3]));
             }
 #pragma unroll 1
-            for (int vs = 0; vs < Ring<D>::VSTEPS; ++vs) {
+            for (int vs = 0; vs < Ring::VSTEPS; ++vs) {
                 const uint32_t from = ring.take(p);
 #pragma unroll
-                for (int u = 0; u < Ring<D>::SUB; ++u) {
-                    const int st = vs * Ring<D>::SUB + u;
+                for (int u = 0; u < Ring::SUB; ++u) {
+                    const int st = vs * Ring::SUB + u;
                     Line<N> x[4];
-                    ring.lines_v(x, from + u * (STEP_BYTES / Ring<D>::SUB));
+                    ring.lines_v(x, from + u * (STEP_BYTES / Ring::SUB));
                     if (mask) {      // a token that is masked away counts as zero, whatever its values are: 0 * NaN would be NaN
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -440,7 +446,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
                     const int r = 2 * t + (i & 1) + 8 * (i >> 1);
 #pragma unroll
                     for (int v = 0; v < N / 8; ++v) {
-                        const uint4 y = lds128(from + Ring<D>::tail_place(r, N / 8 * g + v, true));
+                        const uint4 y = lds128(from + Ring::tail_place(r, N / 8 * g + v, true));
                         x[i][4 * v] = y.x; x[i][4 * v + 1] = y.y; x[i][4 * v + 2] = y.z; x[i][4 * v + 3] = y.w;
                     }
 #pragma unroll
@@ -569,6 +575,9 @@ struct Shape {
 Shape shape_of(int bsz, int H, int G, int T, int rest_start) {
     Shape s;
     const int R = T * G;
+    // More rows than a warp's product has: the tensor cores' kernel reads the planes once for up to 256 rows, this one would once
+    // for 16 (20 rows, 8 x 131072 tokens: 125 us there, 187 here; 48 rows, 16 x 8 x 8190: 128 and 288).  Up to 16 rows it is
+    // bound by HBM and has no chain through three roles of warps to wait for (8 x 32 x 4096, 16 rows: 103 us here, 130 there).
     s.wide = R > ROWS;
     s.groups = R > 128 ? 2 : 1;
     s.rt = s.wide ? (R + 128 * s.groups - 1) / (128 * s.groups) : 1;
@@ -579,12 +588,13 @@ Shape shape_of(int bsz, int H, int G, int T, int rest_start) {
     s.total = s.units * s.tiles;
     s.d = deal(s.total, s.wide ? 1 : WARPS);
     s.team = 0;
-    // A cluster per unit, one launch and no records in memory, where no warp gets more tiles by it (clusters of one size leave some SMs
-    // without any, so an eighth of them is not counted on).  All dealt, merged by a kernel of its own: TEAMTEXT.
+    // Short caches: a cluster per unit, one launch and no records in memory, wherever no warp gets more tiles by it (clusters of one
+    // size leave some SMs without any: an eighth of them is not counted on).  On the device 12.3 us against 14.4 with equal runs and a
+    // merge at 1 x 32 x 777 tokens, 15.7 against 18.0 at 1 x 8 x 4000, and a launch less for the host.
     int ctas = 8;
     while (ctas > 1 && s.units * ctas > sm_count() * 7 / 8) ctas /= 2;
     if (s.wide || s.tiles == 1 || s.units * ctas > sm_count()) return s;
-    const int per = (s.tiles + ctas - 1) / ctas, wpc = per < WARPS ? per : WARPS, n = ctas * wpc;
+    const int per = (s.tiles + ctas - 1) / ctas, wpc = per < TEAM_WARPS ? per : TEAM_WARPS, n = ctas * wpc;
     if ((s.tiles + n - 1) / n <= (s.total + s.d.runs - 1) / s.d.runs) {
         s.team = ctas;
         s.d.grid = (int)s.units * ctas;
@@ -597,12 +607,13 @@ Shape shape_of(int bsz, int H, int G, int T, int rest_start) {
 // (the limit is raised for what eight warps take, whatever this launch does: it is a property of the kernel, not of the call)
 template <class Kernel>
 int launch_warps(Kernel kernel, const Deal& d, cudaStream_t st, const TreeArgs& p) {
-    const int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WARPS * WARP_BYTES),
+    const int bytes = p.team ? warp_bytes<true> : warp_bytes<false>;
+    const int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (p.team ? TEAM_WARPS : WARPS) * bytes),
                                "tree kernel shared memory");
     if (rc != AKV_OK) return rc;
     const dim3 grid(d.grid), block(32 * d.wpc);
-    if (p.team) launch_cluster(kernel, p.team, grid, block, (size_t)d.wpc * WARP_BYTES, st, p);
-    else launch_chained(kernel, grid, block, (size_t)d.wpc * WARP_BYTES, st, p);
+    if (p.team) launch_cluster(kernel, p.team, grid, block, (size_t)d.wpc * bytes, st, p);
+    else launch_chained(kernel, grid, block, (size_t)d.wpc * bytes, st, p);
     return AKV_OK;
 }
 
