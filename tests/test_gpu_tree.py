@@ -129,6 +129,33 @@ def test_masked_drafts_may_hold_anything(akv_lib, D, Hq, H, T):
     assert bool(x.layer.tree_attention(x.q, x.k, x.v, tree)[:, worse].isnan().all())
 
 
+@pytest.mark.parametrize("B,n,Hq,H,D,T", [
+    (40, 300, 8, 4, 128, 3), (75, 450, 2, 2, 64, 8), (150, 129, 1, 1, 128, 2),          # more units than SMs: runs that cross units
+    (1, 20000, 2, 2, 128, 5), (1, 40000, 1, 1, 64, 16),                                 # few units with many tiles
+    (149, 70, 18, 1, 128, 1), (38, 260, 20, 5, 64, 5),                                  # the same with more than 16 rows a unit
+    (1, 20000, 9, 1, 128, 2), (5, 1000, 8, 1, 64, 20), (3, 900, 13, 1, 128, 20)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_work_cut_up_every_way(akv_lib, B, n, Hq, H, D, T, masked):
+    """Runs of whole units, parts of units and both; masks that leave tiles whole, in part and not at all, what they take away not a
+    number."""
+    x = make(B, n, Hq, H, D, T, seed=B + n)
+    mask = wide = None
+    if masked:
+        from alignedkv_b200.decode import DecodeLayer
+        mask = torch.zeros(B, n, dtype=torch.half, device=DEV)
+        for b in range(B):
+            mask[b, :(b * 97 + n // 2) % n] = -math.inf                  # left padding
+            mask[b, n - 1 - b % 50] = -math.inf                          # a single token
+            mask[b, n // 2 + b % 30] = -2.5                              # one that counts less
+        hidden = mask == -math.inf
+        x.kc[hidden], x.vc[hidden] = math.inf, math.nan
+        x.layer = DecodeLayer(B, n + 3, H, D, DEV, n_q_heads=Hq)
+        x.layer.prefill(x.kc, x.vc)
+        wide = torch.zeros(B, 1, 1, n + 1, dtype=torch.half, device=DEV)
+        wide[:, 0, 0, :n] = mask
+    check(x, *x.layer.tree_attention(x.q, x.k, x.v, x.tree, mask=wide, lse=True), mask=mask)
+
+
 def test_one_token_is_a_decode_step(akv_lib):
     """T = 1: the output of `decode` within its read decisions' error, and after a commit the state it leaves, bit for bit."""
     from alignedkv_b200.decode import DecodeLayer
