@@ -815,6 +815,8 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_c
                 if (p.mask && tok < count) add = __half2float(p.mask[s.b * p.mask_stride + at + tok]);
                 const bool gone = tok >= count || add == -INFINITY;
                 add *= LOG2E;
+                float* to = weights + (long long)s.bh * p.L + at + tok;
+                const float before = gone ? 0.f : *to;         // (on its way while the scores are)
                 for (int g = 0; g < groups; ++g, ++done) {
                     bar_wait(bars + 8 * (L::S_FULL + slot), done & 1, dead);
                     __syncwarp();
@@ -850,7 +852,7 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_c
                 if (!gone) {
                     float x = (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     if (*dead) x = __int_as_float(0x7FC00000);
-                    weights[(long long)s.bh * p.L + at + tok] += x;
+                    *to = before + x;
                 }
             }
         }
