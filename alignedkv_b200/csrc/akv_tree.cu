@@ -25,11 +25,6 @@ constexpr int ROWS = 16, WARPS = 8;
 // Token of line i of V step st within a tile, for lane column t: the tokens whose probabilities this lane holds.
 __device__ __forceinline__ int v_token(int st, int t, int i) { return 32 * t + 2 * st + (i & 1) + (i >> 1) * 16; }
 
-// 16 bytes global -> shared past L1; with `there` false zeros, and nothing is read.
-__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-
 // A warp's ring of 4 KB steps in shared memory, filled STEPS - 1 steps ahead by its own asynchronous copies.
 //   K step    16 channels of the tile's 128 tokens: high bytes [block][channel][64], nibbles [block][channel][32] twice
 //   V step    32 (D = 128: 16) tokens: for each 16 of them high bytes [4t + i][D], nibbles [..][D / 2] twice

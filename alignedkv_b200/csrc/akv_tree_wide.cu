@@ -435,19 +435,31 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
     const uint32_t sign = p.scale2 < 0.f ? 0x80008000u : 0u;
     float* xm = reinterpret_cast<float*>(smem + Plan<D>::XM_AT);
     float* xl = reinterpret_cast<float*>(smem + Plan<D>::XL_AT);
-    // Queries of the segment that begins with `tile`, 16-byte piece c of a row's half at c ^ (row & 7).
-    auto queries = [&](int tile, int index) {
+    // Queries of the segment that begins with `tile`, 16-byte piece c of a row's half at c ^ (row & 7): requested all at once (by way of
+    // registers it was four round trips), then handed over.
+    auto query_place = [&](int index, int c) {
+        return base + ((p.groups == 2 ? group : index & 1) ? Plan<D>::Q2_AT : Plan<D>::Q_AT) + idx * 128 + (c >> 3) * Plan<D>::Q_HALF +
+               (((c & 7) ^ (idx & 7)) << 4);
+    };
+    const int c0 = p.groups == 1 ? slot * (D / 16) : 0, c1 = p.groups == 1 ? c0 + D / 16 : D / 8;
+    auto request_queries = [&](int tile, int index) {
         Segment s;
         s.at(p, tile, last);
         const int of_unit = group * p.rowsg + idx, r = s.super * p.rowsu + of_unit;
         const bool mine = idx < p.rowsg && of_unit < p.rowsu && r < R;
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(mine ? row_of(p, s.b, s.h, r) : 0) * D);
-        const uint32_t to = base + ((p.groups == 2 ? group : index & 1) ? Plan<D>::Q2_AT : Plan<D>::Q_AT) + idx * 128;
-        const int c0 = p.groups == 1 ? slot * (D / 16) : 0, c1 = p.groups == 1 ? c0 + D / 16 : D / 8;
+        const __half* src = p.q + (long long)(mine ? row_of(p, s.b, s.h, r) : 0) * D;
 #pragma unroll 4
-        for (int c = c0; c < c1; ++c) {
-            const uint4 x = mine ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-            sts128(to + (c >> 3) * Plan<D>::Q_HALF + (((c & 7) ^ (idx & 7)) << 4), make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign));
+        for (int c = c0; c < c1; ++c) copy16(query_place(index, c), src + 8 * c, mine);
+        cp_async_commit();
+    };
+    auto hand_queries_over = [&](int index) {
+        cp_async_wait<0>();
+        if (sign) {
+#pragma unroll 1
+            for (int c = c0; c < c1; ++c) {
+                const uint4 x = lds128(query_place(index, c));
+                sts128(query_place(index, c), make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign));
+            }
         }
         fence_shared();
         __syncwarp();
@@ -455,7 +467,8 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
     };
     uint32_t done = 0;
     int seg = 0;
-    queries(first, 0);
+    request_queries(first, 0);
+    hand_queries_over(0);
     for (int tile = first; tile < last; ++seg) {
         Segment s;
         s.at(p, tile, last);
@@ -566,10 +579,11 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
         }
         // (this slot's products with the queries are over - with one group the next ones have a place of their own - while its last
         // output is still under way)
-        if (tile < last) queries(tile, seg + 1);
+        if (tile < last) request_queries(tile, seg + 1);
         // ---- the segment's result: with one group the slots' two, joined
         const bool have = n_items > slot;
         if (have) bar_wait(bars + 8 * (Plan<D>::O_FULL + slot), (done - 1) & 1, dead);
+        if (tile < last) hand_queries_over(seg + 1);
         __syncwarp();
         fence_after();
         float f0 = 1.f, f1 = 0.f;
@@ -789,20 +803,22 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_c
             s.at(p, tile, last);
             tile += s.c;
             soft_sync();                               // (all products with the queries before are over: their scores have been read)
+            // (all at once: as loads, one after the other, they took 5 us of a call with 128 rows)
 #pragma unroll 4
             for (int i = threadIdx.x; i < L::padded(rows) * (D / 8); i += 32 * SOFT) {
                 const int r = i / (D / 8), c = i % (D / 8);
-                const uint4 x = r < rows ? __ldg(reinterpret_cast<const uint4*>(p.q + (long long)row_of(p, s.b, s.h, row0 + r) * D) + c) : make_uint4(0, 0, 0, 0);
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(base + L::Q_AT + (c >> 3) * q_half + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
-                             "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+                copy16(base + L::Q_AT + (c >> 3) * q_half + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                       p.q + (long long)(r < rows ? row_of(p, s.b, s.h, row0 + r) : 0) * D + 8 * c, r < rows);
             }
-#pragma unroll 1
-            for (int r = warp * 32; r < L::ROWS; r += 32 * SOFT) {
-                const float x = r + lane < rows ? p.lse[row_of(p, s.b, s.h, row0 + r + lane)] : -INFINITY;
+            cp_async_commit();
+#pragma unroll
+            for (int r = threadIdx.x; r < L::ROWS; r += 32 * SOFT) {
+                const float x = r < rows ? p.lse[row_of(p, s.b, s.h, row0 + r)] : -INFINITY;
                 const uint32_t none = __ballot_sync(0xFFFFFFFFu, x == -INFINITY);
-                off[r + lane] = x == -INFINITY ? x : -x;
+                off[r] = x == -INFINITY ? x : -x;
                 if (lane == 0) absent[r >> 5] = none;
             }
+            cp_async_wait<0>();
             fence_shared();
             soft_sync();                               // (`off` is everybody's)
             if (lane == 0) bar_arrive(bars + 8 * L::Q_FULL);
