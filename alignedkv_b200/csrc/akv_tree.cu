@@ -56,7 +56,7 @@ struct Ring {
         unit = (unsigned)first / (unsigned)p.tiles;
         tile = first - unit * p.tiles;
         left = last - first;
-        bh = (unsigned)unit / (unsigned)p.rt;
+        bh = unit;
 #pragma unroll 1
         for (int i = 0; i < STEPS - 1; ++i) fill(p);
     }
@@ -151,7 +151,7 @@ struct Ring {
                 --left;
                 if (++tile == p.tiles) {
                     tile = 0;
-                    bh = (unsigned)++unit / (unsigned)p.rt;
+                    bh = ++unit;
                 }
             }
         }
@@ -529,15 +529,13 @@ template <int D>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeArgs p) {
     pdl_trigger();
     const int lane = threadIdx.x & 31;
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 5);                        // unit * rowsu + row of the unit
-    const int unit = (unsigned)row / (unsigned)p.rowsu, of_unit = row - unit * p.rowsu;
-    const int bh = (unsigned)unit / (unsigned)p.rt, b = (unsigned)bh / (unsigned)p.H, h = bh - b * p.H;
-    const int r = (unit - bh * p.rt) * p.rowsu + of_unit;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 5), unit = row / ROWS, r = row % ROWS;
+    const int b = (unsigned)unit / (unsigned)p.H, h = unit - b * p.H;
     const int w0 = run_with(p, unit * p.tiles), w1 = run_with(p, unit * p.tiles + p.tiles - 1);
     const long long to = row_of(p, b, h, r);
     // a run's record of its first unit is in slot 0, of its last in slot 1: only the first of this unit's may have begun before it
-    const float* rec = p.part + (size_t)(2 * w0 * p.rowsu + of_unit) * (D + 4);
-    const size_t pitch = (size_t)2 * p.rowsu * (D + 4);
+    const float* rec = p.part + (size_t)(2 * w0 * ROWS + r) * (D + 4);
+    constexpr size_t pitch = (size_t)2 * ROWS * (D + 4);
     const float* rec0 = run_start(p, w0) < unit * p.tiles ? rec + pitch / 2 : rec;
     pdl_wait();
     // (a whole unit has been written by its run)
@@ -706,13 +704,13 @@ int akv_tree_attention(const akv_layer* layer, const void* q, const void* k_new,
     p.nw = s.team ? s.team_runs : s.d.runs;
     p.team = s.team;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    rc = s.wide ? launch_tree_wide(p, D, s.d.grid, st)
-         : s.team ? launch_warps(D == 128 ? tree_kernel<128, true> : tree_kernel<64, true>, s.d, st, p)
-                  : launch_warps(D == 128 ? tree_kernel<128, false> : tree_kernel<64, false>, s.d, st, p);
+    if (s.wide) return launch_tree_wide(p, D, s.d.grid, (int)s.units, st);
+    rc = s.team ? launch_warps(D == 128 ? tree_kernel<128, true> : tree_kernel<64, true>, s.d, st, p)
+                : launch_warps(D == 128 ? tree_kernel<128, false> : tree_kernel<64, false>, s.d, st, p);
     if (rc != AKV_OK) return rc;
     rc = cuda_status(cudaGetLastError(), "tree_attention launch");
     if (rc != AKV_OK || p.tiles == 1 || s.team) return rc;       // (units of one tile: none is shared)
-    launch_chained(D == 128 ? tree_merge_kernel<128> : tree_merge_kernel<64>, dim3((unsigned)((s.units * s.rowsu + 3) / 4)),
+    launch_chained(D == 128 ? tree_merge_kernel<128> : tree_merge_kernel<64>, dim3((unsigned)(s.units * (ROWS / 4))),
                    dim3(128), 0, st, p);
     return cuda_status(cudaGetLastError(), "tree_attention merge launch");
 }

@@ -62,8 +62,8 @@ __device__ __forceinline__ int run_with(const TreeArgs& p, int i) {
 // Tail values that are not finite.  What one row sees of the drafted tokens is masked for another, and 0 * inf would be NaN: such
 // values enter the product as zeros, and a row that sees them adds p . v to what it has written (p relative to 2^base, times `inv`).
 // The rare way: by itself, and out of line.
-template <class T>
-static __device__ __noinline__ void add_odd(const TreeArgs& p, int b, int h, int r, int D, float base, float inv, T* to) {
+template <class To>
+static __device__ __noinline__ void add_odd(const TreeArgs& p, int b, int h, int r, int D, float base, float inv, To to) {
     const __half* q = p.q + (long long)row_of(p, b, h, r) * D;
     const __half* mask = p.mask ? p.mask + b * p.mask_stride + p.nb * BLK : nullptr;
     const uint8_t* seen = p.tree + b * p.tree_stride + (unsigned)r / (unsigned)p.G * p.T;
@@ -85,7 +85,8 @@ static __device__ __noinline__ void add_odd(const TreeArgs& p, int b, int h, int
                 for (int j = 0; j < D; ++j) dot = fmaf(__half2float(q[j]), __half2float(k[j]), dot);
                 pr = ex2(fmaf(dot, p.scale2, add * LOG2E) - base) * inv;
             }
-            to[c] = (T)((float)to[c] + pr * x);
+            auto& y = to[c];
+            y = (float)y + pr * x;
         }
     }
 }
@@ -96,7 +97,7 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w, bool& odd) {
 }
 
 // Tensor-core form (akv_tree_wide.cu).
-int launch_tree_wide(const TreeArgs& p, int D, int ctas, cudaStream_t st);
+int launch_tree_wide(const TreeArgs& p, int D, int ctas, int units, cudaStream_t st);
 int launch_weights_wide(const TreeArgs& p, int D, int ctas, float* weights, cudaStream_t st);
 
 }  // namespace akv

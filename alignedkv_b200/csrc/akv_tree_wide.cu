@@ -426,6 +426,18 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
 }
 
 // ---------------------------------------------------------------- softmax
+// A CTA's part of a row: rows of four channels side by side, as the threads of a warp have them and write them (a row after the other,
+// the lanes' stores met in no line: SEPARATE), the maxima and sums behind them.  As in akv_tree.cu, slot 0 is of a run's first unit, slot 1 of its last.
+struct Record {
+    float* at;
+    int rows, D, row;
+    __device__ __forceinline__ Record(const TreeArgs& p, int D, int index, int row) :
+        at(p.part + (size_t)index * p.rowsu * (D + 4)), rows(p.rowsu), D(D), row(row) {}
+    __device__ __forceinline__ float4* quad(int q) const { return reinterpret_cast<float4*>(at) + q * rows + row; }
+    __device__ __forceinline__ float2* stats() const { return reinterpret_cast<float2*>(at + rows * D) + row; }
+    __device__ __forceinline__ float& operator[](int c) const { return reinterpret_cast<float*>(quad(c >> 2))[c & 3]; }
+};
+
 template <int D>
 __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, uint32_t base, uint32_t bars, uint32_t tmem,
                                              volatile int* dead, volatile int* odd, int first, int last, int warp, int lane) {
@@ -606,7 +618,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
         if (*dead) l = __int_as_float(0x7FC00000);
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int rec_slot = s.unit != (unsigned)first / (unsigned)p.tiles;
-        float* rec = p.part + (size_t)((2 * blockIdx.x + rec_slot) * p.rowsu + of_unit) * (D + 4);
+        const Record rec(p, D, 2 * blockIdx.x + rec_slot, of_unit);
         float4* join = reinterpret_cast<float4*>(smem + (seg & 1 ? Plan<D>::Q2_AT : Plan<D>::Q_AT));              // [16 channel quads][128 rows]
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
@@ -653,18 +665,17 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    reinterpret_cast<float4*>(rec + 4 + c)[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                    *rec.quad(c / 4 + j) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
             }
         }
         if (mine && !(p.groups == 1 && slot)) {
             if (odd_tail) {
                 const float off = (ref == -INFINITY ? 0.f : ref) - WIDE_LIFT;
                 if (whole) add_odd(p, s.b, s.h, r, D, off, inv, p.out + (long long)row_of(p, s.b, s.h, r) * D);
-                else add_odd(p, s.b, s.h, r, D, off, 1.f, rec + 4);
+                else add_odd(p, s.b, s.h, r, D, off, 1.f, rec);
             }
             if (!whole) {
-                rec[0] = ref + (LIFT - WIDE_LIFT);
-                rec[1] = l;
+                *rec.stats() = make_float2(ref, l);
             } else if (p.lse) {
                 p.lse[row_of(p, s.b, s.h, r)] = l == 0.f ? -INFINITY : (ref - WIDE_LIFT + log2f(l)) * LN2;
             }
@@ -733,6 +744,58 @@ __global__ void __launch_bounds__(THREADS, 1) tree_wide_kernel(const __grid_cons
     fence_after();
     if (warp == SOFT + DECODE)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+}
+
+// A thread per row and four channels: the records of the runs that share its unit, in the order of the tokens, four under way at a time.
+template <int D>
+__global__ void __launch_bounds__(2 * D) tree_wide_merge_kernel(const __grid_constant__ TreeArgs p) {
+    pdl_trigger();
+    constexpr int STEP = 4;
+    const int q = threadIdx.x >> 3, row = blockIdx.x * 8 + (threadIdx.x & 7);   // row: unit * rowsu + row of the unit
+    const int unit = (unsigned)row / (unsigned)p.rowsu, of_unit = row - unit * p.rowsu;
+    const int bh = (unsigned)unit / (unsigned)p.rt, b = (unsigned)bh / (unsigned)p.H, h = bh - b * p.H;
+    const int r = (unit - bh * p.rt) * p.rowsu + of_unit;
+    const int w0 = run_with(p, unit * p.tiles), w1 = run_with(p, unit * p.tiles + p.tiles - 1);
+    const long long to = row_of(p, b, h, r);
+    const int skip = run_start(p, w0) < unit * p.tiles;                        // (the first run of the unit's may have begun before it)
+    pdl_wait();
+    // (a whole unit has been written by its run)
+    if ((unsigned)unit >= (unsigned)p.total / (unsigned)p.tiles || r >= p.T * p.G || w0 == w1) return;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, top = -INFINITY;
+#pragma unroll 1
+    for (int w = w0; w <= w1; w += STEP) {
+        float2 ml[STEP];
+        float4 o[STEP];
+#pragma unroll
+        for (int k = 0; k < STEP; ++k) {
+            const Record rec(p, D, 2 * (w + k) + (w + k == w0 ? skip : 0), of_unit);
+            ml[k] = make_float2(-INFINITY, 0.f);
+            o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (w + k > w1) continue;
+            ml[k] = *rec.stats();
+            o[k] = *rec.quad(q);
+        }
+        float t = top;
+#pragma unroll
+        for (int k = 0; k < STEP; ++k) t = fmaxf(t, ml[k].x);
+        const float base = t == -INFINITY ? 0.f : t, keep = ex2(top - base);
+        top = t;
+        l *= keep;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] *= keep;
+#pragma unroll
+        for (int k = 0; k < STEP; ++k) {
+            const float f = ex2(ml[k].x - base);
+            l = fmaf(f, ml[k].y, l);
+            acc[0] = fmaf(f, o[k].x, acc[0]);
+            acc[1] = fmaf(f, o[k].y, acc[1]);
+            acc[2] = fmaf(f, o[k].z, acc[2]);
+            acc[3] = fmaf(f, o[k].w, acc[3]);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(p.out + to * D + 4 * q) = make_uint2(pack_half2(acc[0] * inv, acc[1] * inv), pack_half2(acc[2] * inv, acc[3] * inv));
+    if (p.lse && q == 0) p.lse[to] = l == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) - WIDE_LIFT + log2f(l)) * LN2;
 }
 
 // ---------------------------------------------------------------- weights
@@ -945,14 +1008,17 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_c
 
 }  // namespace
 
-int launch_tree_wide(const TreeArgs& p, int D, int ctas, cudaStream_t st) {
+int launch_tree_wide(const TreeArgs& p, int D, int ctas, int units, cudaStream_t st) {
     auto kernel = D == 128 ? tree_wide_kernel<128> : tree_wide_kernel<64>;
     const int bytes = D == 128 ? Plan<128>::BYTES : Plan<64>::BYTES;
     const int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
                                "tree_attention shared memory");
     if (rc != AKV_OK) return rc;
     launch_chained(kernel, dim3(ctas), dim3(THREADS), (size_t)bytes, st, p);
-    return AKV_OK;
+    if (p.tiles > 1)                                   // (units of one tile: none is shared)
+        launch_chained(D == 128 ? tree_wide_merge_kernel<128> : tree_wide_merge_kernel<64>,
+                       dim3((unsigned)(((long long)units * p.rowsu + 7) / 8)), dim3(2 * D), 0, st, p);
+    return cuda_status(cudaGetLastError(), "tree_attention launch");
 }
 
 int launch_weights_wide(const TreeArgs& p, int D, int ctas, float* weights, cudaStream_t st) {
