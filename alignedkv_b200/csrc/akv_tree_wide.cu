@@ -447,30 +447,34 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
     const uint32_t sign = p.scale2 < 0.f ? 0x80008000u : 0u;
     float* xm = reinterpret_cast<float*>(smem + Plan<D>::XM_AT);
     float* xl = reinterpret_cast<float*>(smem + Plan<D>::XL_AT);
-    // Queries of the segment that begins with `tile`, 16-byte piece c of a row's half at c ^ (row & 7): requested all at once (by way of
-    // registers it was four round trips), then handed over.
-    auto query_place = [&](int index, int c) {
-        return base + ((p.groups == 2 ? group : index & 1) ? Plan<D>::Q2_AT : Plan<D>::Q_AT) + idx * 128 + (c >> 3) * Plan<D>::Q_HALF +
-               (((c & 7) ^ (idx & 7)) << 4);
+    // Queries of the segment that begins with `tile`, 16-byte piece c of a row's half at c ^ (row & 7): a warp's 32 rows (with one group
+    // either slot's warp takes half of their pieces), neighbouring pieces by neighbouring lanes and all on their way at once (a row
+    // a lane, by way of registers or not, took 4 us at the start of 256 rows).  Then they are handed over.
+    const int per = p.groups == 1 ? D / 16 : D / 8, i0 = p.groups == 1 ? slot * per : 0;             // (steps of 32 pieces)
+    auto query_place = [&](int index, int i) {
+        const int row = (warp & 3) * 32 + i * 32 / (D / 8) + lane / (D / 8), c = lane % (D / 8);
+        return base + ((p.groups == 2 ? group : index & 1) ? Plan<D>::Q2_AT : Plan<D>::Q_AT) + row * 128 + (c >> 3) * Plan<D>::Q_HALF +
+               (((c & 7) ^ (row & 7)) << 4);
     };
-    const int c0 = p.groups == 1 ? slot * (D / 16) : 0, c1 = p.groups == 1 ? c0 + D / 16 : D / 8;
     auto request_queries = [&](int tile, int index) {
         Segment s;
         s.at(p, tile, last);
         const int of_unit = group * p.rowsg + idx, r = s.super * p.rowsu + of_unit;
-        const bool mine = idx < p.rowsg && of_unit < p.rowsu && r < R;
-        const __half* src = p.q + (long long)(mine ? row_of(p, s.b, s.h, r) : 0) * D;
+        const int mine = idx < p.rowsg && of_unit < p.rowsu && r < R ? row_of(p, s.b, s.h, r) : -1;
 #pragma unroll 4
-        for (int c = c0; c < c1; ++c) copy16(query_place(index, c), src + 8 * c, mine);
+        for (int i = i0; i < i0 + per; ++i) {
+            const int row = __shfl_sync(0xFFFFFFFFu, mine, i * 32 / (D / 8) + lane / (D / 8));
+            copy16(query_place(index, i), p.q + (long long)max(row, 0) * D + 8 * (lane % (D / 8)), row >= 0);
+        }
         cp_async_commit();
     };
     auto hand_queries_over = [&](int index) {
         cp_async_wait<0>();
         if (sign) {
 #pragma unroll 1
-            for (int c = c0; c < c1; ++c) {
-                const uint4 x = lds128(query_place(index, c));
-                sts128(query_place(index, c), make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign));
+            for (int i = i0; i < i0 + per; ++i) {
+                const uint4 x = lds128(query_place(index, i));
+                sts128(query_place(index, i), make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign));
             }
         }
         fence_shared();
