@@ -117,7 +117,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
 __device__ __forceinline__ constexpr uint32_t instruction(int n, bool b_mn, bool a_mn = false) {
     return 1u << 4 | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
 }
-// 32 columns of this thread's lane
+// 32 columns of this thread's lane.
 __device__ __forceinline__ void tmem_ld(uint32_t (&v)[32], uint32_t at) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
                  "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
@@ -127,6 +127,24 @@ __device__ __forceinline__ void tmem_ld(uint32_t (&v)[32], uint32_t at) {
                    "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
                  : "r"(at) : "memory");
     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+}
+// 16 columns from each of four places, with one wait.
+__device__ __forceinline__ void tmem_ld4(uint32_t (&v)[4][16], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%64];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%65];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47}, [%66];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%67];\n"
+        "tcgen05.wait::ld.sync.aligned;\n"
+        : "=r"(v[0][0]), "=r"(v[0][1]), "=r"(v[0][2]), "=r"(v[0][3]), "=r"(v[0][4]), "=r"(v[0][5]), "=r"(v[0][6]), "=r"(v[0][7]),
+          "=r"(v[0][8]), "=r"(v[0][9]), "=r"(v[0][10]), "=r"(v[0][11]), "=r"(v[0][12]), "=r"(v[0][13]), "=r"(v[0][14]), "=r"(v[0][15]),
+          "=r"(v[1][0]), "=r"(v[1][1]), "=r"(v[1][2]), "=r"(v[1][3]), "=r"(v[1][4]), "=r"(v[1][5]), "=r"(v[1][6]), "=r"(v[1][7]),
+          "=r"(v[1][8]), "=r"(v[1][9]), "=r"(v[1][10]), "=r"(v[1][11]), "=r"(v[1][12]), "=r"(v[1][13]), "=r"(v[1][14]), "=r"(v[1][15]),
+          "=r"(v[2][0]), "=r"(v[2][1]), "=r"(v[2][2]), "=r"(v[2][3]), "=r"(v[2][4]), "=r"(v[2][5]), "=r"(v[2][6]), "=r"(v[2][7]),
+          "=r"(v[2][8]), "=r"(v[2][9]), "=r"(v[2][10]), "=r"(v[2][11]), "=r"(v[2][12]), "=r"(v[2][13]), "=r"(v[2][14]), "=r"(v[2][15]),
+          "=r"(v[3][0]), "=r"(v[3][1]), "=r"(v[3][2]), "=r"(v[3][3]), "=r"(v[3][4]), "=r"(v[3][5]), "=r"(v[3][6]), "=r"(v[3][7]),
+          "=r"(v[3][8]), "=r"(v[3][9]), "=r"(v[3][10]), "=r"(v[3][11]), "=r"(v[3][12]), "=r"(v[3][13]), "=r"(v[3][14]), "=r"(v[3][15])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3) : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
@@ -804,12 +822,23 @@ __global__ void __launch_bounds__(2 * D) tree_wide_merge_kernel(const __grid_con
 
 // ---------------------------------------------------------------- weights
 // weights[t] += sum over the rows of exp(s_t - lse): keys alone, and the product the other way round: S^T = K Q^T, a tile's 128 tokens
-// by up to 256 rows, so that a thread has a token and adds its rows up by itself.  Copy and decode as above, the ring as deep as
-// the queries leave room for; two score slots, the tiles in turn.
+// by up to 128 rows, so that a thread has a token and adds its rows up by itself, whatever their number: no warp has to wait for
+// another's, and the order is always the same.  Copy and decode as above, the ring as deep as the queries leave room for; two score
+// slots, the tiles in turn.  One row is bound by HBM (8 x 32 x 4096 tokens: 50 us, 5.4 TB/s of 6.5); 128 rows (4 x 8 x 8190: 31 us)
+// by the threads' chain of loads and exponentials (5 us less without), the rest is the start and the end of a run of 14 tiles.
 template <int D>
 struct KeysPlan {
     static constexpr int RING = D == 128 ? 6 : 8, TILE_BYTES = TILE * D * 2, SEGMENTS = 8;
     static constexpr int RAW = 0, FULL = RING, EMPTY = 2 * RING, S_FULL = 3 * RING, S_FREE = S_FULL + 2, Q_FULL = S_FREE + 2, BARS = Q_FULL + 1;
+    // A product of 128 channels is eight steps into one fp32 sum, and each of them cuts off what does not fit: 4.3e-6 of the weights at
+    // scores of 25, all to one side.  Rows go in groups of 128, and a group's steps into as many sums as a slot's 256 columns have room
+    // for, added up (and rounded) by the threads: 1.9e-6 with four, 2.2e-6 with two (a plain fp32 product: 1.6e-6), for 2 us of 50.
+    static constexpr int GROUP = 128, MOST_SUMS = 4;
+    static __device__ __forceinline__ int lg_steps(int columns) {             // log2 of the steps into one sum
+        int lg = 0;
+        while ((D / 16 >> lg) > MOST_SUMS || (D / 16 >> lg) * columns > 256) ++lg;
+        return lg;
+    }
     static constexpr int ROWS = 512, OFF_AT = 512, Q_AT = OFF_AT + ROWS * 4 + 512;          // barriers and words; -lse of the rows; queries
     static_assert(8 * BARS + 8 + ROWS / 32 * 4 <= OFF_AT && Q_AT % 1024 == 0, "layout");
     static __host__ __device__ int padded(int rows) { return (rows + 15) & ~15; }
@@ -820,6 +849,42 @@ struct KeysPlan {
     }
     static __host__ __device__ int bytes(int rows) { return 1024 + ring_at(rows) + depth(rows) * TILE_BYTES; }
 };
+
+// exp(score - lse) of a token's first n rows, added to four interleaved sums: 16 rows of SUMS = 4 or 32 of 2 at a time.
+template <int SUMS>
+__device__ __forceinline__ void add_rows(float (&sum)[4], uint32_t s_at, uint32_t columns, int n, const float* off, const uint32_t* absent,
+                                         float scale, float add) {
+    constexpr int ROWS = 64 / SUMS;
+    const uint32_t pair = SUMS == 4 ? 2 * columns : 16;
+#pragma unroll 1
+    for (int c = 0; c < n; c += ROWS) {
+        uint32_t v[4][16];
+        __syncwarp();
+        tmem_ld4(v, s_at + c, s_at + columns + c, s_at + pair + c, s_at + columns + pair + c);
+        float x[ROWS];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            x[e] = __uint_as_float(v[0][e]) + __uint_as_float(v[1][e]);
+            const float y = __uint_as_float(v[2][e]) + __uint_as_float(v[3][e]);
+            if constexpr (SUMS == 4) x[e] += y;
+            else x[16 + e] = y;
+        }
+        if (const uint32_t none = absent[c >> 5] >> (c & 16)) {
+            // (no weight from these, whatever their scores are: 0 - inf)
+#pragma unroll
+            for (int e = 0; e < ROWS; ++e) x[e] = none >> e & 1 ? 0.f : x[e];
+        }
+        // (one rounding of the small difference: scores of 25 are half of 2e-6 off themselves)
+#pragma unroll
+        for (int e = 0; e < ROWS / 4; ++e) {
+            const float4 o = reinterpret_cast<const float4*>(off + c)[e];
+            sum[0] += ex2(fmaf(fmaf(x[4 * e], scale, o.x), LOG2E, add));
+            sum[1] += ex2(fmaf(fmaf(x[4 * e + 1], scale, o.y), LOG2E, add));
+            sum[2] += ex2(fmaf(fmaf(x[4 * e + 2], scale, o.z), LOG2E, add));
+            sum[3] += ex2(fmaf(fmaf(x[4 * e + 3], scale, o.w), LOG2E, add));
+        }
+    }
+}
 
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_constant__ TreeArgs p, float* __restrict__ weights, int row0, int rows) {
@@ -833,7 +898,7 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_c
     float* off = reinterpret_cast<float*>(smem + L::OFF_AT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t ring = L::depth(rows), ring_at = base + L::ring_at(rows), q_half = L::padded(rows) * 128;
-    const int groups = (rows + 255) >> 8;
+    const int groups = (rows + L::GROUP - 1) / L::GROUP;
     const bool has_tail = p.rest > 0;
     if (threadIdx.x == 0) {
 #pragma unroll 1
@@ -904,29 +969,12 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_c
                     bar_wait(bars + 8 * (L::S_FULL + slot), done & 1, dead);
                     __syncwarp();
                     fence_after();
-                    const int n = min(256, rows - 256 * g);
+                    const int n = min(L::GROUP, rows - L::GROUP * g), columns = L::padded(n), sums = D / 16 >> L::lg_steps(columns);
                     if (!__all_sync(0xFFFFFFFFu, gone)) {
-#pragma unroll 1
-                        for (int c = 0; c < n; c += 32) {
-                            uint32_t v[32];
-                            __syncwarp();
-                            tmem_ld(v, s_at + c);
-                            const float4* o4 = reinterpret_cast<const float4*>(off + 256 * g + c);
-                            if (const uint32_t none = absent[8 * g + (c >> 5)]) {
-                                // (no weight from these, whatever their scores are: 0 - inf)
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) v[e] = none >> e & 1 ? 0 : v[e];
-                            }
-                            // exp(score - lse), one rounding of the small difference: scores of 25 are half of 2e-6 off themselves
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const float4 o = o4[e];
-                                sum[0] += ex2(fmaf(fmaf(__uint_as_float(v[4 * e]), p.scale, o.x), LOG2E, add));
-                                sum[1] += ex2(fmaf(fmaf(__uint_as_float(v[4 * e + 1]), p.scale, o.y), LOG2E, add));
-                                sum[2] += ex2(fmaf(fmaf(__uint_as_float(v[4 * e + 2]), p.scale, o.z), LOG2E, add));
-                                sum[3] += ex2(fmaf(fmaf(__uint_as_float(v[4 * e + 3]), p.scale, o.w), LOG2E, add));
-                            }
-                        }
+                        const float* o = off + L::GROUP * g;
+                        const uint32_t* none = absent + L::GROUP / 32 * g;
+                        if (sums == 4) add_rows<4>(sum, s_at, columns, n, o, none, p.scale, add);
+                        else add_rows<2>(sum, s_at, columns, n, o, none, p.scale, add);
                     }
                     fence_before();
                     __syncwarp();
@@ -952,7 +1000,8 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_c
 #pragma unroll 1
             for (int j0 = 0; j0 < s.c; j0 += 2) {
                 for (int g = 0; g < groups; ++g) {
-                    const uint32_t idesc_n = (uint32_t)(min(256, L::padded(rows) - 256 * g) >> 3) << 17;
+                    const int columns = L::padded(min(L::GROUP, rows - L::GROUP * g)), lg = L::lg_steps(columns), first_step = (1 << lg) - 1;
+                    const uint32_t idesc_n = (uint32_t)(columns >> 3) << 17;
 #pragma unroll
                     for (int slot = 0; slot < 2; ++slot) {
                         if (j0 + slot >= s.c) continue;
@@ -968,20 +1017,21 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_c
                         bar_wait(bars + 8 * (L::S_FREE + slot), ((slot ? items1 : items0) & 1) ^ 1, dead);
                         fence_after();
                         const bool tail = has_tail && s.t0 + j0 + slot == p.tiles - 1;
-                        const uint32_t q = operand(base + L::Q_AT + g * 32768, 16), d = tmem + slot * 256, half = q_half >> 4;
+                        const uint32_t q = operand(base + L::Q_AT + g * (L::GROUP * 128), 16), d = tmem + slot * 256, half = q_half >> 4;
                         if (tail) {
                             const uint32_t k = operand(k_at[slot], 16), idesc = instruction(0, false) | idesc_n;
                             if (elect()) {
 #pragma unroll
                                 for (int kk = 0; kk < D / 16; ++kk)
-                                    mma_ss(d, k + (kk >> 2) * (16384 >> 4) + (kk & 3) * (32 >> 4), q + (kk >> 2) * half + (kk & 3) * (32 >> 4), idesc, kk > 0);
+                                    mma_ss(d + (kk >> lg) * columns, k + (kk >> 2) * (16384 >> 4) + (kk & 3) * (32 >> 4),
+                                           q + (kk >> 2) * half + (kk & 3) * (32 >> 4), idesc, kk & first_step);
                             }
                         } else {
                             const uint32_t k = operand(k_at[slot], D * 128), idesc = instruction(0, false, true) | idesc_n;
                             if (elect()) {
 #pragma unroll
                                 for (int kk = 0; kk < D / 16; ++kk)
-                                    mma_ss(d, k + kk * (2048 >> 4), q + (kk >> 2) * half + (kk & 3) * (32 >> 4), idesc, kk > 0);
+                                    mma_ss(d + (kk >> lg) * columns, k + kk * (2048 >> 4), q + (kk >> 2) * half + (kk & 3) * (32 >> 4), idesc, kk & first_step);
                             }
                         }
                         if (elect()) {
