@@ -3,15 +3,19 @@
 // CTA = one SM, a contiguous run of 128-token tiles as in akv_tree.cu; a unit is up to 256 query rows of a (batch, KV head).
 //   warp  17      copies the planes of a tile (K or V: 32 KB at head size 128) into a ring, three bulk copies for 64 tokens
 //   warps 8..15   decode: four warps for 64 tokens' bytes, to fp16 operands in the same place - they take as much - by way of registers
-//   warp  16      one thread issues the products: S = Q K^T (128 rows x 128 tokens), O += P V
+//   warp  16      issues the products: S = Q K^T (128 rows x 128 tokens), O += P V
 //   warps 0..7    two softmax groups of 128 threads, a thread per query row: S from tensor memory, P back into its place
 // Everything comes in twos: S, O, P and a softmax group per slot.  With up to 128 rows the slots take the tiles in turn (each
-// with an output of its own, joined at the end), with more each has half of the rows and takes every tile.  While one slot's
-// softmax runs, the other's products do.
+// with an output of its own, joined at the end), with more (a slot has no more) each has half of the rows and takes every tile.  While
+// one slot's softmax runs, the other's products do.
 // K planes run along tokens and V planes along channels - along the n of either product, not along its sum: the operand tiles
 // are "MN-major", rows of 64 elements (128 bytes), so that a decoded piece of 16 elements is two 16-byte stores.  Only the
 // tail's keys (fp16 rows of channels) are K-major.
 // Tensor memory: columns 0..255 S (P in the same columns as fp16), 256..511 O.
+// What bounds it: up to 128 rows the planes' way into the operands (16 x 8 x 8190 tokens, 48 rows: 125 us, of which the copies alone
+// are 90 and HBM's floor 83: decode, products and softmax share the SM's shared memory with them); 256 rows (4 x 8 x 8192: 65 us)
+// the chain of a slot - 1.3 us of softmax, bound by exponentials, and 1.1 us from P to the next S - and 25 us of a call's start, of
+// the records and of the merge.
 #include <limits.h>
 
 #include "akv_tree.cuh"
@@ -215,7 +219,7 @@ __device__ __forceinline__ Masked mask_of(const __half* mask, int count, int lan
 // Eight elements from their high bytes and nibbles, in the order in which two permutes a pair suffice: 0 2 1 3, 4 6 5 7.  Of K that is
 // the order of the scores' columns, and V's tokens are stored in it; of V it is the order of the output's columns.
 __device__ __forceinline__ constexpr int swapped(int i) { return (i & ~3) | (i & 1) << 1 | (i >> 1 & 1); }     // (its own inverse)
-__device__ __forceinline__ uint4 halves8(uint32_t h0, uint32_t h1, uint32_t m, uint32_t l) {
+__device__ __forceinline__ uint4 swapped8(uint32_t h0, uint32_t h1, uint32_t m, uint32_t l) {
     const uint32_t even = (m & 0xF0F0F0F0u) | ((l >> 4) & 0x0F0F0F0Fu), odd = ((m << 4) & 0xF0F0F0F0u) | (l & 0x0F0F0F0Fu);
     return make_uint4(__byte_perm(even, h0, 0x6140), __byte_perm(odd, h0, 0x7150), __byte_perm(even, h1, 0x6342), __byte_perm(odd, h1, 0x7352));
 }
@@ -347,8 +351,8 @@ __device__ __forceinline__ void decode_role(const TreeArgs& p, uint32_t ring_at,
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const uint32_t f = (u & 1 ? f1 : f0) + (u >> 1) * 4096;
-                    sts128(f, halves8(w[u][0], w[u][1], w[u][4], w[u][6]));
-                    sts128(f ^ 16, halves8(w[u][2], w[u][3], w[u][5], w[u][7]));
+                    sts128(f, swapped8(w[u][0], w[u][1], w[u][4], w[u][6]));
+                    sts128(f ^ 16, swapped8(w[u][2], w[u][3], w[u][5], w[u][7]));
                 }
                 if (some < TILE || left != ALL) {
                     // (a token that does not exist or is masked away counts as zero, whatever there is: 0 * NaN would be NaN)
@@ -444,8 +448,9 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
 }
 
 // ---------------------------------------------------------------- softmax
-// A CTA's part of a row: rows of four channels side by side, as the threads of a warp have them and write them (a row after the other,
-// the lanes' stores met in no line: SEPARATE), the maxima and sums behind them.  As in akv_tree.cu, slot 0 is of a run's first unit, slot 1 of its last.
+// A CTA's part of a unit: four channels of all rows side by side, as the lanes of a warp have and write them (row after row, no two
+// lanes' stores shared a line: 75.5 us against 70.6 at 256 rows x 8192 tokens), the rows' maxima and sums behind them.  As in
+// akv_tree.cu, slot 0 is of a run's first unit, slot 1 of its last.
 struct Record {
     float* at;
     int rows, D, row;

@@ -276,6 +276,30 @@ def test_replayed_and_on_a_side_stream(akv_lib):
         assert torch.equal(x.layer.restk[0, 2:5], x.k[0, [0, 3, 5]]) and torch.equal(x.layer.restv[1, 2:5], x.v[1, [1, 2, 10]])
 
 
+@pytest.mark.parametrize("B,n,Hq,H,T,masked", [(1, 777, 4, 4, 3, False), (20, 300, 8, 8, 2, True), (2, 900, 16, 2, 20, True)])
+def test_captured_twice_side_by_side(akv_lib, B, n, Hq, H, T, masked):
+    """Two graphs of the same layer, each with its own outputs, replayed in turn and at once, against the eager call."""
+    x = make(B, n, Hq, H, 128, T, seed=n)
+    mask = None
+    if masked:
+        mask = torch.zeros(B, 1, 1, n, dtype=torch.half, device=DEV)
+        mask[-1, ..., :n // 2] = -math.inf
+    want = x.layer.tree_attention(x.q, x.k, x.v, x.tree, mask=mask, lse=True)
+    graphs, got = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            got.append(x.layer.tree_attention(x.q, x.k, x.v, x.tree, mask=mask, lse=True))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for out, lse in got:
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
 def test_two_streams_at_once(akv_lib):
     a, b = make(2, 700, 8, 2, 128, 16, seed=1), make(1, 1500, 4, 4, 64, 40, seed=2)
     want = [x.layer.tree_attention(x.q, x.k, x.v, x.tree) for x in (a, b)]
