@@ -79,7 +79,7 @@ __device__ __noinline__ void bar_wait_slow(uint32_t a, uint32_t parity, volatile
             if (t0 == 0) t0 = t;
             else if (t - t0 > 1000000000ull) {
                 *dead = 1;
-                atomicOr(&g_tree_wait_gave_up, 4u);
+                atomicOr(&g_tree_wait_gave_up, 8u);
                 return;
             }
         }

@@ -41,7 +41,7 @@ const char* akv_last_error(void);
 /*
  * Device-side health flag (no counterpart in the reference): non-zero once a bounded wait inside a kernel of this
  * library gave up - the kernel then returned early and its output is invalid.  Never expected in a healthy run.
- * Reading it copies a word from the device, i.e. synchronises; negative values are AKV_ERR_* codes.  (Bit 4: a wait of
+ * Reading it copies a word from the device, i.e. synchronises; negative values are AKV_ERR_* codes.  (Bit 3: a wait of
  * akv_tree_attention or akv_tree_weights, whose outputs are then NaN.)
  */
 int akv_device_error_flag(void);
