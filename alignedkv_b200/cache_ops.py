@@ -123,10 +123,12 @@ def tree_attention(cache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tre
     if out is None:
         out = torch.empty_like(q)
     else:
-        _need("out", out, tuple(q.shape), torch.half, c.index)
+        begin = _need("out", out, tuple(q.shape), torch.half, c.index)
+        if any(begin < t.data_ptr() + 2 * t.numel() and t.data_ptr() < begin + 2 * out.numel() for t in (q, k, v)):
+            raise RuntimeError("out: overlaps q, k or v")
     mask_ptr, mask_stride = c.mask(mask)
     group, lib = Hq // c.H, _lib.load()
-    sums = torch.empty((c.B, T, Hq), dtype=torch.float32, device=c.device) if lse else None
+    sums = q.new_empty((c.B, T, Hq), dtype=torch.float32) if lse else None
     with c.here():
         ws = torch.empty(lib.akv_tree_scratch_bytes(c.B, c.H, group, c.D, rest_start, T), dtype=torch.uint8, device=c.device)
         rc = lib.akv_tree_attention(

@@ -46,9 +46,10 @@ struct Ring {
     int lane, put, get;            // steps: slots filled next, read next
     // what is copied next: step of a tile of (batch, KV head) bh; left = tiles from this one on
     int bh, left, step, tile, unit, plane_tiles;
+    unsigned long long gone;       // a bit per tile from this one on: its mask leaves nothing
 
-    // Tiles first .. last - 1 of units of p.tiles tiles.
-    __device__ __forceinline__ void start(const TreeArgs& p, uint32_t at, int of_lane, int first, int last) {
+    // Tiles first .. last - 1 of units of p.tiles tiles, without those of `masked`.
+    __device__ __forceinline__ void start(const TreeArgs& p, uint32_t at, int of_lane, int first, int last, unsigned long long masked) {
         base = at;
         lane = of_lane;
         put = get = step = 0;
@@ -57,8 +58,21 @@ struct Ring {
         tile = first - unit * p.tiles;
         left = last - first;
         bh = unit;
+        gone = masked;
+        skip(p);
 #pragma unroll 1
         for (int i = 0; i < STEPS - 1; ++i) fill(p);
+    }
+    __device__ __forceinline__ void next(const TreeArgs& p) {
+        --left;
+        gone >>= 1;
+        if (++tile == p.tiles) {
+            tile = 0;
+            bh = ++unit;
+        }
+    }
+    __device__ __forceinline__ void skip(const TreeArgs& p) {
+        while (gone & 1) next(p);
     }
     __device__ __forceinline__ uint32_t slot(int i) const { return base + (uint32_t)i * STEP_BYTES; }
 
@@ -148,11 +162,8 @@ struct Ring {
             }
             if (++step == steps) {
                 step = 0;
-                --left;
-                if (++tile == p.tiles) {
-                    tile = 0;
-                    bh = ++unit;
-                }
+                next(p);
+                skip(p);
             }
         }
         cp_async_commit();
@@ -190,6 +201,24 @@ struct Ring {
         }
     }
 };
+
+// Of a run's first 64 tiles those whose mask takes every token away (left padding): neither copied nor looked at.  (A run is longer
+// than that from 9.7 million cached (token, KV head) rows on; its tiles behind are masked score by score.)
+__device__ __forceinline__ unsigned long long masked_tiles(const TreeArgs& p, int first, int last, int lane) {
+    unsigned long long gone = 0;
+    if (!p.mask) return gone;
+#pragma unroll 4
+    for (int i = 0; i < min(last - first, 64); ++i) {
+        const int unit = (unsigned)(first + i) / (unsigned)p.tiles, tile = first + i - unit * p.tiles, count = p.nb * BLK - tile * TILE;
+        const uint16_t* mask = reinterpret_cast<const uint16_t*>(p.mask) + (unsigned)unit / (unsigned)p.H * p.mask_stride + tile * TILE;
+        bool none = tile < p.tiles - 1;
+#pragma unroll
+        for (int e = 0; e < TILE; e += 32)
+            if (tile < p.tiles - 1 && lane + e < count) none = none && mask[lane + e] == 0xFC00u;
+        gone |= (unsigned long long)__all_sync(0xFFFFFFFFu, none) << i;
+    }
+    return gone;
+}
 
 // Scores of a plane tile: s[j][c] = row g (c < 2) or g + 8, token 16 (2t + (c & 1)) + j.
 template <int D, int STEPS>
@@ -343,7 +372,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
     uint4* qf = reinterpret_cast<uint4*>(smem + (size_t)warp * WARP_BYTES + steps_of<TEAM> * STEP_BYTES);
     uint4* pf = qf + 256;
     Ring ring;
-    ring.start(p, smem_u32(smem) + warp * WARP_BYTES, lane, first, last);
+    unsigned long long gone = masked_tiles(p, first, last, lane);
+    ring.start(p, smem_u32(smem) + warp * WARP_BYTES, lane, first, last, gone);
     // records: of a run's first unit in slot 0, of its last in slot 1 (those between are whole); a team's in place of the rings
     auto record = [&](int unit, int r) {
         return TEAM ? reinterpret_cast<float*>(smem + (size_t)warp * WARP_BYTES) + r * (D + 4)
@@ -361,6 +391,9 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
         for (int j = 0; j < N; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 #pragma unroll 1
         for (int tile = t0; tile < min(t1, p.tiles - 1); ++tile) {
+            const bool none = gone & 1;
+            gone >>= 1;
+            if (none) continue;
             {
                 float s[16][4];
                 plane_scores(s, qf, p, ring);
@@ -410,6 +443,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
             }
         }
         if (t1 == p.tiles) {
+            gone >>= 1;
             // The tail, 16 tokens at a time: rows of fp16 values.
             const uint8_t* seen = p.tree + b * p.tree_stride;
             const uint8_t* mine[2];

@@ -405,8 +405,8 @@ int akv_shard_step(void* k_first_8, void* k_mid_4, void* k_last_4, void* v_first
  * sums over the exact cached values (every plane is read), rounded once.  tree: bytes [T,T] per sequence, tree_stride bytes apart
  * (0 = one for all), non-zero where the row's token sees the column's.  mask (NULL = none): fp16 row per sequence as in
  * akv_decode_step_masked, entries [0, rest_start + rest_len); -inf takes a token away whatever its values are.  A row that sees
- * nothing is 0, its lse -inf.  lse (may be NULL): fp32 [B,T,Hq], log of the sum of exponentials.  scratch: at least
- * akv_tree_scratch_bytes(..., rest_start, drafted) bytes, any contents.
+ * nothing is 0, its lse -inf.  out must not overlap an input.  lse (may be NULL): fp32 [B,T,Hq], log of the sum of exponentials.
+ * scratch: at least akv_tree_scratch_bytes(..., rest_start, drafted) bytes, any contents.
  *
  * akv_tree_weights: weights fp32 [B,Hkv,max_seq_len], entry t of head h += sum over its T * group rows of exp(score - lse[r]) for
  * t < rest_start + rest_len.  No atomics: the same call on the same state gives the same bits.

@@ -334,6 +334,8 @@ def test_refusals(akv_lib):
         L.tree_attention(x.q, x.k, x.v, t, mask=torch.zeros(2, 1, 1, 69, dtype=torch.half, device=DEV))
     with pytest.raises(RuntimeError, match="out: expected"):
         L.tree_attention(x.q, x.k, x.v, t, out=torch.empty(2, 5, 4, 64, dtype=torch.half, device=DEV))
+    with pytest.raises(RuntimeError, match="out: overlaps"):
+        L.tree_attention(x.q, x.k, x.v, t, out=x.q)
     with pytest.raises(RuntimeError, match="drafted tokens"):
         big = torch.zeros(2, 65, 4, 128, dtype=torch.half, device=DEV)
         L.tree_attention(big, big[:, :, :2].contiguous(), big[:, :, :2].contiguous(), t)
