@@ -89,8 +89,8 @@ struct Ring {
             const long long o = there ? (long long)b * D : 0;
             copy16(to + b * 1024 + at, h + o * BLK, there);
             copy16(to + b * 1024 + 512 + (at ^ 64), h + o * BLK + 512, there);
-            copy16(to + 2048 + b * 512 + nib, m + o * (BLK / 2), there);
-            copy16(to + 3072 + b * 512 + nib, l + o * (BLK / 2), there);
+            copy16(to + STEP_BYTES / 2 + b * 512 + nib, m + o * (BLK / 2), there);
+            copy16(to + STEP_BYTES / 4 * 3 + b * 512 + nib, l + o * (BLK / 2), there);
         }
     }
     __device__ __forceinline__ void copy_v(const TreeArgs& p, uint32_t to, int vs) const {
