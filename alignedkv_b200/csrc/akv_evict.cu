@@ -129,7 +129,8 @@ __device__ __forceinline__ uint32_t cluster_ld(const void* p, uint32_t cta) {
 // A cluster per row; a CTA has `share` consecutive places and keeps their keys in shared memory: one read of the weights, whatever is
 // counted.  The keep-th largest key by four counts of eight bits (in eight columns: few lanes of a warp meet, although weights crowd into
 // few exponents), added up over the cluster through distributed shared memory; every CTA draws the same
-// conclusion.  Then ties, free places and survivors behind are numbered in order: per warp, per CTA, per cluster.
+// conclusion.  Then ties, free places and survivors behind are numbered in order: per warp, per CTA, per cluster.  Bound by latency: a
+// load, four rounds of three barriers, three numberings (256 rows of 4096: 18 us of 144; 8 rows of 131072: 32 of 137).
 constexpr int SEL_MOST = 40960, SEL_CTAS = 8;      // keys a CTA can keep, CTAs of a row
 template <int SEL_NT>
 __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
@@ -143,6 +144,10 @@ __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
     uint32_t ctas, rank;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    auto sync_all = [&] {                              // (a cluster's barrier for one CTA costs 2 us of a call)
+        if (ctas == 1) __syncthreads();
+        else cluster_sync();
+    };
     const size_t row = blockIdx.y;
     const float* w = a.weights + row * a.L;
     int* pos = a.positions + row * a.L;
@@ -187,11 +192,13 @@ __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
             for (int j = 0; j < 8; ++j) c += hist[j * 257 + tid];
             sums[round & 1][tid] = c;
         }
-        cluster_sync();
+        sync_all();
         // thread: digit 255 - tid; keys with a larger one, by the sums of the lanes and warps in front
         uint32_t c = 0, above = 0;
         if (tid < 256) {
-            for (uint32_t r = 0; r < ctas; ++r) c += cluster_ld(&sums[round & 1][255 - tid], r);
+            if (ctas == 1) c = sums[round & 1][255 - tid];
+            else
+                for (uint32_t r = 0; r < ctas; ++r) c += cluster_ld(&sums[round & 1][255 - tid], r);
             above = c;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -236,7 +243,7 @@ __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
     for (int i = i0; i < i1; i += 32) ties += __popc(__ballot_sync(0xFFFFFFFFu, i + lane < i1 && at(i + lane) == prefix));
     number(0, ties);
     if (tid == 0) totals[0][0] = scan[0][SEL_W];
-    cluster_sync();
+    sync_all();
     uint32_t tie0 = scan[0][warp];
     for (uint32_t r = 0; r < rank; ++r) tie0 += cluster_ld(&totals[0][0], r);
     // (bits: the place's token stays; as many words as the warp has groups of 32, in the same order twice)
@@ -261,7 +268,7 @@ __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
         totals[1][0] = scan[1][SEL_W];
         totals[1][1] = scan[2][SEL_W];
     }
-    cluster_sync();
+    sync_all();
     uint32_t h = scan[1][warp], m = scan[2][warp];
     for (uint32_t r = 0; r < rank; ++r) {
         h += cluster_ld(&totals[1][0], r);
@@ -282,7 +289,7 @@ __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
         m += __popc(mb);
     }
     if (a.keep == a.n && rank == 0 && tid == 0) start[a.keep / BLK] = 0;      // (no place behind: nothing moves)
-    cluster_sync();                                    // (no CTA leaves while another reads its counts)
+    sync_all();                                    // (no CTA leaves while another reads its counts)
 }
 
 // CTA = one block of 64 places in front of `keep`: its free places take the survivors of the same numbers.  Survivors are read
