@@ -282,26 +282,34 @@ template <int D>
 __device__ __noinline__ bool tail_share(const TreeArgs& p, int b, int h, bool value, uint32_t slot, int warp, int lane) {
     const int region = warp >> 2, k = (warp & 3) * 8 + (lane >> 2), qd = lane & 3, x = ((2 * qd) ^ (k & 7)) << 4;
     const __half *rest = value ? p.restv : p.restk, *drafted = value ? p.vd : p.kd;
-    bool odd = false;
-#pragma unroll 1
+    const int side = D == 128 ? (lane >> 2 ^ lane >> 3) & 1 : 0;
+    auto half_of = [&](int u) { return D == 128 ? (side ^ u) & 1 : 0; };
+    auto row_at = [&](int u) { return (D == 128 ? u >> 1 : u) * 32 + k; };
+    uint4 v[D / 32][2];                                // (all requested before the first is used: one round trip)
+#pragma unroll
     for (int u = 0; u < D / 32; ++u) {
-        const int half = D == 128 ? ((lane >> 2 ^ lane >> 3) ^ u) & 1 : 0, row = (D == 128 ? u >> 1 : u) * 32 + k;
-        const int y = region * BLK + row, d = y - p.rest;
-        uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        const int y = region * BLK + row_at(u), d = y - p.rest;
+        v[u][0] = v[u][1] = make_uint4(0, 0, 0, 0);
         if (y < p.tail) {
             const __half* src = d < 0 ? rest + ((long long)(b * BLK + y) * p.H + h) * D : drafted + ((long long)(b * p.T + d) * p.H + h) * D;
-            const uint4* from = reinterpret_cast<const uint4*>(src + half * 64 + qd * 16);
-            v[0] = __ldg(from);
-            v[1] = __ldg(from + 1);
+            const uint4* from = reinterpret_cast<const uint4*>(src + half_of(u) * 64 + qd * 16);
+            v[u][0] = __ldg(from);
+            v[u][1] = __ldg(from + 1);
         }
+    }
+    bool odd = false;
+#pragma unroll
+    for (int u = 0; u < D / 32; ++u) {
+        const int half = half_of(u), row = row_at(u);
         const uint32_t at = slot + (value ? region * D * 128 + half * 8192 : region * 8192 + half * 16384) + row * 128 + x;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+            uint4 y = v[u][e];
             if (value) {
-                v[e] = make_uint4(finite_halves(v[e].x, odd), finite_halves(v[e].y, odd), finite_halves(v[e].z, odd), finite_halves(v[e].w, odd));
-                v[e] = reorder8(v[e]);
+                y = make_uint4(finite_halves(y.x, odd), finite_halves(y.y, odd), finite_halves(y.z, odd), finite_halves(y.w, odd));
+                y = reorder8(y);
             }
-            sts128(at ^ (16 * e), v[e]);
+            sts128(at ^ (16 * e), y);
         }
     }
     return odd;
@@ -892,7 +900,8 @@ __device__ __forceinline__ void add_rows(float (&sum)[4], uint32_t s_at, uint32_
 }
 
 template <int D>
-__global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_constant__ TreeArgs p, float* __restrict__ weights, int row0, int rows) {
+__global__ void __launch_bounds__(THREADS, 1)
+weights_wide_kernel(const __grid_constant__ TreeArgs p, float* __restrict__ weights, int row0, int rows) {
     using L = KeysPlan<D>;
     extern __shared__ uint8_t raw[];
     uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
@@ -1036,7 +1045,8 @@ __global__ void __launch_bounds__(THREADS, 1) weights_wide_kernel(const __grid_c
                             if (elect()) {
 #pragma unroll
                                 for (int kk = 0; kk < D / 16; ++kk)
-                                    mma_ss(d + (kk >> lg) * columns, k + kk * (2048 >> 4), q + (kk >> 2) * half + (kk & 3) * (32 >> 4), idesc, kk & first_step);
+                                    mma_ss(d + (kk >> lg) * columns, k + kk * (2048 >> 4), q + (kk >> 2) * half + (kk & 3) * (32 >> 4), idesc,
+                                           kk & first_step);
                             }
                         }
                         if (elect()) {
