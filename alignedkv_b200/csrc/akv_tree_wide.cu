@@ -13,7 +13,7 @@
 // tail's keys (fp16 rows of channels) are K-major.
 // Tensor memory: columns 0..255 S (P in the same columns as fp16), 256..511 O.
 // What bounds it: up to 128 rows the planes' way into the operands (16 x 8 x 8190 tokens, 48 rows: 125 us, of which the copies alone
-// are 90 and HBM's floor 83: decode, products and softmax share the SM's shared memory with them); 256 rows (4 x 8 x 8192: 65 us)
+// are 90 and HBM's floor 83: decode, products and softmax share the SM's shared memory with them); 256 rows (4 x 8 x 8192: 66 us)
 // the chain of a slot - 1.3 us of softmax, bound by exponentials, and 1.1 us from P to the next S - and 25 us of a call's start, of
 // the records and of the merge.
 #include <limits.h>
