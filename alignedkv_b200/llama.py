@@ -98,6 +98,7 @@ class LlamaDecoder:
                            for _ in range(cfg.num_hidden_layers)]
             self.vcache = [torch.zeros_like(t) for t in self.kcache]
         self.pos = 0
+        self._drafts = None                         # (pos, keys and values of each layer) of the last `verify`
 
     # ------------------------------------------------------------------ one transformer layer
     def _layer(self, i: int, x: torch.Tensor, pos: torch.Tensor, prompt: bool) -> torch.Tensor:
@@ -243,12 +244,15 @@ class LlamaDecoder:
     def prefill(self, ids: torch.Tensor) -> torch.Tensor:
         """ids [B,S] -> logits [B,V] of the last prompt position; fills every layer's cache."""
         assert self.pos == 0 and ids.shape[0] == self.B and ids.shape[1] <= self.L
+        self._drafts = None
         return self._forward(ids, True)
 
     @torch.no_grad()
     def step(self, ids: torch.Tensor) -> torch.Tensor:
-        """ids [B] (one token per sequence) -> logits [B,V]; appends to every layer's cache."""
+        """ids [B] (one token per sequence) -> logits [B,V]; appends to every layer's cache.  Drafts of an earlier `verify` are
+        dropped: their keys were made for the position that this token takes."""
         assert (self.caches[0].cache_len if self.attention == "alignedkv" else self.pos) + 1 <= self.L
+        self._drafts = None
         if getattr(self, "_segs", None) is not None:
             return self._step_graphs(ids)       # (the returned logits are overwritten by the next step)
         return self._forward(ids.view(self.B, 1), False)
@@ -257,7 +261,8 @@ class LlamaDecoder:
     def verify(self, ids: torch.Tensor, parents: torch.Tensor, weights: bool = False) -> torch.Tensor:
         """Logits [B,T,V] of T drafted tokens (ids [B,T], T at most 64) that are not in the caches yet.  parents: int64 [T], the
         tree they form in every sequence: the node that each one follows, a lower index, or -1 for the last cached token.
-        `accept` appends some of them.  weights=True also adds the queries' attention weights to each layer's (`evict`)."""
+        `accept` appends some of them, as long as neither `step` nor a roll-back comes between.  weights=True also adds the queries'
+        attention weights to each layer's (`evict`)."""
         assert self.attention == "alignedkv", "only the AlignedKV path drafts tokens"
         cfg = self.cfg
         H, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
@@ -287,15 +292,15 @@ class LlamaDecoder:
             h = _rms_norm(x, p["norm2"], cfg.rms_norm_eps)
             gate, wide = F.linear(h, p["w_gate_up"]).chunk(2, dim=-1)
             x = torch.addmm(x.view(B * T, -1), F.silu(gate).mul_(wide).view(B * T, -1), p["w_down"].t()).view(B, T, -1)
-        self._drafts = drafts
+        self._drafts = (self.pos, drafts)
         return F.linear(_rms_norm(x, self.final_norm, cfg.rms_norm_eps), self.lm_head)
 
     @torch.no_grad()
     def accept(self, path: torch.Tensor) -> None:
         """Append nodes path[b, 0..n-1] (int [B,n]: a chain from the root) of the last `verify` to the caches; once."""
-        drafts, self._drafts = getattr(self, "_drafts", None), None
-        if drafts is None:
-            raise RuntimeError("accept: no drafted tokens (call verify first)")
+        (pos, drafts), self._drafts = self._drafts or (None, None), None
+        if pos != self.pos:
+            raise RuntimeError("accept: no drafted tokens at this position (call verify first)")
         path = path.to(device=self.device, dtype=torch.int32).contiguous()
         for cache, (k, v) in zip(self.caches, drafts):
             cache.tree_commit(k, v, path)
