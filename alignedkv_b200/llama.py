@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from . import _lib
+from . import _lib, cache_ops
 from .decode import DecodeLayer
 from .extension._planes import observed
 
@@ -297,14 +297,23 @@ class LlamaDecoder:
 
     @torch.no_grad()
     def accept(self, path: torch.Tensor) -> None:
-        """Append nodes path[b, 0..n-1] (int [B,n]: a chain from the root) of the last `verify` to the caches; once."""
-        (pos, drafts), self._drafts = self._drafts or (None, None), None
+        """Append nodes path[b, 0..n-1] (int [B,n]: a chain from the root) of the last `verify` to the caches; once.  A call that is
+        refused changes nothing and leaves the drafts as they were."""
+        pos, drafts = self._drafts or (None, None)
         if pos != self.pos:
             raise RuntimeError("accept: no drafted tokens at this position (call verify first)")
+        if path.dim() != 2 or path.shape[0] != self.B or not 1 <= path.shape[1] <= cache_ops.MOST_DRAFTED or \
+                path.is_floating_point() or path.dtype is torch.bool:
+            raise RuntimeError(f"path: expected integers of shape [{self.B}, n] with n 1 to {cache_ops.MOST_DRAFTED}")
+        n = path.shape[1]
+        for cache in self.caches:
+            if cache.cache_len + n > cache.L:
+                raise RuntimeError(f"cache is full ({cache.L} tokens): no room for {n} behind {cache.cache_len}")
         path = path.to(device=self.device, dtype=torch.int32).contiguous()
         for cache, (k, v) in zip(self.caches, drafts):
             cache.tree_commit(k, v, path)
-        self.pos += path.shape[1]
+        self._drafts = None
+        self.pos += n
 
     @torch.no_grad()
     def evict(self, keep: int, recent: int = 0) -> None:

@@ -1,4 +1,4 @@
-"""Drafted tokens of `LlamaDecoder.verify` belong to the state that they were made for."""
+"""Drafted tokens of `LlamaDecoder.verify` belong to the state that they were made for, and survive a refused `accept`."""
 import pytest
 import torch
 
@@ -51,6 +51,26 @@ def test_a_roll_back_drops_the_drafts(akv_lib):
     with pytest.raises(RuntimeError, match="call verify"):
         dec.accept(paths(0))
     assert lengths(dec) == [S] * 3
+
+
+def test_a_refused_accept_can_be_made_again(akv_lib):
+    dec, ids = decoder(3)
+    other, _ = decoder(3)
+    for d in (dec, other):
+        d.verify(ids[:, S:S + 4], CHAIN)
+    for bad, text in ((paths(0, 1, 2, 3), "cache is full"), (torch.zeros(1, 2, dtype=torch.int64), "path"),
+                      (torch.zeros(B, 0, dtype=torch.int64), "path"), (torch.zeros(B, dtype=torch.int64), "path"),
+                      (torch.zeros(B, 2), "path"), (torch.zeros(B, 65, dtype=torch.int64), "path")):
+        with pytest.raises(RuntimeError, match=text):
+            dec.accept(bad)
+        assert lengths(dec) == [S] * 3
+    for d in (dec, other):
+        d.accept(paths(0, 1, 2))
+    assert lengths(dec) == [S + 3] * 3
+    for x, y in zip(dec.caches, other.caches):
+        assert torch.equal(x.restk, y.restk) and torch.equal(x.restv, y.restv) and torch.equal(x.k_exp_max, y.k_exp_max)
+    with pytest.raises(RuntimeError, match="call verify"):
+        dec.accept(paths(0))
 
 
 def test_an_eviction_between_is_fine(akv_lib):
