@@ -256,7 +256,7 @@ class DecodeLayer:
         """Reduce the tokens in the planes to the `keep` heaviest per (sequence, KV head) by `weights`, the last `recent`
         positions among them; residual tokens stay (`cache_ops.evict`).  The cache is then keep + rest_len tokens long, and
         `positions` [B,H,L] holds the sequence position of the token in each of the first `arranged` places (place p behind them:
-        p + shift)."""
+        p + shift).  With keep == rest_start nothing goes, and masks and snapshots hold as before."""
         if self.weights is None:
             self.weights = torch.zeros((self.B, self.H, self.L), dtype=torch.float32, device=self.device)
         if self.positions is None:
@@ -264,6 +264,8 @@ class DecodeLayer:
         cache_ops.evict(self, self.weights, self.positions, keep=keep, recent=recent, arranged=self.arranged, shift=self.shift,
                         **self._counts())
         gone = self.rest_start - keep
+        if gone == 0:
+            return
         self.evictions += 1
         self.arranged, self.shift = keep, self.shift + gone
         self.rest_start -= gone
