@@ -70,7 +70,7 @@ class DecodeLayer:
         self._index = self.device.index if self.device.index is not None else torch.cuda.current_device()
         self._q_shape, self._kv_shape = (bsz, 1, self.Hq, head_dim), (bsz, 1, n_heads, head_dim)
         self.launches = 0
-        self.weights = self.positions = None  # fp32 / int32 [B,Hkv,L], made by the first tree_weights or evict
+        self.weights = self.positions = None  # fp32 / int32 [B,Hkv,L], made by the first tree_weights / evict
         self.evictions = self.arranged = self.shift = 0
 
     @property
@@ -256,12 +256,16 @@ class DecodeLayer:
         """Reduce the tokens in the planes to the `keep` heaviest per (sequence, KV head) by `weights`, the last `recent`
         positions among them; residual tokens stay (`cache_ops.evict`).  The cache is then keep + rest_len tokens long, and
         `positions` [B,H,L] holds the sequence position of the token in each of the first `arranged` places (place p behind them:
-        p + shift).  With keep == rest_start nothing goes, and masks and snapshots hold as before."""
-        if self.weights is None:
-            self.weights = torch.zeros((self.B, self.H, self.L), dtype=torch.float32, device=self.device)
+        p + shift).  With keep == rest_start nothing goes, and masks and snapshots hold as before.  Without any votes
+        (`tree_weights`) only recent == keep, a sliding window, says what stays."""
+        if self.weights is None and recent < keep < self.rest_start:
+            raise RuntimeError("weights: no query has voted yet (tree_weights), and `recent` alone does not fill `keep`")
+        weights = self.weights
+        if weights is None:
+            weights = torch.zeros((self.B, self.H, self.L), dtype=torch.float32, device=self.device)
         if self.positions is None:
             self.positions = torch.zeros((self.B, self.H, self.L), dtype=torch.int32, device=self.device)
-        cache_ops.evict(self, self.weights, self.positions, keep=keep, recent=recent, arranged=self.arranged, shift=self.shift,
+        cache_ops.evict(self, weights, self.positions, keep=keep, recent=recent, arranged=self.arranged, shift=self.shift,
                         **self._counts())
         gone = self.rest_start - keep
         if gone == 0:

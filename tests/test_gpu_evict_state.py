@@ -10,6 +10,22 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 
 
+def test_without_votes(akv_lib):
+    """Sums that nobody has formed say nothing about which tokens are heavy: refused, unless `recent` alone decides."""
+    layer, _, _, _ = filled(1, 2, 300, 128, seed=1)
+    with pytest.raises(RuntimeError, match="weights"):
+        layer.evict(128, 64)
+    assert (layer.rest_start, layer.cache_len, layer.evictions) == (256, 300, 0) and layer.weights is None
+    k, v = (t.clone() for t in dense(layer))
+    layer.evict(128, recent=128)
+    assert (layer.rest_start, layer.cache_len, layer.evictions) == (128, 172, 1)
+    # the second half moved into the first, in order
+    assert torch.equal(dense(layer)[0], k[:, :, 128:]) and torch.equal(dense(layer)[1], v[:, :, 128:])
+    assert torch.equal(layer.positions[..., :128], torch.arange(128, 256, dtype=torch.int32, device=DEV).expand(1, 2, -1))
+    with pytest.raises(RuntimeError, match="weights"):
+        layer.evict(64)                               # a window does not vote either
+
+
 def test_nothing_to_evict(akv_lib):
     """keep == the tokens in the planes: all stay in their places, so masks and older snapshots still hold."""
     layer, k, v, gen = filled(2, 2, 200, 128, seed=2, room=100)
