@@ -72,6 +72,7 @@ class DecodeLayer:
         self.launches = 0
         self.weights = self.positions = None  # fp32 / int32 [B,Hkv,L], made by the first tree_weights / evict
         self.evictions = self.arranged = self.shift = 0
+        self.masked = False                   # whether a mask has been given for the cached tokens
 
     @property
     def launches(self) -> int:
@@ -130,6 +131,7 @@ class DecodeLayer:
         self.rest_len = S % column_block
         self.rest_start = full
         self.cache_len = S
+        self.masked = False
 
     @staticmethod
     def _check_token(name: str, t: torch.Tensor | None, shape: tuple) -> None:
@@ -204,6 +206,7 @@ class DecodeLayer:
         if rc != 0:
             _lib.check("decode_step", rc)
         self.last_q = q                                   # (for bytes_accounting)
+        self.masked = self.masked or mask is not None
         flush = append and self.rest_len + 1 == column_block
         qn = self.rest_start + (column_block if flush else 0)
         rest = 0 if flush else self.rest_len + (1 if append else 0)
@@ -228,7 +231,9 @@ class DecodeLayer:
             self._no_mask_after_eviction()
         if q.dim() == 4 and q.shape[2] != self.Hq:
             raise RuntimeError(f"q: {q.shape[2]} query heads, the layer has {self.Hq}")
-        return cache_ops.tree_attention(self, q, k, v, tree, mask=mask, lse=lse, out=out, **self._counts())
+        got = cache_ops.tree_attention(self, q, k, v, tree, mask=mask, lse=lse, out=out, **self._counts())
+        self.masked = self.masked or mask is not None
+        return got
 
     def tree_weights(self, q: torch.Tensor, lse: torch.Tensor, *, mask: torch.Tensor | None = None) -> torch.Tensor:
         """Add the attention weight that these queries give each cached token to `weights` [B,H,L], fp32, and return it
@@ -240,6 +245,7 @@ class DecodeLayer:
         if self.weights is None:
             self.weights = torch.zeros((self.B, self.H, self.L), dtype=torch.float32, device=self.device)
         cache_ops.tree_weights(self, q, lse, self.weights, mask=mask, **self._counts())
+        self.masked = self.masked or mask is not None
         return self.weights
 
     def tree_commit(self, k: torch.Tensor, v: torch.Tensor, path: torch.Tensor) -> None:
@@ -257,7 +263,12 @@ class DecodeLayer:
         positions among them; residual tokens stay (`cache_ops.evict`).  The cache is then keep + rest_len tokens long, and
         `positions` [B,H,L] holds the sequence position of the token in each of the first `arranged` places (place p behind them:
         p + shift).  With keep == rest_start nothing goes, and masks and snapshots hold as before.  Without any votes
-        (`tree_weights`) only recent == keep, a sliding window, says what stays."""
+        (`tree_weights`) only recent == keep, a sliding window, says what stays.
+
+        Refused once a mask has been given for the cached tokens: padding that survives (a sequence may have fewer than `keep` other
+        tokens) lies in places that differ from head to head, where no mask reaches it."""
+        if self.masked and keep < self.rest_start:
+            raise RuntimeError("mask: this cache holds masked tokens; those that survive an eviction could not be masked any more")
         if self.weights is None and recent < keep < self.rest_start:
             raise RuntimeError("weights: no query has voted yet (tree_weights), and `recent` alone does not fill `keep`")
         weights = self.weights
@@ -302,6 +313,7 @@ class DecodeLayer:
         if self.weights is not None and appended:
             self.weights[..., snap["cache_len"]:self.cache_len] = 0
         self.rest_len, self.rest_start, self.cache_len = snap["rest_len"], snap["rest_start"], snap["cache_len"]
+        self.masked = self.masked and self.cache_len > 0
 
     def reset_counters(self) -> None:
         self.launches = 0

@@ -59,3 +59,48 @@ def test_snapshot_over_an_eviction_of_nothing(akv_lib):
     expect(layer, 64, 32)                             # (places count from the start again)
     with pytest.raises(RuntimeError, match="evicted since"):
         layer.restore(snap)
+
+
+@pytest.mark.parametrize("by", ["decode", "attention", "weights"])
+@pytest.mark.parametrize("lowest", [-math.inf, -65504.0])
+def test_a_padded_batch_is_not_evicted(akv_lib, by, lowest):
+    """Survivors lie in places that differ from head to head, where no mask row can take padding away; a sequence with fewer real
+    tokens than `keep` would keep some of its padding."""
+    B, H, D, n = 2, 2, 128, 300
+    from alignedkv_b200.decode import DecodeLayer
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    layer = DecodeLayer(B, n + 100, H, D, DEV)
+    empty = layer.snapshot()
+    k, v = (torch.randn(B, n, H, D, device=DEV, generator=gen).half() for _ in range(2))
+    layer.prefill(k, v)
+    weigh(layer, gen)
+    mask = torch.zeros(B, 1, 1, n + 50, dtype=torch.half, device=DEV)
+    mask[1, ..., :250] = lowest
+    q, one = torch.randn(B, 1, H, D, device=DEV, generator=gen).half(), torch.ones(1, 1, dtype=torch.bool, device=DEV)
+    if by == "decode":
+        layer.decode(q, q, q, mask=mask)
+    elif by == "attention":
+        layer.tree_attention(q, q, q, one, mask=mask)
+    else:
+        layer.tree_weights(q, torch.zeros(B, 1, H, device=DEV), mask=mask)
+    before = layer.cache_len
+    with pytest.raises(RuntimeError, match="mask"):
+        layer.evict(128)
+    assert (layer.cache_len, layer.rest_start, layer.evictions) == (before, 256, 0)
+    layer.evict(256)                                  # nothing goes: nothing to refuse
+    # another prompt in the same layer: no mask has been given for its tokens
+    layer.restore(empty)
+    layer.prefill(k, v)
+    weigh(layer, gen)
+    expect(layer, 128, 0)
+
+
+def test_padding_without_weight_goes_first(akv_lib):
+    """What a program does that knows its padding: -inf as weight, and at least `keep` other tokens everywhere."""
+    from alignedkv_b200 import cache_ops
+    layer, _, _, gen = filled(2, 2, 640, 64, seed=6)
+    weigh(layer, gen, zeros=0.9)
+    layer.weights[1, :, :500] = -math.inf
+    layer.positions = torch.zeros(2, 2, 640, dtype=torch.int32, device=DEV)
+    cache_ops.evict(layer, layer.weights, layer.positions, rest_len=0, rest_start=640, keep=128, recent=30)
+    assert bool((layer.positions[1, :, :128] >= 500).all())
