@@ -206,8 +206,9 @@ def evict(cache, weights: torch.Tensor, positions: torch.Tensor, *, rest_len: in
     _need("positions", positions, (c.B, c.H, c.L), torch.int32, c.index)
     if keep <= 0 or keep % column_block or keep > rest_start:
         raise RuntimeError(f"keep: {keep}, expected a positive multiple of {column_block} of at most {rest_start}")
-    if not 0 <= recent <= keep or not 0 <= arranged <= rest_start or shift < 0:
-        raise RuntimeError(f"recent {recent} [0..keep], arranged {arranged} [0..{rest_start}], shift {shift} [>= 0]")
+    most = 2 ** 31 - 1 - column_block - c.L          # (positions are 32-bit numbers)
+    if not 0 <= recent <= keep or not 0 <= arranged <= rest_start or not 0 <= shift <= most:
+        raise RuntimeError(f"recent {recent} [0..keep], arranged {arranged} [0..{rest_start}], shift {shift} [0..{most}]")
     lib = _lib.load()
     with c.here():
         ws = torch.empty(lib.akv_evict_scratch_bytes(c.B, c.H, rest_start, keep), dtype=torch.uint8, device=c.device)

@@ -95,6 +95,19 @@ def test_a_padded_batch_is_not_evicted(akv_lib, by, lowest):
     expect(layer, 128, 0)
 
 
+def test_shift_beyond_32_bits(akv_lib):
+    """A position that does not fit the positions' type is refused, not cut."""
+    from alignedkv_b200 import cache_ops
+    layer, _, _, gen = filled(1, 1, 128, 64, seed=5)
+    weigh(layer, gen)
+    layer.positions = torch.zeros(1, 1, 128, dtype=torch.int32, device=DEV)
+    for shift in (2 ** 31 - 100, 2 ** 31, 2 ** 32, 2 ** 32 + 7, 2 ** 40):
+        with pytest.raises(RuntimeError, match="shift"):
+            cache_ops.evict(layer, layer.weights, layer.positions, rest_len=0, rest_start=128, keep=64, shift=shift)
+    cache_ops.evict(layer, layer.weights, layer.positions, rest_len=0, rest_start=128, keep=64, recent=64, shift=2 ** 31 - 64 - 129)
+    assert torch.equal(layer.positions[0, 0, :64].long(), torch.arange(64, 128, device=DEV) + 2 ** 31 - 64 - 129)
+
+
 def test_padding_without_weight_goes_first(akv_lib):
     """What a program does that knows its padding: -inf as weight, and at least `keep` other tokens everywhere."""
     from alignedkv_b200 import cache_ops
