@@ -1,0 +1,72 @@
+"""Attention of drafted tokens where its forms meet their edges: short last units, signs of the scale, long runs."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_tree import DEV, check, make
+from tree_reference import attend64, lse_bound, out_bound, score_error, weights64
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("B,n,Hq,H,D,T", [(1, 700, 37, 1, 128, 7), (2, 300, 257, 1, 64, 1), (1, 130, 74, 2, 128, 7), (40, 200, 53, 1, 64, 5)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_last_unit_shorter_than_the_others(akv_lib, B, n, Hq, H, D, T, masked):
+    """More than 256 rows that do not divide into their units."""
+    x = make(B, n, Hq, H, D, T, seed=n)
+    mask = wide = None
+    if masked:
+        mask = torch.zeros(B, n, dtype=torch.half, device=DEV)
+        mask[-1, :n // 2 + 7] = -math.inf
+        mask[0, n - 1] = -1.25
+        wide = mask[:, None, None].contiguous()
+    check(x, *x.layer.tree_attention(x.q, x.k, x.v, x.tree, mask=wide, lse=True), mask=mask)
+
+
+@pytest.mark.parametrize("Hq,H,T", [(4, 2, 3), (8, 1, 3), (8, 1, 20), (8, 1, 40)])
+@pytest.mark.parametrize("scale", [-0.25, -1 / math.sqrt(128), 0.0, 0.4])
+def test_scales(akv_lib, Hq, H, T, scale):
+    """Both signs and none, in the attention's forms (6 to 320 rows) and in the weights."""
+    from alignedkv_b200 import cache_ops
+    B, n, D = 2, 330, 128
+    x = make(B, n, Hq, H, D, T, seed=T, hot=4.0)
+    counts = dict(rest_len=n % 64, rest_start=n - n % 64)
+    mask = torch.zeros(B, 1, 1, n, dtype=torch.half, device=DEV)
+    mask[1, ..., :100] = -math.inf
+    mask[1, ..., 200] = -0.5
+    for m, m2 in ((None, None), (mask, mask[:, 0, 0])):
+        out, lse = cache_ops.tree_attention(x.layer, x.q, x.k, x.v, x.tree, mask=m, scale=scale, lse=True, **counts)
+        want, want_lse, mass, size = attend64(x.q, x.kc, x.vc, x.k, x.v, x.tree, m2, scale=scale)
+        assert bool(((out.double() - want).abs() <= out_bound(want, mass, size, D)).all())
+        assert bool(((lse.double() - want_lse).abs() <= lse_bound(want_lse, size, D, n)).all())
+        weights = torch.zeros(B, H, x.layer.L, device=DEV)
+        cache_ops.tree_weights(x.layer, x.q, lse, weights, mask=m, scale=scale, **counts)
+        w, size = weights64(x.q, x.kc, lse, m2, scale=scale)
+        bound = w * (score_error(size, D) + (T * Hq // H + 8) * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -22 * 40) + 1e-30
+        assert bool(((weights[..., :n].double() - w).abs() <= bound).all())
+
+
+def test_runs_of_more_than_64_tiles(akv_lib):
+    """75 sequences of 131072 tokens: 65 tiles a warp.  What the mask takes away is not a number."""
+    from alignedkv_b200.decode import DecodeLayer
+    B, n, D = 75, 131072, 64
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    new = lambda *s: torch.randn(*s, device=DEV, generator=gen, dtype=torch.half)  # noqa: E731
+    kc, vc = new(B, n, 1, D), new(B, n, 1, D)
+    mask = torch.zeros(B, 1, 1, n, dtype=torch.half, device=DEV)
+    for b in range(B):
+        mask[b, ..., :b * 1733] = -math.inf
+        mask[b, ..., n - 300 + b:n - 290 + b] = -math.inf
+        hidden = mask[b, 0, 0] == -math.inf
+        kc[b, hidden], vc[b, hidden] = math.inf, math.nan
+    layer = DecodeLayer(B, n, 1, D, DEV)
+    layer.prefill(kc, vc)
+    q, k, v = new(B, 1, 1, D), new(B, 1, 1, D), new(B, 1, 1, D)
+    one = torch.ones(1, 1, dtype=torch.bool, device=DEV)
+    out, lse = layer.tree_attention(q, k, v, one, mask=mask, lse=True)
+    for b in range(B):
+        s = slice(b, b + 1)
+        want, want_lse, mass, size = attend64(q[s], kc[s], vc[s], k[s], v[s], one[None], mask[s, 0, 0])
+        assert bool(((out[s].double() - want).abs() <= out_bound(want, mass, size, D)).all()), b
+        assert bool(((lse[s].double() - want_lse).abs() <= lse_bound(want_lse, size, D, n)).all()), b
