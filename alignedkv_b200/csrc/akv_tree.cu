@@ -10,7 +10,7 @@
 // residual tokens with the drafted ones behind them (at most 127).  The tiles of all units in a row are dealt to the warps in equal
 // contiguous runs, so that every SM gets the same whatever the number of units and their length.  A warp needs no other one: it
 // turns plane bytes into operand fragments in registers (akv_planes.cuh), keeps the scores of its tile and the output of its unit
-// there, and leaves a record (maximum, sum, output) where a run begins or ends inside a unit.
+// there, and leaves a record (maximum, sums, output) where a run begins or ends inside a unit.
 // 8 x 32 x 4096 tokens, 16 rows: 103 us with the merge, 5.2 TB/s of 6.5 (its own share 96 us).
 #include <limits.h>
 
@@ -269,10 +269,10 @@ __device__ __forceinline__ void load_q(uint4* qf, const TreeArgs& p, int b, int 
     }
 }
 
-// Running maximum m, sum l (of this lane's tokens) and output o of rows g and g + 8, taken on by scores s to base 2 of NJ n-tiles;
-// s becomes the probabilities, relative to the maximum and times 2^LIFT.
+// Running maximum m, sums l and lr (of this lane's tokens) and output o of rows g and g + 8, taken on by scores s to base 2 of NJ n-tiles;
+// s becomes the probabilities, relative to the maximum and times 2^LIFT.  (lr is taken on by `packed`.)
 template <int NJ, int N>
-__device__ __forceinline__ void soften(float (&s)[NJ][4], float (&m)[2], float (&l)[2], float (&o)[N][4]) {
+__device__ __forceinline__ void soften(float (&s)[NJ][4], float (&m)[2], float (&l)[2], float (&lr)[2], float (&o)[N][4]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         float top = m[i];
@@ -284,6 +284,7 @@ __device__ __forceinline__ void soften(float (&s)[NJ][4], float (&m)[2], float (
         const float keep = ex2((m[i] - LIFT) - base);          // (nothing yet: 0)
         m[i] = top;
         l[i] *= keep;
+        lr[i] *= keep;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             o[j][2 * i] *= keep;
@@ -299,25 +300,32 @@ __device__ __forceinline__ void soften(float (&s)[NJ][4], float (&m)[2], float (
     }
 }
 
+// Two probabilities as they enter their product, added to lr.
+__device__ __forceinline__ uint32_t packed(float x, float y, float& lr) {
+    const uint32_t w = pack_half2(x, y);
+    lr = plus_high(plus_low(lr, w), w);
+    return w;
+}
+
 // One warp per query row: n records of its tokens, in their order, eight under way at a time; record i lies at at(i).
 template <int D, class At>
 __device__ __forceinline__ void join(const TreeArgs& p, At at, int n, long long to, int lane) {
     constexpr int C = D / 32, STEP = 8;                 // channels of a lane
-    float acc[C], l = 0.f, top = -INFINITY;
+    float acc[C], l = 0.f, lr = 0.f, top = -INFINITY;
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = 0.f;
 #pragma unroll 1
     for (int w = 0; w < n; w += STEP) {
-        float2 ml[STEP];
+        float4 ml[STEP];
         float o[STEP][C];
 #pragma unroll
         for (int k = 0; k < STEP; ++k) {
-            ml[k] = make_float2(-INFINITY, 0.f);
+            ml[k] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int c = 0; c < C; ++c) o[k][c] = 0.f;
             if (w + k >= n) continue;
             const float* x = at(w + k);
-            ml[k] = *reinterpret_cast<const float2*>(x);
+            ml[k] = *reinterpret_cast<const float4*>(x);
             if constexpr (C == 4) {
                 const float4 y = *reinterpret_cast<const float4*>(x + 4 + 4 * lane);
                 o[k][0] = y.x; o[k][1] = y.y; o[k][2] = y.z; o[k][3] = y.w;
@@ -332,17 +340,19 @@ __device__ __forceinline__ void join(const TreeArgs& p, At at, int n, long long 
         const float base = t == -INFINITY ? 0.f : t, keep = ex2(top - base);
         top = t;
         l *= keep;
+        lr *= keep;
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[c] *= keep;
 #pragma unroll
         for (int k = 0; k < STEP; ++k) {
             const float f = ex2(ml[k].x - base);
             l = fmaf(f, ml[k].y, l);
+            lr = fmaf(f, ml[k].z, lr);
 #pragma unroll
             for (int c = 0; c < C; ++c) acc[c] = fmaf(f, o[k][c], acc[c]);
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = lr == 0.f ? 0.f : 1.f / lr;
 #pragma unroll
     for (int c = 0; c < C; c += 2)
         *reinterpret_cast<uint32_t*>(p.out + to * D + C * lane + c) = pack_half2(acc[c] * inv, acc[c + 1] * inv);
@@ -385,7 +395,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
         const int t0 = at - unit * p.tiles, t1 = min(p.tiles, last - unit * p.tiles);
         const __half* mask = p.mask ? p.mask + b * p.mask_stride : nullptr;
         load_q<D>(qf, p, b, h, lane);
-        float o[N][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        float o[N][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, lr[2] = {0.f, 0.f};
         bool odd = false;                               // whether the tail has values that are not finite
 #pragma unroll
         for (int j = 0; j < N; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
@@ -415,13 +425,13 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
 #pragma unroll
                         for (int c = 0; c < 4; ++c) s[j][c] *= p.scale2;
                 }
-                soften(s, m, l, o);
+                soften(s, m, l, lr, o);
                 // (through shared memory, every lane its own: the loop over the V steps stays a loop - unrolled eight times, with
                 // the copies in each, the kernel was bound by the fetch of its instructions, 195 us against 113 then at 8 x 32 x 4096 tokens)
 #pragma unroll
                 for (int st = 0; st < 8; ++st)
-                    pf[st * 32 + lane] = make_uint4(pack_half2(s[2 * st][0], s[2 * st + 1][0]), pack_half2(s[2 * st][2], s[2 * st + 1][2]),
-                                                    pack_half2(s[2 * st][1], s[2 * st + 1][1]), pack_half2(s[2 * st][3], s[2 * st + 1][3]));
+                    pf[st * 32 + lane] = make_uint4(packed(s[2 * st][0], s[2 * st + 1][0], lr[0]), packed(s[2 * st][2], s[2 * st + 1][2], lr[1]),
+                                                    packed(s[2 * st][1], s[2 * st + 1][1], lr[0]), packed(s[2 * st][3], s[2 * st + 1][3], lr[1]));
             }
 #pragma unroll 1
             for (int vs = 0; vs < Ring::VSTEPS; ++vs) {
@@ -465,9 +475,9 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
                             s[j][2 * i + c] = here ? fmaf(s[j][2 * i + c], p.scale2, add * LOG2E) : -INFINITY;
                         }
                     }
-                soften(s, m, l, o);
-                const uint4 a = make_uint4(pack_half2(s[0][0], s[0][1]), pack_half2(s[0][2], s[0][3]), pack_half2(s[1][0], s[1][1]),
-                                           pack_half2(s[1][2], s[1][3]));
+                soften(s, m, l, lr, o);
+                const uint4 a = make_uint4(packed(s[0][0], s[0][1], lr[0]), packed(s[0][2], s[0][3], lr[1]), packed(s[1][0], s[1][1], lr[0]),
+                                           packed(s[1][2], s[1][3], lr[1]));
                 const uint32_t from = ring.take(p);
                 uint32_t x[4][N / 2];
 #pragma unroll
@@ -494,11 +504,13 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
         for (int i = 0; i < 2; ++i) {
             l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
             l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
+            lr[i] += __shfl_xor_sync(0xFFFFFFFFu, lr[i], 1);
+            lr[i] += __shfl_xor_sync(0xFFFFFFFFu, lr[i], 2);
             const int r = g + 8 * i;
             if (r >= R) continue;
             if (t0 == 0 && t1 == p.tiles) {
                 const long long row = row_of(p, b, h, r);
-                const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+                const float inv = lr[i] == 0.f ? 0.f : 1.f / lr[i];
                 uint4* dst = reinterpret_cast<uint4*>(p.out + row * D + 2 * N * t);
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
@@ -513,10 +525,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
                 if (p.lse && t == 0) p.lse[row] = l[i] == 0.f ? -INFINITY : (m[i] - LIFT + log2f(l[i])) * LN2;
             } else {
                 float* rec = record(unit, r);
-                if (t == 0) {
-                    rec[0] = m[i];
-                    rec[1] = l[i];
-                }
+                if (t == 0) *reinterpret_cast<float4*>(rec) = make_float4(m[i], l[i], lr[i], 0.f);
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -532,7 +541,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) tree_kernel(const __grid_consta
             for (int i = 0; i < 2; ++i) {
                 const int r = g + 8 * i;
                 if (r >= R) continue;
-                const float top = i ? m[1] : m[0], sum = i ? l[1] : l[0], base = (top == -INFINITY ? 0.f : top) - LIFT;
+                const float top = i ? m[1] : m[0], sum = i ? lr[1] : lr[0], base = (top == -INFINITY ? 0.f : top) - LIFT;
                 if (t0 == 0 && t1 == p.tiles)
                     add_odd(p, b, h, r, D, base, sum == 0.f ? 0.f : 1.f / sum, p.out + (long long)row_of(p, b, h, r) * D);
                 else

@@ -37,6 +37,8 @@ namespace {
 
 constexpr int SOFT = 8, DECODE = 8, THREADS = 32 * (SOFT + DECODE + 2);
 // A row's reference maximum moves only when a score exceeds it by 2^SLACK: probabilities are at most 2^(WIDE_LIFT + SLACK) in fp16.
+// (The largest is then rounded like the others; with the reference always at the maximum it would be a power of two, and outputs that two
+// tokens share a little nearer - and the outputs so far would be read and scaled again in most tiles of a warp's 32 rows.)
 constexpr float WIDE_LIFT = 7.f, SLACK = 8.f;
 
 template <int D>
@@ -47,9 +49,9 @@ struct Plan {
     // slots' outputs are joined (128 rows x 64 channels at a time) where the queries of the segment that ends were.
     static constexpr int JOIN_BYTES = 128 * 64 * 4, Q_PLACE = Q_BYTES > JOIN_BYTES ? Q_BYTES : JOIN_BYTES;
     static constexpr int RING_AT = 0, Q_AT = RING * TILE_BYTES, Q2_AT = Q_AT + Q_PLACE;
-    static constexpr int XM_AT = Q2_AT + Q_PLACE, XL_AT = XM_AT + 512;
+    static constexpr int XM_AT = Q2_AT + Q_PLACE, XL_AT = XM_AT + 512, XR_AT = XL_AT + 512;
     // barriers, 8 bytes each, then the tensor memory's address, the flag that a wait gave up, odd values of the last segments
-    static constexpr int BAR_AT = XL_AT + 512, RAW = 0, FULL = RING, EMPTY = 2 * RING, S_FULL = 3 * RING, P_FULL = S_FULL + 2,
+    static constexpr int BAR_AT = XR_AT + 512, RAW = 0, FULL = RING, EMPTY = 2 * RING, S_FULL = 3 * RING, P_FULL = S_FULL + 2,
                          O_FULL = P_FULL + 2, Q_FULL = O_FULL + 2, BARS = Q_FULL + 1;
     static constexpr int SEGMENTS = 8, BYTES = BAR_AT + 8 * BARS + 8 + 4 * SEGMENTS + 1024;      // (1024: the base is aligned up)
 };
@@ -457,7 +459,8 @@ __device__ __forceinline__ void product_role(const TreeArgs& p, uint32_t base, u
 
 // ---------------------------------------------------------------- softmax
 // A CTA's part of a unit: four channels of all rows side by side, as the lanes of a warp have and write them (row after row, no two
-// lanes' stores shared a line: 75.5 us against 70.6 at 256 rows x 8192 tokens), the rows' maxima and sums behind them.  As in
+// lanes' stores shared a line: 75.5 us against 70.6 at 256 rows x 8192 tokens), behind them the rows' maxima and their sums of the
+// probabilities, as they are and as they entered their product.  As in
 // akv_tree.cu, slot 0 is of a run's first unit, slot 1 of its last.
 struct Record {
     float* at;
@@ -465,7 +468,7 @@ struct Record {
     __device__ __forceinline__ Record(const TreeArgs& p, int D, int index, int row) :
         at(p.part + (size_t)index * p.rowsu * (D + 4)), rows(p.rowsu), D(D), row(row) {}
     __device__ __forceinline__ float4* quad(int q) const { return reinterpret_cast<float4*>(at) + q * rows + row; }
-    __device__ __forceinline__ float2* stats() const { return reinterpret_cast<float2*>(at + rows * D) + row; }
+    __device__ __forceinline__ float4* stats() const { return reinterpret_cast<float4*>(at + rows * D) + row; }
     __device__ __forceinline__ float& operator[](int c) const { return reinterpret_cast<float*>(quad(c >> 2))[c & 3]; }
 };
 
@@ -478,6 +481,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
     const uint32_t sign = p.scale2 < 0.f ? 0x80008000u : 0u;
     float* xm = reinterpret_cast<float*>(smem + Plan<D>::XM_AT);
     float* xl = reinterpret_cast<float*>(smem + Plan<D>::XL_AT);
+    float* xr = reinterpret_cast<float*>(smem + Plan<D>::XR_AT);
     // Queries of the segment that begins with `tile`, 16-byte piece c of a row's half at c ^ (row & 7): a warp's 32 rows (with one group
     // either slot's warp takes half of their pieces), neighbouring pieces by neighbouring lanes and all on their way at once (a row
     // a lane, by way of registers or not, took 4 us at the start of 256 rows).  Then they are handed over.
@@ -532,7 +536,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
             for (int d = 0; d < p.T; ++d) seen |= (unsigned long long)(row[d] != 0) << d;
         }
         const __half* mask = p.mask ? p.mask + s.b * p.mask_stride : nullptr;
-        float ref = -INFINITY, l = 0.f;
+        float ref = -INFINITY, l = 0.f, lr = 0.f;      // (lr: the sum of the rounded probabilities)
         const int n_items = p.groups * s.c;
         bool any = false;
         for (int n = slot; n < n_items; n += 2, ++done) {
@@ -591,6 +595,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                     const float to = fmaxf(ref, top), keep = ref == -INFINITY ? 0.f : ex2(ref - to);
                     ref = to;
                     l *= keep;
+                    lr *= keep;
                     if (any) {
 #pragma unroll 1
                         for (int c = 0; c < D; c += 32) {
@@ -602,7 +607,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                     }
                 }
                 const float off = (ref == -INFINITY ? 0.f : ref) - WIDE_LIFT;
-                float sums[4] = {0.f, 0.f, 0.f, 0.f};
+                float sums[4] = {0.f, 0.f, 0.f, 0.f}, rounded[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
                 for (int c = 0; c < TILE; c += 32) {
                     tmem_ld(v, s_at + c);
@@ -613,10 +618,13 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                         sums[j & 2] += a;
                         sums[(j & 2) + 1] += b;
                         h[j / 2] = pack_half2(a, b);
+                        rounded[j & 2] = plus_low(rounded[j & 2], h[j / 2]);
+                        rounded[(j & 2) + 1] = plus_high(rounded[(j & 2) + 1], h[j / 2]);
                     }
                     tmem_st16(s_at + c / 2, h);
                 }
                 l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                lr += (rounded[0] + rounded[1]) + (rounded[2] + rounded[3]);
                 tmem_st_wait();
                 any = true;
             }
@@ -638,6 +646,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
             if (slot) {
                 xm[idx] = have ? ref : -INFINITY;
                 xl[idx] = have ? l : 0.f;
+                xr[idx] = have ? lr : 0.f;
             }
             soft_sync();
             if (!slot && n_items > 1) {
@@ -646,12 +655,13 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                 f1 = xm[idx] == -INFINITY ? 0.f : ex2(xm[idx] - to);
                 // (a sum that is not a number stays one: 0 * NaN)
                 l = f0 * l + f1 * xl[idx];
+                lr = f0 * lr + f1 * xr[idx];
                 ref = to;
             }
         }
         const bool whole = s.c == p.tiles, odd_tail = with_tail && odd[seg % Plan<D>::SEGMENTS] == seg + 1;
-        if (*dead) l = __int_as_float(0x7FC00000);
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (*dead) l = lr = __int_as_float(0x7FC00000);
+        const float inv = lr == 0.f ? 0.f : 1.f / lr;
         const int rec_slot = s.unit != (unsigned)first / (unsigned)p.tiles;
         const Record rec(p, D, 2 * blockIdx.x + rec_slot, of_unit);
         float4* join = reinterpret_cast<float4*>(smem + (seg & 1 ? Plan<D>::Q2_AT : Plan<D>::Q_AT));              // [16 channel quads][128 rows]
@@ -710,7 +720,7 @@ __device__ __forceinline__ void softmax_role(const TreeArgs& p, uint8_t* smem, u
                 else add_odd(p, s.b, s.h, r, D, off, 1.f, rec);
             }
             if (!whole) {
-                *rec.stats() = make_float2(ref, l);
+                *rec.stats() = make_float4(ref, l, lr, 0.f);
             } else if (p.lse) {
                 p.lse[row_of(p, s.b, s.h, r)] = l == 0.f ? -INFINITY : (ref - WIDE_LIFT + log2f(l)) * LN2;
             }
@@ -796,15 +806,15 @@ __global__ void __launch_bounds__(2 * D) tree_wide_merge_kernel(const __grid_con
     pdl_wait();
     // (a whole unit has been written by its run)
     if ((unsigned)unit >= (unsigned)p.total / (unsigned)p.tiles || r >= p.T * p.G || w0 == w1) return;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, top = -INFINITY;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, lr = 0.f, top = -INFINITY;
 #pragma unroll 1
     for (int w = w0; w <= w1; w += STEP) {
-        float2 ml[STEP];
+        float4 ml[STEP];
         float4 o[STEP];
 #pragma unroll
         for (int k = 0; k < STEP; ++k) {
             const Record rec(p, D, 2 * (w + k) + (w + k == w0 ? skip : 0), of_unit);
-            ml[k] = make_float2(-INFINITY, 0.f);
+            ml[k] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
             o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (w + k > w1) continue;
             ml[k] = *rec.stats();
@@ -816,19 +826,21 @@ __global__ void __launch_bounds__(2 * D) tree_wide_merge_kernel(const __grid_con
         const float base = t == -INFINITY ? 0.f : t, keep = ex2(top - base);
         top = t;
         l *= keep;
+        lr *= keep;
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[c] *= keep;
 #pragma unroll
         for (int k = 0; k < STEP; ++k) {
             const float f = ex2(ml[k].x - base);
             l = fmaf(f, ml[k].y, l);
+            lr = fmaf(f, ml[k].z, lr);
             acc[0] = fmaf(f, o[k].x, acc[0]);
             acc[1] = fmaf(f, o[k].y, acc[1]);
             acc[2] = fmaf(f, o[k].z, acc[2]);
             acc[3] = fmaf(f, o[k].w, acc[3]);
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = lr == 0.f ? 0.f : 1.f / lr;
     *reinterpret_cast<uint2*>(p.out + to * D + 4 * q) = make_uint2(pack_half2(acc[0] * inv, acc[1] * inv), pack_half2(acc[2] * inv, acc[3] * inv));
     if (p.lse && q == 0) p.lse[to] = l == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) - WIDE_LIFT + log2f(l)) * LN2;
 }

@@ -1,4 +1,4 @@
-"""Attention of drafted tokens where its forms meet their edges: short last units, signs of the scale, long runs."""
+"""Attention of drafted tokens where its forms meet their edges: equal values, short last units, signs of the scale, long runs."""
 import math
 
 import pytest
@@ -8,6 +8,31 @@ from test_gpu_tree import DEV, check, make
 from tree_reference import attend64, lse_bound, out_bound, score_error, weights64
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("B,n,Hq,H,D,T", [
+    (2, 60, 4, 4, 128, 16), (2, 62, 4, 1, 64, 4), (1, 0, 8, 8, 128, 12), (3, 700, 4, 2, 128, 5),      # up to 16 rows
+    (40, 300, 8, 4, 128, 3), (1, 1500, 4, 4, 128, 8),
+    (2, 60, 8, 1, 128, 9), (1, 190, 20, 1, 64, 6), (2, 700, 4, 1, 128, 30), (1, 450, 8, 1, 128, 40), (2, 900, 4, 2, 64, 64)])
+def test_average_of_equal_values_is_that_value(akv_lib, B, n, Hq, H, D, T):
+    """All values 2047/1024, of whose half a step is 2^-12: what probabilities lose on the way to their product has to be missing in
+    their sum as well.  The rest is fp32: under n / 8 + 64 additions of 2^-23, so 2^-14 at most, and the value comes out exactly.
+    Few different keys, so that many tokens share a probability and lose the same."""
+    from alignedkv_b200.decode import DecodeLayer
+    x = make(B, n, Hq, H, D, T, seed=n + T, hot=1.0, spread=0.6)
+    x.k[:] = x.k[:, :1]
+    if n:
+        x.kc[:, 1:] = x.kc[:, 1:2]
+        x.kc[:, n // 2:] = x.kc[:, n // 2:n // 2 + 1]
+    x.vc.fill_(2047 / 1024), x.v.fill_(2047 / 1024)
+    x.layer = DecodeLayer(B, n + 3, H, D, DEV, n_q_heads=Hq)
+    if n:
+        x.layer.prefill(x.kc, x.vc)
+    out, lse = x.layer.tree_attention(x.q, x.k, x.v, x.tree, lse=True)
+    off = int((out != 2047 / 1024).sum())
+    assert off == 0, f"{off} of {out.numel()}"
+    _, want, _, size = attend64(x.q, x.kc, x.vc, x.k, x.v, x.tree)
+    assert bool(((lse.double() - want).abs() <= lse_bound(want, size, D, n)).all()), "the logarithm is that of the exact sum"
 
 
 @pytest.mark.parametrize("B,n,Hq,H,D,T", [(1, 700, 37, 1, 128, 7), (2, 300, 257, 1, 64, 1), (1, 130, 74, 2, 128, 7), (40, 200, 53, 1, 64, 5)])
