@@ -117,3 +117,29 @@ def test_padding_without_weight_goes_first(akv_lib):
     layer.positions = torch.zeros(2, 2, 640, dtype=torch.int32, device=DEV)
     cache_ops.evict(layer, layer.weights, layer.positions, rest_len=0, rest_start=640, keep=128, recent=30)
     assert bool((layer.positions[1, :, :128] >= 500).all())
+
+
+@pytest.mark.parametrize("mode", ["exact", "order_free"])
+def test_decode_steps_after_an_eviction(akv_lib, mode):
+    """The survivors in the order of their places, under the maxima of all tokens that were ever there: bit for bit the steps of a
+    cache that was filled so.  (Those maxima decide which planes are read: above the survivors' own they read fewer of them.)"""
+    from alignedkv_b200.decode import DecodeLayer
+    B, H, D, n = 2, 2, 128, 700
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    new = lambda *shape: torch.randn(*shape, device=DEV, generator=gen).half()  # noqa: E731
+    layer, other = (DecodeLayer(B, 800, H, D, DEV, n_q_heads=4, v_mode=mode) for _ in range(2))
+    k, v = new(B, n, H, D), new(B, n, H, D)
+    k[:, 100, :, ::8] *= 30                           # a token that is evicted and whose exponents stay
+    layer.prefill(k, v)
+    weigh(layer, gen)
+    layer.weights[..., 100] = -1.0
+    layer.evict(256, 64)
+    kept_k, kept_v = (t.to(torch.int16).view(torch.half).transpose(1, 2) for t in dense(layer))
+    rest = n % 64
+    other.prefill(torch.cat([kept_k, k[:, n - rest:]], 1).contiguous(), torch.cat([kept_v, v[:, n - rest:]], 1).contiguous())
+    assert bool((layer.k_exp_max >= other.k_exp_max).all()) and not torch.equal(layer.k_exp_max, other.k_exp_max)
+    other.k_exp_max.copy_(layer.k_exp_max)
+    other.v_exp_max.copy_(layer.v_exp_max)
+    for _ in range(80):
+        q, k1, v1 = new(B, 1, 4, D), new(B, 1, H, D), new(B, 1, H, D)
+        assert torch.equal(layer.decode(q, k1, v1), other.decode(q, k1, v1))

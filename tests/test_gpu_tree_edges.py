@@ -95,3 +95,37 @@ def test_runs_of_more_than_64_tiles(akv_lib):
         want, want_lse, mass, size = attend64(q[s], kc[s], vc[s], k[s], v[s], one[None], mask[s, 0, 0])
         assert bool(((out[s].double() - want).abs() <= out_bound(want, mass, size, D)).all()), b
         assert bool(((lse[s].double() - want_lse).abs() <= lse_bound(want_lse, size, D, n)).all()), b
+
+
+@pytest.mark.parametrize("B,n,Hq,H,D,T", [
+    (1, 127, 4, 4, 128, 64), (1, 63, 1, 1, 64, 64), (2, 191, 2, 2, 128, 16),          # the longest tails: 63 residual and all drafted tokens
+    (300, 40, 2, 2, 128, 2), (700, 0, 1, 1, 64, 3), (300, 5, 20, 1, 64, 1), (310, 63, 17, 1, 128, 1), (170, 0, 6, 1, 64, 3)])     # tails alone
+def test_tails(akv_lib, B, n, Hq, H, D, T):
+    x = make(B, n, Hq, H, D, T, seed=B + n)
+    check(x, *x.layer.tree_attention(x.q, x.k, x.v, x.tree, lse=True))
+
+
+@pytest.mark.parametrize("B,n,Hq,H,D,T", [(200, 10, 20, 1, 64, 1), (200, 150, 20, 1, 128, 1), (40, 70, 10, 1, 128, 3), (200, 10, 2, 1, 64, 2),
+                                          (200, 150, 4, 1, 128, 1)])
+def test_values_that_are_not_finite_stay_in_their_sequence(akv_lib, B, n, Hq, H, D, T):
+    """Every third sequence has an infinite residual (or drafted) value: its rows have it, no other sequence notices."""
+    from alignedkv_b200.decode import DecodeLayer
+    x = make(B, n, Hq, H, D, T, seed=B)
+    x.vc[::3, n - 1, :, 7] = math.inf
+    x.v[1::3, 0, :, 9] = -math.inf
+    x.layer = DecodeLayer(B, n + 3, H, D, DEV, n_q_heads=Hq)
+    x.layer.prefill(x.kc, x.vc)
+    tree = torch.ones(B, T, T, dtype=torch.bool, device=DEV)
+    out, lse = x.layer.tree_attention(x.q, x.k, x.v, tree, lse=True)
+    x.vc[::3, n - 1, :, 7], x.v[1::3, 0, :, 9] = 0.0, 0.0
+    want, want_lse, mass, size = attend64(x.q, x.kc, x.vc, x.k, x.v, tree)
+    # a probability times infinity is infinite (or, where it is under the smallest fp32 number, not a number)
+    odd = torch.zeros_like(out, dtype=torch.bool)
+    odd[::3, ..., 7], odd[1::3, ..., 9] = True, True
+    last = x.kc[:, -1].double().repeat_interleave(Hq // H, 1)
+    seen = torch.einsum("bthd,bhd->bth", x.q.double(), last) / math.sqrt(D) - want_lse
+    assert bool(((out.double() - want).abs() <= out_bound(want, mass, size, D))[~odd].all())
+    assert bool(((lse.double() - want_lse).abs() <= lse_bound(want_lse, size, D, n)).all())
+    there = (seen > -40.0)[::3]
+    assert bool((out[::3, ..., 7][there] == math.inf).all()) and not bool(torch.isfinite(out[::3, ..., 7]).any())
+    assert not bool(torch.isfinite(out[1::3, ..., 9]).any())
