@@ -200,7 +200,9 @@ def evict(cache, weights: torch.Tensor, positions: torch.Tensor, *, rest_len: in
     the `recent` positions, goes first; a caller then has to know that every sequence has `keep` other tokens in the planes.
 
     Afterwards: rest_start = keep; K nibble planes behind it are zero as the K writers expect; the residual tokens' weights follow
-    at keep.., zeros behind them.  Exponent maxima stay (they remain upper bounds)."""
+    at keep.., zeros behind them.  Exponent maxima stay, those of the tokens that go among them: `DecodeLayer.decode` then takes the read
+    decisions of a cache that still had those tokens.  Where one of them had a channel's largest exponent, products of other channels
+    look smaller beside it, and fewer of their planes are read than in a cache that was filled with the survivors alone."""
     c = _Call(cache, rest_len, rest_start)
     _need("weights", weights, (c.B, c.H, c.L), torch.float32, c.index)
     _need("positions", positions, (c.B, c.H, c.L), torch.int32, c.index)

@@ -130,7 +130,7 @@ __device__ __forceinline__ uint32_t cluster_ld(const void* p, uint32_t cta) {
 // counted.  The keep-th largest key by four counts of eight bits (in eight columns: few lanes of a warp meet, although weights crowd into
 // few exponents), added up over the cluster through distributed shared memory; every CTA draws the same
 // conclusion.  Then ties, free places and survivors behind are numbered in order: per warp, per CTA, per cluster.  Bound by latency: a
-// load, four rounds of three barriers, three numberings (256 rows of 4096: 18 us of 144; 8 rows of 131072: 32 of 137).
+// load, four rounds of six barriers (one of them the cluster's), three numberings (256 rows of 4096: 18 us of 144; 8 rows of 131072: 32 of 137).
 constexpr int SEL_MOST = 40960, SEL_CTAS = 8;      // keys a CTA can keep, CTAs of a row
 template <int SEL_NT>
 __global__ void __launch_bounds__(SEL_NT) select_kernel(const EvictArgs a) {
@@ -530,8 +530,8 @@ int akv_evict(const akv_layer* layer, void* weights, void* positions, int rest_l
     a.arranged = arranged;
     a.shift = shift;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // CTAs of a row: so many that all SMs have some and none has less than two thousand places, at most eight (what a cluster may
-    // have everywhere)
+    // CTAs of a row: twice as many, up to eight (what a cluster may have everywhere), while one has more places than it can keep the keys
+    // of, or more than 2048 and some SMs have none
     int ctas = 1;
     while (ctas < SEL_CTAS && ((rest_start + ctas - 1) / ctas > SEL_MOST || (rows * ctas < sm_count() && rest_start / ctas > 2048))) ctas *= 2;
     const int threads = (rest_start + ctas - 1) / ctas > 8192 ? 1024 : 512;

@@ -12,10 +12,10 @@
 // are "MN-major", rows of 64 elements (128 bytes), so that a decoded piece of 16 elements is two 16-byte stores.  Only the
 // tail's keys (fp16 rows of channels) are K-major.
 // Tensor memory: columns 0..255 S (P in the same columns as fp16), 256..511 O.
-// What bounds it: up to 128 rows the planes' way into the operands (16 x 8 x 8190 tokens, 48 rows: 125 us, of which the copies alone
-// are 90 and HBM's floor 83: decode, products and softmax share the SM's shared memory with them); 256 rows (4 x 8 x 8192: 66 us)
-// the chain of a slot - 1.3 us of softmax, bound by exponentials, and 1.1 us from P to the next S - and 25 us of a call's start, of
-// the records and of the merge.
+// What bounds it: up to 128 rows the planes' way into the operands (16 x 8 x 8190 tokens, 48 rows: 130 us; the copies alone took 90
+// when the whole took 125, HBM's floor is 83: decode, products and softmax share the SM's shared memory with them); 256 rows (4 x 8 x
+// 8192: 69 us) the chain of a slot - when they took 66: 1.3 us of softmax, bound by exponentials, and 1.1 us from P to the next S - and
+// 25 us of a call's start, of the records and of the merge.
 #include <limits.h>
 
 #include "akv_tree.cuh"
@@ -849,7 +849,7 @@ __global__ void __launch_bounds__(2 * D) tree_wide_merge_kernel(const __grid_con
 // weights[t] += sum over the rows of exp(s_t - lse): keys alone, and the product the other way round: S^T = K Q^T, a tile's 128 tokens
 // by up to 128 rows, so that a thread has a token and adds its rows up by itself, whatever their number: no warp has to wait for
 // another's, and the order is always the same.  Copy and decode as above, the ring as deep as the queries leave room for; two score
-// slots, the tiles in turn.  One row is bound by HBM (8 x 32 x 4096 tokens: 50 us, 5.4 TB/s of 6.5); 128 rows (4 x 8 x 8190: 31 us)
+// slots, the tiles in turn.  One row is bound by HBM (8 x 32 x 4096 tokens: 51 us, 5.4 TB/s of 6.5); 128 rows (4 x 8 x 8190: 30 us)
 // by the threads' chain of loads and exponentials (5 us less without), the rest is the start and the end of a run of 14 tiles.
 template <int D>
 struct KeysPlan {

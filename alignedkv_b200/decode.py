@@ -237,7 +237,8 @@ class DecodeLayer:
 
     def tree_weights(self, q: torch.Tensor, lse: torch.Tensor, *, mask: torch.Tensor | None = None) -> torch.Tensor:
         """Add the attention weight that these queries give each cached token to `weights` [B,H,L], fp32, and return it
-        (`cache_ops.tree_weights`; q and lse as given to and returned by `tree_attention`)."""
+        (`cache_ops.tree_weights`; q and lse as given to and returned by `tree_attention`).  A row whose lse is -inf does not vote: with
+        drafted tokens that may be rejected a program votes once it knows, and takes their rows out so."""
         if mask is not None:
             self._no_mask_after_eviction()
         if q.dim() == 4 and q.shape[2] != self.Hq:
@@ -296,7 +297,8 @@ class DecodeLayer:
         """Roll the cache back to a snapshot (`akv_rollback`): the exponent maxima are put back and the K nibble planes
         of blocks written since are cleared, because the K writer accumulates nibbles
         (extension/csrc/K_cache.cu:52-56).  Tokens that were still in the residual buffer at the snapshot stay
-        there: later appends only wrote rows behind them.  Weights of the tokens that go are set to zero."""
+        there: later appends only wrote rows behind them.  Weights of the tokens that go are set to zero;
+        votes for those that stay are kept, whoever gave them."""
         if snap.get("evictions", 0) != self.evictions:
             raise RuntimeError("restore: tokens have been evicted since the snapshot")
         first_blk = snap["rest_start"] // column_block

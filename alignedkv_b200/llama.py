@@ -261,8 +261,9 @@ class LlamaDecoder:
     def verify(self, ids: torch.Tensor, parents: torch.Tensor, weights: bool = False) -> torch.Tensor:
         """Logits [B,T,V] of T drafted tokens (ids [B,T], T at most 64) that are not in the caches yet.  parents: int64 [T], the
         tree they form in every sequence: the node that each one follows, a lower index, or -1 for the last cached token.
-        `accept` appends some of them, as long as neither `step` nor a roll-back comes between.  weights=True also adds the queries'
-        attention weights to each layer's (`evict`)."""
+        `accept` appends some of them, as long as neither `step` nor a roll-back comes between.  weights=True also adds the
+        attention weights of all T queries to each layer's (`evict`), at once and for good: those of branches that are not accepted
+        and of drafts that are dropped, too."""
         assert self.attention == "alignedkv", "only the AlignedKV path drafts tokens"
         cfg = self.cfg
         H, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim

@@ -421,7 +421,8 @@ int akv_shard_step(void* k_first_8, void* k_mid_4, void* k_last_4, void* v_first
  * Places >= arranged hold tokens in order, place p that at position p + shift.  K nibble planes of the freed blocks are
  * cleared, the residual tokens' weights move to keep.., zeros behind.  scratch: akv_evict_scratch_bytes(...) bytes.  There is no
  * mask: padding is a token like the others (its weight is 0; -inf lets it go first), and what survives of it lies where no mask row
- * reaches it: a cache with masked tokens is evicted only where every sequence has `keep` others in the planes.
+ * reaches it: a cache with masked tokens is evicted only where every sequence has `keep` others in the planes.  Exponent maxima
+ * stay, those of the evicted tokens among them: decode steps take their read decisions under them.
  */
 long long akv_tree_scratch_bytes(int bsz, int n_kv_heads, int group, int head_dim, int n_tokens, int drafted);
 int akv_tree_attention(const akv_layer* layer, const void* q, const void* k_new, const void* v_new, const void* tree,
