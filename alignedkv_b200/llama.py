@@ -310,7 +310,8 @@ class LlamaDecoder:
         for cache in self.caches:
             if cache.cache_len + n > cache.L:
                 raise RuntimeError(f"cache is full ({cache.L} tokens): no room for {n} behind {cache.cache_len}")
-        path = path.to(device=self.device, dtype=torch.int32).contiguous()
+        # (clamped into the tree, as the commit does, before a wide index loses its upper bits)
+        path = path.clamp(0, drafts[0][0].shape[1] - 1).to(device=self.device, dtype=torch.int32).contiguous()
         for cache, (k, v) in zip(self.caches, drafts):
             cache.tree_commit(k, v, path)
         self._drafts = None

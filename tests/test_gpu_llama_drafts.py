@@ -89,3 +89,13 @@ def test_an_eviction_between_is_fine(akv_lib):
     assert dec.pos == other.pos == S + 66
     for x, y in zip(dec.caches, other.caches):
         assert x.cache_len == 64 + 6 + 2 and torch.equal(x.restk[:, 6:8], y.restk[:, 6:8]) and torch.equal(x.restv[:, :8], y.restv[:, :8])
+
+
+def test_wide_indices_are_clamped_like_others(akv_lib):
+    dec, ids = decoder(20)
+    dec.verify(ids[:, S:S + 4], CHAIN)
+    keys = [k for k, _ in dec._drafts[1]]
+    dec.accept(torch.tensor([[-2 ** 40 - 3, 2 ** 32 + 1, 7]] * B))
+    at = S % 64
+    for c, k in zip(dec.caches, keys):
+        assert torch.equal(c.restk[:, at:at + 3], k[:, [0, 3, 3]])
