@@ -670,6 +670,7 @@ int check_layer(const char* fn, const akv_layer* a, const void* q, int T, int re
     AKV_REQUIRE(aligned16(a->k_first_8) && aligned16(a->k_mid_4) && aligned16(a->k_last_4) && aligned16(a->v_first_8) &&
                 aligned16(a->v_mid_4) && aligned16(a->v_last_4) && aligned16(a->restk) && aligned16(a->restv) && aligned16(q),
                 AKV_ERR_ALIGN, "%s: pointers must be 16-byte aligned", fn);
+    AKV_REQUIRE((reinterpret_cast<uintptr_t>(mask) & 1u) == 0, AKV_ERR_ALIGN, "%s: the mask must be 2-byte aligned", fn);
     return AKV_OK;
 }
 
@@ -724,6 +725,7 @@ int akv_tree_attention(const akv_layer* layer, const void* q, const void* k_new,
     AKV_REQUIRE(tree_stride >= 0, AKV_ERR_SHAPE, "tree_attention: negative tree stride");
     AKV_REQUIRE(aligned16(k_new) && aligned16(v_new) && aligned16(out) && aligned16(layer->scratch), AKV_ERR_ALIGN,
                 "tree_attention: pointers must be 16-byte aligned");
+    AKV_REQUIRE((reinterpret_cast<uintptr_t>(lse) & 3u) == 0, AKV_ERR_ALIGN, "tree_attention: lse must be 4-byte aligned");
     const int D = layer->head_dim;
     AKV_REQUIRE(layer->scratch_bytes >= akv_tree_scratch_bytes(layer->bsz, layer->n_kv_heads, layer->group, D, rest_start, drafted),
                 AKV_ERR_SHAPE, "tree_attention: scratch of %lld bytes is too small", layer->scratch_bytes);
@@ -764,6 +766,8 @@ int akv_tree_weights(const akv_layer* layer, const void* q, const void* lse, con
     int rc = check_layer("tree_weights", layer, q, drafted, rest_len, rest_start, mask, mask_stride);
     if (rc != AKV_OK) return rc;
     AKV_REQUIRE(lse && weights, AKV_ERR_NULL, "tree_weights: null pointer");
+    AKV_REQUIRE(((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(weights)) & 3u) == 0, AKV_ERR_ALIGN,
+                "tree_weights: lse and weights must be 4-byte aligned");
     TreeArgs p = make_args(layer, q, drafted, rest_len, rest_start, mask, mask_stride, scale);
     p.lse = static_cast<float*>(const_cast<void*>(lse));
     p.tiles = (p.nb + 1) / 2 + (rest_len > 0);
