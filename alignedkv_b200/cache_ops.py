@@ -130,7 +130,7 @@ def tree_attention(cache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tre
     group, lib = Hq // c.H, _lib.load()
     sums = q.new_empty((c.B, T, Hq), dtype=torch.float32) if lse else None
     with c.here():
-        ws = torch.empty(lib.akv_tree_scratch_bytes(c.B, c.H, group, c.D, rest_start, T), dtype=torch.uint8, device=c.device)
+        ws = torch.empty(max(0, lib.akv_tree_scratch_bytes(c.B, c.H, group, c.D, rest_start, T)), dtype=torch.uint8, device=c.device)
         rc = lib.akv_tree_attention(
             c.layer(group, ws), q.data_ptr(), k_ptr, v_ptr, tree.data_ptr(), T * T if tree.dim() == 3 else 0,
             mask_ptr, mask_stride, out.data_ptr(), sums.data_ptr() if lse else None, T, rest_len, rest_start,
@@ -213,7 +213,7 @@ def evict(cache, weights: torch.Tensor, positions: torch.Tensor, *, rest_len: in
         raise RuntimeError(f"recent {recent} [0..keep], arranged {arranged} [0..{rest_start}], shift {shift} [0..{most}]")
     lib = _lib.load()
     with c.here():
-        ws = torch.empty(lib.akv_evict_scratch_bytes(c.B, c.H, rest_start, keep), dtype=torch.uint8, device=c.device)
+        ws = torch.empty(max(0, lib.akv_evict_scratch_bytes(c.B, c.H, rest_start, keep)), dtype=torch.uint8, device=c.device)
         rc = lib.akv_evict(c.layer(1, ws), weights.data_ptr(), positions.data_ptr(), rest_len, rest_start, keep, recent, arranged,
                            shift, _lib.raw_stream(c.index))
     _lib.check("evict", rc)

@@ -12,6 +12,7 @@ namespace akv {
 namespace {
 
 constexpr int BLK = 64;
+constexpr int MOST_ROWS = 65535;                       // (batch, KV head) rows: along the grid's y
 
 // ------------------------------------------------------------------ accepted path
 // CTA = (batch, KV head) and one of K, V.  Rows in front of the accepted tokens: the residual buffer.  The two together are at most
@@ -444,7 +445,7 @@ int check_planes(const char* fn, const akv_layer* a) {
                 a->max_seq_len <= INT_MAX - 128, AKV_ERR_SHAPE,
                 "%s: unsupported extent (bsz %d, KV heads %d, head_dim %d [64 or 128], max_seq_len %d)", fn, a->bsz, a->n_kv_heads,
                 a->head_dim, a->max_seq_len);
-    AKV_REQUIRE((long long)a->bsz * a->n_kv_heads <= 65535, AKV_ERR_OVERFLOW, "%s: more than 65535 (batch, KV head) rows", fn);
+    AKV_REQUIRE((long long)a->bsz * a->n_kv_heads <= MOST_ROWS, AKV_ERR_OVERFLOW, "%s: more than %d (batch, KV head) rows", fn, MOST_ROWS);
     AKV_REQUIRE(aligned16(a->k_first_8) && aligned16(a->k_mid_4) && aligned16(a->k_last_4) && aligned16(a->v_first_8) &&
                 aligned16(a->v_mid_4) && aligned16(a->v_last_4), AKV_ERR_ALIGN, "%s: pointers must be 16-byte aligned", fn);
     return AKV_OK;
@@ -484,7 +485,7 @@ int akv_tree_commit(const akv_layer* layer, const void* k_new, const void* v_new
 }
 
 long long akv_evict_scratch_bytes(int bsz, int n_kv_heads, int n_tokens, int keep) {
-    if (bsz <= 0 || n_kv_heads <= 0 || keep <= 0 || keep > n_tokens) return -1;
+    if (bsz <= 0 || n_kv_heads <= 0 || (long long)bsz * n_kv_heads > MOST_ROWS || keep <= 0 || keep > n_tokens) return -1;
     const long long most = keep < n_tokens - keep ? keep : n_tokens - keep;
     return (long long)bsz * n_kv_heads * (2 * most + keep / BLK + 1) * 4;
 }

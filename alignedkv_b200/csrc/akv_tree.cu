@@ -653,6 +653,12 @@ int launch_warps(Kernel kernel, const Deal& d, cudaStream_t st, const TreeArgs& 
     return AKV_OK;
 }
 
+// Query rows per drafted token: so few that all indices of rows fit 32 bits.  (The first two factors alone fit 64 bits, not all three.)
+bool few_rows(int bsz, int H, int G) {
+    constexpr long long most = (1ll << 30) / BLK;
+    return (long long)bsz * H < most && (long long)bsz * H * G < most;
+}
+
 int check_layer(const char* fn, const akv_layer* a, const void* q, int T, int rest_len, int rest_start, const void* mask,
                 long long mask_stride) {
     AKV_REQUIRE(a && q && a->k_first_8 && a->k_mid_4 && a->k_last_4 && a->v_first_8 && a->v_mid_4 && a->v_last_4 && a->restk &&
@@ -665,7 +671,7 @@ int check_layer(const char* fn, const akv_layer* a, const void* q, int T, int re
     AKV_REQUIRE(rest_len >= 0 && rest_len < BLK && rest_start >= 0 && rest_start % BLK == 0 &&
                 (long long)rest_start + rest_len <= a->max_seq_len, AKV_ERR_SHAPE,
                 "%s: rest_len %d [0..63] behind %d tokens [multiple of 64] of %d", fn, rest_len, rest_start, a->max_seq_len);
-    AKV_REQUIRE((long long)a->bsz * a->n_kv_heads * a->group < (1ll << 30) / BLK, AKV_ERR_OVERFLOW, "%s: too many rows", fn);
+    AKV_REQUIRE(few_rows(a->bsz, a->n_kv_heads, a->group), AKV_ERR_OVERFLOW, "%s: too many rows", fn);
     AKV_REQUIRE(!mask || mask_stride >= 0, AKV_ERR_SHAPE, "%s: negative mask stride", fn);
     AKV_REQUIRE(aligned16(a->k_first_8) && aligned16(a->k_mid_4) && aligned16(a->k_last_4) && aligned16(a->v_first_8) &&
                 aligned16(a->v_mid_4) && aligned16(a->v_last_4) && aligned16(a->restk) && aligned16(a->restv) && aligned16(q),
@@ -709,7 +715,7 @@ extern "C" {
 
 long long akv_tree_scratch_bytes(int bsz, int n_kv_heads, int group, int head_dim, int n_tokens, int drafted) {
     if (bsz <= 0 || n_kv_heads <= 0 || group <= 0 || (head_dim != 64 && head_dim != 128) || n_tokens < 0 || drafted < 1 ||
-        drafted > BLK)
+        drafted > BLK || !few_rows(bsz, n_kv_heads, group))
         return -1;
     const Shape s = shape_of(bsz, n_kv_heads, group, drafted, n_tokens);
     return 2ll * s.d.runs * s.rowsu * (head_dim + 4) * 4;

@@ -1,12 +1,14 @@
-"""Refusals of the entries around drafted tokens and eviction that keep a kernel from addresses it cannot read: alignments."""
+"""Refusals of the entries around drafted tokens and eviction that keep a kernel from addresses it cannot read: alignments, extents whose
+products do not fit."""
 import ctypes
 
 import pytest
 
 torch = pytest.importorskip("torch")
 
-ALIGN = -3
+SHAPE, ALIGN, OVERFLOW = -2, -3, -4
 P = 256
+MOST = 2 ** 31 - 1
 
 
 def layer(**kw):
@@ -30,3 +32,17 @@ def weights(lib, a, mask=None, lse=P, w=P):
                                     (weights, dict(lse=P + 2)), (weights, dict(w=P + 1)), (weights, dict(w=P + 2))])
 def test_alignment(akv_lib, run, kw):
     assert run(akv_lib, layer(), **kw) == ALIGN and b"align" in akv_lib.akv_last_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="refusals are tried where nothing can be launched")
+@pytest.mark.parametrize("kw", [dict(bsz=MOST, n_kv_heads=MOST, group=4), dict(bsz=1 << 30, n_kv_heads=1 << 30, group=16),
+                                dict(bsz=MOST, n_kv_heads=MOST, group=MOST), dict(bsz=1, n_kv_heads=1, group=1 << 30)])
+def test_rows_beyond_64_bits(akv_lib, kw):
+    assert attention(akv_lib, layer(**kw)) == OVERFLOW and weights(akv_lib, layer(**kw)) == OVERFLOW
+    assert akv_lib.akv_tree_scratch_bytes(kw["bsz"], kw["n_kv_heads"], kw["group"], 128, 128, 5) == -1
+
+
+def test_workspaces_beyond_64_bits(akv_lib):
+    assert akv_lib.akv_evict_scratch_bytes(MOST, MOST, 1 << 20, 1 << 19) == -1
+    assert akv_lib.akv_evict_scratch_bytes(65535, 1, 1 << 20, 1 << 19) == 65535 * (2 * (1 << 19) + (1 << 13) + 1) * 4
+    assert akv_lib.akv_tree_scratch_bytes(1, 1, 1, 128, MOST, 5) > 0

@@ -143,3 +143,12 @@ def test_decode_steps_after_an_eviction(akv_lib, mode):
     for _ in range(80):
         q, k1, v1 = new(B, 1, 4, D), new(B, 1, H, D), new(B, 1, H, D)
         assert torch.equal(layer.decode(q, k1, v1), other.decode(q, k1, v1))
+
+
+def test_too_many_rows_are_refused_by_name(akv_lib):
+    from alignedkv_b200 import cache_ops
+    from alignedkv_b200.decode import DecodeLayer
+    layer = DecodeLayer(65536, 64, 1, 64, DEV)
+    weights, positions = (torch.zeros(65536, 1, 64, dtype=t, device=DEV) for t in (torch.float32, torch.int32))
+    with pytest.raises(RuntimeError, match="65535 .* rows"):
+        cache_ops.evict(layer, weights, positions, rest_len=0, rest_start=64, keep=64)
