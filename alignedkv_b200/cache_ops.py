@@ -195,7 +195,7 @@ def evict(cache, weights: torch.Tensor, positions: torch.Tensor, *, rest_len: in
     places below `keep`.  Places from `arranged` on hold tokens in order, place p that at position p + shift: (0, 0) before the
     first eviction, after one (keep, shift + rest_start - keep).
 
-    There is no mask: padding is a token like the others - its weight is 0, and the lowest places win among equals - and what
+    There is no mask: padding is a token like the others - masked queries give it no weight, and the lowest places win among equals - and what
     survives of it is no longer where a mask row could take it away.  Padding whose weight is set to -inf, and which is not among
     the `recent` positions, goes first; a caller then has to know that every sequence has `keep` other tokens in the planes.
 

@@ -399,7 +399,8 @@ int akv_shard_step(void* k_first_8, void* k_mid_4, void* k_last_4, void* v_first
  * (no counterpart in the reference, which decodes one token at a time and never drops one).  `layer`: planes, residual buffers,
  * extents; exponent maxima and scratch where an entry says so.  rest_len (0..63) tokens in the residual buffers behind rest_start
  * (a multiple of 64) in the planes.  head_dim 64 or 128; `drafted` 1..64 tokens T per sequence.  fp16 tensors contiguous and
- * 16-byte aligned: q, out [B,T,Hq,D], k_new, v_new [B,T,Hkv,D]; query head i reads KV head i / group.
+ * 16-byte aligned: q, out [B,T,Hq,D], k_new, v_new [B,T,Hkv,D]; query head i reads KV head i / group.  Masks are aligned to 2 bytes, lse,
+ * weights, path and positions to 4.
  *
  * akv_tree_attention: out[r] = softmax over the tokens that row r sees of (scale q_r . k + mask), times v; fp32 scores, softmax and
  * sums over the exact cached values (every plane is read), rounded once.  tree: bytes [T,T] per sequence, tree_stride bytes apart
@@ -420,7 +421,7 @@ int akv_shard_step(void* k_first_8, void* k_mid_4, void* k_last_4, void* v_first
  * >= keep moves to the i-th free place < keep with its weight; positions int32 [B,Hkv,max_seq_len] are written for places < keep.
  * Places >= arranged hold tokens in order, place p that at position p + shift.  K nibble planes of the freed blocks are
  * cleared, the residual tokens' weights move to keep.., zeros behind.  scratch: akv_evict_scratch_bytes(...) bytes.  There is no
- * mask: padding is a token like the others (its weight is 0; -inf lets it go first), and what survives of it lies where no mask row
+ * mask: padding is a token like the others (a weight of -inf lets it go first), and what survives of it lies where no mask row
  * reaches it: a cache with masked tokens is evicted only where every sequence has `keep` others in the planes.  Exponent maxima
  * stay, those of the evicted tokens among them: decode steps take their read decisions under them.
  */
