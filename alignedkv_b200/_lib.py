@@ -21,6 +21,12 @@ class Layer(ctypes.Structure):
         (n, ctypes.c_int) for n in ("bsz", "n_kv_heads", "group", "head_dim", "max_seq_len")]
 
 
+class Pool(ctypes.Structure):
+    """`akv_pool`: a pool of pages."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_codes", "v_codes", "k_exps", "v_exps", "k_scales", "v_scales")] + [
+        (n, ctypes.c_int) for n in ("format", "n_pages", "page_size", "n_kv_heads", "head_dim")]
+
+
 def _raw_stream(device_index: int) -> int:
     return torch.cuda.current_stream(device_index).cuda_stream
 
@@ -79,6 +85,12 @@ SIGNATURES = {
     "akv_tree_commit": (_I, [_P] * 4 + [_I] * 4 + [_P]),
     "akv_evict_scratch_bytes": (ctypes.c_longlong, [_I] * 4),
     "akv_evict": (_I, [_P] * 3 + [_I] * 6 + [_P]),
+    "akv_paged_append": (_I, [_P] * 7 + [_I] * 3 + [_P]),
+    "akv_paged_read": (_I, [_P] * 5 + [_I] * 3 + [_P]),
+    "akv_paged_scratch_bytes": (ctypes.c_longlong, [_P] + [_I] * 4),
+    "akv_paged_attention": (_I, [_P] * 7 + [ctypes.c_longlong] + [_I] * 4 + [_F, _P]),
+    "akv_accept_drafts": (_I, [_P] + [ctypes.c_longlong] * 2 + [_P] + [ctypes.c_longlong] * 2 + [_P] * 3 + [ctypes.c_longlong] + [_P] * 3 +
+                          [_I] * 4 + [_P]),
     "akv_timing_reset": (_I, []),
     "akv_timing_read": (_I, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
 }

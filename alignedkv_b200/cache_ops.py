@@ -4,6 +4,7 @@
   tree_weights     adds the attention weight that such queries give each cached token to fp32 sums
   tree_commit      the accepted path of the tree enters the cache
   evict            every (sequence, KV head) keeps its heaviest cached tokens
+  accept_drafts    which drafted tokens are accepted, and the token behind them, from probabilities and random numbers (any cache)
 
 The reference has no counterpart: it decodes one token at a time and never drops one (model/KVCache_AlignedKV.py:81-135).
 
@@ -23,7 +24,7 @@ import torch
 from . import _lib
 from .extension._planes import cdiv, column_block
 
-__all__ = ["tree_attention", "tree_weights", "tree_commit", "evict"]
+__all__ = ["tree_attention", "tree_weights", "tree_commit", "evict", "accept_drafts"]
 
 _nothing = contextlib.nullcontext()
 MOST_DRAFTED = 64
@@ -217,3 +218,56 @@ def evict(cache, weights: torch.Tensor, positions: torch.Tensor, *, rest_len: in
         rc = lib.akv_evict(c.layer(1, ws), weights.data_ptr(), positions.data_ptr(), rest_len, rest_start, keep, recent, arranged,
                            shift, _lib.raw_stream(c.index))
     _lib.check("evict", rc)
+
+
+_PROBABILITIES = {torch.float32: 0, torch.half: 1, torch.bfloat16: 2}
+
+
+def accept_drafts(target: torch.Tensor, draft: torch.Tensor | None, ids: torch.Tensor, coins: torch.Tensor,
+                  parents: torch.Tensor | None = None) -> tuple:
+    """(path, count, token): the drafted tokens that are accepted and the token behind them, such that what comes out has the
+    distribution that sampling from `target` alone would give.
+
+    ids int64 [B,T], T 1 to 64.  Node 0 is taken already (the token that was sampled last); node i >= 1 hangs under node parents[i] < i
+    (int32 [T] or [B,T], on the device; by default a chain) and its token was drawn from draft[b, parents[i]].  An entry of parents that is no earlier node
+    is never reached.  target, draft [B,T,V]: probabilities of what follows each node, fp32, fp16 or bf16, one type, with a unit stride along the
+    vocabulary; rows of draft whose node has no children are not read.  draft=None: the drafts are guesses that no probability was given
+    to (looked up in the prompt, the most likely one of a small model).  coins fp32 [B,T] in [0,1): coins[b, i] decides over node i, coins[b, 0]
+    chooses the token behind the accepted ones.
+
+    The children of the accepted node are asked in order.  With p, q its rows of target and draft, r = max(p - c q, 0), c = 0 and Z = 1
+    at first: x is accepted if coin * Z * q(x) < r(x); if not, c += Z and Z = sum(r).  Without draft: accepted if coin * Z < p(x); if not, Z -= p(x)
+    and p(x) = 0.  (Children under one node are independent draws; guesses may repeat, a second one is not accepted.)  Where no child is left, token
+    is the smallest j with cumsum(r)[j] > coin * sum(r); if r is zero throughout, of p.  Products and sums are formed in 64 bits.  Entries that are
+    not positive and finite count as 0, a token outside the vocabulary has no probability.
+
+    path int32 [B,T]: the accepted nodes, 0 first, -1 behind them; count int32 [B], at least 1; token int64 [B] (-1 where a row has no
+    probability at all).  Sequences accept different numbers of tokens: `tree_commit` takes path[:, :n] for n up to the smallest count, whose
+    nodes are then `LlamaDecoder.accept`'s too."""
+    if not isinstance(target, torch.Tensor) or not target.is_cuda or target.dim() != 3 or target.dtype not in _PROBABILITIES or \
+            target.numel() == 0 or (target.stride(2) != 1 and target.shape[2] > 1):
+        raise RuntimeError("target: expected a CUDA tensor of shape [B, T, V], fp32, fp16 or bf16, with a unit stride along the vocabulary")
+    B, T, V = target.shape
+    index = target.get_device()
+    if T > MOST_DRAFTED:
+        raise RuntimeError(f"target: {T} nodes, expected 1 to {MOST_DRAFTED}")
+    if draft is not None and (not isinstance(draft, torch.Tensor) or draft.shape != target.shape or draft.dtype is not target.dtype or
+                              draft.get_device() != index or (draft.stride(2) != 1 and V > 1)):
+        raise RuntimeError(f"draft: expected a {target.dtype} tensor of shape {tuple(target.shape)} on cuda:{index} with a unit stride along "
+                           "the vocabulary")
+    ids_ptr, coins_ptr = _need("ids", ids, (B, T), torch.int64, index), _need("coins", coins, (B, T), torch.float32, index)
+    parents_ptr, step = None, 0
+    if parents is not None:
+        each = isinstance(parents, torch.Tensor) and parents.dim() == 2
+        parents_ptr, step = _need("parents", parents, (B, T) if each else (T,), torch.int32, index), T if each else 0
+    path = torch.empty((B, T), dtype=torch.int32, device=target.device)
+    count = torch.empty(B, dtype=torch.int32, device=target.device)
+    token = torch.empty(B, dtype=torch.int64, device=target.device)
+    d = target if draft is None else draft
+    with _nothing if torch.cuda.current_device() == index else torch.cuda.device(index):
+        rc = _lib.load().akv_accept_drafts(
+            target.data_ptr(), target.stride(0), target.stride(1), None if draft is None else draft.data_ptr(), d.stride(0), d.stride(1),
+            ids_ptr, coins_ptr, parents_ptr, step, path.data_ptr(), count.data_ptr(), token.data_ptr(), B, T, V,
+            _PROBABILITIES[target.dtype], _lib.raw_stream(index))
+    _lib.check("accept_drafts", rc)
+    return path, count, token

@@ -1,0 +1,250 @@
+// The cache in pages: tokens are quantised as they enter it, and read back as fp16.
+#include "akv_paged.cuh"
+
+namespace akv {
+namespace {
+
+constexpr int THREADS = 256, VALUES = 8;       // a thread has 8 channels: 16 bytes of fp16
+
+struct AppendArgs {
+    Pool pool;
+    const __half* x[2];                        // k, v
+    long long batch[2], token[2], head[2];     // their strides
+    const int* counts;
+    int T;
+};
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// The least e with a <= top 2^add 2^e for the bits of a >= 0 (top's fraction as bits); a = 0 counts as fp16's smallest.
+__device__ __forceinline__ int least_exponent(uint32_t bits, uint32_t top_fraction, int add) {
+    if (bits == 0) return -24 - add;
+    return (int)(bits >> 23) - 127 - add + ((bits & 0x7FFFFFu) > top_fraction);
+}
+// x / s in the nearest fp32, s > 0 with reciprocal r to a few steps: x r is off by steps, what it leaves out is exact in one fused operation,
+// and adding that part puts the quotient within 2^-40 before its one rounding.  Codes change at middles m of few bits; fp16 x is never
+// nearer to m s than 2^-12 of it unless equal, and then the quotient is m itself.
+__device__ __forceinline__ float quotient(float x, float s, float r) {
+    const float y = x * r;
+    return fmaf(fmaf(-y, s, x), r, y);
+}
+
+// Codes of a lane's 8 channels, by the LANES = D / 8 lanes that have a row; row < 0: takes part in the exchange, stores nothing.
+template <int F, int D>
+__device__ __forceinline__ void store_row(uint8_t* codes, int8_t* exps, uint8_t* scales, long long row, int lane, uint4 raw) {
+    constexpr int LANES = D / VALUES;
+    if constexpr (F == AKV_PAGE_FP16) {
+        if (row >= 0) *reinterpret_cast<uint4*>(codes + row * (2 * D) + lane * 16) = raw;
+    } else {
+        float x[VALUES];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = halves_floats(u4w(raw, i));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+        uint32_t top = 0;                      // (as bits: NaN is above infinity, infinity above the rest)
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) top = max(top, abs_bits(x[i]));
+        const uint32_t pair = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));     // of 16 channels
+        top = pair;
+#pragma unroll
+        for (int o = 2; o < LANES; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const bool finite = top < 0x7F800000u;
+        const int e = F == AKV_PAGE_E4M3 ? least_exponent(top, 0x600000u, 8) : least_exponent(top, 0x280000u, 11);
+        const float unit = finite ? power2(-e) : 0.f;
+        if (row >= 0 && lane == 0) exps[row] = (int8_t)(finite ? e : EXP_NAN);
+        if constexpr (F == AKV_PAGE_E4M3) {
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < VALUES; i += 2) {
+                uint16_t c;
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(c) : "f"(x[i + 1] * unit), "f"(x[i] * unit));
+                w[i >> 2] |= (uint32_t)c << (8 * (i & 2));
+            }
+            if (row >= 0) *reinterpret_cast<uint2*>(codes + row * D + lane * VALUES) = finite ? make_uint2(w[0], w[1]) : make_uint2(0, 0);
+        } else {
+            uint16_t sc;
+            const float most = finite ? __fdiv_rn(__uint_as_float(pair) * unit, 6.f) : 0.f;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(sc) : "f"(0.f), "f"(most));
+            if (row >= 0 && (lane & 1) == 0) scales[row * (D / 16) + (lane >> 1)] = (uint8_t)sc;
+            const float s = e4m3_float(sc & 0xFFu), r = s > 0.f ? __frcp_rn(s) : 0.f;
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 0; i < VALUES; i += 2) {
+                uint32_t c;
+                asm("{\n.reg .b8 b;\ncvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\ncvt.u32.u8 %0, b;\n}\n"
+                    : "=r"(c) : "f"(quotient(x[i + 1] * unit, s, r)), "f"(quotient(x[i] * unit, s, r)));
+                w |= c << (4 * i);
+            }
+            if (row >= 0) *reinterpret_cast<uint32_t*>(codes + row * (D / 2) + lane * 4) = finite ? w : 0u;
+        }
+    }
+}
+
+// One row of one tensor per LANES threads; a block has consecutive tokens of one KV head, whose rows lie side by side in a page.
+template <int F, int D>
+__global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
+    constexpr int LANES = D / VALUES, ROWS = THREADS / LANES;
+    pdl_turn();
+    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1;
+    const int i = blockIdx.x * ROWS + threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const int n = a.counts ? min(a.T, a.counts[b]) : a.T;
+    const Pool& p = a.pool;
+    const long long at = (long long)max(0, p.lens[b]) + i;
+    long long row = -1;
+    if (i < n && at < (long long)p.width << p.shift) row = pool_row(p, b, h, at);
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (row >= 0) raw = __ldg(reinterpret_cast<const uint4*>(a.x[which] + b * a.batch[which] + i * a.token[which] + h * a.head[which]) + lane);
+    store_row<F, D>(which ? p.vc : p.kc, which ? p.ve : p.ke, which ? p.vs : p.ks, row, lane, raw);
+}
+
+// fp16 of a value beyond its range: the largest.  (A code may be above the value it stands for: 65504 is held as 65536.)
+__device__ __forceinline__ float saturated(float x) { return fabsf(x) > 65504.f ? copysignf(65504.f, x) : x; }
+
+struct ReadArgs {
+    Pool pool;
+    __half* x[2];
+    int most;
+};
+
+template <int F, int D>
+__global__ void __launch_bounds__(THREADS) read_kernel(ReadArgs a) {
+    constexpr int LANES = D / VALUES, ROWS = THREADS / LANES;
+    pdl_turn();
+    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1;
+    const int i = blockIdx.x * ROWS + threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    if (i >= a.most) return;
+    const Pool& p = a.pool;
+    const long long row = i < length_of(p, b) ? pool_row(p, b, h, i) : -1;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row >= 0) {
+        const uint8_t* codes = which ? p.vc : p.kc;
+        if constexpr (F == AKV_PAGE_FP16) {
+            v = *reinterpret_cast<const uint4*>(codes + row * (2 * D) + lane * 16);
+        } else {
+            const float unit = power2((which ? p.ve : p.ke)[row]);
+            float scale = 1.f;                 // (multiplied first: codes times scales are exact, and far from fp32's ends)
+            uint32_t h2[4];
+            if constexpr (F == AKV_PAGE_E4M3) {
+                const uint2 w = *reinterpret_cast<const uint2*>(codes + row * D + lane * VALUES);
+                h2[0] = e4m3_halves(w.x & 0xFFFFu);
+                h2[1] = e4m3_halves(w.x >> 16);
+                h2[2] = e4m3_halves(w.y & 0xFFFFu);
+                h2[3] = e4m3_halves(w.y >> 16);
+            } else {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + row * (D / 2) + lane * 4);
+                scale = e4m3_float((which ? p.vs : p.ks)[row * (D / 16) + (lane >> 1)]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) h2[k] = e2m1_halves((w >> (8 * k)) & 0xFFu);
+            }
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = halves_floats(h2[k]);
+                const __half2 r = __floats2half2_rn(saturated(f.x * scale * unit), saturated(f.y * scale * unit));
+                o[k] = *reinterpret_cast<const uint32_t*>(&r);
+            }
+            v = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+    *(reinterpret_cast<uint4*>(a.x[which] + (((long long)b * a.most + i) * p.H + h) * D) + lane) = v;
+}
+
+template <int F>
+void launch_append(const AppendArgs& a, int D, int bsz, cudaStream_t st) {
+    const int rows = THREADS / (D / VALUES);
+    const dim3 grid((a.T + rows - 1) / rows, 2 * a.pool.H, bsz);
+    if (D == 128) launch_chained(append_kernel<F, 128>, grid, dim3(THREADS), 0, st, a);
+    else launch_chained(append_kernel<F, 64>, grid, dim3(THREADS), 0, st, a);
+}
+template <int F>
+void launch_read(const ReadArgs& a, int D, int bsz, cudaStream_t st) {
+    const int rows = THREADS / (D / VALUES);
+    const dim3 grid((unsigned)(((long long)a.most + rows - 1) / rows), 2 * a.pool.H, bsz);
+    if (D == 128) launch_chained(read_kernel<F, 128>, grid, dim3(THREADS), 0, st, a);
+    else launch_chained(read_kernel<F, 64>, grid, dim3(THREADS), 0, st, a);
+}
+
+bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+}  // namespace
+
+int fill_pool(const char* what, const akv_pool* pool, const void* pages, const void* lens, int bsz, int width, Pool* p) {
+    AKV_REQUIRE(pool && pages && lens, AKV_ERR_NULL, "%s: null pointer", what);
+    const int D = pool->head_dim, f = pool->format;
+    AKV_REQUIRE(f == AKV_PAGE_FP16 || f == AKV_PAGE_E4M3 || f == AKV_PAGE_E2M1, AKV_ERR_SHAPE, "%s: page format %d", what, f);
+    AKV_REQUIRE(D == 64 || D == 128, AKV_ERR_SHAPE, "%s: head size %d (64 and 128 are covered)", what, D);
+    AKV_REQUIRE(pool->n_pages > 0 && pool->n_kv_heads > 0 && pool->n_kv_heads <= 4096 && bsz > 0 && bsz <= 4096 && width > 0, AKV_ERR_SHAPE,
+                "%s: bad extent (%d sequences, %d pages each, %d KV heads, %d pages in all)", what, bsz, width, pool->n_kv_heads, pool->n_pages);
+    const int P = pool->page_size;
+    AKV_REQUIRE(P >= 16 && P <= 256 && (P & (P - 1)) == 0, AKV_ERR_SHAPE, "%s: page size %d (a power of two from 16 to 256)", what, P);
+    AKV_REQUIRE((long long)width * P <= INT_MAX / 2, AKV_ERR_OVERFLOW, "%s: %d pages of %d tokens in a sequence", what, width, P);
+    AKV_REQUIRE(pool->k_codes && pool->v_codes && (f == AKV_PAGE_FP16 || (pool->k_exps && pool->v_exps)) &&
+                    (f != AKV_PAGE_E2M1 || (pool->k_scales && pool->v_scales)),
+                AKV_ERR_NULL, "%s: null pointer in the pool", what);
+    AKV_REQUIRE(aligned16(pool->k_codes) && aligned16(pool->v_codes) && aligned16(pool->k_exps) && aligned16(pool->v_exps) &&
+                    aligned16(pool->k_scales) && aligned16(pool->v_scales),
+                AKV_ERR_ALIGN, "%s: the pool's pointers must be 16-byte aligned", what);
+    AKV_REQUIRE(!misaligned(pages, 4) && !misaligned(lens, 4), AKV_ERR_ALIGN, "%s: pages and lens must be 4-byte aligned", what);
+    *p = Pool{static_cast<uint8_t*>(pool->k_codes), static_cast<uint8_t*>(pool->v_codes), static_cast<int8_t*>(pool->k_exps),
+              static_cast<int8_t*>(pool->v_exps), static_cast<uint8_t*>(pool->k_scales), static_cast<uint8_t*>(pool->v_scales),
+              pool->n_pages, 0, pool->n_kv_heads, static_cast<const int*>(pages), static_cast<const int*>(lens), width};
+    while ((1 << p->shift) < P) ++p->shift;
+    return AKV_OK;
+}
+
+}  // namespace akv
+
+using namespace akv;
+
+extern "C" {
+
+int akv_paged_append(const akv_pool* pool, const void* k, const void* v, const long long* strides, const void* pages, const void* lens,
+                     const void* counts, int bsz, int width, int tokens, void* stream) {
+    set_error("");
+    AppendArgs a = {};
+    const int rc = fill_pool("paged_append", pool, pages, lens, bsz, width, &a.pool);
+    if (rc != AKV_OK) return rc;
+    AKV_REQUIRE(k && v && strides, AKV_ERR_NULL, "paged_append: null pointer");
+    AKV_REQUIRE(tokens > 0 && tokens <= 1 << 30, AKV_ERR_SHAPE, "paged_append: %d tokens", tokens);
+    bool straight = aligned16(k) && aligned16(v) && !misaligned(counts, 4);
+    for (int i = 0; i < 6; ++i) straight = straight && strides[i] % 8 == 0;
+    AKV_REQUIRE(straight, AKV_ERR_ALIGN, "paged_append: rows of k and v must lie on 16-byte boundaries, counts on 4-byte ones");
+    a.x[0] = static_cast<const __half*>(k);
+    a.x[1] = static_cast<const __half*>(v);
+    for (int w = 0; w < 2; ++w) {
+        a.batch[w] = strides[3 * w];
+        a.token[w] = strides[3 * w + 1];
+        a.head[w] = strides[3 * w + 2];
+    }
+    a.counts = static_cast<const int*>(counts);
+    a.T = tokens;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int D = pool->head_dim;
+    if (pool->format == AKV_PAGE_FP16) launch_append<AKV_PAGE_FP16>(a, D, bsz, st);
+    else if (pool->format == AKV_PAGE_E4M3) launch_append<AKV_PAGE_E4M3>(a, D, bsz, st);
+    else launch_append<AKV_PAGE_E2M1>(a, D, bsz, st);
+    return cuda_status(cudaGetLastError(), "paged_append launch");
+}
+
+int akv_paged_read(const akv_pool* pool, const void* pages, const void* lens, void* k, void* v, int bsz, int width, int most, void* stream) {
+    set_error("");
+    ReadArgs a = {};
+    const int rc = fill_pool("paged_read", pool, pages, lens, bsz, width, &a.pool);
+    if (rc != AKV_OK) return rc;
+    AKV_REQUIRE(k && v, AKV_ERR_NULL, "paged_read: null pointer");
+    AKV_REQUIRE(most > 0 && most <= 1 << 30, AKV_ERR_SHAPE, "paged_read: %d tokens", most);
+    AKV_REQUIRE(aligned16(k) && aligned16(v), AKV_ERR_ALIGN, "paged_read: k and v must be 16-byte aligned");
+    a.x[0] = static_cast<__half*>(k);
+    a.x[1] = static_cast<__half*>(v);
+    a.most = most;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int D = pool->head_dim;
+    if (pool->format == AKV_PAGE_FP16) launch_read<AKV_PAGE_FP16>(a, D, bsz, st);
+    else if (pool->format == AKV_PAGE_E4M3) launch_read<AKV_PAGE_E4M3>(a, D, bsz, st);
+    else launch_read<AKV_PAGE_E2M1>(a, D, bsz, st);
+    return cuda_status(cudaGetLastError(), "paged_read launch");
+}
+
+}  // extern "C"

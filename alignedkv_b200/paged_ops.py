@@ -1,0 +1,162 @@
+"""Operators over a cache in pages: sequences with lengths of their own, quantised as they are written.
+
+  paged_append      keys and values of new tokens enter the pages
+  paged_read        what the pages hold, as dense fp16 tensors
+  paged_attention   the newest tokens of every sequence attend to it
+
+The reference has no counterpart: its cache is one tensor per layer with one length for the whole batch (extension/k_cache_file.py:34-53,
+extension/v_cache_file.py:35-54).
+
+`cache` is anything with a layer's pool as attributes, of which `paged.PagedLayer` is one:
+  k_codes, v_codes    [pages, H, page_size, D] torch.half (as they are) or torch.float8_e4m3fn, or [pages, H, page_size, D / 2] torch.uint8 (e2m1, the
+                      even channel in the lower 4 bits)
+  k_exps, v_exps      int8 [pages, H, page_size], for e4m3 and e2m1: the codes of a row are multiplied by 2**exp
+  k_scales, v_scales  float8_e4m3fn [pages, H, page_size, D / 16], for e2m1: a factor per 16 channels
+D is 64 or 128, page_size a power of two from 16 to 256.  Of a row x of D values, e4m3: exp is the least integer with max |x| <= 448 * 2**exp;
+e2m1: the least with max |x| <= 2688 * 2**exp, and a scale is max |x| * 2**-exp / 6 over its channels; every rounding goes to the nearest value, ties
+to even.  A row with a value that is not finite stands for NaN throughout (exp -128), except in a pool of torch.half.
+
+pages int32 [B, width]: position t of sequence b lies in page pages[b, t // page_size].  An entry outside 0..pages-1 is a page that was given
+up (-1, say): its tokens have no part in attention, are read as zeros, and what would be written there is dropped.  Entries behind a
+sequence's last token are not looked at.  lens int32 [B], on the device: nothing here waits for it, and a captured graph replays with
+what it holds then.  A length beyond the table counts as the table's, a negative one as 0.
+
+Everything is launched on torch's current stream of the pool's device; nothing synchronises.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .cache_ops import _need, _nothing
+
+__all__ = ["paged_append", "paged_read", "paged_attention"]
+
+MOST_ROWS = 64
+_FORMATS = {torch.half: 0, torch.float8_e4m3fn: 1, torch.uint8: 2}
+
+
+class _Call:
+    """A pool's tensors and a batch's table, checked, as the library takes them."""
+    __slots__ = ("device", "index", "B", "W", "H", "D", "P", "pool", "pages", "lens")
+
+    def __init__(self, cache, pages, lens):
+        codes = cache.k_codes
+        if not isinstance(codes, torch.Tensor) or not codes.is_cuda or codes.dim() != 4 or codes.dtype not in _FORMATS:
+            raise RuntimeError("k_codes: expected a CUDA tensor of shape [pages, H, page_size, row], torch.half, torch.float8_e4m3fn or torch.uint8")
+        form = _FORMATS[codes.dtype]
+        self.device, self.index = codes.device, codes.get_device()
+        N, H, P, row = codes.shape
+        D = 2 * row if form == 2 else row
+        if D not in (64, 128):
+            raise RuntimeError(f"head size {D}: these operators cover 64 and 128")
+        if P not in (16, 32, 64, 128, 256):
+            raise RuntimeError(f"page size {P}: expected a power of two from 16 to 256")
+        self.H, self.D, self.P = H, D, P
+        dev, shape = self.index, tuple(codes.shape)
+        ptrs = [_need("k_codes", codes, shape, codes.dtype, dev), _need("v_codes", cache.v_codes, shape, codes.dtype, dev), None, None, None, None]
+        if form:
+            ptrs[2:4] = [_need(n, getattr(cache, n), (N, H, P), torch.int8, dev) for n in ("k_exps", "v_exps")]
+        if form == 2:
+            ptrs[4:] = [_need(n, getattr(cache, n), (N, H, P, D // 16), torch.float8_e4m3fn, dev) for n in ("k_scales", "v_scales")]
+        if not isinstance(pages, torch.Tensor) or pages.dim() != 2 or pages.shape[0] == 0 or pages.shape[1] == 0:
+            raise RuntimeError("pages: expected a tensor of shape [B, width]")
+        self.B, self.W = pages.shape
+        self.pages = _need("pages", pages, (self.B, self.W), torch.int32, dev)
+        self.lens = _need("lens", lens, (self.B,), torch.int32, dev)
+        self.pool = _lib.Pool(*ptrs, form, N, P, H, D)
+
+    def here(self):
+        return _nothing if torch.cuda.current_device() == self.index else torch.cuda.device(self.index)
+
+
+def _rows(name: str, x, like: tuple, index: int) -> list:
+    """Strides (batch, token, head) of x [B,T,H,D] fp16, whose rows of D are contiguous and begin on 16-byte boundaries."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 4 or x.dtype is not torch.half or x.get_device() != index or \
+            (x.shape[0], x.shape[2], x.shape[3]) != like or x.shape[1] == 0 or x.stride(3) != 1 or x.data_ptr() % 16:
+        raise RuntimeError(f"{name}: expected an fp16 tensor of shape [{like[0]}, T, {like[1]}, {like[2]}] on cuda:{index} with a unit stride "
+                           "along the channels, on a 16-byte boundary")
+    strides = [s if n > 1 else 0 for s, n in zip(x.stride()[:3], x.shape)]
+    if any(s % 8 for s in strides):
+        raise RuntimeError(f"{name}: strides {tuple(x.stride())} do not keep its rows on 16-byte boundaries")
+    return strides
+
+
+def paged_append(cache, k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, lens: torch.Tensor, *,
+                 counts: torch.Tensor | None = None) -> None:
+    """Keys and values of new tokens enter the pages, quantised as the pool holds them.
+
+    k, v [B,T,H,D] fp16, of any strides that keep rows of D together and on 16-byte boundaries (a part of a fused projection, say).  The first
+    counts[b] (int32 [B]; by default all T) tokens of sequence b go to positions lens[b], lens[b] + 1, ...; what would lie behind the
+    table's end is dropped.  Nothing else in the pool changes.  lens stays: the caller adds what was appended.  Positions that
+    two sequences share (pages of a common prompt) must not be appended to; where two tokens have one place, either may be left there,
+    or parts of both."""
+    c = _Call(cache, pages, lens)
+    like = (c.B, c.H, c.D)
+    strides = _rows("k", k, like, c.index) + _rows("v", v, like, c.index)
+    T = k.shape[1]
+    if v.shape[1] != T:
+        raise RuntimeError(f"v: {v.shape[1]} tokens, k has {T}")
+    count_ptr = None if counts is None else _need("counts", counts, (c.B,), torch.int32, c.index)
+    with c.here():
+        rc = _lib.load().akv_paged_append(ctypes.byref(c.pool), k.data_ptr(), v.data_ptr(), (ctypes.c_longlong * 6)(*strides), c.pages, c.lens,
+                                          count_ptr, c.B, c.W, T, _lib.raw_stream(c.index))
+    _lib.check("paged_append", rc)
+
+
+def paged_read(cache, pages: torch.Tensor, lens: torch.Tensor, most: int) -> tuple:
+    """(k, v) fp16 [B,most,H,D]: positions 0..most-1 of every sequence as the pages hold them, zeros at and behind lens[b].
+
+    The value of a code is rounded once, to fp16; beyond fp16's range to its largest."""
+    c = _Call(cache, pages, lens)
+    if most < 1:
+        raise RuntimeError(f"most: {most} tokens, expected at least 1")
+    k = torch.empty((c.B, most, c.H, c.D), dtype=torch.half, device=c.device)
+    v = torch.empty_like(k)
+    with c.here():
+        rc = _lib.load().akv_paged_read(ctypes.byref(c.pool), c.pages, c.lens, k.data_ptr(), v.data_ptr(), c.B, c.W, most,
+                                        _lib.raw_stream(c.index))
+    _lib.check("paged_read", rc)
+    return k, v
+
+
+def paged_attention(cache, q: torch.Tensor, pages: torch.Tensor, lens: torch.Tensor, *, scale: float | None = None, lse: bool = False,
+                    out: torch.Tensor | None = None):
+    """Attention output [B,T,Hq,D] of the T newest tokens of every sequence.
+
+    q [B,T,Hq,D] fp16; their keys and values are in the pages and counted by lens (`paged_append` comes first).  Query t sees the
+    positions below lens[b] - (T - 1) + t: a decode step with T = 1, a chain of drafted tokens with more.  Query head i reads KV head
+    i // (Hq / H); T * (Hq / H) is at most 64.  A row that sees nothing - an empty sequence, a query before its sequence's first
+    token, nothing but pages that were given up - is zero.
+
+    The output is that of dense attention over the values that the codes stand for, with fp32 scores (times `scale`, by default
+    D**-0.5), softmax and sums and one rounding to fp16.  What lies in the pages behind lens[b] has no part in it, whatever it is.
+    lse=True also returns the logarithm of the rows' sums of exponentials, fp32 [B,T,Hq] (-inf where nothing is seen)."""
+    c = _Call(cache, pages, lens)
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[0] != c.B or q.shape[3] != c.D or q.dtype is not torch.half or \
+            q.get_device() != c.index or not q.is_contiguous():
+        raise RuntimeError(f"q: expected a contiguous fp16 tensor of shape [{c.B}, T, Hq, {c.D}] on {c.device}")
+    T, Hq = q.shape[1], q.shape[2]
+    if Hq % c.H or Hq == 0:
+        raise RuntimeError(f"q: {Hq} query heads are no multiple of {c.H} KV heads")
+    group = Hq // c.H
+    if not 1 <= T * group <= MOST_ROWS:
+        raise RuntimeError(f"q: {T} tokens of {group} query heads per KV head, expected 1 to {MOST_ROWS} rows")
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        begin = _need("out", out, tuple(q.shape), torch.half, c.index)
+        if begin < q.data_ptr() + 2 * q.numel() and q.data_ptr() < begin + 2 * out.numel():
+            raise RuntimeError("out: overlaps q")
+    lib = _lib.load()
+    sums = q.new_empty((c.B, T, Hq), dtype=torch.float32) if lse else None
+    with c.here():
+        ws = torch.empty(max(0, lib.akv_paged_scratch_bytes(ctypes.byref(c.pool), c.B, c.W, group, T)), dtype=torch.uint8, device=c.device)
+        rc = lib.akv_paged_attention(ctypes.byref(c.pool), q.data_ptr(), c.pages, c.lens, out.data_ptr(), sums.data_ptr() if lse else None,
+                                     ws.data_ptr(), ws.numel(), c.B, c.W, group, T, 1.0 / math.sqrt(c.D) if scale is None else scale,
+                                     _lib.raw_stream(c.index))
+    _lib.check("paged_attention", rc)
+    return (out, sums) if lse else out

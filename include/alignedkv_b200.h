@@ -438,6 +438,66 @@ int akv_evict(const akv_layer* layer, void* weights, void* positions, int rest_l
               int arranged, int shift, void* stream);
 
 /*
+ * A cache in pages (no counterpart in the reference, whose cache is one tensor of one length): sequences have lengths of their own, and
+ * their tokens lie in pages of a pool, in one of three formats.  codes [n_pages, H, page_size] rows of head_dim channels:
+ *   AKV_PAGE_FP16   fp16 as it is; exps and scales NULL
+ *   AKV_PAGE_E4M3   a byte per channel, x = code 2^e: e the least with max |x| <= 448 2^e; scales NULL
+ *   AKV_PAGE_E2M1   4 bits per channel, the even one in the lower bits, x = code s 2^e: e the least with max |x| <= 2688 2^e, s (e4m3) the
+ *                   nearest to max |x| 2^-e / 6 over 16 channels
+ * exps: int8 [n_pages, H, page_size] (e of all zeros: as of fp16's smallest magnitude; -128: a value of the row is not finite, the row stands
+ * for NaN); scales: bytes [n_pages, H, page_size, head_dim / 16].  Roundings to the nearest, ties to even.  head_dim 64 or 128; page_size a power of
+ * two from 16 to 256; every pointer of the pool 16-byte aligned.
+ *
+ * pages: int32 [bsz, width], position t of sequence b lies in page pages[b][t / page_size].  An entry outside 0..n_pages-1 is a page that was
+ * given up: its tokens have no part in attention, are read as zeros, and what would be written there is dropped.  Entries behind a sequence's
+ * last token are not looked at.  lens: int32 [bsz], at most width * page_size tokens count, a negative one is 0.  Up to 4096 sequences and KV heads.
+ *
+ * akv_paged_append: token i < min(tokens, counts[b]) (counts NULL: all) of sequence b goes to position lens[b] + i; what lies behind the
+ * table's end is dropped.  k, v fp16, strides: 6 numbers of halves, {batch, token, head} of k, then of v, multiples of 8.  Positions that two
+ * sequences share must not be written.  The caller adds counts to lens.
+ *
+ * akv_paged_read: k, v fp16 [bsz, most, H, head_dim], positions 0..most-1 of every sequence, zeros at and behind lens[b].  A value beyond fp16 is
+ * read as its largest.
+ *
+ * akv_paged_attention: the `tokens` newest tokens of every sequence, which are in the pages and counted by lens, attend to it: q, out
+ * fp16 [bsz, tokens, H * group, head_dim], query t sees positions below lens[b] - tokens + 1 + t.  At most 64 rows (tokens * group).  fp32 scores, softmax
+ * and sums over the values that the codes stand for, one rounding.  A row that sees nothing is 0, its lse -inf.  lse (may be NULL): fp32
+ * [bsz, tokens, H * group].  out must not overlap an input.  scratch: akv_paged_scratch_bytes(...) bytes, any contents.
+ */
+#define AKV_PAGE_FP16 0
+#define AKV_PAGE_E4M3 1
+#define AKV_PAGE_E2M1 2
+typedef struct akv_pool {
+    void *k_codes, *v_codes, *k_exps, *v_exps, *k_scales, *v_scales;
+    int format, n_pages, page_size, n_kv_heads, head_dim;
+} akv_pool;
+int akv_paged_append(const akv_pool* pool, const void* k, const void* v, const long long* strides, const void* pages, const void* lens,
+                     const void* counts, int bsz, int width, int tokens, void* stream);
+int akv_paged_read(const akv_pool* pool, const void* pages, const void* lens, void* k, void* v, int bsz, int width, int most, void* stream);
+long long akv_paged_scratch_bytes(const akv_pool* pool, int bsz, int width, int group, int tokens);
+int akv_paged_attention(const akv_pool* pool, const void* q, const void* pages, const void* lens, void* out, void* lse, void* scratch,
+                        long long scratch_bytes, int bsz, int width, int group, int tokens, float scale, void* stream);
+
+/*
+ * Which of the drafted tokens are accepted and which token follows, such that the output has the target's distribution (no counterpart in
+ * the reference).  `drafted` nodes (1..64) per sequence; node 0 is taken already, node i >= 1 hangs under parents[i] < i (int32, parents_batch
+ * apart, 0 = one row for all; NULL: a chain; an entry that is no earlier node: never reached).  ids int64 [bsz, drafted].  target: probabilities
+ * [bsz, drafted, vocab] of what follows each node, rows target_row elements apart, sequences target_batch; draft the same for those that each node's children
+ * were drawn from (rows of leaves are not read), or NULL where drafts are guesses.  type AKV_TYPE_*.  coins fp32 [bsz, drafted] in [0,1): coins[i] decides
+ * over node i, coins[0] chooses what follows.  Entries that are not positive and finite count as 0; a token outside the vocabulary has no probability.
+ *   Children of the accepted node are asked in order: r = max(p - c q, 0), c = 0, Z = 1 at first; accepted if u Z q(x) < r(x); rejected: c += Z,
+ *   Z = sum r.  Without draft: accepted if u Z < p(x); rejected: Z -= p(x), p(x) = 0.  At the end the smallest j with cumsum(r)[j] > u sum(r); where
+ *   r sums to 0, of p.
+ * path: int32 [bsz, drafted], the accepted nodes from 0 on, -1 behind them; count int32 [bsz]; token int64 [bsz] (-1 where the row has no probability).
+ */
+#define AKV_TYPE_FP32 0
+#define AKV_TYPE_FP16 1
+#define AKV_TYPE_BF16 2
+int akv_accept_drafts(const void* target, long long target_batch, long long target_row, const void* draft, long long draft_batch,
+                      long long draft_row, const void* ids, const void* coins, const void* parents, long long parents_batch, void* path,
+                      void* count, void* token, int bsz, int drafted, int vocab, int type, void* stream);
+
+/*
  * Benchmark instrumentation (no counterpart in the reference): with akv_set_tuning("timing", 1), akv_decode_step
  * records CUDA events around its q.K^T and P.V launches.  akv_timing_read returns how many steps were recorded
  * since akv_timing_reset and their median launch durations in microseconds; synchronise the stream first.
