@@ -53,6 +53,15 @@ __device__ __forceinline__ uint32_t e2m1_halves(uint32_t two) {
     asm("{\n.reg .b8 b;\ncvt.u8.u32 b, %1;\ncvt.rn.f16x2.e2m1x2 %0, b;\n}\n" : "=r"(h) : "r"(two));
     return h;
 }
+// Four codes of a word, eight.
+__device__ __forceinline__ void e4m3_word(uint32_t (&h)[2], uint32_t word) {
+    asm("{\n.reg .b16 l, u;\nmov.b32 {l, u}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, u;\n}\n" : "=r"(h[0]), "=r"(h[1]) : "r"(word));
+}
+__device__ __forceinline__ void e2m1_word(uint32_t (&h)[4], uint32_t word) {
+    asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %4;\ncvt.rn.f16x2.e2m1x2 %0, a;\ncvt.rn.f16x2.e2m1x2 %1, b;\n"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\ncvt.rn.f16x2.e2m1x2 %3, d;\n}\n"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(word));
+}
 __device__ __forceinline__ float2 halves_floats(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
 __device__ __forceinline__ float e4m3_float(uint32_t code) { return halves_floats(e4m3_halves(code)).x; }
 

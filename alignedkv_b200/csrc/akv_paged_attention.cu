@@ -176,10 +176,11 @@ __device__ __forceinline__ long long row_of(const AttendArgs& a, int unit, int r
 }
 
 // ---------------------------------------------------------------- a warp's run
-template <int F, int D, int NT>
+// ONE: a step's tokens are in one page.
+template <int F, int D, int NT, bool ONE>
 struct Run {
     using S = Shape<F, D, NT>;
-    static constexpr int U = S::U, KW = S::KW, KS = S::KS;
+    static constexpr int U = S::U, KW = S::KW, KS = S::KS, PAGES = ONE ? 1 : U;
     const AttendArgs& a;
     int g, t;
     uint32_t q[KS][NT][2];
@@ -225,72 +226,96 @@ struct Run {
     }
 
     // Pages of a step's tiles; -1 where there is none or nothing of the sequence in it.
-    __device__ __forceinline__ void look(int (&page)[U], int b, int at, int n) const {
+    __device__ __forceinline__ void look(int (&page)[PAGES], int b, int at, int n) const {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < PAGES; ++u) {
             page[u] = -1;
             if (at + 16 * u < n) {
-                const int x = __ldg(a.pool.table + (long long)b * a.pool.width + ((at + 16 * u) >> a.pool.shift));
+                const int x = __ldg(a.pool.table + (unsigned)b * (unsigned)a.pool.width + ((at + 16 * u) >> a.pool.shift));
                 if ((unsigned)x < (unsigned)a.pool.n_pages) page[u] = x;
             }
         }
     }
+    static __device__ __forceinline__ bool missing(const int (&page)[PAGES], int u) { return page[ONE ? 0 : u] < 0; }
     // First row of the pool of a tile (of some page where there is none: what is read from it is not used).
-    __device__ __forceinline__ long long tile_row(int page, int h, int at) const {
-        return (((long long)max(page, 0) * a.pool.H + h) << a.pool.shift) + (at & ((1 << a.pool.shift) - 1));
+    __device__ __forceinline__ unsigned tile_row(const int (&page)[PAGES], int u, int h, int at) const {
+        const int from = ONE ? at : at + 16 * u;
+        return (((unsigned)max(page[ONE ? 0 : u], 0) * (unsigned)a.pool.H + h) << a.pool.shift) + (from & ((1 << a.pool.shift) - 1)) + (ONE ? 16 * u : 0);
     }
-    __device__ __forceinline__ void load_k(const int (&page)[U], int h, int at) {
+    // (Addresses are a tensor's, the step's row's and the lane's; tiles and tokens are constants behind them.)
+    static __device__ __forceinline__ const uint8_t* place(const void* base, unsigned row, int size, int mine) {
+        return static_cast<const uint8_t*>(base) + (unsigned long long)row * size + mine;
+    }
+    __device__ __forceinline__ void load_k(const int (&page)[PAGES], int h, int at) {
+        constexpr int PIECE = S::ROW >= 64 ? 16 : 8;
+        const uint8_t *p = nullptr, *pe = nullptr, *pv = nullptr, *ps = nullptr;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long row = tile_row(page[u], h, at + 16 * u);
+            if (!ONE || u == 0) {
+                const unsigned row = tile_row(page, u, h, at);
+                p = place(a.pool.kc, row, S::ROW, k_token(0) * S::ROW + t * PIECE);
+                if constexpr (F != AKV_PAGE_FP16) {
+                    pe = place(a.pool.ke, row, 1, 4 * (g >> 1));
+                    pv = place(a.pool.ve, row, 1, 4 * (g >> 1));
+                }
+                if constexpr (F == AKV_PAGE_E2M1) ps = place(a.pool.ks, row, D / 16, k_token(0) * (D / 16) + t * (D / 64));
+            }
+            const int tile = ONE ? 16 * u : 0;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const uint8_t* p = a.pool.kc + (row + k_token(half)) * S::ROW;
+                const uint8_t* x = p + (tile + 2 * half) * S::ROW;
                 if constexpr (S::ROW >= 64) {
 #pragma unroll
                     for (int c = 0; c < S::ROW / 64; ++c) {
-                        const uint4 w = stream16(p + c * 64 + t * 16);
+                        const uint4 w = stream16(x + c * 64);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) k[u][half * (KW / 2) + 4 * c + i] = u4w(w, i);
                     }
                 } else {
-                    const uint2 w = stream8(p + t * 8);
+                    const uint2 w = stream8(x);
                     k[u][half * 2] = w.x;
                     k[u][half * 2 + 1] = w.y;
                 }
                 if constexpr (F == AKV_PAGE_E2M1) {
-                    const uint8_t* s = a.pool.ks + (row + k_token(half)) * (D / 16);
-                    ks[u][half] = D == 128 ? load2(s + 2 * t) : load1(s + t);
+                    const uint8_t* y = ps + (tile + 2 * half) * (D / 16);
+                    ks[u][half] = D == 128 ? load2(y) : load1(y);
                 }
             }
             if constexpr (F != AKV_PAGE_FP16) {
-                ke[u] = load4(a.pool.ke + row + 4 * (g >> 1));
-                ve[u] = load4(a.pool.ve + row + 4 * (g >> 1));
+                ke[u] = load4(pe + tile);
+                ve[u] = load4(pv + tile);
             }
         }
     }
-    __device__ __forceinline__ void load_v(const int (&page)[U], int h, int at) {
+    __device__ __forceinline__ void load_v(const int (&page)[PAGES], int h, int at) {
+        constexpr int PIECE = S::ROW >= 128 ? 16 : S::ROW / 8;
+        const uint8_t *p = nullptr, *ps = nullptr;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long row = tile_row(page[u], h, at + 16 * u) + 4 * t;
+            if (!ONE || u == 0) {
+                const unsigned row = tile_row(page, u, h, at);
+                p = place(a.pool.vc, row, S::ROW, 4 * t * S::ROW + g * PIECE);
+                if constexpr (F == AKV_PAGE_E2M1) ps = place(a.pool.vs, row, D / 16, 4 * t * (D / 16) + (D == 128 ? g : g >> 1));
+            }
+            const int tile = ONE ? 16 * u : 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint8_t* p = a.pool.vc + (row + i) * S::ROW;
+                const uint8_t* x = p + (tile + i) * S::ROW;
                 if constexpr (S::ROW >= 128) {
 #pragma unroll
                     for (int c = 0; c < S::ROW / 128; ++c) {
-                        const uint4 w = stream16(p + c * 128 + g * 16);
+                        const uint4 w = stream16(x + c * 128);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) v[u][i * (KW / 4) + 4 * c + j] = u4w(w, j);
                     }
                 } else if constexpr (S::ROW == 64) {
-                    const uint2 w = stream8(p + g * 8);
+                    const uint2 w = stream8(x);
                     v[u][i * 2] = w.x;
                     v[u][i * 2 + 1] = w.y;
                 } else {
-                    v[u][i] = stream4(p + g * 4);
+                    v[u][i] = stream4(x);
                 }
-                if constexpr (F == AKV_PAGE_E2M1) vs[u][i] = load1(a.pool.vs + (row + i) * (D / 16) + (D == 128 ? g : g >> 1));
+                if constexpr (F == AKV_PAGE_E2M1) vs[u][i] = load1(ps + (tile + i) * (D / 16));
             }
         }
     }
@@ -311,54 +336,63 @@ struct Run {
             } else if constexpr (F == AKV_PAGE_E4M3) {
 #pragma unroll
                 for (int i = 0; i < KS; ++i) {
-                    const uint32_t a0 = e4m3_halves(k[u][i] & 0xFFFFu), a2 = e4m3_halves(k[u][i] >> 16);
-                    const uint32_t a1 = e4m3_halves(k[u][H + i] & 0xFFFFu), a3 = e4m3_halves(k[u][H + i] >> 16);
+                    uint32_t x[2], y[2];
+                    e4m3_word(x, k[u][i]);
+                    e4m3_word(y, k[u][H + i]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma(s[u][nt], a0, a1, a2, a3, q[i][nt][0], q[i][nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) mma(s[u][nt], x[0], y[0], x[1], y[1], q[i][nt][0], q[i][nt][1]);
                 }
             } else {
                 const uint32_t s0 = e4m3_halves(ks[u][0]), s1 = e4m3_halves(ks[u][1]);
 #pragma unroll
-                for (int i = 0; i < KS; ++i) {
+                for (int w = 0; w < H; ++w) {
                     // (8 channels of a word: two products; 16 have a scale)
-                    const uint32_t w0 = k[u][i >> 1] >> (16 * (i & 1)), w1 = k[u][H + (i >> 1)] >> (16 * (i & 1));
-                    const uint32_t f0 = __byte_perm(s0, s0, D == 128 && i >= 4 ? 0x3232 : 0x1010);
-                    const uint32_t f1 = __byte_perm(s1, s1, D == 128 && i >= 4 ? 0x3232 : 0x1010);
-                    const uint32_t a0 = hmul2_bits(e2m1_halves(w0 & 0xFFu), f0), a2 = hmul2_bits(e2m1_halves((w0 >> 8) & 0xFFu), f0);
-                    const uint32_t a1 = hmul2_bits(e2m1_halves(w1 & 0xFFu), f1), a3 = hmul2_bits(e2m1_halves((w1 >> 8) & 0xFFu), f1);
+                    const uint32_t f0 = __byte_perm(s0, s0, D == 128 && w >= 2 ? 0x3232 : 0x1010), f1 = __byte_perm(s1, s1, D == 128 && w >= 2 ? 0x3232 : 0x1010);
+                    uint32_t x[4], y[4];
+                    e2m1_word(x, k[u][w]);
+                    e2m1_word(y, k[u][H + w]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma(s[u][nt], a0, a1, a2, a3, q[i][nt][0], q[i][nt][1]);
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma(s[u][nt], hmul2_bits(x[2 * i], f0), hmul2_bits(y[2 * i], f1), hmul2_bits(x[2 * i + 1], f0), hmul2_bits(y[2 * i + 1], f1),
+                                q[2 * w + i][nt][0], q[2 * w + i][nt][1]);
                 }
             }
         }
     }
 
     // Scores to weights of the values, in place, and the running maximum and sum with them.  seen(nt, c): tokens below it are seen by the row; page:
-    // -1 where the tile's tokens are not there.  ALL: every row sees the whole step.
+    // -1 where the tile's tokens are not there.  ALL: every row sees the whole step.  (An exponent of -128 comes out as a factor of
+    // -infinity: times the row's zeros NaN, as it should.)
     template <bool ALL>
-    __device__ __forceinline__ void soften(float (&s)[U][NT][4], const uint32_t (&ke)[U], const uint32_t (&ve)[U], const int (&page)[U], int at,
+    __device__ __forceinline__ void soften(float (&s)[U][NT][4], const uint32_t (&ke)[U], const uint32_t (&ve)[U], const int (&page)[PAGES], int at,
                                            const int (&seen)[NT][2]) {
-        float top[NT][2], unit[U][2];
+        float top[NT][2], f[U][2], unit[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                float f = a.scale2, e = 0.f;
-                unit[u][half] = 1.f;
+                float e = 0.f;
+                f[u][half] = a.scale2;
+                unit[u][half] = LIFT;
                 if constexpr (F != AKV_PAGE_FP16) {
                     const int i = (g & 1) + 2 * half, x = exponent_byte(ve[u], i);
-                    f *= power2(exponent_byte(ke[u], i));
+                    f[u][half] = a.scale2 * __int_as_float((exponent_byte(ke[u], i) + 127) << 23);
+                    unit[u][half] = __int_as_float((x + 127 + 15) << 23);
+                    if (x == EXP_NAN) unit[u][half] = NAN;
                     e = (float)max(x, -40);           // (a row of NaN has no exponent; -35 is the least there is)
-                    unit[u][half] = power2(x);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         float& x = s[u][nt][2 * half + c];
-                        x *= f;
-                        if (!ALL && (page[u] < 0 || at + 16 * u + k_token(half) >= seen[nt][c])) x = -INFINITY;
-                        const float y = x + e;
+                        if (!ALL) {
+                            x *= f[u][half];
+                            if (missing(page, u) || at + 16 * u + k_token(half) >= seen[nt][c]) x = -INFINITY;
+                        }
+                        const float y = ALL ? fmaf(x, f[u][half], e) : x + e;
                         top[nt][c] = u == 0 && half == 0 ? y : fmaxf(top[nt][c], y);
                     }
             }
@@ -374,20 +408,20 @@ struct Run {
         if (__any_sync(0xFFFFFFFFu, higher)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float f[2];
+                float g2[2];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const float y = fmaxf(top[nt][c], m[nt][c]);
-                    f[c] = y == m[nt][c] ? 1.f : ex2(m[nt][c] - y);
+                    g2[c] = y == m[nt][c] ? 1.f : ex2(m[nt][c] - y);
                     m[nt][c] = y;
-                    l[nt][c] *= f[c];
+                    l[nt][c] *= g2[c];
                 }
 #pragma unroll
                 for (int i = 0; i < KS; ++i) {
-                    acc[i][nt][0] *= f[0];
-                    acc[i][nt][1] *= f[1];
-                    acc[i][nt][2] *= f[0];
-                    acc[i][nt][3] *= f[1];
+                    acc[i][nt][0] *= g2[0];
+                    acc[i][nt][1] *= g2[1];
+                    acc[i][nt][2] *= g2[0];
+                    acc[i][nt][3] *= g2[1];
                 }
             }
         }
@@ -401,21 +435,21 @@ struct Run {
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         float& x = s[u][nt][2 * half + c];
-                        const bool gone = !ALL && (page[u] < 0 || at + 16 * u + k_token(half) >= seen[nt][c]);
-                        const float p = ex2(x - base);
+                        const bool gone = !ALL && (missing(page, u) || at + 16 * u + k_token(half) >= seen[nt][c]);
+                        const float p = ex2(ALL ? fmaf(x, f[u][half], -base) : x - base);
                         l[nt][c] += p;                              // (of what is not seen: 0)
-                        x = gone ? 0.f : p * (unit[u][half] * LIFT);
+                        x = gone ? 0.f : p * unit[u][half];
                     }
             }
     }
 
     // Values of a step that lie behind the sequence, or nowhere: zeros, whatever is there.
-    __device__ __forceinline__ void clear_v(const int (&page)[U], int at, int n) {
+    __device__ __forceinline__ void clear_v(const int (&page)[PAGES], int at, int n) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (page[u] < 0 || at + 16 * u + 4 * t + i >= n) {
+                if (missing(page, u) || at + 16 * u + 4 * t + i >= n) {
 #pragma unroll
                     for (int j = 0; j < KW / 4; ++j) v[u][i * (KW / 4) + j] = 0;
                     if constexpr (F == AKV_PAGE_E2M1) vs[u][i] = 0;
@@ -436,20 +470,27 @@ struct Run {
             for (int i = 0; i < KS; ++i) {
                 const uint32_t x = __byte_perm(v[u][i >> 1], v[u][W + (i >> 1)], i & 1 ? 0x7362 : 0x5140);
                 const uint32_t y = __byte_perm(v[u][2 * W + (i >> 1)], v[u][3 * W + (i >> 1)], i & 1 ? 0x7362 : 0x5140);
-                fn(i, e4m3_halves(x & 0xFFFFu), e4m3_halves(x >> 16), e4m3_halves(y & 0xFFFFu), e4m3_halves(y >> 16));
+                uint32_t p[2], r[2];
+                e4m3_word(p, x);
+                e4m3_word(r, y);
+                fn(i, p[0], p[1], r[0], r[1]);
             }
         } else {
-            const uint32_t s0 = e4m3_halves(vs[u][0] | vs[u][1] << 8), s1 = e4m3_halves(vs[u][2] | vs[u][3] << 8);
+            const uint32_t s0 = e4m3_halves(__byte_perm(vs[u][0], vs[u][1], 0x0040)), s1 = e4m3_halves(__byte_perm(vs[u][2], vs[u][3], 0x0040));
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 constexpr uint32_t LOW = 0x0F0F0F0Fu;
                 // two tokens' nibbles of one channel in a byte: even channels, odd ones
                 const uint32_t e0 = (v[u][w] & LOW) | ((v[u][W + w] << 4) & ~LOW), o0 = ((v[u][w] >> 4) & LOW) | (v[u][W + w] & ~LOW);
                 const uint32_t e1 = (v[u][2 * W + w] & LOW) | ((v[u][3 * W + w] << 4) & ~LOW), o1 = ((v[u][2 * W + w] >> 4) & LOW) | (v[u][3 * W + w] & ~LOW);
+                uint32_t x0[4], y0[4], x1[4], y1[4];
+                e2m1_word(x0, e0);
+                e2m1_word(y0, o0);
+                e2m1_word(x1, e1);
+                e2m1_word(y1, o1);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    fn(4 * w + i, hmul2_bits(e2m1_halves((e0 >> (8 * i)) & 0xFFu), s0), hmul2_bits(e2m1_halves((o0 >> (8 * i)) & 0xFFu), s0),
-                       hmul2_bits(e2m1_halves((e1 >> (8 * i)) & 0xFFu), s1), hmul2_bits(e2m1_halves((o1 >> (8 * i)) & 0xFFu), s1));
+                    fn(4 * w + i, hmul2_bits(x0[i], s0), hmul2_bits(y0[i], s0), hmul2_bits(x1[i], s1), hmul2_bits(y1[i], s1));
             }
         }
     }
@@ -597,10 +638,10 @@ __device__ __forceinline__ void join_row(const AttendArgs& a, int unit, int r, i
     if (a.lse && lane == 0) a.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 
-template <int F, int D, int NT>
+template <int F, int D, int NT, bool ONE>
 __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(AttendArgs a) {
     using S = Shape<F, D, NT>;
-    constexpr int WARPS = S::WARPS, U = S::U;
+    constexpr int WARPS = S::WARPS, U = S::U, PAGES = ONE ? 1 : U;
     extern __shared__ __align__(16) float records[];           // [warp][2][rows][D + 4]: of a run's first part and of its last
     int* cum = reinterpret_cast<int*>(records + WARPS * 2 * S::RECORD);
     __shared__ int sums[WARPS], s_unit[2 * WARPS];             // (s_unit: unit of each record, -1 where there is none)
@@ -618,11 +659,11 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
     if (lane < 2) s_unit[2 * warp + lane] = -1;
     __syncwarp();
     if (at < end) {
-        Run<F, D, NT> run(a, lane);
+        Run<F, D, NT, ONE> run(a, lane);
         Part part;
         part.find(cum, units, sequence_with(cum, a.B, units, at), at, end);
         int n = length_of(a.pool, part.b), h = part.unit / a.groups % a.pool.H;
-        int token = part.first * CHUNK, stop = min(n, part.last * CHUNK), page[U];
+        int token = part.first * CHUNK, stop = min(n, part.last * CHUNK), page[PAGES];
         run.look(page, part.b, token, n);
         run.load_k(page, h, token);
         run.load_v(page, h, token);
@@ -642,9 +683,9 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
             // the step behind this one: the unit's next, or the first of the next unit
             const Part was = part;
             const int was_token = token, was_n = n;
-            int was_page[U];
+            int was_page[PAGES];
 #pragma unroll
-            for (int u = 0; u < U; ++u) was_page[u] = page[u];
+            for (int u = 0; u < PAGES; ++u) was_page[u] = page[u];
             token += S::TOKENS;
             fresh = token >= stop;
             if (fresh) {
@@ -670,7 +711,7 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
             if (more) run.load_k(page, h, token);
             bool all = was_token + S::TOKENS <= was_n - a.T + 1;
 #pragma unroll
-            for (int u = 0; u < U; ++u) all = all && was_page[u] >= 0;
+            for (int u = 0; u < PAGES; ++u) all = all && was_page[u] >= 0;
             if (all) {
                 run.template soften<true>(s, ke, ve, was_page, was_token, seen);
             } else {
@@ -757,7 +798,7 @@ Plan plan_of(int rows, int D) {
     return p;
 }
 
-template <int F, int D, int NT>
+template <int F, int D, int NT, bool ONE>
 int launch(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
     using S = Shape<F, D, NT>;
     const int smem = S::SMEM + (a.B + 1) * 4;
@@ -766,20 +807,26 @@ int launch(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && set_for != dev) {
         // (the most it is ever launched with)
-        e = cudaFuncSetAttribute(attend_kernel<F, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM + 4097 * 4);
+        e = cudaFuncSetAttribute(attend_kernel<F, D, NT, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM + 4097 * 4);
         if (e == cudaSuccess) set_for = dev;
     }
     if (e != cudaSuccess) return cuda_status(e, "paged_attention");
-    launch_chained(attend_kernel<F, D, NT>, dim3(p.ctas), dim3(32 * S::WARPS), smem, st, a);
+    launch_chained(attend_kernel<F, D, NT, ONE>, dim3(p.ctas), dim3(32 * S::WARPS), smem, st, a);
     const int rc = cuda_status(cudaGetLastError(), "paged_attention launch");
     if (rc != AKV_OK || !joined || p.ctas == 1) return rc;
     launch_chained(join_kernel<D, NT, S::WARPS>, dim3(p.ctas - 1), dim3(256), (a.B + 1) * 4, st, a, p.ctas);
     return cuda_status(cudaGetLastError(), "paged_attention join launch");
 }
+template <int F, int D, int NT>
+int launch_pages(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
+    if constexpr (Shape<F, D, NT>::U > 1)
+        if (Shape<F, D, NT>::TOKENS > 1 << a.pool.shift) return launch<F, D, NT, false>(a, p, joined, st);
+    return launch<F, D, NT, true>(a, p, joined, st);
+}
 template <int F>
 int launch_format(const AttendArgs& a, const Plan& p, int D, bool joined, cudaStream_t st) {
-    if (D == 128) return p.nt == 1 ? launch<F, 128, 1>(a, p, joined, st) : launch<F, 128, 2>(a, p, joined, st);
-    return p.nt == 1 ? launch<F, 64, 1>(a, p, joined, st) : launch<F, 64, 2>(a, p, joined, st);
+    if (D == 128) return p.nt == 1 ? launch_pages<F, 128, 1>(a, p, joined, st) : launch_pages<F, 128, 2>(a, p, joined, st);
+    return p.nt == 1 ? launch_pages<F, 64, 1>(a, p, joined, st) : launch_pages<F, 64, 2>(a, p, joined, st);
 }
 
 }  // namespace
@@ -810,6 +857,8 @@ int akv_paged_attention(const akv_pool* pool, const void* q, const void* pages, 
     const int D = pool->head_dim;
     const Plan p = plan_of(group * tokens, D);
     AKV_REQUIRE(scratch_bytes >= p.bytes, AKV_ERR_SHAPE, "paged_attention: scratch of %lld bytes is too small", scratch_bytes);
+    AKV_REQUIRE((long long)pool->n_pages * pool->n_kv_heads * pool->page_size <= 1ll << 32 && (long long)bsz * width < INT_MAX, AKV_ERR_OVERFLOW,
+                "paged_attention: a pool of more than 2^32 rows");
     const long long most = ((long long)width * pool->page_size + CHUNK - 1) / CHUNK * bsz * pool->n_kv_heads * p.groups;
     AKV_REQUIRE(most < INT_MAX, AKV_ERR_OVERFLOW, "paged_attention: too many chunks of %d tokens", CHUNK);
     a.q = static_cast<const __half*>(q);
