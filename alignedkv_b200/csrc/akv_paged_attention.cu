@@ -5,7 +5,7 @@
 //   s_rj = scale q_r . k_j, o_r = sum_j exp(s_rj - m_r) v_j / l_r, l_r = sum_j exp(s_rj - m_r), over the tokens j that row r sees.
 //
 // Every byte of the tokens is read once: bound by HBM, and for the 4-bit format almost as much by the instructions that unpack it.
-// Work: a unit is up to 16 query rows of one (sequence, KV head), its tokens in chunks of 64.  The chunks of all units in a row are dealt to
+// Work: a unit is up to 16 query rows of one (sequence, KV head), its tokens in chunks of 32.  The chunks of all units in a row are dealt to
 // the warps in equal contiguous runs: lengths are only known on the device, and every SM gets the same whatever they are.  Each CTA
 // adds up the lengths itself.  A warp needs no other one: codes come straight into registers as operand fragments (no shared memory is
 // on their way), the next step's while this one's are multiplied.  Where a run begins or ends inside a unit it leaves a record, and
@@ -19,7 +19,7 @@
 namespace akv {
 namespace {
 
-constexpr int CHUNK = 64;
+constexpr int CHUNK = 32;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // Probabilities enter their product as two halves (what the first leaves out is the second), times 2^15: 22 bits of each, as long as it is above
 // 2^-28 of the largest, of which the 11 bits of one half would show beside the output's own rounding.
@@ -38,12 +38,18 @@ template <int F, int D, int NT>
 struct Shape {
     static constexpr int ROW = row_bytes<F>(D);
     static constexpr int KW = ROW / 8;                        // words of 16 tokens of K (or of V) in a lane
-    static constexpr int U = KW >= 32 ? 1 : KW >= 8 ? 2 : 4;  // 16-token tiles of a step
+    static constexpr int U = ROW == 256 ? 1 : 2;              // 16-token tiles of a step
     static constexpr int TOKENS = 16 * U;
     static constexpr int KS = D / 16;                         // products over the channels; tiles of 16 channels of the output
-    static constexpr int WARPS = NT == 1 ? 12 : 8;
+    static constexpr int SCALES = F == AKV_PAGE_E2M1 ? D : 0; // bytes of a tile's scales (of K or of V)
+    static constexpr int MORE = F == AKV_PAGE_FP16 ? 0 : 2 * SCALES + 32;                  // ... of its scales and exponents
+    // A step in shared memory: a tile's codes of K and of V, the next tile's, then scales of K, of V, exponents of K, of V by tile.
+    static constexpr int STEP = (U * (32 * ROW + MORE) + 127) / 128 * 128;
+    static constexpr int STEPS = ROW >= 128 ? 2 : F == AKV_PAGE_E2M1 && D == 128 ? 3 : F == AKV_PAGE_E4M3 ? 4 : 6;
+    static constexpr int WARPS = 12;
     static constexpr int RECORD = 8 * NT * (D + 4);           // floats: rows of D sums, then the maximum and the sum
-    static constexpr int SMEM = WARPS * 2 * RECORD * 4;
+    static constexpr int RING = STEPS * STEP, SMEM = WARPS * RING;
+    static_assert(RING >= RECORD * 4, "a run's last record lies in its ring");
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -51,35 +57,13 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-// Streamed once: past L1.
-__device__ __forceinline__ uint4 stream16(const uint8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+// 16 bytes global -> shared past L1; with `there` false zeros, and nothing is read.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ uint2 stream8(const uint8_t* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t stream4(const uint8_t* p) {
-    uint32_t v;
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];\n" : "=r"(v) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t load4(const void* p) {
-    uint32_t v;
-    asm volatile("ld.global.nc.u32 %0, [%1];\n" : "=r"(v) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t load2(const void* p) {
-    uint16_t v;
-    asm volatile("ld.global.nc.u16 %0, [%1];\n" : "=h"(v) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t load1(const void* p) {
-    uint32_t v;
-    asm volatile("ld.global.nc.u8 %0, [%1];\n" : "=r"(v) : "l"(p));
+__device__ __forceinline__ int lds8_signed(uint32_t a) {
+    int v;
+    asm volatile("ld.shared.s8 %0, [%1];\n" : "=r"(v) : "r"(a));
     return v;
 }
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -95,8 +79,6 @@ __device__ __forceinline__ uint32_t halves_bits(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ int exponent_byte(uint32_t word, int i) { return (int)(int8_t)((word >> (8 * i)) & 0xFFu); }
-
 // ---------------------------------------------------------------- which chunks are whose
 // cum[b]: chunks of one unit of the sequences before b; a sequence without tokens has one, so that its rows are written.
 __device__ __forceinline__ int chunks_of(int n) { return max(1, (n + CHUNK - 1) / CHUNK); }
@@ -175,35 +157,143 @@ __device__ __forceinline__ long long row_of(const AttendArgs& a, int unit, int r
     return ((long long)b * a.T + t) * (a.pool.H * a.G) + h * a.G + R - t * a.G;
 }
 
-// ---------------------------------------------------------------- a warp's run
-// ONE: a step's tokens are in one page.
+// ---------------------------------------------------------------- a warp's ring
+// Where 16-byte piece c of row r of a tile lies, so that the 8 lanes of a 16-byte load's (16 of an 8-byte load's) phase read different banks: lane
+// (g, t) = (lane / 4, lane % 4) reads pieces by t of K's rows g, and pieces by g of V's rows 2t, 2t + 1.
+template <int ROW>
+__device__ __forceinline__ int piece(int r, int c) {
+    if constexpr (ROW >= 128) return r * ROW + ((c ^ (r & 7)) << 4);
+    const int line = r * ROW >> 7, slot = ((r * ROW & 127) >> 4) + c;
+    return line * 128 + ((slot ^ (2 * (line & (ROW == 64 ? 3 : 1)))) << 4);
+}
+
+// Steps of a run, copied to shared memory STEPS - 1 ahead by the warp's own asynchronous copies.  ONE: a step's tokens are in one page.
 template <int F, int D, int NT, bool ONE>
-struct Run {
+struct Ring {
     using S = Shape<F, D, NT>;
-    static constexpr int U = S::U, KW = S::KW, KS = S::KS, PAGES = ONE ? 1 : U;
+    static constexpr int U = S::U, ROW = S::ROW, PAGES = ONE ? 1 : U;
+    const AttendArgs& a;
+    const int* cum;
+    uint32_t base, mine;                 // of the ring; where this lane's first piece of codes goes within a tile
+    const uint8_t* more;                 // this lane's piece of scales or exponents: its tensor, bytes of a token there
+    int per_token, lane, put, get;
+    Part part;                           // what is copied next
+    int units, end, at, n, h, token, stop, page[PAGES];
+    uint32_t gone;                       // PAGES bits a step, the oldest in the lowest: the page is not there
+
+    __device__ __forceinline__ Ring(const AttendArgs& args, const int* lengths, uint32_t to, int of_lane, int run_units, int first, int last)
+        : a(args), cum(lengths), base(to), lane(of_lane), put(0), get(0), units(run_units), end(last), at(first), gone(0) {
+        const int bytes = lane * 16;
+        mine = piece<ROW>(bytes / ROW, bytes % ROW / 16);
+        more = nullptr;
+        per_token = 0;
+        if constexpr (F != AKV_PAGE_FP16) {
+            constexpr int N = S::SCALES / 16;                 // pieces of a tile's scales
+            if (lane < 2 * N) {
+                more = (lane < N ? a.pool.ks : a.pool.vs) + lane % (N ? N : 1) * 16;
+                per_token = D / 16;
+            } else if (lane < 2 * N + 2) {
+                more = reinterpret_cast<const uint8_t*>(lane == 2 * N ? a.pool.ke : a.pool.ve);
+                per_token = 1;
+            }
+        }
+        part.find(cum, units, sequence_with(cum, a.B, units, at), at, end);
+        enter();
+        look();
+#pragma unroll 1
+        for (int i = 0; i < S::STEPS - 1; ++i) fill();
+    }
+    __device__ __forceinline__ void enter() {
+        n = length_of(a.pool, part.b);
+        h = part.unit / a.groups % a.pool.H;
+        token = part.first * CHUNK;
+        stop = min(n, part.last * CHUNK);
+    }
+    // Pages of the step at `token`; -1 where there is none or nothing of the sequence in it.
+    __device__ __forceinline__ void look() {
+#pragma unroll
+        for (int u = 0; u < PAGES; ++u) {
+            page[u] = -1;
+            if (token + 16 * u < n) page[u] = __ldg(a.pool.table + (unsigned)part.b * (unsigned)a.pool.width + ((token + 16 * u) >> a.pool.shift));
+        }
+    }
+    // The next step, if there is one; always a group, so that the groups count the steps.
+    __device__ __forceinline__ void fill() {
+        if (at < end) {
+            const uint32_t to = base + put * S::STEP;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int x = page[ONE ? 0 : u], from = ONE ? token : token + 16 * u;
+                const bool there = (unsigned)x < (unsigned)a.pool.n_pages;
+                const unsigned row = (((unsigned)(there ? x : 0) * (unsigned)a.pool.H + h) << a.pool.shift) + (from & ((1 << a.pool.shift) - 1)) + (ONE ? 16 * u : 0);
+                const unsigned long long byte = (unsigned long long)row * ROW + lane * 16;
+                const uint8_t *k = a.pool.kc + byte, *v = a.pool.vc + byte;
+                const uint32_t tile = to + u * 32 * ROW;
+#pragma unroll
+                for (int j = 0; j < ROW / 32; ++j) {
+                    // (512 bytes further: 2, 4, 8 or 16 rows)
+                    const uint32_t dst = tile + (ROW >= 128 ? (mine ^ ((j * (512 / ROW) & 7) << 4)) : mine) + j * 512;
+                    copy16(dst, k + j * 512, there);
+                    copy16(dst + 16 * ROW, v + j * 512, there);
+                }
+                if constexpr (F != AKV_PAGE_FP16)
+                    if (per_token) copy16(to + U * 32 * ROW + u * S::MORE + lane * 16, more + (unsigned long long)row * per_token, there);
+            }
+            uint32_t bits = 0;
+#pragma unroll
+            for (int u = 0; u < PAGES; ++u) bits |= (unsigned)((unsigned)page[u] >= (unsigned)a.pool.n_pages) << u;
+            gone |= bits << ((put >= get ? put - get : put - get + S::STEPS) * PAGES);
+            token += S::TOKENS;
+            if (token >= stop) {
+                at += part.last - part.first;
+                if (at < end) {
+                    part.find(cum, units, part.b, at, end);
+                    enter();
+                }
+            }
+            if (at < end) look();
+        }
+        cp_async_commit();
+        put = put + 1 == S::STEPS ? 0 : put + 1;
+    }
+    // Waits for the step that is read next, requests the one whose place the last read has left; pages that are not there.
+    __device__ __forceinline__ uint32_t take(uint32_t& without) {
+        cp_async_wait<S::STEPS - 2>();
+        __syncwarp();
+        fill();
+        const uint32_t from = base + get * S::STEP;
+        without = gone & ((1u << PAGES) - 1);
+        gone >>= PAGES;
+        get = get + 1 == S::STEPS ? 0 : get + 1;
+        return from;
+    }
+};
+
+// ---------------------------------------------------------------- a warp's unit
+template <int F, int D, int NT, bool ONE>
+struct Unit {
+    using S = Shape<F, D, NT>;
+    static constexpr int U = S::U, KW = S::KW, KS = S::KS, ROW = S::ROW;
     const AttendArgs& a;
     int g, t;
+    uint32_t at_k, at_v;                 // of this lane's first piece within a tile
     uint32_t q[KS][NT][2];
     float acc[KS][NT][4], m[NT][2], l[NT][2];
-    uint32_t k[U][KW], v[U][KW], ke[U], ve[U], ks[U][2], vs[U][4];
 
-    __device__ __forceinline__ Run(const AttendArgs& args, int lane) : a(args), g(lane >> 2), t(lane & 3) {}
-
-    // Token of k index i of a tile's row: rows g and g + 8 of K, k = 2t, 2t + 1, 2t + 8, 2t + 9 of V: a lane's four of V lie side by side.
-    __device__ __forceinline__ int k_token(int half) const { return 4 * (g >> 1) + (g & 1) + 2 * half; }
+    __device__ __forceinline__ Unit(const AttendArgs& args, int lane) : a(args), g(lane >> 2), t(lane & 3) {
+        at_k = ROW >= 128 ? piece<ROW>(g, 2 * t) : ROW == 64 ? piece<ROW>(g, t) : piece<ROW>(g, t >> 1) + (t & 1) * 8;
+        at_v = 16 * ROW + (ROW >= 128 ? piece<ROW>(2 * t, g) : ROW == 64 ? piece<ROW>(2 * t, g >> 1) + (g & 1) * 8 : piece<ROW>(2 * t, g >> 2) + (g & 3) * 4);
+    }
 
     // Channels of the first operand's k = 2t, 2t + 1, 2t + 8, 2t + 9 in product s: this one and the next three.
     __device__ __forceinline__ int k_channel(int s) const {
-        if constexpr (F == AKV_PAGE_FP16) return (s >> 1) * 32 + t * 8 + (s & 1) * 4;
-        else if constexpr (F == AKV_PAGE_E4M3) return (s >> 2) * 64 + t * 16 + (s & 3) * 4;
-        else return t * (D / 4) + s * 4;
+        if constexpr (ROW == 256) return (s >> 2) * 64 + t * 16 + (s & 3) * 4;
+        return t * (D / 4) + s * 4;
     }
-    // Channel of rows g (half 0) and g + 8 (half 1) of output tile i.
-    __device__ __forceinline__ int v_channel(int i, int half) const {
-        if constexpr (F == AKV_PAGE_FP16) return (i >> 2) * 64 + g * 8 + (i & 3) * 2 + half;
-        else if constexpr (F == AKV_PAGE_E4M3) return g * (D / 8) + 2 * i + half;
-        // (8 channels of a word: even ones of the two halves first)
-        else return g * (D / 8) + (i >> 2) * 8 + 2 * (i & 3) + half;
+    // Channel of row g of output tile i; that of row g + 8 is the next.
+    __device__ __forceinline__ int v_channel(int i) const {
+        if constexpr (ROW == 256) return (i >> 2) * 64 + g * 8 + (i & 3) * 2;
+        return g * (D / 8) + 2 * i;
     }
 
     __device__ __forceinline__ void begin(int unit) {
@@ -225,132 +315,56 @@ struct Run {
         }
     }
 
-    // Pages of a step's tiles; -1 where there is none or nothing of the sequence in it.
-    __device__ __forceinline__ void look(int (&page)[PAGES], int b, int at, int n) const {
-#pragma unroll
-        for (int u = 0; u < PAGES; ++u) {
-            page[u] = -1;
-            if (at + 16 * u < n) {
-                const int x = __ldg(a.pool.table + (unsigned)b * (unsigned)a.pool.width + ((at + 16 * u) >> a.pool.shift));
-                if ((unsigned)x < (unsigned)a.pool.n_pages) page[u] = x;
-            }
-        }
-    }
-    static __device__ __forceinline__ bool missing(const int (&page)[PAGES], int u) { return page[ONE ? 0 : u] < 0; }
-    // First row of the pool of a tile (of some page where there is none: what is read from it is not used).
-    __device__ __forceinline__ unsigned tile_row(const int (&page)[PAGES], int u, int h, int at) const {
-        const int from = ONE ? at : at + 16 * u;
-        return (((unsigned)max(page[ONE ? 0 : u], 0) * (unsigned)a.pool.H + h) << a.pool.shift) + (from & ((1 << a.pool.shift) - 1)) + (ONE ? 16 * u : 0);
-    }
-    // (Addresses are a tensor's, the step's row's and the lane's; tiles and tokens are constants behind them.)
-    static __device__ __forceinline__ const uint8_t* place(const void* base, unsigned row, int size, int mine) {
-        return static_cast<const uint8_t*>(base) + (unsigned long long)row * size + mine;
-    }
-    __device__ __forceinline__ void load_k(const int (&page)[PAGES], int h, int at) {
-        constexpr int PIECE = S::ROW >= 64 ? 16 : 8;
-        const uint8_t *p = nullptr, *pe = nullptr, *pv = nullptr, *ps = nullptr;
+    // Scores of a step's tokens, s[u][nt]: rows g (first two) and g + 8 by query rows 2t, 2t + 1.
+    __device__ __forceinline__ void scores(float (&s)[U][NT][4], uint32_t step) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (!ONE || u == 0) {
-                const unsigned row = tile_row(page, u, h, at);
-                p = place(a.pool.kc, row, S::ROW, k_token(0) * S::ROW + t * PIECE);
-                if constexpr (F != AKV_PAGE_FP16) {
-                    pe = place(a.pool.ke, row, 1, 4 * (g >> 1));
-                    pv = place(a.pool.ve, row, 1, 4 * (g >> 1));
-                }
-                if constexpr (F == AKV_PAGE_E2M1) ps = place(a.pool.ks, row, D / 16, k_token(0) * (D / 16) + t * (D / 64));
-            }
-            const int tile = ONE ? 16 * u : 0;
+            const uint32_t from = step + u * 32 * ROW + at_k;
+            constexpr int H = KW / 2;
+            uint32_t k[2][H];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const uint8_t* x = p + (tile + 2 * half) * S::ROW;
-                if constexpr (S::ROW >= 64) {
-#pragma unroll
-                    for (int c = 0; c < S::ROW / 64; ++c) {
-                        const uint4 w = stream16(x + c * 64);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) k[u][half * (KW / 2) + 4 * c + i] = u4w(w, i);
-                    }
+                if constexpr (ROW == 32) {
+                    const uint2 w = lds64(from + half * 8 * ROW);
+                    k[half][0] = w.x;
+                    k[half][1] = w.y;
                 } else {
-                    const uint2 w = stream8(x);
-                    k[u][half * 2] = w.x;
-                    k[u][half * 2 + 1] = w.y;
-                }
-                if constexpr (F == AKV_PAGE_E2M1) {
-                    const uint8_t* y = ps + (tile + 2 * half) * (D / 16);
-                    ks[u][half] = D == 128 ? load2(y) : load1(y);
-                }
-            }
-            if constexpr (F != AKV_PAGE_FP16) {
-                ke[u] = load4(pe + tile);
-                ve[u] = load4(pv + tile);
-            }
-        }
-    }
-    __device__ __forceinline__ void load_v(const int (&page)[PAGES], int h, int at) {
-        constexpr int PIECE = S::ROW >= 128 ? 16 : S::ROW / 8;
-        const uint8_t *p = nullptr, *ps = nullptr;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (!ONE || u == 0) {
-                const unsigned row = tile_row(page, u, h, at);
-                p = place(a.pool.vc, row, S::ROW, 4 * t * S::ROW + g * PIECE);
-                if constexpr (F == AKV_PAGE_E2M1) ps = place(a.pool.vs, row, D / 16, 4 * t * (D / 16) + (D == 128 ? g : g >> 1));
-            }
-            const int tile = ONE ? 16 * u : 0;
+                    for (int c = 0; c < H / 4; ++c) {
+                        const uint4 w = lds128((from ^ ((c & 1) << 4)) + half * 8 * ROW + (c >> 1) * 128);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint8_t* x = p + (tile + i) * S::ROW;
-                if constexpr (S::ROW >= 128) {
-#pragma unroll
-                    for (int c = 0; c < S::ROW / 128; ++c) {
-                        const uint4 w = stream16(x + c * 128);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) v[u][i * (KW / 4) + 4 * c + j] = u4w(w, j);
+                        for (int i = 0; i < 4; ++i) k[half][4 * c + i] = u4w(w, i);
                     }
-                } else if constexpr (S::ROW == 64) {
-                    const uint2 w = stream8(x);
-                    v[u][i * 2] = w.x;
-                    v[u][i * 2 + 1] = w.y;
-                } else {
-                    v[u][i] = stream4(x);
                 }
-                if constexpr (F == AKV_PAGE_E2M1) vs[u][i] = load1(ps + (tile + i) * (D / 16));
             }
-        }
-    }
-
-    // Scores of a step's tokens, s[u][nt]: rows k_token(0) (first two) and k_token(1) by query rows 2t, 2t + 1.
-    __device__ __forceinline__ void scores(float (&s)[U][NT][4]) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = 0.f;
-            constexpr int H = KW / 2;
             if constexpr (F == AKV_PAGE_FP16) {
 #pragma unroll
                 for (int i = 0; i < KS; ++i)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
-                        mma(s[u][nt], k[u][2 * i], k[u][H + 2 * i], k[u][2 * i + 1], k[u][H + 2 * i + 1], q[i][nt][0], q[i][nt][1]);
+                        mma(s[u][nt], k[0][2 * i], k[1][2 * i], k[0][2 * i + 1], k[1][2 * i + 1], q[i][nt][0], q[i][nt][1]);
             } else if constexpr (F == AKV_PAGE_E4M3) {
 #pragma unroll
                 for (int i = 0; i < KS; ++i) {
                     uint32_t x[2], y[2];
-                    e4m3_word(x, k[u][i]);
-                    e4m3_word(y, k[u][H + i]);
+                    e4m3_word(x, k[0][i]);
+                    e4m3_word(y, k[1][i]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma(s[u][nt], x[0], y[0], x[1], y[1], q[i][nt][0], q[i][nt][1]);
                 }
             } else {
-                const uint32_t s0 = e4m3_halves(ks[u][0]), s1 = e4m3_halves(ks[u][1]);
+                const uint32_t scales = step + U * 32 * ROW + u * S::MORE + g * (D / 16) + t * (D / 64);
+                const uint32_t s0 = e4m3_halves(D == 128 ? lds16(scales) : lds8(scales));
+                const uint32_t s1 = e4m3_halves(D == 128 ? lds16(scales + D / 2) : lds8(scales + D / 2));
 #pragma unroll
                 for (int w = 0; w < H; ++w) {
                     // (8 channels of a word: two products; 16 have a scale)
                     const uint32_t f0 = __byte_perm(s0, s0, D == 128 && w >= 2 ? 0x3232 : 0x1010), f1 = __byte_perm(s1, s1, D == 128 && w >= 2 ? 0x3232 : 0x1010);
                     uint32_t x[4], y[4];
-                    e2m1_word(x, k[u][w]);
-                    e2m1_word(y, k[u][H + w]);
+                    e2m1_word(x, k[0][w]);
+                    e2m1_word(y, k[1][w]);
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -362,12 +376,11 @@ struct Run {
         }
     }
 
-    // Scores to weights of the values, in place, and the running maximum and sum with them.  seen(nt, c): tokens below it are seen by the row; page:
-    // -1 where the tile's tokens are not there.  ALL: every row sees the whole step.  (An exponent of -128 comes out as a factor of
+    // Scores to weights of the values, in place, and the running maximum and sum with them.  seen(nt, c): tokens below it are seen by the row;
+    // without: bits of the pages that are not there.  ALL: every row sees the whole step.  (An exponent of -128 comes out as a factor of
     // -infinity: times the row's zeros NaN, as it should.)
     template <bool ALL>
-    __device__ __forceinline__ void soften(float (&s)[U][NT][4], const uint32_t (&ke)[U], const uint32_t (&ve)[U], const int (&page)[PAGES], int at,
-                                           const int (&seen)[NT][2]) {
+    __device__ __forceinline__ void soften(float (&s)[U][NT][4], uint32_t step, uint32_t without, int at, const int (&seen)[NT][2]) {
         float top[NT][2], f[U][2], unit[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -377,8 +390,9 @@ struct Run {
                 f[u][half] = a.scale2;
                 unit[u][half] = LIFT;
                 if constexpr (F != AKV_PAGE_FP16) {
-                    const int i = (g & 1) + 2 * half, x = exponent_byte(ve[u], i);
-                    f[u][half] = a.scale2 * __int_as_float((exponent_byte(ke[u], i) + 127) << 23);
+                    const uint32_t from = step + U * 32 * ROW + u * S::MORE + 2 * S::SCALES + g + 8 * half;
+                    const int x = lds8_signed(from + 16);
+                    f[u][half] = a.scale2 * __int_as_float((lds8_signed(from) + 127) << 23);
                     unit[u][half] = __int_as_float((x + 127 + 15) << 23);
                     if (x == EXP_NAN) unit[u][half] = NAN;
                     e = (float)max(x, -40);           // (a row of NaN has no exponent; -35 is the least there is)
@@ -390,7 +404,7 @@ struct Run {
                         float& x = s[u][nt][2 * half + c];
                         if (!ALL) {
                             x *= f[u][half];
-                            if (missing(page, u) || at + 16 * u + k_token(half) >= seen[nt][c]) x = -INFINITY;
+                            if (missing(without, u) || at + 16 * u + g + 8 * half >= seen[nt][c]) x = -INFINITY;
                         }
                         const float y = ALL ? fmaf(x, f[u][half], e) : x + e;
                         top[nt][c] = u == 0 && half == 0 ? y : fmaxf(top[nt][c], y);
@@ -435,7 +449,7 @@ struct Run {
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         float& x = s[u][nt][2 * half + c];
-                        const bool gone = !ALL && (missing(page, u) || at + 16 * u + k_token(half) >= seen[nt][c]);
+                        const bool gone = !ALL && (missing(without, u) || at + 16 * u + g + 8 * half >= seen[nt][c]);
                         const float p = ex2(ALL ? fmaf(x, f[u][half], -base) : x - base);
                         l[nt][c] += p;                              // (of what is not seen: 0)
                         x = gone ? 0.f : p * unit[u][half];
@@ -443,46 +457,75 @@ struct Run {
             }
     }
 
-    // Values of a step that lie behind the sequence, or nowhere: zeros, whatever is there.
-    __device__ __forceinline__ void clear_v(const int (&page)[PAGES], int at, int n) {
+    static __device__ __forceinline__ bool missing(uint32_t without, int u) { return (without >> (ONE ? 0 : u)) & 1; }
+
+    // A tile's values: tokens 2t, 2t + 1, 2t + 8, 2t + 9; zeros for those that lie behind the sequence (limit: tokens of the tile that do not),
+    // whatever is there.
+    __device__ __forceinline__ void load_v(uint32_t (&v)[KW], uint32_t (&scale)[2], uint32_t step, int u, int limit) {
+        constexpr int W = KW / 4;
+        const uint32_t from = step + u * 32 * ROW + at_v;
+        uint32_t bytes[4];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t x = (ROW >= 128 ? (from ^ ((i & 1) << 4)) + (i & 1) * ROW : from ^ ((i & 1) * ROW)) + (i >> 1) * 8 * ROW;
+            if constexpr (ROW >= 128) {
+#pragma unroll
+                for (int c = 0; c < W / 4; ++c) {
+                    const uint4 w = lds128(x + c * 128);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[i * W + 4 * c + j] = u4w(w, j);
+                }
+            } else if constexpr (ROW == 64) {
+                const uint2 w = lds64(x);
+                v[i * W] = w.x;
+                v[i * W + 1] = w.y;
+            } else {
+                v[i] = lds32(x);
+            }
+            bytes[i] = 0;
+            if constexpr (F == AKV_PAGE_E2M1)
+                bytes[i] = lds8(step + U * 32 * ROW + u * S::MORE + S::SCALES + (2 * t + (i & 1) + (i >> 1) * 8) * (D / 16) + (D == 128 ? g : g >> 1));
+        }
+        if (limit < 16) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (missing(page, u) || at + 16 * u + 4 * t + i >= n) {
+                if (2 * t + (i & 1) + (i >> 1) * 8 >= limit) {
+                    bytes[i] = 0;
 #pragma unroll
-                    for (int j = 0; j < KW / 4; ++j) v[u][i * (KW / 4) + j] = 0;
-                    if constexpr (F == AKV_PAGE_E2M1) vs[u][i] = 0;
+                    for (int j = 0; j < W; ++j) v[i * W + j] = 0;
                 }
+        }
+        if constexpr (F == AKV_PAGE_E2M1) {
+            scale[0] = e4m3_halves(__byte_perm(bytes[0], bytes[1], 0x0040));
+            scale[1] = e4m3_halves(__byte_perm(bytes[2], bytes[3], 0x0040));
+        }
     }
-
-    // fn(i, a0, a1, a2, a3): the first operand of output tile i, of the values of tile u.
+    // fn(i, a0, a1, a2, a3): the first operand of output tile i.
     template <class Fn>
-    __device__ __forceinline__ void tiles(int u, Fn fn) {
+    __device__ __forceinline__ void tiles(const uint32_t (&v)[KW], const uint32_t (&scale)[2], Fn fn) {
         constexpr int W = KW / 4;              // words of a token
         if constexpr (F == AKV_PAGE_FP16) {
 #pragma unroll
             for (int i = 0; i < KS; ++i)
-                fn(i, __byte_perm(v[u][i], v[u][W + i], 0x5410), __byte_perm(v[u][i], v[u][W + i], 0x7632),
-                   __byte_perm(v[u][2 * W + i], v[u][3 * W + i], 0x5410), __byte_perm(v[u][2 * W + i], v[u][3 * W + i], 0x7632));
+                fn(i, __byte_perm(v[i], v[W + i], 0x5410), __byte_perm(v[i], v[W + i], 0x7632),
+                   __byte_perm(v[2 * W + i], v[3 * W + i], 0x5410), __byte_perm(v[2 * W + i], v[3 * W + i], 0x7632));
         } else if constexpr (F == AKV_PAGE_E4M3) {
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
-                const uint32_t x = __byte_perm(v[u][i >> 1], v[u][W + (i >> 1)], i & 1 ? 0x7362 : 0x5140);
-                const uint32_t y = __byte_perm(v[u][2 * W + (i >> 1)], v[u][3 * W + (i >> 1)], i & 1 ? 0x7362 : 0x5140);
+                const uint32_t x = __byte_perm(v[i >> 1], v[W + (i >> 1)], i & 1 ? 0x7362 : 0x5140);
+                const uint32_t y = __byte_perm(v[2 * W + (i >> 1)], v[3 * W + (i >> 1)], i & 1 ? 0x7362 : 0x5140);
                 uint32_t p[2], r[2];
                 e4m3_word(p, x);
                 e4m3_word(r, y);
                 fn(i, p[0], p[1], r[0], r[1]);
             }
         } else {
-            const uint32_t s0 = e4m3_halves(__byte_perm(vs[u][0], vs[u][1], 0x0040)), s1 = e4m3_halves(__byte_perm(vs[u][2], vs[u][3], 0x0040));
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 constexpr uint32_t LOW = 0x0F0F0F0Fu;
                 // two tokens' nibbles of one channel in a byte: even channels, odd ones
-                const uint32_t e0 = (v[u][w] & LOW) | ((v[u][W + w] << 4) & ~LOW), o0 = ((v[u][w] >> 4) & LOW) | (v[u][W + w] & ~LOW);
-                const uint32_t e1 = (v[u][2 * W + w] & LOW) | ((v[u][3 * W + w] << 4) & ~LOW), o1 = ((v[u][2 * W + w] >> 4) & LOW) | (v[u][3 * W + w] & ~LOW);
+                const uint32_t e0 = (v[w] & LOW) | ((v[W + w] << 4) & ~LOW), o0 = ((v[w] >> 4) & LOW) | (v[W + w] & ~LOW);
+                const uint32_t e1 = (v[2 * W + w] & LOW) | ((v[3 * W + w] << 4) & ~LOW), o1 = ((v[2 * W + w] >> 4) & LOW) | (v[3 * W + w] & ~LOW);
                 uint32_t x0[4], y0[4], x1[4], y1[4];
                 e2m1_word(x0, e0);
                 e2m1_word(y0, o0);
@@ -490,16 +533,22 @@ struct Run {
                 e2m1_word(y1, o1);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    fn(4 * w + i, hmul2_bits(x0[i], s0), hmul2_bits(y0[i], s0), hmul2_bits(x1[i], s1), hmul2_bits(y1[i], s1));
+                    fn(4 * w + i, hmul2_bits(x0[i], scale[0]), hmul2_bits(y0[i], scale[0]), hmul2_bits(x1[i], scale[1]), hmul2_bits(y1[i], scale[1]));
             }
         }
     }
-    __device__ __forceinline__ void add_values(const float (&s)[U][NT][4]) {
+    // limit: tokens of the step that are the sequence's.
+    __device__ __forceinline__ void add_values(const float (&s)[U][NT][4], uint32_t step, int at, int limit, const int (&seen)[NT][2]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            uint32_t hi[NT][2], lo[NT][2];
+            uint32_t v[KW], scale[2], hi[NT][2], lo[NT][2];
+            load_v(v, scale, step, u, limit - 16 * u);
             second_operand(s[u], hi, lo);
-            tiles(u, [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+            if (F == AKV_PAGE_FP16 && __any_sync(0xFFFFFFFFu, odd(v))) {
+                add_odd_values(v, hi, lo, at + 16 * u, at + limit, seen);
+                continue;
+            }
+            tiles(v, scale, [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     mma(acc[i][nt], a0, a1, a2, a3, hi[nt][0], hi[nt][1]);
@@ -522,41 +571,36 @@ struct Run {
     }
     // The same where some values are not finite (fp16 pages alone: elsewhere codes are).  0 * inf would be NaN: every query's product is formed by
     // itself, without the newest tokens that it does not see, and the second halves' without what is not finite.
-    __device__ __forceinline__ void add_odd_values(const float (&s)[U][NT][4], int at, int n, const int (&seen)[NT][2]) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            uint32_t hi[NT][2], lo[NT][2];
-            second_operand(s[u], hi, lo);
+    __device__ __forceinline__ void add_odd_values(const uint32_t (&v)[KW], const uint32_t (&hi)[NT][2], const uint32_t (&lo)[NT][2], int at, int n,
+                                                   const int (&seen)[NT][2]) {
+        const uint32_t none[2] = {0, 0};
 #pragma unroll 1
-            for (int limit = n - a.T + 1; limit <= n; ++limit) {
-                bool there[4];
+        for (int limit = n - a.T + 1; limit <= n; ++limit) {
+            bool there[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) there[i] = at + 16 * u + 4 * t + i < limit;
-                const uint32_t m01 = (there[0] ? 0xFFFFu : 0u) | (there[1] ? 0xFFFF0000u : 0u), m23 = (there[2] ? 0xFFFFu : 0u) | (there[3] ? 0xFFFF0000u : 0u);
-                tiles(u, [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+            for (int i = 0; i < 4; ++i) there[i] = at + 2 * t + (i & 1) + (i >> 1) * 8 < limit;
+            const uint32_t m01 = (there[0] ? 0xFFFFu : 0u) | (there[1] ? 0xFFFF0000u : 0u), m23 = (there[2] ? 0xFFFFu : 0u) | (there[3] ? 0xFFFF0000u : 0u);
+            tiles(v, none, [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float c[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma(c, a0 & m01, a1 & m01, a2 & m23, a3 & m23, hi[nt][0], hi[nt][1]);
-                        mma(c, finite(a0 & m01), finite(a1 & m01), finite(a2 & m23), finite(a3 & m23), lo[nt][0], lo[nt][1]);
+                for (int nt = 0; nt < NT; ++nt) {
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma(c, a0 & m01, a1 & m01, a2 & m23, a3 & m23, hi[nt][0], hi[nt][1]);
+                    mma(c, finite(a0 & m01), finite(a1 & m01), finite(a2 & m23), finite(a3 & m23), lo[nt][0], lo[nt][1]);
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            if (seen[nt][x & 1] == limit) acc[i][nt][x] += c[x];
-                    }
-                });
-            }
+                    for (int x = 0; x < 4; ++x)
+                        if (seen[nt][x & 1] == limit) acc[i][nt][x] += c[x];
+                }
+            });
         }
     }
     static __device__ __forceinline__ uint32_t finite(uint32_t w) {
         if ((w & 0x7C00u) == 0x7C00u) w &= 0xFFFF0000u;
         return (w & 0x7C000000u) == 0x7C000000u ? w & 0xFFFFu : w;
     }
-    __device__ __forceinline__ bool odd_values() const {
+    static __device__ __forceinline__ bool odd(const uint32_t (&v)[KW]) {
         uint32_t x[2] = {0, 0};                  // (0 as long as all are finite, then NaN)
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < KW; ++i) x[i & 1] = hfma2_bits(v[u][i], 0, x[i & 1]);
+        for (int i = 0; i < KW; ++i) x[i & 1] = hfma2_bits(v[i], 0, x[i & 1]);
         return finite(x[0]) != x[0] || finite(x[1]) != x[1];
     }
 
@@ -581,7 +625,7 @@ struct Run {
 #pragma unroll
                 for (int i = 0; i < KS; ++i) {
                     const __half2 h = __floats2half2_rn(acc[i][nt][c] * inv, acc[i][nt][2 + c] * inv);
-                    *reinterpret_cast<__half2*>(a.out + row * D + v_channel(i, 0)) = h;
+                    *reinterpret_cast<__half2*>(a.out + row * D + v_channel(i)) = h;
                 }
                 if (a.lse && g == 0) a.lse[row] = l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + log2f(l[nt][c])) * LN2;
             }
@@ -595,18 +639,21 @@ struct Run {
                 float* row = to + (8 * nt + 2 * t + c) * (D + 4);
 #pragma unroll
                 for (int i = 0; i < KS; ++i)
-                    *reinterpret_cast<float2*>(row + v_channel(i, 0)) = make_float2(acc[i][nt][c], acc[i][nt][2 + c]);
+                    *reinterpret_cast<float2*>(row + v_channel(i)) = make_float2(acc[i][nt][c], acc[i][nt][2 + c]);
                 if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[nt][c], l[nt][c]);
             }
     }
 };
 
-// Joins rows of `count` records (lane: D / 32 channels): fn(i) = row of the i-th.  Then to a record, or to out and lse.
+// Joins rows of `count` records (lane: D / 32 channels): fn(i) = row of the i-th, or null.  Then to a record, or to out and lse.
 template <int D, class Fn>
 __device__ __forceinline__ void join_row(const AttendArgs& a, int unit, int r, int count, int lane, Fn fn, float* record) {
     constexpr int N = D / 32;
     float top = -INFINITY;
-    for (int i = 0; i < count; ++i) top = fmaxf(top, fn(i)[D]);
+    for (int i = lane; i < count; i += 32)
+        if (const float* x = fn(i)) top = fmaxf(top, x[D]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     const float base = top == -INFINITY ? 0.f : top;
     float o[N], sum = 0.f;
 #pragma unroll
@@ -614,6 +661,7 @@ __device__ __forceinline__ void join_row(const AttendArgs& a, int unit, int r, i
 #pragma unroll 4
     for (int i = 0; i < count; ++i) {
         const float* x = fn(i);
+        if (!x) continue;
         const float f = ex2(x[D] - base);
         sum = fmaf(f, x[D + 1], sum);
 #pragma unroll
@@ -641,10 +689,10 @@ __device__ __forceinline__ void join_row(const AttendArgs& a, int unit, int r, i
 template <int F, int D, int NT, bool ONE>
 __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(AttendArgs a) {
     using S = Shape<F, D, NT>;
-    constexpr int WARPS = S::WARPS, U = S::U, PAGES = ONE ? 1 : U;
-    extern __shared__ __align__(16) float records[];           // [warp][2][rows][D + 4]: of a run's first part and of its last
-    int* cum = reinterpret_cast<int*>(records + WARPS * 2 * S::RECORD);
-    __shared__ int sums[WARPS], s_unit[2 * WARPS];             // (s_unit: unit of each record, -1 where there is none)
+    constexpr int WARPS = S::WARPS;
+    extern __shared__ __align__(128) uint8_t rings[];
+    int* cum = reinterpret_cast<int*>(rings + S::SMEM);
+    __shared__ int sums[WARPS], s_unit[2 * WARPS];             // (s_unit: units of the records of each run's first part and of its last, or -1)
     pdl_turn();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     add_lengths<32 * WARPS>(a, cum, sums);
@@ -658,80 +706,53 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
     }
     if (lane < 2) s_unit[2 * warp + lane] = -1;
     __syncwarp();
+    // Records: of a part that ends its run in the run's ring, which nobody needs any more; of one in front of others in global memory.
+    float* last_record = reinterpret_cast<float*>(rings + warp * S::RING);
+    float* first_record = a.part + (2ll * gridDim.x + blockIdx.x * WARPS + warp) * S::RECORD;
     if (at < end) {
-        Run<F, D, NT, ONE> run(a, lane);
+        Ring<F, D, NT, ONE> ring(a, cum, smem_u32(last_record), lane, units, at, end);
+        Unit<F, D, NT, ONE> unit(a, lane);
         Part part;
+        part.b = ring.part.b;                                  // (or a later one: found from the run's beginning)
         part.find(cum, units, sequence_with(cum, a.B, units, at), at, end);
-        int n = length_of(a.pool, part.b), h = part.unit / a.groups % a.pool.H;
-        int token = part.first * CHUNK, stop = min(n, part.last * CHUNK), page[PAGES];
-        run.look(page, part.b, token, n);
-        run.load_k(page, h, token);
-        run.load_v(page, h, token);
-        int seen[NT][2];
-        bool fresh = true;
         for (;;) {
-            if (fresh) {
-                run.begin(part.unit);
+            const int n = length_of(a.pool, part.b), stop = min(n, part.last * CHUNK);
+            int seen[NT][2];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        int query;
-                        seen[nt][c] = row_of(a, part.unit, 8 * nt + 2 * run.t + c, &query) < 0 ? 0 : n - a.T + 1 + query;
-                    }
-            }
-            // the step behind this one: the unit's next, or the first of the next unit
-            const Part was = part;
-            const int was_token = token, was_n = n;
-            int was_page[PAGES];
-#pragma unroll
-            for (int u = 0; u < PAGES; ++u) was_page[u] = page[u];
-            token += S::TOKENS;
-            fresh = token >= stop;
-            if (fresh) {
-                at += part.last - part.first;
-                if (at < end) {
-                    part.find(cum, units, part.b, at, end);
-                    n = length_of(a.pool, part.b);
-                    h = part.unit / a.groups % a.pool.H;
-                    token = part.first * CHUNK;
-                    stop = min(n, part.last * CHUNK);
+                for (int c = 0; c < 2; ++c) {
+                    int query;
+                    seen[nt][c] = row_of(a, part.unit, 8 * nt + 2 * unit.t + c, &query) < 0 ? 0 : n - a.T + 1 + query;
                 }
-            }
-            const bool more = !fresh || at < end;
-            if (more) run.look(page, part.b, token, n);
-            float s[U][NT][4];
-            run.scores(s);
-            uint32_t ke[U], ve[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                ke[u] = run.ke[u];
-                ve[u] = run.ve[u];
-            }
-            if (more) run.load_k(page, h, token);
-            bool all = was_token + S::TOKENS <= was_n - a.T + 1;
-#pragma unroll
-            for (int u = 0; u < PAGES; ++u) all = all && was_page[u] >= 0;
-            if (all) {
-                run.template soften<true>(s, ke, ve, was_page, was_token, seen);
+            unit.begin(part.unit);
+            int token = part.first * CHUNK;
+#pragma unroll 1
+            do {
+                uint32_t without;
+                const uint32_t step = ring.take(without);
+                float s[S::U][NT][4];
+                unit.scores(s, step);
+                if (token + S::TOKENS <= n - a.T + 1 && without == 0) unit.template soften<true>(s, step, without, token, seen);
+                else unit.template soften<false>(s, step, without, token, seen);
+                unit.add_values(s, step, token, n - token, seen);
+                token += S::TOKENS;
+            } while (token < stop);
+            unit.close();
+            at += part.last - part.first;
+            if (part.whole()) {
+                unit.write(part.unit);
             } else {
-                run.template soften<false>(s, ke, ve, was_page, was_token, seen);
-                run.clear_v(was_page, was_token, was_n);
-            }
-            if (F == AKV_PAGE_FP16 && __any_sync(0xFFFFFFFFu, run.odd_values())) run.add_odd_values(s, was_token, was_n, seen);
-            else run.add_values(s);
-            if (more) run.load_v(page, h, token);
-            if (fresh) {
-                run.close();
-                if (was.whole()) {
-                    run.write(was.unit);
-                } else {
-                    const int slot = 2 * warp + (was.first == 0);   // (a run has one part that begins in front of it, at most)
-                    run.record(records + slot * S::RECORD);
-                    if (lane == 0) s_unit[slot] = was.unit;
+                const bool over = at >= end;
+                if (over) {
+                    cp_async_wait<0>();
+                    __syncwarp();
                 }
-                if (!more) break;
+                unit.record(over ? last_record : first_record);
+                if (lane == 0) s_unit[2 * warp + over] = part.unit;
             }
+            if (at >= end) break;
+            part.find(cum, units, part.b, at, end);
         }
     }
     __syncthreads();
@@ -745,16 +766,18 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
             ++i;
             continue;
         }
-        int j = i, count = 0;
-        while (j < 2 * WARPS && (s_unit[j] == unit || s_unit[j] < 0)) count += s_unit[j++] == unit;
+        int j = i;
+        while (j < 2 * WARPS && (s_unit[j] == unit || s_unit[j] < 0)) ++j;
         const int b = unit / units, chunks = cum[b + 1] - cum[b], from = cum[b] * units + (unit - b * units) * chunks;
         const bool before = from < begin, whole = !before && from + chunks <= finish;
         for (int r = 0; r < 8 * NT; ++r) {
             if ((groups + r) % WARPS != warp) continue;
-            int list = 0;               // bits: the unit's slots
-            for (int x = i; x < j; ++x) list |= (s_unit[x] == unit) << x;
             float* record = whole ? nullptr : a.part + ((long long)(2 * blockIdx.x + !before) * 8 * NT + r) * (D + 4);
-            join_row<D>(a, unit, r, count, lane, [&](int x) { return records + __fns(list, 0, x + 1) * S::RECORD + r * (D + 4); }, record);
+            join_row<D>(a, unit, r, j - i, lane, [&](int x) -> const float* {
+                const int w = (i + x) >> 1;
+                if (s_unit[i + x] != unit) return nullptr;
+                return ((i + x) & 1 ? reinterpret_cast<const float*>(rings + w * S::RING) : a.part + (2ll * gridDim.x + blockIdx.x * WARPS + w) * S::RECORD) + r * (D + 4);
+            }, record);
         }
         groups += 8 * NT;
         i = j;
@@ -784,6 +807,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a, int ctas) {
         }, nullptr);
 }
 
+constexpr int MOST_WARPS = 12;
 struct Plan {
     int nt, groups, rows, ctas;
     long long bytes;
@@ -794,13 +818,14 @@ Plan plan_of(int rows, int D) {
     p.groups = (rows + 15) / 16;
     p.rows = (rows + p.groups - 1) / p.groups;
     p.ctas = sm_count();
-    p.bytes = 2ll * p.ctas * 8 * p.nt * (D + 4) * 4;
+    p.bytes = (2ll + MOST_WARPS) * p.ctas * 8 * p.nt * (D + 4) * 4;
     return p;
 }
 
 template <int F, int D, int NT, bool ONE>
 int launch(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
     using S = Shape<F, D, NT>;
+    static_assert(S::WARPS <= MOST_WARPS, "workspace");
     const int smem = S::SMEM + (a.B + 1) * 4;
     static thread_local int set_for = -1;
     int dev = 0;
