@@ -14,12 +14,14 @@
 // Operands: tokens are the rows of the products' first operand, query rows the columns of the second - 8 of them, which one KV head's query heads
 // fill, where the other way round 16 would be half empty.  Which channel is which k, and which token which row, is free as long as both
 // operands agree, and chosen so that a lane's loads are 16 bytes and need the fewest permutations.
+#include <type_traits>
+
 #include "akv_paged.cuh"
 
 namespace akv {
 namespace {
 
-constexpr int CHUNK = 32;
+constexpr int CHUNK = 32, MOST_WARPS = 12;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // Probabilities enter their product as two halves (what the first leaves out is the second), times 2^15: 22 bits of each, as long as it is above
 // 2^-28 of the largest, of which the 11 bits of one half would show beside the output's own rounding.
@@ -29,8 +31,9 @@ struct AttendArgs {
     Pool pool;
     const __half* q;
     __half* out;
-    float *lse, *part;
-    int B, T, G, groups, rows;      // units per (sequence, KV head), query rows of a unit
+    float *lse, *part;              // part: two records of each CTA, one of each warp, a border of each CTA
+    int B, T, G, groups, rows, ctas, record;    // record: floats of one
+    // groups: units per (sequence, KV head); rows: query rows of a unit
     float scale2;                   // scale * log2(e)
 };
 
@@ -111,16 +114,18 @@ __device__ __forceinline__ void add_lengths(const AttendArgs& a, int* cum, int* 
     __syncthreads();
 }
 struct Deal {
-    int total, per_cta, runs;       // chunks in all; warps of a CTA that get a run, runs in all
-    __device__ __forceinline__ Deal(int chunks, int ctas, int warps) {
-        total = chunks;
+    int per_cta, each, more;        // warps of a CTA that get a run; chunks of a run: `each`, one more for the first `more` runs
+    __device__ __forceinline__ Deal(int total, int ctas, int warps) {
         per_cta = min(warps, (total + ctas - 1) / ctas);
-        runs = per_cta * ctas;
+        each = (unsigned)total / (unsigned)(per_cta * ctas);
+        more = total - each * per_cta * ctas;
     }
     // First chunk of run w; of run w + 1: its end.
-    __device__ __forceinline__ int start(int w) const {
-        const int each = (unsigned)total / (unsigned)runs;
-        return w * each + min(w, total - each * runs);
+    __device__ __forceinline__ int start(int w) const { return w * each + min(w, more); }
+    // CTA whose runs have chunk i.
+    __device__ __forceinline__ int cta_with(int i) const {
+        const int bound = more * (each + 1);
+        return (i < bound ? i / (each + 1) : more + (i - bound) / each) / per_cta;
     }
 };
 // A run's part of one unit.
@@ -147,6 +152,8 @@ __device__ __forceinline__ int sequence_with(const int* cum, int B, int units, i
     }
     return lo;
 }
+
+__device__ __forceinline__ int2* borders(const AttendArgs& a) { return reinterpret_cast<int2*>(a.part + (2ll + MOST_WARPS) * a.ctas * a.record); }
 
 // Row of q, out and lse [B,T,H*G] that row r of a unit stands for; -1 behind the last.
 __device__ __forceinline__ long long row_of(const AttendArgs& a, int unit, int r, int* query) {
@@ -636,6 +643,7 @@ struct Unit {
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
+                if (8 * nt + 2 * t + c >= a.rows) continue;
                 float* row = to + (8 * nt + 2 * t + c) * (D + 4);
 #pragma unroll
                 for (int i = 0; i < KS; ++i)
@@ -645,35 +653,43 @@ struct Unit {
     }
 };
 
-// Joins rows of `count` records (lane: D / 32 channels): fn(i) = row of the i-th, or null.  Then to a record, or to out and lse.
+// Joins row r of up to `count` records by a warp, lane i having those at i, i + 32, ...: fn(i) = the row in the i-th.  Then to a record, or to
+// out and lse.
 template <int D, class Fn>
 __device__ __forceinline__ void join_row(const AttendArgs& a, int unit, int r, int count, int lane, Fn fn, float* record) {
     constexpr int N = D / 32;
+    using Vec = typename std::conditional<N == 4, float4, float2>::type;
     float top = -INFINITY;
-    for (int i = lane; i < count; i += 32)
-        if (const float* x = fn(i)) top = fmaxf(top, x[D]);
+    for (int i = lane; i < count; i += 32) top = fmaxf(top, fn(i)[D]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     const float base = top == -INFINITY ? 0.f : top;
     float o[N], sum = 0.f;
 #pragma unroll
     for (int c = 0; c < N; ++c) o[c] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-        const float* x = fn(i);
-        if (!x) continue;
-        const float f = ex2(x[D] - base);
-        sum = fmaf(f, x[D + 1], sum);
+    for (int i0 = 0; i0 < count; i0 += 32) {
+        float mine = 0.f, l = 0.f;
+        if (i0 + lane < count) {
+            const float2 x = *reinterpret_cast<const float2*>(fn(i0 + lane) + D);
+            mine = ex2(x.x - base);
+            l = x.y;
+        }
+        const int here = min(32, count - i0);
+#pragma unroll 8
+        for (int i = 0; i < here; ++i) {
+            const Vec x = *reinterpret_cast<const Vec*>(fn(i0 + i) + N * lane);
+            const float f = __shfl_sync(0xFFFFFFFFu, mine, i);
+            sum = fmaf(f, __shfl_sync(0xFFFFFFFFu, l, i), sum);
 #pragma unroll
-        for (int c = 0; c < N; ++c) o[c] = fmaf(f, x[N * lane + c], o[c]);
+            for (int c = 0; c < N; ++c) o[c] = fmaf(f, reinterpret_cast<const float*>(&x)[c], o[c]);
+        }
     }
     if (record) {
+        Vec x;
 #pragma unroll
-        for (int c = 0; c < N; ++c) record[N * lane + c] = o[c];
-        if (lane == 0) {
-            record[D] = top;
-            record[D + 1] = sum;
-        }
+        for (int c = 0; c < N; ++c) reinterpret_cast<float*>(&x)[c] = o[c];
+        *reinterpret_cast<Vec*>(record + N * lane) = x;
+        if (lane == 0) *reinterpret_cast<float2*>(record + D) = make_float2(top, sum);
         return;
     }
     int query;
@@ -692,7 +708,10 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
     constexpr int WARPS = S::WARPS;
     extern __shared__ __align__(128) uint8_t rings[];
     int* cum = reinterpret_cast<int*>(rings + S::SMEM);
-    __shared__ int sums[WARPS], s_unit[2 * WARPS];             // (s_unit: units of the records of each run's first part and of its last, or -1)
+    __shared__ int sums[WARPS], s_unit[2 * WARPS], s_tasks;     // (s_unit: units of the records of each run's first part and of its last, or -1)
+    __shared__ int4 s_task[2 * WARPS];                         // unit, its first of s_slots, how many, where they go
+    __shared__ int s_slots[2 * WARPS];
+    __shared__ int2 s_border;
     pdl_turn();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     add_lengths<32 * WARPS>(a, cum, sums);
@@ -756,58 +775,53 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
         }
     }
     __syncthreads();
-    // Records of one unit lie in a row (slots without one aside).  A unit that begins and ends in this CTA is written, of another one
-    // record is left: slot 0 of the CTA's two where it began in front of it.
-    const int begin = deal.start(blockIdx.x * deal.per_cta), finish = deal.start((blockIdx.x + 1) * deal.per_cta);
-    int groups = 0;
-    for (int i = 0; i < 2 * WARPS;) {
-        const int unit = s_unit[i];
-        if (unit < 0) {
-            ++i;
-            continue;
+    // A unit whose records all are in this CTA is written, of another one record is left: the CTA's first where it began in front of it, else its
+    // second, and for the kernel that joins those the unit and the last CTA that has a part of it.
+    if (warp == 0) {
+        const int unit = lane < 2 * WARPS ? s_unit[lane] : -1;
+        const unsigned same = __match_any_sync(0xFFFFFFFFu, unit);
+        const bool leads = unit >= 0 && (same & ((1u << lane) - 1)) == 0;
+        const unsigned leaders = __ballot_sync(0xFFFFFFFFu, leads), below = (1u << lane) - 1;
+        const int place = __popc(__ballot_sync(0xFFFFFFFFu, unit >= 0) & below);       // records in front of this one
+        if (unit >= 0) s_slots[place] = lane;
+        if (lane == 0) {
+            s_tasks = __popc(leaders);
+            s_border = make_int2(-1, 0);
         }
-        int j = i;
-        while (j < 2 * WARPS && (s_unit[j] == unit || s_unit[j] < 0)) ++j;
-        const int b = unit / units, chunks = cum[b + 1] - cum[b], from = cum[b] * units + (unit - b * units) * chunks;
-        const bool before = from < begin, whole = !before && from + chunks <= finish;
-        for (int r = 0; r < 8 * NT; ++r) {
-            if ((groups + r) % WARPS != warp) continue;
-            float* record = whole ? nullptr : a.part + ((long long)(2 * blockIdx.x + !before) * 8 * NT + r) * (D + 4);
-            join_row<D>(a, unit, r, j - i, lane, [&](int x) -> const float* {
-                const int w = (i + x) >> 1;
-                if (s_unit[i + x] != unit) return nullptr;
-                return ((i + x) & 1 ? reinterpret_cast<const float*>(rings + w * S::RING) : a.part + (2ll * gridDim.x + blockIdx.x * WARPS + w) * S::RECORD) + r * (D + 4);
-            }, record);
+        __syncwarp();
+        if (leads) {
+            const int b = unit / units, chunks = cum[b + 1] - cum[b], from = cum[b] * units + (unit - b * units) * chunks;
+            const bool before = from < deal.start(blockIdx.x * deal.per_cta), after = from + chunks > deal.start((blockIdx.x + 1) * deal.per_cta);
+            if (!before && after) s_border = make_int2(unit, deal.cta_with(from + chunks - 1));
+            s_task[__popc(leaders & below)] = make_int4(unit, place, __popc(same), before ? 0 : after ? 1 : -1);
         }
-        groups += 8 * NT;
-        i = j;
+        __syncwarp();
+        if (lane == 0) borders(a)[blockIdx.x] = s_border;
+    }
+    __syncthreads();
+    for (int x = warp; x < s_tasks * a.rows; x += WARPS) {
+        const int i = x / a.rows, r = x - i * a.rows;
+        const int4 task = s_task[i];
+        float* record = task.w < 0 ? nullptr : a.part + ((long long)(2 * blockIdx.x + task.w) * 8 * NT + r) * (D + 4);
+        join_row<D>(a, task.x, r, task.z, lane, [&](int k) {
+            const int slot = s_slots[task.y + k], w = slot >> 1;
+            return (slot & 1 ? reinterpret_cast<const float*>(rings + w * S::RING) : a.part + (2ll * gridDim.x + blockIdx.x * WARPS + w) * S::RECORD) + r * (D + 4);
+        }, record);
     }
 }
 
-// One CTA per border between two CTAs of attend_kernel: the first inside a unit joins its records.
-template <int D, int NT, int WARPS>
-__global__ void __launch_bounds__(256) join_kernel(AttendArgs a, int ctas) {
-    extern __shared__ int cum[];
-    __shared__ int sums[8];
-    // (what this kernel follows waited for everything in front of it: lens may be read)
-    add_lengths<256>(a, cum, sums);
-    const int units = a.pool.H * a.groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const Deal deal(cum[a.B] * units, ctas, WARPS);
-    const int border = blockIdx.x + 1, at = deal.start(border * deal.per_cta);
+// One CTA per CTA of attend_kernel: where a unit begins there and ends in another one, its records are joined.
+template <int D, int NT>
+__global__ void __launch_bounds__(32 * 8 * NT) join_kernel(AttendArgs a) {
     pdl_turn();
-    if (at >= deal.total) return;
-    const int b = sequence_with(cum, a.B, units, at), chunks = cum[b + 1] - cum[b], u = (at - cum[b] * units) / chunks;
-    const int unit = b * units + u, from = cum[b] * units + u * chunks;
-    if (from == at || from < deal.start((border - 1) * deal.per_cta)) return;
-    int last = border;              // CTA with the unit's end
-    while (deal.start((last + 1) * deal.per_cta) < from + chunks) ++last;
-    for (int r = warp; r < 8 * NT; r += 8)
-        join_row<D>(a, unit, r, last - border + 2, lane, [&](int i) {
-            return a.part + ((long long)(2 * (border - 1 + i) + (i == 0)) * 8 * NT + r) * (D + 4);
-        }, nullptr);
+    const int2 border = borders(a)[blockIdx.x];
+    const int lane = threadIdx.x & 31, r = threadIdx.x >> 5, from = blockIdx.x;
+    if (border.x < 0 || r >= a.rows) return;
+    join_row<D>(a, border.x, r, border.y - from + 1, lane, [&](int i) {
+        return a.part + ((long long)(2 * (from + i) + (i == 0)) * 8 * NT + r) * (D + 4);
+    }, nullptr);
 }
 
-constexpr int MOST_WARPS = 12;
 struct Plan {
     int nt, groups, rows, ctas;
     long long bytes;
@@ -818,7 +832,7 @@ Plan plan_of(int rows, int D) {
     p.groups = (rows + 15) / 16;
     p.rows = (rows + p.groups - 1) / p.groups;
     p.ctas = sm_count();
-    p.bytes = (2ll + MOST_WARPS) * p.ctas * 8 * p.nt * (D + 4) * 4;
+    p.bytes = (2ll + MOST_WARPS) * p.ctas * 8 * p.nt * (D + 4) * 4 + 8ll * p.ctas;
     return p;
 }
 
@@ -839,7 +853,7 @@ int launch(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
     launch_chained(attend_kernel<F, D, NT, ONE>, dim3(p.ctas), dim3(32 * S::WARPS), smem, st, a);
     const int rc = cuda_status(cudaGetLastError(), "paged_attention launch");
     if (rc != AKV_OK || !joined || p.ctas == 1) return rc;
-    launch_chained(join_kernel<D, NT, S::WARPS>, dim3(p.ctas - 1), dim3(256), (a.B + 1) * 4, st, a, p.ctas);
+    launch_chained(join_kernel<D, NT>, dim3(p.ctas), dim3(32 * 8 * NT), 0, st, a);
     return cuda_status(cudaGetLastError(), "paged_attention join launch");
 }
 template <int F, int D, int NT>
@@ -895,6 +909,8 @@ int akv_paged_attention(const akv_pool* pool, const void* q, const void* pages, 
     a.G = group;
     a.groups = p.groups;
     a.rows = p.rows;
+    a.ctas = p.ctas;
+    a.record = 8 * p.nt * (D + 4);
     a.scale2 = scale * LOG2E;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool joined = (long long)width * pool->page_size > CHUNK;      // (units of one chunk are nobody else's)
