@@ -14,7 +14,7 @@
 namespace akv {
 namespace {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, MOST = 64;
+constexpr int THREADS = 512, WARPS = THREADS / 32, MOST = 64, MOST_CTAS = 8;
 
 template <class P>
 struct ChooseArgs {
@@ -25,17 +25,28 @@ struct ChooseArgs {
     const int* parents;
     int *path, *count;
     long long* token;
-    int T, V;
+    int T, V, ctas;            // ctas: of a sequence's cluster
 };
 
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 // What is no probability counts as none.
-template <class P>
-__device__ __forceinline__ float chance(const P* at) {
-    const float x = as_float(__ldg(at));
-    return x > 0.f && x < INFINITY ? x : 0.f;
+__device__ __forceinline__ float chance(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
+
+// E = 16 bytes of probabilities from j on (zeros behind V).  VEC: rows begin on 16-byte boundaries.
+template <class P, bool VEC>
+__device__ __forceinline__ void load(float (&x)[16 / sizeof(P)], const P* row, int j, int V) {
+    constexpr int E = 16 / sizeof(P);
+    if (VEC && j + E <= V) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + j));
+        const P* e = reinterpret_cast<const P*>(&w);
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = chance(as_float(e[i]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = j + i < V ? chance(as_float(row[j + i])) : 0.f;
+    }
 }
 
 __device__ __forceinline__ double warp_sum(double x) {
@@ -43,16 +54,26 @@ __device__ __forceinline__ double warp_sum(double x) {
     for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
     return x;
 }
+// Address of a shared variable of this CTA in another CTA of the cluster.
+__device__ __forceinline__ uint32_t there(const void* p, int cta) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(smem_u32(p)), "r"(cta));
+    return a;
+}
 
-template <class P>
-__global__ void __launch_bounds__(THREADS) choose_kernel(ChooseArgs<P> a) {
-    __shared__ double s_sum[WARPS];
-    __shared__ int s_up[MOST], s_gone[MOST], s_found, s_last;
+// Bound by HBM where the batch is large (a row of p, one of q, read once by the cluster of the sequence and once more, of one warp's part, from
+// L2), by latency where it is small: the numbers of the nodes, the row, two barriers.  The vocabulary is cut into contiguous parts, a
+// warp's each, so that the sums of the parts in front of one tell where the random number falls.
+template <class P, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
+    constexpr int E = 16 / sizeof(P), STEP = 32 * E;
+    __shared__ double s_sum[WARPS], s_cta[2][MOST_CTAS];
+    __shared__ int s_up[MOST], s_gone[MOST], s_first, s_last;
     __shared__ float s_p[MOST], s_q[MOST], s_u[MOST];
     __shared__ long long s_x[MOST];
-    pdl_turn();
-    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int ctas = a.ctas, rank = blockIdx.x % ctas, b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int T = a.T, V = a.V;
+    pdl_turn();
     const P* target = a.target + b * a.target_batch;
     const P* draft = a.draft ? a.draft + b * a.draft_batch : nullptr;
     if (tid < T) {
@@ -62,33 +83,62 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(ChooseArgs<P> a) {
         s_up[tid] = up;
         s_x[tid] = x;
         s_u[tid] = a.coins[(long long)b * T + tid];
-        s_p[tid] = asked ? chance(target + up * a.target_row + x) : 0.f;
-        s_q[tid] = asked && draft ? chance(draft + up * a.draft_row + x) : 0.f;
+        s_p[tid] = asked ? chance(as_float(target[up * a.target_row + x])) : 0.f;
+        s_q[tid] = asked && draft ? chance(as_float(draft[up * a.draft_row + x])) : 0.f;
+    }
+    if (tid == 0) {
+        s_first = V;
+        s_last = -1;
     }
     __syncthreads();
-    const int each = (V + WARPS - 1) / WARPS, first = min(V, warp * each), last = min(V, first + each);
-    int now = 0, count = 1, gone = 0;
+    // parts of whole steps; this warp's begins at `first`
+    const int steps = (V + STEP - 1) / STEP, each = (steps + ctas * WARPS - 1) / (ctas * WARPS);
+    const int first = min(V, (rank * WARPS + warp) * each * STEP), last = min(V, first + each * STEP);
+    int now = 0, count = 1, gone = 0, turn = 0;
     double c = 0.0, left = 1.0;
-    if (tid == 0) a.path[(long long)b * T] = 0;
-    auto rest = [&](int j) -> double {
-        double r = chance(target + now * a.target_row + j);
-        if (draft) {
-            if (c > 0.0) r = fmax(r - c * (double)chance(draft + now * a.draft_row + j), 0.0);
+    if (tid == 0 && rank == 0) a.path[(long long)b * T] = 0;
+    // what is left of E probabilities from j on
+    auto rest = [&](double (&r)[E], int j, int j0) {
+        float x[E];
+        load<P, VEC>(x, target + now * a.target_row, j, V);
+        if (c > 0.0) {
+            float y[E];
+            load<P, VEC>(y, draft + now * a.draft_row, j, V);
+#pragma unroll
+            for (int i = 0; i < E; ++i) r[i] = fmax(fma(-c, (double)y[i], (double)x[i]), 0.0);
         } else {
-            for (int g = 0; g < gone; ++g)
-                if (s_gone[g] == j) r = 0.0;
+            for (int g = 0; g < gone; ++g) {
+                const int k = s_gone[g] - j0;
+                if (k >= 0 && k < STEP)
+#pragma unroll
+                    for (int i = 0; i < E; ++i)
+                        if (k == j - j0 + i) x[i] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < E; ++i) r[i] = x[i];
         }
-        return r;
     };
     auto total = [&]() -> double {
         double sum = 0.0;
-        for (int j = first + lane; j < last; j += 32) sum += rest(j);
+#pragma unroll 2
+        for (int j0 = first; j0 < last; j0 += STEP) {
+            double r[E];
+            rest(r, j0 + lane * E, j0);
+#pragma unroll
+            for (int i = 0; i < E; ++i) sum += r[i];
+        }
         sum = warp_sum(sum);
-        __syncthreads();
+        __syncthreads();                       // (the last sums have been read)
         if (lane == 0) s_sum[warp] = sum;
         __syncthreads();
+        turn ^= 1;
+        if (warp == 0) {
+            const double mine = warp_sum(lane < WARPS ? s_sum[lane] : 0.0);
+            if (lane < ctas) asm volatile("st.shared::cluster.f64 [%0], %1;\n" ::"r"(there(&s_cta[turn][rank], lane)), "d"(mine) : "memory");
+        }
+        cluster_sync();
         sum = 0.0;
-        for (int w = 0; w < WARPS; ++w) sum += s_sum[w];
+        for (int i = 0; i < ctas; ++i) sum += s_cta[turn][i];
         return sum;
     };
     for (int i = 1; i < T; ++i) {
@@ -96,7 +146,7 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(ChooseArgs<P> a) {
         const double u = s_u[i], p = s_p[i], q = s_q[i];
         bool good;
         if (draft) {
-            good = u * left * q < fmax(p - c * q, 0.0);
+            good = u * left * q < fmax(fma(-c, q, p), 0.0);
         } else {
             double r = p;
             for (int g = 0; g < gone; ++g)
@@ -115,11 +165,13 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(ChooseArgs<P> a) {
             c = 0.0;
             left = 1.0;
             gone = 0;
-            if (tid == 0) a.path[(long long)b * T + count] = i;
+            if (tid == 0 && rank == 0) a.path[(long long)b * T + count] = i;
             ++count;
         } else if (draft) {
             c += left;
-            left = total();
+            bool again = false;                // (the sum behind the last child is formed below)
+            for (int k = i + 1; k < T; ++k) again |= s_up[k] == now;
+            if (again) left = total();
         }
     }
     double sum = total();
@@ -128,41 +180,86 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(ChooseArgs<P> a) {
         gone = 0;
         sum = total();
     }
-    if (tid == 0) {
-        a.count[b] = count;
-        s_found = V;
-        s_last = -1;
+    if (rank == 0) {
+        if (tid == 0) a.count[b] = count;
+        for (int i = count + tid; i < T; i += THREADS) a.path[(long long)b * T + i] = -1;
     }
-    for (int i = count + tid; i < T; i += THREADS) a.path[(long long)b * T + i] = -1;
-    __syncthreads();
     const double at = (double)fmaxf(s_u[0], 0.f) * sum;
     double before = 0.0;
+    for (int i = 0; i < rank; ++i) before += s_cta[turn][i];
     for (int w = 0; w < warp; ++w) before += s_sum[w];
-    int found = V, end = -1;
-    for (int j0 = first; j0 < last; j0 += 32) {
-        const int j = j0 + lane;
-        const double r = j < last ? rest(j) : 0.0;
-        double x = r;
+    if (before <= at && before + s_sum[warp] > at) {
+        for (int j0 = first; j0 < last; j0 += STEP) {
+            double r[E], x = 0.0;
+            rest(r, j0 + lane * E, j0);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(0xFFFFFFFFu, x, o);
-            if (lane >= o) x += y;
+            for (int i = 0; i < E; ++i) x += r[i];
+            const double own = x;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+                if (lane >= o) x += y;
+            }
+            if (__any_sync(0xFFFFFFFFu, before + x > at)) {
+                double z = before + (x - own);
+                int found = V;
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    z += r[i];
+                    if (found == V && r[i] > 0.0 && z > at) found = j0 + lane * E + i;
+                }
+                found = __reduce_min_sync(0xFFFFFFFFu, found);
+                if (found < V) {
+                    if (lane == 0) asm volatile("red.shared::cluster.min.s32 [%0], %1;\n" ::"r"(there(&s_first, 0)), "r"(found) : "memory");
+                    break;
+                }
+            }
+            before += __shfl_sync(0xFFFFFFFFu, x, 31);
         }
-        if (r > 0.0) end = j;
-        if (found == V && before + x > at && j < last) found = j;
-        before += __shfl_sync(0xFFFFFFFFu, x, 31);
     }
-    atomicMin(&s_found, found);
-    atomicMax(&s_last, end);
-    __syncthreads();
-    if (tid == 0) a.token[b] = sum > 0.0 ? (s_found < V ? s_found : s_last) : -1;
+    cluster_sync();
+    int found;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(found) : "r"(there(&s_first, 0)) : "memory");
+    cluster_sync();
+    if (found == V && sum > 0.0) {
+        // A random number at the end, or between two parts whose sums were rounded: the first entry behind it, else the last in front of it.
+        before = 0.0;
+        for (int i = 0; i < rank; ++i) before += s_cta[turn][i];
+        for (int w = 0; w < warp; ++w) before += s_sum[w];
+        int low = V, high = -1;
+        for (int j0 = first; j0 < last; j0 += STEP) {
+            double r[E];
+            rest(r, j0 + lane * E, j0);
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (r[i] > 0.0) {
+                    const int j = j0 + lane * E + i;
+                    if (before > at) low = min(low, j);
+                    else high = max(high, j);
+                }
+        }
+        low = __reduce_min_sync(0xFFFFFFFFu, low);
+        high = __reduce_max_sync(0xFFFFFFFFu, high);
+        if (lane == 0) {
+            asm volatile("red.shared::cluster.min.s32 [%0], %1;\n" ::"r"(there(&s_first, 0)), "r"(low) : "memory");
+            asm volatile("red.shared::cluster.max.s32 [%0], %1;\n" ::"r"(there(&s_last, 0)), "r"(high) : "memory");
+        }
+        cluster_sync();
+    }
+    if (rank == 0 && tid == 0) a.token[b] = !(sum > 0.0) ? -1 : s_first < V ? s_first : s_last;
 }
 
 template <class P>
 int launch_choose(ChooseArgs<P> a, const void* target, const void* draft, int bsz, cudaStream_t st) {
     a.target = static_cast<const P*>(target);
     a.draft = static_cast<const P*>(draft);
-    launch_chained(choose_kernel<P>, dim3(bsz), dim3(THREADS), 0, st, a);
+    constexpr int E = 16 / sizeof(P);
+    const bool vec = aligned16(target) && aligned16(draft) && a.target_batch % E == 0 && a.target_row % E == 0 &&
+                     (!draft || (a.draft_batch % E == 0 && a.draft_row % E == 0));
+    // As many CTAs a sequence as keep a step or more for every warp, and all sequences' resident at once.
+    a.ctas = MOST_CTAS;
+    while (a.ctas > 1 && ((long long)a.ctas * WARPS * 32 * E > a.V || (long long)bsz * a.ctas > 2ll * sm_count())) a.ctas /= 2;
+    launch_cluster(vec ? choose_kernel<P, true> : choose_kernel<P, false>, a.ctas, dim3((unsigned)bsz * a.ctas), dim3(THREADS), 0, st, a);
     return cuda_status(cudaGetLastError(), "accept_drafts launch");
 }
 
@@ -176,7 +273,7 @@ extern "C" int akv_accept_drafts(const void* target, long long target_batch, lon
                                  void* path, void* count, void* token, int bsz, int drafted, int vocab, int type, void* stream) {
     set_error("");
     AKV_REQUIRE(target && ids && coins && path && count && token, AKV_ERR_NULL, "accept_drafts: null pointer");
-    AKV_REQUIRE(bsz > 0 && drafted >= 1 && drafted <= MOST && vocab > 0, AKV_ERR_SHAPE,
+    AKV_REQUIRE(bsz > 0 && bsz <= 1 << 24 && drafted >= 1 && drafted <= MOST && vocab > 0, AKV_ERR_SHAPE,
                 "accept_drafts: %d sequences, %d tokens each (1 to %d) of a vocabulary of %d", bsz, drafted, MOST, vocab);
     AKV_REQUIRE(vocab <= 1 << 24, AKV_ERR_OVERFLOW, "accept_drafts: a vocabulary of %d", vocab);
     AKV_REQUIRE(type == AKV_TYPE_FP32 || type == AKV_TYPE_FP16 || type == AKV_TYPE_BF16, AKV_ERR_SHAPE, "accept_drafts: type %d", type);

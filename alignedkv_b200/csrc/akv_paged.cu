@@ -5,6 +5,7 @@ namespace akv {
 namespace {
 
 constexpr int THREADS = 256, VALUES = 8;       // a thread has 8 channels: 16 bytes of fp16
+constexpr int MANY = 4;                        // rows of a thread, whose loads are on their way together
 
 struct AppendArgs {
     Pool pool;
@@ -82,21 +83,35 @@ __device__ __forceinline__ void store_row(uint8_t* codes, int8_t* exps, uint8_t*
     }
 }
 
-// One row of one tensor per LANES threads; a block has consecutive tokens of one KV head, whose rows lie side by side in a page.
+// Rows of one tensor by LANES threads each; a block has consecutive tokens of one KV head, whose rows lie side by side in a page.  Bound by HBM where
+// there is much to do.
 template <int F, int D>
 __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
     constexpr int LANES = D / VALUES, ROWS = THREADS / LANES;
     pdl_turn();
-    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1;
-    const int i = blockIdx.x * ROWS + threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1, lane = threadIdx.x % LANES;
+    const int i0 = blockIdx.x * (MANY * ROWS) + threadIdx.x / LANES;
     const int n = a.counts ? min(a.T, a.counts[b]) : a.T;
+    if (blockIdx.x * (MANY * ROWS) >= n) return;
     const Pool& p = a.pool;
-    const long long at = (long long)max(0, p.lens[b]) + i;
-    long long row = -1;
-    if (i < n && at < (long long)p.width << p.shift) row = pool_row(p, b, h, at);
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (row >= 0) raw = __ldg(reinterpret_cast<const uint4*>(a.x[which] + b * a.batch[which] + i * a.token[which] + h * a.head[which]) + lane);
-    store_row<F, D>(which ? p.vc : p.kc, which ? p.ve : p.ke, which ? p.vs : p.ks, row, lane, raw);
+    const long long at = max(0, p.lens[b]), room = (long long)p.width << p.shift;
+    const __half* x = a.x[which] + b * a.batch[which] + h * a.head[which] + lane * VALUES;
+    uint4 raw[MANY];
+    long long row[MANY];
+#pragma unroll
+    for (int m = 0; m < MANY; ++m) {
+        const int i = i0 + m * ROWS;
+        raw[m] = make_uint4(0, 0, 0, 0);
+        row[m] = -1;
+        if (i < n && at + i < room) {
+            raw[m] = __ldg(reinterpret_cast<const uint4*>(x + i * a.token[which]));
+            row[m] = pool_row(p, b, h, at + i);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MANY; ++m)
+        if (blockIdx.x * (MANY * ROWS) + m * ROWS < n)        // (the same for the block)
+            store_row<F, D>(which ? p.vc : p.kc, which ? p.ve : p.ke, which ? p.vs : p.ks, row[m], lane, raw[m]);
 }
 
 // fp16 of a value beyond its range: the largest.  (A code may be above the value it stands for: 65504 is held as 65536.)
@@ -112,55 +127,77 @@ template <int F, int D>
 __global__ void __launch_bounds__(THREADS) read_kernel(ReadArgs a) {
     constexpr int LANES = D / VALUES, ROWS = THREADS / LANES;
     pdl_turn();
-    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1;
-    const int i = blockIdx.x * ROWS + threadIdx.x / LANES, lane = threadIdx.x % LANES;
-    if (i >= a.most) return;
+    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1, lane = threadIdx.x % LANES;
+    const int i0 = blockIdx.x * (MANY * ROWS) + threadIdx.x / LANES;
     const Pool& p = a.pool;
-    const long long row = i < length_of(p, b) ? pool_row(p, b, h, i) : -1;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row >= 0) {
-        const uint8_t* codes = which ? p.vc : p.kc;
-        if constexpr (F == AKV_PAGE_FP16) {
-            v = *reinterpret_cast<const uint4*>(codes + row * (2 * D) + lane * 16);
-        } else {
-            const float unit = power2((which ? p.ve : p.ke)[row]);
-            float scale = 1.f;                 // (multiplied first: codes times scales are exact, and far from fp32's ends)
+    const int n = length_of(p, b);
+    const uint8_t* codes = (which ? p.vc : p.kc) + lane * (row_bytes<F>(D) / LANES);
+    uint4 w[MANY];
+    int exponent[MANY];
+    uint32_t scale[MANY];
+#pragma unroll
+    for (int m = 0; m < MANY; ++m) {
+        const int i = i0 + m * ROWS;
+        const long long row = i < n && i < a.most ? pool_row(p, b, h, i) : -1;
+        w[m] = make_uint4(0, 0, 0, 0);
+        exponent[m] = 0;
+        scale[m] = 0;
+        if (row >= 0) {
+            if constexpr (F == AKV_PAGE_FP16) {
+                w[m] = __ldg(reinterpret_cast<const uint4*>(codes + row * (2 * D)));
+            } else {
+                if constexpr (F == AKV_PAGE_E4M3) {
+                    const uint2 x = __ldg(reinterpret_cast<const uint2*>(codes + row * D));
+                    w[m].x = x.x;
+                    w[m].y = x.y;
+                } else {
+                    w[m].x = __ldg(reinterpret_cast<const uint32_t*>(codes + row * (D / 2)));
+                    scale[m] = __ldg((which ? p.vs : p.ks) + row * (D / 16) + (lane >> 1));
+                }
+                exponent[m] = __ldg((which ? p.ve : p.ke) + row);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MANY; ++m) {
+        const int i = i0 + m * ROWS;
+        if (i >= a.most) continue;
+        if constexpr (F != AKV_PAGE_FP16) {
+            const float unit = power2(exponent[m]);
+            float s = 1.f;                     // (multiplied first: codes times scales are exact, and far from fp32's ends)
             uint32_t h2[4];
             if constexpr (F == AKV_PAGE_E4M3) {
-                const uint2 w = *reinterpret_cast<const uint2*>(codes + row * D + lane * VALUES);
-                h2[0] = e4m3_halves(w.x & 0xFFFFu);
-                h2[1] = e4m3_halves(w.x >> 16);
-                h2[2] = e4m3_halves(w.y & 0xFFFFu);
-                h2[3] = e4m3_halves(w.y >> 16);
+                uint32_t x[2], y[2];
+                e4m3_word(x, w[m].x);
+                e4m3_word(y, w[m].y);
+                h2[0] = x[0]; h2[1] = x[1]; h2[2] = y[0]; h2[3] = y[1];
             } else {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + row * (D / 2) + lane * 4);
-                scale = e4m3_float((which ? p.vs : p.ks)[row * (D / 16) + (lane >> 1)]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) h2[k] = e2m1_halves((w >> (8 * k)) & 0xFFu);
+                s = e4m3_float(scale[m]);
+                e2m1_word(h2, w[m].x);
             }
             uint32_t o[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float2 f = halves_floats(h2[k]);
-                const __half2 r = __floats2half2_rn(saturated(f.x * scale * unit), saturated(f.y * scale * unit));
+                const __half2 r = __floats2half2_rn(saturated(f.x * s * unit), saturated(f.y * s * unit));
                 o[k] = *reinterpret_cast<const uint32_t*>(&r);
             }
-            v = make_uint4(o[0], o[1], o[2], o[3]);
+            w[m] = make_uint4(o[0], o[1], o[2], o[3]);
         }
+        *(reinterpret_cast<uint4*>(a.x[which] + (((long long)b * a.most + i) * p.H + h) * D) + lane) = w[m];
     }
-    *(reinterpret_cast<uint4*>(a.x[which] + (((long long)b * a.most + i) * p.H + h) * D) + lane) = v;
 }
 
 template <int F>
 void launch_append(const AppendArgs& a, int D, int bsz, cudaStream_t st) {
-    const int rows = THREADS / (D / VALUES);
+    const int rows = MANY * (THREADS / (D / VALUES));
     const dim3 grid((a.T + rows - 1) / rows, 2 * a.pool.H, bsz);
     if (D == 128) launch_chained(append_kernel<F, 128>, grid, dim3(THREADS), 0, st, a);
     else launch_chained(append_kernel<F, 64>, grid, dim3(THREADS), 0, st, a);
 }
 template <int F>
 void launch_read(const ReadArgs& a, int D, int bsz, cudaStream_t st) {
-    const int rows = THREADS / (D / VALUES);
+    const int rows = MANY * (THREADS / (D / VALUES));
     const dim3 grid((unsigned)(((long long)a.most + rows - 1) / rows), 2 * a.pool.H, bsz);
     if (D == 128) launch_chained(read_kernel<F, 128>, grid, dim3(THREADS), 0, st, a);
     else launch_chained(read_kernel<F, 64>, grid, dim3(THREADS), 0, st, a);

@@ -14,7 +14,7 @@ namespace akv {
 //                  least with max |x| <= 6 * 448 2^e, s the nearest to max |x| 2^-e / 6 of its 16 channels.
 // Exponent -128: a row with a value that is not finite; it stands for NaN throughout, its codes are zero.
 constexpr int EXP_NAN = -128;
-template <int F> constexpr int row_bytes(int D) { return F == AKV_PAGE_FP16 ? 2 * D : F == AKV_PAGE_E4M3 ? D : D / 2; }
+template <int F> __host__ __device__ constexpr int row_bytes(int D) { return F == AKV_PAGE_FP16 ? 2 * D : F == AKV_PAGE_E4M3 ? D : D / 2; }
 
 struct Pool {
     uint8_t *kc, *vc;          // codes
