@@ -9,10 +9,10 @@ constexpr int MANY = 4;                        // rows of a thread, whose loads 
 
 struct AppendArgs {
     Pool pool;
-    const __half* x[2];                        // k, v
-    long long batch[2], token[2], head[2];     // their strides
+    const __half *k, *v;
+    long long k_batch, k_token, k_head, v_batch, v_token, v_head;
     const int* counts;
-    int T;
+    int T, blocks;                             // blocks of a sequence's tokens
 };
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
@@ -83,19 +83,35 @@ __device__ __forceinline__ void store_row(uint8_t* codes, int8_t* exps, uint8_t*
     }
 }
 
+// What a block has: K and V of all heads side by side, then the next tokens, then the next sequence; so that what is written at one time lies
+// together (hold, e4m3: HEADFIRST us the other way round).
+struct Place {
+    int b, block, h;
+    bool which;
+    __device__ __forceinline__ Place(int H, int blocks) {
+        const unsigned x = blockIdx.x / (2u * H), y = blockIdx.x - x * 2u * H;
+        which = y >= (unsigned)H;
+        h = which ? y - H : y;
+        b = x / (unsigned)blocks;
+        block = x - b * blocks;
+    }
+};
+
 // Rows of one tensor by LANES threads each; a block has consecutive tokens of one KV head, whose rows lie side by side in a page.  Bound by HBM where
 // there is much to do.
 template <int F, int D>
 __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
     constexpr int LANES = D / VALUES, ROWS = THREADS / LANES;
     pdl_turn();
-    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1, lane = threadIdx.x % LANES;
-    const int i0 = blockIdx.x * (MANY * ROWS) + threadIdx.x / LANES;
-    const int n = a.counts ? min(a.T, a.counts[b]) : a.T;
-    if (blockIdx.x * (MANY * ROWS) >= n) return;
     const Pool& p = a.pool;
+    const Place at0(p.H, a.blocks);
+    const int b = at0.b, h = at0.h, lane = threadIdx.x % LANES, begin = at0.block * (MANY * ROWS), i0 = begin + threadIdx.x / LANES;
+    const bool which = at0.which;
+    const int n = a.counts ? min(a.T, a.counts[b]) : a.T;
+    if (begin >= n) return;
     const long long at = max(0, p.lens[b]), room = (long long)p.width << p.shift;
-    const __half* x = a.x[which] + b * a.batch[which] + h * a.head[which] + lane * VALUES;
+    const __half* x = (which ? a.v + b * a.v_batch + h * a.v_head : a.k + b * a.k_batch + h * a.k_head) + lane * VALUES;
+    const long long step = which ? a.v_token : a.k_token;
     uint4 raw[MANY];
     long long row[MANY];
 #pragma unroll
@@ -104,13 +120,13 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
         raw[m] = make_uint4(0, 0, 0, 0);
         row[m] = -1;
         if (i < n && at + i < room) {
-            raw[m] = __ldg(reinterpret_cast<const uint4*>(x + i * a.token[which]));
+            raw[m] = __ldg(reinterpret_cast<const uint4*>(x + i * step));
             row[m] = pool_row(p, b, h, at + i);
         }
     }
 #pragma unroll
     for (int m = 0; m < MANY; ++m)
-        if (blockIdx.x * (MANY * ROWS) + m * ROWS < n)        // (the same for the block)
+        if (begin + m * ROWS < n)        // (the same for the block)
             store_row<F, D>(which ? p.vc : p.kc, which ? p.ve : p.ke, which ? p.vs : p.ks, row[m], lane, raw[m]);
 }
 
@@ -119,18 +135,20 @@ __device__ __forceinline__ float saturated(float x) { return fabsf(x) > 65504.f 
 
 struct ReadArgs {
     Pool pool;
-    __half* x[2];
-    int most;
+    __half *k, *v;
+    int most, blocks;
 };
 
 template <int F, int D>
 __global__ void __launch_bounds__(THREADS) read_kernel(ReadArgs a) {
     constexpr int LANES = D / VALUES, ROWS = THREADS / LANES;
     pdl_turn();
-    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1, lane = threadIdx.x % LANES;
-    const int i0 = blockIdx.x * (MANY * ROWS) + threadIdx.x / LANES;
     const Pool& p = a.pool;
+    const Place at0(p.H, a.blocks);
+    const int b = at0.b, h = at0.h, lane = threadIdx.x % LANES, i0 = at0.block * (MANY * ROWS) + threadIdx.x / LANES;
+    const bool which = at0.which;
     const int n = length_of(p, b);
+    __half* out = which ? a.v : a.k;
     const uint8_t* codes = (which ? p.vc : p.kc) + lane * (row_bytes<F>(D) / LANES);
     uint4 w[MANY];
     int exponent[MANY];
@@ -184,23 +202,21 @@ __global__ void __launch_bounds__(THREADS) read_kernel(ReadArgs a) {
             }
             w[m] = make_uint4(o[0], o[1], o[2], o[3]);
         }
-        *(reinterpret_cast<uint4*>(a.x[which] + (((long long)b * a.most + i) * p.H + h) * D) + lane) = w[m];
+        __stcs(reinterpret_cast<uint4*>(out + (((long long)b * a.most + i) * p.H + h) * D) + lane, w[m]);
     }
 }
 
+// Blocks of a sequence's `tokens`; blocks of all (b, head, tensor) may not fit a grid.
+int blocks_of(int tokens, int D) { return (tokens + MANY * (THREADS / (D / VALUES)) - 1) / (MANY * (THREADS / (D / VALUES))); }
 template <int F>
-void launch_append(const AppendArgs& a, int D, int bsz, cudaStream_t st) {
-    const int rows = MANY * (THREADS / (D / VALUES));
-    const dim3 grid((a.T + rows - 1) / rows, 2 * a.pool.H, bsz);
-    if (D == 128) launch_chained(append_kernel<F, 128>, grid, dim3(THREADS), 0, st, a);
-    else launch_chained(append_kernel<F, 64>, grid, dim3(THREADS), 0, st, a);
+void launch_append(const AppendArgs& a, int D, unsigned grid, cudaStream_t st) {
+    if (D == 128) launch_chained(append_kernel<F, 128>, dim3(grid), dim3(THREADS), 0, st, a);
+    else launch_chained(append_kernel<F, 64>, dim3(grid), dim3(THREADS), 0, st, a);
 }
 template <int F>
-void launch_read(const ReadArgs& a, int D, int bsz, cudaStream_t st) {
-    const int rows = MANY * (THREADS / (D / VALUES));
-    const dim3 grid((unsigned)(((long long)a.most + rows - 1) / rows), 2 * a.pool.H, bsz);
-    if (D == 128) launch_chained(read_kernel<F, 128>, grid, dim3(THREADS), 0, st, a);
-    else launch_chained(read_kernel<F, 64>, grid, dim3(THREADS), 0, st, a);
+void launch_read(const ReadArgs& a, int D, unsigned grid, cudaStream_t st) {
+    if (D == 128) launch_chained(read_kernel<F, 128>, dim3(grid), dim3(THREADS), 0, st, a);
+    else launch_chained(read_kernel<F, 64>, dim3(grid), dim3(THREADS), 0, st, a);
 }
 
 bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
@@ -248,20 +264,24 @@ int akv_paged_append(const akv_pool* pool, const void* k, const void* v, const l
     bool straight = aligned16(k) && aligned16(v) && !misaligned(counts, 4);
     for (int i = 0; i < 6; ++i) straight = straight && strides[i] % 8 == 0;
     AKV_REQUIRE(straight, AKV_ERR_ALIGN, "paged_append: rows of k and v must lie on 16-byte boundaries, counts on 4-byte ones");
-    a.x[0] = static_cast<const __half*>(k);
-    a.x[1] = static_cast<const __half*>(v);
-    for (int w = 0; w < 2; ++w) {
-        a.batch[w] = strides[3 * w];
-        a.token[w] = strides[3 * w + 1];
-        a.head[w] = strides[3 * w + 2];
-    }
+    const int D = pool->head_dim;
+    a.blocks = blocks_of(tokens, D);
+    const long long grid = 2ll * pool->n_kv_heads * bsz * a.blocks;
+    AKV_REQUIRE(grid < INT_MAX, AKV_ERR_OVERFLOW, "paged_append: too many rows");
+    a.k = static_cast<const __half*>(k);
+    a.v = static_cast<const __half*>(v);
+    a.k_batch = strides[0];
+    a.k_token = strides[1];
+    a.k_head = strides[2];
+    a.v_batch = strides[3];
+    a.v_token = strides[4];
+    a.v_head = strides[5];
     a.counts = static_cast<const int*>(counts);
     a.T = tokens;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int D = pool->head_dim;
-    if (pool->format == AKV_PAGE_FP16) launch_append<AKV_PAGE_FP16>(a, D, bsz, st);
-    else if (pool->format == AKV_PAGE_E4M3) launch_append<AKV_PAGE_E4M3>(a, D, bsz, st);
-    else launch_append<AKV_PAGE_E2M1>(a, D, bsz, st);
+    if (pool->format == AKV_PAGE_FP16) launch_append<AKV_PAGE_FP16>(a, D, (unsigned)grid, st);
+    else if (pool->format == AKV_PAGE_E4M3) launch_append<AKV_PAGE_E4M3>(a, D, (unsigned)grid, st);
+    else launch_append<AKV_PAGE_E2M1>(a, D, (unsigned)grid, st);
     return cuda_status(cudaGetLastError(), "paged_append launch");
 }
 
@@ -273,14 +293,17 @@ int akv_paged_read(const akv_pool* pool, const void* pages, const void* lens, vo
     AKV_REQUIRE(k && v, AKV_ERR_NULL, "paged_read: null pointer");
     AKV_REQUIRE(most > 0 && most <= 1 << 30, AKV_ERR_SHAPE, "paged_read: %d tokens", most);
     AKV_REQUIRE(aligned16(k) && aligned16(v), AKV_ERR_ALIGN, "paged_read: k and v must be 16-byte aligned");
-    a.x[0] = static_cast<__half*>(k);
-    a.x[1] = static_cast<__half*>(v);
+    const int D = pool->head_dim;
+    a.blocks = blocks_of(most, D);
+    const long long grid = 2ll * pool->n_kv_heads * bsz * a.blocks;
+    AKV_REQUIRE(grid < INT_MAX, AKV_ERR_OVERFLOW, "paged_read: too many rows");
+    a.k = static_cast<__half*>(k);
+    a.v = static_cast<__half*>(v);
     a.most = most;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int D = pool->head_dim;
-    if (pool->format == AKV_PAGE_FP16) launch_read<AKV_PAGE_FP16>(a, D, bsz, st);
-    else if (pool->format == AKV_PAGE_E4M3) launch_read<AKV_PAGE_E4M3>(a, D, bsz, st);
-    else launch_read<AKV_PAGE_E2M1>(a, D, bsz, st);
+    if (pool->format == AKV_PAGE_FP16) launch_read<AKV_PAGE_FP16>(a, D, (unsigned)grid, st);
+    else if (pool->format == AKV_PAGE_E4M3) launch_read<AKV_PAGE_E4M3>(a, D, (unsigned)grid, st);
+    else launch_read<AKV_PAGE_E2M1>(a, D, (unsigned)grid, st);
     return cuda_status(cudaGetLastError(), "paged_read launch");
 }
 
