@@ -4,8 +4,9 @@
 namespace akv {
 namespace {
 
-constexpr int THREADS = 256, VALUES = 8;       // a thread has 8 channels: 16 bytes of fp16
-constexpr int MANY = 4;                        // rows of a thread, whose loads are on their way together
+constexpr int THREADS = 256;
+constexpr int PIECES = 2, ROWS_EACH = 2;       // a lane's 16-byte pieces of fp16 of a row, its rows; all are on their way together
+template <int D> constexpr int lanes_of = D / (8 * PIECES);    // lanes of a row: lane i has pieces i, i + lanes, ...
 
 struct AppendArgs {
     Pool pool;
@@ -14,8 +15,6 @@ struct AppendArgs {
     const int* counts;
     int T, blocks;                             // blocks of a sequence's tokens
 };
-
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
 // The least e with a <= top 2^add 2^e for the bits of a >= 0 (top's fraction as bits); a = 0 counts as fp16's smallest.
 __device__ __forceinline__ int least_exponent(uint32_t bits, uint32_t top_fraction, int add) {
@@ -29,62 +28,83 @@ __device__ __forceinline__ float quotient(float x, float s, float r) {
     const float y = x * r;
     return fmaf(fmaf(-y, s, x), r, y);
 }
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+__device__ __forceinline__ uint32_t max_of(uint32_t two) { return max(two & 0xFFFFu, two >> 16); }
+// 2^e in both halves, e in -14..15.
+__device__ __forceinline__ uint32_t power2_halves(int e) { return (uint32_t)(e + 15) * 0x04000400u; }
+// Two e4m3 codes of two halves (x, y of a word each): nearest, ties to even.
+__device__ __forceinline__ uint32_t to_e4m3(uint32_t x, uint32_t y) {
+    uint32_t w;
+    asm("{\n.reg .b16 l, u;\ncvt.rn.satfinite.e4m3x2.f16x2 l, %1;\ncvt.rn.satfinite.e4m3x2.f16x2 u, %2;\nmov.b32 %0, {l, u};\n}\n" : "=r"(w) : "r"(x), "r"(y));
+    return w;
+}
 
-// Codes of a lane's 8 channels, by the LANES = D / 8 lanes that have a row; row < 0: takes part in the exchange, stores nothing.
+// Codes of a lane's pieces, by the lanes that have a row; row < 0: takes part in the exchange, stores nothing.
 template <int F, int D>
-__device__ __forceinline__ void store_row(uint8_t* codes, int8_t* exps, uint8_t* scales, long long row, int lane, uint4 raw) {
-    constexpr int LANES = D / VALUES;
+__device__ __forceinline__ void store_row(uint8_t* codes, int8_t* exps, uint8_t* scales, long long row, int lane, const uint4 (&raw)[PIECES]) {
+    constexpr int LANES = lanes_of<D>;
     if constexpr (F == AKV_PAGE_FP16) {
-        if (row >= 0) *reinterpret_cast<uint4*>(codes + row * (2 * D) + lane * 16) = raw;
+#pragma unroll
+        for (int q = 0; q < PIECES; ++q)
+            if (row >= 0) *reinterpret_cast<uint4*>(codes + row * (2 * D) + (lane + q * LANES) * 16) = raw[q];
     } else {
-        float x[VALUES];
+        // magnitudes as 16 bits: NaN is above infinity, infinity above the rest
+        uint32_t pair[PIECES], top = 0;        // (pair: of 16 channels, two neighbouring lanes)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = halves_floats(u4w(raw, i));
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
+        for (int q = 0; q < PIECES; ++q) {
+            constexpr uint32_t ABS = 0x7FFF7FFFu;
+            pair[q] = max_halves(max_halves(raw[q].x & ABS, raw[q].y & ABS), max_halves(raw[q].z & ABS, raw[q].w & ABS));
+            if constexpr (F == AKV_PAGE_E2M1) pair[q] = max_halves(pair[q], __shfl_xor_sync(0xFFFFFFFFu, pair[q], 1));
+            top = max_halves(top, pair[q]);
         }
-        uint32_t top = 0;                      // (as bits: NaN is above infinity, infinity above the rest)
 #pragma unroll
-        for (int i = 0; i < VALUES; ++i) top = max(top, abs_bits(x[i]));
-        const uint32_t pair = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));     // of 16 channels
-        top = pair;
-#pragma unroll
-        for (int o = 2; o < LANES; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        const bool finite = top < 0x7F800000u;
-        const int e = F == AKV_PAGE_E4M3 ? least_exponent(top, 0x600000u, 8) : least_exponent(top, 0x280000u, 11);
-        const float unit = finite ? power2(-e) : 0.f;
+        for (int o = F == AKV_PAGE_E2M1 ? 2 : 1; o < LANES; o <<= 1) top = max_halves(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const uint32_t most = max_of(top);
+        const bool finite = most < 0x7C00u;
+        const uint32_t bits = __float_as_uint(halves_floats(most).x);
+        const int e = F == AKV_PAGE_E4M3 ? least_exponent(bits, 0x600000u, 8) : least_exponent(bits, 0x280000u, 11);
         if (row >= 0 && lane == 0) exps[row] = (int8_t)(finite ? e : EXP_NAN);
         if constexpr (F == AKV_PAGE_E4M3) {
-            uint32_t w[2] = {0, 0};
 #pragma unroll
-            for (int i = 0; i < VALUES; i += 2) {
-                uint16_t c;
-                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(c) : "f"(x[i + 1] * unit), "f"(x[i] * unit));
-                w[i >> 2] |= (uint32_t)c << (8 * (i & 2));
+            for (int q = 0; q < PIECES; ++q) {
+                // Times 2^-e: exact in fp16 where that makes a value larger; where it makes it smaller what gets lost is far below half
+                // the smallest code.  -e beyond fp16 (a row below 2^-5) takes two factors, of the smallest rows three.
+                const uint32_t one = power2_halves(min(-e, 14)), two = power2_halves(min(max(-e - 14, 0), 14));
+                uint32_t x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = hmul2_bits(hmul2_bits(u4w(raw[q], i), one), two);
+                if (e < -28) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = hmul2_bits(x[i], power2_halves(-e - 28));
+                }
+                const uint2 w = make_uint2(to_e4m3(x[0], x[1]), to_e4m3(x[2], x[3]));
+                if (row >= 0) *reinterpret_cast<uint2*>(codes + row * D + (lane + q * LANES) * 8) = finite ? w : make_uint2(0, 0);
             }
-            if (row >= 0) *reinterpret_cast<uint2*>(codes + row * D + lane * VALUES) = finite ? make_uint2(w[0], w[1]) : make_uint2(0, 0);
         } else {
-            uint16_t sc;
-            const float most = finite ? __fdiv_rn(__uint_as_float(pair) * unit, 6.f) : 0.f;
-            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(sc) : "f"(0.f), "f"(most));
-            if (row >= 0 && (lane & 1) == 0) scales[row * (D / 16) + (lane >> 1)] = (uint8_t)sc;
-            const float s = e4m3_float(sc & 0xFFu), r = s > 0.f ? __frcp_rn(s) : 0.f;
-            uint32_t w = 0;
+            const float unit = finite ? power2(e) : 0.f, back = finite ? power2(-e) : 0.f;
 #pragma unroll
-            for (int i = 0; i < VALUES; i += 2) {
-                uint32_t c;
-                asm("{\n.reg .b8 b;\ncvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\ncvt.u32.u8 %0, b;\n}\n"
-                    : "=r"(c) : "f"(quotient(x[i + 1] * unit, s, r)), "f"(quotient(x[i] * unit, s, r)));
-                w |= c << (4 * i);
+            for (int q = 0; q < PIECES; ++q) {
+                uint16_t sc;
+                const float sixth = finite ? __fdiv_rn(halves_floats(max_of(pair[q])).x * back, 6.f) : 0.f;
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(sc) : "f"(0.f), "f"(sixth));
+                if (row >= 0 && (lane & 1) == 0) scales[row * (D / 16) + ((lane + q * LANES) >> 1)] = (uint8_t)sc;
+                const float s = e4m3_float(sc & 0xFFu) * unit, r = s > 0.f ? __frcp_rn(s) : 0.f;
+                uint32_t c[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = halves_floats(u4w(raw[q], i));
+                    asm("{\n.reg .b8 b;\ncvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\ncvt.u32.u8 %0, b;\n}\n"
+                        : "=r"(c[i]) : "f"(quotient(f.y, s, r)), "f"(quotient(f.x, s, r)));
+                }
+                const uint32_t w = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+                if (row >= 0) *reinterpret_cast<uint32_t*>(codes + row * (D / 2) + (lane + q * LANES) * 4) = finite ? w : 0u;
             }
-            if (row >= 0) *reinterpret_cast<uint32_t*>(codes + row * (D / 2) + lane * 4) = finite ? w : 0u;
         }
     }
 }
 
 // What a block has: K and V of all heads side by side, then the next tokens, then the next sequence; so that what is written at one time lies
-// together (hold, e4m3: HEADFIRST us the other way round).
+// together (16 sequences of 1000 tokens, 32 heads: 119 us, one head after the other 140).
 struct Place {
     int b, block, h;
     bool which;
@@ -101,32 +121,31 @@ struct Place {
 // there is much to do.
 template <int F, int D>
 __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
-    constexpr int LANES = D / VALUES, ROWS = THREADS / LANES;
+    constexpr int LANES = lanes_of<D>, ROWS = THREADS / LANES;
     pdl_turn();
     const Pool& p = a.pool;
     const Place at0(p.H, a.blocks);
-    const int b = at0.b, h = at0.h, lane = threadIdx.x % LANES, begin = at0.block * (MANY * ROWS), i0 = begin + threadIdx.x / LANES;
+    const int b = at0.b, h = at0.h, lane = threadIdx.x % LANES, begin = at0.block * (ROWS_EACH * ROWS), i0 = begin + threadIdx.x / LANES;
     const bool which = at0.which;
     const int n = a.counts ? min(a.T, a.counts[b]) : a.T;
     if (begin >= n) return;
     const long long at = max(0, p.lens[b]), room = (long long)p.width << p.shift;
-    const __half* x = (which ? a.v + b * a.v_batch + h * a.v_head : a.k + b * a.k_batch + h * a.k_head) + lane * VALUES;
+    const __half* x = (which ? a.v + b * a.v_batch + h * a.v_head : a.k + b * a.k_batch + h * a.k_head) + lane * 8;
     const long long step = which ? a.v_token : a.k_token;
-    uint4 raw[MANY];
-    long long row[MANY];
+    uint4 raw[ROWS_EACH][PIECES];
+    long long row[ROWS_EACH];
 #pragma unroll
-    for (int m = 0; m < MANY; ++m) {
+    for (int m = 0; m < ROWS_EACH; ++m) {
         const int i = i0 + m * ROWS;
-        raw[m] = make_uint4(0, 0, 0, 0);
-        row[m] = -1;
-        if (i < n && at + i < room) {
-            raw[m] = __ldg(reinterpret_cast<const uint4*>(x + i * step));
-            row[m] = pool_row(p, b, h, at + i);
-        }
+        const bool there = i < n && at + i < room;
+#pragma unroll
+        for (int q = 0; q < PIECES; ++q)
+            raw[m][q] = there ? __ldg(reinterpret_cast<const uint4*>(x + i * step + q * LANES * 8)) : make_uint4(0, 0, 0, 0);
+        row[m] = there ? pool_row(p, b, h, at + i) : -1;
     }
 #pragma unroll
-    for (int m = 0; m < MANY; ++m)
-        if (begin + m * ROWS < n)        // (the same for the block)
+    for (int m = 0; m < ROWS_EACH; ++m)
+        if (begin + m * ROWS < n)              // (the same for the block)
             store_row<F, D>(which ? p.vc : p.kc, which ? p.ve : p.ke, which ? p.vs : p.ks, row[m], lane, raw[m]);
 }
 
@@ -141,73 +160,87 @@ struct ReadArgs {
 
 template <int F, int D>
 __global__ void __launch_bounds__(THREADS) read_kernel(ReadArgs a) {
-    constexpr int LANES = D / VALUES, ROWS = THREADS / LANES;
+    constexpr int LANES = lanes_of<D>, ROWS = THREADS / LANES, PIECE = row_bytes<F>(D) / (LANES * PIECES);
     pdl_turn();
     const Pool& p = a.pool;
     const Place at0(p.H, a.blocks);
-    const int b = at0.b, h = at0.h, lane = threadIdx.x % LANES, i0 = at0.block * (MANY * ROWS) + threadIdx.x / LANES;
+    const int b = at0.b, h = at0.h, lane = threadIdx.x % LANES, i0 = at0.block * (ROWS_EACH * ROWS) + threadIdx.x / LANES;
     const bool which = at0.which;
     const int n = length_of(p, b);
-    __half* out = which ? a.v : a.k;
-    const uint8_t* codes = (which ? p.vc : p.kc) + lane * (row_bytes<F>(D) / LANES);
-    uint4 w[MANY];
-    int exponent[MANY];
-    uint32_t scale[MANY];
+    const uint8_t *codes = (which ? p.vc : p.kc) + lane * PIECE, *scales = which ? p.vs : p.ks;
+    const int8_t* exps = which ? p.ve : p.ke;
+    __half* out = (which ? a.v : a.k) + lane * 8;
+    uint4 w[ROWS_EACH][PIECES];
+    int exponent[ROWS_EACH];
+    uint32_t scale[ROWS_EACH][PIECES];
 #pragma unroll
-    for (int m = 0; m < MANY; ++m) {
+    for (int m = 0; m < ROWS_EACH; ++m) {
         const int i = i0 + m * ROWS;
         const long long row = i < n && i < a.most ? pool_row(p, b, h, i) : -1;
-        w[m] = make_uint4(0, 0, 0, 0);
         exponent[m] = 0;
-        scale[m] = 0;
-        if (row >= 0) {
-            if constexpr (F == AKV_PAGE_FP16) {
-                w[m] = __ldg(reinterpret_cast<const uint4*>(codes + row * (2 * D)));
-            } else {
-                if constexpr (F == AKV_PAGE_E4M3) {
-                    const uint2 x = __ldg(reinterpret_cast<const uint2*>(codes + row * D));
-                    w[m].x = x.x;
-                    w[m].y = x.y;
+#pragma unroll
+        for (int q = 0; q < PIECES; ++q) {
+            w[m][q] = make_uint4(0, 0, 0, 0);
+            scale[m][q] = 0;
+            if (row >= 0) {
+                const uint8_t* x = codes + row * row_bytes<F>(D) + q * LANES * PIECE;
+                if constexpr (F == AKV_PAGE_FP16) {
+                    w[m][q] = __ldg(reinterpret_cast<const uint4*>(x));
+                } else if constexpr (F == AKV_PAGE_E4M3) {
+                    const uint2 y = __ldg(reinterpret_cast<const uint2*>(x));
+                    w[m][q].x = y.x;
+                    w[m][q].y = y.y;
                 } else {
-                    w[m].x = __ldg(reinterpret_cast<const uint32_t*>(codes + row * (D / 2)));
-                    scale[m] = __ldg((which ? p.vs : p.ks) + row * (D / 16) + (lane >> 1));
+                    w[m][q].x = __ldg(reinterpret_cast<const uint32_t*>(x));
+                    scale[m][q] = __ldg(scales + row * (D / 16) + ((lane + q * LANES) >> 1));
                 }
-                exponent[m] = __ldg((which ? p.ve : p.ke) + row);
             }
         }
+        if (F != AKV_PAGE_FP16 && row >= 0) exponent[m] = __ldg(exps + row);
     }
 #pragma unroll
-    for (int m = 0; m < MANY; ++m) {
+    for (int m = 0; m < ROWS_EACH; ++m) {
         const int i = i0 + m * ROWS;
         if (i >= a.most) continue;
-        if constexpr (F != AKV_PAGE_FP16) {
-            const float unit = power2(exponent[m]);
-            float s = 1.f;                     // (multiplied first: codes times scales are exact, and far from fp32's ends)
-            uint32_t h2[4];
-            if constexpr (F == AKV_PAGE_E4M3) {
-                uint32_t x[2], y[2];
-                e4m3_word(x, w[m].x);
-                e4m3_word(y, w[m].y);
-                h2[0] = x[0]; h2[1] = x[1]; h2[2] = y[0]; h2[3] = y[1];
-            } else {
-                s = e4m3_float(scale[m]);
-                e2m1_word(h2, w[m].x);
-            }
-            uint32_t o[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float2 f = halves_floats(h2[k]);
-                const __half2 r = __floats2half2_rn(saturated(f.x * s * unit), saturated(f.y * s * unit));
-                o[k] = *reinterpret_cast<const uint32_t*>(&r);
+        for (int q = 0; q < PIECES; ++q) {
+            if constexpr (F != AKV_PAGE_FP16) {
+                uint32_t x[4], s = 0;
+                if constexpr (F == AKV_PAGE_E4M3) {
+                    uint32_t y[2], z[2];
+                    e4m3_word(y, w[m][q].x);
+                    e4m3_word(z, w[m][q].y);
+                    x[0] = y[0]; x[1] = y[1]; x[2] = z[0]; x[3] = z[1];
+                } else {
+                    s = e4m3_halves(scale[m][q] * 0x0101u);
+                    e2m1_word(x, w[m][q].x);
+                }
+                // In fp16 where the factor and every product fit it (448 * 2^7, 6 * 448 * 2^4; down to 2^-14 all are exact), else in fp32.
+                if (exponent[m] >= -14 && exponent[m] <= (F == AKV_PAGE_E4M3 ? 7 : 4)) {
+                    const uint32_t unit = power2_halves(exponent[m]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] = hmul2_bits(F == AKV_PAGE_E2M1 ? hmul2_bits(x[k], s) : x[k], unit);
+                } else {
+                    const float unit = power2(exponent[m]), f = F == AKV_PAGE_E2M1 ? halves_floats(s).x : 1.f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 y = halves_floats(x[k]);
+                        const __half2 r = __floats2half2_rn(saturated(y.x * f * unit), saturated(y.y * f * unit));
+                        x[k] = *reinterpret_cast<const uint32_t*>(&r);
+                    }
+                }
+                w[m][q] = make_uint4(x[0], x[1], x[2], x[3]);
             }
-            w[m] = make_uint4(o[0], o[1], o[2], o[3]);
+            __stcs(reinterpret_cast<uint4*>(out + (((long long)b * a.most + i) * p.H + h) * D + q * LANES * 8), w[m][q]);
         }
-        __stcs(reinterpret_cast<uint4*>(out + (((long long)b * a.most + i) * p.H + h) * D) + lane, w[m]);
     }
 }
 
 // Blocks of a sequence's `tokens`; blocks of all (b, head, tensor) may not fit a grid.
-int blocks_of(int tokens, int D) { return (tokens + MANY * (THREADS / (D / VALUES)) - 1) / (MANY * (THREADS / (D / VALUES))); }
+int blocks_of(int tokens, int D) {
+    const int rows = ROWS_EACH * THREADS / (D / (8 * PIECES));
+    return (tokens + rows - 1) / rows;
+}
 template <int F>
 void launch_append(const AppendArgs& a, int D, unsigned grid, cudaStream_t st) {
     if (D == 128) launch_chained(append_kernel<F, 128>, dim3(grid), dim3(THREADS), 0, st, a);
