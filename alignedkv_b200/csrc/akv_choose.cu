@@ -67,10 +67,9 @@ __device__ __forceinline__ uint32_t there(const void* p, int cta) {
 template <class P, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
     constexpr int E = 16 / sizeof(P), STEP = 32 * E;
-    __shared__ double s_sum[WARPS], s_cta[2][MOST_CTAS];
-    __shared__ int s_up[MOST], s_gone[MOST], s_first, s_last;
+    __shared__ double s_sum[WARPS], s_step[WARPS], s_cta[2][MOST_CTAS];
+    __shared__ int s_up[MOST], s_x[MOST], s_first, s_last, s_mine;     // (s_x: -1 outside the vocabulary)
     __shared__ float s_p[MOST], s_q[MOST], s_u[MOST];
-    __shared__ long long s_x[MOST];
     const int ctas = a.ctas, rank = blockIdx.x % ctas, b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int T = a.T, V = a.V;
     pdl_turn();
@@ -79,36 +78,36 @@ __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
     if (tid < T) {
         const int up = tid == 0 ? -1 : a.parents ? a.parents[b * a.parents_batch + tid] : tid - 1;
         const long long x = a.ids[(long long)b * T + tid];
-        const bool asked = up >= 0 && up < tid && x >= 0 && x < V;
-        s_up[tid] = up;
-        s_x[tid] = x;
+        const bool word = x >= 0 && x < V, asked = up >= 0 && up < tid && word;
+        s_up[tid] = up < tid ? up : -1;
+        s_x[tid] = word ? (int)x : -1;
         s_u[tid] = a.coins[(long long)b * T + tid];
         s_p[tid] = asked ? chance(as_float(target[up * a.target_row + x])) : 0.f;
         s_q[tid] = asked && draft ? chance(as_float(draft[up * a.draft_row + x])) : 0.f;
     }
     if (tid == 0) {
-        s_first = V;
+        s_first = s_mine = V;
         s_last = -1;
     }
     __syncthreads();
     // parts of whole steps; this warp's begins at `first`
     const int steps = (V + STEP - 1) / STEP, each = (steps + ctas * WARPS - 1) / (ctas * WARPS);
     const int first = min(V, (rank * WARPS + warp) * each * STEP), last = min(V, first + each * STEP);
-    int now = 0, count = 1, gone = 0, turn = 0;
+    int now = 0, count = 1, turn = 0;
+    unsigned long long gone = 0;               // bits: guesses that were rejected at this node
     double c = 0.0, left = 1.0;
     if (tid == 0 && rank == 0) a.path[(long long)b * T] = 0;
-    // what is left of E probabilities from j on
+    // what is left of E probabilities from j on, in the step that begins with j0
     auto rest = [&](double (&r)[E], int j, int j0) {
-        float x[E];
+        float x[E], y[E];
         load<P, VEC>(x, target + now * a.target_row, j, V);
         if (c > 0.0) {
-            float y[E];
             load<P, VEC>(y, draft + now * a.draft_row, j, V);
 #pragma unroll
             for (int i = 0; i < E; ++i) r[i] = fmax(fma(-c, (double)y[i], (double)x[i]), 0.0);
         } else {
-            for (int g = 0; g < gone; ++g) {
-                const int k = s_gone[g] - j0;
+            for (unsigned long long g = gone; g; g &= g - 1) {
+                const int k = s_x[__ffsll(g) - 1] - j0;
                 if (k >= 0 && k < STEP)
 #pragma unroll
                     for (int i = 0; i < E; ++i)
@@ -120,7 +119,7 @@ __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
     };
     auto total = [&]() -> double {
         double sum = 0.0;
-#pragma unroll 2
+#pragma unroll 4
         for (int j0 = first; j0 < last; j0 += STEP) {
             double r[E];
             rest(r, j0 + lane * E, j0);
@@ -141,37 +140,40 @@ __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
         for (int i = 0; i < ctas; ++i) sum += s_cta[turn][i];
         return sum;
     };
-    for (int i = 1; i < T; ++i) {
-        if (s_up[i] != now) continue;
-        const double u = s_u[i], p = s_p[i], q = s_q[i];
-        bool good;
-        if (draft) {
-            good = u * left * q < fmax(fma(-c, q, p), 0.0);
-        } else {
-            double r = p;
-            for (int g = 0; g < gone; ++g)
-                if (s_gone[g] == s_x[i]) r = 0.0;
-            good = u * left < r;
-            if (!good) {
-                left -= r;
-                __syncthreads();
-                if (tid == 0) s_gone[gone] = s_x[i] >= 0 && s_x[i] < V ? (int)s_x[i] : -1;
-                ++gone;
-                __syncthreads();
+    // Every warp walks by itself, its lanes holding the nodes' parents.
+    const int up0 = lane < T ? s_up[lane] : -1, up1 = lane + 32 < T ? s_up[lane + 32] : -1;
+    for (bool on = true; on;) {
+        on = false;
+        unsigned long long children = __ballot_sync(0xFFFFFFFFu, up0 == now) | (unsigned long long)__ballot_sync(0xFFFFFFFFu, up1 == now) << 32;
+        while (children) {
+            const int i = __ffsll(children) - 1;
+            children &= children - 1;
+            const double u = s_u[i], p = s_p[i], q = s_q[i];
+            if (draft) {
+                on = u * left * q < fmax(fma(-c, q, p), 0.0);
+            } else {
+                double r = p;
+                for (unsigned long long g = gone; g; g &= g - 1)
+                    if (s_x[__ffsll(g) - 1] == s_x[i]) r = 0.0;
+                on = u * left < r;
+                if (!on) {
+                    left -= r;
+                    gone |= 1ull << i;
+                }
             }
-        }
-        if (good) {
-            now = i;
-            c = 0.0;
-            left = 1.0;
-            gone = 0;
-            if (tid == 0 && rank == 0) a.path[(long long)b * T + count] = i;
-            ++count;
-        } else if (draft) {
-            c += left;
-            bool again = false;                // (the sum behind the last child is formed below)
-            for (int k = i + 1; k < T; ++k) again |= s_up[k] == now;
-            if (again) left = total();
+            if (on) {
+                now = i;
+                c = 0.0;
+                left = 1.0;
+                gone = 0;
+                if (tid == 0 && rank == 0) a.path[(long long)b * T + count] = i;
+                ++count;
+                break;
+            }
+            if (draft) {
+                c += left;
+                if (children) left = total();  // (the sum behind the last child is formed below)
+            }
         }
     }
     double sum = total();
@@ -187,11 +189,24 @@ __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
     const double at = (double)fmaxf(s_u[0], 0.f) * sum;
     double before = 0.0;
     for (int i = 0; i < rank; ++i) before += s_cta[turn][i];
-    for (int w = 0; w < warp; ++w) before += s_sum[w];
-    if (before <= at && before + s_sum[warp] > at) {
-        for (int j0 = first; j0 < last; j0 += STEP) {
+    // The warp's part in which `at` falls; the CTA looks through it together, a step per warp.
+    int owner = -1;
+    for (int w = 0; w < WARPS; ++w) {
+        const double next = before + s_sum[w];
+        if (before <= at && next > at) {
+            owner = w;
+            break;
+        }
+        before = next;
+    }
+    if (owner >= 0) {
+        const int from = min(V, (rank * WARPS + owner) * each * STEP), to = min(V, from + each * STEP);
+        for (int j1 = from; j1 < to; j1 += WARPS * STEP) {
+            const int j0 = j1 + warp * STEP;
             double r[E], x = 0.0;
-            rest(r, j0 + lane * E, j0);
+#pragma unroll
+            for (int i = 0; i < E; ++i) r[i] = 0.0;
+            if (j0 < to) rest(r, j0 + lane * E, j0);
 #pragma unroll
             for (int i = 0; i < E; ++i) x += r[i];
             const double own = x;
@@ -200,22 +215,26 @@ __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
                 const double y = __shfl_up_sync(0xFFFFFFFFu, x, o);
                 if (lane >= o) x += y;
             }
-            if (__any_sync(0xFFFFFFFFu, before + x > at)) {
-                double z = before + (x - own);
-                int found = V;
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    z += r[i];
-                    if (found == V && r[i] > 0.0 && z > at) found = j0 + lane * E + i;
-                }
-                found = __reduce_min_sync(0xFFFFFFFFu, found);
-                if (found < V) {
-                    if (lane == 0) asm volatile("red.shared::cluster.min.s32 [%0], %1;\n" ::"r"(there(&s_first, 0)), "r"(found) : "memory");
-                    break;
-                }
+            if (lane == 31) s_step[warp] = x;
+            __syncthreads();
+            double z = before;
+            for (int w = 0; w < WARPS; ++w) {
+                if (w < warp) z += s_step[w];
+                before += s_step[w];
             }
-            before += __shfl_sync(0xFFFFFFFFu, x, 31);
+            z += x - own;
+            int found = V;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                z += r[i];
+                if (found == V && r[i] > 0.0 && z > at) found = j0 + lane * E + i;
+            }
+            found = __reduce_min_sync(0xFFFFFFFFu, found);
+            if (lane == 0 && found < V) atomicMin(&s_mine, found);
+            __syncthreads();
+            if (s_mine < V) break;
         }
+        if (tid == 0 && s_mine < V) asm volatile("red.shared::cluster.min.s32 [%0], %1;\n" ::"r"(there(&s_first, 0)), "r"(s_mine) : "memory");
     }
     cluster_sync();
     int found;
