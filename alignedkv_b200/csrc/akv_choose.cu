@@ -31,22 +31,28 @@ struct ChooseArgs {
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-// What is no probability counts as none.
-__device__ __forceinline__ float chance(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
+// What is no probability counts as none: negative, infinite, NaN (as bits all are above the largest finite value).
+__device__ __forceinline__ float chance(float x) { return __float_as_uint(x) < 0x7F800000u ? x : 0.f; }
+__device__ __forceinline__ double left_of(double p, double c, double q) {
+    const double r = fma(-c, q, p);
+    return r > 0.0 ? r : 0.0;
+}
 
-// E = 16 bytes of probabilities from j on (zeros behind V).  VEC: rows begin on 16-byte boundaries.
+// E = 16 bytes of probabilities from j on (zeros behind `end`).  VEC: rows begin on 16-byte boundaries.
 template <class P, bool VEC>
-__device__ __forceinline__ void load(float (&x)[16 / sizeof(P)], const P* row, int j, int V) {
+__device__ __forceinline__ uint4 load(const P* row, int j, int end) {
     constexpr int E = 16 / sizeof(P);
-    if (VEC && j + E <= V) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + j));
-        const P* e = reinterpret_cast<const P*>(&w);
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (VEC && j + E <= end) return __ldg(reinterpret_cast<const uint4*>(row + j));
+    P* e = reinterpret_cast<P*>(&w);
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = chance(as_float(e[i]));
-    } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = j + i < V ? chance(as_float(row[j + i])) : 0.f;
-    }
+    for (int i = 0; i < E; ++i)
+        if (j + i < end) e[i] = row[j + i];
+    return w;
+}
+template <class P>
+__device__ __forceinline__ float element(const uint4& w, int i) {
+    return chance(as_float(reinterpret_cast<const P*>(&w)[i]));
 }
 
 __device__ __forceinline__ double warp_sum(double x) {
@@ -68,7 +74,7 @@ template <class P, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
     constexpr int E = 16 / sizeof(P), STEP = 32 * E;
     __shared__ double s_sum[WARPS], s_step[WARPS], s_cta[2][MOST_CTAS];
-    __shared__ int s_up[MOST], s_x[MOST], s_first, s_last, s_mine;     // (s_x: -1 outside the vocabulary)
+    __shared__ int s_up[MOST], s_x[MOST], s_first, s_mine;     // (s_x: -1 outside the vocabulary)
     __shared__ float s_p[MOST], s_q[MOST], s_u[MOST];
     const int ctas = a.ctas, rank = blockIdx.x % ctas, b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int T = a.T, V = a.V;
@@ -85,9 +91,12 @@ __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
         s_p[tid] = asked ? chance(as_float(target[up * a.target_row + x])) : 0.f;
         s_q[tid] = asked && draft ? chance(as_float(draft[up * a.draft_row + x])) : 0.f;
     }
-    if (tid == 0) {
-        s_first = s_mine = V;
-        s_last = -1;
+    if (tid == 0) s_first = s_mine = V;
+    __syncthreads();
+    if (!draft && tid < T) {                   // a guess that was made and rejected before has nothing left
+        bool twice = false;
+        for (int k = 1; k < tid; ++k) twice |= s_up[k] == s_up[tid] && s_x[k] == s_x[tid];
+        if (twice) s_p[tid] = 0.f;
     }
     __syncthreads();
     // parts of whole steps; this warp's begins at `first`
@@ -98,31 +107,48 @@ __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
     double c = 0.0, left = 1.0;
     if (tid == 0 && rank == 0) a.path[(long long)b * T] = 0;
     // what is left of E probabilities from j on, in the step that begins with j0
-    auto rest = [&](double (&r)[E], int j, int j0) {
-        float x[E], y[E];
-        load<P, VEC>(x, target + now * a.target_row, j, V);
+    auto rest = [&](double (&r)[E], int j, int j0, int end) {
+        const uint4 x = load<P, VEC>(target + now * a.target_row, j, end);
         if (c > 0.0) {
-            load<P, VEC>(y, draft + now * a.draft_row, j, V);
+            const uint4 y = load<P, VEC>(draft + now * a.draft_row, j, end);
 #pragma unroll
-            for (int i = 0; i < E; ++i) r[i] = fmax(fma(-c, (double)y[i], (double)x[i]), 0.0);
+            for (int i = 0; i < E; ++i) r[i] = left_of(element<P>(x, i), c, element<P>(y, i));
         } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) r[i] = element<P>(x, i);
             for (unsigned long long g = gone; g; g &= g - 1) {
                 const int k = s_x[__ffsll(g) - 1] - j0;
                 if (k >= 0 && k < STEP)
 #pragma unroll
                     for (int i = 0; i < E; ++i)
-                        if (k == j - j0 + i) x[i] = 0.f;
+                        if (k == j - j0 + i) r[i] = 0.0;
             }
-#pragma unroll
-            for (int i = 0; i < E; ++i) r[i] = x[i];
         }
     };
     auto total = [&]() -> double {
+        constexpr int BATCH = 4;               // steps whose loads are on their way together
         double sum = 0.0;
-#pragma unroll 4
-        for (int j0 = first; j0 < last; j0 += STEP) {
+        int j0 = first;
+        if (VEC && c > 0.0) {
+            const P *x = target + now * a.target_row + lane * E, *y = draft + now * a.draft_row + lane * E;
+#pragma unroll 1
+            for (; j0 + BATCH * STEP <= last; j0 += BATCH * STEP) {
+                uint4 p[BATCH], q[BATCH];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    p[k] = __ldg(reinterpret_cast<const uint4*>(x + j0 + k * STEP));
+                    q[k] = __ldg(reinterpret_cast<const uint4*>(y + j0 + k * STEP));
+                }
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) sum += left_of(element<P>(p[k], i), c, element<P>(q[k], i));
+            }
+        }
+#pragma unroll 2
+        for (; j0 < last; j0 += STEP) {
             double r[E];
-            rest(r, j0 + lane * E, j0);
+            rest(r, j0 + lane * E, j0, last);
 #pragma unroll
             for (int i = 0; i < E; ++i) sum += r[i];
         }
@@ -150,14 +176,11 @@ __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
             children &= children - 1;
             const double u = s_u[i], p = s_p[i], q = s_q[i];
             if (draft) {
-                on = u * left * q < fmax(fma(-c, q, p), 0.0);
+                on = u * left * q < left_of(p, c, q);
             } else {
-                double r = p;
-                for (unsigned long long g = gone; g; g &= g - 1)
-                    if (s_x[__ffsll(g) - 1] == s_x[i]) r = 0.0;
-                on = u * left < r;
+                on = u * left < p;
                 if (!on) {
-                    left -= r;
+                    left -= p;
                     gone |= 1ull << i;
                 }
             }
@@ -206,7 +229,7 @@ __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
             double r[E], x = 0.0;
 #pragma unroll
             for (int i = 0; i < E; ++i) r[i] = 0.0;
-            if (j0 < to) rest(r, j0 + lane * E, j0);
+            if (j0 < to) rest(r, j0 + lane * E, j0, to);
 #pragma unroll
             for (int i = 0; i < E; ++i) x += r[i];
             const double own = x;
@@ -236,36 +259,44 @@ __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
         }
         if (tid == 0 && s_mine < V) asm volatile("red.shared::cluster.min.s32 [%0], %1;\n" ::"r"(there(&s_first, 0)), "r"(s_mine) : "memory");
     }
-    cluster_sync();
-    int found;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(found) : "r"(there(&s_first, 0)) : "memory");
-    cluster_sync();
-    if (found == V && sum > 0.0) {
-        // A random number at the end, or between two parts whose sums were rounded: the first entry behind it, else the last in front of it.
+    // The first CTA waits for the others and has the rest to itself.
+    __syncthreads();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    if (rank != 0) return;
+    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    if (s_first == V && sum > 0.0 && warp == 0) {
+        // A random number of 1, or one between two parts whose sums were rounded: one warp adds up the row from its beginning, so that nothing lies
+        // between; where that does not reach the number, the last entry.  Rare.
         before = 0.0;
-        for (int i = 0; i < rank; ++i) before += s_cta[turn][i];
-        for (int w = 0; w < warp; ++w) before += s_sum[w];
         int low = V, high = -1;
-        for (int j0 = first; j0 < last; j0 += STEP) {
-            double r[E];
-            rest(r, j0 + lane * E, j0);
+        for (int j0 = 0; j0 < V && low == V; j0 += STEP) {
+            double r[E], x = 0.0;
+            rest(r, j0 + lane * E, j0, V);
 #pragma unroll
-            for (int i = 0; i < E; ++i)
+            for (int i = 0; i < E; ++i) x += r[i];
+            const double own = x;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+                if (lane >= o) x += y;
+            }
+            double z = before + (x - own);
+            int found = V, last_one = -1;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                z += r[i];
                 if (r[i] > 0.0) {
-                    const int j = j0 + lane * E + i;
-                    if (before > at) low = min(low, j);
-                    else high = max(high, j);
+                    last_one = j0 + lane * E + i;
+                    if (found == V && z > at) found = last_one;
                 }
+            }
+            low = __reduce_min_sync(0xFFFFFFFFu, found);
+            high = max(high, __reduce_max_sync(0xFFFFFFFFu, last_one));
+            before += __shfl_sync(0xFFFFFFFFu, x, 31);
         }
-        low = __reduce_min_sync(0xFFFFFFFFu, low);
-        high = __reduce_max_sync(0xFFFFFFFFu, high);
-        if (lane == 0) {
-            asm volatile("red.shared::cluster.min.s32 [%0], %1;\n" ::"r"(there(&s_first, 0)), "r"(low) : "memory");
-            asm volatile("red.shared::cluster.max.s32 [%0], %1;\n" ::"r"(there(&s_last, 0)), "r"(high) : "memory");
-        }
-        cluster_sync();
+        if (lane == 0) s_first = low < V ? low : high;
     }
-    if (rank == 0 && tid == 0) a.token[b] = !(sum > 0.0) ? -1 : s_first < V ? s_first : s_last;
+    if (tid == 0) a.token[b] = sum > 0.0 ? s_first : -1;
 }
 
 template <class P>
