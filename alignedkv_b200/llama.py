@@ -16,9 +16,10 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from . import _lib, cache_ops
+from . import _lib, cache_ops, paged_ops
 from .decode import DecodeLayer
-from .extension._planes import observed
+from .extension._planes import cdiv, observed
+from .paged import PagedLayer, PageTable
 
 __all__ = ["LlamaConfig", "LlamaDecoder"]
 
@@ -44,11 +45,11 @@ def _rms_norm(x, w, eps):
 
 
 def _rope_tables(pos, D, theta):
-    """cos / signed sin tables [1,S,1,D] (fp32) of the rotate_half form of the rotary embedding (as HF Llama)."""
+    """cos / signed sin tables [1,S,1,D] (fp32) of the rotate_half form of the rotary embedding (as HF Llama); [B,S,1,D] of positions [B,S]."""
     inv = 1.0 / (theta ** (torch.arange(0, D, 2, device=pos.device, dtype=torch.float32) / D))
-    ang = pos.float()[:, None] * inv[None, :]                       # S, D/2
-    cos = torch.cat([ang.cos(), ang.cos()], -1)[None, :, None, :]
-    sin = torch.cat([-ang.sin(), ang.sin()], -1)[None, :, None, :]  # sign of rotate_half folded in
+    ang = (pos if pos.dim() == 2 else pos[None]).float()[..., None] * inv      # B or 1, S, D/2
+    cos = torch.cat([ang.cos(), ang.cos()], -1)[:, :, None, :]
+    sin = torch.cat([-ang.sin(), ang.sin()], -1)[:, :, None, :]     # sign of rotate_half folded in
     return cos, sin
 
 
@@ -67,13 +68,17 @@ def _plain(x: torch.Tensor) -> bool:
 
 
 class LlamaDecoder:
-    """Random-init Llama decoder with one AlignedKV `DecodeLayer` per transformer layer."""
+    """Random-init Llama decoder with one AlignedKV `DecodeLayer` per transformer layer.
+
+    attention="paged" instead keeps the tokens in the pages of one `PagedLayer` per layer (kv_format "fp16", "e4m3" or "e2m1", n_pages of page_size
+    tokens; by default enough for all sequences) behind one `PageTable`: sequences then have lengths of their own.  attention="dense" is
+    fp16 torch attention over a plain cache."""
 
     def __init__(self, cfg: LlamaConfig, bsz: int, max_seq_len: int, device, seed: int = 0, v_mode: str = "exact",
-                 attention: str = "alignedkv"):
+                 attention: str = "alignedkv", kv_format: str = "e4m3", page_size: int = 64, n_pages: int | None = None):
         self.cfg, self.B, self.L = cfg, bsz, max_seq_len
         self.device = torch.device(device)
-        self.attention = attention                  # "alignedkv" or "dense" (fp16 torch attention over a plain cache)
+        self.attention = attention
         g = torch.Generator(device=self.device).manual_seed(seed)
         H, Hkv, D, E, Fi = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, cfg.hidden_size, \
             cfg.intermediate_size
@@ -93,6 +98,10 @@ class LlamaDecoder:
         if attention == "alignedkv":
             self.caches = [DecodeLayer(bsz, max_seq_len, Hkv, D, self.device, n_q_heads=H, v_mode=v_mode)
                            for _ in range(cfg.num_hidden_layers)]
+        elif attention == "paged":
+            n_pages = bsz * cdiv(max_seq_len, page_size) if n_pages is None else n_pages
+            self.table = PageTable(bsz, max_seq_len, n_pages, page_size, self.device)
+            self.caches = [PagedLayer(n_pages, page_size, Hkv, D, self.device, kv_format) for _ in range(cfg.num_hidden_layers)]
         else:
             self.kcache = [torch.zeros(bsz, max_seq_len, Hkv, D, dtype=torch.half, device=self.device)
                            for _ in range(cfg.num_hidden_layers)]
@@ -239,10 +248,65 @@ class LlamaDecoder:
         x = _rms_norm(x[:, -1:], self.final_norm, self.cfg.rms_norm_eps)
         return F.linear(x, self.lm_head)[:, 0]                                   # logits of the last position [B,V]
 
+    # ------------------------------------------------------------------ any number of tokens
+    def _around(self, p: dict, x: torch.Tensor, tables: tuple, attend) -> torch.Tensor:
+        """One layer with `attend(q, k, v)` for its attention."""
+        cfg = self.cfg
+        H, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        B, T, _ = x.shape
+        qkv = F.linear(_rms_norm(x, p["norm1"], cfg.rms_norm_eps), p["wqkv"]).view(B, T, H + 2 * Hkv, D)
+        qk = _rope(qkv[:, :, :H + Hkv], tables)
+        o = attend(qk[:, :, :H].contiguous(), qk[:, :, H:], qkv[:, :, H + Hkv:])
+        x = torch.addmm(x.view(B * T, -1), o.reshape(B * T, H * D), p["wo"].t()).view(B, T, -1)
+        gate, wide = F.linear(_rms_norm(x, p["norm2"], cfg.rms_norm_eps), p["w_gate_up"]).chunk(2, dim=-1)
+        return torch.addmm(x.view(B * T, -1), F.silu(gate).mul_(wide).view(B * T, -1), p["w_down"].t()).view(B, T, -1)
+
+    def _paged(self, ids: torch.Tensor, counts: list, prompt: bool) -> torch.Tensor:
+        """Hidden states [B,T,E] of the next tokens, of which counts[b] are sequence b's: they enter the pages, and attend to what the pages then
+        hold - a piece of a prompt by dense attention over it as it is read back, few tokens through the pages.  The table does not
+        count them yet."""
+        B, T = ids.shape
+        table, H = self.table, self.cfg.num_attention_heads
+        table.reserve(counts)
+        new = torch.tensor(counts, dtype=torch.int32, device=self.device)
+        after = table.lens + new
+        at = table.lens[:, None] + torch.arange(T, device=self.device)
+        tables = _rope_tables(at, self.cfg.head_dim, self.cfg.rope_theta)
+        if prompt:
+            most = max(n + c for n, c in zip(table.lengths, counts))
+            seen = (torch.arange(most, device=self.device) <= at[:, :, None])[:, None]
+        x = self.embed[ids]
+        for p, cache in zip(self.layers, self.caches):
+            def attend(q, k, v):
+                cache.append(k, v, table, new)
+                if not prompt:
+                    return cache.attention(q, table, after)
+                kk, vv = (t.transpose(1, 2).repeat_interleave(H // t.shape[2], dim=1) for t in cache.read(table, most, after))
+                return F.scaled_dot_product_attention(q.transpose(1, 2), kk, vv, attn_mask=seen).transpose(1, 2)
+            x = self._around(p, x, tables, attend)
+        return x
+
+    def _logits(self, x: torch.Tensor) -> torch.Tensor:
+        return F.linear(_rms_norm(x, self.final_norm, self.cfg.rms_norm_eps), self.lm_head)
+
     # ------------------------------------------------------------------ public
     @torch.no_grad()
-    def prefill(self, ids: torch.Tensor) -> torch.Tensor:
-        """ids [B,S] -> logits [B,V] of the last prompt position; fills every layer's cache."""
+    def prefill(self, ids: torch.Tensor, lens: list | None = None) -> torch.Tensor:
+        """ids [B,S] -> logits [B,V] of the last prompt position; fills every layer's cache.
+
+        With attention="paged" sequences may differ: lens (numbers, one per sequence) says how many of its S tokens each one has, and further
+        calls append further pieces; a sequence without tokens in a call has no meaningful logits there."""
+        if self.attention == "paged":
+            B, S = ids.shape
+            counts = [S] * B if lens is None else [int(n) for n in lens]
+            if B != self.B or len(counts) != B or not all(0 <= n <= S for n in counts):
+                raise RuntimeError(f"prefill: expected ids of {self.B} sequences and for each how many of them it has")
+            x = self._paged(ids, counts, True)
+            self.table.advance(counts)
+            self._drafts = None
+            last = torch.tensor([max(0, n - 1) for n in counts], device=self.device)
+            return self._logits(x[torch.arange(B, device=self.device), last][:, None])[:, 0]
+        assert lens is None, "sequences have lengths of their own with attention='paged' only"
         assert self.pos == 0 and ids.shape[0] == self.B and ids.shape[1] <= self.L
         self._drafts = None
         return self._forward(ids, True)
@@ -251,6 +315,11 @@ class LlamaDecoder:
     def step(self, ids: torch.Tensor) -> torch.Tensor:
         """ids [B] (one token per sequence) -> logits [B,V]; appends to every layer's cache.  Drafts of an earlier `verify` are
         dropped: their keys were made for the position that this token takes."""
+        if self.attention == "paged":
+            x = self._paged(ids.view(self.B, 1), [1] * self.B, False)
+            self.table.advance(1)
+            self._drafts = None
+            return self._logits(x)[:, 0]
         assert (self.caches[0].cache_len if self.attention == "alignedkv" else self.pos) + 1 <= self.L
         self._drafts = None
         if getattr(self, "_segs", None) is not None:
@@ -258,17 +327,27 @@ class LlamaDecoder:
         return self._forward(ids.view(self.B, 1), False)
 
     @torch.no_grad()
-    def verify(self, ids: torch.Tensor, parents: torch.Tensor, weights: bool = False) -> torch.Tensor:
+    def verify(self, ids: torch.Tensor, parents: torch.Tensor | None = None, weights: bool = False) -> torch.Tensor:
         """Logits [B,T,V] of T drafted tokens (ids [B,T], T at most 64) that are not in the caches yet.  parents: int64 [T], the
         tree they form in every sequence: the node that each one follows, a lower index, or -1 for the last cached token.
         `accept` appends some of them, as long as neither `step` nor a roll-back comes between.  weights=True also adds the
         attention weights of all T queries to each layer's (`evict`), at once and for good: those of branches that are not accepted
-        and of drafts that are dropped, too."""
-        assert self.attention == "alignedkv", "only the AlignedKV path drafts tokens"
+        and of drafts that are dropped, too.  parents=None is a chain, the only form with attention="paged" (T tokens of at most 64 query rows per
+        KV head, no weights): its keys and values enter the pages behind the cached tokens, where `accept` lets them count."""
         cfg = self.cfg
-        H, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         B, T = ids.shape
-        up = parents.tolist()
+        if self.attention == "paged":
+            if weights or parents is not None and parents.tolist() != list(range(-1, T - 1)):
+                raise RuntimeError("verify: a paged cache takes chains of drafts, and no weights")
+            rows = T * (cfg.num_attention_heads // cfg.num_key_value_heads)
+            if rows > paged_ops.MOST_ROWS:
+                raise RuntimeError(f"verify: {T} tokens are {rows} query rows per KV head, at most {paged_ops.MOST_ROWS}")
+            x = self._paged(ids, [T] * B, False)
+            self._drafts = (list(self.table.lengths), T)
+            return self._logits(x)
+        assert self.attention == "alignedkv", "only the AlignedKV and paged paths draft tokens"
+        D = cfg.head_dim
+        up = list(range(-1, T - 1)) if parents is None else parents.tolist()
         if len(up) != T or any(type(j) is not int or not -1 <= j < i for i, j in enumerate(up)):
             raise RuntimeError(f"parents: expected {T} indices of earlier nodes, or -1")
         tree = torch.eye(T, dtype=torch.bool)
@@ -280,26 +359,36 @@ class LlamaDecoder:
         x = self.embed[ids]
         drafts = []
         for p, cache in zip(self.layers, self.caches):
-            h = _rms_norm(x, p["norm1"], cfg.rms_norm_eps)
-            qkv = F.linear(h, p["wqkv"]).view(B, T, H + 2 * Hkv, D)
-            qk = _rope(qkv[:, :, :H + Hkv], tables)
-            q, k, v = qk[:, :, :H].contiguous(), qk[:, :, H:].contiguous(), qkv[:, :, H + Hkv:].contiguous()
-            o = cache.tree_attention(q, k, v, tree, lse=weights)
-            if weights:
-                o, lse = o
-                cache.tree_weights(q, lse)
-            drafts.append((k, v))
-            x = torch.addmm(x.view(B * T, -1), o.view(B * T, H * D), p["wo"].t()).view(B, T, -1)
-            h = _rms_norm(x, p["norm2"], cfg.rms_norm_eps)
-            gate, wide = F.linear(h, p["w_gate_up"]).chunk(2, dim=-1)
-            x = torch.addmm(x.view(B * T, -1), F.silu(gate).mul_(wide).view(B * T, -1), p["w_down"].t()).view(B, T, -1)
+            def attend(q, k, v):
+                k, v = k.contiguous(), v.contiguous()
+                o = cache.tree_attention(q, k, v, tree, lse=weights)
+                if weights:
+                    o, lse = o
+                    cache.tree_weights(q, lse)
+                drafts.append((k, v))
+                return o
+            x = self._around(p, x, tables, attend)
         self._drafts = (self.pos, drafts)
-        return F.linear(_rms_norm(x, self.final_norm, cfg.rms_norm_eps), self.lm_head)
+        return self._logits(x)
 
     @torch.no_grad()
     def accept(self, path: torch.Tensor) -> None:
         """Append nodes path[b, 0..n-1] (int [B,n]: a chain from the root) of the last `verify` to the caches; once.  A call that is
-        refused changes nothing and leaves the drafts as they were."""
+        refused changes nothing and leaves the drafts as they were.
+
+        With attention="paged": the first path[b] tokens of each sequence's chain (int [B], 0 to T) count from now on."""
+        if self.attention == "paged":
+            lengths, T = self._drafts or (None, 0)
+            if lengths != self.table.lengths:
+                raise RuntimeError("accept: no drafted tokens at this position (call verify first)")
+            if path.shape != (self.B,) or path.is_floating_point() or path.dtype is torch.bool:
+                raise RuntimeError(f"path: expected integers of shape [{self.B}], the accepted tokens of each sequence's chain")
+            counts = path.tolist()
+            if not all(0 <= n <= T for n in counts):
+                raise RuntimeError(f"path: {counts}, expected 0 to {T}")
+            self.table.advance(counts)
+            self._drafts = None
+            return
         pos, drafts = self._drafts or (None, None)
         if pos != self.pos:
             raise RuntimeError("accept: no drafted tokens at this position (call verify first)")
@@ -318,8 +407,32 @@ class LlamaDecoder:
         self.pos += n
 
     @torch.no_grad()
+    def choose(self, logits: torch.Tensor, draft: torch.Tensor | None, ids: torch.Tensor, coins: torch.Tensor,
+               parents: torch.Tensor | None = None, temperature: float = 1.0) -> tuple:
+        """After `verify(ids, parents)`, whose logits are given: which of the drafts are accepted (`cache_ops.accept_drafts`; ids[:, 0] is taken, it
+        was sampled before), so that the output is distributed as sampling from softmax(logits / temperature) alone.  draft fp32 [B,T,V]: row i
+        the probabilities that node i's children were drawn from, or None; parents int64 [T] as given to `verify`; coins fp32 [B,T].
+
+        The accepted tokens enter the cache.  Returns (tokens int64 [B], counts [B] numbers): how many of its nodes each sequence has gone on by -
+        with attention="alignedkv" the same number for all, the smallest, since that cache has one length - and the token behind them, to be
+        the next ids[:, 0]."""
+        T = ids.shape[1]
+        target = torch.softmax(logits.float() / temperature, -1)
+        up = None if parents is None else parents.to(device=self.device, dtype=torch.int32)      # (a second root hangs under no node)
+        path, count, token = cache_ops.accept_drafts(target, draft, ids.contiguous(), coins, up)
+        counts = count.tolist()
+        if self.attention == "paged":
+            self.accept(count)
+            return token, counts
+        n = min(counts)
+        further = ids.gather(1, path[:, min(n, T - 1)].clamp(min=0).long()[:, None])[:, 0]
+        self.accept(path[:, :n])
+        return torch.where(count > n, further, token), [n] * self.B
+
+    @torch.no_grad()
     def evict(self, keep: int, recent: int = 0) -> None:
         """Reduce every layer's quantized tokens to the `keep` heaviest per head (`DecodeLayer.evict`); positions go on counting."""
+        assert self.attention == "alignedkv", "only the AlignedKV path evicts tokens"
         for cache in self.caches:
             cache.evict(keep, recent)
 
