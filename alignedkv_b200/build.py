@@ -11,7 +11,7 @@ LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libalignedkv_b200.so")
 SOURCES = ["akv_api.cu", "akv_save.cu", "akv_k_compute.cu", "akv_v_compute.cu", "akv_v_split.cu", "akv_decode.cu", "akv_prefill.cu",
            "akv_exchange.cu", "akv_operators.cu", "akv_dense.cu", "akv_tree.cu", "akv_tree_wide.cu", "akv_evict.cu", "akv_paged.cu",
-           "akv_paged_attention.cu", "akv_choose.cu"]
+           "akv_paged_attention.cu", "akv_paged_fp16.cu", "akv_paged_e4m3.cu", "akv_paged_e2m1.cu", "akv_choose.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 

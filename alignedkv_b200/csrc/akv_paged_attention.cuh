@@ -1,0 +1,874 @@
+// Attention of the newest tokens of each sequence over its pages.
+//   attend_kernel   query rows of a (sequence, KV head) against its tokens; one pass with a running maximum and sum
+//   join_kernel     joins the partial results of units that several CTAs share
+//
+//   s_rj = scale q_r . k_j, o_r = sum_j exp(s_rj - m_r) v_j / l_r, l_r = sum_j exp(s_rj - m_r), over the tokens j that row r sees.
+//
+// Every byte of the tokens is read once: bound by HBM, and for the 4-bit format almost as much by the instructions that unpack it.
+// Work: a unit is up to 16 query rows of one (sequence, KV head), its tokens in chunks of 32.  The chunks of all units in a row are dealt to
+// the warps in equal contiguous runs: lengths are only known on the device, and every SM gets the same whatever they are.  Each CTA
+// adds up the lengths itself.  A warp needs no other one: codes come straight into registers as operand fragments (no shared memory is
+// on their way), the next step's while this one's are multiplied.  Where a run begins or ends inside a unit it leaves a record, and
+// the CTA joins those of its warps; what is left between CTAs is join_kernel's.
+//
+// Operands: tokens are the rows of the products' first operand, query rows the columns of the second - 8 of them, which one KV head's query heads
+// fill, where the other way round 16 would be half empty.  Which channel is which k, and which token which row, is free as long as both
+// operands agree, and chosen so that a lane's loads are 16 bytes and need the fewest permutations.
+#pragma once
+#include <type_traits>
+
+#include "akv_paged_attention.h"
+
+namespace akv {
+namespace {
+
+constexpr float LN2 = 0.6931471805599453f;
+// Probabilities (times 2^exponent of their token's values) enter their product as fp16, since both operands have one type and the codes are exact there;
+// relative to the largest and times 2^15 they keep all 11 bits down to 2^-29 of it.  A second product with what the rounding leaves took the error
+// against 64 bits from 2.3e-4 to 2.1e-4, which is the output's own rounding, and 5% of the time of 4-bit pages: not kept.
+constexpr float LIFT = 32768.f;
+
+
+template <int F, int D, int NT>
+struct Shape {
+    static constexpr int ROW = row_bytes<F>(D);
+    static constexpr int KW = ROW / 8;                        // words of 16 tokens of K (or of V) in a lane
+    static constexpr int U = ROW == 256 ? 1 : 2;              // 16-token tiles of a step
+    static constexpr int TOKENS = 16 * U;
+    static constexpr int KS = D / 16;                         // products over the channels; tiles of 16 channels of the output
+    static constexpr int SCALES = F == AKV_PAGE_E2M1 ? D : 0; // bytes of a tile's scales (of K or of V)
+    static constexpr int MORE = F == AKV_PAGE_FP16 ? 0 : 2 * SCALES + 32;                  // ... of its scales and exponents
+    // A step in shared memory: a tile's codes of K and of V, the next tile's, then scales of K, of V, exponents of K, of V by tile.
+    static constexpr int STEP = (U * (32 * ROW + MORE) + 127) / 128 * 128;
+    static constexpr int STEPS = ROW >= 128 ? 2 : F == AKV_PAGE_E2M1 && D == 128 ? 3 : F == AKV_PAGE_E4M3 ? 4 : 6;
+    // Up to 16 rows: operands of the queries stay in registers.  More: in shared memory, and the output takes the registers of a third of the warps.
+    static constexpr bool FEW = NT <= 2;
+    static constexpr int WARPS = FEW ? 12 : 8;
+    static constexpr int RECORD = 8 * NT * (D + 4);           // floats: rows of D sums, then the maximum and the sum
+    static constexpr int TABLE = F == AKV_PAGE_FP16 ? 0 : TOKENS * 16;       // of a step's tokens: factor, exponent, weight
+    static constexpr int RING = STEPS * STEP, QUERIES = FEW ? 0 : KS * 4 * 32 * 8, OWN = RING + QUERIES + TABLE, SMEM = WARPS * OWN;
+    static_assert(OWN >= RECORD * 4, "a run's last record lies where its ring was");
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+// 16 bytes global -> shared past L1; with `there` false zeros, and nothing is read.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ int lds8_signed(uint32_t a) {
+    int v;
+    asm volatile("ld.shared.s8 %0, [%1];\n" : "=r"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t halves_bits(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// ---------------------------------------------------------------- which chunks are whose
+// cum[b]: chunks of one unit of the sequences before b; a sequence without tokens has one, so that its rows are written.
+__device__ __forceinline__ int chunks_of(int n) { return max(1, (n + CHUNK - 1) / CHUNK); }
+
+template <int THREADS>
+__device__ __forceinline__ void add_lengths(const AttendArgs& a, int* cum, int* sums) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += THREADS) {
+        const int b = b0 + tid;
+        int x = b < a.B ? chunks_of(length_of(a.pool, b)) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) sums[warp] = x;
+        __syncthreads();
+        int total = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) {
+            if (w == warp) x += total;
+            total += sums[w];
+        }
+        if (b < a.B) cum[b + 1] = before + x;
+        before += total;
+        __syncthreads();
+    }
+    if (tid == 0) cum[0] = 0;
+    __syncthreads();
+}
+struct Deal {
+    int per_cta, each, more;        // warps of a CTA that get a run; chunks of a run: `each`, one more for the first `more` runs
+    __device__ __forceinline__ Deal(int total, int ctas, int warps) {
+        per_cta = min(warps, (total + ctas - 1) / ctas);
+        each = (unsigned)total / (unsigned)(per_cta * ctas);
+        more = total - each * per_cta * ctas;
+    }
+    // First chunk of run w; of run w + 1: its end.
+    __device__ __forceinline__ int start(int w) const { return w * each + min(w, more); }
+    // CTA whose runs have chunk i.
+    __device__ __forceinline__ int cta_with(int i) const {
+        const int bound = more * (each + 1);
+        return (i < bound ? i / (each + 1) : more + (i - bound) / each) / per_cta;
+    }
+};
+// A run's part of one unit.
+struct Part {
+    int b, unit, first, last, chunks;   // sequence; unit of all; chunks of the unit: [first, last) of `chunks`
+    // The part that begins with chunk `at`, of a run that ends with `end`; b: where to begin looking.
+    __device__ __forceinline__ void find(const int* cum, int units, int b0, int at, int end) {
+        b = b0;
+        while (at >= cum[b + 1] * units) ++b;
+        chunks = cum[b + 1] - cum[b];
+        const int rest = at - cum[b] * units, u = (unsigned)rest / (unsigned)chunks;
+        unit = b * units + u;
+        first = rest - u * chunks;
+        last = min(chunks, first + end - at);
+    }
+    __device__ __forceinline__ bool whole() const { return first == 0 && last == chunks; }
+};
+__device__ __forceinline__ int sequence_with(const int* cum, int B, int units, int at) {
+    int lo = 0, hi = B - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (cum[mid] * units <= at) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ int2* borders(const AttendArgs& a) { return reinterpret_cast<int2*>(a.part + (2ll + MOST_WARPS) * a.ctas * a.record); }
+
+// Row of q, out and lse [B,T,H*G] that row r of a unit stands for; -1 behind the last.
+__device__ __forceinline__ long long row_of(const AttendArgs& a, int unit, int r, int* query) {
+    const int group = unit % a.groups, bh = unit / a.groups, h = bh % a.pool.H, b = bh / a.pool.H, R = group * a.rows + r;
+    const int t = (unsigned)R / (unsigned)a.G;
+    *query = t;
+    if (r >= a.rows || t >= a.T) return -1;
+    return ((long long)b * a.T + t) * (a.pool.H * a.G) + h * a.G + R - t * a.G;
+}
+
+// ---------------------------------------------------------------- a warp's ring
+// Where 16-byte piece c of row r of a tile lies, so that the 8 lanes of a 16-byte load's (16 of an 8-byte load's) phase read different banks: lane
+// (g, t) = (lane / 4, lane % 4) reads pieces by t of K's rows g, and pieces by g of V's rows 2t, 2t + 1.
+template <int ROW>
+__device__ __forceinline__ int piece(int r, int c) {
+    if constexpr (ROW >= 128) return r * ROW + ((c ^ (r & 7)) << 4);
+    const int line = r * ROW >> 7, slot = ((r * ROW & 127) >> 4) + c;
+    return line * 128 + ((slot ^ (2 * (line & (ROW == 64 ? 3 : 1)))) << 4);
+}
+
+// Steps of a run, copied to shared memory STEPS - 1 ahead by the warp's own asynchronous copies.  ONE: a step's tokens are in one page.
+template <int F, int D, int NT, bool ONE>
+struct Ring {
+    using S = Shape<F, D, NT>;
+    static constexpr int U = S::U, ROW = S::ROW, PAGES = ONE ? 1 : U;
+    const AttendArgs& a;
+    const int* cum;
+    uint32_t base, mine;                 // of the ring; where this lane's first piece of codes goes within a tile
+    const uint8_t* more;                 // this lane's piece of scales or exponents: its tensor, bytes of a token there
+    int per_token, lane, put, get;
+    Part part;                           // what is copied next
+    int units, end, at, n, h, token, stop, page[PAGES];
+    uint32_t gone;                       // PAGES bits a step, the oldest in the lowest: the page is not there
+
+    __device__ __forceinline__ Ring(const AttendArgs& args, const int* lengths, uint32_t to, int of_lane, int run_units, int first, int last)
+        : a(args), cum(lengths), base(to), lane(of_lane), put(0), get(0), units(run_units), end(last), at(first), gone(0) {
+        const int bytes = lane * 16;
+        mine = piece<ROW>(bytes / ROW, bytes % ROW / 16);
+        more = nullptr;
+        per_token = 0;
+        if constexpr (F != AKV_PAGE_FP16) {
+            constexpr int N = S::SCALES / 16;                 // pieces of a tile's scales
+            if (lane < 2 * N) {
+                more = (lane < N ? a.pool.ks : a.pool.vs) + lane % (N ? N : 1) * 16;
+                per_token = D / 16;
+            } else if (lane < 2 * N + 2) {
+                more = reinterpret_cast<const uint8_t*>(lane == 2 * N ? a.pool.ke : a.pool.ve);
+                per_token = 1;
+            }
+        }
+        part.find(cum, units, sequence_with(cum, a.B, units, at), at, end);
+        enter();
+        look();
+#pragma unroll 1
+        for (int i = 0; i < S::STEPS - 1; ++i) fill();
+    }
+    __device__ __forceinline__ void enter() {
+        n = length_of(a.pool, part.b);
+        h = part.unit / a.groups % a.pool.H;
+        token = part.first * CHUNK;
+        stop = min(n, part.last * CHUNK);
+    }
+    // Pages of the step at `token`; -1 where there is none or nothing of the sequence in it.
+    __device__ __forceinline__ void look() {
+#pragma unroll
+        for (int u = 0; u < PAGES; ++u) {
+            page[u] = -1;
+            if (token + 16 * u < n) page[u] = __ldg(a.pool.table + (unsigned)part.b * (unsigned)a.pool.width + ((token + 16 * u) >> a.pool.shift));
+        }
+    }
+    // The next step, if there is one; always a group, so that the groups count the steps.
+    __device__ __forceinline__ void fill() {
+        if (at < end) {
+            const uint32_t to = base + put * S::STEP;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int x = page[ONE ? 0 : u], from = ONE ? token : token + 16 * u;
+                const bool there = (unsigned)x < (unsigned)a.pool.n_pages;
+                const unsigned row = (((unsigned)(there ? x : 0) * (unsigned)a.pool.H + h) << a.pool.shift) + (from & ((1 << a.pool.shift) - 1)) + (ONE ? 16 * u : 0);
+                const unsigned long long byte = (unsigned long long)row * ROW + lane * 16;
+                const uint8_t *k = a.pool.kc + byte, *v = a.pool.vc + byte;
+                const uint32_t tile = to + u * 32 * ROW;
+#pragma unroll
+                for (int j = 0; j < ROW / 32; ++j) {
+                    // (512 bytes further: 2, 4, 8 or 16 rows)
+                    const uint32_t dst = tile + (ROW >= 128 ? (mine ^ ((j * (512 / ROW) & 7) << 4)) : mine) + j * 512;
+                    copy16(dst, k + j * 512, there);
+                    copy16(dst + 16 * ROW, v + j * 512, there);
+                }
+                if constexpr (F != AKV_PAGE_FP16)
+                    if (per_token) copy16(to + U * 32 * ROW + u * S::MORE + lane * 16, more + (unsigned long long)row * per_token, there);
+            }
+            uint32_t bits = 0;
+#pragma unroll
+            for (int u = 0; u < PAGES; ++u) bits |= (unsigned)((unsigned)page[u] >= (unsigned)a.pool.n_pages) << u;
+            gone |= bits << ((put >= get ? put - get : put - get + S::STEPS) * PAGES);
+            token += S::TOKENS;
+            if (token >= stop) {
+                at += part.last - part.first;
+                if (at < end) {
+                    part.find(cum, units, part.b, at, end);
+                    enter();
+                }
+            }
+            if (at < end) look();
+        }
+        cp_async_commit();
+        put = put + 1 == S::STEPS ? 0 : put + 1;
+    }
+    // Waits for the step that is read next, requests the one whose place the last read has left; pages that are not there.
+    __device__ __forceinline__ uint32_t take(uint32_t& without) {
+        cp_async_wait<S::STEPS - 2>();
+        __syncwarp();
+        fill();
+        const uint32_t from = base + get * S::STEP;
+        without = gone & ((1u << PAGES) - 1);
+        gone >>= PAGES;
+        get = get + 1 == S::STEPS ? 0 : get + 1;
+        return from;
+    }
+};
+
+// ---------------------------------------------------------------- a warp's unit
+template <int F, int D, int NT, bool ONE>
+struct Unit {
+    using S = Shape<F, D, NT>;
+    static constexpr int U = S::U, KW = S::KW, KS = S::KS, ROW = S::ROW;
+    const AttendArgs& a;
+    int g, t;
+    uint32_t at_k, at_v;                 // of this lane's first piece within a tile
+    uint32_t queries, table;             // shared memory
+    uint32_t q[S::FEW ? KS : 1][NT][2];
+    float acc[KS][NT][4], m[NT][2], l[NT][2];
+
+    __device__ __forceinline__ Unit(const AttendArgs& args, int lane, uint32_t own)
+        : a(args), g(lane >> 2), t(lane & 3), queries(own + S::RING), table(own + S::RING + S::QUERIES) {
+        at_k = ROW >= 128 ? piece<ROW>(g, 2 * t) : ROW == 64 ? piece<ROW>(g, t) : piece<ROW>(g, t >> 1) + (t & 1) * 8;
+        at_v = 16 * ROW + (ROW >= 128 ? piece<ROW>(2 * t, g) : ROW == 64 ? piece<ROW>(2 * t, g >> 1) + (g & 1) * 8 : piece<ROW>(2 * t, g >> 2) + (g & 3) * 4);
+    }
+
+    // Channels of the first operand's k = 2t, 2t + 1, 2t + 8, 2t + 9 in product s: this one and the next three.
+    __device__ __forceinline__ int k_channel(int s) const {
+        if constexpr (ROW == 256) return (s >> 2) * 64 + t * 16 + (s & 3) * 4;
+        return t * (D / 4) + s * 4;
+    }
+    // Channel of row g of output tile i; that of row g + 8 is the next.
+    __device__ __forceinline__ int v_channel(int i) const {
+        if constexpr (ROW == 256) return (i >> 2) * 64 + g * 8 + (i & 3) * 2;
+        return g * (D / 8) + 2 * i;
+    }
+
+    // (operands of two groups of 8 rows side by side)
+    __device__ __forceinline__ uint32_t query_place(int s, int nt) const { return queries + (((s * 2 + (nt >> 1)) * 32 + 4 * g + t) * 2 + (nt & 1)) * 8; }
+    __device__ __forceinline__ void multiply_keys(float (&s)[NT][4], int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+        if constexpr (S::FEW) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma(s[nt], a0, a1, a2, a3, q[i][nt][0], q[i][nt][1]);
+        } else {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt += 2) {
+                const uint4 w = lds128(query_place(i, nt));
+                mma(s[nt], a0, a1, a2, a3, w.x, w.y);
+                if (nt + 1 < NT) mma(s[nt + 1], a0, a1, a2, a3, w.z, w.w);
+            }
+        }
+    }
+
+    __device__ __forceinline__ void begin(int unit) {
+        if constexpr (!S::FEW) __syncwarp();     // (the last unit's have been read)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            int query;
+            const long long row = row_of(a, unit, 8 * nt + g, &query);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                uint2 w = make_uint2(0, 0);
+                if (row >= 0) w = *reinterpret_cast<const uint2*>(a.q + row * D + k_channel(s));
+                if constexpr (S::FEW) {
+                    q[s][nt][0] = w.x;
+                    q[s][nt][1] = w.y;
+                } else {
+                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};\n" ::"r"(query_place(s, nt)), "r"(w.x), "r"(w.y) : "memory");
+                }
+            }
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) acc[i][nt][0] = acc[i][nt][1] = acc[i][nt][2] = acc[i][nt][3] = 0.f;
+        }
+        if constexpr (!S::FEW) __syncwarp();
+    }
+
+    // What a step's exponents are needed as, a token per lane: its scores' factor, the exponent of its values, its values' weight.  (An exponent of
+    // -128 comes out as a factor of -infinity: times the row's zeros NaN, as it should; the maximum takes -40, below what there is.)
+    __device__ __forceinline__ void unfold(uint32_t step) {
+        if constexpr (F != AKV_PAGE_FP16) {
+            const int i = 4 * g + t;
+            if (i < S::TOKENS) {
+                const uint32_t from = step + U * 32 * ROW + (i >> 4) * S::MORE + 2 * S::SCALES + (i & 15);
+                const int k = lds8_signed(from), v = lds8_signed(from + 16);
+                const float weight = v == EXP_NAN ? NAN : __int_as_float((v + 127 + 15) << 23);
+                asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%3};\n" ::"r"(table + i * 16), "f"(a.scale2 * __int_as_float((k + 127) << 23)),
+                             "f"((float)max(v, -40)), "f"(weight) : "memory");
+            }
+            __syncwarp();
+        }
+    }
+
+    // Scores of a step's tokens, s[u][nt]: rows g (first two) and g + 8 by query rows 2t, 2t + 1.
+    __device__ __forceinline__ void scores(float (&s)[U][NT][4], uint32_t step) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t from = step + u * 32 * ROW + at_k;
+            constexpr int H = KW / 2;
+            uint32_t k[2][H];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                if constexpr (ROW == 32) {
+                    const uint2 w = lds64(from + half * 8 * ROW);
+                    k[half][0] = w.x;
+                    k[half][1] = w.y;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < H / 4; ++c) {
+                        const uint4 w = lds128((from ^ ((c & 1) << 4)) + half * 8 * ROW + (c >> 1) * 128);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) k[half][4 * c + i] = u4w(w, i);
+                    }
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = 0.f;
+            if constexpr (F == AKV_PAGE_FP16) {
+#pragma unroll
+                for (int i = 0; i < KS; ++i) multiply_keys(s[u], i, k[0][2 * i], k[1][2 * i], k[0][2 * i + 1], k[1][2 * i + 1]);
+            } else if constexpr (F == AKV_PAGE_E4M3) {
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    uint32_t x[2], y[2];
+                    e4m3_word(x, k[0][i]);
+                    e4m3_word(y, k[1][i]);
+                    multiply_keys(s[u], i, x[0], y[0], x[1], y[1]);
+                }
+            } else {
+                const uint32_t scales = step + U * 32 * ROW + u * S::MORE + g * (D / 16) + t * (D / 64);
+                const uint32_t s0 = e4m3_halves(D == 128 ? lds16(scales) : lds8(scales));
+                const uint32_t s1 = e4m3_halves(D == 128 ? lds16(scales + D / 2) : lds8(scales + D / 2));
+#pragma unroll
+                for (int w = 0; w < H; ++w) {
+                    // (8 channels of a word: two products; 16 have a scale)
+                    const uint32_t f0 = __byte_perm(s0, s0, D == 128 && w >= 2 ? 0x3232 : 0x1010), f1 = __byte_perm(s1, s1, D == 128 && w >= 2 ? 0x3232 : 0x1010);
+                    uint32_t x[4], y[4];
+                    e2m1_word(x, k[0][w]);
+                    e2m1_word(y, k[1][w]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        multiply_keys(s[u], 2 * w + i, hmul2_bits(x[2 * i], f0), hmul2_bits(y[2 * i], f1), hmul2_bits(x[2 * i + 1], f0),
+                                      hmul2_bits(y[2 * i + 1], f1));
+                }
+            }
+        }
+    }
+
+    // Scores to weights of the values, in place, and the running maximum and sum with them.  seen(nt, c): tokens below it are seen by the row;
+    // without: bits of the pages that are not there.  ALL: every row sees the whole step.
+    template <bool ALL>
+    __device__ __forceinline__ void soften(float (&s)[U][NT][4], uint32_t without, int at, const int (&seen)[NT][2]) {
+        float top[NT][2], f[U][2], unit[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float e = 0.f;
+                f[u][half] = a.scale2;
+                unit[u][half] = LIFT;
+                if constexpr (F != AKV_PAGE_FP16) {
+                    const uint4 w = lds128(table + (16 * u + 8 * half + g) * 16);
+                    f[u][half] = __uint_as_float(w.x);
+                    e = __uint_as_float(w.y);
+                    unit[u][half] = __uint_as_float(w.z);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float& x = s[u][nt][2 * half + c];
+                        if (!ALL) {
+                            x *= f[u][half];
+                            if (missing(without, u) || at + 16 * u + g + 8 * half >= seen[nt][c]) x = -INFINITY;
+                        }
+                        const float y = ALL ? fmaf(x, f[u][half], e) : x + e;
+                        top[nt][c] = u == 0 && half == 0 ? y : fmaxf(top[nt][c], y);
+                    }
+            }
+        bool higher = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(0xFFFFFFFFu, top[nt][c], o));
+                higher |= top[nt][c] > m[nt][c];
+            }
+        if (__any_sync(0xFFFFFFFFu, higher)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float g2[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float y = fmaxf(top[nt][c], m[nt][c]);
+                    g2[c] = y == m[nt][c] ? 1.f : ex2(m[nt][c] - y);
+                    m[nt][c] = y;
+                    l[nt][c] *= g2[c];
+                }
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    acc[i][nt][0] *= g2[0];
+                    acc[i][nt][1] *= g2[1];
+                    acc[i][nt][2] *= g2[0];
+                    acc[i][nt][3] *= g2[1];
+                }
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const float base = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        float& x = s[u][nt][2 * half + c];
+                        const bool gone = !ALL && (missing(without, u) || at + 16 * u + g + 8 * half >= seen[nt][c]);
+                        const float p = ex2(ALL ? fmaf(x, f[u][half], -base) : x - base);
+                        l[nt][c] += p;                              // (of what is not seen: 0)
+                        x = gone ? 0.f : p * unit[u][half];
+                    }
+            }
+    }
+
+    static __device__ __forceinline__ bool missing(uint32_t without, int u) { return (without >> (ONE ? 0 : u)) & 1; }
+
+    // A tile's values: tokens 2t, 2t + 1, 2t + 8, 2t + 9; zeros for those that lie behind the sequence (limit: tokens of the tile that do not),
+    // whatever is there.
+    __device__ __forceinline__ void load_v(uint32_t (&v)[KW], uint32_t (&scale)[2], uint32_t step, int u, int limit) {
+        constexpr int W = KW / 4;
+        const uint32_t from = step + u * 32 * ROW + at_v;
+        uint32_t bytes[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t x = (ROW >= 128 ? (from ^ ((i & 1) << 4)) + (i & 1) * ROW : from ^ ((i & 1) * ROW)) + (i >> 1) * 8 * ROW;
+            if constexpr (ROW >= 128) {
+#pragma unroll
+                for (int c = 0; c < W / 4; ++c) {
+                    const uint4 w = lds128(x + c * 128);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[i * W + 4 * c + j] = u4w(w, j);
+                }
+            } else if constexpr (ROW == 64) {
+                const uint2 w = lds64(x);
+                v[i * W] = w.x;
+                v[i * W + 1] = w.y;
+            } else {
+                v[i] = lds32(x);
+            }
+            bytes[i] = 0;
+            if constexpr (F == AKV_PAGE_E2M1)
+                bytes[i] = lds8(step + U * 32 * ROW + u * S::MORE + S::SCALES + (2 * t + (i & 1) + (i >> 1) * 8) * (D / 16) + (D == 128 ? g : g >> 1));
+        }
+        if (limit < 16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (2 * t + (i & 1) + (i >> 1) * 8 >= limit) {
+                    bytes[i] = 0;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) v[i * W + j] = 0;
+                }
+        }
+        if constexpr (F == AKV_PAGE_E2M1) {
+            scale[0] = e4m3_halves(__byte_perm(bytes[0], bytes[1], 0x0040));
+            scale[1] = e4m3_halves(__byte_perm(bytes[2], bytes[3], 0x0040));
+        }
+    }
+    // fn(i, a0, a1, a2, a3): the first operand of output tile i.
+    template <class Fn>
+    __device__ __forceinline__ void tiles(const uint32_t (&v)[KW], const uint32_t (&scale)[2], Fn fn) {
+        constexpr int W = KW / 4;              // words of a token
+        if constexpr (F == AKV_PAGE_FP16) {
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+                fn(i, __byte_perm(v[i], v[W + i], 0x5410), __byte_perm(v[i], v[W + i], 0x7632),
+                   __byte_perm(v[2 * W + i], v[3 * W + i], 0x5410), __byte_perm(v[2 * W + i], v[3 * W + i], 0x7632));
+        } else if constexpr (F == AKV_PAGE_E4M3) {
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                const uint32_t x = __byte_perm(v[i >> 1], v[W + (i >> 1)], i & 1 ? 0x7362 : 0x5140);
+                const uint32_t y = __byte_perm(v[2 * W + (i >> 1)], v[3 * W + (i >> 1)], i & 1 ? 0x7362 : 0x5140);
+                uint32_t p[2], r[2];
+                e4m3_word(p, x);
+                e4m3_word(r, y);
+                fn(i, p[0], p[1], r[0], r[1]);
+            }
+        } else {
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                constexpr uint32_t LOW = 0x0F0F0F0Fu;
+                // two tokens' nibbles of one channel in a byte: even channels, odd ones
+                const uint32_t e0 = (v[w] & LOW) | ((v[W + w] << 4) & ~LOW), o0 = ((v[w] >> 4) & LOW) | (v[W + w] & ~LOW);
+                const uint32_t e1 = (v[2 * W + w] & LOW) | ((v[3 * W + w] << 4) & ~LOW), o1 = ((v[2 * W + w] >> 4) & LOW) | (v[3 * W + w] & ~LOW);
+                uint32_t x0[4], y0[4], x1[4], y1[4];
+                e2m1_word(x0, e0);
+                e2m1_word(y0, o0);
+                e2m1_word(x1, e1);
+                e2m1_word(y1, o1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    fn(4 * w + i, hmul2_bits(x0[i], scale[0]), hmul2_bits(y0[i], scale[0]), hmul2_bits(x1[i], scale[1]), hmul2_bits(y1[i], scale[1]));
+            }
+        }
+    }
+    // limit: tokens of the step that are the sequence's.
+    __device__ __forceinline__ void add_values(const float (&s)[U][NT][4], uint32_t step, int at, int limit, const int (&seen)[NT][2]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            uint32_t v[KW], scale[2], w[NT][2];
+            load_v(v, scale, step, u, limit - 16 * u);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                w[nt][0] = transposed(halves_bits(s[u][nt][0], s[u][nt][1]));
+                w[nt][1] = transposed(halves_bits(s[u][nt][2], s[u][nt][3]));
+            }
+            if (F == AKV_PAGE_FP16 && __any_sync(0xFFFFFFFFu, odd(v))) {
+                add_odd_values(v, w, at + 16 * u, at + limit, seen);
+                continue;
+            }
+            tiles(v, scale, [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma(acc[i][nt], a0, a1, a2, a3, w[nt][0], w[nt][1]);
+            });
+        }
+    }
+    // The same where some values are not finite (fp16 pages alone: elsewhere codes are).  0 * inf would be NaN: every query's product is formed by
+    // itself, without the newest tokens that it does not see.
+    __device__ __forceinline__ void add_odd_values(const uint32_t (&v)[KW], const uint32_t (&w)[NT][2], int at, int n, const int (&seen)[NT][2]) {
+        const uint32_t none[2] = {0, 0};
+#pragma unroll 1
+        for (int limit = n - a.T + 1; limit <= n; ++limit) {
+            bool there[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) there[i] = at + 2 * t + (i & 1) + (i >> 1) * 8 < limit;
+            const uint32_t m01 = (there[0] ? 0xFFFFu : 0u) | (there[1] ? 0xFFFF0000u : 0u), m23 = (there[2] ? 0xFFFFu : 0u) | (there[3] ? 0xFFFF0000u : 0u);
+            tiles(v, none, [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma(c, a0 & m01, a1 & m01, a2 & m23, a3 & m23, w[nt][0], w[nt][1]);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        if (seen[nt][x & 1] == limit) acc[i][nt][x] += c[x];
+                }
+            });
+        }
+    }
+    static __device__ __forceinline__ uint32_t finite(uint32_t w) {
+        if ((w & 0x7C00u) == 0x7C00u) w &= 0xFFFF0000u;
+        return (w & 0x7C000000u) == 0x7C000000u ? w & 0xFFFFu : w;
+    }
+    static __device__ __forceinline__ bool odd(const uint32_t (&v)[KW]) {
+        uint32_t x[2] = {0, 0};                  // (0 as long as all are finite, then NaN)
+#pragma unroll
+        for (int i = 0; i < KW; ++i) x[i & 1] = hfma2_bits(v[i], 0, x[i & 1]);
+        return finite(x[0]) != x[0] || finite(x[1]) != x[1];
+    }
+
+    // The unit's result: sums over the lanes, then to rows.
+    __device__ __forceinline__ void close() {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l[nt][c] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][c], o);
+    }
+    __device__ __forceinline__ void write(int unit) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                int query;
+                const long long row = row_of(a, unit, 8 * nt + 2 * t + c, &query);
+                if (row < 0) continue;
+                const float inv = l[nt][c] == 0.f ? 0.f : 1.f / (l[nt][c] * LIFT);
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    const __half2 h = __floats2half2_rn(acc[i][nt][c] * inv, acc[i][nt][2 + c] * inv);
+                    *reinterpret_cast<__half2*>(a.out + row * D + v_channel(i)) = h;
+                }
+                if (a.lse && g == 0) a.lse[row] = l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + log2f(l[nt][c])) * LN2;
+            }
+    }
+    // Record: rows of D + 4 floats, output sums, then maximum and sum.
+    __device__ __forceinline__ void record(float* to) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                if (8 * nt + 2 * t + c >= a.rows) continue;
+                float* row = to + (8 * nt + 2 * t + c) * (D + 4);
+#pragma unroll
+                for (int i = 0; i < KS; ++i)
+                    *reinterpret_cast<float2*>(row + v_channel(i)) = make_float2(acc[i][nt][c], acc[i][nt][2 + c]);
+                if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[nt][c], l[nt][c]);
+            }
+    }
+};
+
+// Joins row r of up to `count` records by a warp, lane i having those at i, i + 32, ...: fn(i) = the row in the i-th.  Then to a record, or to
+// out and lse.
+template <int D, class Fn>
+__device__ __forceinline__ void join_row(const AttendArgs& a, int unit, int r, int count, int lane, Fn fn, float* record) {
+    constexpr int N = D / 32;
+    using Vec = typename std::conditional<N == 4, float4, float2>::type;
+    float top = -INFINITY;
+    for (int i = lane; i < count; i += 32) top = fmaxf(top, fn(i)[D]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const float base = top == -INFINITY ? 0.f : top;
+    float o[N], sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < N; ++c) o[c] = 0.f;
+    for (int i0 = 0; i0 < count; i0 += 32) {
+        float mine = 0.f, l = 0.f;
+        if (i0 + lane < count) {
+            const float2 x = *reinterpret_cast<const float2*>(fn(i0 + lane) + D);
+            mine = ex2(x.x - base);
+            l = x.y;
+        }
+        const int here = min(32, count - i0);
+#pragma unroll 8
+        for (int i = 0; i < here; ++i) {
+            const Vec x = *reinterpret_cast<const Vec*>(fn(i0 + i) + N * lane);
+            const float f = __shfl_sync(0xFFFFFFFFu, mine, i);
+            sum = fmaf(f, __shfl_sync(0xFFFFFFFFu, l, i), sum);
+#pragma unroll
+            for (int c = 0; c < N; ++c) o[c] = fmaf(f, reinterpret_cast<const float*>(&x)[c], o[c]);
+        }
+    }
+    if (record) {
+        Vec x;
+#pragma unroll
+        for (int c = 0; c < N; ++c) reinterpret_cast<float*>(&x)[c] = o[c];
+        *reinterpret_cast<Vec*>(record + N * lane) = x;
+        if (lane == 0) *reinterpret_cast<float2*>(record + D) = make_float2(top, sum);
+        return;
+    }
+    int query;
+    const long long row = row_of(a, unit, r, &query);
+    if (row < 0) return;
+    const float inv = sum == 0.f ? 0.f : 1.f / (sum * LIFT);
+#pragma unroll
+    for (int c = 0; c < N; c += 2)
+        *reinterpret_cast<__half2*>(a.out + row * D + N * lane + c) = __floats2half2_rn(o[c] * inv, o[c + 1] * inv);
+    if (a.lse && lane == 0) a.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+}
+
+template <int F, int D, int NT, bool ONE>
+__global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(AttendArgs a) {
+    using S = Shape<F, D, NT>;
+    constexpr int WARPS = S::WARPS;
+    extern __shared__ __align__(128) uint8_t rings[];
+    int* cum = reinterpret_cast<int*>(rings + S::SMEM);
+    __shared__ int sums[WARPS], s_unit[2 * WARPS], s_tasks;     // (s_unit: units of the records of each run's first part and of its last, or -1)
+    __shared__ int4 s_task[2 * WARPS];                         // unit, its first of s_slots, how many, where they go
+    __shared__ int s_slots[2 * WARPS];
+    __shared__ int2 s_border;
+    pdl_turn();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    add_lengths<32 * WARPS>(a, cum, sums);
+    const int units = a.pool.H * a.groups;
+    const Deal deal(cum[a.B] * units, gridDim.x, WARPS);
+    const int me = blockIdx.x * deal.per_cta + warp;
+    int at = 0, end = 0;
+    if (warp < deal.per_cta) {
+        at = deal.start(me);
+        end = deal.start(me + 1);
+    }
+    if (lane < 2) s_unit[2 * warp + lane] = -1;
+    __syncwarp();
+    // Records: of a part that ends its run in the run's ring, which nobody needs any more; of one in front of others in global memory.
+    float* last_record = reinterpret_cast<float*>(rings + warp * S::OWN);
+    float* first_record = a.part + (2ll * gridDim.x + blockIdx.x * WARPS + warp) * S::RECORD;
+    if (at < end) {
+        Ring<F, D, NT, ONE> ring(a, cum, smem_u32(last_record), lane, units, at, end);
+        Unit<F, D, NT, ONE> unit(a, lane, smem_u32(last_record));
+        Part part;
+        part.b = ring.part.b;                                  // (or a later one: found from the run's beginning)
+        part.find(cum, units, sequence_with(cum, a.B, units, at), at, end);
+        for (;;) {
+            const int n = length_of(a.pool, part.b), stop = min(n, part.last * CHUNK);
+            int seen[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    int query;
+                    seen[nt][c] = row_of(a, part.unit, 8 * nt + 2 * unit.t + c, &query) < 0 ? 0 : n - a.T + 1 + query;
+                }
+            unit.begin(part.unit);
+            int token = part.first * CHUNK;
+#pragma unroll 1
+            do {
+                uint32_t without;
+                const uint32_t step = ring.take(without);
+                float s[S::U][NT][4];
+                unit.unfold(step);
+                unit.scores(s, step);
+                if (token + S::TOKENS <= n - a.T + 1 && without == 0) unit.template soften<true>(s, without, token, seen);
+                else unit.template soften<false>(s, without, token, seen);
+                unit.add_values(s, step, token, n - token, seen);
+                token += S::TOKENS;
+            } while (token < stop);
+            unit.close();
+            at += part.last - part.first;
+            if (part.whole()) {
+                unit.write(part.unit);
+            } else {
+                const bool over = at >= end;
+                if (over) {
+                    cp_async_wait<0>();
+                    __syncwarp();
+                }
+                unit.record(over ? last_record : first_record);
+                if (lane == 0) s_unit[2 * warp + over] = part.unit;
+            }
+            if (at >= end) break;
+            part.find(cum, units, part.b, at, end);
+        }
+    }
+    __syncthreads();
+    // A unit whose records all are in this CTA is written, of another one record is left: the CTA's first where it began in front of it, else its
+    // second, and for the kernel that joins those the unit and the last CTA that has a part of it.
+    if (warp == 0) {
+        const int unit = lane < 2 * WARPS ? s_unit[lane] : -1;
+        const unsigned same = __match_any_sync(0xFFFFFFFFu, unit);
+        const bool leads = unit >= 0 && (same & ((1u << lane) - 1)) == 0;
+        const unsigned leaders = __ballot_sync(0xFFFFFFFFu, leads), below = (1u << lane) - 1;
+        const int place = __popc(__ballot_sync(0xFFFFFFFFu, unit >= 0) & below);       // records in front of this one
+        if (unit >= 0) s_slots[place] = lane;
+        if (lane == 0) {
+            s_tasks = __popc(leaders);
+            s_border = make_int2(-1, 0);
+        }
+        __syncwarp();
+        if (leads) {
+            const int b = unit / units, chunks = cum[b + 1] - cum[b], from = cum[b] * units + (unit - b * units) * chunks;
+            const bool before = from < deal.start(blockIdx.x * deal.per_cta), after = from + chunks > deal.start((blockIdx.x + 1) * deal.per_cta);
+            if (!before && after) s_border = make_int2(unit, deal.cta_with(from + chunks - 1));
+            s_task[__popc(leaders & below)] = make_int4(unit, place, __popc(same), before ? 0 : after ? 1 : -1);
+        }
+        __syncwarp();
+        if (lane == 0) borders(a)[blockIdx.x] = s_border;
+    }
+    __syncthreads();
+    for (int x = warp; x < s_tasks * a.rows; x += WARPS) {
+        const int i = x / a.rows, r = x - i * a.rows;
+        const int4 task = s_task[i];
+        float* record = task.w < 0 ? nullptr : a.part + ((long long)(2 * blockIdx.x + task.w) * 8 * NT + r) * (D + 4);
+        join_row<D>(a, task.x, r, task.z, lane, [&](int k) {
+            const int slot = s_slots[task.y + k], w = slot >> 1;
+            return (slot & 1 ? reinterpret_cast<const float*>(rings + w * S::OWN) : a.part + (2ll * gridDim.x + blockIdx.x * WARPS + w) * S::RECORD) + r * (D + 4);
+        }, record);
+    }
+}
+
+// One CTA per CTA of attend_kernel: where a unit begins there and ends in another one, its records are joined.
+template <int D, int NT>
+__global__ void __launch_bounds__(32 * 8 * NT) join_kernel(AttendArgs a) {
+    pdl_turn();
+    const int2 border = borders(a)[blockIdx.x];
+    const int lane = threadIdx.x & 31, r = threadIdx.x >> 5, from = blockIdx.x;
+    if (border.x < 0 || r >= a.rows) return;
+    join_row<D>(a, border.x, r, border.y - from + 1, lane, [&](int i) {
+        return a.part + ((long long)(2 * (from + i) + (i == 0)) * 8 * NT + r) * (D + 4);
+    }, nullptr);
+}
+
+template <int F, int D, int NT, bool ONE>
+int launch(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
+    using S = Shape<F, D, NT>;
+    static_assert(S::WARPS <= MOST_WARPS, "workspace");
+    const int smem = S::SMEM + (a.B + 1) * 4;
+    static thread_local int set_for = -1;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && set_for != dev) {
+        // (the most it is ever launched with)
+        e = cudaFuncSetAttribute(attend_kernel<F, D, NT, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM + 4097 * 4);
+        if (e == cudaSuccess) set_for = dev;
+    }
+    if (e != cudaSuccess) return cuda_status(e, "paged_attention");
+    launch_chained(attend_kernel<F, D, NT, ONE>, dim3(p.ctas), dim3(32 * S::WARPS), smem, st, a);
+    const int rc = cuda_status(cudaGetLastError(), "paged_attention launch");
+    if (rc != AKV_OK || !joined || p.ctas == 1) return rc;
+    launch_chained(join_kernel<D, NT>, dim3(p.ctas), dim3(32 * 8 * NT), 0, st, a);
+    return cuda_status(cudaGetLastError(), "paged_attention join launch");
+}
+template <int F, int D, int NT>
+int launch_pages(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
+    if constexpr (Shape<F, D, NT>::U > 1)
+        if (Shape<F, D, NT>::TOKENS > 1 << a.pool.shift) return launch<F, D, NT, false>(a, p, joined, st);
+    return launch<F, D, NT, true>(a, p, joined, st);
+}
+template <int F, int D>
+int launch_rows(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
+    if (p.nt == 1) return launch_pages<F, D, 1>(a, p, joined, st);
+    if (p.nt == 2) return launch_pages<F, D, 2>(a, p, joined, st);
+    if (p.nt == 3) return launch_pages<F, D, 3>(a, p, joined, st);
+    return launch_pages<F, D, 4>(a, p, joined, st);
+}
+
+}  // namespace
+}  // namespace akv

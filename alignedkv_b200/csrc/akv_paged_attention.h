@@ -1,0 +1,30 @@
+// Arguments of the attention over pages, and its launchers by page format (each has a file of its own).
+#pragma once
+#include "akv_paged.cuh"
+
+namespace akv {
+
+constexpr int CHUNK = 32, MOST_WARPS = 12;
+
+struct AttendArgs {
+    Pool pool;
+    const __half* q;
+    __half* out;
+    float *lse, *part;              // part: two records of each CTA, one of each warp, a border of each CTA
+    int B, T, G, groups, rows, ctas, record;    // record: floats of one
+    // groups: units per (sequence, KV head); rows: query rows of a unit
+    float scale2;                   // scale * log2(e)
+};
+
+// Rows of a unit in groups of 8 (nt), CTAs, workspace.
+struct Plan {
+    int nt, groups, rows, ctas;
+    long long bytes;
+};
+
+// joined: units may be shared by CTAs.
+int launch_attend_fp16(const AttendArgs& a, const Plan& p, int D, bool joined, cudaStream_t st);
+int launch_attend_e4m3(const AttendArgs& a, const Plan& p, int D, bool joined, cudaStream_t st);
+int launch_attend_e2m1(const AttendArgs& a, const Plan& p, int D, bool joined, cudaStream_t st);
+
+}  // namespace akv
