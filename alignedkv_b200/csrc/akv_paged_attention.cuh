@@ -15,8 +15,6 @@
 // fill, where the other way round 16 would be half empty.  Which channel is which k, and which token which row, is free as long as both
 // operands agree, and chosen so that a lane's loads are 16 bytes and need the fewest permutations.
 #pragma once
-#include <type_traits>
-
 #include "akv_paged_attention.h"
 
 namespace akv {
@@ -666,53 +664,47 @@ struct Unit {
     }
 };
 
-// Joins row r of up to `count` records by a warp, lane i having those at i, i + 32, ...: fn(i) = the row in the i-th.  Then to a record, or to
-// out and lse.
-template <int D, class Fn>
-__device__ __forceinline__ void join_row(const AttendArgs& a, int unit, int r, int count, int lane, Fn fn, float* record) {
-    constexpr int N = D / 32;
-    using Vec = typename std::conditional<N == 4, float4, float2>::type;
-    float top = -INFINITY;
-    for (int i = lane; i < count; i += 32) top = fmaxf(top, fn(i)[D]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    const float base = top == -INFINITY ? 0.f : top;
-    float o[N], sum = 0.f;
-#pragma unroll
-    for (int c = 0; c < N; ++c) o[c] = 0.f;
-    for (int i0 = 0; i0 < count; i0 += 32) {
-        float mine = 0.f, l = 0.f;
-        if (i0 + lane < count) {
-            const float2 x = *reinterpret_cast<const float2*>(fn(i0 + lane) + D);
-            mine = ex2(x.x - base);
-            l = x.y;
-        }
-        const int here = min(32, count - i0);
-#pragma unroll 8
-        for (int i = 0; i < here; ++i) {
-            const Vec x = *reinterpret_cast<const Vec*>(fn(i0 + i) + N * lane);
-            const float f = __shfl_sync(0xFFFFFFFFu, mine, i);
-            sum = fmaf(f, __shfl_sync(0xFFFFFFFFu, l, i), sum);
-#pragma unroll
-            for (int c = 0; c < N; ++c) o[c] = fmaf(f, reinterpret_cast<const float*>(&x)[c], o[c]);
-        }
-    }
-    if (record) {
-        Vec x;
-#pragma unroll
-        for (int c = 0; c < N; ++c) reinterpret_cast<float*>(&x)[c] = o[c];
-        *reinterpret_cast<Vec*>(record + N * lane) = x;
-        if (lane == 0) *reinterpret_cast<float2*>(record + D) = make_float2(top, sum);
-        return;
-    }
+// A row's result to out and lse: sums x of 4 channels from `channel` on, over (maximum, sum).
+template <int D>
+__device__ __forceinline__ void write_row(const AttendArgs& a, int unit, int r, int channel, float4 x, float top, float sum) {
     int query;
     const long long row = row_of(a, unit, r, &query);
     if (row < 0) return;
     const float inv = sum == 0.f ? 0.f : 1.f / (sum * LIFT);
+    const __half2 lo = __floats2half2_rn(x.x * inv, x.y * inv), hi = __floats2half2_rn(x.z * inv, x.w * inv);
+    *reinterpret_cast<uint2*>(a.out + row * D + channel) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    if (a.lse && channel == 0) a.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+}
+// Joins a row of `count` records by 8 lanes (sub: which of them); fn(i) = the row in the i-th.  (A warp has four rows at a time: what it waits for are a
+// few loads, one after the other.)
+template <int D, class Fn>
+__device__ __forceinline__ void join_few(const AttendArgs& a, int unit, int r, int count, int sub, Fn fn, float* record) {
+    constexpr int N = D / 32;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) top = fmaxf(top, fn(i)[D]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float4 o[N];
 #pragma unroll
-    for (int c = 0; c < N; c += 2)
-        *reinterpret_cast<__half2*>(a.out + row * D + N * lane + c) = __floats2half2_rn(o[c] * inv, o[c + 1] * inv);
-    if (a.lse && lane == 0) a.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * LN2;
+    for (int c = 0; c < N; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (int i = 0; i < count; ++i) {
+        const float* x = fn(i);
+        const float2 ml = *reinterpret_cast<const float2*>(x + D);
+        const float f = ex2(ml.x - base);
+        sum = fmaf(f, ml.y, sum);
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+            const float4 y = *reinterpret_cast<const float4*>(x + 32 * c + 4 * sub);
+            o[c] = make_float4(fmaf(f, y.x, o[c].x), fmaf(f, y.y, o[c].y), fmaf(f, y.z, o[c].z), fmaf(f, y.w, o[c].w));
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        if (record) *reinterpret_cast<float4*>(record + 32 * c + 4 * sub) = o[c];
+        else write_row<D>(a, unit, r, 32 * c + 4 * sub, o[c], top, sum);
+    }
+    if (record && sub == 0) *reinterpret_cast<float2*>(record + D) = make_float2(top, sum);
 }
 
 template <int F, int D, int NT, bool ONE>
@@ -813,27 +805,72 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
         if (lane == 0) borders(a)[blockIdx.x] = s_border;
     }
     __syncthreads();
-    for (int x = warp; x < s_tasks * a.rows; x += WARPS) {
+    for (int x = warp * 4 + (lane >> 3); x < s_tasks * a.rows; x += 4 * WARPS) {
         const int i = x / a.rows, r = x - i * a.rows;
         const int4 task = s_task[i];
         float* record = task.w < 0 ? nullptr : a.part + ((long long)(2 * blockIdx.x + task.w) * 8 * NT + r) * (D + 4);
-        join_row<D>(a, task.x, r, task.z, lane, [&](int k) {
+        join_few<D>(a, task.x, r, task.z, lane & 7, [&](int k) {
             const int slot = s_slots[task.y + k], w = slot >> 1;
             return (slot & 1 ? reinterpret_cast<const float*>(rings + w * S::OWN) : a.part + (2ll * gridDim.x + blockIdx.x * WARPS + w) * S::RECORD) + r * (D + 4);
         }, record);
     }
 }
 
-// One CTA per CTA of attend_kernel: where a unit begins there and ends in another one, its records are joined.
+// One CTA per CTA of attend_kernel: where a unit begins there and ends in another one, its records are joined, a row by as many warps as there are
+// for it, whose parts are joined in shared memory.
+constexpr int JOINERS = 16;
 template <int D, int NT>
-__global__ void __launch_bounds__(32 * 8 * NT) join_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(32 * JOINERS) join_kernel(AttendArgs a) {
+    __shared__ __align__(16) float parts[JOINERS][D + 4];
     pdl_turn();
     const int2 border = borders(a)[blockIdx.x];
-    const int lane = threadIdx.x & 31, r = threadIdx.x >> 5, from = blockIdx.x;
-    if (border.x < 0 || r >= a.rows) return;
-    join_row<D>(a, border.x, r, border.y - from + 1, lane, [&](int i) {
-        return a.part + ((long long)(2 * (from + i) + (i == 0)) * 8 * NT + r) * (D + 4);
-    }, nullptr);
+    if (border.x < 0) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, from = blockIdx.x, count = border.y - from + 1;
+    const int shares = max(1, JOINERS / a.rows), each = (count + shares - 1) / shares;     // (warps of a row, records of each)
+    for (int r0 = 0; r0 < a.rows; r0 += JOINERS / shares) {
+        const int r = r0 + warp / shares, first = warp % shares * each, last = min(count, first + each);
+        const bool mine = warp / shares < JOINERS / shares && r < a.rows;
+        if (mine) {
+            // (4 channels a lane, of 128; of 64 half of the lanes have none)
+            const int channel = 4 * lane;
+            float top = -INFINITY, sum = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto row = [&](int i) { return a.part + ((long long)(2 * (from + i) + (i == 0)) * 8 * NT + r) * (D + 4); };
+            for (int i0 = first; i0 < last; i0 += 32) {
+                float2 ml = make_float2(-INFINITY, 0.f);
+                if (i0 + lane < last) ml = *reinterpret_cast<const float2*>(row(i0 + lane) + D);
+                float m = ml.x;
+#pragma unroll
+                for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
+                m = fmaxf(m, top);
+                const float base = m == -INFINITY ? 0.f : m, was = ex2(top - base), f = ex2(ml.x - base);
+                o = make_float4(o.x * was, o.y * was, o.z * was, o.w * was);
+                sum *= was;
+                top = m;
+                const int here = min(32, last - i0);
+#pragma unroll 8
+                for (int i = 0; i < here; ++i) {
+                    const float g = __shfl_sync(0xFFFFFFFFu, f, i);
+                    sum = fmaf(g, __shfl_sync(0xFFFFFFFFu, ml.y, i), sum);
+                    if (channel < D) {
+                        const float4 y = *reinterpret_cast<const float4*>(row(i0 + i) + channel);
+                        o = make_float4(fmaf(g, y.x, o.x), fmaf(g, y.y, o.y), fmaf(g, y.z, o.z), fmaf(g, y.w, o.w));
+                    }
+                }
+            }
+            if (shares == 1) {
+                if (channel < D) write_row<D>(a, border.x, r, channel, o, top, sum);
+            } else {
+                if (channel < D) *reinterpret_cast<float4*>(parts[warp] + channel) = o;
+                if (lane == 0) *reinterpret_cast<float2*>(parts[warp] + D) = make_float2(top, sum);
+            }
+        }
+        if (shares > 1) {                      // (then one round takes all rows)
+            __syncthreads();
+            if (mine && warp % shares == 0 && lane < 8)
+                join_few<D>(a, border.x, r, min(shares, (count + each - 1) / each), lane, [&](int i) { return parts[warp + i]; }, nullptr);
+        }
+    }
 }
 
 template <int F, int D, int NT, bool ONE>
@@ -853,7 +890,7 @@ int launch(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
     launch_chained(attend_kernel<F, D, NT, ONE>, dim3(p.ctas), dim3(32 * S::WARPS), smem, st, a);
     const int rc = cuda_status(cudaGetLastError(), "paged_attention launch");
     if (rc != AKV_OK || !joined || p.ctas == 1) return rc;
-    launch_chained(join_kernel<D, NT>, dim3(p.ctas), dim3(32 * 8 * NT), 0, st, a);
+    launch_chained(join_kernel<D, NT>, dim3(p.ctas), dim3(32 * JOINERS), 0, st, a);
     return cuda_status(cudaGetLastError(), "paged_attention join launch");
 }
 template <int F, int D, int NT>
