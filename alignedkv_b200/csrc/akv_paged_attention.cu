@@ -16,6 +16,16 @@ Plan plan_of(int rows, int D) {
     return p;
 }
 
+// CTAs of a cluster per unit, where that is better than equal runs over all SMs, or 0.  A cluster joins its records itself, without a second
+// kernel and without adding up lengths; but its SMs are a power of two per unit, and all of them wait for the longest sequence.  So: where units leave SMs
+// idle, and the longest sequence that the table can hold gives a warp few chunks.
+int team_of(long long units, long long most_chunks, int sms, int warps) {
+    int team = 8;
+    while (team > 1 && units * team > sms * 7 / 8) team /= 2;
+    if (units * team > sms || most_chunks > (units * team >= sms / 2 ? 8 : 3) * (long long)warps * team) return 0;
+    return team;
+}
+
 }  // namespace
 }  // namespace akv
 
@@ -60,6 +70,7 @@ int akv_paged_attention(const akv_pool* pool, const void* q, const void* pages, 
     a.ctas = p.ctas;
     a.record = 8 * p.nt * (D + 4);
     a.scale2 = scale * LOG2E;
+    a.team = team_of(bsz * pool->n_kv_heads * p.groups, ((long long)width * pool->page_size + CHUNK - 1) / CHUNK, p.ctas, p.nt <= 2 ? 12 : 8);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool joined = (long long)width * pool->page_size > CHUNK;      // (units of one chunk are nobody else's)
     if (pool->format == AKV_PAGE_FP16) return launch_attend_fp16(a, p, D, joined, st);

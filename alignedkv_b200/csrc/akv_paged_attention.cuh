@@ -181,8 +181,9 @@ struct Ring {
     int units, end, at, n, h, token, stop, page[PAGES];
     uint32_t gone;                       // PAGES bits a step, the oldest in the lowest: the page is not there
 
-    __device__ __forceinline__ Ring(const AttendArgs& args, const int* lengths, uint32_t to, int of_lane, int run_units, int first, int last)
-        : a(args), cum(lengths), base(to), lane(of_lane), put(0), get(0), units(run_units), end(last), at(first), gone(0) {
+    // (begins with a part whose first chunk is `from`, and ends in front of chunk `last`)
+    __device__ __forceinline__ Ring(const AttendArgs& args, const int* lengths, uint32_t to, int of_lane, int run_units, const Part& begin, int from, int last)
+        : a(args), cum(lengths), base(to), lane(of_lane), put(0), get(0), part(begin), units(run_units), end(last), at(from), gone(0) {
         const int bytes = lane * 16;
         mine = piece<ROW>(bytes / ROW, bytes % ROW / 16);
         more = nullptr;
@@ -197,7 +198,6 @@ struct Ring {
                 per_token = 1;
             }
         }
-        part.find(cum, units, sequence_with(cum, a.B, units, at), at, end);
         enter();
         look();
 #pragma unroll 1
@@ -707,7 +707,50 @@ __device__ __forceinline__ void join_few(const AttendArgs& a, int unit, int r, i
     if (record && sub == 0) *reinterpret_cast<float2*>(record + D) = make_float2(top, sum);
 }
 
-template <int F, int D, int NT, bool ONE>
+// Joins row r of `count` records by `shares` warps, of which this is number `share`, through parts [shares][D + 4] in shared memory; row(i): the i-th.
+// Every warp of the block calls it (sync), those without a row with count 0.
+template <int D, class Fn>
+__device__ __forceinline__ void join_many(const AttendArgs& a, int unit, int r, int count, int share, int shares, int lane, float (*parts)[D + 4], Fn row) {
+    const int each = (count + shares - 1) / shares, first = share * each, last = min(count, first + each), channel = 4 * lane;
+    float top = -INFINITY, sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);          // (4 channels a lane, of 128; of 64 half of the lanes have none)
+    for (int i0 = first; i0 < last; i0 += 32) {
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (i0 + lane < last) ml = *reinterpret_cast<const float2*>(row(i0 + lane) + D);
+        float m = ml.x;
+#pragma unroll
+        for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
+        m = fmaxf(m, top);
+        const float base = m == -INFINITY ? 0.f : m, was = ex2(top - base), f = ex2(ml.x - base);
+        o = make_float4(o.x * was, o.y * was, o.z * was, o.w * was);
+        sum *= was;
+        top = m;
+        const int here = min(32, last - i0);
+#pragma unroll 8
+        for (int i = 0; i < here; ++i) {
+            const float g = __shfl_sync(0xFFFFFFFFu, f, i);
+            sum = fmaf(g, __shfl_sync(0xFFFFFFFFu, ml.y, i), sum);
+            if (channel < D) {
+                const float4 y = *reinterpret_cast<const float4*>(row(i0 + i) + channel);
+                o = make_float4(fmaf(g, y.x, o.x), fmaf(g, y.y, o.y), fmaf(g, y.z, o.z), fmaf(g, y.w, o.w));
+            }
+        }
+    }
+    if (shares == 1) {
+        if (count > 0 && channel < D) write_row<D>(a, unit, r, channel, o, top, sum);
+        return;
+    }
+    if (count > 0) {
+        if (channel < D) *reinterpret_cast<float4*>(parts[share] + channel) = o;
+        if (lane == 0) *reinterpret_cast<float2*>(parts[share] + D) = make_float2(top, sum);
+    }
+    __syncthreads();
+    if (count > 0 && share == 0 && lane < 8) join_few<D>(a, unit, r, min(shares, (count + each - 1) / each), lane, [&](int i) { return parts[i]; }, nullptr);
+    __syncthreads();
+}
+
+// TEAM: a cluster of CTAs has one unit, and its records are joined there.
+template <int F, int D, int NT, bool ONE, bool TEAM>
 __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(AttendArgs a) {
     using S = Shape<F, D, NT>;
     constexpr int WARPS = S::WARPS;
@@ -717,28 +760,44 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
     __shared__ int4 s_task[2 * WARPS];                         // unit, its first of s_slots, how many, where they go
     __shared__ int s_slots[2 * WARPS];
     __shared__ int2 s_border;
+    __shared__ __align__(16) float s_parts[TEAM ? WARPS : 1][D + 4];
     pdl_turn();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    add_lengths<32 * WARPS>(a, cum, sums);
     const int units = a.pool.H * a.groups;
-    const Deal deal(cum[a.B] * units, gridDim.x, WARPS);
-    const int me = blockIdx.x * deal.per_cta + warp;
+    // what is dealt: the chunks of all units to all warps, or the chunks of the cluster's unit to its warps
+    Part part;
+    int total, ctas = gridDim.x, cta = blockIdx.x;
+    if constexpr (TEAM) {
+        ctas = a.team;
+        part.unit = blockIdx.x / ctas;
+        cta = blockIdx.x - part.unit * ctas;
+        part.b = part.unit / units;
+        total = part.chunks = chunks_of(length_of(a.pool, part.b));
+    } else {
+        add_lengths<32 * WARPS>(a, cum, sums);
+        total = cum[a.B] * units;
+    }
+    const Deal deal(total, ctas, WARPS);
+    const int me = cta * deal.per_cta + warp;
     int at = 0, end = 0;
     if (warp < deal.per_cta) {
         at = deal.start(me);
         end = deal.start(me + 1);
     }
-    if (lane < 2) s_unit[2 * warp + lane] = -1;
+    if (!TEAM && lane < 2) s_unit[2 * warp + lane] = -1;
     __syncwarp();
     // Records: of a part that ends its run in the run's ring, which nobody needs any more; of one in front of others in global memory.
     float* last_record = reinterpret_cast<float*>(rings + warp * S::OWN);
     float* first_record = a.part + (2ll * gridDim.x + blockIdx.x * WARPS + warp) * S::RECORD;
     if (at < end) {
-        Ring<F, D, NT, ONE> ring(a, cum, smem_u32(last_record), lane, units, at, end);
+        if constexpr (TEAM) {
+            part.first = at;
+            part.last = end;
+        } else {
+            part.find(cum, units, sequence_with(cum, a.B, units, at), at, end);
+        }
+        Ring<F, D, NT, ONE> ring(a, cum, smem_u32(last_record), lane, units, part, at, end);
         Unit<F, D, NT, ONE> unit(a, lane, smem_u32(last_record));
-        Part part;
-        part.b = ring.part.b;                                  // (or a later one: found from the run's beginning)
-        part.find(cum, units, sequence_with(cum, a.B, units, at), at, end);
         for (;;) {
             const int n = length_of(a.pool, part.b), stop = min(n, part.last * CHUNK);
             int seen[NT][2];
@@ -768,17 +827,32 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
             if (part.whole()) {
                 unit.write(part.unit);
             } else {
-                const bool over = at >= end;
+                const bool over = TEAM || at >= end;
                 if (over) {
                     cp_async_wait<0>();
                     __syncwarp();
                 }
                 unit.record(over ? last_record : first_record);
-                if (lane == 0) s_unit[2 * warp + over] = part.unit;
+                if (!TEAM && lane == 0) s_unit[2 * warp + over] = part.unit;
             }
-            if (at >= end) break;
+            if (TEAM || at >= end) break;
             part.find(cum, units, part.b, at, end);
         }
+    }
+    if constexpr (TEAM) {
+        if (total == 1) return;                                // (written; the same in the whole cluster)
+        cluster_sync();
+        // Runs that got something, in order; the cluster's CTAs take the rows in turn, all warps of a CTA one row.
+        const int count = min(total, deal.per_cta * ctas);
+        for (int r = cta; r < a.rows; r += ctas)
+            join_many<D>(a, part.unit, r, count, warp, WARPS, lane, s_parts, [&](int i) -> const float* {
+                const int c = i / deal.per_cta;
+                unsigned long long there;
+                asm("mapa.u64 %0, %1, %2;\n" : "=l"(there) : "l"(rings + (i - c * deal.per_cta) * S::OWN), "r"(c));
+                return reinterpret_cast<const float*>(there) + r * (D + 4);
+            });
+        cluster_sync();                                        // (nobody leaves while its records are read)
+        return;
     }
     __syncthreads();
     // A unit whose records all are in this CTA is written, of another one record is left: the CTA's first where it began in front of it, else its
@@ -826,54 +900,16 @@ __global__ void __launch_bounds__(32 * JOINERS) join_kernel(AttendArgs a) {
     const int2 border = borders(a)[blockIdx.x];
     if (border.x < 0) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, from = blockIdx.x, count = border.y - from + 1;
-    const int shares = max(1, JOINERS / a.rows), each = (count + shares - 1) / shares;     // (warps of a row, records of each)
-    for (int r0 = 0; r0 < a.rows; r0 += JOINERS / shares) {
-        const int r = r0 + warp / shares, first = warp % shares * each, last = min(count, first + each);
-        const bool mine = warp / shares < JOINERS / shares && r < a.rows;
-        if (mine) {
-            // (4 channels a lane, of 128; of 64 half of the lanes have none)
-            const int channel = 4 * lane;
-            float top = -INFINITY, sum = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            auto row = [&](int i) { return a.part + ((long long)(2 * (from + i) + (i == 0)) * 8 * NT + r) * (D + 4); };
-            for (int i0 = first; i0 < last; i0 += 32) {
-                float2 ml = make_float2(-INFINITY, 0.f);
-                if (i0 + lane < last) ml = *reinterpret_cast<const float2*>(row(i0 + lane) + D);
-                float m = ml.x;
-#pragma unroll
-                for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
-                m = fmaxf(m, top);
-                const float base = m == -INFINITY ? 0.f : m, was = ex2(top - base), f = ex2(ml.x - base);
-                o = make_float4(o.x * was, o.y * was, o.z * was, o.w * was);
-                sum *= was;
-                top = m;
-                const int here = min(32, last - i0);
-#pragma unroll 8
-                for (int i = 0; i < here; ++i) {
-                    const float g = __shfl_sync(0xFFFFFFFFu, f, i);
-                    sum = fmaf(g, __shfl_sync(0xFFFFFFFFu, ml.y, i), sum);
-                    if (channel < D) {
-                        const float4 y = *reinterpret_cast<const float4*>(row(i0 + i) + channel);
-                        o = make_float4(fmaf(g, y.x, o.x), fmaf(g, y.y, o.y), fmaf(g, y.z, o.z), fmaf(g, y.w, o.w));
-                    }
-                }
-            }
-            if (shares == 1) {
-                if (channel < D) write_row<D>(a, border.x, r, channel, o, top, sum);
-            } else {
-                if (channel < D) *reinterpret_cast<float4*>(parts[warp] + channel) = o;
-                if (lane == 0) *reinterpret_cast<float2*>(parts[warp] + D) = make_float2(top, sum);
-            }
-        }
-        if (shares > 1) {                      // (then one round takes all rows)
-            __syncthreads();
-            if (mine && warp % shares == 0 && lane < 8)
-                join_few<D>(a, border.x, r, min(shares, (count + each - 1) / each), lane, [&](int i) { return parts[warp + i]; }, nullptr);
-        }
+    const int shares = max(1, JOINERS / a.rows), at_once = JOINERS / shares, mine = warp / shares;      // (warps of a row, rows at a time)
+    for (int r0 = 0; r0 < a.rows; r0 += at_once) {
+        const int r = r0 + mine;
+        join_many<D>(a, border.x, r, mine < at_once && r < a.rows ? count : 0, warp % shares, shares, lane, parts + mine * shares, [&](int i) {
+            return a.part + ((long long)(2 * (from + i) + (i == 0)) * 8 * NT + r) * (D + 4);
+        });
     }
 }
 
-template <int F, int D, int NT, bool ONE>
+template <int F, int D, int NT, bool ONE, bool TEAM>
 int launch(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
     using S = Shape<F, D, NT>;
     static_assert(S::WARPS <= MOST_WARPS, "workspace");
@@ -883,11 +919,15 @@ int launch(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && set_for != dev) {
         // (the most it is ever launched with)
-        e = cudaFuncSetAttribute(attend_kernel<F, D, NT, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM + 4097 * 4);
+        e = cudaFuncSetAttribute(attend_kernel<F, D, NT, ONE, TEAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM + 4097 * 4);
         if (e == cudaSuccess) set_for = dev;
     }
     if (e != cudaSuccess) return cuda_status(e, "paged_attention");
-    launch_chained(attend_kernel<F, D, NT, ONE>, dim3(p.ctas), dim3(32 * S::WARPS), smem, st, a);
+    if constexpr (TEAM) {
+        launch_cluster(attend_kernel<F, D, NT, ONE, TEAM>, a.team, dim3((unsigned)(a.B * a.pool.H * a.groups * a.team)), dim3(32 * S::WARPS), S::SMEM, st, a);
+        return cuda_status(cudaGetLastError(), "paged_attention launch");
+    }
+    launch_chained(attend_kernel<F, D, NT, ONE, TEAM>, dim3(p.ctas), dim3(32 * S::WARPS), smem, st, a);
     const int rc = cuda_status(cudaGetLastError(), "paged_attention launch");
     if (rc != AKV_OK || !joined || p.ctas == 1) return rc;
     launch_chained(join_kernel<D, NT>, dim3(p.ctas), dim3(32 * JOINERS), 0, st, a);
@@ -896,8 +936,9 @@ int launch(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
 template <int F, int D, int NT>
 int launch_pages(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
     if constexpr (Shape<F, D, NT>::U > 1)
-        if (Shape<F, D, NT>::TOKENS > 1 << a.pool.shift) return launch<F, D, NT, false>(a, p, joined, st);
-    return launch<F, D, NT, true>(a, p, joined, st);
+        if (Shape<F, D, NT>::TOKENS > 1 << a.pool.shift)
+            return a.team ? launch<F, D, NT, false, true>(a, p, joined, st) : launch<F, D, NT, false, false>(a, p, joined, st);
+    return a.team ? launch<F, D, NT, true, true>(a, p, joined, st) : launch<F, D, NT, true, false>(a, p, joined, st);
 }
 template <int F, int D>
 int launch_rows(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {

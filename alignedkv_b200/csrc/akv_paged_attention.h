@@ -11,7 +11,7 @@ struct AttendArgs {
     const __half* q;
     __half* out;
     float *lse, *part;              // part: two records of each CTA, one of each warp, a border of each CTA
-    int B, T, G, groups, rows, ctas, record;    // record: floats of one
+    int B, T, G, groups, rows, ctas, record, team;    // record: floats of one; team: CTAs of a cluster that has a unit to itself, or 0
     // groups: units per (sequence, KV head); rows: query rows of a unit
     float scale2;                   // scale * log2(e)
 };

@@ -204,6 +204,12 @@ def test_attention(form, B, H, group, T, D, page, lens):
     check(pool, pages, N, form, q, lens, out, lse, page=page)
     again, _ = paged_ops.paged_attention(pool, q, pages, i32(*lens), lse=True)
     assert torch.equal(out, again)
+    # the same behind a table for long sequences, whose entries behind the last token may be anything: the work is cut up in another way
+    wide = torch.cat([pages, torch.randint(-2 ** 31, 2 ** 31 - 1, (B, 200000 // page), generator=gen).to(torch.int32).to(DEV)], 1)
+    out, lse = paged_ops.paged_attention(pool, q, wide, i32(*lens), lse=True)
+    check(pool, pages, N, form, q, lens, out, lse, page=page)
+    again, _ = paged_ops.paged_attention(pool, q, wide, i32(*lens), lse=True)
+    assert torch.equal(out, again)
 
 
 @pytest.mark.parametrize("form", ref.FORMS)
@@ -233,6 +239,9 @@ def test_attention_past_pages_given_up(form):
     out, lse = paged_ops.paged_attention(pool, q, pages, i32(*lens), lse=True)
     check(pool, pages, N, form, q, lens, out, lse, page=32)
     assert not out[2].any()
+    wide = torch.cat([pages, torch.full((4, 3000), -1, dtype=torch.int32, device=DEV)], 1)
+    out, lse = paged_ops.paged_attention(pool, q, wide, i32(*lens), lse=True)
+    check(pool, pages, N, form, q, lens, out, lse, page=32)
 
 
 @pytest.mark.parametrize("form", ref.FORMS)
