@@ -707,13 +707,13 @@ __device__ __forceinline__ void join_few(const AttendArgs& a, int unit, int r, i
     if (record && sub == 0) *reinterpret_cast<float2*>(record + D) = make_float2(top, sum);
 }
 
-// Joins row r of `count` records by `shares` warps, of which this is number `share`, through parts [shares][D + 4] in shared memory; row(i): the i-th.
-// Every warp of the block calls it (sync), those without a row with count 0.
+// Joins the records first .. last - 1 of a row by a warp, 4 channels a lane (of 128; of 64 half of the lanes have none); row(i): the i-th.
 template <int D, class Fn>
-__device__ __forceinline__ void join_many(const AttendArgs& a, int unit, int r, int count, int share, int shares, int lane, float (*parts)[D + 4], Fn row) {
-    const int each = (count + shares - 1) / shares, first = share * each, last = min(count, first + each), channel = 4 * lane;
-    float top = -INFINITY, sum = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);          // (4 channels a lane, of 128; of 64 half of the lanes have none)
+__device__ __forceinline__ void join_row(int first, int last, int lane, Fn row, float4& o, float& top, float& sum) {
+    const int channel = 4 * lane;
+    top = -INFINITY;
+    sum = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i0 = first; i0 < last; i0 += 32) {
         float2 ml = make_float2(-INFINITY, 0.f);
         if (i0 + lane < last) ml = *reinterpret_cast<const float2*>(row(i0 + lane) + D);
@@ -736,12 +736,21 @@ __device__ __forceinline__ void join_many(const AttendArgs& a, int unit, int r, 
             }
         }
     }
+}
+// Row r of `count` records by `shares` warps, of which this is number `share`, through parts [shares][D + 4] in shared memory.  Every warp of the
+// block calls it (it synchronises), those without a row with count 0.
+template <int D, class Fn>
+__device__ __forceinline__ void join_many(const AttendArgs& a, int unit, int r, int count, int share, int shares, int lane, float (*parts)[D + 4], Fn row) {
+    const int each = (count + shares - 1) / shares, first = share * each;
+    float4 o;
+    float top, sum;
+    join_row<D>(first, min(count, first + each), lane, row, o, top, sum);
     if (shares == 1) {
-        if (count > 0 && channel < D) write_row<D>(a, unit, r, channel, o, top, sum);
+        if (count > 0 && 4 * lane < D) write_row<D>(a, unit, r, 4 * lane, o, top, sum);
         return;
     }
     if (count > 0) {
-        if (channel < D) *reinterpret_cast<float4*>(parts[share] + channel) = o;
+        if (4 * lane < D) *reinterpret_cast<float4*>(parts[share] + 4 * lane) = o;
         if (lane == 0) *reinterpret_cast<float2*>(parts[share] + D) = make_float2(top, sum);
     }
     __syncthreads();
@@ -879,19 +888,35 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
         if (lane == 0) borders(a)[blockIdx.x] = s_border;
     }
     __syncthreads();
-    for (int x = warp * 4 + (lane >> 3); x < s_tasks * a.rows; x += 4 * WARPS) {
+    // A row by a warp where there are few (8 x 32 heads x 4096 tokens: 51.6 us, four rows at a time 55.3), else four (32 sequences of 5 tokens and 4
+    // heads a row: 66 us, one 81).
+    const int rows = s_tasks * a.rows;
+    const bool few = rows <= 2 * WARPS;
+    for (int x = few ? warp : warp * 4 + (lane >> 3); x < rows; x += few ? WARPS : 4 * WARPS) {
         const int i = x / a.rows, r = x - i * a.rows;
         const int4 task = s_task[i];
         float* record = task.w < 0 ? nullptr : a.part + ((long long)(2 * blockIdx.x + task.w) * 8 * NT + r) * (D + 4);
-        join_few<D>(a, task.x, r, task.z, lane & 7, [&](int k) {
+        auto row = [&](int k) {
             const int slot = s_slots[task.y + k], w = slot >> 1;
             return (slot & 1 ? reinterpret_cast<const float*>(rings + w * S::OWN) : a.part + (2ll * gridDim.x + blockIdx.x * WARPS + w) * S::RECORD) + r * (D + 4);
-        }, record);
+        };
+        if (few) {
+            float4 o;
+            float top, sum;
+            join_row<D>(0, task.z, lane, row, o, top, sum);
+            if (4 * lane < D) {
+                if (record) *reinterpret_cast<float4*>(record + 4 * lane) = o;
+                else write_row<D>(a, task.x, r, 4 * lane, o, top, sum);
+            }
+            if (record && lane == 0) *reinterpret_cast<float2*>(record + D) = make_float2(top, sum);
+        } else {
+            join_few<D>(a, task.x, r, task.z, lane & 7, row, record);
+        }
     }
 }
 
-// One CTA per CTA of attend_kernel: where a unit begins there and ends in another one, its records are joined, a row by as many warps as there are
-// for it, whose parts are joined in shared memory.
+// One CTA per CTA of attend_kernel: where a unit begins there and ends in another one, its records are joined: a row by a warp, by
+// all that there are for it where the records are many (their parts are joined in shared memory).
 constexpr int JOINERS = 16;
 template <int D, int NT>
 __global__ void __launch_bounds__(32 * JOINERS) join_kernel(AttendArgs a) {
@@ -900,7 +925,7 @@ __global__ void __launch_bounds__(32 * JOINERS) join_kernel(AttendArgs a) {
     const int2 border = borders(a)[blockIdx.x];
     if (border.x < 0) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, from = blockIdx.x, count = border.y - from + 1;
-    const int shares = max(1, JOINERS / a.rows), at_once = JOINERS / shares, mine = warp / shares;      // (warps of a row, rows at a time)
+    const int shares = count <= 8 ? 1 : max(1, JOINERS / a.rows), at_once = JOINERS / shares, mine = warp / shares;      // (warps of a row, rows at a time)
     for (int r0 = 0; r0 < a.rows; r0 += at_once) {
         const int r = r0 + mine;
         join_many<D>(a, border.x, r, mine < at_once && r < a.rows ? count : 0, warp % shares, shares, lane, parts + mine * shares, [&](int i) {
