@@ -915,22 +915,51 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
     }
 }
 
-// One CTA per CTA of attend_kernel: where a unit begins there and ends in another one, its records are joined: a row by a warp, by
-// all that there are for it where the records are many (their parts are joined in shared memory).
+// One CTA per CTA of attend_kernel: where a unit begins there and ends in another one, its records are joined: a row by a warp, by all that
+// there are for it where the records are many (their parts are joined in shared memory).  Bound by latency: the first two records, if there are any, lie
+// where they always do and are loaded before it is known whether there are.
 constexpr int JOINERS = 16;
 template <int D, int NT>
 __global__ void __launch_bounds__(32 * JOINERS) join_kernel(AttendArgs a) {
     __shared__ __align__(16) float parts[JOINERS][D + 4];
     pdl_turn();
-    const int2 border = borders(a)[blockIdx.x];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, from = blockIdx.x;
+    auto record = [&](int r, int i) { return a.part + ((long long)(2 * (from + i) + (i == 0)) * 8 * NT + r) * (D + 4); };
+    float4 y[2];
+    float2 ml[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const bool there = warp < a.rows && from + 1 < a.ctas;
+        y[i] = there && 4 * lane < D ? *reinterpret_cast<const float4*>(record(warp, i) + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        ml[i] = there ? *reinterpret_cast<const float2*>(record(warp, i) + D) : make_float2(0.f, 0.f);
+    }
+    const int2 border = borders(a)[from];
     if (border.x < 0) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, from = blockIdx.x, count = border.y - from + 1;
-    const int shares = count <= 8 ? 1 : max(1, JOINERS / a.rows), at_once = JOINERS / shares, mine = warp / shares;      // (warps of a row, rows at a time)
+    const int count = border.y - from + 1;
+    if (count <= 8) {
+        for (int r = warp; r < a.rows; r += JOINERS) {
+            float4 o;
+            float top, sum;
+            if (r == warp) {
+                join_row<D>(2, count, lane, [&](int i) { return record(r, i); }, o, top, sum);
+                const float m = fmaxf(top, fmaxf(ml[0].x, ml[1].x)), base = m == -INFINITY ? 0.f : m;
+                const float f = ex2(top - base), f0 = ex2(ml[0].x - base), f1 = ex2(ml[1].x - base);
+                o = make_float4(fmaf(f0, y[0].x, fmaf(f1, y[1].x, f * o.x)), fmaf(f0, y[0].y, fmaf(f1, y[1].y, f * o.y)),
+                                fmaf(f0, y[0].z, fmaf(f1, y[1].z, f * o.z)), fmaf(f0, y[0].w, fmaf(f1, y[1].w, f * o.w)));
+                sum = fmaf(f0, ml[0].y, fmaf(f1, ml[1].y, f * sum));
+                top = m;
+            } else {
+                join_row<D>(0, count, lane, [&](int i) { return record(r, i); }, o, top, sum);
+            }
+            if (4 * lane < D) write_row<D>(a, border.x, r, 4 * lane, o, top, sum);
+        }
+        return;
+    }
+    const int shares = max(1, JOINERS / a.rows), at_once = JOINERS / shares, mine = warp / shares;      // (warps of a row, rows at a time)
     for (int r0 = 0; r0 < a.rows; r0 += at_once) {
         const int r = r0 + mine;
-        join_many<D>(a, border.x, r, mine < at_once && r < a.rows ? count : 0, warp % shares, shares, lane, parts + mine * shares, [&](int i) {
-            return a.part + ((long long)(2 * (from + i) + (i == 0)) * 8 * NT + r) * (D + 4);
-        });
+        join_many<D>(a, border.x, r, mine < at_once && r < a.rows ? count : 0, warp % shares, shares, lane, parts + mine * shares,
+                     [&](int i) { return record(r, i); });
     }
 }
 
