@@ -17,13 +17,13 @@ Plan plan_of(int rows, int D) {
 }
 
 // CTAs of a cluster per unit, where that is better than equal runs over all SMs, or 0.  A cluster joins its records itself, without a second
-// kernel and without adding up lengths; but its SMs are a power of two per unit, and all of them wait for the longest sequence.  So: where units leave SMs
-// idle, and the longest sequence that the table can hold gives a warp few chunks.
+// kernel and without adding up lengths; but its SMs are a power of two per unit, all of them wait for the longest sequence, and not all SMs can be in
+// clusters of one size.  So: where units leave SMs idle, and the longest sequence that the table can hold gives a warp few chunks.  No more CTAs than
+// give every warp a chunk.
 int team_of(long long units, long long most_chunks, int sms, int warps) {
     int team = 8;
-    while (team > 1 && units * team > sms * 7 / 8) team /= 2;
-    if (units * team > sms || most_chunks > (units * team >= sms / 2 ? 8 : 3) * (long long)warps * team) return 0;
-    return team;
+    while (team > 1 && (units * team > sms * 3 / 4 || (team / 2) * warps >= most_chunks)) team /= 2;
+    return units * team > sms || most_chunks > 4ll * warps * team ? 0 : team;
 }
 
 }  // namespace

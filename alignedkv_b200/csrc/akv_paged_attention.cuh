@@ -5,7 +5,7 @@
 //   s_rj = scale q_r . k_j, o_r = sum_j exp(s_rj - m_r) v_j / l_r, l_r = sum_j exp(s_rj - m_r), over the tokens j that row r sees.
 //
 // Every byte of the tokens is read once: bound by HBM, and for the 4-bit format almost as much by the instructions that unpack it.
-// Work: a unit is up to 16 query rows of one (sequence, KV head), its tokens in chunks of 32.  The chunks of all units in a row are dealt to
+// Work: a unit is up to 16 query rows of one (sequence, KV head), its tokens in chunks of 64.  The chunks of all units in a row are dealt to
 // the warps in equal contiguous runs: lengths are only known on the device, and every SM gets the same whatever they are.  Each CTA
 // adds up the lengths itself.  A warp needs no other one: codes come straight into registers as operand fragments (no shared memory is
 // on their way), the next step's while this one's are multiplied.  Where a run begins or ends inside a unit it leaves a record, and
@@ -851,15 +851,18 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
     if constexpr (TEAM) {
         if (total == 1) return;                                // (written; the same in the whole cluster)
         cluster_sync();
-        // Runs that got something, in order; the cluster's CTAs take the rows in turn, all warps of a CTA one row.
-        const int count = min(total, deal.per_cta * ctas);
-        for (int r = cta; r < a.rows; r += ctas)
-            join_many<D>(a, part.unit, r, count, warp, WARPS, lane, s_parts, [&](int i) -> const float* {
+        // Runs that got something, in order; the cluster's CTAs take the rows in turn, a warp or more of them a row.
+        const int count = min(total, deal.per_cta * ctas), rows = (a.rows - cta + ctas - 1) / ctas;
+        const int shares = count <= 8 ? 1 : max(1, WARPS / max(1, rows)), at_once = WARPS / shares, mine = warp / shares;
+        for (int x0 = 0; x0 < rows; x0 += at_once) {
+            const int x = x0 + mine, r = cta + x * ctas;
+            join_many<D>(a, part.unit, r, mine < at_once && x < rows ? count : 0, warp % shares, shares, lane, s_parts + mine * shares, [&](int i) -> const float* {
                 const int c = i / deal.per_cta;
                 unsigned long long there;
                 asm("mapa.u64 %0, %1, %2;\n" : "=l"(there) : "l"(rings + (i - c * deal.per_cta) * S::OWN), "r"(c));
                 return reinterpret_cast<const float*>(there) + r * (D + 4);
             });
+        }
         cluster_sync();                                        // (nobody leaves while its records are read)
         return;
     }

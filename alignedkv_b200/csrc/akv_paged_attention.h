@@ -4,7 +4,7 @@
 
 namespace akv {
 
-constexpr int CHUNK = 32, MOST_WARPS = 12;
+constexpr int CHUNK = 64, MOST_WARPS = 12;
 
 struct AttendArgs {
     Pool pool;
