@@ -19,11 +19,11 @@ Plan plan_of(int rows, int D) {
 // CTAs of a cluster per unit, where that is better than equal runs over all SMs, or 0.  A cluster joins its records itself, without a second
 // kernel and without adding up lengths; but its SMs are a power of two per unit, all of them wait for the longest sequence, and not all SMs can be in
 // clusters of one size.  So: where units leave SMs idle, and the longest sequence that the table can hold gives a warp few chunks.  No more CTAs than
-// give every warp a chunk.
+// leave half of the warps without a chunk.
 int team_of(long long units, long long most_chunks, int sms, int warps) {
     int team = 8;
-    while (team > 1 && (units * team > sms * 3 / 4 || (team / 2) * warps >= most_chunks)) team /= 2;
-    return units * team > sms || most_chunks > 4ll * warps * team ? 0 : team;
+    while (team > 1 && (units * team > sms * 3 / 4 || (team / 2) * warps >= 2 * most_chunks)) team /= 2;
+    return units * team > sms || most_chunks > 8ll * warps * team ? 0 : team;
 }
 
 }  // namespace
@@ -56,6 +56,7 @@ int akv_paged_attention(const akv_pool* pool, const void* q, const void* pages, 
     AKV_REQUIRE(scratch_bytes >= p.bytes, AKV_ERR_SHAPE, "paged_attention: scratch of %lld bytes is too small", scratch_bytes);
     AKV_REQUIRE((long long)pool->n_pages * pool->n_kv_heads * pool->page_size <= 1ll << 32 && (long long)bsz * width < INT_MAX, AKV_ERR_OVERFLOW,
                 "paged_attention: a pool of more than 2^32 rows");
+    AKV_REQUIRE((long long)bsz * tokens * pool->n_kv_heads * group < INT_MAX / 256, AKV_ERR_OVERFLOW, "paged_attention: too many query rows");
     const long long most = ((long long)width * pool->page_size + CHUNK - 1) / CHUNK * bsz * pool->n_kv_heads * p.groups;
     AKV_REQUIRE(most < INT_MAX, AKV_ERR_OVERFLOW, "paged_attention: too many chunks of %d tokens", CHUNK);
     a.q = static_cast<const __half*>(q);
@@ -65,12 +66,13 @@ int akv_paged_attention(const akv_pool* pool, const void* q, const void* pages, 
     a.B = bsz;
     a.T = tokens;
     a.G = group;
+    a.over_g = (65536 + group - 1) / group;
     a.groups = p.groups;
     a.rows = p.rows;
     a.ctas = p.ctas;
     a.record = 8 * p.nt * (D + 4);
     a.scale2 = scale * LOG2E;
-    a.team = team_of(bsz * pool->n_kv_heads * p.groups, ((long long)width * pool->page_size + CHUNK - 1) / CHUNK, p.ctas, p.nt <= 2 ? 12 : 8);
+    a.team = team_of(bsz * pool->n_kv_heads * p.groups, ((long long)width * pool->page_size + TEAM_CHUNK - 1) / TEAM_CHUNK, p.ctas, p.nt <= 2 ? 12 : 8);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool joined = (long long)width * pool->page_size > CHUNK;      // (units of one chunk are nobody else's)
     if (pool->format == AKV_PAGE_FP16) return launch_attend_fp16(a, p, D, joined, st);

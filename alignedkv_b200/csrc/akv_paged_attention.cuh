@@ -77,7 +77,8 @@ __device__ __forceinline__ uint32_t halves_bits(float lo, float hi) {
 }
 // ---------------------------------------------------------------- which chunks are whose
 // cum[b]: chunks of one unit of the sequences before b; a sequence without tokens has one, so that its rows are written.
-__device__ __forceinline__ int chunks_of(int n) { return max(1, (n + CHUNK - 1) / CHUNK); }
+template <int TOKENS>
+__device__ __forceinline__ int chunks_of(int n) { return max(1, (n + TOKENS - 1) / TOKENS); }
 
 template <int THREADS>
 __device__ __forceinline__ void add_lengths(const AttendArgs& a, int* cum, int* sums) {
@@ -85,7 +86,7 @@ __device__ __forceinline__ void add_lengths(const AttendArgs& a, int* cum, int* 
     int before = 0;
     for (int b0 = 0; b0 < a.B; b0 += THREADS) {
         const int b = b0 + tid;
-        int x = b < a.B ? chunks_of(length_of(a.pool, b)) : 0;
+        int x = b < a.B ? chunks_of<CHUNK>(length_of(a.pool, b)) : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
@@ -123,14 +124,20 @@ struct Deal {
 };
 // A run's part of one unit.
 struct Part {
-    int b, unit, first, last, chunks;   // sequence; unit of all; chunks of the unit: [first, last) of `chunks`
+    int b, unit, h, group, first, last, chunks;   // sequence; unit of all; KV head, group of its rows; chunks of the unit: [first, last) of `chunks`
+    // u: of the sequence's units
+    __device__ __forceinline__ void place(int u, int groups) {
+        h = groups == 1 ? u : (unsigned)u / (unsigned)groups;
+        group = u - h * groups;
+    }
     // The part that begins with chunk `at`, of a run that ends with `end`; b: where to begin looking.
-    __device__ __forceinline__ void find(const int* cum, int units, int b0, int at, int end) {
+    __device__ __forceinline__ void find(const int* cum, int units, int groups, int b0, int at, int end) {
         b = b0;
         while (at >= cum[b + 1] * units) ++b;
         chunks = cum[b + 1] - cum[b];
         const int rest = at - cum[b] * units, u = (unsigned)rest / (unsigned)chunks;
         unit = b * units + u;
+        place(u, groups);
         first = rest - u * chunks;
         last = min(chunks, first + end - at);
     }
@@ -148,13 +155,20 @@ __device__ __forceinline__ int sequence_with(const int* cum, int B, int units, i
 
 __device__ __forceinline__ int2* borders(const AttendArgs& a) { return reinterpret_cast<int2*>(a.part + (2ll + MOST_WARPS) * a.ctas * a.record); }
 
-// Row of q, out and lse [B,T,H*G] that row r of a unit stands for; -1 behind the last.
-__device__ __forceinline__ long long row_of(const AttendArgs& a, int unit, int r, int* query) {
-    const int group = unit % a.groups, bh = unit / a.groups, h = bh % a.pool.H, b = bh / a.pool.H, R = group * a.rows + r;
-    const int t = (unsigned)R / (unsigned)a.G;
-    *query = t;
-    if (r >= a.rows || t >= a.T) return -1;
-    return ((long long)b * a.T + t) * (a.pool.H * a.G) + h * a.G + R - t * a.G;
+// Rows of q, out and lse [B,T,H*G] that a unit's rows stand for.
+struct Rows {
+    int first, base;                    // first row of the unit among the KV head's T * G; row of the tensors for query 0, head 0 of the KV head
+    __device__ __forceinline__ Rows(const AttendArgs& a, int b, int h, int group) : first(group * a.rows), base(b * a.T * a.pool.H * a.G + h * a.G) {}
+    // The tensors' row of row r and its query; -1 behind the last.  (Fewer than 64 rows: the quotient by G is that of a multiplication.)
+    __device__ __forceinline__ int row(const AttendArgs& a, int r, int* query) const {
+        const int R = first + r, t = (R * a.over_g) >> 16;
+        *query = t;
+        return r >= a.rows || t >= a.T ? -1 : base + t * (a.pool.H * a.G) + R - t * a.G;
+    }
+};
+__device__ __forceinline__ Rows rows_of(const AttendArgs& a, int unit) {
+    const unsigned bh = (unsigned)unit / (unsigned)a.groups, b = bh / (unsigned)a.pool.H;
+    return Rows(a, b, bh - b * a.pool.H, unit - bh * a.groups);
 }
 
 // ---------------------------------------------------------------- a warp's ring
@@ -168,17 +182,17 @@ __device__ __forceinline__ int piece(int r, int c) {
 }
 
 // Steps of a run, copied to shared memory STEPS - 1 ahead by the warp's own asynchronous copies.  ONE: a step's tokens are in one page.
-template <int F, int D, int NT, bool ONE>
+template <int F, int D, int NT, bool ONE, bool TEAM>
 struct Ring {
     using S = Shape<F, D, NT>;
-    static constexpr int U = S::U, ROW = S::ROW, PAGES = ONE ? 1 : U;
+    static constexpr int U = S::U, ROW = S::ROW, PAGES = ONE ? 1 : U, TOKENS_OF = TEAM ? TEAM_CHUNK : CHUNK;    // (of a chunk)
     const AttendArgs& a;
     const int* cum;
     uint32_t base, mine;                 // of the ring; where this lane's first piece of codes goes within a tile
     const uint8_t* more;                 // this lane's piece of scales or exponents: its tensor, bytes of a token there
     int per_token, lane, put, get;
     Part part;                           // what is copied next
-    int units, end, at, n, h, token, stop, page[PAGES];
+    int units, end, at, n, token, stop, page[PAGES];
     uint32_t gone;                       // PAGES bits a step, the oldest in the lowest: the page is not there
 
     // (begins with a part whose first chunk is `from`, and ends in front of chunk `last`)
@@ -205,9 +219,8 @@ struct Ring {
     }
     __device__ __forceinline__ void enter() {
         n = length_of(a.pool, part.b);
-        h = part.unit / a.groups % a.pool.H;
-        token = part.first * CHUNK;
-        stop = min(n, part.last * CHUNK);
+        token = part.first * TOKENS_OF;
+        stop = min(n, part.last * TOKENS_OF);
     }
     // Pages of the step at `token`; -1 where there is none or nothing of the sequence in it.
     __device__ __forceinline__ void look() {
@@ -225,7 +238,7 @@ struct Ring {
             for (int u = 0; u < U; ++u) {
                 const int x = page[ONE ? 0 : u], from = ONE ? token : token + 16 * u;
                 const bool there = (unsigned)x < (unsigned)a.pool.n_pages;
-                const unsigned row = (((unsigned)(there ? x : 0) * (unsigned)a.pool.H + h) << a.pool.shift) + (from & ((1 << a.pool.shift) - 1)) + (ONE ? 16 * u : 0);
+                const unsigned row = (((unsigned)(there ? x : 0) * (unsigned)a.pool.H + part.h) << a.pool.shift) + (from & ((1 << a.pool.shift) - 1)) + (ONE ? 16 * u : 0);
                 const unsigned long long byte = (unsigned long long)row * ROW + lane * 16;
                 const uint8_t *k = a.pool.kc + byte, *v = a.pool.vc + byte;
                 const uint32_t tile = to + u * 32 * ROW;
@@ -247,7 +260,7 @@ struct Ring {
             if (token >= stop) {
                 at += part.last - part.first;
                 if (at < end) {
-                    part.find(cum, units, part.b, at, end);
+                    part.find(cum, units, a.groups, part.b, at, end);
                     enter();
                 }
             }
@@ -314,12 +327,12 @@ struct Unit {
         }
     }
 
-    __device__ __forceinline__ void begin(int unit) {
+    __device__ __forceinline__ void begin(const Rows& rows) {
         if constexpr (!S::FEW) __syncwarp();     // (the last unit's have been read)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             int query;
-            const long long row = row_of(a, unit, 8 * nt + g, &query);
+            const long long row = rows.row(a, 8 * nt + g, &query);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 uint2 w = make_uint2(0, 0);
@@ -631,13 +644,13 @@ struct Unit {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[nt][c] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][c], o);
     }
-    __device__ __forceinline__ void write(int unit) {
+    __device__ __forceinline__ void write(const Rows& rows) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 int query;
-                const long long row = row_of(a, unit, 8 * nt + 2 * t + c, &query);
+                const long long row = rows.row(a, 8 * nt + 2 * t + c, &query);
                 if (row < 0) continue;
                 const float inv = l[nt][c] == 0.f ? 0.f : 1.f / (l[nt][c] * LIFT);
 #pragma unroll
@@ -668,7 +681,7 @@ struct Unit {
 template <int D>
 __device__ __forceinline__ void write_row(const AttendArgs& a, int unit, int r, int channel, float4 x, float top, float sum) {
     int query;
-    const long long row = row_of(a, unit, r, &query);
+    const long long row = rows_of(a, unit).row(a, r, &query);
     if (row < 0) return;
     const float inv = sum == 0.f ? 0.f : 1.f / (sum * LIFT);
     const __half2 lo = __floats2half2_rn(x.x * inv, x.y * inv), hi = __floats2half2_rn(x.z * inv, x.w * inv);
@@ -781,7 +794,8 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
         part.unit = blockIdx.x / ctas;
         cta = blockIdx.x - part.unit * ctas;
         part.b = part.unit / units;
-        total = part.chunks = chunks_of(length_of(a.pool, part.b));
+        part.place(part.unit - part.b * units, a.groups);
+        total = part.chunks = chunks_of<TEAM_CHUNK>(length_of(a.pool, part.b));
     } else {
         add_lengths<32 * WARPS>(a, cum, sums);
         total = cum[a.B] * units;
@@ -803,22 +817,24 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
             part.first = at;
             part.last = end;
         } else {
-            part.find(cum, units, sequence_with(cum, a.B, units, at), at, end);
+            part.find(cum, units, a.groups, sequence_with(cum, a.B, units, at), at, end);
         }
-        Ring<F, D, NT, ONE> ring(a, cum, smem_u32(last_record), lane, units, part, at, end);
+        Ring<F, D, NT, ONE, TEAM> ring(a, cum, smem_u32(last_record), lane, units, part, at, end);
         Unit<F, D, NT, ONE> unit(a, lane, smem_u32(last_record));
         for (;;) {
-            const int n = length_of(a.pool, part.b), stop = min(n, part.last * CHUNK);
+            constexpr int TOKENS_OF = TEAM ? TEAM_CHUNK : CHUNK;
+            const Rows rows(a, part.b, part.h, part.group);
+            const int n = length_of(a.pool, part.b), stop = min(n, part.last * TOKENS_OF);
             int seen[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     int query;
-                    seen[nt][c] = row_of(a, part.unit, 8 * nt + 2 * unit.t + c, &query) < 0 ? 0 : n - a.T + 1 + query;
+                    seen[nt][c] = rows.row(a, 8 * nt + 2 * unit.t + c, &query) < 0 ? 0 : n - a.T + 1 + query;
                 }
-            unit.begin(part.unit);
-            int token = part.first * CHUNK;
+            unit.begin(rows);
+            int token = part.first * TOKENS_OF;
 #pragma unroll 1
             do {
                 uint32_t without;
@@ -834,7 +850,7 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
             unit.close();
             at += part.last - part.first;
             if (part.whole()) {
-                unit.write(part.unit);
+                unit.write(rows);
             } else {
                 const bool over = TEAM || at >= end;
                 if (over) {
@@ -845,7 +861,7 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
                 if (!TEAM && lane == 0) s_unit[2 * warp + over] = part.unit;
             }
             if (TEAM || at >= end) break;
-            part.find(cum, units, part.b, at, end);
+            part.find(cum, units, a.groups, part.b, at, end);
         }
     }
     if constexpr (TEAM) {

@@ -4,14 +4,14 @@
 
 namespace akv {
 
-constexpr int CHUNK = 64, MOST_WARPS = 12;
+constexpr int CHUNK = 64, TEAM_CHUNK = 32, MOST_WARPS = 12;       // (TEAM_CHUNK: where a cluster has a unit to itself)
 
 struct AttendArgs {
     Pool pool;
     const __half* q;
     __half* out;
     float *lse, *part;              // part: two records of each CTA, one of each warp, a border of each CTA
-    int B, T, G, groups, rows, ctas, record, team;    // record: floats of one; team: CTAs of a cluster that has a unit to itself, or 0
+    int B, T, G, groups, rows, ctas, record, team, over_g;    // record: floats of one; team: CTAs of a cluster that has a unit to itself, or 0; over_g: 2^16 / G, rounded up
     // groups: units per (sequence, KV head); rows: query rows of a unit
     float scale2;                   // scale * log2(e)
 };
