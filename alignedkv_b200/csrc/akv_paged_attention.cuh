@@ -193,6 +193,8 @@ struct Ring {
     int per_token, lane, put, get;
     Part part;                           // what is copied next
     int units, end, at, n, token, stop, page[PAGES];
+    int cached;                          // this lane's entry of the table, of the 32 from cached_from on
+    unsigned cached_from;
     uint32_t gone;                       // PAGES bits a step, the oldest in the lowest: the page is not there
 
     // (begins with a part whose first chunk is `from`, and ends in front of chunk `last`)
@@ -221,13 +223,20 @@ struct Ring {
         n = length_of(a.pool, part.b);
         token = part.first * TOKENS_OF;
         stop = min(n, part.last * TOKENS_OF);
+        cached_from = 1u << 31;              // (far from any page: the first look reads)
     }
-    // Pages of the step at `token`; -1 where there is none or nothing of the sequence in it.
+    // Pages of the step at `token`; -1 where there is none or nothing of the sequence in it.  The table is read 32 entries at a time, one per lane.
     __device__ __forceinline__ void look() {
 #pragma unroll
         for (int u = 0; u < PAGES; ++u) {
-            page[u] = -1;
-            if (token + 16 * u < n) page[u] = __ldg(a.pool.table + (unsigned)part.b * (unsigned)a.pool.width + ((token + 16 * u) >> a.pool.shift));
+            const int at_page = (token + 16 * u) >> a.pool.shift;
+            if (at_page - cached_from >= 32u) {
+                cached_from = at_page;
+                cached = -1;
+                if (at_page + lane <= (n - 1) >> a.pool.shift) cached = __ldg(a.pool.table + (unsigned)part.b * (unsigned)a.pool.width + at_page + lane);
+            }
+            const int x = __shfl_sync(0xFFFFFFFFu, cached, at_page - cached_from);
+            page[u] = token + 16 * u < n ? x : -1;
         }
     }
     // The next step, if there is one; always a group, so that the groups count the steps.
