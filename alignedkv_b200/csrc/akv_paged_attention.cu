@@ -6,12 +6,17 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-Plan plan_of(int rows, int D) {
+long long chunks_of_table(const akv_pool* pool, int width) { return ((long long)width * pool->page_size + CHUNK - 1) / CHUNK; }
+// rows: of a KV head; heads: (sequence, KV head) pairs; most_chunks: of the longest sequence that the table can hold.  As many rows as a unit takes, so that
+// codes are unpacked once for all of them; but 8 where that still leaves a warp two chunks or fewer, since the time is then one warp's over all
+// its rows (20 sequences of 42 tokens, 32 rows: 6.2 us, in units of 32 11.5).
+Plan plan_of(int rows, int D, long long heads, long long most_chunks) {
     Plan p;
-    p.groups = (rows + 31) / 32;
+    p.ctas = sm_count();
+    const int eights = (rows + 7) / 8;
+    p.groups = heads * eights * most_chunks <= 2ll * p.ctas * MOST_WARPS ? eights : (rows + 31) / 32;
     p.rows = (rows + p.groups - 1) / p.groups;
     p.nt = (p.rows + 7) / 8;
-    p.ctas = sm_count();
     p.bytes = (2ll + MOST_WARPS) * p.ctas * 8 * p.nt * (D + 4) * 4 + 8ll * p.ctas;
     return p;
 }
@@ -37,7 +42,7 @@ long long akv_paged_scratch_bytes(const akv_pool* pool, int bsz, int width, int 
     if (!pool || bsz <= 0 || width <= 0 || group <= 0 || tokens <= 0 || group > 64 || tokens > 64 || group * tokens > 64 ||
         (pool->head_dim != 64 && pool->head_dim != 128))
         return -1;
-    return plan_of(group * tokens, pool->head_dim).bytes;
+    return plan_of(group * tokens, pool->head_dim, (long long)bsz * pool->n_kv_heads, chunks_of_table(pool, width)).bytes;
 }
 
 int akv_paged_attention(const akv_pool* pool, const void* q, const void* pages, const void* lens, void* out, void* lse, void* scratch,
@@ -52,12 +57,12 @@ int akv_paged_attention(const akv_pool* pool, const void* q, const void* pages, 
     AKV_REQUIRE(aligned16(q) && aligned16(out) && aligned16(scratch) && (reinterpret_cast<uintptr_t>(lse) & 3u) == 0, AKV_ERR_ALIGN,
                 "paged_attention: q, out and scratch must be 16-byte aligned, lse 4-byte");
     const int D = pool->head_dim;
-    const Plan p = plan_of(group * tokens, D);
+    const Plan p = plan_of(group * tokens, D, (long long)bsz * pool->n_kv_heads, chunks_of_table(pool, width));
     AKV_REQUIRE(scratch_bytes >= p.bytes, AKV_ERR_SHAPE, "paged_attention: scratch of %lld bytes is too small", scratch_bytes);
     AKV_REQUIRE((long long)pool->n_pages * pool->n_kv_heads * pool->page_size <= 1ll << 32 && (long long)bsz * width < INT_MAX, AKV_ERR_OVERFLOW,
                 "paged_attention: a pool of more than 2^32 rows");
     AKV_REQUIRE((long long)bsz * tokens * pool->n_kv_heads * group < INT_MAX / 256, AKV_ERR_OVERFLOW, "paged_attention: too many query rows");
-    const long long most = ((long long)width * pool->page_size + CHUNK - 1) / CHUNK * bsz * pool->n_kv_heads * p.groups;
+    const long long most = chunks_of_table(pool, width) * bsz * pool->n_kv_heads * p.groups;
     AKV_REQUIRE(most < INT_MAX, AKV_ERR_OVERFLOW, "paged_attention: too many chunks of %d tokens", CHUNK);
     a.q = static_cast<const __half*>(q);
     a.out = static_cast<__half*>(out);
@@ -72,7 +77,8 @@ int akv_paged_attention(const akv_pool* pool, const void* q, const void* pages, 
     a.ctas = p.ctas;
     a.record = 8 * p.nt * (D + 4);
     a.scale2 = scale * LOG2E;
-    a.team = team_of(bsz * pool->n_kv_heads * p.groups, ((long long)width * pool->page_size + TEAM_CHUNK - 1) / TEAM_CHUNK, p.ctas, p.nt <= 2 ? 12 : 8);
+    a.team = team_of(bsz * pool->n_kv_heads * p.groups, ((long long)width * pool->page_size + TEAM_CHUNK - 1) / TEAM_CHUNK, p.ctas,
+                     pool->format == AKV_PAGE_E2M1 && D == 128 && p.nt == 1 ? 16 : p.nt <= 2 ? 12 : 8);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool joined = (long long)width * pool->page_size > CHUNK;      // (units of one chunk are nobody else's)
     if (pool->format == AKV_PAGE_FP16) return launch_attend_fp16(a, p, D, joined, st);
