@@ -31,8 +31,9 @@ template <int F, int D, int NT>
 struct Shape {
     static constexpr int ROW = row_bytes<F>(D);
     static constexpr int KW = ROW / 8;                        // words of 16 tokens of K (or of V) in a lane
-    static constexpr int U = ROW == 256 ? 1 : 2;              // 16-token tiles of a step
-    static constexpr int TOKENS = 16 * U;
+    // (four for narrow rows: what a step costs beside its products is that of 32 tokens; 64 sequences of up to 8192 tokens, 8 heads, e4m3: 61.9 -> 56.2 us)
+    static constexpr int U = ROW == 256 ? 1 : ROW < 128 && D == 64 && NT <= 2 ? 4 : 2;     // 16-token tiles of a step
+    static constexpr int TOKENS = 16 * U, TEAM_TOKENS = TOKENS > 32 ? TOKENS : 32;         // tokens of a cluster's chunk
     static constexpr int KS = D / 16;                         // products over the channels; tiles of 16 channels of the output
     static constexpr int SCALES = F == AKV_PAGE_E2M1 ? D : 0; // bytes of a tile's scales (of K or of V)
     static constexpr int MORE = F == AKV_PAGE_FP16 ? 0 : 2 * SCALES + 32;                  // ... of its scales and exponents
@@ -40,7 +41,7 @@ struct Shape {
     static constexpr int STEP = (U * (32 * ROW + MORE) + 127) / 128 * 128;
     // (4-bit rows of 128 channels are bound by the instructions that unpack them: 16 warps, 45.5 us instead of 47.3 for 8 heads x 131072 tokens)
     static constexpr bool MANY = F == AKV_PAGE_E2M1 && D == 128 && NT == 1;
-    static constexpr int STEPS = ROW >= 128 || MANY ? 2 : F == AKV_PAGE_E2M1 && D == 128 ? 3 : F == AKV_PAGE_E4M3 ? 4 : 6;
+    static constexpr int STEPS = ROW >= 128 || MANY ? 2 : F == AKV_PAGE_E2M1 && D == 128 ? 3 : F == AKV_PAGE_E4M3 ? (U == 4 ? 2 : 4) : (U == 4 ? 3 : 6);
     // Up to 16 rows: operands of the queries stay in registers.  More: in shared memory, and the output takes the registers of a third of the warps.
     static constexpr bool FEW = NT <= 2;
     static constexpr int WARPS = MANY ? 16 : FEW ? 12 : 8;
@@ -187,7 +188,7 @@ __device__ __forceinline__ int piece(int r, int c) {
 template <int F, int D, int NT, bool ONE, bool TEAM>
 struct Ring {
     using S = Shape<F, D, NT>;
-    static constexpr int U = S::U, ROW = S::ROW, PAGES = ONE ? 1 : U, TOKENS_OF = TEAM ? TEAM_CHUNK : CHUNK;    // (of a chunk)
+    static constexpr int U = S::U, ROW = S::ROW, PAGES = ONE ? 1 : U, TOKENS_OF = TEAM ? S::TEAM_TOKENS : CHUNK;    // (of a chunk)
     const AttendArgs& a;
     const int* cum;
     uint32_t base, mine;                 // of the ring; where this lane's first piece of codes goes within a tile
@@ -367,8 +368,8 @@ struct Unit {
     // -128 comes out as a factor of -infinity: times the row's zeros NaN, as it should; the maximum takes -40, below what there is.)
     __device__ __forceinline__ void unfold(uint32_t step) {
         if constexpr (F != AKV_PAGE_FP16) {
-            const int i = 4 * g + t;
-            if (i < S::TOKENS) {
+#pragma unroll
+            for (int i = 4 * g + t; i < S::TOKENS; i += 32) {
                 const uint32_t from = step + U * 32 * ROW + (i >> 4) * S::MORE + 2 * S::SCALES + (i & 15);
                 const int k = lds8_signed(from), v = lds8_signed(from + 16);
                 const float weight = v == EXP_NAN ? NAN : __int_as_float((v + 127 + 15) << 23);
@@ -806,7 +807,7 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
         cta = blockIdx.x - part.unit * ctas;
         part.b = part.unit / units;
         part.place(part.unit - part.b * units, a.groups);
-        total = part.chunks = chunks_of<TEAM_CHUNK>(length_of(a.pool, part.b));
+        total = part.chunks = chunks_of<S::TEAM_TOKENS>(length_of(a.pool, part.b));
     } else {
         add_lengths<32 * WARPS>(a, cum, sums);
         total = cum[a.B] * units;
@@ -833,7 +834,7 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
         Ring<F, D, NT, ONE, TEAM> ring(a, cum, smem_u32(last_record), lane, units, part, at, end);
         Unit<F, D, NT, ONE> unit(a, lane, smem_u32(last_record));
         for (;;) {
-            constexpr int TOKENS_OF = TEAM ? TEAM_CHUNK : CHUNK;
+            constexpr int TOKENS_OF = TEAM ? S::TEAM_TOKENS : CHUNK;
             const Rows rows(a, part.b, part.h, part.group);
             const int n = length_of(a.pool, part.b), stop = min(n, part.last * TOKENS_OF);
             int seen[NT][2];

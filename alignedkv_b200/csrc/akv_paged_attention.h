@@ -4,7 +4,7 @@
 
 namespace akv {
 
-constexpr int CHUNK = 64, TEAM_CHUNK = 32, MOST_WARPS = 16;       // (TEAM_CHUNK: where a cluster has a unit to itself)
+constexpr int CHUNK = 64, TEAM_CHUNK = 32, MOST_WARPS = 16;       // (TEAM_CHUNK: where a cluster has a unit to itself; a step where that is more)
 
 struct AttendArgs {
     Pool pool;
