@@ -18,7 +18,7 @@ struct AttendArgs {
 
 // Rows of a unit in groups of 8 (nt), CTAs, workspace.
 struct Plan {
-    int nt, groups, rows, ctas;
+    int nt, groups, rows, ctas, team;
     long long bytes;
 };
 

@@ -36,38 +36,44 @@ from .cache_ops import _need, _nothing
 __all__ = ["paged_append", "paged_read", "paged_attention"]
 
 MOST_ROWS = 64
+_PAGES = (16, 32, 64, 128, 256)
 _FORMATS = {torch.half: 0, torch.float8_e4m3fn: 1, torch.uint8: 2}
 
 
 class _Call:
-    """A pool's tensors and a batch's table, checked, as the library takes them."""
+    """A pool's tensors and a batch's table, checked, as the library takes them.  (As in `cache_ops`, the checks are most of what a call on few
+    tokens costs: one expression each.)"""
     __slots__ = ("device", "index", "B", "W", "H", "D", "P", "pool", "pages", "lens")
 
     def __init__(self, cache, pages, lens):
-        codes = cache.k_codes
-        if not isinstance(codes, torch.Tensor) or not codes.is_cuda or codes.dim() != 4 or codes.dtype not in _FORMATS:
+        k, v = cache.k_codes, cache.v_codes
+        if not isinstance(k, torch.Tensor) or not k.is_cuda or k.dim() != 4 or k.dtype not in _FORMATS:
             raise RuntimeError("k_codes: expected a CUDA tensor of shape [pages, H, page_size, row], torch.half, torch.float8_e4m3fn or torch.uint8")
-        form = _FORMATS[codes.dtype]
-        self.device, self.index = codes.device, codes.get_device()
-        N, H, P, row = codes.shape
+        dtype, shape = k.dtype, k.shape
+        form = _FORMATS[dtype]
+        self.device, self.index = k.device, k.get_device()
+        N, H, P, row = shape
         D = 2 * row if form == 2 else row
-        if D not in (64, 128):
+        if D != 128 and D != 64:
             raise RuntimeError(f"head size {D}: these operators cover 64 and 128")
-        if P not in (16, 32, 64, 128, 256):
+        if P not in _PAGES:
             raise RuntimeError(f"page size {P}: expected a power of two from 16 to 256")
         self.H, self.D, self.P = H, D, P
-        dev, shape = self.index, tuple(codes.shape)
-        ptrs = [_need("k_codes", codes, shape, codes.dtype, dev), _need("v_codes", cache.v_codes, shape, codes.dtype, dev), None, None, None, None]
+        dev, ke, ve, ks, vs = self.index, None, None, None, None
+        kp, vp = _need("k_codes", k, shape, dtype, dev), _need("v_codes", v, shape, dtype, dev)
         if form:
-            ptrs[2:4] = [_need(n, getattr(cache, n), (N, H, P), torch.int8, dev) for n in ("k_exps", "v_exps")]
-        if form == 2:
-            ptrs[4:] = [_need(n, getattr(cache, n), (N, H, P, D // 16), torch.float8_e4m3fn, dev) for n in ("k_scales", "v_scales")]
-        if not isinstance(pages, torch.Tensor) or pages.dim() != 2 or pages.shape[0] == 0 or pages.shape[1] == 0:
+            part = (N, H, P)
+            ke, ve = _need("k_exps", cache.k_exps, part, torch.int8, dev), _need("v_exps", cache.v_exps, part, torch.int8, dev)
+            if form == 2:
+                part = (N, H, P, D // 16)
+                ks = _need("k_scales", cache.k_scales, part, torch.float8_e4m3fn, dev)
+                vs = _need("v_scales", cache.v_scales, part, torch.float8_e4m3fn, dev)
+        if not isinstance(pages, torch.Tensor) or pages.dim() != 2 or pages.numel() == 0:
             raise RuntimeError("pages: expected a tensor of shape [B, width]")
         self.B, self.W = pages.shape
         self.pages = _need("pages", pages, (self.B, self.W), torch.int32, dev)
         self.lens = _need("lens", lens, (self.B,), torch.int32, dev)
-        self.pool = _lib.Pool(*ptrs, form, N, P, H, D)
+        self.pool = _lib.Pool(kp, vp, ke, ve, ks, vs, form, N, P, H, D)
 
     def here(self):
         return _nothing if torch.cuda.current_device() == self.index else torch.cuda.device(self.index)
@@ -79,8 +85,9 @@ def _rows(name: str, x, like: tuple, index: int) -> list:
             (x.shape[0], x.shape[2], x.shape[3]) != like or x.shape[1] == 0 or x.stride(3) != 1 or x.data_ptr() % 16:
         raise RuntimeError(f"{name}: expected an fp16 tensor of shape [{like[0]}, T, {like[1]}, {like[2]}] on cuda:{index} with a unit stride "
                            "along the channels, on a 16-byte boundary")
-    strides = [s if n > 1 else 0 for s, n in zip(x.stride()[:3], x.shape)]
-    if any(s % 8 for s in strides):
+    b, t, h, _ = x.stride()
+    strides = [b if x.shape[0] > 1 else 0, t if x.shape[1] > 1 else 0, h if x.shape[2] > 1 else 0]
+    if (strides[0] | strides[1] | strides[2]) & 7:
         raise RuntimeError(f"{name}: strides {tuple(x.stride())} do not keep its rows on 16-byte boundaries")
     return strides
 
@@ -151,12 +158,13 @@ def paged_attention(cache, q: torch.Tensor, pages: torch.Tensor, lens: torch.Ten
         begin = _need("out", out, tuple(q.shape), torch.half, c.index)
         if begin < q.data_ptr() + 2 * q.numel() and q.data_ptr() < begin + 2 * out.numel():
             raise RuntimeError("out: overlaps q")
-    lib = _lib.load()
-    sums = q.new_empty((c.B, T, Hq), dtype=torch.float32) if lse else None
+    lib, pool = _lib.load(), ctypes.byref(c.pool)
+    sums = torch.empty((c.B, T, Hq), dtype=torch.float32, device=c.device) if lse else None
     with c.here():
-        ws = torch.empty(max(0, lib.akv_paged_scratch_bytes(ctypes.byref(c.pool), c.B, c.W, group, T)), dtype=torch.uint8, device=c.device)
-        rc = lib.akv_paged_attention(ctypes.byref(c.pool), q.data_ptr(), c.pages, c.lens, out.data_ptr(), sums.data_ptr() if lse else None,
-                                     ws.data_ptr(), ws.numel(), c.B, c.W, group, T, 1.0 / math.sqrt(c.D) if scale is None else scale,
-                                     _lib.raw_stream(c.index))
+        size = lib.akv_paged_scratch_bytes(pool, c.B, c.W, group, T)
+        ws = torch.empty(size, dtype=torch.uint8, device=c.device) if size > 0 else None
+        rc = lib.akv_paged_attention(pool, q.data_ptr(), c.pages, c.lens, out.data_ptr(), sums.data_ptr() if lse else None,
+                                     None if ws is None else ws.data_ptr(), size, c.B, c.W, group, T,
+                                     1.0 / math.sqrt(c.D) if scale is None else scale, _lib.raw_stream(c.index))
     _lib.check("paged_attention", rc)
     return (out, sums) if lse else out

@@ -462,7 +462,8 @@ int akv_evict(const akv_layer* layer, void* weights, void* positions, int rest_l
  * akv_paged_attention: the `tokens` newest tokens of every sequence, which are in the pages and counted by lens, attend to it: q, out
  * fp16 [bsz, tokens, H * group, head_dim], query t sees positions below lens[b] - tokens + 1 + t.  At most 64 rows (tokens * group).  fp32 scores, softmax
  * and sums over the values that the codes stand for, one rounding.  A row that sees nothing is 0, its lse -inf.  lse (may be NULL): fp32
- * [bsz, tokens, H * group].  out must not overlap an input.  scratch: akv_paged_scratch_bytes(...) bytes, any contents.
+ * [bsz, tokens, H * group].  out must not overlap an input.  scratch: akv_paged_scratch_bytes(...) bytes, any contents (0 for
+ * short tables: scratch may be NULL).
  */
 #define AKV_PAGE_FP16 0
 #define AKV_PAGE_E4M3 1
