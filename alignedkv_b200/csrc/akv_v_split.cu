@@ -208,10 +208,13 @@ bool v_split_takes_probe(int group, int reference, int n) {
     return group == 1 && !reference && tuning().v_split_impl == 0 && n >= 512;
 }
 
+// Enough for any number of tokens up to n: a shorter sequence may be cut into more chunks than a longer one, since chunks are
+// whole 128 tokens (75 rows: 12288 tokens into 16, 12352 into 14).  Never more than split_plan aims at, nor than n has of its
+// smallest chunks.
 long long v_split_scratch_bytes(int bsz, int H, int group, int n) {
-    int ct, ch;
-    split_plan(bsz * H, n, &ct, &ch);
-    return (long long)bsz * H * group * ch * 128 * (long long)sizeof(float);
+    const long long BH = (long long)bsz * H, want = (sm_count() * 8 + BH - 1) / BH, most = ((long long)n + 255) / 256;
+    const long long ch = want < most ? want : most;
+    return BH * group * (ch < 1 ? 1 : ch) * 128 * (long long)sizeof(float);
 }
 
 // Order-free P.V over n quantized tokens (head_dim 128).  o16 / o32: [B, Hq, D], either may be null.
