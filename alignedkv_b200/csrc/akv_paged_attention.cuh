@@ -615,7 +615,7 @@ struct Unit {
         }
     }
     // The same where some values are not finite (fp16 pages alone: elsewhere codes are).  0 * inf would be NaN: every query's product is formed by
-    // itself, without the newest tokens that it does not see.
+    // itself, without the newest tokens that it does not see, and comes out as if those were not there.
     __device__ __forceinline__ void add_odd_values(const uint32_t (&v)[KW], const uint32_t (&w)[NT][2], int at, int n, const int (&seen)[NT][2]) {
         const uint32_t none[2] = {0, 0};
 #pragma unroll 1
@@ -627,11 +627,11 @@ struct Unit {
             tiles(v, none, [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    float c[4] = {acc[i][nt][0], acc[i][nt][1], acc[i][nt][2], acc[i][nt][3]};
                     mma(c, a0 & m01, a1 & m01, a2 & m23, a3 & m23, w[nt][0], w[nt][1]);
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
-                        if (seen[nt][x & 1] == limit) acc[i][nt][x] += c[x];
+                        if (seen[nt][x & 1] == limit) acc[i][nt][x] = c[x];
                 }
             });
         }
