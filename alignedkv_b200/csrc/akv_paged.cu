@@ -28,6 +28,11 @@ __device__ __forceinline__ float quotient(float x, float s, float r) {
     const float y = x * r;
     return fmaf(fmaf(-y, s, x), r, y);
 }
+__device__ __forceinline__ float reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
 __device__ __forceinline__ uint32_t max_of(uint32_t two) { return max(two & 0xFFFFu, two >> 16); }
 // 2^e in both halves, e in -14..15.
@@ -85,10 +90,10 @@ __device__ __forceinline__ void store_row(uint8_t* codes, int8_t* exps, uint8_t*
 #pragma unroll
             for (int q = 0; q < PIECES; ++q) {
                 uint16_t sc;
-                const float sixth = finite ? __fdiv_rn(halves_floats(max_of(pair[q])).x * back, 6.f) : 0.f;
+                const float sixth = finite ? quotient(halves_floats(max_of(pair[q])).x * back, 6.f, 1.f / 6.f) : 0.f;      // (middles of e4m3 have 5 bits)
                 asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(sc) : "f"(0.f), "f"(sixth));
                 if (row >= 0 && (lane & 1) == 0) scales[row * (D / 16) + ((lane + q * LANES) >> 1)] = (uint8_t)sc;
-                const float s = e4m3_float(sc & 0xFFu) * unit, r = s > 0.f ? __frcp_rn(s) : 0.f;
+                const float s = e4m3_float(sc & 0xFFu) * unit, r = s > 0.f ? reciprocal(s) : 0.f;
                 uint32_t c[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
