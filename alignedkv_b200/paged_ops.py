@@ -40,6 +40,14 @@ _PAGES = (16, 32, 64, 128, 256)
 _FORMATS = {torch.half: 0, torch.float8_e4m3fn: 1, torch.uint8: 2}
 
 
+def _two(name: str, a, b, shape: tuple, dtype: torch.dtype, index: int) -> tuple:
+    """The addresses of k_<name> and v_<name>, contiguous tensors of that shape and type on that device: one look at both."""
+    if isinstance(a, torch.Tensor) and isinstance(b, torch.Tensor) and a.shape == shape and b.shape == shape and a.dtype is dtype and \
+            b.dtype is dtype and a.get_device() == index and b.get_device() == index and a.is_contiguous() and b.is_contiguous():
+        return a.data_ptr(), b.data_ptr()
+    return _need("k_" + name, a, tuple(shape), dtype, index), _need("v_" + name, b, tuple(shape), dtype, index)       # (says which and why)
+
+
 class _Call:
     """A pool's tensors and a batch's table, checked, as the library takes them.  (As in `cache_ops`, the checks are most of what a call on few
     tokens costs: one expression each.)"""
@@ -51,7 +59,7 @@ class _Call:
             raise RuntimeError("k_codes: expected a CUDA tensor of shape [pages, H, page_size, row], torch.half, torch.float8_e4m3fn or torch.uint8")
         dtype, shape = k.dtype, k.shape
         form = _FORMATS[dtype]
-        self.device, self.index = k.device, k.get_device()
+        self.index, self.device = k.get_device(), k.device
         N, H, P, row = shape
         D = 2 * row if form == 2 else row
         if D != 128 and D != 64:
@@ -60,19 +68,20 @@ class _Call:
             raise RuntimeError(f"page size {P}: expected a power of two from 16 to 256")
         self.H, self.D, self.P = H, D, P
         dev, ke, ve, ks, vs = self.index, None, None, None, None
-        kp, vp = _need("k_codes", k, shape, dtype, dev), _need("v_codes", v, shape, dtype, dev)
+        kp, vp = _two("codes", k, v, shape, dtype, dev)
         if form:
-            part = (N, H, P)
-            ke, ve = _need("k_exps", cache.k_exps, part, torch.int8, dev), _need("v_exps", cache.v_exps, part, torch.int8, dev)
+            ke, ve = _two("exps", cache.k_exps, cache.v_exps, (N, H, P), torch.int8, dev)
             if form == 2:
-                part = (N, H, P, D // 16)
-                ks = _need("k_scales", cache.k_scales, part, torch.float8_e4m3fn, dev)
-                vs = _need("v_scales", cache.v_scales, part, torch.float8_e4m3fn, dev)
-        if not isinstance(pages, torch.Tensor) or pages.dim() != 2 or pages.numel() == 0:
-            raise RuntimeError("pages: expected a tensor of shape [B, width]")
-        self.B, self.W = pages.shape
-        self.pages = _need("pages", pages, (self.B, self.W), torch.int32, dev)
-        self.lens = _need("lens", lens, (self.B,), torch.int32, dev)
+                ks, vs = _two("scales", cache.k_scales, cache.v_scales, (N, H, P, D // 16), torch.float8_e4m3fn, dev)
+        if not isinstance(pages, torch.Tensor) or pages.dim() != 2 or pages.dtype is not torch.int32 or pages.get_device() != dev or \
+                not pages.is_contiguous() or pages.numel() == 0:
+            raise RuntimeError(f"pages: expected a contiguous {torch.int32} tensor of shape [B, width] on cuda:{dev}")
+        self.B, self.W = B, _ = pages.shape
+        self.pages = pages.data_ptr()
+        if not isinstance(lens, torch.Tensor) or lens.dtype is not torch.int32 or lens.get_device() != dev or lens.dim() != 1 or \
+                lens.shape[0] != B or not lens.is_contiguous():
+            raise RuntimeError(f"lens: expected a contiguous {torch.int32} tensor of shape ({B},) on cuda:{dev}")
+        self.lens = lens.data_ptr()
         self.pool = _lib.Pool(kp, vp, ke, ve, ks, vs, form, N, P, H, D)
 
     def here(self):
