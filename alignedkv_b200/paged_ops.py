@@ -14,7 +14,8 @@ extension/v_cache_file.py:35-54).
   k_scales, v_scales  float8_e4m3fn [pages, H, page_size, D / 16], for e2m1: a factor per 16 channels
 D is 64 or 128, page_size a power of two from 16 to 256.  Of a row x of D values, e4m3: exp is the least integer with max |x| <= 448 * 2**exp;
 e2m1: the least with max |x| <= 2688 * 2**exp, and a scale is max |x| * 2**-exp / 6 over its channels; every rounding goes to the nearest value, ties
-to even.  A row with a value that is not finite stands for NaN throughout (exp -128), except in a pool of torch.half.
+to even.  A row with a value that is not finite stands for NaN throughout (exp -128), except in a pool of torch.half.  (Appended exponents are
+-35 to 8; of pools that something else fills, attention takes -100 to 100.)
 
 pages int32 [B, width]: position t of sequence b lies in page pages[b, t // page_size].  An entry outside 0..pages-1 is a page that was given
 up (-1, say): its tokens have no part in attention, are read as zeros, and what would be written there is dropped.  Entries behind a

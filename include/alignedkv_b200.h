@@ -445,7 +445,7 @@ int akv_evict(const akv_layer* layer, void* weights, void* positions, int rest_l
  *   AKV_PAGE_E2M1   4 bits per channel, the even one in the lower bits, x = code s 2^e: e the least with max |x| <= 2688 2^e, s (e4m3) the
  *                   nearest to max |x| 2^-e / 6 over 16 channels
  * exps: int8 [n_pages, H, page_size] (e of all zeros: as of fp16's smallest magnitude; -128: a value of the row is not finite, the row stands
- * for NaN); scales: bytes [n_pages, H, page_size, head_dim / 16].  Roundings to the nearest, ties to even.  head_dim 64 or 128; page_size a power of
+ * for NaN; appended ones are -35 to 8, attention takes -100 to 100); scales: bytes [n_pages, H, page_size, head_dim / 16].  Roundings to the nearest, ties to even.  head_dim 64 or 128; page_size a power of
  * two from 16 to 256; every pointer of the pool 16-byte aligned.
  *
  * pages: int32 [bsz, width], position t of sequence b lies in page pages[b][t / page_size].  An entry outside 0..n_pages-1 is a page that was
