@@ -122,8 +122,9 @@ struct Place {
     }
 };
 
-// Rows of one tensor by LANES threads each; a block has consecutive tokens of one KV head, whose rows lie side by side in a page.  Bound by HBM where
-// there is much to do.
+// Rows of one tensor by LANES threads each; a block has consecutive tokens of one KV head, whose rows lie side by side in a page.  Bound by HBM
+// and, nearly as much, by the instructions of the maxima and conversions: up to 1000 tokens of 16 x 32 heads of 128 channels 36 us in e4m3 (5.6 TB/s, 83%
+// of the issue slots), up to 8190 of 4 x 8 13 us in e2m1.  (One row a lane, four, 128 or 512 threads: slower or the same.)
 template <int F, int D>
 __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
     constexpr int LANES = lanes_of<D>, ROWS = THREADS / LANES;
@@ -163,6 +164,8 @@ struct ReadArgs {
     int most, blocks;
 };
 
+// The same places.  Bound by HBM's writes: what append left above takes 51 us from e4m3 (5.1 TB/s, three
+// quarters of them written), 27 us from e2m1.
 template <int F, int D>
 __global__ void __launch_bounds__(THREADS) read_kernel(ReadArgs a) {
     constexpr int LANES = lanes_of<D>, ROWS = THREADS / LANES, PIECE = row_bytes<F>(D) / (LANES * PIECES);

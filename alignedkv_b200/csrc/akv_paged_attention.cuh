@@ -4,12 +4,15 @@
 //
 //   s_rj = scale q_r . k_j, o_r = sum_j exp(s_rj - m_r) v_j / l_r, l_r = sum_j exp(s_rj - m_r), over the tokens j that row r sees.
 //
-// Every byte of the tokens is read once: bound by HBM, and for the 4-bit format almost as much by the instructions that unpack it.
-// Work: a unit is up to 16 query rows of one (sequence, KV head), its tokens in chunks of 64.  The chunks of all units in a row are dealt to
-// the warps in equal contiguous runs: lengths are only known on the device, and every SM gets the same whatever they are.  Each CTA
-// adds up the lengths itself.  A warp needs no other one: codes come straight into registers as operand fragments (no shared memory is
-// on their way), the next step's while this one's are multiplied.  Where a run begins or ends inside a unit it leaves a record, and
-// the CTA joins those of its warps; what is left between CTAs is join_kernel's.
+// Every byte of the tokens is read once: bound by HBM in 16 and 8 bits (8 x 32 x 4096 tokens of 128 channels, e4m3: 48.2 us, 5.6 TB/s; up to 8192 of
+// 64 x 8 heads: 95.2 us, 5.9 TB/s), by the instructions that unpack the codes in 4 (8 heads x 131072 tokens: 43.2 us, 3.5 TB/s, 61% of the issue
+// slots), and with many rows by the chain of products and softmax in few warps (20 rows, 32 x 8 heads x up to 4096: 56 us).
+// Work: a unit is the query rows of one (sequence, KV head), up to 32, its tokens in chunks of 64.  The chunks of all units in a row are dealt in
+// equal contiguous runs to the CTAs, then to a CTA's warps: lengths are only known on the device, and every SM gets the same whatever they
+// are.  Each CTA adds up the lengths itself.  A warp needs no other one: it fills a ring in shared memory by asynchronous copies and drains it, codes go
+// from there into registers as operand fragments.  (Loads straight into registers: 75 us where the ring took 63.  A ring for the whole CTA would
+// need a barrier a step.)  Where a run begins or ends inside a unit it leaves a record, and the CTA joins those of its warps; what is left
+// between CTAs is join_kernel's.  With few units and short tables a cluster has a unit to itself and joins its records in shared memory.
 //
 // Operands: tokens are the rows of the products' first operand, query rows the columns of the second - 8 of them, which one KV head's query heads
 // fill, where the other way round 16 would be half empty.  Which channel is which k, and which token which row, is free as long as both
@@ -43,6 +46,7 @@ struct Shape {
     static constexpr bool MANY = F == AKV_PAGE_E2M1 && D == 128 && NT == 1;
     static constexpr int STEPS = ROW >= 128 || MANY ? 2 : F == AKV_PAGE_E2M1 && D == 128 ? 3 : F == AKV_PAGE_E4M3 ? (U == 4 ? 2 : 4) : (U == 4 ? 3 : 6);
     // Up to 16 rows: operands of the queries stay in registers.  More: in shared memory, and the output takes the registers of a third of the warps.
+    // (20 rows of 4 bits, 32 x 8 heads x up to 4096 tokens: 56 us; ten warps spill, 69; steps of 16 tokens 63; units of 16 rows 67, of 8 64.)
     static constexpr bool FEW = NT <= 2;
     static constexpr int WARPS = MANY ? 16 : FEW ? 12 : 8;
     static constexpr int RECORD = 8 * NT * (D + 4);           // floats: rows of D sums, then the maximum and the sum
