@@ -38,6 +38,17 @@ def _need(name: str, t, shape: tuple, dtype: torch.dtype, index: int) -> int:
     return t.data_ptr()
 
 
+def _run(what: str, index: int, entry, *args) -> None:
+    """The library's entry on torch's current stream of that device.  (Without a context manager where the device is the current one.)"""
+    if torch.cuda.current_device() == index:
+        rc = entry(*args, _lib.raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, _lib.raw_stream(index))
+    if rc:
+        _lib.check(what, rc)
+
+
 class _Call:
     """A cache's tensors, checked, as the library takes them; a context in which its device is the current one.  (The checks are most of
     what a call on a short cache costs, so they are few: one look at shape, type, device and layout of each tensor that is used.)"""
@@ -245,7 +256,7 @@ def accept_drafts(target: torch.Tensor, draft: torch.Tensor | None, ids: torch.T
     probability at all).  Sequences accept different numbers of tokens: `tree_commit` takes path[:, :n] for n up to the smallest count, whose
     nodes are then `LlamaDecoder.accept`'s too."""
     if not isinstance(target, torch.Tensor) or not target.is_cuda or target.dim() != 3 or target.dtype not in _PROBABILITIES or \
-            target.numel() == 0 or (target.stride(2) != 1 and target.shape[2] > 1):
+            not target.numel() or ((strides := target.stride())[2] != 1 and target.shape[2] > 1):
         raise RuntimeError("target: expected a CUDA tensor of shape [B, T, V], fp32, fp16 or bf16, with a unit stride along the vocabulary")
     B, T, V = target.shape
     index = target.get_device()
@@ -260,14 +271,12 @@ def accept_drafts(target: torch.Tensor, draft: torch.Tensor | None, ids: torch.T
     if parents is not None:
         each = isinstance(parents, torch.Tensor) and parents.dim() == 2
         parents_ptr, step = _need("parents", parents, (B, T) if each else (T,), torch.int32, index), T if each else 0
-    path = torch.empty((B, T), dtype=torch.int32, device=target.device)
-    count = torch.empty(B, dtype=torch.int32, device=target.device)
-    token = torch.empty(B, dtype=torch.int64, device=target.device)
-    d = target if draft is None else draft
-    with _nothing if torch.cuda.current_device() == index else torch.cuda.device(index):
-        rc = _lib.load().akv_accept_drafts(
-            target.data_ptr(), target.stride(0), target.stride(1), None if draft is None else draft.data_ptr(), d.stride(0), d.stride(1),
-            ids_ptr, coins_ptr, parents_ptr, step, path.data_ptr(), count.data_ptr(), token.data_ptr(), B, T, V,
-            _PROBABILITIES[target.dtype], _lib.raw_stream(index))
-    _lib.check("accept_drafts", rc)
+    device = target.device
+    path = torch.empty(B, T, dtype=torch.int32, device=device)
+    count = torch.empty(B, dtype=torch.int32, device=device)
+    token = torch.empty(B, dtype=torch.int64, device=device)
+    (batch, row, _), (draft_batch, draft_row, _) = strides, strides if draft is None else draft.stride()
+    _run("accept_drafts", index, _lib.load().akv_accept_drafts, target.data_ptr(), batch, row, None if draft is None else draft.data_ptr(),
+         draft_batch, draft_row, ids_ptr, coins_ptr, parents_ptr, step, path.data_ptr(), count.data_ptr(), token.data_ptr(), B, T, V,
+         _PROBABILITIES[target.dtype])
     return path, count, token

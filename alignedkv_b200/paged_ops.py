@@ -27,18 +27,20 @@ Everything is launched on torch's current stream of the pool's device; nothing s
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
 
 from . import _lib
-from .cache_ops import _need, _nothing
+from .cache_ops import _need, _run
 
 __all__ = ["paged_append", "paged_read", "paged_attention"]
 
 MOST_ROWS = 64
 _PAGES = (16, 32, 64, 128, 256)
 _FORMATS = {torch.half: 0, torch.float8_e4m3fn: 1, torch.uint8: 2}
+_Strides = ctypes.c_longlong * 6
 
 
 def _two(name: str, a, b, shape: tuple, dtype: torch.dtype, index: int) -> tuple:
@@ -56,11 +58,10 @@ class _Call:
 
     def __init__(self, cache, pages, lens):
         k, v = cache.k_codes, cache.v_codes
-        if not isinstance(k, torch.Tensor) or not k.is_cuda or k.dim() != 4 or k.dtype not in _FORMATS:
+        if not isinstance(k, torch.Tensor) or not k.is_cuda or k.dim() != 4 or (form := _FORMATS.get(k.dtype)) is None:
             raise RuntimeError("k_codes: expected a CUDA tensor of shape [pages, H, page_size, row], torch.half, torch.float8_e4m3fn or torch.uint8")
         dtype, shape = k.dtype, k.shape
-        form = _FORMATS[dtype]
-        self.index, self.device = k.get_device(), k.device
+        self.index, self.device = dev, _ = k.get_device(), k.device
         N, H, P, row = shape
         D = 2 * row if form == 2 else row
         if D != 128 and D != 64:
@@ -68,14 +69,14 @@ class _Call:
         if P not in _PAGES:
             raise RuntimeError(f"page size {P}: expected a power of two from 16 to 256")
         self.H, self.D, self.P = H, D, P
-        dev, ke, ve, ks, vs = self.index, None, None, None, None
+        ke = ve = ks = vs = None
         kp, vp = _two("codes", k, v, shape, dtype, dev)
         if form:
             ke, ve = _two("exps", cache.k_exps, cache.v_exps, (N, H, P), torch.int8, dev)
             if form == 2:
                 ks, vs = _two("scales", cache.k_scales, cache.v_scales, (N, H, P, D // 16), torch.float8_e4m3fn, dev)
         if not isinstance(pages, torch.Tensor) or pages.dim() != 2 or pages.dtype is not torch.int32 or pages.get_device() != dev or \
-                not pages.is_contiguous() or pages.numel() == 0:
+                not pages.is_contiguous() or not pages.numel():
             raise RuntimeError(f"pages: expected a contiguous {torch.int32} tensor of shape [B, width] on cuda:{dev}")
         self.B, self.W = B, _ = pages.shape
         self.pages = pages.data_ptr()
@@ -85,21 +86,30 @@ class _Call:
         self.lens = lens.data_ptr()
         self.pool = _lib.Pool(kp, vp, ke, ve, ks, vs, form, N, P, H, D)
 
-    def here(self):
-        return _nothing if torch.cuda.current_device() == self.index else torch.cuda.device(self.index)
+
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(index: int, form: int, P: int, H: int, D: int, B: int, W: int, group: int, T: int) -> int:
+    """Bytes of the attention's workspace on that device."""
+    with torch.cuda.device(index):
+        return _lib.load().akv_paged_scratch_bytes(ctypes.byref(_lib.Pool(None, None, None, None, None, None, form, 1, P, H, D)), B, W, group, T)
 
 
-def _rows(name: str, x, like: tuple, index: int) -> list:
-    """Strides (batch, token, head) of x [B,T,H,D] fp16, whose rows of D are contiguous and begin on 16-byte boundaries."""
-    if not isinstance(x, torch.Tensor) or x.dim() != 4 or x.dtype is not torch.half or x.get_device() != index or \
-            (x.shape[0], x.shape[2], x.shape[3]) != like or x.shape[1] == 0 or x.stride(3) != 1 or x.data_ptr() % 16:
-        raise RuntimeError(f"{name}: expected an fp16 tensor of shape [{like[0]}, T, {like[1]}, {like[2]}] on cuda:{index} with a unit stride "
-                           "along the channels, on a 16-byte boundary")
-    b, t, h, _ = x.stride()
-    strides = [b if x.shape[0] > 1 else 0, t if x.shape[1] > 1 else 0, h if x.shape[2] > 1 else 0]
-    if (strides[0] | strides[1] | strides[2]) & 7:
-        raise RuntimeError(f"{name}: strides {tuple(x.stride())} do not keep its rows on 16-byte boundaries")
-    return strides
+def _rows(name: str, x, c: _Call) -> tuple:
+    """(address, tokens, strides of batch, token and head) of x [B,T,H,D] fp16, whose rows of D are contiguous and begin on 16-byte boundaries."""
+    if isinstance(x, torch.Tensor) and x.dim() == 4 and x.dtype is torch.half and x.get_device() == c.index:
+        (B, T, H, D), (b, t, h, unit), begin = x.shape, x.stride(), x.data_ptr()
+        if B == c.B and H == c.H and D == c.D and T and unit == 1 and not begin & 15:
+            if B == 1:
+                b = 0
+            if T == 1:
+                t = 0
+            if H == 1:
+                h = 0
+            if (b | t | h) & 7:
+                raise RuntimeError(f"{name}: strides {tuple(x.stride())} do not keep its rows on 16-byte boundaries")
+            return begin, T, b, t, h
+    raise RuntimeError(f"{name}: expected an fp16 tensor of shape [{c.B}, T, {c.H}, {c.D}] on cuda:{c.index} with a unit stride along the channels, on a "
+                       "16-byte boundary")
 
 
 def paged_append(cache, k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, lens: torch.Tensor, *,
@@ -112,16 +122,13 @@ def paged_append(cache, k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, l
     two sequences share (pages of a common prompt) must not be appended to; where two tokens have one place, either may be left there,
     or parts of both."""
     c = _Call(cache, pages, lens)
-    like = (c.B, c.H, c.D)
-    strides = _rows("k", k, like, c.index) + _rows("v", v, like, c.index)
-    T = k.shape[1]
-    if v.shape[1] != T:
-        raise RuntimeError(f"v: {v.shape[1]} tokens, k has {T}")
+    k_ptr, T, *of_k = _rows("k", k, c)
+    v_ptr, Tv, *of_v = _rows("v", v, c)
+    if Tv != T:
+        raise RuntimeError(f"v: {Tv} tokens, k has {T}")
     count_ptr = None if counts is None else _need("counts", counts, (c.B,), torch.int32, c.index)
-    with c.here():
-        rc = _lib.load().akv_paged_append(ctypes.byref(c.pool), k.data_ptr(), v.data_ptr(), (ctypes.c_longlong * 6)(*strides), c.pages, c.lens,
-                                          count_ptr, c.B, c.W, T, _lib.raw_stream(c.index))
-    _lib.check("paged_append", rc)
+    _run("paged_append", c.index, _lib.load().akv_paged_append, ctypes.byref(c.pool), k_ptr, v_ptr, _Strides(*of_k, *of_v), c.pages, c.lens, count_ptr,
+         c.B, c.W, T)
 
 
 def paged_read(cache, pages: torch.Tensor, lens: torch.Tensor, most: int) -> tuple:
@@ -131,12 +138,9 @@ def paged_read(cache, pages: torch.Tensor, lens: torch.Tensor, most: int) -> tup
     c = _Call(cache, pages, lens)
     if most < 1:
         raise RuntimeError(f"most: {most} tokens, expected at least 1")
-    k = torch.empty((c.B, most, c.H, c.D), dtype=torch.half, device=c.device)
+    k = torch.empty(c.B, most, c.H, c.D, dtype=torch.half, device=c.device)
     v = torch.empty_like(k)
-    with c.here():
-        rc = _lib.load().akv_paged_read(ctypes.byref(c.pool), c.pages, c.lens, k.data_ptr(), v.data_ptr(), c.B, c.W, most,
-                                        _lib.raw_stream(c.index))
-    _lib.check("paged_read", rc)
+    _run("paged_read", c.index, _lib.load().akv_paged_read, ctypes.byref(c.pool), c.pages, c.lens, k.data_ptr(), v.data_ptr(), c.B, c.W, most)
     return k, v
 
 
@@ -153,10 +157,11 @@ def paged_attention(cache, q: torch.Tensor, pages: torch.Tensor, lens: torch.Ten
     D**-0.5), softmax and sums and one rounding to fp16.  What lies in the pages behind lens[b] has no part in it, whatever it is.
     lse=True also returns the logarithm of the rows' sums of exponentials, fp32 [B,T,Hq] (-inf where nothing is seen)."""
     c = _Call(cache, pages, lens)
-    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[0] != c.B or q.shape[3] != c.D or q.dtype is not torch.half or \
-            q.get_device() != c.index or not q.is_contiguous():
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.dtype is not torch.half or q.get_device() != c.index or not q.is_contiguous():
         raise RuntimeError(f"q: expected a contiguous fp16 tensor of shape [{c.B}, T, Hq, {c.D}] on {c.device}")
-    T, Hq = q.shape[1], q.shape[2]
+    B, T, Hq, D = q.shape
+    if B != c.B or D != c.D:
+        raise RuntimeError(f"q: expected a contiguous fp16 tensor of shape [{c.B}, T, Hq, {c.D}] on {c.device}")
     if Hq % c.H or Hq == 0:
         raise RuntimeError(f"q: {Hq} query heads are no multiple of {c.H} KV heads")
     group = Hq // c.H
@@ -168,13 +173,10 @@ def paged_attention(cache, q: torch.Tensor, pages: torch.Tensor, lens: torch.Ten
         begin = _need("out", out, tuple(q.shape), torch.half, c.index)
         if begin < q.data_ptr() + 2 * q.numel() and q.data_ptr() < begin + 2 * out.numel():
             raise RuntimeError("out: overlaps q")
-    lib, pool = _lib.load(), ctypes.byref(c.pool)
-    sums = torch.empty((c.B, T, Hq), dtype=torch.float32, device=c.device) if lse else None
-    with c.here():
-        size = lib.akv_paged_scratch_bytes(pool, c.B, c.W, group, T)
-        ws = torch.empty(size, dtype=torch.uint8, device=c.device) if size > 0 else None
-        rc = lib.akv_paged_attention(pool, q.data_ptr(), c.pages, c.lens, out.data_ptr(), sums.data_ptr() if lse else None,
-                                     None if ws is None else ws.data_ptr(), size, c.B, c.W, group, T,
-                                     1.0 / math.sqrt(c.D) if scale is None else scale, _lib.raw_stream(c.index))
-    _lib.check("paged_attention", rc)
+    sums = torch.empty(B, T, Hq, dtype=torch.float32, device=c.device) if lse else None
+    size = _scratch_bytes(c.index, c.pool.format, c.P, c.H, D, B, c.W, group, T)
+    ws = torch.empty(size, dtype=torch.uint8, device=c.device) if size > 0 else None
+    _run("paged_attention", c.index, _lib.load().akv_paged_attention, ctypes.byref(c.pool), q.data_ptr(), c.pages, c.lens, out.data_ptr(),
+         sums.data_ptr() if lse else None, None if ws is None else ws.data_ptr(), size, B, c.W, group, T,
+         1.0 / math.sqrt(D) if scale is None else scale)
     return (out, sums) if lse else out
