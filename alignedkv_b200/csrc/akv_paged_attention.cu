@@ -29,7 +29,7 @@ Plan plan_of(int rows, const akv_pool* pool, int bsz, int width) {
     p.rows = (rows + p.groups - 1) / p.groups;
     p.nt = (p.rows + 7) / 8;
     p.team = team_of(heads * p.groups, chunks_of_table(pool, width, TEAM_CHUNK), p.ctas,
-                     pool->format == AKV_PAGE_E2M1 && D == 128 && p.nt == 1 ? 16 : p.nt <= 2 ? 12 : 8);
+                     warps_of(pool->format, D, p.nt));
     p.bytes = p.team ? 0 : (2ll + MOST_WARPS) * p.ctas * 8 * p.nt * (D + 4) * 4 + 8ll * p.ctas;
     return p;
 }

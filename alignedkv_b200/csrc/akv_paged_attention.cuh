@@ -42,13 +42,13 @@ struct Shape {
     static constexpr int MORE = F == AKV_PAGE_FP16 ? 0 : 2 * SCALES + 32;                  // ... of its scales and exponents
     // A step in shared memory: a tile's codes of K and of V, the next tile's, then scales of K, of V, exponents of K, of V by tile.
     static constexpr int STEP = (U * (32 * ROW + MORE) + 127) / 128 * 128;
-    // (4-bit rows of 128 channels are bound by the instructions that unpack them: 16 warps, 45.5 us instead of 47.3 for 8 heads x 131072 tokens)
-    static constexpr bool MANY = F == AKV_PAGE_E2M1 && D == 128 && NT == 1;
-    static constexpr int STEPS = ROW >= 128 || MANY ? 2 : F == AKV_PAGE_E2M1 && D == 128 ? 3 : F == AKV_PAGE_E4M3 ? (U == 4 ? 2 : 4) : (U == 4 ? 3 : 6);
-    // Up to 16 rows: operands of the queries stay in registers.  More: in shared memory, and the output takes the registers of a third of the warps.
+    static constexpr bool MANY = warps_of(F, D, NT) == 16;
+    static constexpr int STEPS = ROW >= 128 || MANY ? 2 : F == AKV_PAGE_E2M1 && D == 128 ? 3 : D == 64 && NT == 3 ? (F == AKV_PAGE_E4M3 ? 3 : 4)
+                                 : F == AKV_PAGE_E4M3 ? (U == 4 ? 2 : 4) : (U == 4 ? 3 : 6);
+    // Up to 16 rows: operands of the queries stay in registers.  More: in shared memory.
     // (20 rows of 4 bits, 32 x 8 heads x up to 4096 tokens: 56 us; ten warps spill, 69; steps of 16 tokens 63; units of 16 rows 67, of 8 64.)
     static constexpr bool FEW = NT <= 2;
-    static constexpr int WARPS = MANY ? 16 : FEW ? 12 : 8;
+    static constexpr int WARPS = warps_of(F, D, NT);
     static constexpr int RECORD = 8 * NT * (D + 4);           // floats: rows of D sums, then the maximum and the sum
     static constexpr int TABLE = F == AKV_PAGE_FP16 ? 0 : TOKENS * 16;       // of a step's tokens: factor, exponent, weight
     static constexpr int RING = STEPS * STEP, QUERIES = FEW ? 0 : KS * 4 * 32 * 8, OWN = RING + QUERIES + TABLE, SMEM = WARPS * OWN;

@@ -6,6 +6,15 @@ namespace akv {
 
 constexpr int CHUNK = 64, TEAM_CHUNK = 32, MOST_WARPS = 16;       // (TEAM_CHUNK: where a cluster has a unit to itself; a step where that is more)
 
+// Warps of a CTA for units of 8 nt rows.  As many as have room for their sums and queries: 12 at 168 registers each, 8 at 255.  (16 rows of 128 channels in
+// 12 warps spill a little; 32 x 8 heads x up to 4096 tokens, 12 rows: fp16 63.4 us, in 8 warps 57.6, e4m3 43.8 and 39.5, e2m1 42.6 and 40.5;
+// 24 rows of 64 channels fit them in 8 and 4 bits: 20 rows, e4m3 39.5 us in 8 warps, 35.7 in 12.)  One tile of
+// 4-bit rows of 128 channels is bound by the instructions that unpack them: 16 (8 heads x 131072 tokens 45.5 us, 12 warps 47.3).
+constexpr int warps_of(int format, int D, int nt) {
+    if (format == AKV_PAGE_E2M1 && D == 128 && nt == 1) return 16;
+    return nt == 1 || (D == 64 && (nt == 2 || (nt == 3 && format != AKV_PAGE_FP16))) ? 12 : 8;
+}
+
 struct AttendArgs {
     Pool pool;
     const __half* q;
