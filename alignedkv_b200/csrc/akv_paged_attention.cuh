@@ -5,7 +5,7 @@
 //   s_rj = scale q_r . k_j, o_r = sum_j exp(s_rj - m_r) v_j / l_r, l_r = sum_j exp(s_rj - m_r), over the tokens j that row r sees.
 //
 // Every byte of the tokens is read once: bound by HBM in 16 and 8 bits (8 x 32 x 4096 tokens of 128 channels, e4m3: 48.2 us, 5.6 TB/s; up to 8192 of
-// 64 x 8 heads: 95.2 us, 5.9 TB/s), by the instructions that unpack the codes in 4 (8 heads x 131072 tokens: 43.2 us, 3.5 TB/s, 61% of the issue
+// 64 x 8 heads: 95.9 us, 5.8 TB/s), by the instructions that unpack the codes in 4 (8 heads x 131072 tokens: 43.2 us, 3.5 TB/s, 61% of the issue
 // slots), and with many rows by the chain of products and softmax in few warps (20 rows, 32 x 8 heads x up to 4096: 56 us).
 // Work: a unit is the query rows of one (sequence, KV head), up to 32, its tokens in chunks of 64.  The chunks of all units in a row are dealt in
 // equal contiguous runs to the CTAs, then to a CTA's warps: lengths are only known on the device, and every SM gets the same whatever they
