@@ -750,6 +750,49 @@ __device__ __forceinline__ void join_few(const AttendArgs& a, int unit, int r, i
     if (record && sub == 0) *reinterpret_cast<float2*>(record + D) = make_float2(top, sum);
 }
 
+// The same, two records at a time and their maxima with their sums: where a CTA has many rows to join its warps wait for these loads again and again (20
+// rows, 32 x 8 heads x up to 4096 tokens, 4 bits: 56.1 -> 54.7 us; one query row a head 31.6 -> 32.1).
+template <int D, class Fn>
+__device__ __forceinline__ void join_pairs(const AttendArgs& a, int unit, int r, int count, int sub, Fn fn, float* record) {
+    constexpr int N = D / 32;
+    float top = -INFINITY, sum = 0.f;
+    float4 o[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int i = 0; i < count; i += 2) {
+        const bool two = i + 1 < count;
+        const float *x = fn(i), *z = two ? fn(i + 1) : x;
+        const float2 ml = *reinterpret_cast<const float2*>(x + D);
+        float2 nl = *reinterpret_cast<const float2*>(z + D);
+        float4 y[N], w[N];
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+            y[c] = *reinterpret_cast<const float4*>(x + 32 * c + 4 * sub);
+            w[c] = *reinterpret_cast<const float4*>(z + 32 * c + 4 * sub);
+        }
+        if (!two) {
+            nl = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int c = 0; c < N; ++c) w[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        const float m = fmaxf(top, fmaxf(ml.x, nl.x)), base = m == -INFINITY ? 0.f : m;
+        const float was = ex2(top - base), f = ex2(ml.x - base), g = ex2(nl.x - base);
+        sum = fmaf(g, nl.y, fmaf(f, ml.y, was * sum));
+        top = m;
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+            o[c] = make_float4(fmaf(g, w[c].x, fmaf(f, y[c].x, was * o[c].x)), fmaf(g, w[c].y, fmaf(f, y[c].y, was * o[c].y)),
+                               fmaf(g, w[c].z, fmaf(f, y[c].z, was * o[c].z)), fmaf(g, w[c].w, fmaf(f, y[c].w, was * o[c].w)));
+    }
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        if (record) *reinterpret_cast<float4*>(record + 32 * c + 4 * sub) = o[c];
+        else write_row<D>(a, unit, r, 32 * c + 4 * sub, o[c], top, sum);
+    }
+    if (record && sub == 0) *reinterpret_cast<float2*>(record + D) = make_float2(top, sum);
+}
+
 // Joins the records first .. last - 1 of a row by a warp, 4 channels a lane (of 128; of 64 half of the lanes have none); row(i): the i-th.
 template <int D, class Fn>
 __device__ __forceinline__ void join_row(int first, int last, int lane, Fn row, float4& o, float& top, float& sum) {
@@ -954,7 +997,8 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
             }
             if (record && lane == 0) *reinterpret_cast<float2*>(record + D) = make_float2(top, sum);
         } else {
-            join_few<D>(a, task.x, r, task.z, lane & 7, row, record);
+            if constexpr (NT == 1) join_few<D>(a, task.x, r, task.z, lane & 7, row, record);
+            else join_pairs<D>(a, task.x, r, task.z, lane & 7, row, record);
         }
     }
 }
