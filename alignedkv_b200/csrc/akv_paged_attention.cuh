@@ -6,7 +6,7 @@
 //
 // Every byte of the tokens is read once: bound by HBM in 16 and 8 bits (8 x 32 x 4096 tokens of 128 channels, e4m3: 48.2 us, 5.6 TB/s; up to 8192 of
 // 64 x 8 heads: 95.9 us, 5.8 TB/s), by the instructions that unpack the codes in 4 (8 heads x 131072 tokens: 43.2 us, 3.5 TB/s, 61% of the issue
-// slots), and with many rows by the chain of products and softmax in few warps (20 rows, 32 x 8 heads x up to 4096: 56 us).
+// slots), and with many rows by the chain of products and softmax in few warps (20 rows, 32 x 8 heads x up to 4096: 54 us).
 // Work: a unit is the query rows of one (sequence, KV head), up to 32, its tokens in chunks of 64.  The chunks of all units in a row are dealt in
 // equal contiguous runs to the CTAs, then to a CTA's warps: lengths are only known on the device, and every SM gets the same whatever they
 // are.  Each CTA adds up the lengths itself.  A warp needs no other one: it fills a ring in shared memory by asynchronous copies and drains it, codes go
@@ -46,7 +46,7 @@ struct Shape {
     static constexpr int STEPS = ROW >= 128 || MANY ? 2 : F == AKV_PAGE_E2M1 && D == 128 ? 3 : D == 64 && NT == 3 ? (F == AKV_PAGE_E4M3 ? 3 : 4)
                                  : F == AKV_PAGE_E4M3 ? (U == 4 ? 2 : 4) : (U == 4 ? 3 : 6);
     // Up to 16 rows: operands of the queries stay in registers.  More: in shared memory.
-    // (20 rows of 4 bits, 32 x 8 heads x up to 4096 tokens: 56 us; ten warps spill, 69; steps of 16 tokens 63; units of 16 rows 67, of 8 64.)
+    // (20 rows of 4 bits, 32 x 8 heads x up to 4096 tokens, 56 us then: ten warps spill, 69; steps of 16 tokens 63; units of 16 rows 67, of 8 64.)
     static constexpr bool FEW = NT <= 2;
     static constexpr int WARPS = warps_of(F, D, NT);
     static constexpr int RECORD = 8 * NT * (D + 4);           // floats: rows of D sums, then the maximum and the sum
