@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
     __shared__ float s_p[MOST], s_q[MOST], s_u[MOST];
     const int ctas = a.ctas, rank = blockIdx.x % ctas, b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int T = a.T, V = a.V;
+    cluster_arrive();
     pdl_turn();
     const P* target = a.target + b * a.target_batch;
     const P* draft = a.draft ? a.draft + b * a.draft_batch : nullptr;
@@ -103,6 +104,7 @@ __global__ void __launch_bounds__(THREADS, 2) choose_kernel(ChooseArgs<P> a) {
         if (twice) s_p[tid] = 0.f;
     }
     __syncthreads();
+    cluster_wait();                            // (all CTAs of the cluster run: total() stores into their shared memory)
     // parts of whole steps; this warp's begins at `first`
     const int steps = (V + STEP - 1) / STEP, each = (steps + ctas * WARPS - 1) / (ctas * WARPS);
     const int first = min(V, (rank * WARPS + warp) * each * STEP), last = min(V, first + each * STEP);

@@ -82,6 +82,13 @@ static inline cudaError_t launch_cluster(Kernel kernel, int ctas, dim3 grid, dim
     count_launch();
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
+// A CTA's shared memory may be written by another one once that CTA has started: every thread arrives at its kernel's beginning and waits in front of the
+// first remote store.  (No memory is ordered by these two.)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
