@@ -313,8 +313,12 @@ struct Ring {
 };
 
 // ---------------------------------------------------------------- a warp's unit
-template <int F, int D, int NT, bool ONE>
+// TWICE: 4 rows or fewer.  Their tile has them twice, in its columns 0 to 3 and 4 to 7: the scores are the same, and the values' product takes the rounded
+// probabilities in the first and what rounding took in the others, so that it needs no second one (8 heads x 131072 tokens, e2m1: @@ us, with a second
+// product @@).
+template <int F, int D, int NT, bool ONE, bool TWICE>
 struct Unit {
+    static_assert(!TWICE || NT == 1, "one tile");
     using S = Shape<F, D, NT>;
     static constexpr int U = S::U, KW = S::KW, KS = S::KS, ROW = S::ROW;
     const AttendArgs& a;
@@ -357,12 +361,15 @@ struct Unit {
         }
     }
 
+    // Row of the unit that column c of tile nt has.
+    __device__ __forceinline__ int row_at(int nt, int c) const { return 8 * nt + (TWICE ? c & 3 : c); }
+
     __device__ __forceinline__ void begin(const Rows& rows) {
         if constexpr (!S::FEW) __syncwarp();     // (the last unit's have been read)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             int query;
-            const long long row = rows.row(a, 8 * nt + g, &query);
+            const long long row = rows.row(a, row_at(nt, g), &query);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 uint2 w = make_uint2(0, 0);
@@ -615,26 +622,37 @@ struct Unit {
     __device__ __forceinline__ void add_values(const float (&s)[U][NT][4], uint32_t step, int at, int limit, const int (&seen)[NT][2]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            uint32_t v[KW], scale[2], w[NT][2];
+            uint32_t v[KW], scale[2], w[NT][2], rest[NT][2];
             load_v(v, scale, step, u, limit - 16 * u);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                w[nt][0] = transposed(halves_bits(s[u][nt][0], s[u][nt][1]));
-                w[nt][1] = transposed(halves_bits(s[u][nt][2], s[u][nt][3]));
-            }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float x = s[u][nt][2 * i], y = s[u][nt][2 * i + 1];
+                    const uint32_t near = halves_bits(x, y);
+                    const float2 f = halves_floats(near);
+                    rest[nt][i] = halves_bits(x - f.x, y - f.y);
+                    w[nt][i] = transposed(TWICE && t >= 2 ? rest[nt][i] : near);
+                    if (!TWICE) rest[nt][i] = transposed(rest[nt][i]);
+                }
             if (F == AKV_PAGE_FP16 && __any_sync(0xFFFFFFFFu, odd(v))) {
-                add_odd_values(v, w, at + 16 * u, at + limit, seen);
+                add_odd_values(v, w, rest, at + 16 * u, at + limit, seen);
                 continue;
             }
             tiles(v, scale, [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) mma(acc[i][nt], a0, a1, a2, a3, w[nt][0], w[nt][1]);
+                if (TWICE) return;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma(acc[i][nt], a0, a1, a2, a3, rest[nt][0], rest[nt][1]);
             });
         }
     }
     // The same where some values are not finite (fp16 pages alone: elsewhere codes are).  0 * inf would be NaN: every query's product is formed by
-    // itself, without the newest tokens that it does not see, and comes out as if those were not there.
-    __device__ __forceinline__ void add_odd_values(const uint32_t (&v)[KW], const uint32_t (&w)[NT][2], int at, int n, const int (&seen)[NT][2]) {
+    // itself, without the newest tokens that it does not see, and comes out as if those were not there.  What rounding took from a probability has any
+    // sign, and multiplies the finite values alone.
+    __device__ __forceinline__ void add_odd_values(const uint32_t (&v)[KW], const uint32_t (&w)[NT][2], const uint32_t (&rest)[NT][2], int at, int n,
+                                                   const int (&seen)[NT][2]) {
         const uint32_t none[2] = {0, 0};
 #pragma unroll 1
         for (int limit = n - a.T + 1; limit <= n; ++limit) {
@@ -643,10 +661,17 @@ struct Unit {
             for (int i = 0; i < 4; ++i) there[i] = at + 2 * t + (i & 1) + (i >> 1) * 8 < limit;
             const uint32_t m01 = (there[0] ? 0xFFFFu : 0u) | (there[1] ? 0xFFFF0000u : 0u), m23 = (there[2] ? 0xFFFFu : 0u) | (there[3] ? 0xFFFF0000u : 0u);
             tiles(v, none, [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                a0 &= m01, a1 &= m01, a2 &= m23, a3 &= m23;
+                const uint32_t f0 = finite(a0), f1 = finite(a1), f2 = finite(a2), f3 = finite(a3);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float c[4] = {acc[i][nt][0], acc[i][nt][1], acc[i][nt][2], acc[i][nt][3]};
-                    mma(c, a0 & m01, a1 & m01, a2 & m23, a3 & m23, w[nt][0], w[nt][1]);
+                    float y[4] = {c[0], c[1], c[2], c[3]};
+                    mma(c, a0, a1, a2, a3, w[nt][0], w[nt][1]);
+                    mma(TWICE ? y : c, f0, f1, f2, f3, TWICE ? w[nt][0] : rest[nt][0], TWICE ? w[nt][1] : rest[nt][1]);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        if (TWICE && t >= 2) c[x] = y[x];
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
                         if (seen[nt][x & 1] == limit) acc[i][nt][x] = c[x];
@@ -673,6 +698,12 @@ struct Unit {
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[nt][c] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][c], o);
+        if (TWICE) {
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) acc[i][0][x] += __shfl_xor_sync(0xFFFFFFFFu, acc[i][0][x], 2);
+        }
     }
     __device__ __forceinline__ void write(const Rows& rows) {
 #pragma unroll
@@ -845,7 +876,7 @@ __device__ __forceinline__ void join_many(const AttendArgs& a, int unit, int r, 
 }
 
 // TEAM: a cluster of CTAs has one unit, and its records are joined there.
-template <int F, int D, int NT, bool ONE, bool TEAM>
+template <int F, int D, int NT, bool ONE, bool TEAM, bool TWICE>
 __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(AttendArgs a) {
     using S = Shape<F, D, NT>;
     constexpr int WARPS = S::WARPS;
@@ -888,7 +919,7 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
             part.find(cum, units, a.groups, sequence_with(cum, a.B, units, at), at, end);
         }
         Ring<F, D, NT, ONE, TEAM> ring(a, cum, smem_u32(last_record), lane, units, part, at, end);
-        Unit<F, D, NT, ONE> unit(a, lane, smem_u32(last_record));
+        Unit<F, D, NT, ONE, TWICE> unit(a, lane, smem_u32(last_record));
         for (;;) {
             constexpr int TOKENS_OF = TEAM ? S::TEAM_TOKENS : CHUNK;
             const Rows rows(a, part.b, part.h, part.group);
@@ -899,7 +930,7 @@ __global__ void __launch_bounds__(32 * Shape<F, D, NT>::WARPS, 1) attend_kernel(
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     int query;
-                    seen[nt][c] = rows.row(a, 8 * nt + 2 * unit.t + c, &query) < 0 ? 0 : n - a.T + 1 + query;
+                    seen[nt][c] = rows.row(a, unit.row_at(nt, 2 * unit.t + c), &query) < 0 ? 0 : n - a.T + 1 + query;
                 }
             unit.begin(rows);
             int token = part.first * TOKENS_OF;
@@ -1051,7 +1082,7 @@ __global__ void __launch_bounds__(32 * JOINERS) join_kernel(AttendArgs a) {
     }
 }
 
-template <int F, int D, int NT, bool ONE, bool TEAM>
+template <int F, int D, int NT, bool ONE, bool TEAM, bool TWICE>
 int launch(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
     using S = Shape<F, D, NT>;
     static_assert(S::WARPS <= MOST_WARPS, "workspace");
@@ -1061,26 +1092,32 @@ int launch(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && set_for != dev) {
         // (the most it is ever launched with)
-        e = cudaFuncSetAttribute(attend_kernel<F, D, NT, ONE, TEAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM + 4097 * 4);
+        e = cudaFuncSetAttribute(attend_kernel<F, D, NT, ONE, TEAM, TWICE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM + 4097 * 4);
         if (e == cudaSuccess) set_for = dev;
     }
     if (e != cudaSuccess) return cuda_status(e, "paged_attention");
     if constexpr (TEAM) {
-        launch_cluster(attend_kernel<F, D, NT, ONE, TEAM>, a.team, dim3((unsigned)(a.B * a.pool.H * a.groups * a.team)), dim3(32 * S::WARPS), S::SMEM, st, a);
+        launch_cluster(attend_kernel<F, D, NT, ONE, TEAM, TWICE>, a.team, dim3((unsigned)(a.B * a.pool.H * a.groups * a.team)), dim3(32 * S::WARPS), S::SMEM, st, a);
         return cuda_status(cudaGetLastError(), "paged_attention launch");
     }
-    launch_chained(attend_kernel<F, D, NT, ONE, TEAM>, dim3(p.ctas), dim3(32 * S::WARPS), smem, st, a);
+    launch_chained(attend_kernel<F, D, NT, ONE, TEAM, TWICE>, dim3(p.ctas), dim3(32 * S::WARPS), smem, st, a);
     const int rc = cuda_status(cudaGetLastError(), "paged_attention launch");
     if (rc != AKV_OK || !joined || p.ctas == 1) return rc;
     launch_chained(join_kernel<D, NT>, dim3(p.ctas), dim3(32 * JOINERS), 0, st, a);
     return cuda_status(cudaGetLastError(), "paged_attention join launch");
 }
+template <int F, int D, int NT, bool ONE, bool TEAM>
+int launch_twice(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
+    if constexpr (NT == 1)
+        if (a.rows <= 4) return launch<F, D, NT, ONE, TEAM, true>(a, p, joined, st);
+    return launch<F, D, NT, ONE, TEAM, false>(a, p, joined, st);
+}
 template <int F, int D, int NT>
 int launch_pages(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
     if constexpr (Shape<F, D, NT>::U > 1)
         if (Shape<F, D, NT>::TOKENS > 1 << a.pool.shift)
-            return a.team ? launch<F, D, NT, false, true>(a, p, joined, st) : launch<F, D, NT, false, false>(a, p, joined, st);
-    return a.team ? launch<F, D, NT, true, true>(a, p, joined, st) : launch<F, D, NT, true, false>(a, p, joined, st);
+            return a.team ? launch_twice<F, D, NT, false, true>(a, p, joined, st) : launch_twice<F, D, NT, false, false>(a, p, joined, st);
+    return a.team ? launch_twice<F, D, NT, true, true>(a, p, joined, st) : launch_twice<F, D, NT, true, false>(a, p, joined, st);
 }
 template <int F, int D>
 int launch_rows(const AttendArgs& a, const Plan& p, bool joined, cudaStream_t st) {
