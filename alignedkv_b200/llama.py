@@ -71,8 +71,8 @@ class LlamaDecoder:
     """Random-init Llama decoder with one AlignedKV `DecodeLayer` per transformer layer.
 
     attention="paged" instead keeps the tokens in the pages of one `PagedLayer` per layer (kv_format "fp16", "e4m3" or "e2m1", n_pages of page_size
-    tokens; by default enough for all sequences) behind one `PageTable`: sequences then have lengths of their own.  attention="dense" is
-    fp16 torch attention over a plain cache."""
+    tokens; by default enough for all sequences) behind one `PageTable`: sequences then have lengths of their own, and `table.release(b)` ends one.
+    attention="dense" is fp16 torch attention over a plain cache."""
 
     def __init__(self, cfg: LlamaConfig, bsz: int, max_seq_len: int, device, seed: int = 0, v_mode: str = "exact",
                  attention: str = "alignedkv", kv_format: str = "e4m3", page_size: int = 64, n_pages: int | None = None):
@@ -286,6 +286,14 @@ class LlamaDecoder:
             x = self._around(p, x, tables, attend)
         return x
 
+    def _active(self, active) -> list:
+        """Which sequences of a paged batch take part: `active`, one truth value each; by default those that are not over (all, if all are)."""
+        over = self.table.over
+        take = [not o or all(over) for o in over] if active is None else [bool(x) for x in active]
+        if len(take) != self.B:
+            raise RuntimeError(f"active: {len(take)} truth values for {self.B} sequences")
+        return take
+
     def _logits(self, x: torch.Tensor) -> torch.Tensor:
         return F.linear(_rms_norm(x, self.final_norm, self.cfg.rms_norm_eps), self.lm_head)
 
@@ -312,14 +320,20 @@ class LlamaDecoder:
         return self._forward(ids, True)
 
     @torch.no_grad()
-    def step(self, ids: torch.Tensor) -> torch.Tensor:
+    def step(self, ids: torch.Tensor, active=None) -> torch.Tensor:
         """ids [B] (one token per sequence) -> logits [B,V]; appends to every layer's cache.  Drafts of an earlier `verify` are
-        dropped: their keys were made for the position that this token takes."""
+        dropped: their keys were made for the position that this token takes.
+
+        With attention="paged", active (a truth value per sequence) says which sequences get their token; the others stay as they are and have no
+        meaningful logits (their ids are any words).  By default sequences that were released and have had no tokens since are left out, unless
+        all were."""
         if self.attention == "paged":
-            x = self._paged(ids.view(self.B, 1), [1] * self.B, False)
-            self.table.advance(1)
+            counts = [int(x) for x in self._active(active)]
+            x = self._paged(ids.view(self.B, 1), counts, False)
+            self.table.advance(counts)
             self._drafts = None
             return self._logits(x)[:, 0]
+        assert active is None, "sequences are left out with attention='paged' only"
         assert (self.caches[0].cache_len if self.attention == "alignedkv" else self.pos) + 1 <= self.L
         self._drafts = None
         if getattr(self, "_segs", None) is not None:
@@ -327,13 +341,13 @@ class LlamaDecoder:
         return self._forward(ids.view(self.B, 1), False)
 
     @torch.no_grad()
-    def verify(self, ids: torch.Tensor, parents: torch.Tensor | None = None, weights: bool = False) -> torch.Tensor:
+    def verify(self, ids: torch.Tensor, parents: torch.Tensor | None = None, weights: bool = False, active=None) -> torch.Tensor:
         """Logits [B,T,V] of T drafted tokens (ids [B,T], T at most 64) that are not in the caches yet.  parents: int64 [T], the
         tree they form in every sequence: the node that each one follows, a lower index, or -1 for the last cached token.
         `accept` appends some of them, as long as neither `step` nor a roll-back comes between.  weights=True also adds the
         attention weights of all T queries to each layer's (`evict`), at once and for good: those of branches that are not accepted
         and of drafts that are dropped, too.  parents=None is a chain, the only form with attention="paged" (T tokens of at most 64 query rows per
-        KV head, no weights): its keys and values enter the pages behind the cached tokens, where `accept` lets them count."""
+        KV head, no weights): its keys and values enter the pages behind the cached tokens, where `accept` lets them count; active as for `step`."""
         cfg = self.cfg
         B, T = ids.shape
         if self.attention == "paged":
@@ -342,9 +356,11 @@ class LlamaDecoder:
             rows = T * (cfg.num_attention_heads // cfg.num_key_value_heads)
             if rows > paged_ops.MOST_ROWS:
                 raise RuntimeError(f"verify: {T} tokens are {rows} query rows per KV head, at most {paged_ops.MOST_ROWS}")
-            x = self._paged(ids, [T] * B, False)
-            self._drafts = (list(self.table.lengths), T)
+            counts = [T * int(x) for x in self._active(active)]
+            x = self._paged(ids, counts, False)
+            self._drafts = (list(self.table.lengths), counts)
             return self._logits(x)
+        assert active is None, "sequences are left out with attention='paged' only"
         assert self.attention == "alignedkv", "only the AlignedKV and paged paths draft tokens"
         D = cfg.head_dim
         up = list(range(-1, T - 1)) if parents is None else parents.tolist()
@@ -376,16 +392,16 @@ class LlamaDecoder:
         """Append nodes path[b, 0..n-1] (int [B,n]: a chain from the root) of the last `verify` to the caches; once.  A call that is
         refused changes nothing and leaves the drafts as they were.
 
-        With attention="paged": the first path[b] tokens of each sequence's chain (int [B], 0 to T) count from now on."""
+        With attention="paged": the first path[b] tokens of each sequence's chain (int [B], 0 to T; 0 where it took no part) count from now on."""
         if self.attention == "paged":
-            lengths, T = self._drafts or (None, 0)
+            lengths, drafted = self._drafts or (None, ())
             if lengths != self.table.lengths:
                 raise RuntimeError("accept: no drafted tokens at this position (call verify first)")
             if path.shape != (self.B,) or path.is_floating_point() or path.dtype is torch.bool:
                 raise RuntimeError(f"path: expected integers of shape [{self.B}], the accepted tokens of each sequence's chain")
             counts = path.tolist()
-            if not all(0 <= n <= T for n in counts):
-                raise RuntimeError(f"path: {counts}, expected 0 to {T}")
+            if not all(0 <= n <= T for n, T in zip(counts, drafted)):
+                raise RuntimeError(f"path: {counts}, expected 0 to {drafted}")
             self.table.advance(counts)
             self._drafts = None
             return
@@ -415,14 +431,18 @@ class LlamaDecoder:
 
         The accepted tokens enter the cache.  Returns (tokens int64 [B], counts [B] numbers): how many of its nodes each sequence has gone on by -
         with attention="alignedkv" the same number for all, the smallest, since that cache has one length - and the token behind them, to be
-        the next ids[:, 0]."""
+        the next ids[:, 0].  (A sequence that took no part in `verify` goes on by 0 and keeps ids[:, 0].)"""
         T = ids.shape[1]
         target = torch.softmax(logits.float() / temperature, -1)
         up = None if parents is None else parents.to(device=self.device, dtype=torch.int32)      # (a second root hangs under no node)
         path, count, token = cache_ops.accept_drafts(target, draft, ids.contiguous(), coins, up)
         counts = count.tolist()
         if self.attention == "paged":
-            self.accept(count)
+            drafted = (self._drafts or (None, [T] * self.B))[1]
+            if 0 in drafted:
+                counts = [n if m else 0 for n, m in zip(counts, drafted)]
+                token = torch.where(torch.tensor([m > 0 for m in drafted], device=token.device), token, ids[:, 0])
+            self.accept(torch.tensor(counts))
             return token, counts
         n = min(counts)
         further = ids.gather(1, path[:, min(n, T - 1)].clamp(min=0).long()[:, None])[:, 0]

@@ -24,7 +24,7 @@ class PageTable:
       table.reserve(n)        pages for n more tokens (a number, or one per sequence)
       layer.append(...)       ... of every layer, at positions lens ..
       table.advance(n)        they count from now on
-      table.release(b)        sequence b is over, its pages are free
+      table.release(b)        sequence b is over, its pages are free; until tokens are reserved for it again, over[b] is true
     """
     def __init__(self, bsz: int, max_seq_len: int, n_pages: int, page_size: int, device):
         if bsz < 1 or max_seq_len < 1 or n_pages < 1:
@@ -36,6 +36,7 @@ class PageTable:
         self.lens = torch.zeros(bsz, dtype=torch.int32, device=self.device)
         self.lengths = [0] * bsz
         self.owned = [[] for _ in range(bsz)]
+        self.over = [False] * bsz
         self.free = list(range(n_pages - 1, -1, -1))
 
     def _counts(self, n) -> list:
@@ -55,6 +56,7 @@ class PageTable:
         if sum(need) > len(self.free):
             raise RuntimeError(f"{sum(need)} pages are needed, {len(self.free)} of {self.n_pages} are free")
         places = []
+        self.over = [o and not c for o, c in zip(self.over, counts)]
         for b, m in enumerate(need):
             for _ in range(m):
                 page = self.free.pop()
@@ -81,6 +83,7 @@ class PageTable:
         self.free.extend(reversed(self.owned[b]))
         self.owned[b] = []
         self.lengths[b] = 0
+        self.over[b] = True
         self.pages[b] = -1
         self.lens[b] = 0
 

@@ -80,3 +80,17 @@ def test_layers():
     assert c.v_codes.dtype is torch.half and c.v_exps is None
     with pytest.raises(ValueError):
         PagedLayer(4, 16, 2, 64, "cpu", "int8")
+
+
+def test_a_released_sequence_is_over_until_it_has_tokens_again():
+    t = table()
+    t.reserve(3)
+    t.advance(3)
+    t.release(1)
+    assert t.over == [False, True, False]
+    t.reserve([1, 0, 1])
+    with pytest.raises(RuntimeError):
+        t.reserve([0, 200, 0])
+    assert t.over == [False, True, False]
+    t.reserve([0, 5, 0])
+    assert t.over == [False] * 3
