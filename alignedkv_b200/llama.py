@@ -432,6 +432,8 @@ class LlamaDecoder:
         The accepted tokens enter the cache.  Returns (tokens int64 [B], counts [B] numbers): how many of its nodes each sequence has gone on by -
         with attention="alignedkv" the same number for all, the smallest, since that cache has one length - and the token behind them, to be
         the next ids[:, 0].  (A sequence that took no part in `verify` goes on by 0 and keeps ids[:, 0].)"""
+        if isinstance(temperature, (int, float)) and not temperature > 0:
+            raise RuntimeError(f"choose: a temperature of {temperature}, expected a positive one (a small one takes the likeliest word)")
         T = ids.shape[1]
         target = torch.softmax(logits.float() / temperature, -1)
         up = None if parents is None else parents.to(device=self.device, dtype=torch.int32)      # (a second root hangs under no node)
