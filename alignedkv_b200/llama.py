@@ -435,7 +435,7 @@ class LlamaDecoder:
         if isinstance(temperature, (int, float)) and not temperature > 0:
             raise RuntimeError(f"choose: a temperature of {temperature}, expected a positive one (a small one takes the likeliest word)")
         T = ids.shape[1]
-        if self.attention == "paged" and parents is not None and parents.tolist() != list(range(-1, T - 1)):
+        if self.attention == "paged" and parents is not None and any(up != list(range(-1, T - 1)) for up in parents.reshape(-1, T).tolist()):
             raise RuntimeError("choose: a paged cache takes chains of drafts")
         target = torch.softmax(logits.float() / temperature, -1)
         up = None if parents is None else parents.to(device=self.device, dtype=torch.int32)      # (a second root hangs under no node)

@@ -15,7 +15,7 @@ def test_temperatures_that_give_no_distribution(temperature):
         LlamaDecoder.choose(None, torch.zeros(1, 2, 4), None, torch.zeros(1, 2, dtype=torch.long), torch.zeros(1, 2), temperature=temperature)
 
 
-@pytest.mark.parametrize("parents", [[-1, 0, 0], [-1, -1, 0], [[-1, 0, 1]]])
+@pytest.mark.parametrize("parents", [[-1, 0, 0], [-1, -1, 0], [[-1, 0, 1], [-1, 0, 0]]])
 def test_trees_over_a_paged_cache(parents):
     """Of a tree's path nodes 0, 2, say, the count of 2 would have let the tokens of nodes 0 and 1 enter the cache."""
     from alignedkv_b200.llama import LlamaDecoder
