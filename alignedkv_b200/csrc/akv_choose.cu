@@ -5,12 +5,14 @@
 // normalised; times Z that is max(p - (c + Z) q, 0), since max(max(a, 0) - b, 0) = max(a - b, 0) for b >= 0.  So the residual after any number of
 // rejections is one coefficient, and the tests are u Z q(x) < r(x) with Z = sum r.  Without q a child is a guess of probability one:
 // accepted with probability p(x) / Z, and its p leaves the row when it is not.  Where no child is left, the smallest j with
-// cumsum(r)[j] > u_0 sum(r) follows.  Products and sums in 64 bits: the differences of fp32 probabilities are exact there, and what the order
-// of additions changes is too little to move a border across a random number.
-// Bound by HBM's latency and by barriers: a walk is a chain of sums over a vocabulary, one for each rejection that another child, or the last token, asks
-// after, and each waits for the one before it.  A cluster of up to 8 CTAs has a sequence; of 64 sequences, 8 nodes, 131072 words in fp32 (four CTAs
-// each, 16 loads of 16 bytes a thread and row) 20.8 us.  (A CTA a sequence 526; a cluster whose CTAs take each step of the walk together 49; a warp that
-// walks by itself 31; now loads in batches too.)  8 x 32 guesses of 32000 words: 9.6 us, one sequence of 5 nodes 6.0.
+// cumsum(r)[j] > u_0 sum(r) follows.  Products and sums in 64 bits: a difference p - c q is one fused operation, off by 2^-53 of itself, a sum of V by V 2^-53
+// at most, so that a border moves across a random number only where that comes as near to it.
+// A walk forms one sum over a vocabulary for each rejection that another child asks after, each behind the one before it, and one for the last token: of a
+// chain that one alone.  A cluster of up to 8 CTAs has a sequence; of 64 chains of 8 nodes, 131072 words in fp32 (four CTAs each), 20.8 us.  Stamps in it: 1.5 us until the
+// nodes' numbers are there, 1.0 of walk (3.3 the longest), 8.5 of pass over a row of p and one of q (66 MB in all, at the rate of a copy), 1.6 until the
+// cluster has its sum, 1.6 for the token; the median CTA is done after 14.4, those of the longest walks, whose pass begins last, after 20.  (A CTA a sequence
+// 526 us; a cluster whose CTAs take each step of the walk together 49; a warp that walks by itself 31; now loads in batches too.)  8 x 32 guesses of 32000 words: 9.6 us,
+// one sequence of 5 nodes 6.0.
 #include <cuda_bf16.h>
 
 #include "akv_common.cuh"

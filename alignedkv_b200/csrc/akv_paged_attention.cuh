@@ -4,9 +4,9 @@
 //
 //   s_rj = scale q_r . k_j, o_r = sum_j exp(s_rj - m_r) v_j / l_r, l_r = sum_j exp(s_rj - m_r), over the tokens j that row r sees.
 //
-// Every byte of the tokens is read once: bound by HBM in 16 and 8 bits (8 x 32 x 4096 tokens of 128 channels, e4m3: 48.2 us, 5.6 TB/s; up to 8192 of
-// 64 x 8 heads: 95.9 us, 5.8 TB/s), by the instructions that unpack the codes in 4 (8 heads x 131072 tokens: 43.2 us, 3.5 TB/s, 61% of the issue
-// slots), and with many rows by the chain of products and softmax in few warps (20 rows, 32 x 8 heads x up to 4096: 54 us).
+// Every byte of the tokens is read once: bound by HBM in 16 and 8 bits (8 x 32 x 4096 tokens of 128 channels, e4m3: 48.5 us, 5.6 TB/s; up to 8192 of
+// 64 x 8 heads: 95.5 us, 5.8 TB/s), in 4 by the instructions that unpack the codes and by their chains (8 heads x 131072 tokens: 43.9 us, 3.5 TB/s, 62% of the issue
+// slots, no pipe full), and with many rows by the chain of products and softmax in few warps (20 rows, 32 x 8 heads x up to 4096: 59.8 us).
 // Work: a unit is the query rows of one (sequence, KV head), up to 32, its tokens in chunks of 64.  The chunks of all units in a row are dealt in
 // equal contiguous runs to the CTAs, then to a CTA's warps: lengths are only known on the device, and every SM gets the same whatever they
 // are.  Each CTA adds up the lengths itself.  A warp needs no other one: it fills a ring in shared memory by asynchronous copies and drains it, codes go
@@ -28,8 +28,9 @@ constexpr float LN2 = 0.6931471805599453f;
 // relative to the largest and times 2^15 they keep all 11 bits down to 2^-29 of it.  What the rounding takes is rounded to fp16 as well and multiplied too:
 // 22 bits of a probability, 2^-39 of the largest at the least.  Against 64 bits outputs are then off by their own rounding alone (2.06 to 2.11e-4 in the 2-norm, to
 // the digit what sums in 32 bits give; without the second part up to 3% more, 9 to 19% of the outputs a step away, where now 0.4 to 0.8% are, and an average of
-// equal values was not that value).  It costs nothing up to 4 rows (`TWICE`), 0 to 2% with more in 16 and 8 bits, up to 9% in 4 (20 rows, 32 x 8 heads x up to
-// 4096 tokens: 54.7 -> 59.7 us).
+// equal values was not that value).  It costs 0 to 2% up to 4 rows (`TWICE`) and 2 to 16% with more
+// (32 x 8 heads x up to 4096 tokens: 12 rows fp16 56.9 -> 57.5 us, e4m3 38.5 -> 41.5, e2m1 39.8 -> 43.7; 20 rows 66.7 -> 69.6, 54.6 -> 59.6, 54.7 -> 59.8; 32 rows
+// 83.7 -> 89.6, 74.6 -> 86.7, 73.3 -> 79.9).
 constexpr float LIFT = 32768.f;
 
 
@@ -317,7 +318,7 @@ struct Ring {
 
 // ---------------------------------------------------------------- a warp's unit
 // TWICE: 4 rows or fewer.  Their tile has them twice, in its columns 0 to 3 and 4 to 7: the scores are the same, and the values' product takes the rounded
-// probabilities in the first and what rounding took in the others, so that it needs no second one (8 heads x 131072 tokens, e2m1: 43.8 us, with a second
+// probabilities in the first and what rounding took in the others, so that it needs no second one (8 heads x 131072 tokens, e2m1: 43.9 us, with a second
 // product 46.3).
 template <int F, int D, int NT, bool ONE, bool TWICE>
 struct Unit {

@@ -7,9 +7,10 @@ namespace akv {
 constexpr int CHUNK = 64, TEAM_CHUNK = 32, MOST_WARPS = 16;       // (TEAM_CHUNK: where a cluster has a unit to itself; a step where that is more)
 
 // Warps of a CTA for units of 8 nt rows.  As many as have room for their sums and queries: 12 at 168 registers each, 8 at 255.  (16 rows of 128 channels in
-// 12 warps spill a little; 32 x 8 heads x up to 4096 tokens, 12 rows: fp16 63.4 us, in 8 warps 57.6, e4m3 43.8 and 39.5, e2m1 42.6 and 40.5;
-// 24 rows of 64 channels fit them in 8 and 4 bits: 20 rows, e4m3 39.5 us in 8 warps, 35.7 in 12.)  One tile of
-// 4-bit rows of 128 channels is bound by the instructions that unpack them: 16 (8 heads x 131072 tokens 45.5 us, 12 warps 47.3).
+// 12 warps spill 64 to 296 bytes; 32 x 8 heads x up to 4096 tokens, 12 rows: fp16 68.6 us, in 8 warps 57.5, e4m3 56.2 and 41.5, e2m1 46.3 and 43.7.
+// 24 rows of 64 channels do with them in 8 and 4 bits: 20 rows, e4m3 40.2 us in 8 warps, 39.2 in 12, e2m1 41.4 and 39.7.)  One tile of
+// 4-bit rows of 128 channels is bound by the instructions that unpack them: 16 (8 heads x 131072 tokens 43.9 us, 12 warps 45.5).  Spilled for all that, as
+// ptxas says: one tile of 128 channels up to 24 bytes, two and three of 64 up to 32, four of 128 28 to 208.
 constexpr int warps_of(int format, int D, int nt) {
     if (format == AKV_PAGE_E2M1 && D == 128 && nt == 1) return 16;
     return nt == 1 || (D == 64 && (nt == 2 || (nt == 3 && format != AKV_PAGE_FP16))) ? 12 : 8;

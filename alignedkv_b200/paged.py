@@ -25,7 +25,9 @@ class PageTable:
       layer.append(...)       ... of every layer, at positions lens ..
       table.advance(n)        they count from now on
       table.release(b)        sequence b is over, its pages are free; until tokens are reserved for it again, over[b] is true
-    """
+
+    A page has one owner, and `pages` holds what was handed out: nothing else writes it.  (The operators take tables in which sequences share pages, or
+    have given some up; such a table is the caller's own.)"""
     def __init__(self, bsz: int, max_seq_len: int, n_pages: int, page_size: int, device):
         if bsz < 1 or max_seq_len < 1 or n_pages < 1:
             raise ValueError(f"{bsz} sequences of up to {max_seq_len} tokens in {n_pages} pages")
