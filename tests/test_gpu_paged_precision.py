@@ -68,3 +68,34 @@ def test_outputs_are_rounded_once(form, D, group, T):
             free = mass * (2 * 3 * 2.0 ** -24 * 2 * size[..., None] + 2.0 ** -20 + 2.0 ** -22 + (n / 16 + 64) * 2.0 ** -23) + n * 2.0 ** -38 * top[..., None]
             low, high = (want - free).half(), (want + free).half()
             assert bool(((low <= out[b]) & (out[b] <= high)).all()), (b, n, int(((out[b] < low) | (out[b] > high)).sum()), out[b].numel())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("group,T", ROWS)
+def test_infinities_have_no_part_in_what_rounding_took(D, group, T):
+    """fp16 pages: a value of infinity comes out as that in the rows that see it and in its channel alone, whatever sign the rest of its probability has;
+    two of different signs as NaN.  Tables that take one tile of rows, several by clusters, and several by equal runs."""
+    from alignedkv_b200 import paged_ops
+    import paged_plan
+    gen = torch.Generator().manual_seed(D * 5 + group * T)
+    B, H, page, n = paged_plan.B, paged_plan.H, 16, 150
+    N = B * -(-n // page)
+    pool, pages = ref.make_pool(N, page, H, D, "fp16", DEV, gen), paged.table(B, N // B, N, gen)
+    k, v = (torch.randn(B, n, H, D, generator=gen).half().to(DEV) for _ in range(2))
+    v[:, n - 1, 0, 3], v[:, 20, 1, 5], v[:, n // 2, 2, 7], v[:, n // 3, 2, 7] = math.inf, -math.inf, math.inf, -math.inf
+    v[:, n - 1, 3, 9] = math.nan
+    paged_ops.paged_append(pool, k, v, pages, i32(*[0] * B))
+    q = (torch.randn(B, T, H * group, D, generator=gen) * 0.3).half().to(DEV)
+    odd = torch.zeros(T, H * group, D, device=DEV)
+    odd[T - 1, :group, 3], odd[:, group:2 * group, 5] = math.inf, -math.inf
+    odd[:, 2 * group:3 * group, 7] = odd[T - 1, 3 * group:, 9] = math.nan
+    for table in (n,) + paged_plan.TABLES:
+        more = max(0, -(-table // page) - pages.shape[1])
+        wide = torch.cat([pages, torch.randint(-2 ** 31, 2 ** 31 - 1, (B, more), generator=gen).to(torch.int32).to(DEV)], 1)
+        out = paged_ops.paged_attention(pool, q, wide, i32(*[n] * B))
+        clean = torch.where(v.isfinite(), v, 0).double()
+        for b in (0, B - 1):
+            want, _, mass, size, top = ref.attend64(q[b], k[b].double(), clean[b], torch.ones(n, dtype=torch.bool, device=DEV), 1 / math.sqrt(D))
+            assert torch.equal(torch.where(odd == 0, 0, out[b].float()).nan_to_num(7, 8, 9), odd.nan_to_num(7, 8, 9))
+            bound = ref.out_bound(want, mass, size, top, D, n)
+            assert bool((((out[b].double() - want).abs() <= bound) | (odd != 0)).all())
